@@ -1,4 +1,5 @@
 // Host orchestration and the C ABI of the engine (see include/culsh_b200.h).
+#include "api.cuh"
 #include "common.cuh"
 #include "index_build.cuh"
 #include "minhash.cuh"
@@ -18,13 +19,6 @@
 #include <functional>
 
 using namespace culsh_b200;
-
-// -----------------------------------------------------------------------------------------
-// Objects behind the opaque pointers
-// -----------------------------------------------------------------------------------------
-struct culsh_handle {
-    CtxPtr ctx;
-};
 
 // Hash parameters of an index; immutable once generated, so indexes built on one handle with
 // the same (family, L, k, d, window, dtype, seed) share one set.
@@ -47,48 +41,7 @@ struct culsh_index {
     std::shared_ptr<ParamSet> params = std::make_shared<ParamSet>();  // may be shared between indexes
 };
 
-struct culsh_candidates {
-    CtxPtr ctx;
-    int n_queries = 0;
-    uint64_t total = 0;
-    DevBuf<int32_t> indices;
-    DevBuf<uint64_t> counts;
-    DevBuf<uint64_t> offsets;
-    bool empty() const { return !indices.p && !counts.p && !offsets.p; }
-};
-
 namespace {
-
-thread_local std::string g_last_error;
-
-template <typename F>
-int guarded(F&& f) {
-    try {
-        f();
-        return CULSH_OK;
-    } catch (const Error& e) {
-        g_last_error = e.what();
-        return e.status;
-    } catch (const std::bad_alloc&) {
-        g_last_error = "host allocation failed";
-        return CULSH_ERR_ALLOC;
-    } catch (const std::exception& e) {
-        g_last_error = e.what();
-        return CULSH_ERR_INTERNAL;
-    }
-}
-
-struct DeviceGuard {
-    int prev = -1;
-    explicit DeviceGuard(int dev) {
-        CU_CHECK(cudaGetDevice(&prev));
-        if (prev != dev) CU_CHECK(cudaSetDevice(dev));
-        else prev = -1;
-    }
-    ~DeviceGuard() {
-        if (prev >= 0) cudaSetDevice(prev);
-    }
-};
 
 struct StageTimer {
     const CtxPtr& c;
