@@ -24,4 +24,14 @@ if not _building:
     from .rp_lsh import RPLSH, RPLSHModel  # noqa: E402
 
     __all__ = ["RPLSH", "RPLSHModel", "MinHashLSH", "MinHashLSHModel", "PStableLSH", "PStableLSHModel",
-               "Candidates"]
+               "Candidates", "MXRows", "LogProbs", "log_probs", "log_probs_backward", "rank"]
+
+    # the ranking layer works on torch tensors; it is imported when one of its names is first used, so that programs that only
+    # build and query indexes do not import torch
+    _RANKING = ("MXRows", "LogProbs", "log_probs", "log_probs_backward", "rank")
+
+    def __getattr__(name):
+        if name in _RANKING:
+            from . import ranking
+            return getattr(ranking, name)
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

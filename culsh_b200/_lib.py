@@ -39,6 +39,7 @@ class Stats(C.Structure):
 VP = C.c_void_p
 I = C.c_int
 U64 = C.c_uint64
+I64 = C.c_int64
 PP = C.POINTER(C.c_void_p)
 
 # name -> argtypes (every function returns int unless listed in _VOID / _CHARP)
@@ -98,6 +99,15 @@ SIGNATURES = {
     "culsh_candidates_attach_indices": [VP, VP, U64],
     "culsh_merge_shard_candidates_noalloc": [VP, I, I, PP, PP, C.POINTER(C.c_int64), VP, U64, VP, VP,
                                              C.POINTER(C.c_uint64)],
+    "culsh_mx_quantize": [VP, VP, I, I, I, I64, VP, VP, VP, VP],
+    "culsh_mx_dequantize": [VP, VP, VP, I, I, VP, I, VP],
+    "culsh_mx_product": [VP, VP, VP, VP, I, VP, VP, VP, I, I, I, VP, I, I64, VP],
+    "culsh_mx_product_check": [VP, VP],
+    "culsh_mx_score": [VP, VP, I, I, I64, VP, VP, VP, I, I, I, VP, VP, I64, VP, VP],
+    "culsh_candidates_after": [VP, VP, VP],
+    "culsh_log_probs_workspace": [VP, I, I64, I, I64, C.POINTER(C.c_uint64)],
+    "culsh_log_probs": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, I, VP, VP, VP, VP, VP, VP, U64, VP],
+    "culsh_log_probs_backward": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, VP, VP, VP, VP, VP, VP],
 }
 _VOID = {"culsh_index_free": [VP], "culsh_candidates_free": [VP]}
 _CHARP = {"culsh_last_error": []}

@@ -301,6 +301,71 @@ int culsh_merge_shard_candidates_noalloc(culsh_handle* h, int n_shards, int n_qu
                                          uint64_t* out_counts, uint64_t* out_offsets,
                                          uint64_t* total_out);
 
+/* ---- ranking (no upstream counterpart: upstream returns candidates unranked) ------------ */
+/* Rows held in microscaled 4-bit floating point, their products with queries, scores of candidate
+ * lists, and log probabilities over scores with their gradient.  Unlike the calls above these take
+ * device memory only, run on the stream that is given (a cudaStream_t of the handle's device, NULL
+ * for the default one) and return when their work is queued; they allocate nothing. */
+typedef enum culsh_type { CULSH_F32 = 0, CULSH_F64 = 1, CULSH_F16 = 2, CULSH_BF16 = 3 } culsh_type;
+typedef enum culsh_metric {
+    CULSH_DOT = 0,      /* q . x                                    */
+    CULSH_COSINE = 1,   /* q . x / (|q| |x|), 0 for a row of zeros  */
+    CULSH_EUCLIDEAN = 2 /* -|q - x|^2                               */
+} culsh_metric;
+
+/* X: [n][d], rows ld entries apart, of any type.  Blocks of 32 values share the power of two
+ * 2^(floor(log2 max) - 2); a value is the nearest of +-{0, .5, 1, 1.5, 2, 3, 4, 6} times it, ties to
+ * the even code, larger ones 6.  A block with a NaN or an infinity is NaN.  With
+ * G = ceil(d / 128), T = ceil(n / 128):
+ *   codes  [n][64 G]            two to a byte, the first in the low half (sign, exponent, exponent,
+ *                               fraction), zeros behind a row's end
+ *   scales [T][G][32][4][4]     exponent + 127 of block 4 g + b of row 128 t + 32 j + i at [t][g][i][j][b];
+ *                               255 is NaN
+ *   norms  [n]                  squared length of the row as held
+ * codes and scales begin at a multiple of 16 bytes. */
+int culsh_mx_quantize(culsh_handle* h, const void* X, int type, int n, int d, int64_t ld, uint8_t* codes, uint8_t* scales,
+                      float* norms, void* stream);
+/* out: [n][d] of any type. */
+int culsh_mx_dequantize(culsh_handle* h, const uint8_t* codes, const uint8_t* scales, int n, int d, void* out, int type,
+                        void* stream);
+/* out[q][i] (float32, float16 or bfloat16, rows ld entries apart): the metric of query q and row i, both held in 4 bits. */
+int culsh_mx_product(culsh_handle* h, const uint8_t* q_codes, const uint8_t* q_scales, const float* q_norms, int n_queries,
+                     const uint8_t* codes, const uint8_t* scales, const float* norms, int n, int d, int metric, void* out,
+                     int type, int64_t ld, void* stream);
+/* Waits for the stream and says whether a bounded wait of a product ran out since the last such call
+ * (CULSH_ERR_INTERNAL; the scores that it should have made are NaN). */
+int culsh_mx_product_check(culsh_handle* h, void* stream);
+/* out[c], c in [offsets[q], offsets[q + 1]): the metric of query q as it is (any type, rows ldq apart)
+ * and row ids[c]; NaN where ids[c] is no row.  offsets: n_queries + 1, from 0 to total. */
+int culsh_mx_score(culsh_handle* h, const void* Q, int type, int n_queries, int64_t ldq, const uint8_t* codes,
+                   const uint8_t* scales, const float* norms, int n, int d, int metric, const int32_t* ids,
+                   const int64_t* offsets, int64_t total, float* out, void* stream);
+/* What the result's handle does from now on waits for what the stream holds so far: call it behind work
+ * that reads a result's device arrays (culsh_candidates_device_ptrs), which may then be freed at once. */
+int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* stream);
+
+/* Rows of scores (float32, float16, bfloat16): a matrix [m][cols] with rows ld apart (offsets and ids
+ * NULL), or m lists, offsets[m + 1] from 0 to total, with ids ascending in each (ids may be NULL
+ * where there are no targets: entries are then named by their place).  With z = scores / temperature:
+ *   lse            log of the sum of exp(z); -inf for a row with nothing in it that is not -inf
+ *   entropy        of the distribution exp(z - lse); 0 there
+ *   log_probs      z - lse of the entry targets[r] (column, or id of the list); -inf if the row has none such
+ *   top_*  [m][k]  the k <= 128 largest, the earlier of equal ones first; -inf and -1 behind the last one
+ * A NaN or +inf makes its row's numbers NaN.  targets / log_probs may be NULL.  workspace: device, as
+ * many bytes as culsh_log_probs_workspace says, aligned to 16. */
+int culsh_log_probs_workspace(culsh_handle* h, int m, int64_t cols, int is_lists, int64_t total, uint64_t* bytes);
+int culsh_log_probs(culsh_handle* h, const void* scores, int type, int m, int64_t cols, int64_t ld, const int64_t* offsets,
+                    const int32_t* ids, int64_t total, double temperature, const int64_t* targets, int k, float* log_probs,
+                    float* entropy, float* lse, float* top_log_probs, int32_t* top_ids, void* workspace,
+                    uint64_t workspace_bytes, void* stream);
+/* grad_scores ([m][cols] without gaps, or as the lists; the scores' type) from the gradients of log_probs
+ * and entropy (either may be NULL) and what the forward call returned.  A log probability of -inf has
+ * no gradient, nor has an entry of -inf. */
+int culsh_log_probs_backward(culsh_handle* h, const void* scores, int type, int m, int64_t cols, int64_t ld,
+                             const int64_t* offsets, const int32_t* ids, int64_t total, double temperature,
+                             const int64_t* targets, const float* lse, const float* entropy, const float* grad_log_probs,
+                             const float* grad_entropy, void* grad_scores, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
