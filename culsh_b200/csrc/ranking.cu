@@ -33,6 +33,7 @@ void need(bool ok, const char* what) {
 }
 void check_rows(const void* codes, const void* scales, int n, int d) {
     need(n > 0 && d > 0, "rows and features must be positive");
+    need(n <= 0x7FFFFF80, "at most 2,147,483,520 rows");
     need(d <= 1 << 20, "at most 1,048,576 features");
     need(codes && scales, "null argument");
     need((((uintptr_t)codes | (uintptr_t)scales) & 15) == 0, "codes and scales have to begin at a multiple of 16 bytes");

@@ -186,7 +186,8 @@ class MXRows:
 
     def product(self, Q, metric: str = "dot", dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """Scores [n_queries, n_rows] of queries against every row: dot products, cosines or negative squared
-        distances ("euclidean").  ``Q``: MXRows, or an array that is held in 4 bits for the call."""
+        distances ("euclidean").  ``Q``: MXRows, or an array that is held in 4 bits for the call.  Rows of many scores begin at multiples of
+        128 bytes, so that the result of an odd number of rows is not contiguous."""
         m = _metric(metric)
         if dtype not in _SCORE_TYPES:
             raise TypeError(f"Unsupported dtype: {dtype}. Supported dtypes are float32, float16, bfloat16.")
@@ -196,12 +197,15 @@ class MXRows:
             raise ValueError(f"queries are on {Q.device}, rows on {self.device}")
         if Q._d != self._d:
             raise ValueError(f"Query features ({Q._d}) != row features ({self._d})")
-        out = torch.empty((Q._n, self._n), dtype=dtype, device=self.device)
+        # rows that share their first and last 32 bytes with others take the memory twice as long (1,000 x 999,999 float32 scores 2,036 us against 792)
+        line = 128 // dtype.itemsize
+        pitch = self._n if self._n < 8 * line else -(-self._n // line) * line
+        out = torch.empty((Q._n, pitch), dtype=dtype, device=self.device)[:, :self._n]
         if out.numel():
             h = self._h
             _lib.check(h.lib.culsh_mx_product(
                 h.ptr, Q.codes.data_ptr(), Q.scales.data_ptr(), Q.norms.data_ptr(), Q._n, self.codes.data_ptr(), self.scales.data_ptr(),
-                self.norms.data_ptr(), self._n, self._d, m, out.data_ptr(), _TYPES[dtype], self._n, _stream(self.device)))
+                self.norms.data_ptr(), self._n, self._d, m, out.data_ptr(), _TYPES[dtype], pitch, _stream(self.device)))
         return out
 
     def check(self) -> None:
