@@ -69,17 +69,35 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
                  "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+// A wait of a whole warp, with one answer.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_error) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, d_error));
+}
+// The MMAs are issued by a whole warp, whose elected lane (the same each time) does it: what a single lane computes on its own does not get into the uniform registers that these
+// instructions take their operands from without one instruction, and its latency, for each.
 // 32 rows of 16 bytes into four columns of 32 lanes, the same for each quarter of the lanes.
 __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xFFFFFFFF;\n\t"
+        "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc)
+        : "memory");
 }
 __device__ __forceinline__ void tc_mma_mxf4(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                             uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xFFFFFFFF;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
         ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_warp(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xFFFFFFFF;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
         : "memory");
 }
 // Descriptor of a K-major tile of SPAN-byte rows, swizzled over the span: groups of 8 rows one behind the other.
@@ -159,7 +177,7 @@ __device__ __forceinline__ void mx_epilogue_few(const MxProductArgs& a, uint32_t
         const int row = (int)u * MXP_B + quarter * 32 + lane;
         const float term = norm_term(a.metric, norm);
         norm = norm_of(u + gridDim.x);  // on its way while this unit is waited for
-        if (live) live = mbar_wait(&acc_full[ab], parity, s_abort, a.d_error);
+        if (live) live = mbar_wait_warp(&acc_full[ab], parity, s_abort, a.d_error);
         tc_fence_after();
         OUT* o = reinterpret_cast<OUT*>(a.out) + row;
         for (int q0 = 0; q0 < a.nq; q0 += 16) {
@@ -253,7 +271,7 @@ __device__ __forceinline__ void mx_epilogue_many(const MxProductArgs& a, uint32_
             __syncwarp();
             fetch(u + TURNS * gridDim.x);
         }
-        if (live) live = mbar_wait(&acc_full[ab], (nth / ACCS) & 1u, s_abort, a.d_error);
+        if (live) live = mbar_wait_warp(&acc_full[ab], (nth / ACCS) & 1u, s_abort, a.d_error);
         tc_fence_after();
         OUT* const o = reinterpret_cast<OUT*>(a.out) + (int64_t)q0 * a.ld + n0;
 #pragma unroll 1
@@ -356,38 +374,36 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t s = 0, parity = 0, ab = 0, acc_parity = 1, slot = 0;
-            bool live = true;
-            for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x) {
-                const MxUnit at(u, a);
-                const int ib = FEW ? at.chunk : at.tile;
-                const int n_mma = min(MXP_B, (a.b_rows - ib * MXP_B + 15) & ~15);
-                if (!mbar_wait(&acc_empty[ab], acc_parity, s_abort, a.d_error)) break;
+        uint32_t s = 0, parity = 0, ab = 0, acc_parity = 1, slot = 0;
+        bool live = true;
+        for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x) {
+            const MxUnit at(u, a);
+            const int ib = FEW ? at.chunk : at.tile;
+            const int n_mma = min(MXP_B, (a.b_rows - ib * MXP_B + 15) & ~15);
+            if (!mbar_wait_warp(&acc_empty[ab], acc_parity, s_abort, a.d_error)) break;
+            tc_fence_after();
+            const uint32_t d_tmem = tmem + ab * a.acc_cols;
+            const uint32_t id0 = mx_idesc(n_mma, 0), id1 = mx_idesc(n_mma, 2);
+            for (int g0 = 0; g0 < a.groups; g0 += Cfg::GROUPS) {
+                if (!mbar_wait_warp(&full[s], parity, s_abort, a.d_error)) { live = false; break; }
                 tc_fence_after();
-                const uint32_t d_tmem = tmem + ab * a.acc_cols;
-                const uint32_t id0 = mx_idesc(n_mma, 0), id1 = mx_idesc(n_mma, 2);
-                for (int g0 = 0; g0 < a.groups; g0 += Cfg::GROUPS) {
-                    if (!mbar_wait(&full[s], parity, s_abort, a.d_error)) { live = false; break; }
-                    tc_fence_after();
-                    const uint32_t st = smem_u32(base + (size_t)s * Cfg::STAGE_BYTES);
-                    const uint64_t da = mx_tile_desc<SPAN>(st), db = mx_tile_desc<SPAN>(st + Cfg::A_BYTES);
-                    const uint64_t dsa = mx_scale_desc(st + Cfg::A_BYTES + Cfg::B_BYTES), dsb = dsa + (Cfg::S_BYTES >> 4);
+                const uint32_t st = smem_u32(base + (size_t)s * Cfg::STAGE_BYTES);
+                const uint64_t da = mx_tile_desc<SPAN>(st), db = mx_tile_desc<SPAN>(st + Cfg::A_BYTES);
+                const uint64_t dsa = mx_scale_desc(st + Cfg::A_BYTES + Cfg::B_BYTES), dsb = dsa + (Cfg::S_BYTES >> 4);
 #pragma unroll
-                    for (int g = 0; g < Cfg::GROUPS; ++g) {
-                        const uint32_t sfa = tmem + Cfg::ACC_COLS + slot * 8, sfb = sfa + 4;
-                        if (++slot == Cfg::SF_SLOTS) slot = 0;
-                        tc_copy_scales(sfa, dsa + g * (MX_TILE_BYTES >> 4));
-                        tc_copy_scales(sfb, dsb + g * (MX_TILE_BYTES >> 4));
-                        tc_mma_mxf4(d_tmem, da + g * 4, db + g * 4, id0, sfa, sfb, (g0 | g) != 0);
-                        tc_mma_mxf4(d_tmem, da + g * 4 + 2, db + g * 4 + 2, id1, sfa, sfb, 1u);
-                    }
-                    tc_commit(&empty[s]);
-                    if (++s == STAGES) { s = 0; parity ^= 1u; }
+                for (int g = 0; g < Cfg::GROUPS; ++g) {
+                    const uint32_t sfa = tmem + Cfg::ACC_COLS + slot * 8, sfb = sfa + 4;
+                    if (++slot == Cfg::SF_SLOTS) slot = 0;
+                    tc_copy_scales(sfa, dsa + g * (MX_TILE_BYTES >> 4));
+                    tc_copy_scales(sfb, dsb + g * (MX_TILE_BYTES >> 4));
+                    tc_mma_mxf4(d_tmem, da + g * 4, db + g * 4, id0, sfa, sfb, (g0 | g) != 0);
+                    tc_mma_mxf4(d_tmem, da + g * 4 + 2, db + g * 4 + 2, id1, sfa, sfb, 1u);
                 }
-                if (live) tc_commit(&acc_full[ab]);
-                if (++ab == accs) { ab = 0; acc_parity ^= 1u; }
+                tc_commit_warp(&empty[s]);
+                if (++s == STAGES) { s = 0; parity ^= 1u; }
             }
+            if (live) tc_commit_warp(&acc_full[ab]);
+            if (++ab == accs) { ab = 0; acc_parity ^= 1u; }
         }
     } else {
         float* const terms = s_terms + (warp - 2) * Cfg::TERM_COUNT;

@@ -38,6 +38,9 @@ void check_rows(const void* codes, const void* scales, int n, int d) {
     need(codes && scales, "null argument");
     need((((uintptr_t)codes | (uintptr_t)scales) & 15) == 0, "codes and scales have to begin at a multiple of 16 bytes");
 }
+void need_workspace(const void* p, uint64_t have, size_t bytes) {
+    if (bytes && (have < bytes || !p || ((uintptr_t)p & 15))) fail(CULSH_ERR_INVALID, "the workspace has to be %zu bytes, aligned to 16", bytes);
+}
 cudaStream_t stream_of(void* stream) { return static_cast<cudaStream_t>(stream); }
 int* wait_word(const CtxPtr& c) { return c->d_error + 6; }
 
@@ -119,8 +122,17 @@ int culsh_mx_product_check(culsh_handle* h, void* stream) {
     });
 }
 
+int culsh_mx_score_workspace(culsh_handle* h, int n_queries, int d, int64_t total, uint64_t* bytes) {
+    return guarded([&] {
+        need(h && bytes, "null argument");
+        need(n_queries >= 0 && d > 0 && total >= 0, "sizes must not be negative");
+        *bytes = total ? mx_score_workspace(n_queries, d, total) : 0;
+    });
+}
+
 int culsh_mx_score(culsh_handle* h, const void* Q, int type, int n_queries, int64_t ldq, const uint8_t* codes, const uint8_t* scales, const float* norms,
-                   int n, int d, int metric, const int32_t* ids, const int64_t* offsets, int64_t total, float* out, void* stream) {
+                   int n, int d, int metric, const int32_t* ids, const int64_t* offsets, int64_t total, float* out, void* workspace,
+                   uint64_t workspace_bytes, void* stream) {
     return guarded([&] {
         need(h && Q && norms && offsets && (total == 0 || (ids && out)), "null argument");
         check_rows(codes, scales, n, d);
@@ -129,11 +141,12 @@ int culsh_mx_score(culsh_handle* h, const void* Q, int type, int n_queries, int6
         need(ldq >= d, "rows must not overlap");
         need(total >= 0, "total must not be negative");
         if (total == 0) return;
+        need_workspace(workspace, workspace_bytes, mx_score_workspace(n_queries, d, total));
         DeviceGuard g(h->ctx->device);
         MxScoreArgs a{};
         a.codes = codes, a.scales = scales, a.norms = norms, a.ids = ids, a.offsets = offsets, a.out = out;
         a.ldq = ldq, a.total = total, a.n = n, a.nq = n_queries, a.d = d, a.groups = mx_groups(d), a.metric = metric;
-        by_type(type, ALL_TYPES, Q, [&](auto* q) { mx_score(q, a, stream_of(stream)); });
+        by_type(type, ALL_TYPES, Q, [&](auto* q) { mx_score(h->ctx, q, a, workspace, wait_word(h->ctx), stream_of(stream)); });
     });
 }
 

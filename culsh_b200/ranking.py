@@ -230,9 +230,12 @@ class MXRows:
             if not self._n:
                 return out.fill_(float("nan"))
             h, stream = self._h, _stream(self.device)
+            need = C.c_uint64()
+            _lib.check(h.lib.culsh_mx_score_workspace(h.ptr, lists.n, self._d, lists.total, C.byref(need)))
+            work = torch.empty(need.value, dtype=torch.uint8, device=self.device)
             _lib.check(h.lib.culsh_mx_score(
                 h.ptr, Q.data_ptr(), _TYPES[Q.dtype], lists.n, _pitch(Q), self.codes.data_ptr(), self.scales.data_ptr(),
-                self.norms.data_ptr(), self._n, self._d, m, lists.ids, lists.offsets, lists.total, out.data_ptr(), stream))
+                self.norms.data_ptr(), self._n, self._d, m, lists.ids, lists.offsets, lists.total, out.data_ptr(), work.data_ptr(), need.value, stream))
             lists.done(h, stream)
         return out
 

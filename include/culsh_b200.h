@@ -336,10 +336,13 @@ int culsh_mx_product(culsh_handle* h, const uint8_t* q_codes, const uint8_t* q_s
  * (CULSH_ERR_INTERNAL; the scores that it should have made are NaN). */
 int culsh_mx_product_check(culsh_handle* h, void* stream);
 /* out[c], c in [offsets[q], offsets[q + 1]): the metric of query q as it is (any type, rows ldq apart)
- * and row ids[c]; NaN where ids[c] is no row.  offsets: n_queries + 1, from 0 to total. */
+ * and row ids[c]; NaN where ids[c] is no row.  offsets: n_queries + 1, from 0 to total.  Queries are taken in
+ * 32 bits; of a block's values, bits below 2^-126 of the largest do not count.  workspace: device, as many bytes as
+ * culsh_mx_score_workspace says, aligned to 16. */
+int culsh_mx_score_workspace(culsh_handle* h, int n_queries, int d, int64_t total, uint64_t* bytes);
 int culsh_mx_score(culsh_handle* h, const void* Q, int type, int n_queries, int64_t ldq, const uint8_t* codes,
                    const uint8_t* scales, const float* norms, int n, int d, int metric, const int32_t* ids,
-                   const int64_t* offsets, int64_t total, float* out, void* stream);
+                   const int64_t* offsets, int64_t total, float* out, void* workspace, uint64_t workspace_bytes, void* stream);
 /* What the result's handle does from now on waits for what the stream holds so far: call it behind work
  * that reads a result's device arrays (culsh_candidates_device_ptrs), which may then be freed at once. */
 int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* stream);

@@ -615,3 +615,75 @@ def test_refusals(culsh):
     with pytest.raises(RuntimeError, match="16 bytes"):  # codes that TMA cannot load
         codes = torch.zeros(10 * 64 + 16, dtype=torch.uint8, device="cuda")[1:641].view(10, 64)
         culsh.MXRows.from_parts(codes, rows.scales, rows.norms, 40).dequantize()
+
+
+@pytest.mark.parametrize("metric", ["dot", "cosine", "euclidean"])
+@pytest.mark.parametrize("d,nq,mean", [(100, 300, 1500), (128, 3, 150_000), (256, 40, 6000), (384, 30, 5000), (512, 500, 900), (700, 20, 4000), (2300, 9, 4000)])
+def test_score_of_many_candidates(culsh, d, nq, mean, metric):
+    """Lists long enough for the tensor cores, of all lengths around a tile's, with ids that are no rows, against float64 on the device."""
+    g, n = gen(d + nq), 200_000 if d <= 256 else 30_000
+    X = torch.randn(n, d, generator=g, device="cuda")
+    X[::1000] = 0
+    Q = torch.randn(nq, d, generator=g, device="cuda")
+    length = torch.randint(0, 2 * mean, (nq,), generator=g, device="cuda")
+    length[::5] = torch.tensor([0, 1, 127, 128, 129, 256, 383], device="cuda").repeat(nq)[:length[::5].numel()]
+    offsets = torch.zeros(nq + 1, dtype=torch.int64, device="cuda")
+    offsets[1:] = torch.cumsum(length, 0)
+    total = int(offsets[-1])
+    ids = torch.randint(0, n, (total,), generator=g, device="cuda").int()
+    ids[::977] = -1
+    ids[5::1013] = n
+    rows = culsh.MXRows(X)
+    got = rows.score(Q, (ids, offsets), metric=metric).double()
+    assert torch.equal(got.isnan(), (ids < 0) | (ids >= n))
+    x, q = rows.dequantize(torch.float64), Q.double()
+    owner = torch.repeat_interleave(torch.arange(nq, device="cuda"), length)
+    x2, q2 = (x * x).sum(1), (q * q).sum(1)
+    for at in range(0, total, 200_000):
+        i, o = ids[at:at + 200_000].long().clamp(0, n - 1), owner[at:at + 200_000]
+        dot, size = (x[i] * q[o]).sum(1), (x[i] * q[o]).abs().sum(1)
+        if metric == "dot":
+            want, bound = dot, (d + 2) * ULP * size
+        elif metric == "cosine":
+            length2 = (x2[i] * q2[o]).sqrt()
+            want = torch.where(length2 > 0, dot / length2, torch.zeros_like(dot))
+            bound = torch.where(length2 > 0, (2 * d + 10) * ULP * size / length2, torch.ones_like(dot) * ULP)
+        else:
+            want, bound = 2 * dot - x2[i] - q2[o], (d + 4) * ULP * (2 * size + x2[i] + q2[o])
+        part = got[at:at + 200_000]
+        assert bool(((part - want).abs() <= bound)[~part.isnan()].all())
+    assert torch.equal(rows.score(Q, (ids, offsets), metric=metric).nan_to_num(9.0), got.float().nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("law", ["one_term", "wide", "decades", "whole", "tiny", "huge"])
+def test_score_of_many_candidates_holds_small_terms_of_a_query(culsh, law):
+    d, n, times = 96, 96, 4000
+    X = torch.eye(n, device="cuda")
+    Q = torch.randn(3, d, generator=gen(1), device="cuda")
+    if law == "wide":
+        Q *= torch.exp2(torch.randint(-30, 31, (3, d), generator=gen(2), device="cuda").float())
+    elif law == "decades":
+        Q *= torch.exp2(torch.linspace(-50, 50, d, device="cuda"))[None]
+    elif law == "whole":
+        Q = torch.randint(-255, 256, (3, d), generator=gen(2), device="cuda").float()
+    elif law == "tiny":
+        Q *= 2.0 ** -90
+    elif law == "huge":
+        Q *= 2.0 ** 120
+    ids = torch.arange(n, dtype=torch.int32, device="cuda").repeat(3 * times)
+    got = culsh.MXRows(X).score(Q, (ids, torch.arange(4, device="cuda") * n * times)).view(3, times, n)
+    assert bool((got == got[:, :1]).all())
+    assert bool(((got[:, 0].double() - Q.double()).abs() <= ULP * Q.double().abs()).all())
+
+
+def test_score_of_more_queries_than_the_workspace_holds(culsh):
+    n, d, nq, each = 5000, 600, 4000, 130  # 2,900 of these queries are 64 MB of slices
+    X, Q = torch.randn(n, d, generator=gen(), device="cuda"), torch.randn(nq, d, generator=gen(1), device="cuda")
+    ids = torch.randint(0, n, (nq * each,), generator=gen(2), device="cuda").int()
+    offsets = torch.arange(nq + 1, device="cuda") * each
+    rows = culsh.MXRows(X)
+    got = rows.score(Q, (ids, offsets)).view(nq, each).double()
+    x = rows.dequantize(torch.float64)
+    for q in (0, 1, 2800, 2900, 3000, nq - 1):
+        r = x[ids[q * each:(q + 1) * each].long()] * Q[q].double()
+        assert bool(((got[q] - r.sum(1)).abs() <= (d + 2) * ULP * r.abs().sum(1)).all())
