@@ -33,5 +33,6 @@ if not _building:
     def __getattr__(name):
         if name in _RANKING:
             from . import ranking
-            return getattr(ranking, name)
+            globals().update((n, getattr(ranking, n)) for n in _RANKING)
+            return globals()[name]
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -102,11 +102,12 @@ SIGNATURES = {
     "culsh_mx_quantize": [VP, VP, I, I, I, I64, VP, VP, VP, VP],
     "culsh_mx_dequantize": [VP, VP, VP, I, I, VP, I, VP],
     "culsh_mx_product": [VP, VP, VP, VP, I, VP, VP, VP, I, I, I, VP, I, I64, VP],
+    "culsh_mx_product_dense": [VP, VP, I, I, I64, VP, VP, VP, I, I, I, VP, I, I64, VP, U64, VP],
     "culsh_mx_product_check": [VP, VP],
     "culsh_mx_score_workspace": [VP, I, I, I64, C.POINTER(C.c_uint64)],
     "culsh_mx_score": [VP, VP, I, I, I64, VP, VP, VP, I, I, I, VP, VP, I64, VP, VP, U64, VP],
     "culsh_candidates_after": [VP, VP, VP],
-    "culsh_log_probs_workspace": [VP, I, I64, I, I64, C.POINTER(C.c_uint64)],
+    "culsh_log_probs_workspace": [VP, I, I, I64, I, I64, C.POINTER(C.c_uint64)],
     "culsh_log_probs": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, I, VP, VP, VP, VP, VP, VP, U64, VP],
     "culsh_log_probs_backward": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, VP, VP, VP, VP, VP, VP],
 }

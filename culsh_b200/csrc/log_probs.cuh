@@ -2,17 +2,18 @@
 //   lse = log sum exp z,   log p of a given entry = z - lse,   entropy = lse - sum p z,   and the k most likely entries,
 // and the gradient of the first and the second with respect to s:  ds_i = (g ([i = given] - p_i) - h p_i (log p_i + entropy)) / temperature.
 //
-// One pass over the scores.  A warp takes chunks of 512 neighbouring entries, 16 to a lane, and keeps the largest score so far m and two sums relative to it,
+// One pass over the scores.  A warp takes chunks of 512 neighbouring entries, or 1,024 of 16 bits, and keeps the largest score so far m and two sums relative to it,
 //   l = sum 2^d,   e = sum d 2^d,   d = (s - m) log2(e) / temperature,
-// in 32 bits; entropy = log l - log(2) e / l.  A larger m rescales both.  Parts (m, l, e) are joined in a fixed order, so results do not depend on how CTAs are scheduled.
-// d is cut at -10,000, far below where 2^d is 0, so that an entry of -inf is 0 in both sums; m starts at the lowest finite value for the same reason.  NaN and +inf reach the sums and make
-// them NaN.
+// in 32 bits; entropy = log l - log(2) e / l.  A larger m rescales both.  d is one multiply-add, of s with the rounded product of m: what its rounding moved all d by is taken out of
+// the sums at the end.  Parts (m, l, e) are joined in a fixed order, so results do not depend on how CTAs are scheduled.  An entry of -inf counts as a score so low that 2^d is 0 and d is finite;
+// where m itself is that low, d is cut at -10,000 instead.  NaN and +inf reach the sums and make them NaN.
+// Sixteen bits: bound by the issue of five instructions and an exponential for an entry (a pass of eight took 579 us for 1,000 x 1M, this one NNN, of 305 at the copy's rate).
 //
-// The k largest come from the chunks' maxima, which the pass leaves behind: the k largest entries (the earlier of equal ones first) lie in the k chunks whose
-// maxima are the largest (the earlier of equal ones first), as every chunk before another in that order has an entry that comes before all of the other's.  So k chunks are read again,
-// whatever the scores are.
+// The k largest: the pass leaves the largest entry of each thread and of each chunk behind.  The k-th largest of the threads' is a bound that at least k entries reach, and hardly more do (of 1M
+// drawn at random and 256 threads about k + 1): only chunks that reach it are read again, and the entries that do are sorted, by score and then by place.  Where more entries are alike than
+// there is room to sort at once, they are sorted in turns.
 //
-// Rows begin anywhere: positions count from a 16-byte boundary at or in front of the array, chunks begin at multiples of 512 of those, and the first and the last one of a row
+// Rows begin anywhere: positions count from a 16-byte boundary at or in front of the array, chunks begin at multiples of their length of those, and the first and the last one of a row
 // load entry by entry.
 #pragma once
 
@@ -20,10 +21,14 @@
 
 namespace culsh_b200 {
 
-constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_PER_LANE = 16, LP_CHUNK = 32 * LP_PER_LANE;
-constexpr int LP_CHUNKS = 1024;                 // maxima that a CTA keeps of a row; a longer row's stand for several chunks each
-constexpr int LP_STEP = 4 * LP_THREADS;         // entries that are looked at before the collected ones are counted
-constexpr int LP_KEYS = 2 * LP_STEP, LP_MAX_K = 128;
+constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
+// A lane has 64 bytes of a chunk, and 64 of the next one on their way.
+template <typename T>
+constexpr int LP_PER_LANE = 64 / sizeof(T);
+template <typename T>
+constexpr int LP_CHUNK = 32 * LP_PER_LANE<T>;
+constexpr int LP_LEAST_CHUNK = 512, LP_MOST_CHUNK = 1024;
+constexpr int LP_MAX_K = 128;
 constexpr float LP_FLOOR = -10000.f;
 
 // Where rows are: a matrix with rows `ld` apart and `cols` long, or lists.  Positions of row r: [begin, end).
@@ -50,7 +55,7 @@ struct LpArgs {
     int m, k;
     float c, inv_t;           // log2(e) / temperature, 1 / temperature
     // rows taken by several CTAs
-    int64_t unit;             // positions of a CTA, a multiple of 512
+    int64_t unit;             // positions of a CTA, a multiple of 1,024
     int units_per_row;        // of a matrix
     float4* parts;
     uint32_t* maxima;         // of the chunks; row r's from chunk_slot(r) on
@@ -104,61 +109,163 @@ __device__ __forceinline__ float score_of(float s) { return s; }
 __device__ __forceinline__ float score_of(__half s) { return __half2float(s); }
 __device__ __forceinline__ float score_of(__nv_bfloat16 s) { return __bfloat162float(s); }
 
-// Position of entry i of a lane's 16 in its chunk.
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float warp_max(float v) {  // NaN where all are
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// A lane's scores of a chunk as they are loaded.  LOW: what -inf counts as, while the largest is above SAFE.
+template <typename T>
+struct LpRaw;
+template <>
+struct LpRaw<float> {
+    static constexpr float LOW = -1e34f, SAFE = -1e33f;
+    alignas(16) float v[LP_PER_LANE<float>];
+    __device__ __forceinline__ void put(int j, uint4 w) { *reinterpret_cast<uint4*>(&v[4 * j]) = w; }
+    __device__ __forceinline__ void set(int i, float s) { v[i] = s; }
+    __device__ __forceinline__ float get(int i) const { return v[i]; }
+    __device__ __forceinline__ float top() const {
+        float t = fmaxf(v[0], v[1]);
+#pragma unroll
+        for (int i = 2; i < LP_PER_LANE<float>; ++i) t = fmaxf(t, v[i]);
+        return t;
+    }
+    __device__ __forceinline__ float2 pair(int i) const { return make_float2(max_nan(v[2 * i], LOW), max_nan(v[2 * i + 1], LOW)); }
+};
+template <typename H>
+struct LpRaw16 {
+    alignas(16) uint32_t v[LP_PER_LANE<__half> / 2];
+    __device__ __forceinline__ void put(int j, uint4 w) { *reinterpret_cast<uint4*>(&v[4 * j]) = w; }
+    __device__ __forceinline__ uint32_t half(int i) const { return (i & 1) ? v[i >> 1] >> 16 : v[i >> 1] & 0xFFFFu; }
+    __device__ __forceinline__ void put_half(int i, uint32_t h) { v[i >> 1] = (i & 1) ? (v[i >> 1] & 0xFFFFu) | h << 16 : (v[i >> 1] & 0xFFFF0000u) | h; }
+};
+template <>
+struct LpRaw<__nv_bfloat16> : LpRaw16<__nv_bfloat16> {
+    static constexpr float LOW = -9.8e33f, SAFE = -1e33f;
+    __device__ __forceinline__ void set(int i, float s) { put_half(i, __float_as_uint(s) >> 16); }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(half(i) << 16); }
+    __device__ __forceinline__ float top() const {
+        uint32_t t = v[0];
+#pragma unroll
+        for (int i = 1; i < LP_PER_LANE<__half> / 2; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(t) : "r"(v[i]));
+        return fmaxf(__uint_as_float(t << 16), __uint_as_float(t & 0xFFFF0000u));
+    }
+    __device__ __forceinline__ float2 pair(int i) const {
+        uint32_t w;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(v[i]), "r"(0xF7F2F7F2u));  // LOW
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    }
+};
+template <>
+struct LpRaw<__half> : LpRaw16<__half> {
+    static constexpr float LOW = -65504.f, SAFE = -40000.f;
+    __device__ __forceinline__ void set(int i, float s) { put_half(i, __half_as_ushort(__float2half_rn(s))); }
+    __device__ __forceinline__ float get(int i) const { return __half2float(__ushort_as_half((unsigned short)half(i))); }
+    __device__ __forceinline__ float top() const {
+        uint32_t t = v[0];
+#pragma unroll
+        for (int i = 1; i < LP_PER_LANE<__half> / 2; ++i) asm("max.f16x2 %0, %0, %1;" : "+r"(t) : "r"(v[i]));
+        const float2 f = half_pair(t);
+        return fmaxf(f.x, f.y);
+    }
+    __device__ __forceinline__ float2 pair(int i) const {
+        uint32_t w;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(w) : "r"(v[i]), "r"(0xFBFFFBFFu));  // LOW
+        return half_pair(w);
+    }
+};
+
+// Position of a lane's entry i in its chunk.
 template <typename T>
 __device__ __forceinline__ int lp_place(int lane, int i) {
     constexpr int V = 16 / sizeof(T);
     return ((i / V) * 32 + lane) * V + i % V;
 }
-// The lane's 16 scores of a chunk, -inf outside [begin, end).  `x`: position 0.
+// The lane's scores of a chunk, -inf outside [begin, end).  `x`: position 0.
 template <typename T>
-__device__ __forceinline__ void lp_load(const T* __restrict__ x, int64_t chunk, int64_t begin, int64_t end, int lane, float (&s)[LP_PER_LANE]) {
+__device__ __forceinline__ void lp_load(const T* __restrict__ x, int64_t chunk, int64_t begin, int64_t end, int lane, LpRaw<T>& s) {
     constexpr int V = 16 / sizeof(T);
-    const int64_t p0 = chunk * LP_CHUNK;
-    if (p0 >= begin && p0 + LP_CHUNK <= end) {
-        uint4 w[LP_PER_LANE / V];
+    const int64_t p0 = chunk * LP_CHUNK<T>;
+    if (p0 >= begin && p0 + LP_CHUNK<T> <= end) {
 #pragma unroll
-        for (int j = 0; j < LP_PER_LANE / V; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(x + p0) + j * 32 + lane);
-#pragma unroll
-        for (int i = 0; i < LP_PER_LANE; ++i) s[i] = score_of(reinterpret_cast<const T*>(&w[i / V])[i % V]);
+        for (int j = 0; j < LP_PER_LANE<T> / V; ++j) s.put(j, __ldg(reinterpret_cast<const uint4*>(x + p0) + j * 32 + lane));
     } else {
 #pragma unroll
-        for (int i = 0; i < LP_PER_LANE; ++i) {
+        for (int i = 0; i < LP_PER_LANE<T>; ++i) {
             const int64_t p = p0 + lp_place<T>(lane, i);
-            s[i] = p >= begin && p < end ? score_of(x[p]) : -INFINITY;
+            s.set(i, p >= begin && p < end ? score_of(x[p]) : -INFINITY);
         }
     }
 }
 
-// A warp's chunks first, first + step, ... below last, all in one row; `leave(chunk, largest)` takes the maxima.
+// A warp's chunks first, first + step, ... below last, all in one row; `leave(chunk, top)` takes the chunks' maxima, `largest` becomes the
+// lane's.  The next chunk is on its way while one is summed.
 template <typename T, typename Leave>
 __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t first, int64_t last, int step, int64_t begin, int64_t end, float c, int lane,
-                                            Leave leave) {
-    LpPart part = LpPart::none();  // m is the same in all lanes
+                                            float& largest, Leave leave) {
+    float m = LpPart::none().m, mc = m * c;  // the same in all lanes; mc: what d counts from in the short way
+    const bool common = c > 0.01f && c < 1e4f;
+    auto in_short = [&]() { return common && m > LpRaw<T>::SAFE && fabsf(mc) < 1e33f; };
+    float2 l = make_float2(0.f, 0.f), e = l;
+    LpRaw<T> next;
+    if (first < last) lp_load(x, first, begin, end, lane, next);
+#pragma unroll 1
     for (int64_t chunk = first; chunk < last; chunk += step) {
-        float s[LP_PER_LANE];
-        lp_load(x, chunk, begin, end, lane, s);
-        float top = s[0];
-#pragma unroll
-        for (int i = 1; i < LP_PER_LANE; ++i) top = fmaxf(top, s[i]);
+        const LpRaw<T> s = next;
+        if (chunk + step < last) lp_load(x, chunk + step, begin, end, lane, next);
+        float top = s.top();
+        largest = fmaxf(largest, top);
+        top = warp_max(top);
         if (top != top) top = -INFINITY;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         leave(chunk, top);
-        if (top > part.m) part.raise(top, c);
-        float l0 = 0.f, l1 = 0.f, e0 = 0.f, e1 = 0.f;
-#pragma unroll
-        for (int i = 0; i < LP_PER_LANE; i += 2) {
-            const float d0 = max_nan((s[i] - part.m) * c, LP_FLOOR), d1 = max_nan((s[i + 1] - part.m) * c, LP_FLOOR);
-            const float p0 = exp2_fast(d0), p1 = exp2_fast(d1);
-            l0 += p0;
-            l1 += p1;
-            e0 = fmaf(p0, d0, e0);
-            e1 = fmaf(p1, d1, e1);
+        if (top > m) {
+            const float to = top * c, d = max_nan(in_short() ? mc - to : (m - top) * c, LP_FLOOR), f = exp2_fast(d);
+            e.x = (e.x + l.x * d) * f;
+            e.y = (e.y + l.y * d) * f;
+            l.x *= f;
+            l.y *= f;
+            m = top;
+            mc = to;
         }
-        part.l += l0 + l1;
-        part.e += e0 + e1;
+        if (in_short()) {
+            const float2 c2 = make_float2(c, c), from = make_float2(-mc, -mc);
+#pragma unroll
+            for (int i = 0; i < LP_PER_LANE<T> / 2; ++i) {
+                const float2 d = fma2(s.pair(i), c2, from), p = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+                l = add2(l, p);
+                e = fma2(p, d, e);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < LP_PER_LANE<T>; ++i) {
+                const float d = max_nan((s.get(i) - m) * c, LP_FLOOR), p = exp2_fast(d);
+                l.x += p;
+                e.x = fmaf(p, d, e.x);
+            }
+        }
     }
+    LpPart part{m, l.x + l.y, e.x + e.y};
+    const float off = in_short() ? fmaf(m, c, -mc) : 0.f, f = exp2_fast(-off);  // from mc to m itself
+    part.e = (part.e - off * part.l) * f;
+    part.l *= f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         part.l += __shfl_xor_sync(0xFFFFFFFFu, part.l, o);
@@ -167,30 +274,37 @@ __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t fir
     return part;
 }
 
+// What a CTA of TH threads shares.
+template <int TH>
 struct LpShared {
-    uint64_t keys[LP_KEYS];
-    uint32_t maxima[LP_CHUNKS];
-    LpPart parts[LP_WARPS];
+    static constexpr int CHUNKS = 4 * TH;     // maxima that a CTA keeps of a row; a longer row's stand for several chunks each
+    static constexpr int STEP = 4 * TH;       // entries that are looked at before the collected ones are counted
+    static constexpr int KEYS = STEP + (STEP > LP_MAX_K ? STEP : LP_MAX_K);
+    uint64_t keys[KEYS];
+    uint32_t maxima[CHUNKS];
+    LpPart parts[TH / 32];
     int count;
     int64_t target;  // position of the given entry, or -1
 };
 
 // The CTA's part from its warps', in the order of the warps; for all threads.
-__device__ __forceinline__ LpPart lp_join_warps(LpShared& sh, const LpPart& mine, float c) {
+template <int TH>
+__device__ __forceinline__ LpPart lp_join_warps(LpShared<TH>& sh, const LpPart& mine, float c) {
     if ((threadIdx.x & 31) == 0) sh.parts[threadIdx.x >> 5] = mine;
     __syncthreads();
     LpPart all = sh.parts[0];
 #pragma unroll
-    for (int w = 1; w < LP_WARPS; ++w) all.join(sh.parts[w], c);
+    for (int w = 1; w < TH / 32; ++w) all.join(sh.parts[w], c);
     return all;
 }
 
 // Sorts keys[0, n), n a power of two, the largest first.
+template <int TH>
 __device__ __forceinline__ void lp_sort(uint64_t* keys, int n) {
     for (int size = 2; size <= n; size *= 2) {
         for (int stride = size / 2; stride; stride >>= 1) {
             __syncthreads();
-            for (int i = threadIdx.x; i < n / 2; i += LP_THREADS) {
+            for (int i = threadIdx.x; i < n / 2; i += TH) {
                 const int at = 2 * i - (i & (stride - 1));
                 const uint64_t a = keys[at], b = keys[at + stride];
                 if ((a < b) == ((at & size) == 0)) {
@@ -203,34 +317,35 @@ __device__ __forceinline__ void lp_sort(uint64_t* keys, int n) {
     __syncthreads();
 }
 // Sorts the collected keys, keeps the k largest.
-__device__ __forceinline__ void lp_settle(LpShared& sh, int k) {
+template <int TH>
+__device__ __forceinline__ void lp_settle(LpShared<TH>& sh, int k) {
     __syncthreads();
     const int count = sh.count;
     int n = 2;
     while (n < count) n *= 2;
-    for (int i = count + threadIdx.x; i < n; i += LP_THREADS) sh.keys[i] = 0;
-    lp_sort(sh.keys, n);
+    for (int i = count + threadIdx.x; i < n; i += TH) sh.keys[i] = 0;
+    lp_sort<TH>(sh.keys, n);
     if (threadIdx.x == 0) sh.count = min(count, k);
     __syncthreads();
 }
 // The k largest keys of key(0 .. n - 1) that are at least `least`, sorted, into sh.keys; sh.count of them.  Keys differ from one another, 0 is none.
-template <typename Key>
-__device__ __forceinline__ void lp_largest(LpShared& sh, int64_t n, int k, uint64_t least, Key key) {
+template <int TH, typename Key>
+__device__ __forceinline__ void lp_largest(LpShared<TH>& sh, int64_t n, int k, uint64_t least, Key key) {
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    for (int64_t i0 = 0; i0 < n; i0 += LP_STEP) {
-        uint64_t v[LP_STEP / LP_THREADS];
+    for (int64_t i0 = 0; i0 < n; i0 += LpShared<TH>::STEP) {
+        uint64_t v[LpShared<TH>::STEP / TH];
 #pragma unroll
-        for (int j = 0; j < LP_STEP / LP_THREADS; ++j) {
-            const int64_t i = i0 + j * LP_THREADS + threadIdx.x;
+        for (int j = 0; j < LpShared<TH>::STEP / TH; ++j) {
+            const int64_t i = i0 + j * TH + threadIdx.x;
             v[j] = i < n ? key(i) : 0ull;
         }
 #pragma unroll
-        for (int j = 0; j < LP_STEP / LP_THREADS; ++j)
+        for (int j = 0; j < LpShared<TH>::STEP / TH; ++j)
             if (v[j] && v[j] >= least) sh.keys[atomicAdd(&sh.count, 1)] = v[j];
         __syncthreads();
-        if (sh.count > LP_KEYS - LP_STEP) {
+        if (sh.count > LpShared<TH>::KEYS - LpShared<TH>::STEP) {
             lp_settle(sh, k);
             if (sh.count == k) least = max(least, sh.keys[k - 1]);
         }
@@ -238,30 +353,51 @@ __device__ __forceinline__ void lp_largest(LpShared& sh, int64_t n, int k, uint6
     }
     lp_settle(sh, k);
 }
-
-// Position of the entry that `target` names in row r, or -1; by one warp.
-__device__ __forceinline__ int64_t lp_find(const LpArgs& a, int64_t begin, int64_t end, int64_t target) {
-    if (!a.ids) return target >= 0 && target < end - begin ? begin + target : -1;
-    const int lane = threadIdx.x & 31;
-    const int32_t* __restrict__ ids = a.ids - a.rows.shift;
-    int64_t lo = begin, hi = end;  // ids below lo are smaller, at and behind hi larger
-    while (hi > lo) {
-        const int64_t step = (hi - lo + 31) / 32, p = lo + lane * step;
-        const int32_t id = p < hi ? __ldg(ids + p) : 0x7FFFFFFF;
-        const unsigned smaller = __ballot_sync(0xFFFFFFFFu, p < hi && id < target), same = __ballot_sync(0xFFFFFFFFu, p < hi && id == target);
-        if (same) return lo + (int64_t)(__ffs((int)same) - 1) * step;
-        const int n = __popc(smaller);  // the first n probes
-        if (!n) return -1;
-        hi = min(hi, lo + n * step);
-        lo = lo + (n - 1) * step + 1;
-    }
-    return -1;
+// The k-th largest of the threads' scores, k <= TH.
+template <int TH>
+__device__ __forceinline__ float lp_bound(LpShared<TH>& sh, float mine, int k) {
+    __syncthreads();
+    sh.keys[threadIdx.x] = lp_order(mine);
+    lp_sort<TH>(sh.keys, TH);
+    const float bound = lp_score((uint32_t)sh.keys[k - 1]);
+    __syncthreads();
+    return bound;
 }
 
-// What a row's result is made of, by the whole CTA.  `maxima`: orders of the largest scores of groups of 512 << wide entries from first_chunk on.
-template <typename T>
-__device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs& a, LpShared& sh, int row, int64_t begin, int64_t end, LpPart all,
-                                          const uint32_t* maxima, int64_t first_chunk, int groups, int wide) {
+// Position of the entry that a target names in a row, or -1; by one warp.  The first 32 ids that it looks at can be asked for long before.
+struct LpFind {
+    int64_t lo, hi, step, target;  // ids below lo are smaller, at and behind hi larger
+    int32_t id;
+    __device__ __forceinline__ void probe(const int32_t* __restrict__ ids) {
+        step = (hi - lo + 31) / 32;
+        const int64_t p = lo + (threadIdx.x & 31) * step;
+        id = p < hi ? __ldg(ids + p) : 0x7FFFFFFF;
+    }
+    __device__ __forceinline__ LpFind(const LpArgs& a, int row, int64_t begin, int64_t end) : lo(begin), hi(end), step(1), target(__ldg(a.targets + row)), id(0) {
+        if (a.ids && hi > lo) probe(a.ids - a.rows.shift);
+    }
+    __device__ __forceinline__ int64_t operator()(const LpArgs& a) {
+        if (!a.ids) return target >= 0 && target < hi - lo ? lo + target : -1;
+        const int lane = threadIdx.x & 31;
+        while (hi > lo) {
+            const bool in = lo + lane * step < hi;
+            const unsigned smaller = __ballot_sync(0xFFFFFFFFu, in && id < target), same = __ballot_sync(0xFFFFFFFFu, in && id == target);
+            if (same) return lo + (int64_t)(__ffs((int)same) - 1) * step;
+            const int n = __popc(smaller);  // the first n probes
+            if (!n) return -1;
+            hi = min(hi, lo + n * step);
+            lo = lo + (n - 1) * step + 1;
+            if (hi > lo) probe(a.ids - a.rows.shift);
+        }
+        return -1;
+    }
+};
+
+// What a row's result is made of, by the whole CTA.  `maxima`: orders of the largest scores of groups of 1 << wide chunks from first_chunk on; `largest`: a thread's own score, of no
+// other's entry.
+template <int TH, typename T>
+__device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs& a, LpShared<TH>& sh, int row, int64_t begin, int64_t end, LpPart all,
+                                          const uint32_t* maxima, int64_t first_chunk, int64_t last_chunk, int wide, float largest) {
     const float log_l = logf(all.l);
     const float z_max = all.m * a.inv_t;
     float lse = z_max + log_l, entropy = log_l - 0.69314718056f * (all.e / all.l);
@@ -277,19 +413,39 @@ __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs&
         if (a.targets) a.log_probs[row] = sh.target < 0 ? -INFINITY : log_p(score_of(x[sh.target]));
     }
     if (!a.k) return;
-    lp_largest(sh, groups, a.k, 0, [&](int64_t g) { return (uint64_t)maxima[g] << 32 | (0xFFFFFFFFu - (uint32_t)g); });
-    const int kept = sh.count;
-    __shared__ uint32_t s_groups[LP_MAX_K];
-    for (int i = threadIdx.x; i < kept; i += LP_THREADS) s_groups[i] = 0xFFFFFFFFu - (uint32_t)sh.keys[i];
-    const uint64_t least = kept == a.k ? sh.keys[kept - 1] & 0xFFFFFFFF00000000ull : 0ull;  // k entries are as large as the k-th of the maxima
-    const int shift = 9 + wide;
-    lp_largest(sh, (int64_t)kept << shift, a.k, least, [&](int64_t i) {
-        const int64_t p = ((first_chunk + ((int64_t)s_groups[i >> shift] << wide)) << 9) + (i & ((1ll << shift) - 1));
-        if (p < begin || p >= end) return 0ull;
-        const uint32_t o = lp_order(score_of(x[p]));
-        return o ? (unsigned long long)o << 32 | (0xFFFFFFFFu - (uint32_t)(p - begin)) : 0ull;
-    });
-    for (int i = threadIdx.x; i < a.k; i += LP_THREADS) {
+    const float bound = lp_bound(sh, largest, a.k);
+    const uint32_t least = max(lp_order(bound), 0x00800000u);  // more than -inf
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int64_t c0 = first_chunk + warp * 32; c0 < last_chunk; c0 += TH) {  // a lane looks at a chunk's maximum
+        const int64_t mine = c0 + lane;
+        unsigned reach = __ballot_sync(0xFFFFFFFFu, mine < last_chunk && maxima[(mine - first_chunk) >> wide] >= least);
+        for (; reach; reach &= reach - 1) {
+            const int64_t chunk = c0 + __ffs((int)reach) - 1;
+            LpRaw<T> s;
+            lp_load(x, chunk, begin, end, lane, s);
+            if (!(s.top() >= bound)) continue;
+#pragma unroll
+            for (int j = 0; j < LP_PER_LANE<T>; ++j) {
+                const float v = s.get(j);
+                if (v >= bound && v > -INFINITY) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < LpShared<TH>::KEYS) sh.keys[at] = (uint64_t)lp_order(v) << 32 | (0xFFFFFFFFu - (uint32_t)(chunk * LP_CHUNK<T> + lp_place<T>(lane, j) - begin));
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (sh.count <= LpShared<TH>::KEYS) {
+        lp_settle(sh, a.k);
+    } else {  // many that are alike
+        lp_largest(sh, end - begin, a.k, (uint64_t)least << 32, [&](int64_t i) {
+            const float v = score_of(x[begin + i]);
+            return v > -INFINITY ? (unsigned long long)lp_order(v) << 32 | (0xFFFFFFFFu - (uint32_t)i) : 0ull;
+        });
+    }
+    for (int i = threadIdx.x; i < a.k; i += TH) {
         float lp = -INFINITY;
         int32_t id = -1;
         if (i < sh.count) {
@@ -305,29 +461,35 @@ __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs&
     }
 }
 
-// A CTA for each row.
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_row_kernel(const T* __restrict__ x, LpArgs a) {
-    __shared__ LpShared sh;
+// A CTA of TH threads for each row.
+template <int TH, typename T>
+__global__ void __launch_bounds__(TH) log_probs_row_kernel(const T* __restrict__ x, LpArgs a) {
+    __shared__ LpShared<TH> sh;
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t begin = a.rows.begin(row), end = a.rows.end(row);
-    const int64_t first = begin / LP_CHUNK, last = end > begin ? (end + LP_CHUNK - 1) / LP_CHUNK : first;
+    const int64_t first = begin / LP_CHUNK<T>, last = end > begin ? (end + LP_CHUNK<T> - 1) / LP_CHUNK<T> : first;
     int wide = 0;
-    while ((last - first + (1ll << wide) - 1) >> wide > LP_CHUNKS) ++wide;
+    while ((last - first + (1ll << wide) - 1) >> wide > LpShared<TH>::CHUNKS) ++wide;
     const int groups = (int)((last - first + (1ll << wide) - 1) >> wide);
     if (a.k) {
-        for (int i = threadIdx.x; i < groups; i += LP_THREADS) sh.maxima[i] = 0;
+        for (int i = threadIdx.x; i < groups; i += TH) sh.maxima[i] = 0;
         __syncthreads();
     }
-    if (warp == 0 && a.targets) {
-        const int64_t at = lp_find(a, begin, end, __ldg(a.targets + row));
-        if (lane == 0) sh.target = at;
-    }
-    const LpPart mine = lp_chunks(x, first + warp, last, LP_WARPS, begin, end, a.c, lane, [&](int64_t chunk, float top) {
+    auto leave = [&](int64_t chunk, float top) {
         if (a.k && lane == 0) atomicMax(&sh.maxima[(chunk - first) >> wide], lp_order(top));
-    });
+    };
+    LpPart mine;
+    float largest = -INFINITY;
+    if (warp == TH / 32 - 1 && a.targets) {  // the warp with the fewest chunks
+        LpFind find(a, row, begin, end);
+        mine = lp_chunks(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
+        const int64_t at = find(a);
+        if (lane == 0) sh.target = at;
+    } else {
+        mine = lp_chunks(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
+    }
     const LpPart all = lp_join_warps(sh, mine, a.c);
-    lp_finish(x, a, sh, row, begin, end, all, sh.maxima, first, groups, wide);
+    lp_finish(x, a, sh, row, begin, end, all, sh.maxima, first, last, wide, largest);
 }
 
 // Rows taken by several CTAs.  Slots of a row's units and chunks: blocks of `size` positions from the one that it begins in on; lists share the numbering of all
@@ -335,11 +497,12 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_row_kernel(const T* __re
 __device__ __forceinline__ int64_t lp_slot(const LpArgs& a, int row, int64_t begin, int64_t size, int64_t per_row) {
     return a.rows.offsets ? begin / size + row : (int64_t)row * per_row;
 }
-__device__ __forceinline__ int64_t lp_chunks_per_row(const LpArgs& a) { return a.rows.cols / LP_CHUNK + 2; }
+template <typename T>
+__device__ __forceinline__ int64_t lp_chunks_per_row(const LpArgs& a) { return a.rows.cols / LP_CHUNK<T> + 2; }
 
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __restrict__ x, LpArgs a) {
-    __shared__ LpShared sh;
+    __shared__ LpShared<LP_THREADS> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int row;
     int64_t nth;
@@ -359,8 +522,9 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __r
     const int64_t begin = a.rows.begin(row), end = a.rows.end(row);
     const int64_t from = max((begin / a.unit + nth) * a.unit, begin), to = min((begin / a.unit + nth + 1) * a.unit, end);
     if (from >= to) return;
-    const int64_t slot = lp_slot(a, row, begin, LP_CHUNK, lp_chunks_per_row(a)), first = begin / LP_CHUNK;
-    const LpPart mine = lp_chunks(x, from / LP_CHUNK + warp, (to + LP_CHUNK - 1) / LP_CHUNK, LP_WARPS, begin, end, a.c, lane, [&](int64_t chunk, float top) {
+    const int64_t slot = lp_slot(a, row, begin, LP_CHUNK<T>, lp_chunks_per_row<T>(a)), first = begin / LP_CHUNK<T>;
+    float largest = -INFINITY;
+    const LpPart mine = lp_chunks(x, from / LP_CHUNK<T> + warp, (to + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, a.c, lane, largest, [&](int64_t chunk, float top) {
         if (a.k && lane == 0) a.maxima[slot + chunk - first] = lp_order(top);
     });
     const LpPart all = lp_join_warps(sh, mine, a.c);
@@ -369,11 +533,11 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __r
 
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __restrict__ x, LpArgs a) {
-    __shared__ LpShared sh;
+    __shared__ LpShared<LP_THREADS> sh;
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t begin = a.rows.begin(row), end = a.rows.end(row);
     if (warp == 0 && a.targets) {
-        const int64_t at = lp_find(a, begin, end, __ldg(a.targets + row));
+        const int64_t at = LpFind(a, row, begin, end)(a);
         if (lane == 0) sh.target = at;
     }
     const int64_t units = end > begin ? (end - 1) / a.unit - begin / a.unit + 1 : 0, slot = lp_slot(a, row, begin, a.unit, a.units_per_row);
@@ -385,8 +549,19 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __r
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine.join(mine.shuffled(o), a.c);
     const LpPart all = lp_join_warps(sh, mine, a.c);
-    const int64_t first = begin / LP_CHUNK, last = end > begin ? (end + LP_CHUNK - 1) / LP_CHUNK : first;
-    lp_finish(x, a, sh, row, begin, end, all, a.maxima + lp_slot(a, row, begin, LP_CHUNK, lp_chunks_per_row(a)), first, (int)(last - first), 0);
+    const int64_t first = begin / LP_CHUNK<T>, last = end > begin ? (end + LP_CHUNK<T> - 1) / LP_CHUNK<T> : first;
+    const uint32_t* const maxima = a.maxima + lp_slot(a, row, begin, LP_CHUNK<T>, lp_chunks_per_row<T>(a));
+    float largest = -INFINITY;
+    if (a.k && last - first >= LP_THREADS) {  // of every 256th chunk
+        for (int64_t c = threadIdx.x; c < last - first; c += LP_THREADS) largest = fmaxf(largest, lp_score(max(maxima[c], 0x007FFFFFu)));
+    } else if (a.k) {  // too few: of every eighth chunk's entries of a lane
+        for (int64_t c = first + warp; c < last; c += LP_WARPS) {
+            LpRaw<T> s;
+            lp_load(x, c, begin, end, lane, s);
+            largest = fmaxf(largest, s.top());
+        }
+    }
+    lp_finish(x, a, sh, row, begin, end, all, maxima, first, last, 0, largest);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -415,7 +590,7 @@ __device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, cons
     float g = b.f.targets && b.g ? __ldg(b.g + row) : 0.f;
     r.target = -1;
     if (b.f.targets && b.g) {
-        r.target = lp_find(b.f, begin, end, __ldg(b.f.targets + row));
+        r.target = LpFind(b.f, row, begin, end)(b.f);
         if (r.target < 0 || score_of(x[r.target]) * b.f.inv_t == -INFINITY) {  // a log probability of -inf stays where it is
             r.target = -1;
             g = 0.f;
@@ -449,13 +624,13 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_backward_kernel(const T*
     if (rows.offsets) {
         if (n >= b.chunks) return;
         chunk = n;
-        row = owner_of(rows.offsets, b.f.m, max(chunk * LP_CHUNK - rows.shift, (int64_t)0));
+        row = owner_of(rows.offsets, b.f.m, max(chunk * LP_LEAST_CHUNK - rows.shift, (int64_t)0));
     } else {
         row = (int)(n / b.chunks);
         if (row >= b.f.m) return;
-        chunk = rows.begin(row) / LP_CHUNK + n % b.chunks;
+        chunk = rows.begin(row) / LP_LEAST_CHUNK + n % b.chunks;
     }
-    const int64_t p0 = chunk * LP_CHUNK, p1 = p0 + LP_CHUNK;
+    const int64_t p0 = chunk * LP_LEAST_CHUNK, p1 = p0 + LP_LEAST_CHUNK;
     for (; row < b.f.m; ++row) {
         const int64_t begin = rows.begin(row), end = rows.end(row);
         if (begin >= p1) break;
@@ -481,17 +656,18 @@ struct LpPlan {
     size_t bytes() const { return split ? (size_t)units * sizeof(float4) + (size_t)chunks * sizeof(uint32_t) : 0; }
 };
 
-// Rows that fill the chip with a CTA each, and short ones, take one; others are taken by several.  total: entries of all lists.
-inline LpPlan lp_plan(int m, int64_t cols, int64_t total, bool lists, int sm_count) {
+// A row takes one CTA, or several where that is sooner: one of 128 threads takes 8 KB of a row in a microsecond, all of them together 6 GB in a millisecond, and joining the parts 15 us and
+// 0.07 for each row (300 rows of 100,000 bfloat16 36 us in one CTA each and 49 in several; 600 of 1M 264 and 240).  total: entries of all lists; size: bytes of one.
+inline LpPlan lp_plan(int m, int64_t cols, int64_t total, bool lists, int size, int sm_count) {
     LpPlan p;
     const int64_t entries = lists ? total : (int64_t)m * cols, mean = m ? entries / m : 0;
-    p.split = m < 4 * sm_count && mean > 16384;
+    p.split = mean > 16384 && (double)mean * size / 8200 > (double)entries * size / 6e6 + 15 + 0.07 * m;
     if (!p.split) return p;
     p.unit = 4096;
     while (p.unit < 32768 && entries / p.unit > 16ll * sm_count) p.unit *= 2;
     p.units_per_row = (int)(cols / p.unit + 2);
     p.units = lists ? (total + 16) / p.unit + m + 1 : (int64_t)m * p.units_per_row;
-    p.chunks = lists ? (total + 16) / LP_CHUNK + m + 1 : (int64_t)m * (cols / LP_CHUNK + 2);
+    p.chunks = lists ? (total + 16) / LP_LEAST_CHUNK + m + 1 : (int64_t)m * (cols / LP_LEAST_CHUNK + 2);
     return p;
 }
 
@@ -500,9 +676,15 @@ inline void log_probs(const CtxPtr& c, const T* scores, LpArgs a, void* workspac
     constexpr int V = 16 / sizeof(T);
     a.rows.shift = (int64_t)((uintptr_t)scores / sizeof(T) % V);
     const T* x = scores - a.rows.shift;
-    const LpPlan p = lp_plan(a.m, a.rows.cols, a.rows.total, a.rows.offsets != nullptr, c->sm_count);
+    const LpPlan p = lp_plan(a.m, a.rows.cols, a.rows.total, a.rows.offsets != nullptr, sizeof(T), c->sm_count);
     if (!p.split) {
-        log_probs_row_kernel<T><<<(unsigned)a.m, LP_THREADS, 0, stream>>>(x, a);
+        // What follows the pass is mostly waits, which an SM hides among many rows.  With fewer rows than it takes, larger CTAs do (10,000 lists of 18,000 float32: 32 threads 211 us, 128
+        // 239; 20,000 of 300: 72 and 170; 2,000 of 60,000: 307 and 137).  The bound of the k largest takes k threads.
+        const int64_t mean = a.rows.offsets ? a.rows.total / a.m : a.rows.cols;
+        int th = mean <= 1024 || (a.m >= 32 * c->sm_count && mean <= 32768) ? 32 : a.m >= 16 * c->sm_count && mean <= 16384 ? 64 : 128;
+        while (th < a.k) th *= 2;
+        auto kern = th == 32 ? log_probs_row_kernel<32, T> : th == 64 ? log_probs_row_kernel<64, T> : log_probs_row_kernel<128, T>;
+        kern<<<(unsigned)a.m, th, 0, stream>>>(x, a);
         KERNEL_CHECK();
         return;
     }
@@ -523,8 +705,8 @@ inline void log_probs_backward(const T* scores, T* out, LpBackward b, cudaStream
     constexpr int V = 16 / sizeof(T);
     LpRows& r = b.f.rows;
     r.shift = (int64_t)((uintptr_t)scores / sizeof(T) % V);
-    if (r.offsets) b.chunks = (int64_t)ceil_div((size_t)(r.total + r.shift), LP_CHUNK);
-    else b.chunks = r.cols / LP_CHUNK + 2;
+    if (r.offsets) b.chunks = (int64_t)ceil_div((size_t)(r.total + r.shift), LP_LEAST_CHUNK);
+    else b.chunks = r.cols / LP_LEAST_CHUNK + 2;
     const size_t grid = ceil_div(r.offsets ? (size_t)b.chunks : (size_t)b.chunks * b.f.m, LP_WARPS);
     if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "too many entries for one call");
     log_probs_backward_kernel<T><<<(unsigned)grid, LP_THREADS, 0, stream>>>(scores - r.shift, out, b);

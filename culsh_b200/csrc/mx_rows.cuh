@@ -202,6 +202,9 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __res
 // ------------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------------
+// Bytes of n rows: codes, scales, norms, one behind the other.
+inline size_t mx_bytes(int n, int d) { return (size_t)n * mx_groups(d) * (MX_GROUP / 2) + (size_t)mx_tiles(n) * mx_groups(d) * MX_TILE_BYTES + (size_t)n * 4; }
+
 inline bool aligned16(const void* p, int64_t pitch_bytes) { return (((uintptr_t)p | (uintptr_t)pitch_bytes) & 15u) == 0; }
 
 template <typename T>

@@ -109,6 +109,29 @@ int culsh_mx_product(culsh_handle* h, const uint8_t* q_codes, const uint8_t* q_s
     });
 }
 
+int culsh_mx_product_dense(culsh_handle* h, const void* Q, int q_type, int n_queries, int64_t ldq, const uint8_t* codes, const uint8_t* scales,
+                           const float* norms, int n, int d, int metric, void* out, int type, int64_t ld, void* workspace, uint64_t workspace_bytes,
+                           void* stream) {
+    return guarded([&] {
+        need(h && Q && out && norms, "null argument");
+        check_rows(codes, scales, n, d);
+        need(n_queries > 0, "queries must be positive");
+        need(metric >= 0 && metric <= 2, "metric must be 0, 1 or 2");
+        need(ld >= n && ldq >= d, "rows must not overlap");
+        need_workspace(workspace, workspace_bytes, mx_bytes(n_queries, d));
+        DeviceGuard g(h->ctx->device);
+        uint8_t* const q_codes = static_cast<uint8_t*>(workspace);
+        uint8_t* const q_scales = q_codes + (size_t)n_queries * mx_groups(d) * (MX_GROUP / 2);
+        float* const q_norms = reinterpret_cast<float*>(q_scales + (size_t)mx_tiles(n_queries) * mx_groups(d) * MX_TILE_BYTES);
+        by_type(type, SCORE_TYPES, out, [&](auto* o) {
+            if constexpr (!std::is_same<decltype(o), double*>::value) {
+                by_type(q_type, ALL_TYPES, Q, [&](auto* q) { mx_quantize(q, n_queries, d, ldq, q_codes, q_scales, q_norms, stream_of(stream)); });
+                mx_product(h->ctx, q_codes, q_scales, q_norms, n_queries, codes, scales, norms, n, d, metric, o, ld, wait_word(h->ctx), stream_of(stream));
+            }
+        });
+    });
+}
+
 int culsh_mx_product_check(culsh_handle* h, void* stream) {
     return guarded([&] {
         need(h, "null handle");
@@ -159,11 +182,11 @@ int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* str
     });
 }
 
-int culsh_log_probs_workspace(culsh_handle* h, int m, int64_t cols, int is_lists, int64_t total, uint64_t* bytes) {
+int culsh_log_probs_workspace(culsh_handle* h, int type, int m, int64_t cols, int is_lists, int64_t total, uint64_t* bytes) {
     return guarded([&] {
         need(h && bytes, "null argument");
         need(m > 0 && cols >= 0 && total >= 0, "sizes must not be negative");
-        *bytes = lp_plan(m, cols, total, is_lists != 0, h->ctx->sm_count).bytes();
+        *bytes = lp_plan(m, cols, total, is_lists != 0, type == CULSH_F32 ? 4 : 2, h->ctx->sm_count).bytes();
     });
 }
 

@@ -16,6 +16,7 @@ return when their work is queued.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple, Optional, Tuple, Union
 
 import numpy as np
@@ -43,7 +44,8 @@ def _on_device(x, device=None) -> torch.Tensor:
 
 def _matrix(x, device=None) -> torch.Tensor:
     """A 2-D CUDA tensor whose rows have no gaps inside and do not overlap."""
-    x = _on_device(x, device)
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and (device is None or x.device == device)):
+        x = _on_device(x, device)
     if x.ndim != 2:
         raise ValueError(f"Expected 2D array, got {x.ndim}D")
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
@@ -55,8 +57,11 @@ def _pitch(x: torch.Tensor) -> int:
     return int(x.stride(0)) if x.shape[0] > 1 else max(int(x.shape[1]), 1)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without a Stream object, whose making costs as much as an allocation
+
+
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
 
 
 def _metric(name: str) -> int:
@@ -66,12 +71,13 @@ def _metric(name: str) -> int:
 
 
 def _floats(x, name, shape, device) -> torch.Tensor:
-    x = _on_device(x, device)
-    if tuple(x.shape) != tuple(shape):
+    if not (isinstance(x, torch.Tensor) and x.device == device):
+        x = _on_device(x, device)
+    if x.shape != shape:
         raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(x.shape)}")
     if x.dtype != torch.float32:
         raise TypeError(f"{name} must be float32, got {x.dtype}")
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
 class _Lists:
@@ -132,18 +138,17 @@ class MXRows:
         n, d = int(X.shape[0]), int(X.shape[1])
         if d == 0:
             raise ValueError("rows have no features")
-        self._allocate(n, d, X.device)
+        self._n, self._d, self._h = n, d, get_handle(X.device.index)
+        groups = -(-d // 128)
+        # codes and scales in one allocation; the tensors that show them are made when they are asked for
+        self._codes = self._scales = None
+        self._held = torch.empty(64 * groups * n + 512 * groups * -(-n // 128), dtype=torch.uint8, device=X.device)
+        self.norms = torch.empty(n, dtype=torch.float32, device=X.device)
+        at = self._held.data_ptr()
+        self._at = (at, at + 64 * groups * n, self.norms.data_ptr())
         if n:
             h = self._h
-            _lib.check(h.lib.culsh_mx_quantize(h.ptr, X.data_ptr(), _TYPES[X.dtype], n, d, _pitch(X), self.codes.data_ptr(),
-                                               self.scales.data_ptr(), self.norms.data_ptr(), _stream(X.device)))
-
-    def _allocate(self, n, d, device):
-        groups, tiles = -(-d // 128), -(-n // 128)
-        self._n, self._d, self._h = n, d, get_handle(device.index)
-        self.codes = torch.empty((n, 64 * groups), dtype=torch.uint8, device=device)
-        self.scales = torch.empty((tiles, groups, 32, 4, 4), dtype=torch.uint8, device=device)
-        self.norms = torch.empty(n, dtype=torch.float32, device=device)
+            _lib.check(h.lib.culsh_mx_quantize(h.ptr, X.data_ptr(), _TYPES[X.dtype], n, d, _pitch(X), *self._at, _stream(X.device)))
 
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, norms: torch.Tensor, n_features: int) -> "MXRows":
@@ -164,12 +169,26 @@ class MXRows:
             raise ValueError("codes, scales and norms must be on one CUDA device")
         self = cls.__new__(cls)
         self._n, self._d, self._h = n, d, get_handle(codes.device.index)
-        self.codes, self.scales, self.norms = codes.contiguous(), scales.contiguous(), norms.contiguous()
+        self._codes, self._scales, self.norms = codes.contiguous(), scales.contiguous(), norms.contiguous()
+        self._at = (self._codes.data_ptr(), self._scales.data_ptr(), self.norms.data_ptr())
         return self
 
     n_rows = property(lambda self: self._n)
     n_features = property(lambda self: self._d)
-    device = property(lambda self: self.codes.device)
+    device = property(lambda self: self.norms.device)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._held[:64 * -(-self._d // 128) * self._n].view(self._n, -1) if self._n else self._held.view(0, 64 * -(-self._d // 128))
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            groups = -(-self._d // 128)
+            self._scales = self._held[64 * groups * self._n:].view(-(-self._n // 128), groups, 32, 4, 4)
+        return self._scales
 
     def size_bytes(self) -> int:
         return self.codes.numel() + self.scales.numel() + 4 * self.norms.numel()
@@ -180,8 +199,8 @@ class MXRows:
             raise TypeError(f"Unsupported dtype: {dtype}. Supported dtypes are float32, float64, float16, bfloat16.")
         out = torch.empty((self._n, self._d), dtype=dtype, device=self.device)
         if self._n:
-            _lib.check(self._h.lib.culsh_mx_dequantize(self._h.ptr, self.codes.data_ptr(), self.scales.data_ptr(), self._n, self._d,
-                                                       out.data_ptr(), _TYPES[dtype], _stream(self.device)))
+            _lib.check(self._h.lib.culsh_mx_dequantize(self._h.ptr, self._at[0], self._at[1], self._n, self._d, out.data_ptr(), _TYPES[dtype],
+                                                       _stream(self.device)))
         return out
 
     def product(self, Q, metric: str = "dot", dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -191,21 +210,36 @@ class MXRows:
         m = _metric(metric)
         if dtype not in _SCORE_TYPES:
             raise TypeError(f"Unsupported dtype: {dtype}. Supported dtypes are float32, float16, bfloat16.")
-        if not isinstance(Q, MXRows):
-            Q = MXRows(_matrix(Q, self.device))
-        elif Q.device != self.device:
-            raise ValueError(f"queries are on {Q.device}, rows on {self.device}")
-        if Q._d != self._d:
-            raise ValueError(f"Query features ({Q._d}) != row features ({self._d})")
+        device = self.device
+        held = isinstance(Q, MXRows)
+        if held:
+            if Q.device != device:
+                raise ValueError(f"queries are on {Q.device}, rows on {device}")
+            nq, d = Q._n, Q._d
+        else:
+            Q = _matrix(Q, device)
+            if Q.dtype not in _TYPES:
+                raise TypeError(f"Unsupported dtype: {Q.dtype}. Supported dtypes are float32, float64, float16, bfloat16.")
+            nq, d = Q.shape
+        if d != self._d:
+            raise ValueError(f"Query features ({d}) != row features ({self._d})")
+        n = self._n
         # rows that share their first and last 32 bytes with others take the memory twice as long (1,000 x 999,999 float32 scores 2,036 us against 792)
         line = 128 // dtype.itemsize
-        pitch = self._n if self._n < 8 * line else -(-self._n // line) * line
-        out = torch.empty((Q._n, pitch), dtype=dtype, device=self.device)[:, :self._n]
-        if out.numel():
-            h = self._h
-            _lib.check(h.lib.culsh_mx_product(
-                h.ptr, Q.codes.data_ptr(), Q.scales.data_ptr(), Q.norms.data_ptr(), Q._n, self.codes.data_ptr(), self.scales.data_ptr(),
-                self.norms.data_ptr(), self._n, self._d, m, out.data_ptr(), _TYPES[dtype], pitch, _stream(self.device)))
+        pitch = n if n < 8 * line else -(-n // line) * line
+        out = torch.empty((nq, pitch), dtype=dtype, device=device)
+        if pitch != n:
+            out = out[:, :n]
+        if n and nq:
+            h, stream = self._h, _stream(device)
+            if held:
+                _lib.check(h.lib.culsh_mx_product(h.ptr, *Q._at, nq, *self._at, n, d, m, out.data_ptr(), _TYPES[dtype], pitch, stream))
+            else:
+                groups = -(-d // 128)
+                need = 64 * groups * nq + 512 * groups * -(-nq // 128) + 4 * nq
+                work = torch.empty(need, dtype=torch.uint8, device=device)
+                _lib.check(h.lib.culsh_mx_product_dense(h.ptr, Q.data_ptr(), _TYPES[Q.dtype], nq, _pitch(Q), *self._at, n, d, m, out.data_ptr(),
+                                                        _TYPES[dtype], pitch, work.data_ptr(), need, stream))
         return out
 
     def check(self) -> None:
@@ -232,10 +266,10 @@ class MXRows:
             h, stream = self._h, _stream(self.device)
             need = C.c_uint64()
             _lib.check(h.lib.culsh_mx_score_workspace(h.ptr, lists.n, self._d, lists.total, C.byref(need)))
-            work = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+            work = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
             _lib.check(h.lib.culsh_mx_score(
-                h.ptr, Q.data_ptr(), _TYPES[Q.dtype], lists.n, _pitch(Q), self.codes.data_ptr(), self.scales.data_ptr(),
-                self.norms.data_ptr(), self._n, self._d, m, lists.ids, lists.offsets, lists.total, out.data_ptr(), work.data_ptr(), need.value, stream))
+                h.ptr, Q.data_ptr(), _TYPES[Q.dtype], lists.n, _pitch(Q), *self._at, self._n, self._d, m, lists.ids, lists.offsets, lists.total,
+                out.data_ptr(), work.data_ptr() if need.value else None, need.value, stream))
             lists.done(h, stream)
         return out
 
@@ -273,12 +307,13 @@ def _scores(scores, lists):
 def _targets(targets, lists, m, device):
     if targets is None:
         return None
-    targets = _on_device(targets, device)
-    if tuple(targets.shape) != (m,) or targets.dtype not in (torch.int64, torch.int32):
+    if not (isinstance(targets, torch.Tensor) and targets.device == device):
+        targets = _on_device(targets, device)
+    if targets.shape != (m,) or targets.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"targets must be int64 or int32 of the shape {(m,)}, got {targets.dtype} {tuple(targets.shape)}")
     if lists is not None and not lists.ids:
         raise ValueError("targets of lists need the lists' ids")
-    return targets.to(torch.int64).contiguous()
+    return targets if targets.dtype == torch.int64 and targets.is_contiguous() else targets.to(torch.int64).contiguous()
 
 
 def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None, top_k: int = 0, temperature: float = 1.0) -> LogProbs:
@@ -290,7 +325,7 @@ def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None
     top_k = int(top_k)
     if not 0 <= top_k <= MAX_TOP_K:
         raise ValueError(f"top_k must be between 0 and {MAX_TOP_K}")
-    if not (temperature > 0 and np.isfinite(temperature)):
+    if not (temperature > 0 and math.isfinite(temperature)):
         raise ValueError("temperature must be positive")
     scores, lists, m, cols, pitch = _scores(scores, lists)
     device = scores.device
@@ -300,7 +335,8 @@ def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None
     if top_k:
         top = torch.empty((m, top_k), dtype=torch.float32, device=device)
         ids = torch.empty((m, top_k), dtype=torch.int32, device=device)
-    result = LogProbs(few[0] if targets is not None else None, few[1], few[2], top, ids)
+    log_p, entropy, lse = few.unbind()
+    result = LogProbs(log_p if targets is not None else None, entropy, lse, top, ids)
     if m == 0:
         return result
     if lists is None and cols == 0:  # rows of nothing
@@ -313,7 +349,7 @@ def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None
     h, stream = get_handle(device.index), _stream(device)
     total = 0 if lists is None else lists.total
     need = C.c_uint64()
-    _lib.check(h.lib.culsh_log_probs_workspace(h.ptr, m, cols, lists is not None, total, C.byref(need)))
+    _lib.check(h.lib.culsh_log_probs_workspace(h.ptr, _TYPES[scores.dtype], m, cols, lists is not None, total, C.byref(need)))
     work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
     at = few.data_ptr()
     _lib.check(h.lib.culsh_log_probs(
@@ -330,7 +366,7 @@ def log_probs_backward(scores, targets, lse, entropy, grad_log_probs=None, grad_
     """Gradient with respect to ``scores``, in their type, from the gradients of the log probabilities and of the entropies of
     ``log_probs(scores, targets, lists, temperature=temperature)``, whose ``lse`` and ``entropy`` it takes.  A target that is not in
     its row, or is masked with -inf, has no gradient."""
-    if not (temperature > 0 and np.isfinite(temperature)):
+    if not (temperature > 0 and math.isfinite(temperature)):
         raise ValueError("temperature must be positive")
     scores, lists, m, cols, pitch = _scores(scores, lists)
     device = scores.device

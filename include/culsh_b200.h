@@ -332,6 +332,11 @@ int culsh_mx_dequantize(culsh_handle* h, const uint8_t* codes, const uint8_t* sc
 int culsh_mx_product(culsh_handle* h, const uint8_t* q_codes, const uint8_t* q_scales, const float* q_norms, int n_queries,
                      const uint8_t* codes, const uint8_t* scales, const float* norms, int n, int d, int metric, void* out,
                      int type, int64_t ld, void* stream);
+/* The same for queries of any type (rows ldq apart), which are held in 4 bits for the call: in workspace, device, aligned
+ * to 16, of 64 G n_queries + 512 G ceil(n_queries / 128) + 4 n_queries bytes. */
+int culsh_mx_product_dense(culsh_handle* h, const void* Q, int q_type, int n_queries, int64_t ldq, const uint8_t* codes,
+                           const uint8_t* scales, const float* norms, int n, int d, int metric, void* out, int type, int64_t ld,
+                           void* workspace, uint64_t workspace_bytes, void* stream);
 /* Waits for the stream and says whether a bounded wait of a product ran out since the last such call
  * (CULSH_ERR_INTERNAL; the scores that it should have made are NaN). */
 int culsh_mx_product_check(culsh_handle* h, void* stream);
@@ -356,7 +361,7 @@ int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* str
  *   top_*  [m][k]  the k <= 128 largest, the earlier of equal ones first; -inf and -1 behind the last one
  * A NaN or +inf makes its row's numbers NaN.  targets / log_probs may be NULL.  workspace: device, as
  * many bytes as culsh_log_probs_workspace says, aligned to 16. */
-int culsh_log_probs_workspace(culsh_handle* h, int m, int64_t cols, int is_lists, int64_t total, uint64_t* bytes);
+int culsh_log_probs_workspace(culsh_handle* h, int type, int m, int64_t cols, int is_lists, int64_t total, uint64_t* bytes);
 int culsh_log_probs(culsh_handle* h, const void* scores, int type, int m, int64_t cols, int64_t ld, const int64_t* offsets,
                     const int32_t* ids, int64_t total, double temperature, const int64_t* targets, int k, float* log_probs,
                     float* entropy, float* lse, float* top_log_probs, int32_t* top_ids, void* workspace,

@@ -12,11 +12,12 @@ def test_null_arguments_are_a_status():
         lib.culsh_mx_quantize(None, None, 0, 1, 1, 1, None, None, None, None),
         lib.culsh_mx_dequantize(None, None, None, 1, 1, None, 0, None),
         lib.culsh_mx_product(None, None, None, None, 1, None, None, None, 1, 1, 0, None, 0, 1, None),
+        lib.culsh_mx_product_dense(None, None, 0, 1, 1, None, None, None, 1, 1, 0, None, 0, 1, None, 0, None),
         lib.culsh_mx_product_check(None, None),
         lib.culsh_mx_score(None, None, 0, 1, 1, None, None, None, 1, 1, 0, None, None, 0, None, None, 0, None),
         lib.culsh_mx_score_workspace(None, 1, 1, 0, C.byref(need)),
         lib.culsh_candidates_after(None, None, None),
-        lib.culsh_log_probs_workspace(None, 1, 1, 0, 0, C.byref(need)),
+        lib.culsh_log_probs_workspace(None, 0, 1, 1, 0, 0, C.byref(need)),
         lib.culsh_log_probs(None, None, 0, 1, 1, 1, None, None, 0, 1.0, None, 0, None, None, None, None, None, None, 0, None),
         lib.culsh_log_probs_backward(None, None, 0, 1, 1, 1, None, None, 0, 1.0, None, None, None, None, None, None, None),
     ):
