@@ -109,7 +109,7 @@ SIGNATURES = {
     "culsh_candidates_after": [VP, VP, VP],
     "culsh_log_probs_workspace": [VP, I, I, I64, I, I64, C.POINTER(C.c_uint64)],
     "culsh_log_probs": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, I, VP, VP, VP, VP, VP, VP, U64, VP],
-    "culsh_log_probs_backward": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, VP, VP, VP, VP, VP, VP],
+    "culsh_log_probs_backward": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, VP, VP, VP, VP, VP, I64, VP],
 }
 _VOID = {"culsh_index_free": [VP], "culsh_candidates_free": [VP]}
 _CHARP = {"culsh_last_error": []}

@@ -27,7 +27,7 @@ template <typename T>
 constexpr int LP_PER_LANE = 64 / sizeof(T);
 template <typename T>
 constexpr int LP_CHUNK = 32 * LP_PER_LANE<T>;
-constexpr int LP_LEAST_CHUNK = 512, LP_MOST_CHUNK = 1024;
+constexpr int LP_LEAST_CHUNK = 512;
 constexpr int LP_MAX_K = 128;
 constexpr float LP_FLOOR = -10000.f;
 
@@ -122,6 +122,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
         "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
@@ -573,21 +581,26 @@ struct LpBackward {
     const float* entropy;
     const float* g;         // of the log probabilities, or null
     const float* h;         // of the entropies, or null
-    int64_t chunks;         // of all positions (lists), or of each row at most (a matrix)
+    int64_t ldo;            // of the result, where it is a matrix
+    int64_t units;          // spans of positions: of all lists, or that a matrix's row can reach into
+    int span;               // positions of lists for a warp
 };
 
-// Constants of a row: ds = p (a - b log p) - g p, and g (1 - p) in place of -g p at the given entry; log p = z - lse, a = -h entropy / temperature, b = h / temperature,
-// g by the temperature.
+// Constants of a row: ds = p (a - b log p), and more at the given entry; log p = z - lse, a = -(h entropy + g) / temperature, b = h / temperature, g by the temperature.
 struct LpRowTerms {
     float lse, a, b, g;
     int64_t target;
+    bool bad;  // lse is NaN: so is everything but what is masked
 };
 
 template <typename T>
 __device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, const LpBackward& b, int row, int64_t begin, int64_t end) {
     LpRowTerms r;
-    const float lse = __ldg(b.lse + row), h = b.h ? __ldg(b.h + row) : 0.f;
+    const float h = b.h ? __ldg(b.h + row) : 0.f, entropy = __ldg(b.entropy + row);
     float g = b.f.targets && b.g ? __ldg(b.g + row) : 0.f;
+    r.lse = __ldg(b.lse + row);
+    if (r.lse == -INFINITY) r.lse = 0.f;  // all masked: 2^-inf is 0 then
+    r.bad = r.lse != r.lse;
     r.target = -1;
     if (b.f.targets && b.g) {
         r.target = LpFind(b.f, row, begin, end)(b.f);
@@ -596,53 +609,123 @@ __device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, cons
             g = 0.f;
         }
     }
-    r.lse = lse;
-    r.a = -h * __ldg(b.entropy + row) * b.f.inv_t;
+    r.a = -(h * entropy + g) * b.f.inv_t;
     r.b = h * b.f.inv_t;
     r.g = g * b.f.inv_t;
     return r;
 }
-// 1 - p of an entry that is nearly certain is as exact as its log p: lists of one or two entries have hardly anything else.
-__device__ __forceinline__ float lp_grad(const LpRowTerms& r, float s, float inv_t, bool given) {
-    const float z = s * inv_t;
-    if (z == -INFINITY) return 0.f;
-    const float lp = max_nan(z - r.lse, LP_FLOOR), p = exp2_fast(lp * 1.4426950409f);  // no 0 times infinity for the lowest finite values
-    return fmaf(p, fmaf(-r.b, lp, r.a), r.g * (given ? -expm1f(lp) : -p));
+__device__ __forceinline__ float2 lp_grad(const LpRowTerms& r, float2 s, float inv_t) {
+    float2 lp = fma2(s, make_float2(inv_t, inv_t), make_float2(-r.lse, -r.lse));
+    lp = make_float2(max_nan(lp.x, LP_FLOOR), max_nan(lp.y, LP_FLOOR));  // no 0 times infinity for what is masked, or as low as that
+    const float2 q = mul2(lp, make_float2(1.4426950409f, 1.4426950409f));
+    float2 v = mul2(make_float2(exp2_fast(q.x), exp2_fast(q.y)), fma2(make_float2(-r.b, -r.b), lp, make_float2(r.a, r.a)));
+    if (r.bad) v = make_float2(s.x == -INFINITY ? 0.f : v.x, s.y == -INFINITY ? 0.f : v.y);
+    return v;
+}
+// At the given entry.  1 - p of one that is nearly certain is as exact as its log p: lists of one or two entries have hardly anything else.
+__device__ __forceinline__ float lp_grad_given(const LpRowTerms& r, float s, float inv_t) {
+    const float lp = max_nan(fmaf(s, inv_t, -r.lse), LP_FLOOR), p = exp2_fast(lp * 1.4426950409f);
+    return fmaf(p, fmaf(-r.b, lp, r.a + r.g), -r.g * expm1f(lp));
 }
 __device__ __forceinline__ void put_grad(float* o, float v) { *o = v; }
 __device__ __forceinline__ void put_grad(__half* o, float v) { *o = __float2half_rn(v); }
 __device__ __forceinline__ void put_grad(__nv_bfloat16* o, float v) { *o = __float2bfloat16_rn(v); }
 
-// A warp for each chunk, and for each row in it.
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_backward_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
-    const int lane = threadIdx.x & 31;
-    const int64_t n = (int64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5);
-    const LpRows& rows = b.f.rows;
-    int row;
-    int64_t chunk;
-    if (rows.offsets) {
-        if (n >= b.chunks) return;
-        chunk = n;
-        row = owner_of(rows.offsets, b.f.m, max(chunk * LP_LEAST_CHUNK - rows.shift, (int64_t)0));
-    } else {
-        row = (int)(n / b.chunks);
-        if (row >= b.f.m) return;
-        chunk = rows.begin(row) / LP_LEAST_CHUNK + n % b.chunks;
+// Positions [from, to) of a row by `threads` threads, whose `thread` this is, 64 bytes of each in flight; `x` and `o`: position 0 of the scores, on a 16-byte boundary, and of the gradient.
+// ALIKE: that is on a boundary, too, in every row.
+template <bool ALIKE, typename T>
+__device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __restrict__ o, const LpRowTerms& r, float inv_t, int64_t from, int64_t to, int thread,
+                                                 int threads) {
+    constexpr int V = 16 / sizeof(T);
+    if constexpr (!ALIKE) {  // an entry at a time, sixteen of them on their way
+#pragma unroll 1
+        for (int64_t p0 = from + thread; p0 < to; p0 += (int64_t)16 * threads) {
+            float s[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = p0 + (int64_t)i * threads < to ? score_of(x[p0 + (int64_t)i * threads]) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float2 d = lp_grad(r, make_float2(s[i], s[i + 1]), inv_t);
+                const int64_t p = p0 + (int64_t)i * threads, p1 = p + threads;
+                if (p < to) put_grad(o + p, p == r.target ? lp_grad_given(r, s[i], inv_t) : d.x);
+                if (p1 < to) put_grad(o + p1, p1 == r.target ? lp_grad_given(r, s[i + 1], inv_t) : d.y);
+            }
+        }
+        return;
     }
-    const int64_t p0 = chunk * LP_LEAST_CHUNK, p1 = p0 + LP_LEAST_CHUNK;
-    for (; row < b.f.m; ++row) {
+    for (int64_t p0 = from / V * V + (int64_t)thread * V; p0 < to; p0 += (int64_t)4 * threads * V) {
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t p = p0 + (int64_t)j * threads * V;
+            if (p >= from && p + V <= to) {
+                w[j] = __ldg(reinterpret_cast<const uint4*>(x + p));
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) reinterpret_cast<T*>(&w[j])[i] = p + i >= from && p + i < to ? x[p + i] : T(0.f);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t p = p0 + (int64_t)j * threads * V;
+            if (p >= to) break;
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const T* const t = reinterpret_cast<const T*>(&w[j]) + i;
+                const float2 d = lp_grad(r, make_float2(score_of(t[0]), score_of(t[1])), inv_t);
+                v[i] = d.x;
+                v[i + 1] = d.y;
+            }
+            if (r.target >= p && r.target < p + V) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (p + i == r.target) v[i] = lp_grad_given(r, score_of(reinterpret_cast<const T*>(&w[j])[i]), inv_t);
+            }
+            if (p >= from && p + V <= to) {
+                uint4 u;
+                if constexpr (sizeof(T) == 4) {
+                    u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                } else {
+                    u = make_uint4(pack_scores(o, v[0], v[1]), pack_scores(o, v[2], v[3]), pack_scores(o, v[4], v[5]), pack_scores(o, v[6], v[7]));
+                }
+                *reinterpret_cast<uint4*>(o + p) = u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (p + i >= from && p + i < to) put_grad(o + p + i, v[i]);
+            }
+        }
+    }
+}
+
+// A CTA for a span of a matrix's row.
+template <typename T>
+constexpr int LP_ROW_SPAN = 4 * LP_THREADS * (16 / sizeof(T));
+template <bool ALIKE, typename T>
+__global__ void __launch_bounds__(LP_THREADS) log_probs_backward_rows_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+    const int64_t row = blockIdx.x / (unsigned)b.units, begin = b.f.rows.begin((int)row), end = b.f.rows.end((int)row);
+    const int64_t span = begin / LP_ROW_SPAN<T> + (blockIdx.x - (unsigned)row * (unsigned)b.units);
+    const int64_t from = max(span * LP_ROW_SPAN<T>, begin), to = min((span + 1) * LP_ROW_SPAN<T>, end);
+    if (from >= to) return;
+    const LpRowTerms r = lp_row_terms(x, b, (int)row, begin, end);
+    lp_backward_span<ALIKE>(x, out + (row * b.ldo - begin), r, b.f.inv_t, from, to, threadIdx.x, LP_THREADS);
+}
+
+// A warp for a span of all lists' positions, and for each list in it: what it has to know of a list takes longer than a short one.
+template <bool ALIKE, typename T>
+__global__ void __launch_bounds__(LP_THREADS) log_probs_backward_lists_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+    const int64_t n = (int64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5);
+    if (n >= b.units) return;
+    const LpRows& rows = b.f.rows;
+    const int64_t p0 = n * b.span, p1 = p0 + b.span;
+    for (int row = owner_of(rows.offsets, b.f.m, max(p0 - rows.shift, (int64_t)0)); row < b.f.m; ++row) {
         const int64_t begin = rows.begin(row), end = rows.end(row);
         if (begin >= p1) break;
         const int64_t from = max(begin, p0), to = min(end, p1);
-        if (from < to) {
-            const LpRowTerms r = lp_row_terms(x, b, row, begin, end);
-            T* const o = out + (rows.offsets ? -rows.shift : (int64_t)row * rows.cols - begin);
-            for (int64_t p = from + lane; p < to; p += 32) {
-                put_grad(o + p, lp_grad(r, score_of(x[p]), b.f.inv_t, p == r.target));
-            }
-        }
-        if (!rows.offsets) break;
+        if (from >= to) continue;
+        const LpRowTerms r = lp_row_terms(x, b, row, begin, end);
+        lp_backward_span<ALIKE>(x, out - rows.shift, r, b.f.inv_t, from, to, threadIdx.x & 31, 32);
     }
 }
 
@@ -705,11 +788,15 @@ inline void log_probs_backward(const T* scores, T* out, LpBackward b, cudaStream
     constexpr int V = 16 / sizeof(T);
     LpRows& r = b.f.rows;
     r.shift = (int64_t)((uintptr_t)scores / sizeof(T) % V);
-    if (r.offsets) b.chunks = (int64_t)ceil_div((size_t)(r.total + r.shift), LP_LEAST_CHUNK);
-    else b.chunks = r.cols / LP_LEAST_CHUNK + 2;
-    const size_t grid = ceil_div(r.offsets ? (size_t)b.chunks : (size_t)b.chunks * b.f.m, LP_WARPS);
+    const int64_t mean = r.total / b.f.m;
+    b.span = mean >= 1024 ? 512 : mean >= 64 ? 128 : 32;
+    b.units = r.offsets ? (int64_t)ceil_div((size_t)(r.total + r.shift), (size_t)b.span) : r.cols / LP_ROW_SPAN<T> + 2;
+    const size_t grid = r.offsets ? ceil_div((size_t)b.units, LP_WARPS) : (size_t)b.units * b.f.m;
     if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "too many entries for one call");
-    log_probs_backward_kernel<T><<<(unsigned)grid, LP_THREADS, 0, stream>>>(scores - r.shift, out, b);
+    const bool alike = (((uintptr_t)(out - r.shift) | (r.offsets ? 0u : (uintptr_t)((b.ldo - r.ld) * (int64_t)sizeof(T)))) & 15u) == 0;
+    auto kern = r.offsets ? (alike ? log_probs_backward_lists_kernel<true, T> : log_probs_backward_lists_kernel<false, T>)
+                          : (alike ? log_probs_backward_rows_kernel<true, T> : log_probs_backward_rows_kernel<false, T>);
+    kern<<<(unsigned)grid, LP_THREADS, 0, stream>>>(scores - r.shift, out, b);
     KERNEL_CHECK();
 }
 

@@ -6,13 +6,16 @@
 
 namespace culsh_b200 {
 
-// Largest i with offsets[i] <= at, i < n.
+// Largest i with offsets[i] <= at, i < n, by a warp: 32 of what is left are looked at at a time.
 __device__ __forceinline__ int owner_of(const int64_t* __restrict__ offsets, int n, int64_t at) {
+    const int lane = threadIdx.x & 31;
     int lo = 0, hi = n;  // offsets[lo] <= at < offsets[hi]
     while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(offsets + mid) <= at) lo = mid;
-        else hi = mid;
+        const int step = (int)(((unsigned)(hi - lo) + 31u) / 32u);
+        const int64_t p = (int64_t)lo + (int64_t)lane * step;
+        const unsigned below = __ballot_sync(0xFFFFFFFFu, lane == 0 || (p < hi && __ldg(offsets + p) <= at));
+        lo += (31 - __clz((int)below)) * step;
+        hi = min(hi, lo + step);
     }
     return lo;
 }

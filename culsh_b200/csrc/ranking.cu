@@ -209,7 +209,7 @@ int culsh_log_probs(culsh_handle* h, const void* scores, int type, int m, int64_
 
 int culsh_log_probs_backward(culsh_handle* h, const void* scores, int type, int m, int64_t cols, int64_t ld, const int64_t* offsets,
                              const int32_t* ids, int64_t total, double temperature, const int64_t* targets, const float* lse, const float* entropy,
-                             const float* grad_log_probs, const float* grad_entropy, void* grad_scores, void* stream) {
+                             const float* grad_log_probs, const float* grad_entropy, void* grad_scores, int64_t ld_grad, void* stream) {
     return guarded([&] {
         need(h && lse && entropy, "null argument");
         need(!grad_log_probs || targets, "the gradient of log probabilities needs their targets");
@@ -217,6 +217,8 @@ int culsh_log_probs_backward(culsh_handle* h, const void* scores, int type, int 
         b.f = log_probs_args(scores, m, cols, ld, offsets, ids, total, temperature, targets);
         if (offsets && total == 0) return;
         need(grad_scores, "null argument");
+        need(offsets || ld_grad >= cols, "rows must not overlap");
+        b.ldo = ld_grad;
         b.lse = lse, b.entropy = entropy, b.g = grad_log_probs, b.h = grad_entropy;
         DeviceGuard g(h->ctx->device);
         by_type(type, SCORE_TYPES, scores, [&](auto* s) {

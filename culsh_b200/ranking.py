@@ -383,7 +383,7 @@ def log_probs_backward(scores, targets, lse, entropy, grad_log_probs=None, grad_
     _lib.check(h.lib.culsh_log_probs_backward(
         h.ptr, scores.data_ptr(), _TYPES[scores.dtype], m, cols, pitch, lists.offsets if lists else None, (lists.ids or None) if lists else None,
         lists.total if lists else 0, float(temperature), targets.data_ptr() if targets is not None else None, lse.data_ptr(), entropy.data_ptr(),
-        g.data_ptr() if g is not None else None, e.data_ptr() if e is not None else None, out.data_ptr(), stream))
+        g.data_ptr() if g is not None else None, e.data_ptr() if e is not None else None, out.data_ptr(), cols, stream))
     if lists is not None:
         lists.done(h, stream)
     return out

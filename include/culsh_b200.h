@@ -366,13 +366,13 @@ int culsh_log_probs(culsh_handle* h, const void* scores, int type, int m, int64_
                     const int32_t* ids, int64_t total, double temperature, const int64_t* targets, int k, float* log_probs,
                     float* entropy, float* lse, float* top_log_probs, int32_t* top_ids, void* workspace,
                     uint64_t workspace_bytes, void* stream);
-/* grad_scores ([m][cols] without gaps, or as the lists; the scores' type) from the gradients of log_probs
+/* grad_scores ([m][cols], rows ld_grad apart, or as the lists; the scores' type) from the gradients of log_probs
  * and entropy (either may be NULL) and what the forward call returned.  A log probability of -inf has
  * no gradient, nor has an entry of -inf. */
 int culsh_log_probs_backward(culsh_handle* h, const void* scores, int type, int m, int64_t cols, int64_t ld,
                              const int64_t* offsets, const int32_t* ids, int64_t total, double temperature,
                              const int64_t* targets, const float* lse, const float* entropy, const float* grad_log_probs,
-                             const float* grad_entropy, void* grad_scores, void* stream);
+                             const float* grad_entropy, void* grad_scores, int64_t ld_grad, void* stream);
 
 #ifdef __cplusplus
 }

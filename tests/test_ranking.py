@@ -19,7 +19,7 @@ def test_null_arguments_are_a_status():
         lib.culsh_candidates_after(None, None, None),
         lib.culsh_log_probs_workspace(None, 0, 1, 1, 0, 0, C.byref(need)),
         lib.culsh_log_probs(None, None, 0, 1, 1, 1, None, None, 0, 1.0, None, 0, None, None, None, None, None, None, 0, None),
-        lib.culsh_log_probs_backward(None, None, 0, 1, 1, 1, None, None, 0, 1.0, None, None, None, None, None, None, None),
+        lib.culsh_log_probs_backward(None, None, 0, 1, 1, 1, None, None, 0, 1.0, None, None, None, None, None, None, 1, None),
     ):
         assert status == -1
         assert b"null" in lib.culsh_last_error()
