@@ -651,49 +651,49 @@ __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __r
                 if (p1 < to) put_grad(o + p1, p1 == r.target ? lp_grad_given(r, s[i + 1], inv_t) : d.y);
             }
         }
-        return;
-    }
-    for (int64_t p0 = from / V * V + (int64_t)thread * V; p0 < to; p0 += (int64_t)4 * threads * V) {
-        uint4 w[4];
+    } else {
+        for (int64_t p0 = from / V * V + (int64_t)thread * V; p0 < to; p0 += (int64_t)4 * threads * V) {
+            uint4 w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t p = p0 + (int64_t)j * threads * V;
-            if (p >= from && p + V <= to) {
-                w[j] = __ldg(reinterpret_cast<const uint4*>(x + p));
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) reinterpret_cast<T*>(&w[j])[i] = p + i >= from && p + i < to ? x[p + i] : T(0.f);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t p = p0 + (int64_t)j * threads * V;
-            if (p >= to) break;
-            float v[V];
-#pragma unroll
-            for (int i = 0; i < V; i += 2) {
-                const T* const t = reinterpret_cast<const T*>(&w[j]) + i;
-                const float2 d = lp_grad(r, make_float2(score_of(t[0]), score_of(t[1])), inv_t);
-                v[i] = d.x;
-                v[i + 1] = d.y;
-            }
-            if (r.target >= p && r.target < p + V) {
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (p + i == r.target) v[i] = lp_grad_given(r, score_of(reinterpret_cast<const T*>(&w[j])[i]), inv_t);
-            }
-            if (p >= from && p + V <= to) {
-                uint4 u;
-                if constexpr (sizeof(T) == 4) {
-                    u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            for (int j = 0; j < 4; ++j) {
+                const int64_t p = p0 + (int64_t)j * threads * V;
+                if (p >= from && p + V <= to) {
+                    w[j] = __ldg(reinterpret_cast<const uint4*>(x + p));
                 } else {
-                    u = make_uint4(pack_scores(o, v[0], v[1]), pack_scores(o, v[2], v[3]), pack_scores(o, v[4], v[5]), pack_scores(o, v[6], v[7]));
-                }
-                *reinterpret_cast<uint4*>(o + p) = u;
-            } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (p + i >= from && p + i < to) put_grad(o + p + i, v[i]);
+                    for (int i = 0; i < V; ++i) reinterpret_cast<T*>(&w[j])[i] = p + i >= from && p + i < to ? x[p + i] : T(0.f);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t p = p0 + (int64_t)j * threads * V;
+                if (p >= to) break;
+                float v[V];
+#pragma unroll
+                for (int i = 0; i < V; i += 2) {
+                    const T* const t = reinterpret_cast<const T*>(&w[j]) + i;
+                    const float2 d = lp_grad(r, make_float2(score_of(t[0]), score_of(t[1])), inv_t);
+                    v[i] = d.x;
+                    v[i + 1] = d.y;
+                }
+                if (r.target >= p && r.target < p + V) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (p + i == r.target) v[i] = lp_grad_given(r, score_of(reinterpret_cast<const T*>(&w[j])[i]), inv_t);
+                }
+                if (p >= from && p + V <= to) {
+                    uint4 u;
+                    if constexpr (sizeof(T) == 4) {
+                        u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                    } else {
+                        u = make_uint4(pack_scores(o, v[0], v[1]), pack_scores(o, v[2], v[3]), pack_scores(o, v[4], v[5]), pack_scores(o, v[6], v[7]));
+                    }
+                    *reinterpret_cast<uint4*>(o + p) = u;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (p + i >= from && p + i < to) put_grad(o + p + i, v[i]);
+                }
             }
         }
     }

@@ -31,14 +31,12 @@ struct MxScoreArgs {
     int n, nq, d, groups, metric;
 };
 
-constexpr int MXS_PER_WARP = 64;
-
-// A warp takes 64 neighbouring candidates, eight at a time; four lanes share one and take its blocks of 32 values (16 bytes) in turn.
+// A warp takes `per` neighbouring candidates, eight at a time; four lanes share one and take its blocks of 32 values (16 bytes) in turn.
 template <typename T>
-__global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, MxScoreArgs a) {
+__global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, MxScoreArgs a, int per) {
     const int lane = threadIdx.x & 31, t = lane & 3;
-    int64_t at = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * MXS_PER_WARP;
-    const int64_t end = min(at + MXS_PER_WARP, a.total);
+    int64_t at = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * per;
+    const int64_t end = min(at + per, a.total);
     if (at >= end) return;
     int q = owner_of(a.offsets, a.nq, at);
     while (at < end) {
@@ -103,8 +101,9 @@ __global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, 
 // bits at least, so that a query of float32 values within a factor of 2^10 of one another in a block is the sum of about 18 slices, one of bytes that of five: nothing is rounded
 // off.  Sixteen, 32, 48 or 64 slices of a query are the N side of the MMAs; those beyond 64 would be below 2^-126 of the block's largest value.  The M side are 128 candidates of a list, whose codes
 // and scales are gathered by cp.async to where the MMAs take them, and the score is the sum of the accumulator's columns.  No code is unpacked by an instruction:
-// 180M candidates of 128 values 12.0 -> 3.9 ms (3.0 without norms).  Bound by the gather: a row's 64 bytes of
-// codes and 4 of scales, and its norm, are a request of an SM to L2 each, and it makes one in two cycles.
+// 180M candidates of 128 values 12.0 -> 3.9 ms.  Of 100,000 rows, which lie in L2, they take 2.5 ms: what a warp does for a
+// tile; of a million the gather takes longer: L2 gives 8 TB/s in pieces of 32 and 64 bytes, 174 bytes a candidate with its norm (3.1 ms without).  Codes gathered by TMA took 3.4 ms
+// in either case.
 //
 // One persistent CTA per SM.  Warps 0 - 7 gather (four a stage), 8 loads slices, 9 - 11 issue MMAs (a tile each: what a warp does for one takes 1,300 cycles), 12 - 19 epilogue
 // (four a tile).  All walk the same tiles: a CTA has those that begin in its share of the positions, where each list counts for 128 more than
@@ -526,7 +525,8 @@ inline size_t mx_score_workspace(int nq, int d, int64_t total) {
 template <typename T>
 inline void mx_score(const CtxPtr& c, const T* Q, const MxScoreArgs& a, void* workspace, int* d_error, cudaStream_t stream) {
     if (mx_score_few(a.total, a.groups, a.nq)) {
-        mx_score_kernel<T><<<(unsigned)ceil_div((size_t)a.total, 8 * MXS_PER_WARP), 256, 0, stream>>>(Q, a);
+        const int per = 8 * (int)std::min<int64_t>(8, std::max<int64_t>(1, a.total / (8 * 32 * c->sm_count)));  // 32 warps for an SM first
+        mx_score_kernel<T><<<(unsigned)ceil_div((size_t)a.total, 8 * (size_t)per), 256, 0, stream>>>(Q, a, per);
         KERNEL_CHECK();
         return;
     }
