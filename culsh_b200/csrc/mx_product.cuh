@@ -24,25 +24,27 @@ enum MxMetric : int { MX_DOT = 0, MX_COSINE = 1, MX_EUCLIDEAN = 2 };
 constexpr int MXP_B = 128;  // entries of either side in a unit
 constexpr int MXP_OUT_BYTES = 8192;  // 32 queries by 256 bytes
 
-// More than 64 queries; up to 64; up to 16.  The fewer there are, the shorter is a unit, and the less of it the issuing threads and the epilogue can overlap: few queries have
+// More than 64 queries; the same of 1,024 values and more; up to 64; up to 16.  With more queries, loads in flight and warps of epilogue share the SM: short rows wait for the scores to be
+// stored, long ones for L2 (4,099 x 32,771 x 2,048: twelve warps and 102 KB of stages 244 us, eight and 136 KB 211, four and 170 KB 203; 1,000 x 1M x 128 cosines 432, 507 and worse).  The fewer there are, the shorter is a unit, and the less of it the issuing threads and the epilogue can overlap: few queries have
 // two or four CTAs on an SM, which share its tensor memory (one query, 1M x 128 rows: one CTA with twice the epilogue warps 38 us, four 27).
-enum MxpKind { MXP_MANY, MXP_FEW, MXP_FEWEST };
-constexpr int MXP_FEW_MAX = 64, MXP_FEWEST_MAX = 16;
+enum MxpKind { MXP_MANY, MXP_LONG, MXP_FEW, MXP_FEWEST };
+constexpr int MXP_FEW_MAX = 64, MXP_FEWEST_MAX = 16, MXP_LONG_GROUPS = 8;
 
-// SPAN: bytes of a row in a stage, the swizzle span: 64 (one group) or 128 (two).
+// SPAN: bytes of a row in a stage, the swizzle span: 64 (one group) or 128 (two; of a row with an odd number of them the last stage has one, and zeros).
 template <int SPAN, MxpKind KIND>
 struct MxpCfg {
-    static constexpr bool FEW = KIND != MXP_MANY;
-    static constexpr int CTAS = KIND == MXP_MANY ? 1 : KIND == MXP_FEW ? 2 : 4;
+    static constexpr bool FEW = KIND == MXP_FEW || KIND == MXP_FEWEST;
+    static constexpr int CTAS = !FEW ? 1 : KIND == MXP_FEW ? 2 : 4;
     static constexpr int GROUPS = SPAN / 64;
     static constexpr int A_BYTES = MXP_B * SPAN, S_BYTES = GROUPS * MX_TILE_BYTES;
-    static constexpr int B_BYTES = (KIND == MXP_MANY ? MXP_B : KIND == MXP_FEW ? MXP_FEW_MAX : MXP_FEWEST_MAX) * SPAN;
+    static constexpr int B_BYTES = (!FEW ? MXP_B : KIND == MXP_FEW ? MXP_FEW_MAX : MXP_FEWEST_MAX) * SPAN;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + 2 * S_BYTES;
-    static constexpr int STAGES = (KIND == MXP_FEWEST ? 4 : KIND == MXP_FEW ? 8 : 6) / GROUPS;
-    static constexpr int EPI_WARPS = FEW ? 4 : 12, THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr int EPI_WARPS = FEW || KIND == MXP_LONG ? 4 : SPAN == 64 ? 12 : 8;
+    static constexpr int STAGES = (KIND == MXP_FEWEST ? 4 : KIND == MXP_FEW ? 8 : KIND == MXP_LONG ? 10 : SPAN == 64 ? 6 : 8) / GROUPS;
+    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int OUT_BYTES = FEW ? 0 : EPI_WARPS * MXP_OUT_BYTES;
     static constexpr int TERM_COUNT = FEW ? MXP_FEW_MAX : MXP_B, TERMS = EPI_WARPS * TERM_COUNT * 4;
-    static constexpr int TMEM_COLS = 512 / CTAS, ACC_COLS = KIND == MXP_MANY ? 384 : TMEM_COLS / 2;
+    static constexpr int TMEM_COLS = 512 / CTAS, ACC_COLS = !FEW ? 384 : TMEM_COLS / 2;
     static constexpr int SF_SLOTS = (TMEM_COLS - ACC_COLS) / 8, MAX_ACCS = ACC_COLS / 16;
     static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + TERMS + 1024 /*barriers*/ + 1024 /*alignment slack*/;
     static_assert(STAGE_BYTES % 1024 == 0 && CTAS * (SMEM + 1024) <= 228 * 1024, "");
@@ -356,19 +358,20 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         if (lane == 0) {
             uint32_t s = 0, parity = 1;
             bool live = true;
-            const uint32_t bytes = Cfg::A_BYTES + (uint32_t)(a.box_b * SPAN) + 2 * Cfg::S_BYTES;
+            const uint32_t bytes = Cfg::A_BYTES + (uint32_t)(a.box_b * SPAN);
             for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x) {
                 const MxUnit at(u, a);
                 const int ia = FEW ? at.tile : at.chunk, ib = FEW ? at.chunk : at.tile;
                 for (int g = 0; g < a.groups; g += Cfg::GROUPS) {
                     if (!mbar_wait(&empty[s], parity, s_abort, a.d_error)) { live = false; break; }
                     unsigned char* st = base + (size_t)s * Cfg::STAGE_BYTES;
-                    mbar_expect_tx(&full[s], bytes);
+                    const uint32_t scales = (uint32_t)min(Cfg::GROUPS, a.groups - g) * MX_TILE_BYTES;
+                    mbar_expect_tx(&full[s], bytes + 2 * scales);
                     tma_load_2d(st, &tmA, &full[s], g * 64, ia * MXP_B);
                     tma_load_2d(st + Cfg::A_BYTES, &tmB, &full[s], g * 64, ib * MXP_B);
-                    bulk_load(st + Cfg::A_BYTES + Cfg::B_BYTES, a.a_scales + ((size_t)ia * a.groups + g) * MX_TILE_BYTES, Cfg::S_BYTES, &full[s]);
+                    bulk_load(st + Cfg::A_BYTES + Cfg::B_BYTES, a.a_scales + ((size_t)ia * a.groups + g) * MX_TILE_BYTES, scales, &full[s]);
                     bulk_load(st + Cfg::A_BYTES + Cfg::B_BYTES + Cfg::S_BYTES, a.b_scales + ((size_t)ib * a.groups + g) * MX_TILE_BYTES,
-                              Cfg::S_BYTES, &full[s]);
+                              scales, &full[s]);
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
             }
@@ -390,14 +393,19 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                 const uint32_t st = smem_u32(base + (size_t)s * Cfg::STAGE_BYTES);
                 const uint64_t da = mx_tile_desc<SPAN>(st), db = mx_tile_desc<SPAN>(st + Cfg::A_BYTES);
                 const uint64_t dsa = mx_scale_desc(st + Cfg::A_BYTES + Cfg::B_BYTES), dsb = dsa + (Cfg::S_BYTES >> 4);
-#pragma unroll
-                for (int g = 0; g < Cfg::GROUPS; ++g) {
+                auto group = [&](int g) {
                     const uint32_t sfa = tmem + Cfg::ACC_COLS + slot * 8, sfb = sfa + 4;
                     if (++slot == Cfg::SF_SLOTS) slot = 0;
                     tc_copy_scales(sfa, dsa + g * (MX_TILE_BYTES >> 4));
                     tc_copy_scales(sfb, dsb + g * (MX_TILE_BYTES >> 4));
                     tc_mma_mxf4(d_tmem, da + g * 4, db + g * 4, id0, sfa, sfb, (g0 | g) != 0);
                     tc_mma_mxf4(d_tmem, da + g * 4 + 2, db + g * 4 + 2, id1, sfa, sfb, 1u);
+                };
+                if (Cfg::GROUPS == 1 || g0 + 1 == a.groups) {
+                    group(0);
+                } else {
+                    group(0);
+                    group(1);
                 }
                 tc_commit_warp(&empty[s]);
                 if (++s == STAGES) { s = 0; parity ^= 1u; }
@@ -467,11 +475,16 @@ inline void mx_product(const CtxPtr& c, const uint8_t* q_codes, const uint8_t* q
     a.wide = aligned16(out, ld * (int64_t)sizeof(OUT));
     auto go = [&](auto kind) {
         constexpr MxpKind K = decltype(kind)::value;
-        if (a.groups % 2 == 0) mx_product_launch<128, OUT, K>(c, codes, q_codes, a, stream);
-        else mx_product_launch<64, OUT, K>(c, codes, q_codes, a, stream);
+        if constexpr (K == MXP_LONG) {
+            mx_product_launch<128, OUT, K>(c, codes, q_codes, a, stream);
+        } else {
+            if (a.groups > 1) mx_product_launch<128, OUT, K>(c, codes, q_codes, a, stream);
+            else mx_product_launch<64, OUT, K>(c, codes, q_codes, a, stream);
+        }
     };
     if (nq <= MXP_FEWEST_MAX) go(std::integral_constant<MxpKind, MXP_FEWEST>());
     else if (few) go(std::integral_constant<MxpKind, MXP_FEW>());
+    else if (a.groups >= MXP_LONG_GROUPS) go(std::integral_constant<MxpKind, MXP_LONG>());
     else go(std::integral_constant<MxpKind, MXP_MANY>());
 }
 
