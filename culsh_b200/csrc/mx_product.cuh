@@ -6,9 +6,9 @@
 //   more: the queries, so that a lane holds neighbouring scores of a query, which it packs into 16 bytes.  They go through shared memory, from where sixteen lanes store
 //   256 bytes of a query side by side.  (Stores by TMA were slower: 1,000 x 1M float32 scores 992 us against 792.)
 // Codes come by TMA, swizzled; scale tiles of 512 bytes (128 rows by 4 blocks) lie in memory as the tensor cores
-// take them and go from shared into tensor memory by tcgen05.cp, issued by the thread that issues the MMAs, in front of the two MMAs (64 values each) that read them.
+// take them and go from shared into tensor memory by tcgen05.cp, issued by the warp that issues the MMAs, in front of the two MMAs (64 values each) that read them.
 //
-// Persistent CTAs with a warp for the TMA loads, one for the MMAs and four or eight of epilogue; accumulators in turn.  Every wait is bounded
+// Persistent CTAs with a warp for the TMA loads, one for the MMAs and four, eight or twelve of epilogue; accumulators in turn.  Every wait is bounded
 // (mbar_wait); a CTA whose wait ran out records it and fills what it has not done with NaN.  No load uses cluster multicast.
 #pragma once
 
@@ -24,9 +24,11 @@ enum MxMetric : int { MX_DOT = 0, MX_COSINE = 1, MX_EUCLIDEAN = 2 };
 constexpr int MXP_B = 128;  // entries of either side in a unit
 constexpr int MXP_OUT_BYTES = 8192;  // 32 queries by 256 bytes
 
-// More than 64 queries; the same of 1,024 values and more; up to 64; up to 16.  With more queries, loads in flight and warps of epilogue share the SM: short rows wait for the scores to be
-// stored, long ones for L2 (4,099 x 32,771 x 2,048: twelve warps and 102 KB of stages 244 us, eight and 136 KB 211, four and 170 KB 203; 1,000 x 1M x 128 cosines 432, 507 and worse).  The fewer there are, the shorter is a unit, and the less of it the issuing threads and the epilogue can overlap: few queries have
-// two or four CTAs on an SM, which share its tensor memory (one query, 1M x 128 rows: one CTA with twice the epilogue warps 38 us, four 27).
+// More than 64 queries; the same of 1,024 values and more; up to 64; up to 16.
+// With more queries, loads in flight and warps of epilogue share the SM: short rows wait for the scores to be stored (1,000 x 1M x 128 cosines: twelve warps 432 us, eight 507), long ones
+// for L2 (4,099 x 32,771 x 2,048: twelve warps and 102 KB of stages 244 us, eight and 136 KB 211, four and 170 KB 203).  The scores of 1,000 x 1M x 128 are written at 4.5 TB/s in bfloat16 and
+// 5.3 in float32 (a fill of the memory: 3.9).  The fewer queries there are, the shorter is a unit, and the less of it the issuing warps and the epilogue can overlap: few queries have
+// two or four CTAs on an SM, which share its tensor memory (one query, 1M x 128 rows: one CTA with eight warps of epilogue 38 us, four 21; 11.6 at the copy's rate).
 enum MxpKind { MXP_MANY, MXP_LONG, MXP_FEW, MXP_FEWEST };
 constexpr int MXP_FEW_MAX = 64, MXP_FEWEST_MAX = 16, MXP_LONG_GROUPS = 8;
 

@@ -105,9 +105,8 @@ __global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, 
 // tile; of a million the gather takes longer: L2 gives 8 TB/s in pieces of 32 and 64 bytes, 174 bytes a candidate with its norm (3.1 ms without).  Codes gathered by TMA took 3.4 ms
 // in either case.
 //
-// One persistent CTA per SM.  Warps 0 - 7 gather (four a stage), 8 loads slices, 9 - 11 issue MMAs (a tile each: what a warp does for one takes 1,300 cycles), 12 - 19 epilogue
-// (four a tile).  All walk the same tiles: a CTA has those that begin in its share of the positions, where each list counts for 128 more than
-// it has.
+// One persistent CTA per SM.  Warps 0 - 11 gather (four a stage), 12 loads slices, 13 - 18 issue MMAs (a tile each: what a warp does for one takes 1,300 cycles), 19 - 30 epilogue (four a tile).
+// All walk the same tiles: a CTA has those that begin in its share of the positions, where each list counts for 128 more than it has.
 // ------------------------------------------------------------------------------------------
 constexpr int MXS_SLICES = 64, MXS_B_BYTES = MXS_SLICES * 64 + MX_TILE_BYTES;  // of a query and a group: codes, swizzled, and scales
 constexpr int MXS_ROWS = 128, MXS_A_BYTES = MXS_ROWS * 64 + MX_TILE_BYTES;

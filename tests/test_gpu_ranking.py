@@ -687,3 +687,14 @@ def test_score_of_more_queries_than_the_workspace_holds(culsh):
     for q in (0, 1, 2800, 2900, 3000, nq - 1):
         r = x[ids[q * each:(q + 1) * each].long()] * Q[q].double()
         assert bool(((got[q] - r.sum(1)).abs() <= (d + 2) * ULP * r.abs().sum(1)).all())
+
+
+def test_the_example_finds_and_learns():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "rank_candidates.py")
+    spec = importlib.util.spec_from_file_location("rank_candidates", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    found, recall, loss = example.main(rows=20_000, queries=500, features=64, top=5, tables=16, hashes=10)
+    assert found > 0.8 and recall > 0.3 and loss[1] < loss[0]
