@@ -510,7 +510,8 @@ template <typename T>
 __device__ __forceinline__ int64_t lp_chunks_per_row(const LpArgs& a) { return a.rows.cols / LP_CHUNK<T> + 2; }
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __restrict__ x, LpArgs a) {
+__global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __restrict__ x, LpArgs a, KernelBefore before) {
+    behind_kernel_before(x, before);
     __shared__ LpShared<LP_THREADS> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int row;
@@ -541,7 +542,8 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __r
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __restrict__ x, LpArgs a) {
+__global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __restrict__ x, LpArgs a, KernelBefore before) {
+    behind_kernel_before(x, before);
     __shared__ LpShared<LP_THREADS> sh;
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t begin = a.rows.begin(row), end = a.rows.end(row);
@@ -778,9 +780,9 @@ inline void log_probs(const CtxPtr& c, const T* scores, LpArgs a, void* workspac
     a.units_per_row = p.units_per_row;
     a.parts = static_cast<float4*>(workspace);
     a.maxima = reinterpret_cast<uint32_t*>(a.parts + p.units);
-    log_probs_unit_kernel<T><<<(unsigned)p.units, LP_THREADS, 0, stream>>>(x, a);
+    launch_next(stream, log_probs_unit_kernel<T>, (size_t)p.units, (unsigned)LP_THREADS, 0, x, a);
     KERNEL_CHECK();
-    log_probs_join_kernel<T><<<(unsigned)a.m, LP_THREADS, 0, stream>>>(x, a);
+    launch_next(stream, log_probs_join_kernel<T>, (size_t)a.m, (unsigned)LP_THREADS, 0, x, a);
     KERNEL_CHECK();
 }
 

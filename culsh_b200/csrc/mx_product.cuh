@@ -318,7 +318,8 @@ __device__ __forceinline__ void mx_epilogue_many(const MxProductArgs& a, uint32_
 
 template <int SPAN, typename OUT, MxpKind KIND>
 __global__ void __launch_bounds__((MxpCfg<SPAN, KIND>::THREADS), (MxpCfg<SPAN, KIND>::CTAS))
-mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, MxProductArgs a) {
+mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, MxProductArgs a, KernelBefore before) {
+    behind_kernel_before(before);
     using Cfg = MxpCfg<SPAN, KIND>;
     constexpr int STAGES = Cfg::STAGES;
     constexpr bool FEW = Cfg::FEW;
@@ -455,7 +456,8 @@ inline void mx_product_launch(const CtxPtr& c, const uint8_t* codes, const uint8
         CU_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
         if (c->device < 64) ready |= 1ull << c->device;
     }
-    kern<<<std::min<unsigned>(a.units, (unsigned)(c->sm_count * Cfg::CTAS)), Cfg::THREADS, Cfg::SMEM, stream>>>(FEW ? tx : tq, FEW ? tq : tx, a);
+    launch_next(stream, mx_product_kernel<SPAN, OUT, KIND>, std::min<unsigned>(a.units, (unsigned)(c->sm_count * Cfg::CTAS)), (unsigned)Cfg::THREADS,
+                (size_t)Cfg::SMEM, FEW ? tx : tq, FEW ? tq : tx, a);
     KERNEL_CHECK();
 }
 

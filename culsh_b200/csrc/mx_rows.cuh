@@ -123,7 +123,8 @@ struct MxEncode<double> {
 // HBM-bound: n d z read, 17/32 n d + 4 n written (1M x 128 float32 130 us, 4.5 TB/s).  Rows behind the last one of the last tile get scales of 0.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ X, int n, int d, int64_t ld, int lanes, uint8_t* __restrict__ codes,
-                                                          uint8_t* __restrict__ scales, float* __restrict__ norms) {
+                                                          uint8_t* __restrict__ scales, float* __restrict__ norms, KernelBefore before) {
+    behind_kernel_before(X, codes, scales, norms, before);
     __shared__ float s_norm[8];
     const int groups = mx_groups(d), per_cta = 256 / lanes;
     const int64_t row = (int64_t)blockIdx.x * per_cta + threadIdx.x / lanes, rows = (int64_t)mx_tiles(n) * MX_TILE_ROWS;
@@ -212,8 +213,8 @@ inline void mx_quantize(const T* X, int n, int d, int64_t ld, uint8_t* codes, ui
     int lanes = 16;
     while (lanes < 256 && lanes < 16 * mx_groups(d)) lanes *= 2;
     const unsigned grid = (unsigned)ceil_div((size_t)mx_tiles(n) * MX_TILE_ROWS, 256 / lanes);
-    auto kern = aligned16(X, ld * (int64_t)sizeof(T)) ? mx_quantize_kernel<T, true> : mx_quantize_kernel<T, false>;
-    kern<<<grid, 256, 0, stream>>>(X, n, d, ld, lanes, codes, scales, norms);
+    if (aligned16(X, ld * (int64_t)sizeof(T))) launch_next(stream, mx_quantize_kernel<T, true>, grid, 256u, 0, X, n, d, ld, lanes, codes, scales, norms);
+    else launch_next(stream, mx_quantize_kernel<T, false>, grid, 256u, 0, X, n, d, ld, lanes, codes, scales, norms);
     KERNEL_CHECK();
 }
 

@@ -118,7 +118,8 @@ constexpr int MXS_SMEM = MXS_STAGES * MXS_A_BYTES + MXS_B_SLOTS * MXS_B_BYTES + 
 // Slices of queries first .. first + gridDim.x - 1, a CTA each: of[q] [groups][MXS_B_BYTES], their number (a multiple of 16) and the squared length.
 template <typename T>
 __global__ void __launch_bounds__(128) mx_slices_kernel(const T* __restrict__ Q, int64_t ldq, int d, int groups, int first, uint8_t* __restrict__ slices,
-                                                        int* __restrict__ counts, float* __restrict__ norms) {
+                                                        int* __restrict__ counts, float* __restrict__ norms, KernelBefore before) {
+    behind_kernel_before(Q, slices, counts, norms, before);
     __shared__ int s_need[4];
     __shared__ float s_norm[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -268,7 +269,8 @@ __device__ __forceinline__ void copy_async4(uint32_t to, const void* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
-__global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatch b) {
+__global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatch b, KernelBefore before) {
+    behind_kernel_before(before);
     extern __shared__ unsigned char mxs_smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mxs_smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* s_b = base + MXS_STAGES * MXS_A_BYTES;
@@ -545,9 +547,9 @@ inline void mx_score(const CtxPtr& c, const T* Q, const MxScoreArgs& a, void* wo
         b.stages = MXS_STAGES / (b.warps * a.groups) ? MXS_STAGES / (b.warps * a.groups) * (b.warps * a.groups) : MXS_STAGES;
         if (!b.kept) b.stages = MXS_STAGES;
         b.lists = b.kept ? MXS_B_SLOTS / a.groups : MXS_B_SLOTS;
-        mx_slices_kernel<T><<<(unsigned)(b.last - q), 128, 0, stream>>>(Q, a.ldq, a.d, a.groups, q, slices, counts, norms);
+        launch_next(stream, mx_slices_kernel<T>, (size_t)(b.last - q), 128u, 0, Q, a.ldq, a.d, a.groups, q, slices, counts, norms);
         KERNEL_CHECK();
-        mx_score_tc_kernel<<<(unsigned)c->sm_count, MXS_THREADS, MXS_SMEM, stream>>>(b);
+        launch_next(stream, mx_score_tc_kernel, (size_t)c->sm_count, (unsigned)MXS_THREADS, (size_t)MXS_SMEM, b);
         KERNEL_CHECK();
     }
 }

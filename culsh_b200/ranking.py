@@ -348,9 +348,11 @@ def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None
         return result
     h, stream = get_handle(device.index), _stream(device)
     total = 0 if lists is None else lists.total
-    need = C.c_uint64()
-    _lib.check(h.lib.culsh_log_probs_workspace(h.ptr, _TYPES[scores.dtype], m, cols, lists is not None, total, C.byref(need)))
-    work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    need, work = C.c_uint64(), None
+    if max(cols, total // m) > 16384:  # rows that are shorter on average need none
+        _lib.check(h.lib.culsh_log_probs_workspace(h.ptr, _TYPES[scores.dtype], m, cols, lists is not None, total, C.byref(need)))
+        if need.value:
+            work = torch.empty(need.value, dtype=torch.uint8, device=device)
     at = few.data_ptr()
     _lib.check(h.lib.culsh_log_probs(
         h.ptr, scores.data_ptr(), _TYPES[scores.dtype], m, cols, pitch, lists.offsets if lists else None, (lists.ids or None) if lists else None,
