@@ -141,7 +141,7 @@ int culsh_mx_product_check(culsh_handle* h, void* stream) {
         CU_CHECK(cudaStreamSynchronize(stream_of(stream)));
         if (!word) return;
         CU_CHECK(cudaMemsetAsync(wait_word(h->ctx), 0, sizeof(word), stream_of(stream)));
-        fail(CULSH_ERR_INTERNAL, "a wait in the product ran out of time; its scores are NaN");
+        fail(CULSH_ERR_INTERNAL, "a wait in a product or in scores ran out of time; what they should have made is NaN");
     });
 }
 

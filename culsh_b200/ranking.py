@@ -243,7 +243,7 @@ class MXRows:
         return out
 
     def check(self) -> None:
-        """Waits for the current stream; raises if a product had to give up a wait (its scores are NaN then)."""
+        """Waits for the current stream; raises if a product or scores had to give up a wait (and are NaN in part)."""
         _lib.check(self._h.lib.culsh_mx_product_check(self._h.ptr, _stream(self.device)))
 
     def score(self, Q, candidates: Union[Candidates, Tuple], metric: str = "dot") -> torch.Tensor:

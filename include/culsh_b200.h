@@ -337,8 +337,8 @@ int culsh_mx_product(culsh_handle* h, const uint8_t* q_codes, const uint8_t* q_s
 int culsh_mx_product_dense(culsh_handle* h, const void* Q, int q_type, int n_queries, int64_t ldq, const uint8_t* codes,
                            const uint8_t* scales, const float* norms, int n, int d, int metric, void* out, int type, int64_t ld,
                            void* workspace, uint64_t workspace_bytes, void* stream);
-/* Waits for the stream and says whether a bounded wait of a product ran out since the last such call
- * (CULSH_ERR_INTERNAL; the scores that it should have made are NaN). */
+/* Waits for the stream and says whether a bounded wait of a product, or of scores, ran out since the last
+ * such call (CULSH_ERR_INTERNAL; the scores that it should have made are NaN). */
 int culsh_mx_product_check(culsh_handle* h, void* stream);
 /* out[c], c in [offsets[q], offsets[q + 1]): the metric of query q as it is (any type, rows ldq apart)
  * and row ids[c]; NaN where ids[c] is no row.  offsets: n_queries + 1, from 0 to total.  Queries are taken in
