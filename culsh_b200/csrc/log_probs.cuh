@@ -208,14 +208,14 @@ __device__ __forceinline__ int lp_place(int lane, int i) {
     constexpr int V = 16 / sizeof(T);
     return ((i / V) * 32 + lane) * V + i % V;
 }
-// The lane's scores of a chunk, -inf outside [begin, end).  `x`: position 0.
+// The lane's scores of a chunk, -inf outside [begin, end), by L2 (see EightOf).  `x`: position 0.
 template <typename T>
 __device__ __forceinline__ void lp_load(const T* __restrict__ x, int64_t chunk, int64_t begin, int64_t end, int lane, LpRaw<T>& s) {
     constexpr int V = 16 / sizeof(T);
     const int64_t p0 = chunk * LP_CHUNK<T>;
     if (p0 >= begin && p0 + LP_CHUNK<T> <= end) {
 #pragma unroll
-        for (int j = 0; j < LP_PER_LANE<T> / V; ++j) s.put(j, __ldg(reinterpret_cast<const uint4*>(x + p0) + j * 32 + lane));
+        for (int j = 0; j < LP_PER_LANE<T> / V; ++j) s.put(j, __ldcg(reinterpret_cast<const uint4*>(x + p0) + j * 32 + lane));
     } else {
 #pragma unroll
         for (int i = 0; i < LP_PER_LANE<T>; ++i) {

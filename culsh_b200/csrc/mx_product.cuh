@@ -167,14 +167,14 @@ __device__ __forceinline__ void mx_epilogue_few(const MxProductArgs& a, uint32_t
     const int quarter = warp & 3;
     const uint32_t accs = Cfg::ACC_COLS / a.acc_cols;
     if (a.metric != MX_DOT) {  // of the queries; each warp for itself
-        for (int q = lane; q < a.nq; q += 32) s_terms[q] = norm_term(a.metric, __ldg(a.q_norms + q));
+        for (int q = lane; q < a.nq; q += 32) s_terms[q] = norm_term(a.metric, __ldcg(a.q_norms + q));
         __syncwarp();
     }
     bool live = true;
     uint32_t ab = 0, parity = 0;
     auto norm_of = [&](unsigned v) {
         const int64_t row = (int64_t)v * MXP_B + quarter * 32 + lane;
-        return a.metric != MX_DOT && v < a.units && row < a.n ? __ldg(a.norms + row) : 0.f;
+        return a.metric != MX_DOT && v < a.units && row < a.n ? __ldcg(a.norms + row) : 0.f;
     };
     float norm = norm_of(blockIdx.x);
     for (unsigned u = blockIdx.x; u < a.units; u += gridDim.x) {
@@ -255,11 +255,11 @@ __device__ __forceinline__ void mx_epilogue_many(const MxProductArgs& a, uint32_
         if (a.metric == MX_DOT || u >= a.units) return;
         const MxUnit at(u, a);
         const int q = at.chunk * MXP_B + quarter * 32 + lane;
-        q_norm = q < a.nq ? __ldg(a.q_norms + q) : 0.f;
+        q_norm = q < a.nq ? __ldcg(a.q_norms + q) : 0.f;
 #pragma unroll
         for (int i = 0; i < MXP_B / 32; ++i) {
             const int64_t row = (int64_t)at.tile * MXP_B + i * 32 + lane;
-            norm[i] = row < a.n ? __ldg(a.norms + row) : 0.f;
+            norm[i] = row < a.n ? __ldcg(a.norms + row) : 0.f;
         }
     };
     uint32_t nth = group;  // unit of the CTA

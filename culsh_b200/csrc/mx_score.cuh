@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
             bool live = true;
             while (tiles.live() && live) {
                 const int q = tiles.q - b.first;
-                const uint32_t codes = (uint32_t)__ldg(b.counts + q) * 64u;
+                const uint32_t codes = (uint32_t)__ldcg(b.counts + q) * 64u;
                 for (int g = 0; g < a.groups; ++g) {
                     if (!b.kept || g == 0) {
                         if (!mbar_wait(&b_empty[slot], parity, s_abort, b.d_error)) { live = false; break; }
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
         while (tiles.live() && live) {
             if (tiles.q != q) {
                 q = tiles.q;
-                count = __ldg(b.counts + q - b.first);
+                count = __ldcg(b.counts + q - b.first);
             }
             const uint32_t id0 = mx_idesc(count, 0), id1 = mx_idesc(count, 2);
             if (!mbar_wait_warp(&acc_empty[acc.at], acc.parity, s_abort, b.d_error)) break;
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
             return t;
         };
         auto norm_of = [&](Ahead& t) {
-            if (a.metric != MX_DOT && (uint32_t)t.id < (uint32_t)a.n) t.norm = __ldg(a.norms + t.id);
+            if (a.metric != MX_DOT && (uint32_t)t.id < (uint32_t)a.n) t.norm = __ldcg(a.norms + t.id);
         };
         Ahead now = take(), next = take();
         norm_of(now);
@@ -474,8 +474,8 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
             norm_of(next);
             if (now.q != q) {
                 q = now.q;
-                count = __ldg(b.counts + q);
-                q_term = norm_term(a.metric, __ldg(b.q_norms + q));
+                count = __ldcg(b.counts + q);
+                q_term = norm_term(a.metric, __ldcg(b.q_norms + q));
             }
             if (live) live = mbar_wait_warp(&acc_full[acc.at], acc.parity, s_abort, b.d_error);
             tc_fence_after();

@@ -698,3 +698,30 @@ def test_the_example_finds_and_learns():
     spec.loader.exec_module(example)
     found, recall, loss = example.main(rows=20_000, queries=500, features=64, top=5, tables=16, hashes=10)
     assert found > 0.8 and recall > 0.3 and loss[1] < loss[0]
+
+
+def test_calls_behind_one_another_do_not_see_what_was_there_before(culsh):
+    """Kernels that are set up early read what the one in front wrote, in memory that earlier calls had used for the same: calls on changing data
+    without a wait between them give what they give one at a time."""
+    n, d, nq = 60_000, 128, 40
+    g = gen(11)
+    sets = [(torch.randn(n, d, generator=g, device="cuda"), torch.randn(nq, d, generator=g, device="cuda")) for _ in range(3)]
+    ids = torch.randint(0, n, (nq * 9000,), generator=g, device="cuda").int()
+    offsets = torch.arange(nq + 1, device="cuda") * 9000
+
+    def step(X, Q):
+        rows = culsh.MXRows(X)
+        s = rows.score(Q, (ids, offsets), metric="cosine")
+        p = rows.product(Q, metric="euclidean")
+        held = rows.product(culsh.MXRows(Q), metric="cosine")
+        r = culsh.log_probs(p[:3], top_k=7)  # long rows, several CTAs each
+        return s, p[:, ::997].clone(), held[:, ::997].clone(), r.lse, r.entropy, r.top_ids, r.top_log_probs
+
+    want = []
+    for X, Q in sets:
+        want.append([x.clone() for x in step(X, Q)])
+        torch.cuda.synchronize()
+    got = [(i % 3, step(*sets[i % 3])) for i in range(60)]
+    torch.cuda.synchronize()
+    for i, r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
