@@ -576,7 +576,8 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __r
 }
 
 // ------------------------------------------------------------------------------------------
-// Gradient.  Bound by HBM: 1,000 x 200,003 bfloat16 174 us (4.6 TB/s, half of it written), float32 289 (5.5); rows of scores and gradient that begin differently, 360.
+// Gradient.  Bound by HBM: 1,000 x 200,003 bfloat16 151 us (5.3 TB/s, half of it written), float32 266 (6.0); rows of scores and gradient that begin differently 300 and 361.  Two loads of a thread
+// in flight and six CTAs an SM: four loads and the four CTAs that they leave room for took 174 and 289.
 // ------------------------------------------------------------------------------------------
 struct LpBackward {
     LpArgs f;
@@ -634,7 +635,7 @@ __device__ __forceinline__ void put_grad(float* o, float v) { *o = v; }
 __device__ __forceinline__ void put_grad(__half* o, float v) { *o = __float2half_rn(v); }
 __device__ __forceinline__ void put_grad(__nv_bfloat16* o, float v) { *o = __float2bfloat16_rn(v); }
 
-// Positions [from, to) of a row by `threads` threads, whose `thread` this is, 64 bytes of each in flight; `x` and `o`: position 0 of the scores, on a 16-byte boundary, and of the gradient.
+// Positions [from, to) of a row by `threads` threads, whose `thread` this is, 32 bytes of each in flight; `x` and `o`: position 0 of the scores, on a 16-byte boundary, and of the gradient.
 // ALIKE: that is on a boundary, too, in every row.
 template <bool ALIKE, typename T>
 __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __restrict__ o, const LpRowTerms& r, float inv_t, int64_t from, int64_t to, int thread,
@@ -655,10 +656,10 @@ __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __r
             }
         }
     } else {
-        for (int64_t p0 = from / V * V + (int64_t)thread * V; p0 < to; p0 += (int64_t)4 * threads * V) {
-            uint4 w[4];
+        for (int64_t p0 = from / V * V + (int64_t)thread * V; p0 < to; p0 += (int64_t)2 * threads * V) {
+            uint4 w[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 const int64_t p = p0 + (int64_t)j * threads * V;
                 if (p >= from && p + V <= to) {
                     w[j] = __ldg(reinterpret_cast<const uint4*>(x + p));
@@ -668,7 +669,7 @@ __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __r
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 const int64_t p = p0 + (int64_t)j * threads * V;
                 if (p >= to) break;
                 float v[V];
@@ -706,7 +707,7 @@ __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __r
 template <typename T>
 constexpr int LP_ROW_SPAN = 4 * LP_THREADS * (16 / sizeof(T));
 template <bool ALIKE, typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_backward_rows_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+__global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_rows_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
     const int64_t row = blockIdx.x / (unsigned)b.units, begin = b.f.rows.begin((int)row), end = b.f.rows.end((int)row);
     const int64_t span = begin / LP_ROW_SPAN<T> + (blockIdx.x - (unsigned)row * (unsigned)b.units);
     const int64_t from = max(span * LP_ROW_SPAN<T>, begin), to = min((span + 1) * LP_ROW_SPAN<T>, end);
@@ -717,7 +718,7 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_backward_rows_kernel(con
 
 // A warp for a span of all lists' positions, and for each list in it: what it has to know of a list takes longer than a short one.
 template <bool ALIKE, typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_backward_lists_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+__global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_lists_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
     const int64_t n = (int64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5);
     if (n >= b.units) return;
     const LpRows& rows = b.f.rows;
