@@ -7,7 +7,7 @@
 // in 32 bits; entropy = log l - log(2) e / l.  A larger m rescales both.  d is one multiply-add, of s with the rounded product of m: what its rounding moved all d by is taken out of
 // the sums at the end.  Parts (m, l, e) are joined in a fixed order, so results do not depend on how CTAs are scheduled.  An entry of -inf counts as a score so low that 2^d is 0 and d is finite;
 // where m itself is that low, d is cut at -10,000 instead.  NaN and +inf reach the sums and make them NaN.
-// Bound by HBM with 32 bits (1,000 x 1M 584 us, 6.8 TB/s), by the issue of five instructions and an exponential for an entry with 16 (363 us, 5.5 TB/s, 325 of them without the k largest;
+// Bound by HBM with 32 bits (1,000 x 1M 584 us, 6.8 TB/s), by the issue of five instructions and an exponential for an entry with 16 (369 us, 5.4 TB/s, 325 of them without the k largest;
 // a pass of eight instructions 579). 10,000 lists of 18,000 float32 211 us, 148 without the k largest: what follows the pass is waits.
 //
 // The k largest: the pass leaves the largest entry of each thread and of each chunk behind.  The k-th largest of the threads' is a bound that at least k entries reach, and hardly more do (of 1M
@@ -256,12 +256,15 @@ __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t fir
         }
         if (in_short()) {
             const float2 c2 = make_float2(c, c), from = make_float2(-mc, -mc);
+            float2 lc = make_float2(0.f, 0.f), ec = lc;  // of the chunk: thousands of terms one by one into one sum cost it two digits
 #pragma unroll
             for (int i = 0; i < LP_PER_LANE<T> / 2; ++i) {
                 const float2 d = fma2(s.pair(i), c2, from), p = make_float2(exp2_fast(d.x), exp2_fast(d.y));
-                l = add2(l, p);
-                e = fma2(p, d, e);
+                lc = add2(lc, p);
+                ec = fma2(p, d, ec);
             }
+            l = add2(l, lc);
+            e = add2(e, ec);
         } else {
 #pragma unroll
             for (int i = 0; i < LP_PER_LANE<T>; ++i) {

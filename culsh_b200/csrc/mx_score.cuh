@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, 
 // bits at least, so that a query of float32 values within a factor of 2^10 of one another in a block is the sum of about 18 slices, one of bytes that of five: nothing is rounded
 // off.  Sixteen, 32, 48 or 64 slices of a query are the N side of the MMAs; those beyond 64 would be below 2^-126 of the block's largest value.  The M side are 128 candidates of a list, whose codes
 // and scales are gathered by cp.async to where the MMAs take them, and the score is the sum of the accumulator's columns.  No code is unpacked by an instruction:
-// 180M candidates of 128 values 12.0 -> 3.9 ms.  Of 100,000 rows, which lie in L2, they take 2.5 ms: what a warp does for a
-// tile; of a million the gather takes longer: L2 gives 8 TB/s in pieces of 32 and 64 bytes, 174 bytes a candidate with its norm (3.1 ms without).  Codes gathered by TMA took 3.4 ms
+// 180M candidates of 128 values 12.0 -> 3.7 ms.  Of 100,000 rows, which lie in L2, they take 2.5 ms: what a warp does for a
+// tile; of a million the gather takes longer: L2 gives 8 TB/s in pieces of 32 and 64 bytes, 174 bytes a candidate with its norm (3.1 ms without it).  Codes gathered by TMA took 3.4 ms
 // in either case.
 //
 // One persistent CTA per SM.  Warps 0 - 11 gather (four a stage), 12 loads slices, 13 - 18 issue MMAs (a tile each: what a warp does for one takes 1,300 cycles), 19 - 30 epilogue (four a tile).
