@@ -50,7 +50,8 @@ LpArgs log_probs_args(const void* scores, int m, int64_t cols, int64_t ld, const
     need(m > 0, "rows must be positive");
     need(temperature > 0 && std::isfinite(temperature) && std::isfinite(1 / (float)temperature), "temperature must be positive");
     if (offsets) {
-        need(total >= 0 && total < (1ll << 40), "total must not be negative");
+        need(total >= 0, "total must not be negative");
+        if (total >= (ids ? 1ll << 32 : 1ll << 31)) fail(CULSH_ERR_UNSUPPORTED, "%lld entries are too many for one call", (long long)total);  // places have 32 bits
         need(!(targets && !ids), "targets of lists need the lists' ids");
     } else {
         need(cols > 0 && cols < (1ll << 31), "columns must be positive and below 2^31");

@@ -359,6 +359,7 @@ int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* str
  *   entropy        of the distribution exp(z - lse); 0 there
  *   log_probs      z - lse of the entry targets[r] (column, or id of the list); -inf if the row has none such
  *   top_*  [m][k]  the k <= 128 largest, the earlier of equal ones first; -inf and -1 behind the last one
+ * At most 2^32 - 1 entries of lists in a call, 2^31 - 1 without ids.
  * A NaN or +inf makes its row's numbers NaN.  targets / log_probs may be NULL.  workspace: device, as
  * many bytes as culsh_log_probs_workspace says (0 for rows of up to 16,384 entries on average), aligned to 16. */
 int culsh_log_probs_workspace(culsh_handle* h, int type, int m, int64_t cols, int is_lists, int64_t total, uint64_t* bytes);

@@ -725,3 +725,13 @@ def test_calls_behind_one_another_do_not_see_what_was_there_before(culsh):
     torch.cuda.synchronize()
     for i, r in got:
         assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_more_entries_than_places_have_bits_for_are_refused(culsh):
+    from culsh_b200 import _lib
+    from culsh_b200._culsh_core import get_handle
+    h, x = get_handle(0), torch.zeros(64, dtype=torch.int64, device="cuda")
+    at = x.data_ptr()
+    for ids, total in ((None, 2 ** 31), (at, 2 ** 32)):
+        status = h.lib.culsh_log_probs(h.ptr, at, 0, 1, 0, 0, at, ids, total, 1.0, None, 0, None, at, at, None, None, None, 0, None)
+        assert status == -5 and b"too many" in _lib.load().culsh_last_error()
