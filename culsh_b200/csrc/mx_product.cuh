@@ -79,6 +79,7 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
 }
 // The MMAs are issued by a whole warp, whose elected lane (the same each time) does it: what a single lane computes on its own does not get into the uniform registers that these
 // instructions take their operands from without one instruction, and its latency, for each.
+// Only whole warps may call these: the election waits for all 32 lanes, without a bound, so whatever leads to them has one answer for the warp (mbar_wait_warp).
 // 32 rows of 16 bytes into four columns of 32 lanes, the same for each quarter of the lanes.
 __device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
     asm volatile(
