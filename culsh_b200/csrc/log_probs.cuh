@@ -5,7 +5,7 @@
 // One pass over the scores.  A warp takes chunks of 512 neighbouring entries, or 1,024 of 16 bits, and keeps the largest score so far m and two sums relative to it,
 //   l = sum 2^d,   e = sum d 2^d,   d = (s - m) log2(e) / temperature,
 // in 32 bits; entropy = log l - log(2) e / l.  A larger m rescales both.  d is one multiply-add, of s with the rounded product of m: what its rounding moved all d by is taken out of
-// the sums at the end.  Parts (m, l, e) are joined in a fixed order, so results do not depend on how CTAs are scheduled.  An entry of -inf counts as a score so low that 2^d is 0 and d is finite;
+// the sums at the end; of scores of 2^24 bits and more, where it would move d by whole bits, d is (s - m) log2(e) / temperature as it stands.  Parts (m, l, e) are joined in a fixed order, so results do not depend on how CTAs are scheduled.  An entry of -inf counts as a score so low that 2^d is 0 and d is finite;
 // where m itself is that low, d is cut at -10,000 instead.  NaN and +inf reach the sums and make them NaN.
 // Bound by HBM with 32 bits (1,000 x 1M 584 us, 6.8 TB/s), by the issue of five instructions and an exponential for an entry with 16 (369 us, 5.4 TB/s, 325 of them without the k largest;
 // a pass of eight instructions 579). 10,000 lists of 18,000 float32 211 us, 148 without the k largest: what follows the pass is waits.
@@ -31,6 +31,8 @@ constexpr int LP_CHUNK = 32 * LP_PER_LANE<T>;
 constexpr int LP_LEAST_CHUNK = 512;
 constexpr int LP_MAX_K = 128;
 constexpr float LP_FLOOR = -10000.f;
+// Products of the largest score with c up to which d counts from the rounded product: that is half a bit off at most, and 2^d of the largest entry close to 1.
+constexpr float LP_SHORT = 16777216.f;
 
 // Where rows are: a matrix with rows `ld` apart and `cols` long, or lists.  Positions of row r: [begin, end).
 struct LpRows {
@@ -232,7 +234,8 @@ __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t fir
                                             float& largest, Leave leave) {
     float m = LpPart::none().m, mc = m * c;  // the same in all lanes; mc: what d counts from in the short way
     const bool common = c > 0.01f && c < 1e4f;
-    auto in_short = [&]() { return common && m > LpRaw<T>::SAFE && fabsf(mc) < 1e33f; };
+    auto is_short = [&](float m, float mc) { return common && m > LpRaw<T>::SAFE && fabsf(mc) < LP_SHORT; };
+    auto in_short = [&]() { return is_short(m, mc); };
     float2 l = make_float2(0.f, 0.f), e = l;
     LpRaw<T> next;
     if (first < last) lp_load(x, first, begin, end, lane, next);
@@ -246,7 +249,10 @@ __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t fir
         if (top != top) top = -INFINITY;
         leave(chunk, top);
         if (top > m) {
-            const float to = top * c, d = max_nan(in_short() ? mc - to : (m - top) * c, LP_FLOOR), f = exp2_fast(d);
+            const float to = top * c;
+            const bool was = in_short(), is = is_short(top, to);
+            // from what the sums are relative to, mc or m c itself, to what they will be
+            const float d = max_nan(was ? (is ? mc - to : -fmaf(top, c, -mc)) : is ? fmaf(m, c, -to) : (m - top) * c, LP_FLOOR), f = exp2_fast(d);
             e.x = (e.x + l.x * d) * f;
             e.y = (e.y + l.y * d) * f;
             l.x *= f;
