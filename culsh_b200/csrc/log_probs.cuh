@@ -30,6 +30,7 @@ template <typename T>
 constexpr int LP_CHUNK = 32 * LP_PER_LANE<T>;
 constexpr int LP_LEAST_CHUNK = 512;
 constexpr int LP_MAX_K = 128;
+constexpr uint32_t LP_NO_PLACE = 0xFFFFFFFFu;
 constexpr float LP_FLOOR = -10000.f;
 // Products of the largest score with c up to which d counts from the rounded product: that is half a bit off at most, and 2^d of the largest entry close to 1.
 constexpr float LP_SHORT = 16777216.f;
@@ -48,7 +49,7 @@ struct LpRows {
 
 struct LpArgs {
     LpRows rows;
-    const int32_t* ids;       // names of the entries of lists, ascending in each, or null
+    const int32_t* ids;       // names of the entries of lists, or null
     const int64_t* targets;   // or null
     float* log_probs;         // or null, with targets
     float* entropy;
@@ -56,6 +57,7 @@ struct LpArgs {
     float* top_log_probs;     // or null, with k = 0
     int32_t* top_ids;
     int m, k;
+    bool placed;              // log_probs_places_kernel has been launched in front
     float c, inv_t;           // log2(e) / temperature, 1 / temperature
     // rows taken by several CTAs
     int64_t unit;             // positions of a CTA, a multiple of 1,024
@@ -382,7 +384,8 @@ __device__ __forceinline__ float lp_bound(LpShared<TH>& sh, float mine, int k) {
     return bound;
 }
 
-// Position of the entry that a target names in a row, or -1; by one warp.  The first 32 ids that it looks at can be asked for long before.
+// Position of the entry that a target names in a row, or -1 where it does not stand where ascending ids would have it; by one warp.  The first 32 ids that it looks at (all, where there
+// are no more) can be asked for long before.
 struct LpFind {
     int64_t lo, hi, step, target;  // ids below lo are smaller, at and behind hi larger
     int32_t id;
@@ -411,11 +414,78 @@ struct LpFind {
     }
 };
 
+// The first entry of [begin, end) that a target names, of those that thread `thread` of `threads` looks at, or `end`.  For lists in any order: that the search does not find an id says nothing
+// of them.  N loads of a thread are on their way at a time.
+template <int N>
+__device__ __forceinline__ int64_t lp_first_named(const int32_t* __restrict__ names, int64_t begin, int64_t end, int64_t target, int thread, int threads) {
+    const int32_t name = (int32_t)target;
+    if (name != target) return end;
+#pragma unroll 1
+    for (int64_t p0 = begin - (int64_t)((uintptr_t)(names + begin) / 4 % 4) + 4 * thread; p0 < end; p0 += (int64_t)4 * N * threads) {
+        int4 w[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int64_t p = p0 + (int64_t)4 * j * threads;
+            if (p >= begin && p + 4 <= end) {
+                w[j] = __ldcg(reinterpret_cast<const int4*>(names + p));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) reinterpret_cast<int32_t*>(&w[j])[i] = p + i >= begin && p + i < end ? __ldcg(names + p + i) : ~name;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = w[j].x == name ? 0 : w[j].y == name ? 1 : w[j].z == name ? 2 : w[j].w == name ? 3 : -1;
+            if (at >= 0) return p0 + (int64_t)4 * j * threads + at;
+        }
+    }
+    return end;
+}
+// By a CTA whose threads have seen that `found`, in shared memory, is -1: the first entry of the row, if there is one.
+template <int N = 4>
+__device__ __forceinline__ void lp_find_in_any_order(const LpArgs& a, int row, int64_t begin, int64_t end, int64_t& found, int threads) {
+    const int64_t first = lp_first_named<N>(a.ids - a.rows.shift, begin, end, __ldg(a.targets + row), threadIdx.x, threads);
+    __syncthreads();
+    if (first < end) atomicMin(reinterpret_cast<unsigned long long*>(&found), (unsigned long long)first);
+    __syncthreads();
+}
+// Whether a list can have an entry that the search did not find.
+__device__ __forceinline__ bool lp_may_be_left(int64_t begin, int64_t end) { return end - begin > 32; }
+
+// Lists [0, m) by CTAs of LP_WARPS warps, of which this is the one `cta` of `ctas`: look(row) by a warp for those that may(row) says so of, then rest(row) by the CTA where that was true.
+template <typename May, typename Look, typename Rest>
+__device__ __forceinline__ void lp_by_warps_then_ctas(int m, int cta, int ctas, May may, Look look, Rest rest) {
+    __shared__ unsigned s_left[LP_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = min((m - 1) / (ctas * LP_WARPS) + 1, 32);  // lists for a warp at a time
+    for (int64_t row0 = (int64_t)cta * LP_WARPS * per; row0 < m; row0 += (int64_t)ctas * LP_WARPS * per) {
+        const int64_t mine = row0 + warp * per + lane;
+        unsigned left = 0;
+        for (unsigned some = __ballot_sync(0xFFFFFFFFu, lane < per && mine < m && may((int)mine)); some; some &= some - 1)
+            if (look((int)(row0 + warp * per) + __ffs((int)some) - 1)) left |= some & -some;
+        if (lane == 0) s_left[warp] = left;
+        __syncthreads();
+        for (int w = 0; w < LP_WARPS; ++w)
+            for (unsigned some = s_left[w]; some; some &= some - 1) rest((int)(row0 + w * per) + __ffs((int)some) - 1);
+        __syncthreads();
+    }
+}
+
 // What a row's result is made of, by the whole CTA.  `maxima`: orders of the largest scores of groups of 1 << wide chunks from first_chunk on; `largest`: a thread's own score, of no
 // other's entry.
 template <int TH, typename T>
 __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs& a, LpShared<TH>& sh, int row, int64_t begin, int64_t end, LpPart all,
                                           const uint32_t* maxima, int64_t first_chunk, int64_t last_chunk, int wide, float largest) {
+    if (a.targets && a.ids) {
+        if (a.placed) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");  // for log_probs_places_kernel
+            if (threadIdx.x == 0) {  // who needs it and overwrites it
+                const uint32_t place = __ldcg(reinterpret_cast<const uint32_t*>(a.log_probs) + row);
+                sh.target = place == LP_NO_PLACE ? -1 : begin + place;
+            }
+        } else if (sh.target < 0 && lp_may_be_left(begin, end)) {
+            lp_find_in_any_order(a, row, begin, end, sh.target, TH);
+        }
+    }
     const float log_l = logf(all.l);
     const float z_max = all.m * a.inv_t;
     float lse = z_max + log_l, entropy = log_l - 0.69314718056f * (all.e / all.l);
@@ -479,6 +549,29 @@ __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs&
     }
 }
 
+// Long lists: where the entries are that targets name, before the pass needs to know.  A list whose target is not where a search finds it is looked through, for which a CTA of the pass may be a
+// warp: that warp's list took twice as long, and was the last (10,000 lists of 18,000 float32, a tenth of the targets in none: 324 us, 210 without looking through).  Places in the
+// list wait in the row's log probability until the pass puts that there.
+__global__ void __launch_bounds__(LP_THREADS) log_probs_places_kernel(LpArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ int64_t s_found;
+    uint32_t* const places = reinterpret_cast<uint32_t*>(a.log_probs);
+    lp_by_warps_then_ctas(
+        a.m, blockIdx.x, gridDim.x, [](int) { return true; },
+        [&](int row) {
+            const int64_t begin = a.rows.begin(row), end = a.rows.end(row), at = LpFind(a, row, begin, end)(a);
+            if ((threadIdx.x & 31) == 0) places[row] = at < 0 ? LP_NO_PLACE : (uint32_t)(at - begin);
+            return at < 0 && lp_may_be_left(begin, end);
+        },
+        [&](int row) {
+            const int64_t begin = a.rows.begin(row), end = a.rows.end(row);
+            if (threadIdx.x == 0) s_found = -1;
+            lp_find_in_any_order<8>(a, row, begin, end, s_found, LP_THREADS);
+            if (threadIdx.x == 0 && s_found >= 0) places[row] = (uint32_t)(s_found - begin);
+            __syncthreads();
+        });
+}
+
 // A CTA of TH threads for each row.
 template <int TH, typename T>
 __global__ void __launch_bounds__(TH) log_probs_row_kernel(const T* __restrict__ x, LpArgs a) {
@@ -498,7 +591,7 @@ __global__ void __launch_bounds__(TH) log_probs_row_kernel(const T* __restrict__
     };
     LpPart mine;
     float largest = -INFINITY;
-    if (warp == TH / 32 - 1 && a.targets) {  // the warp with the fewest chunks
+    if (warp == TH / 32 - 1 && a.targets && !a.placed) {  // the warp with the fewest chunks
         LpFind find(a, row, begin, end);
         mine = lp_chunks(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
         const int64_t at = find(a);
@@ -597,6 +690,7 @@ struct LpBackward {
     int64_t ldo;            // of the result, where it is a matrix
     int64_t units;          // spans of positions: of all lists, or that a matrix's row can reach into
     int span;               // positions of lists for a warp
+    int whole, shares;      // CTAs in front of the others, and how many of them have a list, see lp_backward_whole
 };
 
 // Constants of a row: ds = p (a - b log p), and more at the given entry; log p = z - lse, a = -(h entropy + g) / temperature, b = h / temperature, g by the temperature.
@@ -607,25 +701,30 @@ struct LpRowTerms {
 };
 
 template <typename T>
-__device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, const LpBackward& b, int row, int64_t begin, int64_t end) {
+__device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, const LpBackward& b, int row, int64_t target) {
     LpRowTerms r;
     const float h = b.h ? __ldg(b.h + row) : 0.f, entropy = __ldg(b.entropy + row);
     float g = b.f.targets && b.g ? __ldg(b.g + row) : 0.f;
     r.lse = __ldg(b.lse + row);
     if (r.lse == -INFINITY) r.lse = 0.f;  // all masked: 2^-inf is 0 then
     r.bad = r.lse != r.lse;
-    r.target = -1;
-    if (b.f.targets && b.g) {
-        r.target = LpFind(b.f, row, begin, end)(b.f);
-        if (r.target < 0 || score_of(x[r.target]) * b.f.inv_t == -INFINITY) {  // a log probability of -inf stays where it is
-            r.target = -1;
-            g = 0.f;
-        }
+    r.target = target;
+    if (target < 0 || score_of(x[target]) * b.f.inv_t == -INFINITY) {  // a log probability of -inf stays where it is
+        r.target = -1;
+        g = 0.f;
     }
     r.a = -(h * entropy + g) * b.f.inv_t;
     r.b = h * b.f.inv_t;
     r.g = g * b.f.inv_t;
     return r;
+}
+// The entry that has the gradient of a row's log probability, or -1; by a warp.  `whole`: it takes the whole row to say.
+__device__ __forceinline__ int64_t lp_given(const LpBackward& b, int row, int64_t begin, int64_t end, bool& whole) {
+    whole = false;
+    if (!b.f.targets || !b.g) return -1;
+    const int64_t at = LpFind(b.f, row, begin, end)(b.f);
+    whole = at < 0 && b.f.ids && lp_may_be_left(begin, end);
+    return at;
 }
 __device__ __forceinline__ float2 lp_grad(const LpRowTerms& r, float2 s, float inv_t) {
     float2 lp = fma2(s, make_float2(inv_t, inv_t), make_float2(-r.lse, -r.lse));
@@ -721,14 +820,45 @@ __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_
     const int64_t span = begin / LP_ROW_SPAN<T> + (blockIdx.x - (unsigned)row * (unsigned)b.units);
     const int64_t from = max(span * LP_ROW_SPAN<T>, begin), to = min((span + 1) * LP_ROW_SPAN<T>, end);
     if (from >= to) return;
-    const LpRowTerms r = lp_row_terms(x, b, (int)row, begin, end);
+    bool whole;
+    const LpRowTerms r = lp_row_terms(x, b, (int)row, lp_given(b, (int)row, begin, end, whole));
     lp_backward_span<ALIKE>(x, out + (row * b.ldo - begin), r, b.f.inv_t, from, to, threadIdx.x, LP_THREADS);
+}
+
+// Lists that have to be looked at as a whole before any of their gradient is known: those whose target is not where a search finds it.  Each has a CTA of the first ones, which look
+// at the others for that only; the warps with spans leave them alone.
+template <bool ALIKE, typename T>
+__device__ __forceinline__ void lp_backward_whole(const T* __restrict__ x, T* __restrict__ out, const LpBackward& b) {
+    __shared__ int64_t s_target;
+    const LpRows& rows = b.f.rows;
+    // few lists have several CTAs each, which look through all of it and take their share of what follows
+    const int share = (int)blockIdx.x % b.shares;
+    lp_by_warps_then_ctas(
+        b.f.m, (int)blockIdx.x / b.shares, b.whole / b.shares, [&](int row) { return lp_may_be_left(rows.begin(row), rows.end(row)); },
+        [&](int row) {
+            bool whole;
+            lp_given(b, row, rows.begin(row), rows.end(row), whole);
+            return whole;
+        },
+        [&](int row) {
+            const int64_t begin = rows.begin(row), end = rows.end(row);
+            if (threadIdx.x == 0) s_target = -1;
+            lp_find_in_any_order(b.f, row, begin, end, s_target, LP_THREADS);
+            const LpRowTerms r = lp_row_terms(x, b, row, s_target);
+            const int64_t each = ((end - begin) / b.shares / 16 + 1) * 16, from = begin + share * each;
+            lp_backward_span<ALIKE>(x, out - rows.shift, r, b.f.inv_t, from, min(from + each, end), threadIdx.x, LP_THREADS);
+            __syncthreads();
+        });
 }
 
 // A warp for a span of all lists' positions, and for each list in it: what it has to know of a list takes longer than a short one.
 template <bool ALIKE, typename T>
 __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_lists_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
-    const int64_t n = (int64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5);
+    if (blockIdx.x < (unsigned)b.whole) {
+        lp_backward_whole<ALIKE>(x, out, b);
+        return;
+    }
+    const int64_t n = (int64_t)(blockIdx.x - (unsigned)b.whole) * LP_WARPS + (threadIdx.x >> 5);
     if (n >= b.units) return;
     const LpRows& rows = b.f.rows;
     const int64_t p0 = n * b.span, p1 = p0 + b.span;
@@ -737,7 +867,10 @@ __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_
         if (begin >= p1) break;
         const int64_t from = max(begin, p0), to = min(end, p1);
         if (from >= to) continue;
-        const LpRowTerms r = lp_row_terms(x, b, row, begin, end);
+        bool whole;
+        const int64_t target = lp_given(b, row, begin, end, whole);
+        if (whole) continue;
+        const LpRowTerms r = lp_row_terms(x, b, row, target);
         lp_backward_span<ALIKE>(x, out - rows.shift, r, b.f.inv_t, from, to, threadIdx.x & 31, 32);
     }
 }
@@ -780,8 +913,22 @@ inline void log_probs(const CtxPtr& c, const T* scores, LpArgs a, void* workspac
         int th = mean <= 1024 || (a.m >= 32 * c->sm_count && mean <= 32768) ? 32 : a.m >= 16 * c->sm_count && mean <= 16384 ? 64 : 128;
         while (th < a.k) th *= 2;
         auto kern = th == 32 ? log_probs_row_kernel<32, T> : th == 64 ? log_probs_row_kernel<64, T> : log_probs_row_kernel<128, T>;
-        kern<<<(unsigned)a.m, th, 0, stream>>>(x, a);
-        KERNEL_CHECK();
+        cudaLaunchAttribute attr[1]{};
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)a.m);
+        cfg.blockDim = dim3((unsigned)th);
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        a.placed = a.ids && a.targets && mean > 1024;
+        if (a.placed) {
+            // Set up and begun while that runs: all that the pass reads had been written before that began.  It waits where it needs the places.
+            log_probs_places_kernel<<<(unsigned)std::min((a.m - 1) / LP_WARPS + 1, 8 * c->sm_count), LP_THREADS, 0, stream>>>(a);
+            KERNEL_CHECK();
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.numAttrs = 1;
+        }
+        CU_CHECK(launch_cast(cfg, kern, x, a));
         return;
     }
     if (workspace_bytes < p.bytes() || !workspace || ((uintptr_t)workspace & 15)) fail(CULSH_ERR_INVALID, "the workspace has to be %zu bytes, aligned to 16", p.bytes());
@@ -797,14 +944,18 @@ inline void log_probs(const CtxPtr& c, const T* scores, LpArgs a, void* workspac
 }
 
 template <typename T>
-inline void log_probs_backward(const T* scores, T* out, LpBackward b, cudaStream_t stream) {
+inline void log_probs_backward(const CtxPtr& c, const T* scores, T* out, LpBackward b, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     LpRows& r = b.f.rows;
     r.shift = (int64_t)((uintptr_t)scores / sizeof(T) % V);
     const int64_t mean = r.total / b.f.m;
     b.span = mean >= 1024 ? 512 : mean >= 64 ? 128 : 32;
     b.units = r.offsets ? (int64_t)ceil_div((size_t)(r.total + r.shift), (size_t)b.span) : r.cols / LP_ROW_SPAN<T> + 2;
-    const size_t grid = r.offsets ? ceil_div((size_t)b.units, LP_WARPS) : (size_t)b.units * b.f.m;
+    b.whole = r.offsets && b.f.ids && b.f.targets && b.g ? 2 * c->sm_count : 0;
+    b.shares = 1;
+    while (b.shares < 16 && 2 * b.shares * ((b.f.m - 1) / LP_WARPS + 1) <= b.whole) b.shares *= 2;
+    b.whole = std::min((b.f.m - 1) / LP_WARPS + 1, b.whole / b.shares) * b.shares;
+    const size_t grid = r.offsets ? b.whole + ceil_div((size_t)b.units, LP_WARPS) : (size_t)b.units * b.f.m;
     if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "too many entries for one call");
     const bool alike = (((uintptr_t)(out - r.shift) | (r.offsets ? 0u : (uintptr_t)((b.ldo - r.ld) * (int64_t)sizeof(T)))) & 15u) == 0;
     auto kern = r.offsets ? (alike ? log_probs_backward_lists_kernel<true, T> : log_probs_backward_lists_kernel<false, T>)

@@ -224,7 +224,7 @@ int culsh_log_probs_backward(culsh_handle* h, const void* scores, int type, int 
         DeviceGuard g(h->ctx->device);
         by_type(type, SCORE_TYPES, scores, [&](auto* s) {
             using T = std::remove_const_t<std::remove_pointer_t<decltype(s)>>;
-            if constexpr (!std::is_same<T, double>::value) log_probs_backward(s, static_cast<T*>(grad_scores), b, stream_of(stream));
+            if constexpr (!std::is_same<T, double>::value) log_probs_backward(h->ctx, s, static_cast<T*>(grad_scores), b, stream_of(stream));
         });
     });
 }

@@ -1,6 +1,6 @@
 """Ranking of candidates: rows held in 4 bits, their scores against queries, and log probabilities over scores.
 
-``query`` answers with the ids of candidate rows, in no order.  Here the rows are kept in microscaled 4-bit floating point
+``query`` answers with the ids of candidate rows, not ranked.  Here the rows are kept in microscaled 4-bit floating point
 (``MXRows``: 17 bytes for 32 values), queries are scored against their candidates (``MXRows.score``) or against every
 row (``MXRows.product``), and ``log_probs`` turns scores into what an answer needs: the most likely rows, their log
 probabilities, and the entropy of the distribution; ``log_probs_backward`` is its gradient, for training an encoder on candidate lists.
@@ -321,7 +321,7 @@ def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None
 
     ``scores``: [m, n] (``MXRows.product``), or the scores of candidate lists (``MXRows.score``) with ``lists`` the Candidates or a pair
     (ids or None, offsets); float32, float16 or bfloat16; -inf takes an entry out.
-    ``targets``: [m] columns, or ids of the lists.  ``top_k``: at most 128; of equal scores the first one goes first."""
+    ``targets``: [m] columns, or ids of the lists, each of which may stand in any order and holds an id once.  ``top_k``: at most 128; of equal scores the first one goes first."""
     top_k = int(top_k)
     if not 0 <= top_k <= MAX_TOP_K:
         raise ValueError(f"top_k must be between 0 and {MAX_TOP_K}")

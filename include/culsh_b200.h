@@ -353,8 +353,8 @@ int culsh_mx_score(culsh_handle* h, const void* Q, int type, int n_queries, int6
 int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* stream);
 
 /* Rows of scores (float32, float16, bfloat16): a matrix [m][cols] with rows ld apart (offsets and ids
- * NULL), or m lists, offsets[m + 1] from 0 to total, with ids ascending in each (ids may be NULL
- * where there are no targets: entries are then named by their place).  With z = scores / temperature:
+ * NULL), or m lists, offsets[m + 1] from 0 to total, with distinct ids in each, in any order (targets are found sooner in
+ * ascending ones; ids may be NULL where there are no targets: entries are then named by their place).  With z = scores / temperature:
  *   lse            log of the sum of exp(z); -inf for a row with nothing in it that is not -inf
  *   entropy        of the distribution exp(z - lse); 0 there
  *   log_probs      z - lse of the entry targets[r] (column, or id of the list); -inf if the row has none such

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_ranking import HALF_ULP, ULP, csr, gen, gradient_of, held
+from test_gpu_ranking import HALF_ULP, ULP, gen, gradient_of
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,76 @@ def test_log_probs_of_large_scores(culsh, top, temperature, n, dtype):
         order = np.lexsort((np.arange(n), -z))[:3]
         assert r.top_ids[i].tolist() == order.tolist()
         assert np.all(np.abs(r.top_log_probs[i].double().cpu().numpy() - lp[order]) <= few + 4 * ULP * np.abs(lp[order]))
+
+
+# ---- lists in any order ---------------------------------------------------------------------------------------------
+def mixed(lengths, n, order, seed):
+    """Lists of distinct ids: ascending, ascending but for the last one, descending, or shuffled."""
+    rng = np.random.RandomState(seed)
+    lists = []
+    for m in lengths:
+        mine = np.cumsum(rng.randint(1, max(n // max(m, 1), 1) + 1, m)) - 1  # distinct and below n
+        if order == "last" and m > 1:  # a positive behind ascending negatives
+            at = rng.randint(m - 1)
+            mine = np.append(np.delete(mine, at), mine[at])
+        elif order == "down":
+            mine = mine[::-1]
+        elif order == "any":
+            mine = rng.permutation(mine)
+        lists.append(mine)
+    offsets = torch.from_numpy(np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64))
+    return torch.from_numpy(np.concatenate(lists).astype(np.int32)).cuda(), offsets.cuda()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("order", ["last", "down", "any"])
+@pytest.mark.parametrize("lengths", [[31, 0, 32, 33, 64, 1, 65, 0, 2, 129, 1000, 2050, 7], [64] * 600, [50_000, 0, 3, 70_001], [300_000] + [40] * 2000, [40] * 9 + [3] * 20_000,
+                                     [3000] * 200, [20_000] * 300])
+def test_targets_of_lists_in_any_order(culsh, lengths, order, dtype):
+    n, temperature = 3 * max(lengths), 0.5
+    all_ids, offsets = mixed(lengths, n, order, 5)
+    m, total = len(lengths), all_ids.shape[0]
+    for lead in (0, 1, 3):  # ids and scores that begin off a boundary, too
+        ids = torch.cat([all_ids[:lead], all_ids])[lead:]
+        s = torch.randn(total + lead, generator=gen(3), device="cuda").to(dtype)[lead:]
+        ends = offsets.tolist()
+        if order == "last":
+            at = [max(k - 1, 0) for k in lengths]
+        else:
+            at = [(7 * i + 3) % k if k else 0 for i, k in enumerate(lengths)]
+        targets = torch.tensor([n + 1 if i % 6 == 5 or not k else int(v) for i, (k, v) in enumerate(zip(
+            lengths, ids.cpu()[(offsets[:-1].cpu() + torch.tensor(at)).clamp(max=total - 1)]))], device="cuda")
+        r = culsh.log_probs(s, targets, (ids, offsets), temperature=temperature)
+        gl, ge = torch.randn(m, generator=gen(6), device="cuda"), torch.randn(m, generator=gen(7), device="cuda")
+        got = culsh.log_probs_backward(s, targets, r.lse, r.entropy, gl, ge, (ids, offsets), temperature)
+        got, z, lp = got.double().cpu().numpy(), s.double().cpu().numpy(), r.log_probs.double().cpu().numpy()
+        t = targets.tolist()
+        for i in sorted(set(range(min(m, 20))) | {m - 1}):
+            k = lengths[i]
+            if not k:
+                assert lp[i] == -math.inf
+                continue
+            mine = z[ends[i]:ends[i + 1]]
+            place = None if t[i] > n else at[i]
+            _, _, want, _ = answer_of(mine, temperature)
+            tol = ULP * (32 + 4 * math.log(max(k, 2)))
+            assert lp[i] == -math.inf if place is None else abs(lp[i] - want[place]) <= tol + 4 * ULP * abs(want[place]), (i, lp[i])
+            # p errs by what log p does, of its own size; entropy and log p of no more than 100 by h p
+            a, h = float(gl[i]), float(ge[i])
+            grad = gradient_of(mine / temperature, place, a, h, temperature)
+            bound = 8 * ULP * 64 * (abs(a) + 64 * abs(h)) / temperature + HALF_ULP[dtype] * np.abs(grad) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+            assert np.all(np.abs(got[ends[i]:ends[i + 1]] - grad) <= bound), i
+
+
+def test_rank_finds_targets_among_candidates_in_any_order(culsh):
+    n, nq, mean = 5000, 50, 400
+    X, Q = torch.randn(n, 64, generator=gen(), device="cuda"), torch.randn(nq, 64, generator=gen(1), device="cuda")
+    rows = culsh.MXRows(X)
+    up, offsets = mixed([mean] * nq, n, "up", 2)
+    ids = up.view(nq, mean)[:, torch.randperm(mean, generator=gen(3), device="cuda")].reshape(-1)
+    targets = ids[offsets[:-1] + 7].long()
+    a = culsh.rank(rows, Q, (up, offsets), top_k=5, metric="cosine", temperature=0.1, targets=targets)
+    b = culsh.rank(rows, Q, (ids, offsets), top_k=5, metric="cosine", temperature=0.1, targets=targets)
+    assert bool(torch.isfinite(b.log_probs).all())
+    assert torch.allclose(a.log_probs, b.log_probs, rtol=0, atol=1e-4)  # float32 scores of other lanes and sums
+    assert torch.equal(a.top_ids, b.top_ids)
