@@ -32,6 +32,9 @@ constexpr int LP_LEAST_CHUNK = 512;
 constexpr int LP_MAX_K = 128;
 constexpr uint32_t LP_NO_PLACE = 0xFFFFFFFFu;
 constexpr float LP_FLOOR = -10000.f;
+constexpr int LP_LOOK = 1024;  // entries of a list that a warp of the gradient looks through by itself
+// Largest |lse| from which the gradient counts log p: the rounding of lse is an error of every p, of 4e-6 there.
+constexpr float LP_NEAR = 64.f;
 // Products of the largest score with c up to which d counts from the rounded product: that is half a bit off at most, and 2^d of the largest entry close to 1.
 constexpr float LP_SHORT = 16777216.f;
 
@@ -234,7 +237,7 @@ __device__ __forceinline__ void lp_load(const T* __restrict__ x, int64_t chunk, 
 template <typename T, typename Leave>
 __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t first, int64_t last, int step, int64_t begin, int64_t end, float c, int lane,
                                             float& largest, Leave leave) {
-    float m = LpPart::none().m, mc = m * c;  // the same in all lanes; mc: what d counts from in the short way
+    float m = LpPart::none().m, mc = __fmul_rn(m, c);  // the same in all lanes; mc: what d counts from in the short way, rounded wherever it is used
     const bool common = c > 0.01f && c < 1e4f;
     auto is_short = [&](float m, float mc) { return common && m > LpRaw<T>::SAFE && fabsf(mc) < LP_SHORT; };
     auto in_short = [&]() { return is_short(m, mc); };
@@ -251,7 +254,7 @@ __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t fir
         if (top != top) top = -INFINITY;
         leave(chunk, top);
         if (top > m) {
-            const float to = top * c;
+            const float to = __fmul_rn(top, c);
             const bool was = in_short(), is = is_short(top, to);
             // from what the sums are relative to, mc or m c itself, to what they will be
             const float d = max_nan(was ? (is ? mc - to : -fmaf(top, c, -mc)) : is ? fmaf(m, c, -to) : (m - top) * c, LP_FLOOR), f = exp2_fast(d);
@@ -690,14 +693,15 @@ struct LpBackward {
     int64_t ldo;            // of the result, where it is a matrix
     int64_t units;          // spans of positions: of all lists, or that a matrix's row can reach into
     int span;               // positions of lists for a warp
-    int whole, shares;      // CTAs in front of the others, and how many of them have a list, see lp_backward_whole
+    int whole, shares;      // CTAs of log_probs_backward_whole_kernel, and how many of them have a row
 };
 
 // Constants of a row: ds = p (a - b log p), and more at the given entry; log p = z - lse, a = -(h entropy + g) / temperature, b = h / temperature, g by the temperature.
 struct LpRowTerms {
     float lse, a, b, g;
+    float base;  // log p = (s - base) / temperature - lse where a row is taken as a whole; else 0, and not used
     int64_t target;
-    bool bad;  // lse is NaN: so is everything but what is masked
+    bool bad;    // lse is NaN: so is everything but what is masked
 };
 
 template <typename T>
@@ -708,6 +712,7 @@ __device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, cons
     r.lse = __ldg(b.lse + row);
     if (r.lse == -INFINITY) r.lse = 0.f;  // all masked: 2^-inf is 0 then
     r.bad = r.lse != r.lse;
+    r.base = 0.f;
     r.target = target;
     if (target < 0 || score_of(x[target]) * b.f.inv_t == -INFINITY) {  // a log probability of -inf stays where it is
         r.target = -1;
@@ -718,15 +723,28 @@ __device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, cons
     r.g = g * b.f.inv_t;
     return r;
 }
-// The entry that has the gradient of a row's log probability, or -1; by a warp.  `whole`: it takes the whole row to say.
+__device__ __forceinline__ bool lp_far(const LpBackward& b, int row) {
+    const float lse = __ldg(b.lse + row);
+    return fabsf(lse) > LP_NEAR && lse != -INFINITY;
+}
+// The entry that has the gradient of a row's log probability, or -1; by a warp.  `whole`: it takes the whole row to say, or to say what p is.
 __device__ __forceinline__ int64_t lp_given(const LpBackward& b, int row, int64_t begin, int64_t end, bool& whole) {
-    whole = false;
-    if (!b.f.targets || !b.g) return -1;
-    const int64_t at = LpFind(b.f, row, begin, end)(b.f);
-    whole = at < 0 && b.f.ids && lp_may_be_left(begin, end);
+    whole = lp_far(b, row);
+    if (whole || !b.f.targets || !b.g) return -1;
+    int64_t at = LpFind(b.f, row, begin, end)(b.f);
+    if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) {
+        whole = end - begin > LP_LOOK;
+        if (!whole) {
+            at = lp_first_named<2>(b.f.ids - b.f.rows.shift, begin, end, __ldg(b.f.targets + row), threadIdx.x & 31, 32);
+            const unsigned first = __reduce_min_sync(0xFFFFFFFFu, (unsigned)(at - begin));
+            at = first < (unsigned)(end - begin) ? begin + first : -1;
+        }
+    }
     return at;
 }
+template <bool WHOLE>
 __device__ __forceinline__ float2 lp_grad(const LpRowTerms& r, float2 s, float inv_t) {
+    if constexpr (WHOLE) s = make_float2(s.x - r.base, s.y - r.base);
     float2 lp = fma2(s, make_float2(inv_t, inv_t), make_float2(-r.lse, -r.lse));
     lp = make_float2(max_nan(lp.x, LP_FLOOR), max_nan(lp.y, LP_FLOOR));  // no 0 times infinity for what is masked, or as low as that
     const float2 q = mul2(lp, make_float2(1.4426950409f, 1.4426950409f));
@@ -735,7 +753,9 @@ __device__ __forceinline__ float2 lp_grad(const LpRowTerms& r, float2 s, float i
     return v;
 }
 // At the given entry.  1 - p of one that is nearly certain is as exact as its log p: lists of one or two entries have hardly anything else.
+template <bool WHOLE>
 __device__ __forceinline__ float lp_grad_given(const LpRowTerms& r, float s, float inv_t) {
+    if constexpr (WHOLE) s -= r.base;
     const float lp = max_nan(fmaf(s, inv_t, -r.lse), LP_FLOOR), p = exp2_fast(lp * 1.4426950409f);
     return fmaf(p, fmaf(-r.b, lp, r.a + r.g), -r.g * expm1f(lp));
 }
@@ -745,7 +765,7 @@ __device__ __forceinline__ void put_grad(__nv_bfloat16* o, float v) { *o = __flo
 
 // Positions [from, to) of a row by `threads` threads, whose `thread` this is, 32 bytes of each in flight; `x` and `o`: position 0 of the scores, on a 16-byte boundary, and of the gradient.
 // ALIKE: that is on a boundary, too, in every row.
-template <bool ALIKE, typename T>
+template <bool ALIKE, bool WHOLE, typename T>
 __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __restrict__ o, const LpRowTerms& r, float inv_t, int64_t from, int64_t to, int thread,
                                                  int threads) {
     constexpr int V = 16 / sizeof(T);
@@ -757,10 +777,10 @@ __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __r
             for (int i = 0; i < 16; ++i) s[i] = p0 + (int64_t)i * threads < to ? score_of(x[p0 + (int64_t)i * threads]) : 0.f;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                const float2 d = lp_grad(r, make_float2(s[i], s[i + 1]), inv_t);
+                const float2 d = lp_grad<WHOLE>(r, make_float2(s[i], s[i + 1]), inv_t);
                 const int64_t p = p0 + (int64_t)i * threads, p1 = p + threads;
-                if (p < to) put_grad(o + p, p == r.target ? lp_grad_given(r, s[i], inv_t) : d.x);
-                if (p1 < to) put_grad(o + p1, p1 == r.target ? lp_grad_given(r, s[i + 1], inv_t) : d.y);
+                if (p < to) put_grad(o + p, p == r.target ? lp_grad_given<WHOLE>(r, s[i], inv_t) : d.x);
+                if (p1 < to) put_grad(o + p1, p1 == r.target ? lp_grad_given<WHOLE>(r, s[i + 1], inv_t) : d.y);
             }
         }
     } else {
@@ -784,14 +804,14 @@ __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __r
 #pragma unroll
                 for (int i = 0; i < V; i += 2) {
                     const T* const t = reinterpret_cast<const T*>(&w[j]) + i;
-                    const float2 d = lp_grad(r, make_float2(score_of(t[0]), score_of(t[1])), inv_t);
+                    const float2 d = lp_grad<WHOLE>(r, make_float2(score_of(t[0]), score_of(t[1])), inv_t);
                     v[i] = d.x;
                     v[i + 1] = d.y;
                 }
                 if (r.target >= p && r.target < p + V) {
 #pragma unroll
                     for (int i = 0; i < V; ++i)
-                        if (p + i == r.target) v[i] = lp_grad_given(r, score_of(reinterpret_cast<const T*>(&w[j])[i]), inv_t);
+                        if (p + i == r.target) v[i] = lp_grad_given<WHOLE>(r, score_of(reinterpret_cast<const T*>(&w[j])[i]), inv_t);
                 }
                 if (p >= from && p + V <= to) {
                     uint4 u;
@@ -816,49 +836,23 @@ template <typename T>
 constexpr int LP_ROW_SPAN = 4 * LP_THREADS * (16 / sizeof(T));
 template <bool ALIKE, typename T>
 __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_rows_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int64_t row = blockIdx.x / (unsigned)b.units, begin = b.f.rows.begin((int)row), end = b.f.rows.end((int)row);
     const int64_t span = begin / LP_ROW_SPAN<T> + (blockIdx.x - (unsigned)row * (unsigned)b.units);
     const int64_t from = max(span * LP_ROW_SPAN<T>, begin), to = min((span + 1) * LP_ROW_SPAN<T>, end);
     if (from >= to) return;
     bool whole;
-    const LpRowTerms r = lp_row_terms(x, b, (int)row, lp_given(b, (int)row, begin, end, whole));
-    lp_backward_span<ALIKE>(x, out + (row * b.ldo - begin), r, b.f.inv_t, from, to, threadIdx.x, LP_THREADS);
-}
-
-// Lists that have to be looked at as a whole before any of their gradient is known: those whose target is not where a search finds it.  Each has a CTA of the first ones, which look
-// at the others for that only; the warps with spans leave them alone.
-template <bool ALIKE, typename T>
-__device__ __forceinline__ void lp_backward_whole(const T* __restrict__ x, T* __restrict__ out, const LpBackward& b) {
-    __shared__ int64_t s_target;
-    const LpRows& rows = b.f.rows;
-    // few lists have several CTAs each, which look through all of it and take their share of what follows
-    const int share = (int)blockIdx.x % b.shares;
-    lp_by_warps_then_ctas(
-        b.f.m, (int)blockIdx.x / b.shares, b.whole / b.shares, [&](int row) { return lp_may_be_left(rows.begin(row), rows.end(row)); },
-        [&](int row) {
-            bool whole;
-            lp_given(b, row, rows.begin(row), rows.end(row), whole);
-            return whole;
-        },
-        [&](int row) {
-            const int64_t begin = rows.begin(row), end = rows.end(row);
-            if (threadIdx.x == 0) s_target = -1;
-            lp_find_in_any_order(b.f, row, begin, end, s_target, LP_THREADS);
-            const LpRowTerms r = lp_row_terms(x, b, row, s_target);
-            const int64_t each = ((end - begin) / b.shares / 16 + 1) * 16, from = begin + share * each;
-            lp_backward_span<ALIKE>(x, out - rows.shift, r, b.f.inv_t, from, min(from + each, end), threadIdx.x, LP_THREADS);
-            __syncthreads();
-        });
+    const int64_t target = lp_given(b, (int)row, begin, end, whole);
+    if (whole) return;
+    const LpRowTerms r = lp_row_terms(x, b, (int)row, target);
+    lp_backward_span<ALIKE, false>(x, out + (row * b.ldo - begin), r, b.f.inv_t, from, to, threadIdx.x, LP_THREADS);
 }
 
 // A warp for a span of all lists' positions, and for each list in it: what it has to know of a list takes longer than a short one.
 template <bool ALIKE, typename T>
 __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_lists_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
-    if (blockIdx.x < (unsigned)b.whole) {
-        lp_backward_whole<ALIKE>(x, out, b);
-        return;
-    }
-    const int64_t n = (int64_t)(blockIdx.x - (unsigned)b.whole) * LP_WARPS + (threadIdx.x >> 5);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t n = (int64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5);
     if (n >= b.units) return;
     const LpRows& rows = b.f.rows;
     const int64_t p0 = n * b.span, p1 = p0 + b.span;
@@ -871,8 +865,61 @@ __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_
         const int64_t target = lp_given(b, row, begin, end, whole);
         if (whole) continue;
         const LpRowTerms r = lp_row_terms(x, b, row, target);
-        lp_backward_span<ALIKE>(x, out - rows.shift, r, b.f.inv_t, from, to, threadIdx.x & 31, 32);
+        lp_backward_span<ALIKE, false>(x, out - rows.shift, r, b.f.inv_t, from, to, threadIdx.x & 31, 32);
     }
+}
+
+// Rows that have to be looked at as a whole before any of their gradient is known.  Lists whose target is not where a search finds it; and rows whose lse is large, so that it says p only to its
+// rounding (squared distances of bytes by a temperature of 0.05: to 10 %): their log p counts from the largest score, as in the forward pass, with sums made again.  The kernels with spans
+// leave such rows alone, so that this may run beside them: it waits for them at its end only.  (As CTAs of their launch it took registers from the spans: 1,000 x 200,003 bfloat16 186 us in
+// place of 157; behind them 1,000 lists of 200 took 24 us.)
+template <bool ALIKE, typename T>
+__global__ void __launch_bounds__(LP_THREADS) log_probs_backward_whole_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+    __shared__ int64_t s_target;
+    __shared__ LpPart s_parts[LP_WARPS];
+    const LpRows& rows = b.f.rows;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // few rows have several CTAs each, which look through all of it and take their share of what follows
+    const int share = (int)blockIdx.x % b.shares;
+    lp_by_warps_then_ctas(
+        b.f.m, (int)blockIdx.x / b.shares, b.whole / b.shares,
+        [&](int row) { return (b.f.ids && b.g && rows.end(row) - rows.begin(row) > LP_LOOK) || lp_far(b, row); },
+        [&](int row) {
+            bool whole;
+            lp_given(b, row, rows.begin(row), rows.end(row), whole);
+            return whole;
+        },
+        [&](int row) {
+            const int64_t begin = rows.begin(row), end = rows.end(row);
+            if (threadIdx.x == 0) s_target = -1;
+            __syncthreads();
+            if (b.f.targets && b.g) {
+                const int64_t at = LpFind(b.f, row, begin, end)(b.f);  // the same in all warps
+                if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) lp_find_in_any_order(b.f, row, begin, end, s_target, LP_THREADS);
+                else if (threadIdx.x == 0) s_target = at;
+            }
+            const bool far = lp_far(b, row);
+            if (far) {
+                float largest = 0.f;
+                const LpPart mine = lp_chunks(x, begin / LP_CHUNK<T> + warp, (end + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, b.f.c, lane, largest, [](int64_t, float) {});
+                if (lane == 0) s_parts[warp] = mine;
+            }
+            __syncthreads();
+            LpRowTerms r = lp_row_terms(x, b, row, s_target);
+            if (far) {
+                LpPart all = s_parts[0];
+                for (int w = 1; w < LP_WARPS; ++w) all.join(s_parts[w], b.f.c);
+                const float log_l = logf(all.l), lse = all.m * b.f.inv_t + log_l;
+                if (all.l > 0.f && (lse == r.lse || fabsf(lse - r.lse) <= 4.8e-7f * fabsf(lse))) {  // it is that of these scores, but for its rounding
+                    r.base = all.m;
+                    r.lse = log_l;
+                }
+            }
+            const int64_t each = ((end - begin) / b.shares / 16 + 1) * 16, from = begin + share * each;
+            lp_backward_span<ALIKE, true>(x, rows.offsets ? out - rows.shift : out + ((int64_t)row * b.ldo - begin), r, b.f.inv_t, from, min(from + each, end), threadIdx.x, LP_THREADS);
+            __syncthreads();
+        });
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // what comes next waits for both
 }
 
 // ------------------------------------------------------------------------------------------
@@ -900,6 +947,22 @@ inline LpPlan lp_plan(int m, int64_t cols, int64_t total, bool lists, int size, 
     return p;
 }
 
+// A launch behind a kernel that lets it begin at once (and was itself launched as usual, so that all that came before it is done): what the two do does not depend on the other but for
+// what is behind a griddepcontrol.wait.
+template <typename... P, typename... A>
+inline void launch_beside(cudaStream_t stream, void (*kern)(P...), size_t grid, int threads, A... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    CU_CHECK(launch_cast(cfg, kern, args...));
+}
+
 template <typename T>
 inline void log_probs(const CtxPtr& c, const T* scores, LpArgs a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
@@ -913,22 +976,15 @@ inline void log_probs(const CtxPtr& c, const T* scores, LpArgs a, void* workspac
         int th = mean <= 1024 || (a.m >= 32 * c->sm_count && mean <= 32768) ? 32 : a.m >= 16 * c->sm_count && mean <= 16384 ? 64 : 128;
         while (th < a.k) th *= 2;
         auto kern = th == 32 ? log_probs_row_kernel<32, T> : th == 64 ? log_probs_row_kernel<64, T> : log_probs_row_kernel<128, T>;
-        cudaLaunchAttribute attr[1]{};
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)a.m);
-        cfg.blockDim = dim3((unsigned)th);
-        cfg.stream = stream;
-        cfg.attrs = attr;
         a.placed = a.ids && a.targets && mean > 1024;
         if (a.placed) {
-            // Set up and begun while that runs: all that the pass reads had been written before that began.  It waits where it needs the places.
             log_probs_places_kernel<<<(unsigned)std::min((a.m - 1) / LP_WARPS + 1, 8 * c->sm_count), LP_THREADS, 0, stream>>>(a);
             KERNEL_CHECK();
-            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-            attr[0].val.programmaticStreamSerializationAllowed = 1;
-            cfg.numAttrs = 1;
+            launch_beside(stream, kern, (size_t)a.m, th, x, a);
+            return;
         }
-        CU_CHECK(launch_cast(cfg, kern, x, a));
+        kern<<<(unsigned)a.m, th, 0, stream>>>(x, a);
+        KERNEL_CHECK();
         return;
     }
     if (workspace_bytes < p.bytes() || !workspace || ((uintptr_t)workspace & 15)) fail(CULSH_ERR_INVALID, "the workspace has to be %zu bytes, aligned to 16", p.bytes());
@@ -951,17 +1007,18 @@ inline void log_probs_backward(const CtxPtr& c, const T* scores, T* out, LpBackw
     const int64_t mean = r.total / b.f.m;
     b.span = mean >= 1024 ? 512 : mean >= 64 ? 128 : 32;
     b.units = r.offsets ? (int64_t)ceil_div((size_t)(r.total + r.shift), (size_t)b.span) : r.cols / LP_ROW_SPAN<T> + 2;
-    b.whole = r.offsets && b.f.ids && b.f.targets && b.g ? 2 * c->sm_count : 0;
+    b.whole = 2 * c->sm_count;
     b.shares = 1;
     while (b.shares < 16 && 2 * b.shares * ((b.f.m - 1) / LP_WARPS + 1) <= b.whole) b.shares *= 2;
     b.whole = std::min((b.f.m - 1) / LP_WARPS + 1, b.whole / b.shares) * b.shares;
-    const size_t grid = r.offsets ? b.whole + ceil_div((size_t)b.units, LP_WARPS) : (size_t)b.units * b.f.m;
+    const size_t grid = r.offsets ? ceil_div((size_t)b.units, LP_WARPS) : (size_t)b.units * b.f.m;
     if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "too many entries for one call");
     const bool alike = (((uintptr_t)(out - r.shift) | (r.offsets ? 0u : (uintptr_t)((b.ldo - r.ld) * (int64_t)sizeof(T)))) & 15u) == 0;
     auto kern = r.offsets ? (alike ? log_probs_backward_lists_kernel<true, T> : log_probs_backward_lists_kernel<false, T>)
                           : (alike ? log_probs_backward_rows_kernel<true, T> : log_probs_backward_rows_kernel<false, T>);
     kern<<<(unsigned)grid, LP_THREADS, 0, stream>>>(scores - r.shift, out, b);
     KERNEL_CHECK();
+    launch_beside(stream, alike ? log_probs_backward_whole_kernel<true, T> : log_probs_backward_whole_kernel<false, T>, (size_t)b.whole, LP_THREADS, scores - r.shift, out, b);
 }
 
 }  // namespace culsh_b200

@@ -131,3 +131,58 @@ def test_rank_finds_targets_among_candidates_in_any_order(culsh):
     assert bool(torch.isfinite(b.log_probs).all())
     assert torch.allclose(a.log_probs, b.log_probs, rtol=0, atol=1e-4)  # float32 scores of other lanes and sums
     assert torch.equal(a.top_ids, b.top_ids)
+
+
+# ---- gradients of scores of any size --------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1.0, 0.05])
+@pytest.mark.parametrize("m,n,pad", [(7, 1, 0), (6, 20, 1), (9, 1000, 0), (5, 1003, 5), (3, 70_001, 0), (2000, 130, 0), (1, 300_000, 3)])
+@pytest.mark.parametrize("lists", [False, True])
+def test_gradient_of_large_scores(culsh, lists, m, n, pad, temperature, dtype):
+    """Scores around squared distances of bytes: p comes from the scores' differences, whatever their size, and a row's gradient sums to nothing."""
+    g = gen(m + n)
+    near = {torch.float32: -2.0e5, torch.float16: -6.0e4, torch.bfloat16: -2.0e5}[dtype]
+    if dtype == torch.float32:
+        s = near + 3 * temperature * torch.randn(m, n + pad, generator=g, device="cuda")
+    else:  # whole steps of the type; most of p lies at the largest few
+        s = near - abs(near) * float(torch.finfo(dtype).eps) * torch.randint(0, 3, (m, n + pad), generator=g, device="cuda")
+    s[::3] -= near  # rows of ordinary size among them
+    if n > 4:
+        s[:, 2] = -math.inf
+    s = s.to(dtype)[:, pad // 2:pad // 2 + n]
+    t = torch.randint(0, n, (m,), generator=g, device="cuda")
+    if m > 4:
+        t[4] = -1
+    gl, ge = torch.randn(m, generator=g, device="cuda"), torch.randn(m, generator=g, device="cuda")
+    if lists:
+        lengths = torch.full((m,), n, device="cuda")
+        offsets = torch.zeros(m + 1, dtype=torch.int64, device="cuda")
+        offsets[1:] = torch.cumsum(lengths, 0)
+        ids = (2 * torch.arange(n, device="cuda", dtype=torch.int32)).repeat(m)
+        flat = torch.cat([s.new_zeros(pad), s.reshape(-1)])[pad:]
+        r = culsh.log_probs(flat, 2 * t, (ids, offsets), temperature=temperature)
+        got = culsh.log_probs_backward(flat, 2 * t, r.lse, r.entropy, gl, ge, (ids, offsets), temperature).view(m, n)
+    else:
+        r = culsh.log_probs(s, t, temperature=temperature)
+        got = culsh.log_probs_backward(s, t, r.lse, r.entropy, gl, ge, temperature=temperature)
+    for i in sorted(set(range(min(m, 12))) | {m - 1}):
+        z = s[i].double().cpu().numpy()
+        place = int(t[i]) if 0 <= int(t[i]) < n and z[int(t[i])] > -math.inf else None
+        want = gradient_of((z - z.max(initial=-1e30)) / temperature if np.any(z > -math.inf) else z, place, float(gl[i]), float(ge[i]), temperature)
+        a, h = abs(float(gl[i])), abs(float(ge[i]))
+        mine = got[i].double().cpu().numpy()
+        bound = 8 * ULP * 64 * (a + 64 * h) / temperature  # log p errs by no more than some units of 64, whatever the scores; entropy and log p below 64
+        assert np.all(np.abs(mine - want) <= bound + HALF_ULP[dtype] * np.abs(want) + (2.0 ** -25 if dtype == torch.float16 else 0.0)), i
+        if dtype == torch.float32:
+            assert abs(mine.sum()) * temperature <= ULP * (64 + 4 * math.log(n + 1)) * 8 * (a + 64 * h), i
+
+
+def test_gradient_takes_the_lse_that_it_is_given(culsh):
+    """An lse that is not these scores' own, of rows that other processes hold parts of: p is what it says."""
+    s = 100 + torch.randn(4, 500, generator=gen(), device="cuda")
+    t, gl = torch.arange(4, device="cuda"), torch.ones(4, device="cuda")
+    lse = torch.logsumexp(s, 1) + 1.0
+    got = culsh.log_probs_backward(s, t, lse, torch.zeros(4, device="cuda"), gl)
+    want = -torch.exp(s.double() - lse.double()[:, None])
+    want[torch.arange(4), t] += 1
+    assert bool(((got.double() - want).abs() <= 8 * ULP * 128).all())
