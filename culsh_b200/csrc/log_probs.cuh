@@ -696,9 +696,9 @@ struct LpBackward {
     int whole, shares;      // CTAs of log_probs_backward_whole_kernel, and how many of them have a row
 };
 
-// Constants of a row: ds = p (a - b log p), and more at the given entry; log p = z - lse, a = -(h entropy + g) / temperature, b = h / temperature, g by the temperature.
+// Constants of a row: ds = p (a - b log p), and more at the given entry; log p = z - lse, a = own - g, own = -h entropy / temperature, b = h / temperature, g by the temperature.
 struct LpRowTerms {
-    float lse, a, b, g;
+    float lse, a, b, g, own;
     float base;  // log p = (s - base) / temperature - lse where a row is taken as a whole; else 0, and not used
     int64_t target;
     bool bad;    // lse is NaN: so is everything but what is masked
@@ -718,9 +718,10 @@ __device__ __forceinline__ LpRowTerms lp_row_terms(const T* __restrict__ x, cons
         r.target = -1;
         g = 0.f;
     }
-    r.a = -(h * entropy + g) * b.f.inv_t;
+    r.own = -(h * entropy) * b.f.inv_t;
     r.b = h * b.f.inv_t;
     r.g = g * b.f.inv_t;
+    r.a = r.own - r.g;
     return r;
 }
 __device__ __forceinline__ bool lp_far(const LpBackward& b, int row) {
@@ -752,12 +753,12 @@ __device__ __forceinline__ float2 lp_grad(const LpRowTerms& r, float2 s, float i
     if (r.bad) v = make_float2(s.x == -INFINITY ? 0.f : v.x, s.y == -INFINITY ? 0.f : v.y);
     return v;
 }
-// At the given entry.  1 - p of one that is nearly certain is as exact as its log p: lists of one or two entries have hardly anything else.
+// At the given entry.  1 - p of one that is nearly certain is as exact as its log p: lists of one or two entries have hardly anything else; nor may a large g take the entropy's part with it.
 template <bool WHOLE>
 __device__ __forceinline__ float lp_grad_given(const LpRowTerms& r, float s, float inv_t) {
     if constexpr (WHOLE) s -= r.base;
     const float lp = max_nan(fmaf(s, inv_t, -r.lse), LP_FLOOR), p = exp2_fast(lp * 1.4426950409f);
-    return fmaf(p, fmaf(-r.b, lp, r.a + r.g), -r.g * expm1f(lp));
+    return fmaf(p, fmaf(-r.b, lp, r.own), -r.g * expm1f(lp));
 }
 __device__ __forceinline__ void put_grad(float* o, float v) { *o = v; }
 __device__ __forceinline__ void put_grad(__half* o, float v) { *o = __float2half_rn(v); }

@@ -186,3 +186,26 @@ def test_gradient_takes_the_lse_that_it_is_given(culsh):
     want = -torch.exp(s.double() - lse.double()[:, None])
     want[torch.arange(4), t] += 1
     assert bool(((got.double() - want).abs() <= 8 * ULP * 128).all())
+
+
+@pytest.mark.parametrize("lists", [False, True])
+@pytest.mark.parametrize("g,h", [(1e4, 1.0), (-3e5, 2.0), (1e-3, 1.0), (1e6, 0.5)])
+def test_gradient_of_an_entry_that_is_nearly_certain(culsh, g, h, lists):
+    """What the entropy's gradient adds there is small beside what goes into it and stays, however large the other gradient is."""
+    n = 60
+    s = torch.full((3, n), -14.0, device="cuda")
+    s[:, 7] = 0.0
+    s[1, 8:] = -20.0
+    s[2, 8] = -3.0
+    t = torch.full((3,), 7, device="cuda")
+    gl, ge = torch.full((3,), g, device="cuda"), torch.full((3,), h, device="cuda")
+    csr_of = (torch.arange(n, device="cuda", dtype=torch.int32).repeat(3), torch.arange(4, device="cuda") * n) if lists else None
+    scores = s.reshape(-1) if lists else s
+    r = culsh.log_probs(scores, t, csr_of)
+    got = culsh.log_probs_backward(scores, t, r.lse, r.entropy, gl, ge, csr_of).view(3, n)
+    for i in range(3):
+        z, lse, entropy = s[i].double().cpu().numpy(), float(r.lse[i]), float(r.entropy[i])  # of what the call is given
+        lp = z[7] - lse
+        first, second = -g * math.expm1(lp), -h * math.exp(lp) * (lp + entropy)
+        # each part to some units of what goes into it
+        assert abs(float(got[i, 7]) - (first + second)) <= 4 * ULP * abs(first) + 8 * ULP * h * (abs(lp) + entropy), (i, float(got[i, 7]), first, second)
