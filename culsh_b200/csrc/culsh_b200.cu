@@ -1246,6 +1246,7 @@ int culsh_create(int device, culsh_handle** out) {
         for (auto& e : c->ev_pass) CU_CHECK(cudaEventCreate(&e));
         for (auto& e : c->ev_dedupe) CU_CHECK(cudaEventCreate(&e));
         CU_CHECK(cudaEventCreateWithFlags(&c->counted, cudaEventDisableTiming));
+        CU_CHECK(cudaEventCreateWithFlags(&c->read_by, cudaEventDisableTiming));
         for (auto& e : c->copy_done) CU_CHECK(cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
         for (auto& e : c->chunk_free) CU_CHECK(cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
         CU_CHECK(cudaMallocHost(&c->pinned, 64 * sizeof(uint64_t)));

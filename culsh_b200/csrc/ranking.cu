@@ -178,8 +178,12 @@ int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* str
     return guarded([&] {
         need(h && c, "null argument");
         DeviceGuard g(c->ctx->device);
-        CU_CHECK(cudaEventRecord(c->ctx->counted, stream_of(stream)));
-        CU_CHECK(cudaStreamWaitEvent(c->ctx->stream, c->ctx->counted, 0));
+        cudaStreamCaptureStatus capture;
+        CU_CHECK(cudaStreamIsCapturing(stream_of(stream), &capture));
+        if (capture != cudaStreamCaptureStatusNone) return;  // a wait would make the engine's stream part of the graph
+        std::lock_guard<std::mutex> lock(c->ctx->read_by_lock);
+        CU_CHECK(cudaEventRecord(c->ctx->read_by, stream_of(stream)));
+        CU_CHECK(cudaStreamWaitEvent(c->ctx->stream, c->ctx->read_by, 0));
     });
 }
 

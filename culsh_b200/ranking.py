@@ -11,7 +11,7 @@ probabilities, and the entropy of the distribution; ``log_probs_backward`` is it
     best.top_ids, best.top_log_probs, best.entropy
 
 Results are torch tensors on the device of the rows.  Unlike the index's calls these run on torch's current stream and
-return when their work is queued.
+return when their work is queued.  In a graph, keep the Candidates that it reads.
 """
 from __future__ import annotations
 
@@ -118,7 +118,8 @@ class _Lists:
             self.ids = self.offsets  # no list has an entry: nothing is read through it
 
     def done(self, handle, stream):
-        """The device arrays of a Candidates object may go as soon as it does: its handle waits for what has been queued."""
+        """The device arrays of a Candidates object may go as soon as it does: its handle waits for what has been queued (not for a graph that is being
+        captured, whose candidates have to stay as long as it does)."""
         if self.result is not None:
             _lib.check(handle.lib.culsh_candidates_after(handle.ptr, self.result._ptr, stream))
             if getattr(self.result, "_keepalive", None) is not None:  # a receive buffer that other processes write

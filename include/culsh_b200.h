@@ -349,7 +349,8 @@ int culsh_mx_score(culsh_handle* h, const void* Q, int type, int n_queries, int6
                    const uint8_t* scales, const float* norms, int n, int d, int metric, const int32_t* ids,
                    const int64_t* offsets, int64_t total, float* out, void* workspace, uint64_t workspace_bytes, void* stream);
 /* What the result's handle does from now on waits for what the stream holds so far: call it behind work
- * that reads a result's device arrays (culsh_candidates_device_ptrs), which may then be freed at once. */
+ * that reads a result's device arrays (culsh_candidates_device_ptrs), which may then be freed at once.  Any thread may
+ * call it.  It does nothing while the stream is being captured: a result that a graph reads has to stay as long as the graph. */
 int culsh_candidates_after(culsh_handle* h, const culsh_candidates* c, void* stream);
 
 /* Rows of scores (float32, float16, bfloat16): a matrix [m][cols] with rows ld apart (offsets and ids

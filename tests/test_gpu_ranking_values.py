@@ -209,3 +209,35 @@ def test_gradient_of_an_entry_that_is_nearly_certain(culsh, g, h, lists):
         first, second = -g * math.expm1(lp), -h * math.exp(lp) * (lp + entropy)
         # each part to some units of what goes into it
         assert abs(float(got[i, 7]) - (first + second)) <= 4 * ULP * abs(first) + 8 * ULP * h * (abs(lp) + entropy), (i, float(got[i, 7]), first, second)
+
+
+# ---- graphs, results that go ----------------------------------------------------------------------------------------
+def test_candidates_in_a_graph(culsh):
+    """The engine's stream stays out of the graph, and works on meanwhile and behind it."""
+    rng = np.random.RandomState(3)
+    X = rng.randn(4000, 32).astype(np.float32)
+    near = X[:100] + 0.05 * rng.randn(100, 32).astype(np.float32)
+    model = culsh.RPLSH(8, 8, seed=0).fit(X)
+    cand = model.query(near)
+    rows, Q = culsh.MXRows(X), torch.from_numpy(near).cuda()
+    t = torch.arange(100, device="cuda")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        culsh.rank(rows, Q, cand, top_k=5, metric="cosine", targets=t)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r = culsh.rank(rows, Q, cand, top_k=5, metric="cosine", targets=t)
+        s = rows.score(Q, cand)
+        grad = culsh.log_probs_backward(s, t, r.lse, r.entropy, torch.ones(100, device="cuda"), lists=cand)
+    again = model.query(near)
+    assert np.array_equal(again.get_indices(), cand.get_indices())
+    for seed in (1, 2):
+        Q.copy_(torch.randn(100, 32, generator=gen(seed), device="cuda"))
+        graph.replay()
+        want = culsh.rank(rows, Q, cand, top_k=5, metric="cosine", targets=t)
+        assert torch.equal(r.top_ids, want.top_ids) and torch.equal(r.lse, want.lse) and torch.equal(r.log_probs, want.log_probs)
+        one = rows.score(Q, cand)
+        assert torch.equal(s, one)
+        assert torch.equal(grad, culsh.log_probs_backward(one, t, want.lse, want.entropy, torch.ones(100, device="cuda"), lists=cand))
+
