@@ -241,3 +241,41 @@ def test_candidates_in_a_graph(culsh):
         assert torch.equal(s, one)
         assert torch.equal(grad, culsh.log_probs_backward(one, t, want.lse, want.entropy, torch.ones(100, device="cuda"), lists=cand))
 
+
+@pytest.mark.parametrize("what", ["score", "log_probs", "backward", "rank"])
+def test_results_that_go_before_they_are_read(culsh, what):
+    """Work that reads a result waits behind long work of its stream when the result goes and queries of the same size take its memory."""
+    rng = np.random.RandomState(5)
+    X = rng.randn(20_000, 64).astype(np.float32)
+    Q = X[:3000] + 0.1 * rng.randn(3000, 64).astype(np.float32)
+    other = Q[::-1].copy()
+    model = culsh.RPLSH(8, 10, seed=0).fit(X)
+    rows, Qd = culsh.MXRows(X), torch.from_numpy(Q).cuda()
+    kept = model.query(Q)
+    t = torch.arange(3000, device="cuda")
+    scores = rows.score(Qd, kept, metric="cosine")
+    r = culsh.log_probs(scores, t, kept, temperature=0.1)
+    ones = torch.ones(3000, device="cuda")
+    calls = {"score": lambda c: (rows.score(Qd, c, metric="cosine"),),
+             "log_probs": lambda c: culsh.log_probs(scores, t, c, top_k=4, temperature=0.1),
+             "backward": lambda c: (culsh.log_probs_backward(scores, t, r.lse, r.entropy, ones, ones, c, 0.1),),
+             "rank": lambda c: culsh.rank(rows, Qd, c, top_k=4, metric="cosine", targets=t)}
+    want = [x.clone() for x in calls[what](kept)]
+    big = torch.randn(8000, 8000, device="cuda")
+    torch.cuda.synchronize()
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    for _ in range(3):
+        cand = model.query(Q)
+        with torch.cuda.stream(side):
+            x = big
+            for _ in range(8):
+                x = x @ big * 1e-2  # some milliseconds each in float32
+            got = calls[what](cand)
+            done.record(side)
+        pending = not done.query()
+        del cand
+        again = [model.query(other) for _ in range(2)]
+        side.synchronize()
+        assert pending, "the work in front was done too soon to show anything"
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del again
