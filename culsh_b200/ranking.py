@@ -84,7 +84,7 @@ class _Lists:
     """Candidate lists as device addresses: a Candidates object, or a pair (ids, offsets)."""
 
     def __init__(self, lists, device, need_ids=True):
-        self.result = None
+        self.result, self.device = None, device
         if isinstance(lists, Candidates):
             if lists._h.device != device.index:
                 raise ValueError(f"candidates are on cuda:{lists._h.device}, not on {device}")
@@ -123,7 +123,7 @@ class _Lists:
         if self.result is not None:
             _lib.check(handle.lib.culsh_candidates_after(handle.ptr, self.result._ptr, stream))
             if getattr(self.result, "_keepalive", None) is not None:  # a receive buffer that other processes write
-                torch.cuda.current_stream().synchronize()
+                torch.cuda.current_stream(self.device).synchronize()
 
 
 class MXRows:

@@ -19,3 +19,40 @@ def test_results_are_waited_for_by_an_event_of_their_own():
     assert body.index("cudaStreamIsCapturing") < lock < record < wait
     others = [f for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")) and f != "ranking.cu" and re.search(r"(Record|Wait\w*|Synchronize)\([^;]*\bread_by\b", source(f))]
     assert not others
+
+
+def test_a_receive_buffer_is_waited_for_on_the_device_that_reads_it(monkeypatch):
+    """Results of an exchange lie in a buffer that other processes write next: the stream that read it is waited for, whatever device is current."""
+    import torch
+
+    from culsh_b200 import ranking
+    waited = []
+
+    class Stream:
+        def __init__(self, device):
+            self.device = device
+
+        def synchronize(self):
+            waited.append(self.device)
+
+    class Result:
+        _ptr, _keepalive, n_queries, n_total_candidates = 1, object(), 3, 7
+        _h = type("Handle", (), {"device": 1})
+
+        def empty(self):
+            return False
+
+        def device_pointers(self):
+            return 16, 16, 16
+
+    after = []
+    lib = type("Lib", (), {"culsh_candidates_after": lambda self, *a: after.append(a) or 0})()
+    handle = type("Handle", (), {"lib": lib, "ptr": 5})()
+    monkeypatch.setattr(ranking, "Candidates", Result)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(device))
+    lists = ranking._Lists(Result(), torch.device("cuda", 1))
+    lists.done(handle, 77)
+    assert after == [(5, 1, 77)] and waited == [torch.device("cuda", 1)]
+    Result._keepalive = None
+    lists.done(handle, 77)
+    assert len(after) == 2 and len(waited) == 1
