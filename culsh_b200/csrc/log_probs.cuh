@@ -43,10 +43,10 @@ struct LpRows {
     const int64_t* offsets;
     int64_t ld, cols, shift, total;  // shift: entries between the boundary and the array; total: entries of all lists
     __device__ __forceinline__ int64_t begin(int r) const {
-        return (offsets ? min(max(__ldg(offsets + r), (int64_t)0), total) : (int64_t)r * ld) + shift;
+        return (offsets ? min(max(__ldcg(offsets + r), (int64_t)0), total) : (int64_t)r * ld) + shift;
     }
     __device__ __forceinline__ int64_t end(int r) const {
-        return offsets ? max(min(__ldg(offsets + r + 1), total) + shift, begin(r)) : (int64_t)r * ld + cols + shift;
+        return offsets ? max(min(__ldcg(offsets + r + 1), total) + shift, begin(r)) : (int64_t)r * ld + cols + shift;
     }
 };
 
@@ -215,8 +215,9 @@ __device__ __forceinline__ int lp_place(int lane, int i) {
     constexpr int V = 16 / sizeof(T);
     return ((i / V) * 32 + lane) * V + i % V;
 }
-// The lane's scores of a chunk, -inf outside [begin, end), by L2 (see EightOf).  `x`: position 0.
-template <typename T>
+// The lane's scores of a chunk, -inf outside [begin, end).  EARLY: in a kernel that is launched early, all of them by L2 (see EightOf; single ones by L1 leave the others eight
+// registers: 1,000 x 1M bfloat16 396 us, 440 by L2).  `x`: position 0.
+template <bool EARLY, typename T>
 __device__ __forceinline__ void lp_load(const T* __restrict__ x, int64_t chunk, int64_t begin, int64_t end, int lane, LpRaw<T>& s) {
     constexpr int V = 16 / sizeof(T);
     const int64_t p0 = chunk * LP_CHUNK<T>;
@@ -227,14 +228,14 @@ __device__ __forceinline__ void lp_load(const T* __restrict__ x, int64_t chunk, 
 #pragma unroll
         for (int i = 0; i < LP_PER_LANE<T>; ++i) {
             const int64_t p = p0 + lp_place<T>(lane, i);
-            s.set(i, p >= begin && p < end ? score_of(x[p]) : -INFINITY);
+            s.set(i, p >= begin && p < end ? score_of(EARLY ? __ldcg(x + p) : x[p]) : -INFINITY);
         }
     }
 }
 
 // A warp's chunks first, first + step, ... below last, all in one row; `leave(chunk, top)` takes the chunks' maxima, `largest` becomes the
 // lane's.  The next chunk is on its way while one is summed.
-template <typename T, typename Leave>
+template <bool EARLY, typename T, typename Leave>
 __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t first, int64_t last, int step, int64_t begin, int64_t end, float c, int lane,
                                             float& largest, Leave leave) {
     float m = LpPart::none().m, mc = __fmul_rn(m, c);  // the same in all lanes; mc: what d counts from in the short way, rounded wherever it is used
@@ -243,11 +244,11 @@ __device__ __forceinline__ LpPart lp_chunks(const T* __restrict__ x, int64_t fir
     auto in_short = [&]() { return is_short(m, mc); };
     float2 l = make_float2(0.f, 0.f), e = l;
     LpRaw<T> next;
-    if (first < last) lp_load(x, first, begin, end, lane, next);
+    if (first < last) lp_load<EARLY>(x, first, begin, end, lane, next);
 #pragma unroll 1
     for (int64_t chunk = first; chunk < last; chunk += step) {
         const LpRaw<T> s = next;
-        if (chunk + step < last) lp_load(x, chunk + step, begin, end, lane, next);
+        if (chunk + step < last) lp_load<EARLY>(x, chunk + step, begin, end, lane, next);
         float top = s.top();
         largest = fmaxf(largest, top);
         top = warp_max(top);
@@ -395,9 +396,9 @@ struct LpFind {
     __device__ __forceinline__ void probe(const int32_t* __restrict__ ids) {
         step = (hi - lo + 31) / 32;
         const int64_t p = lo + (threadIdx.x & 31) * step;
-        id = p < hi ? __ldg(ids + p) : 0x7FFFFFFF;
+        id = p < hi ? __ldcg(ids + p) : 0x7FFFFFFF;
     }
-    __device__ __forceinline__ LpFind(const LpArgs& a, int row, int64_t begin, int64_t end) : lo(begin), hi(end), step(1), target(__ldg(a.targets + row)), id(0) {
+    __device__ __forceinline__ LpFind(const LpArgs& a, int row, int64_t begin, int64_t end) : lo(begin), hi(end), step(1), target(__ldcg(a.targets + row)), id(0) {
         if (a.ids && hi > lo) probe(a.ids - a.rows.shift);
     }
     __device__ __forceinline__ int64_t operator()(const LpArgs& a) {
@@ -447,7 +448,7 @@ __device__ __forceinline__ int64_t lp_first_named(const int32_t* __restrict__ na
 // By a CTA whose threads have seen that `found`, in shared memory, is -1: the first entry of the row, if there is one.
 template <int N = 4>
 __device__ __forceinline__ void lp_find_in_any_order(const LpArgs& a, int row, int64_t begin, int64_t end, int64_t& found, int threads) {
-    const int64_t first = lp_first_named<N>(a.ids - a.rows.shift, begin, end, __ldg(a.targets + row), threadIdx.x, threads);
+    const int64_t first = lp_first_named<N>(a.ids - a.rows.shift, begin, end, __ldcg(a.targets + row), threadIdx.x, threads);
     __syncthreads();
     if (first < end) atomicMin(reinterpret_cast<unsigned long long*>(&found), (unsigned long long)first);
     __syncthreads();
@@ -473,11 +474,11 @@ __device__ __forceinline__ void lp_by_warps_then_ctas(int m, int cta, int ctas, 
     }
 }
 
-// What a row's result is made of, by the whole CTA.  `maxima`: orders of the largest scores of groups of 1 << wide chunks from first_chunk on; `largest`: a thread's own score, of no
+// What a row's result is made of, by the whole CTA.  `maximum`: orders of the largest scores of groups of 1 << wide chunks from first_chunk on; `largest`: a thread's own score, of no
 // other's entry.
-template <int TH, typename T>
+template <int TH, bool EARLY, typename T, typename Maximum>
 __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs& a, LpShared<TH>& sh, int row, int64_t begin, int64_t end, LpPart all,
-                                          const uint32_t* maxima, int64_t first_chunk, int64_t last_chunk, int wide, float largest) {
+                                          Maximum maximum, int64_t first_chunk, int64_t last_chunk, int wide, float largest) {
     if (a.targets && a.ids) {
         if (a.placed) {
             asm volatile("griddepcontrol.wait;" ::: "memory");  // for log_probs_places_kernel
@@ -501,7 +502,7 @@ __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs&
     if (threadIdx.x == 0) {
         a.lse[row] = lse;
         a.entropy[row] = entropy;
-        if (a.targets) a.log_probs[row] = sh.target < 0 ? -INFINITY : log_p(score_of(x[sh.target]));
+        if (a.targets) a.log_probs[row] = sh.target < 0 ? -INFINITY : log_p(score_of(__ldcg(x + sh.target)));
     }
     if (!a.k) return;
     const float bound = lp_bound(sh, largest, a.k);
@@ -511,11 +512,11 @@ __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs&
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int64_t c0 = first_chunk + warp * 32; c0 < last_chunk; c0 += TH) {  // a lane looks at a chunk's maximum
         const int64_t mine = c0 + lane;
-        unsigned reach = __ballot_sync(0xFFFFFFFFu, mine < last_chunk && maxima[(mine - first_chunk) >> wide] >= least);
+        unsigned reach = __ballot_sync(0xFFFFFFFFu, mine < last_chunk && maximum((mine - first_chunk) >> wide) >= least);
         for (; reach; reach &= reach - 1) {
             const int64_t chunk = c0 + __ffs((int)reach) - 1;
             LpRaw<T> s;
-            lp_load(x, chunk, begin, end, lane, s);
+            lp_load<EARLY>(x, chunk, begin, end, lane, s);
             if (!(s.top() >= bound)) continue;
 #pragma unroll
             for (int j = 0; j < LP_PER_LANE<T>; ++j) {
@@ -532,7 +533,7 @@ __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs&
         lp_settle(sh, a.k);
     } else {  // many that are alike
         lp_largest(sh, end - begin, a.k, (uint64_t)least << 32, [&](int64_t i) {
-            const float v = score_of(x[begin + i]);
+            const float v = score_of(__ldcg(x + begin + i));
             return v > -INFINITY ? (unsigned long long)lp_order(v) << 32 | (0xFFFFFFFFu - (uint32_t)i) : 0ull;
         });
     }
@@ -544,7 +545,7 @@ __device__ __forceinline__ void lp_finish(const T* __restrict__ x, const LpArgs&
             const float s = lp_score((uint32_t)(sh.keys[i] >> 32));
             if (s * a.inv_t > -INFINITY) {
                 lp = log_p(s);
-                id = a.ids ? __ldg(a.ids - a.rows.shift + begin + at) : (int32_t)at;
+                id = a.ids ? __ldcg(a.ids - a.rows.shift + begin + at) : (int32_t)at;
             }
         }
         a.top_log_probs[(int64_t)row * a.k + i] = lp;
@@ -596,14 +597,14 @@ __global__ void __launch_bounds__(TH) log_probs_row_kernel(const T* __restrict__
     float largest = -INFINITY;
     if (warp == TH / 32 - 1 && a.targets && !a.placed) {  // the warp with the fewest chunks
         LpFind find(a, row, begin, end);
-        mine = lp_chunks(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
+        mine = lp_chunks<false>(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
         const int64_t at = find(a);
         if (lane == 0) sh.target = at;
     } else {
-        mine = lp_chunks(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
+        mine = lp_chunks<false>(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
     }
     const LpPart all = lp_join_warps(sh, mine, a.c);
-    lp_finish(x, a, sh, row, begin, end, all, sh.maxima, first, last, wide, largest);
+    lp_finish<TH, false>(x, a, sh, row, begin, end, all, [&](int64_t i) { return sh.maxima[i]; }, first, last, wide, largest);
 }
 
 // Rows taken by several CTAs.  Slots of a row's units and chunks: blocks of `size` positions from the one that it begins in on; lists share the numbering of all
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __r
     if (from >= to) return;
     const int64_t slot = lp_slot(a, row, begin, LP_CHUNK<T>, lp_chunks_per_row<T>(a)), first = begin / LP_CHUNK<T>;
     float largest = -INFINITY;
-    const LpPart mine = lp_chunks(x, from / LP_CHUNK<T> + warp, (to + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, a.c, lane, largest, [&](int64_t chunk, float top) {
+    const LpPart mine = lp_chunks<true>(x, from / LP_CHUNK<T> + warp, (to + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, a.c, lane, largest, [&](int64_t chunk, float top) {
         if (a.k && lane == 0) a.maxima[slot + chunk - first] = lp_order(top);
     });
     const LpPart all = lp_join_warps(sh, mine, a.c);
@@ -659,7 +660,7 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __r
     const int64_t units = end > begin ? (end - 1) / a.unit - begin / a.unit + 1 : 0, slot = lp_slot(a, row, begin, a.unit, a.units_per_row);
     LpPart mine = LpPart::none();
     for (int64_t u = threadIdx.x; u < units; u += LP_THREADS) {
-        const float4 p = a.parts[slot + u];
+        const float4 p = __ldcg(a.parts + slot + u);
         mine.join(LpPart{p.x, p.y, p.z}, a.c);
     }
 #pragma unroll
@@ -667,17 +668,18 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __r
     const LpPart all = lp_join_warps(sh, mine, a.c);
     const int64_t first = begin / LP_CHUNK<T>, last = end > begin ? (end + LP_CHUNK<T> - 1) / LP_CHUNK<T> : first;
     const uint32_t* const maxima = a.maxima + lp_slot(a, row, begin, LP_CHUNK<T>, lp_chunks_per_row<T>(a));
+    auto maximum = [&](int64_t i) { return __ldcg(maxima + i); };
     float largest = -INFINITY;
     if (a.k && last - first >= LP_THREADS) {  // of every 256th chunk
-        for (int64_t c = threadIdx.x; c < last - first; c += LP_THREADS) largest = fmaxf(largest, lp_score(max(maxima[c], 0x007FFFFFu)));
+        for (int64_t c = threadIdx.x; c < last - first; c += LP_THREADS) largest = fmaxf(largest, lp_score(max(maximum(c), 0x007FFFFFu)));
     } else if (a.k) {  // too few: of every eighth chunk's entries of a lane
         for (int64_t c = first + warp; c < last; c += LP_WARPS) {
             LpRaw<T> s;
-            lp_load(x, c, begin, end, lane, s);
+            lp_load<true>(x, c, begin, end, lane, s);
             largest = fmaxf(largest, s.top());
         }
     }
-    lp_finish(x, a, sh, row, begin, end, all, maxima, first, last, 0, largest);
+    lp_finish<LP_THREADS, true>(x, a, sh, row, begin, end, all, maximum, first, last, 0, largest);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -902,7 +904,7 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_backward_whole_kernel(co
             const bool far = lp_far(b, row);
             if (far) {
                 float largest = 0.f;
-                const LpPart mine = lp_chunks(x, begin / LP_CHUNK<T> + warp, (end + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, b.f.c, lane, largest, [](int64_t, float) {});
+                const LpPart mine = lp_chunks<false>(x, begin / LP_CHUNK<T> + warp, (end + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, b.f.c, lane, largest, [](int64_t, float) {});
                 if (lane == 0) s_parts[warp] = mine;
             }
             __syncthreads();

@@ -54,8 +54,8 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&y)[8]) {
     return w;
 }
 
-// Eight values of a row from column c on, zeros behind its end.  VEC: 16-byte loads where all eight are there.  They go by L2, as everything does that a kernel in front may have
-// written while one that is launched early was waiting.
+// Eight values of a row from column c on, zeros behind its end.  VEC: 16-byte loads where all eight are there.  They go by L2, as everything does that a kernel that is
+// launched early reads of what one in front may have written: a line of L1 can be from before its wait.
 template <typename T, bool VEC>
 struct EightOf {
     alignas(16) T v[8];
@@ -66,7 +66,7 @@ struct EightOf {
                 reinterpret_cast<uint4*>(v)[i] = __ldcg(reinterpret_cast<const uint4*>(x + c) + i);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = c + i < d ? x[c + i] : T(0.f);
+            for (int i = 0; i < 8; ++i) v[i] = c + i < d ? __ldcg(x + c + i) : T(0.f);
         }
     }
 };

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(128) mx_slices_kernel(const T* __restrict__ Q,
     const T* __restrict__ q = Q + (int64_t)(first + blockIdx.x) * ldq;
     auto value = [&](int block) {
         const int c = block * MX_BLOCK + lane;
-        return c < d ? (float)q[c] : 0.f;
+        return c < d ? (float)__ldcg(q + c) : 0.f;
     };
     // exponent of a block's first slice (of a value that is not finite: no slices, and a scale that is NaN)
     auto exponent = [&](float v, bool& bad) {
@@ -269,8 +269,8 @@ __device__ __forceinline__ void copy_async4(uint32_t to, const void* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
-__global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatch b, KernelBefore before) {
-    behind_kernel_before(before);
+// Launched as usual: it reads ids, offsets and scales (4 bytes by cp.async) by L1.
+__global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatch b) {
     extern __shared__ unsigned char mxs_smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(mxs_smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* s_b = base + MXS_STAGES * MXS_A_BYTES;
@@ -549,7 +549,7 @@ inline void mx_score(const CtxPtr& c, const T* Q, const MxScoreArgs& a, void* wo
         b.lists = b.kept ? MXS_B_SLOTS / a.groups : MXS_B_SLOTS;
         launch_next(stream, mx_slices_kernel<T>, (size_t)(b.last - q), 128u, 0, Q, a.ldq, a.d, a.groups, q, slices, counts, norms);
         KERNEL_CHECK();
-        launch_next(stream, mx_score_tc_kernel, (size_t)c->sm_count, (unsigned)MXS_THREADS, (size_t)MXS_SMEM, b);
+        mx_score_tc_kernel<<<(unsigned)c->sm_count, MXS_THREADS, MXS_SMEM, stream>>>(b);
         KERNEL_CHECK();
     }
 }

@@ -279,3 +279,40 @@ def test_results_that_go_before_they_are_read(culsh, what):
         assert pending, "the work in front was done too soon to show anything"
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         del again
+
+
+@pytest.mark.parametrize("d,lead", [(77, 1), (33, 3), (130, 0)])
+def test_calls_behind_one_another_on_changing_lists(culsh, d, lead):
+    """As for whole rows: odd lengths, scores off the boundaries, ids, offsets and targets that change from call to call in the same memory, long lists."""
+    n, nq, total = 30_000, 20, 20 * 60_000
+    g = gen(d)
+    sets = []
+    for i in range(3):
+        ends = torch.sort(torch.randint(0, total, (nq - 1,), generator=g, device="cuda")).values
+        offsets = torch.cat([torch.zeros(1, dtype=torch.int64, device="cuda"), ends, torch.full((1,), total, device="cuda")])
+        ids = torch.randint(0, n, (total,), generator=g, device="cuda").int()
+        targets = ids[(offsets[:-1] + 17 * i).clamp(max=total - 1)].long()
+        sets.append((torch.randn(n, d, generator=g, device="cuda"), torch.randn(nq, d, generator=g, device="cuda"), ids, offsets, targets,
+                     torch.randn(5, 100_003 + lead, generator=g, device="cuda")))
+    X, Q, ids, offsets, targets, wide = (x.clone() for x in sets[0])
+    held = torch.zeros(n, d + 1, device="cuda")[:, 1:]  # rows off the boundaries
+
+    def step(given):
+        for to, of in zip((X, Q, ids, offsets, targets, wide), given):
+            to.copy_(of)
+        held.copy_(X)
+        rows = culsh.MXRows(held)
+        s = rows.score(Q, (ids, offsets), metric="cosine")
+        r = culsh.log_probs(s, targets, (ids, offsets), top_k=5, temperature=0.2)
+        one = culsh.log_probs(wide[:, lead:], targets[:5], top_k=6)
+        p = rows.product(Q[:, :], metric="euclidean")
+        return s, r.lse, r.entropy, r.log_probs, r.top_ids, one.lse, one.log_probs, one.top_ids, culsh.log_probs(p[:3], top_k=3).top_ids
+
+    want = []
+    for given in sets:
+        want.append([x.clone() for x in step(given)])
+        torch.cuda.synchronize()
+    got = [(i % 3, step(sets[i % 3])) for i in range(45)]
+    torch.cuda.synchronize()
+    for i, r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i]))

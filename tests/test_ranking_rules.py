@@ -56,3 +56,31 @@ def test_a_receive_buffer_is_waited_for_on_the_device_that_reads_it(monkeypatch)
     Result._keepalive = None
     lists.done(handle, 77)
     assert len(after) == 2 and len(waited) == 1
+
+
+class Functions:
+    """Bodies of the functions and structs of a source by their names."""
+
+    def __init__(self, name):
+        self.text = source(name)
+
+    def __getitem__(self, name):
+        m = re.search(r"^(?:__global__|__device__|struct|inline)[^\n]*?\b%s\b[^;{]*\{\n" % name, self.text, re.M)
+        return self.text[m.end():re.compile(r"^\}", re.M).search(self.text, m.end()).start()]
+
+
+def test_kernels_launched_early_read_by_l2():
+    """A kernel that is launched early begins while those in front still write: what it reads of theirs must not come from a line that L1 already has, nor by
+    loads that take memory for constant."""
+    rows, score, lp = (Functions(f) for f in ("mx_rows.cuh", "mx_score.cuh", "log_probs.cuh"))
+    used = [rows["EightOf"], rows["mx_quantize_kernel"], score["mx_slices_kernel"]]
+    used += [lp[n] for n in ("LpRows", "lp_load", "lp_chunks", "LpFind", "lp_first_named", "lp_find_in_any_order", "lp_finish", "log_probs_unit_kernel", "log_probs_join_kernel")]
+    assert "EARLY ? __ldcg(x + p) : x[p]" in lp["lp_load"] and "<false" not in lp["log_probs_unit_kernel"] + lp["log_probs_join_kernel"]
+    for body in used:
+        body = body.replace("EARLY ? __ldcg(x + p) : x[p]", "")
+        assert "__ldg" not in body
+        assert not re.search(r"(?<![\w.])(?:x|q|X|Q|ids|names|targets|offsets)\[(?!32\b)", body), body
+        assert not re.search(r"= a\.\w+\[", body), body
+    assert "__ldg" not in source("mx_product.cuh")
+    # the kernel that gathers scales by L1 is launched as usual
+    assert re.search(r"\bmx_score_tc_kernel<<<", score["mx_score"]) and "KernelBefore" not in source("mx_score.cuh").split("mx_score_tc_kernel(")[1].split("{")[0]
