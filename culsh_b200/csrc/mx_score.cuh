@@ -20,6 +20,9 @@ __device__ __forceinline__ int owner_of(const int64_t* __restrict__ offsets, int
     return lo;
 }
 
+// Scores whose sums pass float32 are NaN, as are those of queries that are not finite: the two kernels below add in different orders, in which infinities of both signs can meet.
+__device__ __forceinline__ float finite_or_nan(float v) { return fabsf(v) < INFINITY ? v : __int_as_float(0x7FFFFFFF); }
+
 struct MxScoreArgs {
     const uint8_t* codes;
     const uint8_t* scales;
@@ -87,8 +90,8 @@ __global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, 
                 float v = dot;
                 if (!ok) v = __int_as_float(0x7FFFFFFF);
                 else if (a.metric == MX_COSINE) v = dot * inverse_length(__ldg(a.norms + id)) * inverse_length(q2);
-                else if (a.metric == MX_EUCLIDEAN) v = 2.f * dot - q2 - __ldg(a.norms + id);
-                a.out[c] = v;
+                else if (a.metric == MX_EUCLIDEAN) v = fmaf(2.f, dot, -q2) - __ldg(a.norms + id);
+                a.out[c] = finite_or_nan(v);
             }
         }
         at = last;
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
             if (lane == 0) mbar_arrive(&acc_empty[acc.at]);
             if (a.metric == MX_COSINE) v = v * inverse_length(now.norm) * q_term;
             else if (a.metric == MX_EUCLIDEAN) v = fmaf(2.f, v, -q_term) - now.norm;
-            if (now.at >= 0) a.out[now.at] = (uint32_t)now.id < (uint32_t)a.n && live ? v : __int_as_float(0x7FFFFFFF);
+            if (now.at >= 0) a.out[now.at] = (uint32_t)now.id < (uint32_t)a.n && live ? finite_or_nan(v) : __int_as_float(0x7FFFFFFF);
             now = next;
             next = later;
         }

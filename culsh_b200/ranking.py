@@ -250,7 +250,7 @@ class MXRows:
     def score(self, Q, candidates: Union[Candidates, Tuple], metric: str = "dot") -> torch.Tensor:
         """Scores of queries against their candidates, float32, in the order of the candidates' ids.  ``Q`` stays as it is
         (float32, float64, float16 or bfloat16).  ``candidates``: what ``query`` returned for Q, or a pair (ids, offsets) of int32 and int64.
-        A candidate that is no row gets NaN."""
+        A candidate that is no row gets NaN, and so do all of a query that has an infinity or a NaN, and scores whose sums pass float32."""
         m = _metric(metric)
         Q = _matrix(Q, self.device)
         if Q.dtype not in _TYPES:

@@ -316,3 +316,55 @@ def test_calls_behind_one_another_on_changing_lists(culsh, d, lead):
     torch.cuda.synchronize()
     for i, r in got:
         assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+# ---- scores by few and by many candidates ---------------------------------------------------------------------------
+def few_and_many(rows, Q, n, metric):
+    """Scores of every row for each query, by a call of few candidates and by one of many (of which all rounds are alike)."""
+    nq, times = Q.shape[0], 60_000 // n + 1
+    ids = torch.arange(n, dtype=torch.int32, device="cuda")
+    few = torch.stack([rows.score(Q[i:i + 1], (ids, torch.tensor([0, n], device="cuda")), metric=metric) for i in range(nq)])
+    many = rows.score(Q, (ids.repeat(nq * times), torch.arange(nq + 1, device="cuda") * n * times), metric=metric).view(nq, times, n)
+    assert torch.equal(many.nan_to_num(nan=7e37), many[:, :1].expand_as(many).nan_to_num(nan=7e37))
+    return few, many[:, 0]
+
+
+@pytest.mark.parametrize("metric", ["dot", "cosine", "euclidean"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_scores_of_queries_that_are_not_finite(culsh, dtype, metric):
+    n, d = 70, 96
+    X = torch.randn(n, d, generator=gen(), device="cuda")
+    X[3] = 0
+    X[4, :32] = 0
+    Q = torch.randn(7, d, generator=gen(1), device="cuda").to(dtype)
+    Q[1, 5], Q[2, 40], Q[3, 95] = math.inf, -math.inf, math.nan
+    Q[4, 0], Q[4, 1] = math.inf, -math.inf
+    bad = [1, 2, 3, 4]
+    if dtype == torch.float64:
+        Q[5, 9] = 1e300  # beyond 32 bits, which queries are taken in
+        bad.append(5)
+    for scores in few_and_many(culsh.MXRows(X), Q, n, metric):
+        for i in range(7):
+            assert bool(scores[i].isnan().all()) if i in bad else bool(scores[i].isfinite().all()), i
+
+
+@pytest.mark.parametrize("metric", ["dot", "euclidean"])
+def test_scores_beyond_float32(culsh, metric):
+    n, d = 64, 64
+    X = torch.randn(n, d, generator=gen(), device="cuda")
+    X[::2] *= 2.0 ** 60
+    Q = torch.randn(2, d, generator=gen(1), device="cuda") * 2.0 ** 70
+    Q[1] *= 2.0 ** -70
+    rows = culsh.MXRows(X)
+    q, x = Q.double(), rows.dequantize(torch.float64)
+    want, size = q @ x.T, q.abs() @ x.abs().T
+    if metric == "euclidean":
+        q2, x2 = (q * q).sum(1)[:, None], (x * x).sum(1)[None]
+        want, size = 2 * want - q2 - x2, 2 * size + q2 + x2
+    beyond, within = want.abs() > 2.0 ** 128, size < 2.0 ** 127  # in between a sum may pass the type before it comes back
+    assert bool(beyond[0].any()) and bool(within[1].any())
+    for scores in few_and_many(rows, Q, n, metric):
+        assert not bool(scores.isinf().any())
+        assert bool(scores[beyond].isnan().all())
+        ok = ~scores.isnan()
+        assert bool(ok[within].all()) and bool(((scores.double() - want).abs() <= (d + 4) * ULP * size)[ok].all())
