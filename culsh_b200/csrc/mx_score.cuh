@@ -102,7 +102,9 @@ __global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, 
 // Many candidates: on the tensor cores.  An MMA of 4-bit operands needs the query in 4 bits too, so a query becomes a sum of slices, each a row in
 // microscaled 4 bits: slice j of a block holds the rest behind slice j - 1, to the nearest of +-{0, .5, 1, 1.5, 2, 3, 4, 6} times 2^(E - 2 j).  The rest is exact, and each slice takes two
 // bits at least, so that a query of float32 values within a factor of 2^10 of one another in a block is the sum of about 18 slices, one of bytes that of five: nothing is rounded
-// off.  Sixteen, 32, 48 or 64 slices of a query are the N side of the MMAs; those beyond 64 would be below 2^-126 of the block's largest value.  The M side are 128 candidates of a list, whose codes
+// off.  Sixteen, 32, 48 or 64 slices of a query are the N side of the MMAs; those beyond 64 would be below 2^-126 of the block's largest value.  A scale is no less than 2^-127: a query whose
+// values are all below 2^-64 is multiplied by a power of two that brings the largest there, and its scores are by that less, so that no bit above 2^-63 of a query's largest value is
+// lost (and no sum of such a query can pass float32, whatever the rows' scales).  The M side are 128 candidates of a list, whose codes
 // and scales are gathered by cp.async to where the MMAs take them, and the score is the sum of the accumulator's columns.  No code is unpacked by an instruction:
 // 180M candidates of 128 values 12.0 -> 3.7 ms.  Of 100,000 rows, which lie in L2, they take 2.5 ms: what a warp does for a
 // tile; of a million the gather takes longer: L2 gives 8 TB/s in pieces of 32 and 64 bytes, 174 bytes a candidate with its norm (3.1 ms without it).  Codes gathered by TMA took 3.4 ms
@@ -118,12 +120,17 @@ constexpr int MXS_SETS = 3, MXS_GATHER_WARPS = 4 * MXS_SETS, MXS_MMA_WARPS = 6, 
 constexpr int MXS_ACCS = 6, MXS_SF_COL = MXS_ACCS * MXS_SLICES, MXS_SF_SLOTS = (512 - MXS_SF_COL) / 8 / MXS_MMA_WARPS;  // slots of each
 constexpr int MXS_SMEM = MXS_STAGES * MXS_A_BYTES + MXS_B_SLOTS * MXS_B_BYTES + 1024 + 1024;
 
-// Slices of queries first .. first + gridDim.x - 1, a CTA each: of[q] [groups][MXS_B_BYTES], their number (a multiple of 16) and the squared length.
+// What is known of a query's slices, in a word: their number (a multiple of 16), and the power of two that they have been multiplied by.
+__device__ __forceinline__ int mxs_count(int word) { return word & 255; }
+__device__ __forceinline__ float mxs_down(int word) { return __uint_as_float((uint32_t)(127 - (word >> 8)) << 23); }
+
+// Slices of queries first .. first + gridDim.x - 1, a CTA each: of[q] [groups][MXS_B_BYTES], that word and the squared length.
 template <typename T>
 __global__ void __launch_bounds__(128) mx_slices_kernel(const T* __restrict__ Q, int64_t ldq, int d, int groups, int first, uint8_t* __restrict__ slices,
                                                         int* __restrict__ counts, float* __restrict__ norms, KernelBefore before) {
     behind_kernel_before(Q, slices, counts, norms, before);
     __shared__ int s_need[4];
+    __shared__ uint32_t s_top[4];
     __shared__ float s_norm[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const T* __restrict__ q = Q + (int64_t)(first + blockIdx.x) * ldq;
@@ -131,6 +138,15 @@ __global__ void __launch_bounds__(128) mx_slices_kernel(const T* __restrict__ Q,
         const int c = block * MX_BLOCK + lane;
         return c < d ? (float)__ldcg(q + c) : 0.f;
     };
+    uint32_t top = 0;
+    for (int b = warp; b < groups * 4; b += 4) top = max(top, __float_as_uint(value(b)) & 0x7FFFFFFFu);
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+    top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+    const int exponent_of_top = top >= 0x800000u ? (int)(top >> 23) - 127 : -118 - __clz((int)top);  // of the smallest ones, too
+    const int shift = top != 0 && exponent_of_top < -64 ? -64 - exponent_of_top : 0;
+    const float up = __uint_as_float((uint32_t)(127 + shift) << 23);
     // exponent of a block's first slice (of a value that is not finite: no slices, and a scale that is NaN)
     auto exponent = [&](float v, bool& bad) {
         const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu);
@@ -140,8 +156,9 @@ __global__ void __launch_bounds__(128) mx_slices_kernel(const T* __restrict__ Q,
     int need = 1;
     float norm = 0.f;
     for (int b = warp; b < groups * 4; b += 4) {
-        const float v = value(b);
+        float v = value(b);
         norm = fmaf(v, v, norm);
+        v *= up;
         bool bad;
         const int e = exponent(v, bad);
         // the lowest bit of the block's values, as an exponent
@@ -159,12 +176,12 @@ __global__ void __launch_bounds__(128) mx_slices_kernel(const T* __restrict__ Q,
     need = max(max(s_need[0], s_need[1]), max(s_need[2], s_need[3]));
     const int count = min((need + 15) & ~15, MXS_SLICES);
     if (threadIdx.x == 0) {
-        counts[blockIdx.x] = count;
+        counts[blockIdx.x] = count | shift << 8;
         norms[blockIdx.x] = (s_norm[0] + s_norm[1]) + (s_norm[2] + s_norm[3]);
     }
     for (int b = warp; b < groups * 4; b += 4) {
         uint8_t* const to = slices + ((size_t)blockIdx.x * groups + (b >> 2)) * MXS_B_BYTES;
-        float rest = value(b);
+        float rest = value(b) * up;
         bool bad;
         int e = exponent(rest, bad);
         for (int j = 0; j < count; ++j, e -= 2) {
@@ -373,7 +390,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
             bool live = true;
             while (tiles.live() && live) {
                 const int q = tiles.q - b.first;
-                const uint32_t codes = (uint32_t)__ldcg(b.counts + q) * 64u;
+                const uint32_t codes = (uint32_t)mxs_count(__ldcg(b.counts + q)) * 64u;
                 for (int g = 0; g < a.groups; ++g) {
                     if (!b.kept || g == 0) {
                         if (!mbar_wait(&b_empty[slot], parity, s_abort, b.d_error)) { live = false; break; }
@@ -411,7 +428,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
         while (tiles.live() && live) {
             if (tiles.q != q) {
                 q = tiles.q;
-                count = __ldcg(b.counts + q - b.first);
+                count = mxs_count(__ldcg(b.counts + q - b.first));
             }
             const uint32_t id0 = mx_idesc(count, 0), id1 = mx_idesc(count, 2);
             if (!mbar_wait_warp(&acc_empty[acc.at], acc.parity, s_abort, b.d_error)) break;
@@ -471,13 +488,15 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
         norm_of(now);
         bool live = true;
         int q = -1, count = 0;
-        float q_term = 0.f;
+        float q_term = 0.f, down = 1.f;
         for (MxRing acc{(uint32_t)set, 0u}; now.q >= 0; acc.on(MXS_SETS, MXS_ACCS)) {
             const Ahead later = take();
             norm_of(next);
             if (now.q != q) {
                 q = now.q;
-                count = __ldcg(b.counts + q);
+                const int word = __ldcg(b.counts + q);
+                count = mxs_count(word);
+                down = mxs_down(word);
                 q_term = norm_term(a.metric, __ldcg(b.q_norms + q));
             }
             if (live) live = mbar_wait_warp(&acc_full[acc.at], acc.parity, s_abort, b.d_error);
@@ -495,6 +514,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
                     v += (w[7] + w[6]) + (w[5] + w[4]);
                     v += (w[3] + w[2]) + (w[1] + w[0]);
                 }
+                v *= down;
             }
             tc_fence_before();
             __syncwarp();

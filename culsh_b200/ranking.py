@@ -248,8 +248,8 @@ class MXRows:
         _lib.check(self._h.lib.culsh_mx_product_check(self._h.ptr, _stream(self.device)))
 
     def score(self, Q, candidates: Union[Candidates, Tuple], metric: str = "dot") -> torch.Tensor:
-        """Scores of queries against their candidates, float32, in the order of the candidates' ids.  ``Q`` stays as it is
-        (float32, float64, float16 or bfloat16).  ``candidates``: what ``query`` returned for Q, or a pair (ids, offsets) of int32 and int64.
+        """Scores of queries against their candidates, float32, in the order of the candidates' ids.  ``Q`` (float32,
+        float64, float16 or bfloat16) is taken in 32 bits, not in 4.  ``candidates``: what ``query`` returned for Q, or a pair (ids, offsets) of int32 and int64.
         A candidate that is no row gets NaN, and so do all of a query that has an infinity or a NaN, and scores whose sums pass float32."""
         m = _metric(metric)
         Q = _matrix(Q, self.device)

@@ -343,7 +343,7 @@ int culsh_mx_product_check(culsh_handle* h, void* stream);
 /* out[c], c in [offsets[q], offsets[q + 1]): the metric of query q as it is (any type, rows ldq apart)
  * and row ids[c]; NaN where ids[c] is no row, where a value of the query is not finite, and where the score, or a
  * sum on the way to it, is beyond float32.  offsets: n_queries + 1, from 0 to total.  Queries are taken in
- * 32 bits; of a block's values, bits below 2^-126 of the largest do not count.  workspace: device, as many bytes as
+ * 32 bits; of many candidates' scores, bits below 2^-63 of a query's largest value may not count.  workspace: device, as many bytes as
  * culsh_mx_score_workspace says, aligned to 16. */
 int culsh_mx_score_workspace(culsh_handle* h, int n_queries, int d, int64_t total, uint64_t* bytes);
 int culsh_mx_score(culsh_handle* h, const void* Q, int type, int n_queries, int64_t ldq, const uint8_t* codes,

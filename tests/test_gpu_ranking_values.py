@@ -368,3 +368,25 @@ def test_scores_beyond_float32(culsh, metric):
         assert bool(scores[beyond].isnan().all())
         ok = ~scores.isnan()
         assert bool(ok[within].all()) and bool(((scores.double() - want).abs() <= (d + 4) * ULP * size)[ok].all())
+
+
+@pytest.mark.parametrize("size", [-60, -64, -66, -90, -110, -120])
+@pytest.mark.parametrize("law", ["alike", "wide"])
+def test_scores_of_small_queries(culsh, size, law):
+    """Queries of values around 2^size: as exact by many candidates as by few, against rows that pick single values out and rows that sum them."""
+    d = n = 64
+    X = torch.cat([torch.eye(32, d, device="cuda"), torch.randn(n - 32, d, generator=gen(), device="cuda")])
+    X[40:] *= 2.0 ** 40
+    Q = torch.randn(4, d, generator=gen(1), device="cuda")
+    if law == "wide":
+        Q *= torch.exp2(torch.randint(-5, 6, (4, d), generator=gen(2), device="cuda").float())
+    Q *= 2.0 ** size
+    Q[3] = 0
+    Q[3, 5] = 3 * 2.0 ** -149  # the smallest ones there are
+    rows = culsh.MXRows(X)
+    x, q = rows.dequantize(torch.float64), Q.double()
+    want, bound = q @ x.T, (d + 2) * ULP * (q.abs() @ x.abs().T)
+    # products of the smallest numbers with 0.5 are cut to whole steps of 2^-149 before the scale
+    least = 2.0 ** -149 * d * x.abs().amax(1)[None, :].clamp(min=1)
+    for scores in few_and_many(rows, Q, n, "dot"):
+        assert bool(((scores.double() - want).abs() <= bound + least).all())
