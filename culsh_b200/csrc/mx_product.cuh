@@ -133,8 +133,10 @@ __device__ __forceinline__ uint32_t pack_scores(const __nv_bfloat16*, float lo, 
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// 1 / length; 0 for a row of zeros, whose cosines are 0.
-__device__ __forceinline__ float inverse_length(float norm) { return norm == 0.f ? 0.f : rsqrtf(norm); }
+// 1 / length; 0 for a row of zeros, whose cosines are 0; NaN where the square says too little of the length, or nothing: below 2^-126, and beyond the type.
+__device__ __forceinline__ float inverse_length(float norm) {
+    return norm == 0.f ? 0.f : norm >= 1.175494351e-38f && norm < INFINITY ? rsqrtf(norm) : __int_as_float(0x7FFFFFFF);
+}
 // What a squared norm adds to a score.
 __device__ __forceinline__ float norm_term(int metric, float norm) { return metric == MX_COSINE ? inverse_length(norm) : norm; }
 // Scores from dot products with one entry of one side and N of the other.

@@ -9,7 +9,7 @@
 // Layout (mx_shape): codes row-major, two to a byte, the first in the low half, rows padded with zeros to groups of 128 values (64 bytes), which is what TMA
 // loads and what a gathered row is read in.  Scales lie as the tensor cores take them: for 128 rows by 4 blocks (128 values) one tile of
 // 512 bytes, byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4, so a row's four scales of a group are one aligned word and a tile goes into tensor memory as it is.
-// norms[row] is the squared length of the row that is held.
+// norms[row] is the squared length of the row that is held, 0 for a row of zeros alone: MX_LEAST for what is too small for a square in 32 bits, infinite for what is too large.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -19,6 +19,7 @@
 
 namespace culsh_b200 {
 
+constexpr float MX_LEAST = 1.401298464e-45f;  // 2^-149
 constexpr int MX_BLOCK = 32, MX_GROUP = 128, MX_TILE_ROWS = 128, MX_TILE_BYTES = 512;
 
 // Host and device: groups of 128 values in a row of d, tiles of 128 rows.
@@ -158,6 +159,13 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const T* __restrict__ 
         }
     }
     for (int o = 1; o < min(lanes, 32); o *= 2) norm += __shfl_xor_sync(0xFFFFFFFFu, norm, o);
+    if (norm == 0.f) {  // for all lanes of the row in this warp: zeros, or too small for squares (from 2^-129 on the largest value is not rounded to 0)
+        bool some = false;
+        if (row < n)
+            for (int g = at / 16; g < groups; g += lanes / 16)
+                for (int c = g * MX_GROUP + (at & 15) * 8; c < min(g * MX_GROUP + (at & 15) * 8 + 8, d); ++c) some = some || fabsf((float)__ldcg(X + row * ld + c)) > 1.469367939e-39f;
+        if (__any_sync(lanes == 16 ? 0xFFFFu << (threadIdx.x & 16) : 0xFFFFFFFFu, some)) norm = MX_LEAST;
+    }
     if (lanes > 32) {
         if ((threadIdx.x & 31) == 0) s_norm[threadIdx.x >> 5] = norm;
         __syncthreads();

@@ -52,11 +52,14 @@ __global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, 
         const T* __restrict__ x = Q + (int64_t)q * a.ldq;
         float q2 = 0.f;
         if (a.metric != MX_DOT) {
+            bool zero = true;
             for (int i = lane; i < a.d; i += 32) {
                 const float v = (float)x[i];
                 q2 = fmaf(v, v, q2);
+                zero = zero && v == 0.f;
             }
             for (int o = 16; o; o >>= 1) q2 += __shfl_xor_sync(0xFFFFFFFFu, q2, o);
+            if (!__all_sync(0xFFFFFFFFu, zero) && q2 == 0.f) q2 = MX_LEAST;
         }
         for (; at < last; at += 8) {
             const int64_t c = at + (lane >> 2);
@@ -177,7 +180,8 @@ __global__ void __launch_bounds__(128) mx_slices_kernel(const T* __restrict__ Q,
     const int count = min((need + 15) & ~15, MXS_SLICES);
     if (threadIdx.x == 0) {
         counts[blockIdx.x] = count | shift << 8;
-        norms[blockIdx.x] = (s_norm[0] + s_norm[1]) + (s_norm[2] + s_norm[3]);
+        const float all = (s_norm[0] + s_norm[1]) + (s_norm[2] + s_norm[3]);
+        norms[blockIdx.x] = all == 0.f && top != 0 ? MX_LEAST : all;
     }
     for (int b = warp; b < groups * 4; b += 4) {
         uint8_t* const to = slices + ((size_t)blockIdx.x * groups + (b >> 2)) * MXS_B_BYTES;

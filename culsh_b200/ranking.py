@@ -155,7 +155,7 @@ class MXRows:
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, norms: torch.Tensor, n_features: int) -> "MXRows":
         """Rows from the arrays of another MXRows, e.g. loaded from a file: ``codes`` [n, 64 G] (two to a byte, the first in the
         low half, zeros behind the row's end) with G = ceil(n_features / 128), ``scales`` [ceil(n / 128), G, 32, 4, 4] (127 + exponent of block 4 g + b
-        of row 128 t + 32 j + i at [t, g, i, j, b]), ``norms`` [n] float32 (squared lengths)."""
+        of row 128 t + 32 j + i at [t, g, i, j, b]), ``norms`` [n] float32 (squared lengths, 0 for rows of zeros alone)."""
         d = int(n_features)
         if d <= 0:
             raise ValueError("n_features must be positive")
@@ -206,7 +206,7 @@ class MXRows:
 
     def product(self, Q, metric: str = "dot", dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """Scores [n_queries, n_rows] of queries against every row: dot products, cosines or negative squared
-        distances ("euclidean").  ``Q``: MXRows, or an array that is held in 4 bits for the call.  Rows of many scores begin at multiples of
+        distances ("euclidean").  Cosines with a row of zeros are 0, with lengths outside of 1.1e-19 to 1.8e19 NaN.  ``Q``: MXRows, or an array that is held in 4 bits for the call.  Rows of many scores begin at multiples of
         128 bytes, so that the result of an odd number of rows is not contiguous."""
         m = _metric(metric)
         if dtype not in _SCORE_TYPES:
@@ -250,7 +250,8 @@ class MXRows:
     def score(self, Q, candidates: Union[Candidates, Tuple], metric: str = "dot") -> torch.Tensor:
         """Scores of queries against their candidates, float32, in the order of the candidates' ids.  ``Q`` (float32,
         float64, float16 or bfloat16) is taken in 32 bits, not in 4.  ``candidates``: what ``query`` returned for Q, or a pair (ids, offsets) of int32 and int64.
-        A candidate that is no row gets NaN, and so do all of a query that has an infinity or a NaN, and scores whose sums pass float32."""
+        A candidate that is no row gets NaN, and so do all of a query that has an infinity or a NaN, and scores whose sums pass float32; cosines as in
+        ``product``."""
         m = _metric(metric)
         Q = _matrix(Q, self.device)
         if Q.dtype not in _TYPES:

@@ -309,7 +309,7 @@ int culsh_merge_shard_candidates_noalloc(culsh_handle* h, int n_shards, int n_qu
 typedef enum culsh_type { CULSH_F32 = 0, CULSH_F64 = 1, CULSH_F16 = 2, CULSH_BF16 = 3 } culsh_type;
 typedef enum culsh_metric {
     CULSH_DOT = 0,      /* q . x                                    */
-    CULSH_COSINE = 1,   /* q . x / (|q| |x|), 0 for a row of zeros  */
+    CULSH_COSINE = 1,   /* q . x / (|q| |x|), 0 for a row of zeros; NaN for other lengths below 2^-63 (1.1e-19) or from 2^64 (1.8e19) on */
     CULSH_EUCLIDEAN = 2 /* -|q - x|^2                               */
 } culsh_metric;
 
@@ -321,7 +321,7 @@ typedef enum culsh_metric {
  *                               fraction), zeros behind a row's end
  *   scales [T][G][32][4][4]     exponent + 127 of block 4 g + b of row 128 t + 32 j + i at [t][g][i][j][b];
  *                               255 is NaN
- *   norms  [n]                  squared length of the row as held
+ *   norms  [n]                  squared length of the row as held; 2^-149 where that is smaller, 0 for rows of zeros
  * codes and scales begin at a multiple of 16 bytes. */
 int culsh_mx_quantize(culsh_handle* h, const void* X, int type, int n, int d, int64_t ld, uint8_t* codes, uint8_t* scales,
                       float* norms, void* stream);

@@ -390,3 +390,38 @@ def test_scores_of_small_queries(culsh, size, law):
     least = 2.0 ** -149 * d * x.abs().amax(1)[None, :].clamp(min=1)
     for scores in few_and_many(rows, Q, n, "dot"):
         assert bool(((scores.double() - want).abs() <= bound + least).all())
+
+
+# ---- lengths --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("nq", [8, 80])  # rows or queries on the M side
+@pytest.mark.parametrize("d", [96, 200, 1000, 2500])
+def test_cosines_of_rows_of_any_length(culsh, d, nq):
+    """Right where squares of lengths are floats, NaN where they are not, 0 for zeros."""
+    sizes = [-140, -100, -80, -70, -50, -20, 0, 30, 50, 70, 100]
+    g = gen(nq)
+    size = lambda n: torch.exp2(torch.tensor([float(sizes[i % len(sizes)]) for i in range(n)], device="cuda"))[:, None]  # noqa: E731
+    X, Q = torch.randn(66, d, generator=g, device="cuda") * size(66), torch.randn(nq, d, generator=g, device="cuda") * size(nq)
+    X[5] = 0
+    Q[6] = 0
+    X[16, 1:] = 0  # one value of 2^0 or so
+    rows = culsh.MXRows(X)
+    x = rows.dequantize(torch.float64)
+    x2 = (x * x).sum(1)
+    assert torch.equal(rows.norms == 0, x2 == 0) and torch.equal(rows.norms.isinf(), x2 > 2.0 ** 128)
+
+    def check(scores, q):
+        q2 = (q * q).sum(1)
+        dot, many = q @ x.T, q.abs() @ x.abs().T
+        length = q2.sqrt()[:, None] * x2.sqrt()[None, :]
+        fits = lambda v: (v >= 2.0 ** -126) & (v < 2.0 ** 128) | (v == 0)  # noqa: E731
+        ok = fits(q2)[:, None] & fits(x2)[None, :]
+        assert torch.equal(~scores.isnan(), ok)
+        want = torch.where(length > 0, dot / length, torch.zeros_like(dot))
+        bound = torch.where(length > 0, (2 * d + 10) * ULP * many / length, torch.zeros_like(dot))
+        assert bool(((scores.double() - want).abs() <= bound)[ok].all())
+
+    held = culsh.MXRows(Q)
+    check(rows.product(Q, metric="cosine"), held.dequantize(torch.float64))
+    check(rows.product(held, metric="cosine"), held.dequantize(torch.float64))
+    for scores in few_and_many(rows, Q, 66, "cosine"):
+        check(scores, Q.double())
