@@ -9,7 +9,8 @@
 // take them and go from shared into tensor memory by tcgen05.cp, issued by the warp that issues the MMAs, in front of the two MMAs (64 values each) that read them.
 //
 // Persistent CTAs with a warp for the TMA loads, one for the MMAs and four, eight or twelve of epilogue; accumulators in turn.  Every wait is bounded
-// (mbar_wait); a CTA whose wait ran out records it and fills what it has not done with NaN.  No load uses cluster multicast.
+// (mbar_wait); a CTA whose wait ran out records it, fills what it has not done with NaN, and waits, with the same bound, for what it has in flight before it gives its memory back.  No load
+// uses cluster multicast.
 #pragma once
 
 #include <algorithm>
@@ -50,7 +51,7 @@ struct MxpCfg {
     static constexpr int SF_SLOTS = (TMEM_COLS - ACC_COLS) / 8, MAX_ACCS = ACC_COLS / 16;
     static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + TERMS + 1024 /*barriers*/ + 1024 /*alignment slack*/;
     static_assert(STAGE_BYTES % 1024 == 0 && CTAS * (SMEM + 1024) <= 228 * 1024, "");
-    static_assert((2 * STAGES + 2 * MAX_ACCS) * 8 + 16 <= 1024, "");
+    static_assert((2 * STAGES + 2 * MAX_ACCS + 1) * 8 + 16 <= 1024, "");
 };
 
 struct MxProductArgs {
@@ -76,6 +77,15 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 // A wait of a whole warp, with one answer.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_error) {
     return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, d_error));
+}
+// For a CTA that gives up: waits, whatever its flag says, until `fills` loads in turn into a ring of `n` have landed.
+__device__ __forceinline__ void mbar_wait_landed(uint64_t* bars, uint32_t n, uint32_t fills) {
+    const long long t0 = clock64();
+    for (uint32_t s = 0; s < n; ++s) {
+        const uint32_t of_this = fills / n + (s < fills % n);
+        while (of_this && !mbar_try_wait(&bars[s], (of_this - 1) & 1u))
+            if (clock64() - t0 > TC_WAIT_CYCLES) return;
+    }
 }
 // The MMAs are issued by a whole warp, whose elected lane (the same each time) does it: what a single lane computes on its own does not get into the uniform registers that these
 // instructions take their operands from without one instruction, and its latency, for each.
@@ -334,8 +344,10 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     uint64_t* empty = full + STAGES;
     uint64_t* acc_full = empty + STAGES;
     uint64_t* acc_empty = acc_full + Cfg::MAX_ACCS;
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(acc_empty + Cfg::MAX_ACCS);
+    uint64_t* drained = acc_empty + Cfg::MAX_ACCS;
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+    uint32_t* s_fills = s_tmem + 2;  // stages that have been loaded
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t accs = Cfg::ACC_COLS / a.acc_cols;
 
@@ -348,6 +360,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             mbar_init(&acc_full[b], 1);
             mbar_init(&acc_empty[b], 4);
         }
+        mbar_init(drained, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -362,7 +375,7 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t s = 0, parity = 1;
+            uint32_t s = 0, parity = 1, fills = 0;
             bool live = true;
             const uint32_t bytes = Cfg::A_BYTES + (uint32_t)(a.box_b * SPAN);
             for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x) {
@@ -378,9 +391,11 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
                     bulk_load(st + Cfg::A_BYTES + Cfg::B_BYTES, a.a_scales + ((size_t)ia * a.groups + g) * MX_TILE_BYTES, scales, &full[s]);
                     bulk_load(st + Cfg::A_BYTES + Cfg::B_BYTES + Cfg::S_BYTES, a.b_scales + ((size_t)ib * a.groups + g) * MX_TILE_BYTES,
                               scales, &full[s]);
+                    ++fills;
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
             }
+            *s_fills = fills;
         }
     } else if (warp == 1) {
         uint32_t s = 0, parity = 0, ab = 0, acc_parity = 1, slot = 0;
@@ -427,6 +442,14 @@ mx_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (*s_abort) {  // all roles are done: what they issued may not be
+        if (threadIdx.x == 0) mbar_wait_landed(full, STAGES, *s_fills);
+        if (warp == 1) {
+            tc_commit_warp(drained);
+            mbar_wait_landed(drained, 1, 1);
+        }
+        __syncthreads();
+    }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::TMEM_COLS) : "memory");
 }
 

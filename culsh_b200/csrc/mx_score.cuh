@@ -304,8 +304,10 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
     uint64_t* b_empty = b_full + MXS_B_SLOTS;
     uint64_t* acc_full = b_empty + MXS_B_SLOTS;
     uint64_t* acc_empty = acc_full + MXS_ACCS;
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(acc_empty + MXS_ACCS);
+    uint64_t* drained = acc_empty + MXS_ACCS;
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+    uint32_t* s_fills = s_tmem + 2;  // slots of slices that have been loaded
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const MxScoreArgs& a = b.a;
 
@@ -322,6 +324,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
             mbar_init(&acc_full[s], 1);
             mbar_init(&acc_empty[s], 4);
         }
+        mbar_init(drained, MXS_MMA_WARPS);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
         while (in_flight) land();
     } else if (warp == MXS_GATHER_WARPS) {
         if (lane == 0) {
-            uint32_t slot = 0, parity = 1;
+            uint32_t slot = 0, parity = 1, fills = 0;
             bool live = true;
             while (tiles.live() && live) {
                 const int q = tiles.q - b.first;
@@ -399,6 +402,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
                     if (!b.kept || g == 0) {
                         if (!mbar_wait(&b_empty[slot], parity, s_abort, b.d_error)) { live = false; break; }
                         mbar_expect_tx(&b_full[slot], (codes + MX_TILE_BYTES) * (b.kept ? (uint32_t)a.groups : 1u));
+                        ++fills;
                     }
                     unsigned char* to = s_b + (b.kept ? slot * a.groups + g : slot) * MXS_B_BYTES;
                     const uint8_t* from = b.slices + ((size_t)q * a.groups + g) * MXS_B_BYTES;
@@ -409,6 +413,7 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
                 if (b.kept) tiles.next_list();
                 else tiles.next(1);
             }
+            *s_fills = fills;
         }
     } else if (warp <= MXS_GATHER_WARPS + MXS_MMA_WARPS) {
         // Tiles go to the warps in turn where the ring holds a multiple of the warps' tiles: each barrier of a stage or an accumulator is waited for by the same warp then.  Longer
@@ -533,6 +538,14 @@ __global__ void __launch_bounds__(MXS_THREADS, 1) mx_score_tc_kernel(MxScoreBatc
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (*s_abort) {  // all roles are done: what they issued may not be (the gathering warps have waited for their copies)
+        if (threadIdx.x == 32 * MXS_GATHER_WARPS) mbar_wait_landed(b_full, (uint32_t)b.lists, *s_fills);
+        if (warp > MXS_GATHER_WARPS && warp <= MXS_GATHER_WARPS + MXS_MMA_WARPS) {
+            tc_commit_warp(drained);
+            mbar_wait_landed(drained, 1, 1);
+        }
+        __syncthreads();
+    }
     if (warp == MXS_GATHER_WARPS + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

@@ -84,3 +84,46 @@ def test_kernels_launched_early_read_by_l2():
     assert "__ldg" not in source("mx_product.cuh")
     # the kernel that gathers scales by L1 is launched as usual
     assert re.search(r"\bmx_score_tc_kernel<<<", score["mx_score"]) and "KernelBefore" not in source("mx_score.cuh").split("mx_score_tc_kernel(")[1].split("{")[0]
+
+
+def test_a_kernel_that_gives_up_waits_for_what_it_has_in_flight():
+    """Where a bounded wait ran out, loads and tensor-core work may still be on their way to memory that the CTA is about to give back: behind the barrier at which all
+    roles are done, and before tensor memory is freed, both are waited for, without regard to the flag that ends the other waits."""
+    for name, kernel in (("mx_product.cuh", "mx_product_kernel"), ("mx_score.cuh", "mx_score_tc_kernel")):
+        text = source(name)
+        end = text[text.index(kernel + "("):]
+        end = end[:end.index("tcgen05.dealloc")]
+        last = end[end.rindex("tc_fence_before"):]
+        assert re.search(r"__syncthreads\(\);.*if \(\*s_abort\) \{.*mbar_wait_landed\(\w*full, .*tc_commit_warp\(drained\);\s*mbar_wait_landed\(drained, 1, 1\);.*__syncthreads\(\);", last, re.S), name
+        assert end.count("++fills;") == 1 and "*s_fills = fills;" in end
+    wait = source("mx_product.cuh")
+    wait = wait[wait.index("void mbar_wait_landed("):]
+    wait = wait[:wait.index("\n}\n")]
+    assert "TC_WAIT_CYCLES" in wait and "abort" not in wait
+
+
+def test_loads_that_landed_are_told_from_their_number(tmp_path):
+    """The phase of a ring's barrier that its last load ends: loads go to the slots in turn, a phase for each."""
+    from native import run_native
+    body = source("mx_product.cuh")
+    line = re.search(r"const uint32_t of_this = ([^;]+);", body).group(1)
+    parity = re.search(r"mbar_try_wait\(&bars\[s\], ([^)]*\)[^)]*)\)\)", body).group(1)
+    out = run_native(tmp_path, """
+#include <cstdint>
+#include <cstdio>
+#include <vector>
+int main() {
+    for (uint32_t n = 1; n <= 12; ++n)
+        for (uint32_t fills = 0; fills < 40; ++fills) {
+            std::vector<uint32_t> phases(n, 0);
+            for (uint32_t i = 0; i < fills; ++i) ++phases[i %% n];
+            for (uint32_t s = 0; s < n; ++s) {
+                const uint32_t of_this = %s;
+                if (of_this != phases[s]) return 1;
+                if (of_this && (%s) != ((phases[s] - 1) %% 2)) return 2;
+            }
+        }
+    puts("ok");
+}
+""" % (line, parity))
+    assert out == "ok\n"
