@@ -730,14 +730,14 @@ __device__ __forceinline__ bool lp_far(const LpBackward& b, int row) {
     const float lse = __ldg(b.lse + row);
     return fabsf(lse) > LP_NEAR && lse != -INFINITY;
 }
-// The entry that has the gradient of a row's log probability, or -1; by a warp.  `whole`: it takes the whole row to say, or to say what p is.
-__device__ __forceinline__ int64_t lp_given(const LpBackward& b, int row, int64_t begin, int64_t end, bool& whole) {
-    whole = lp_far(b, row);
-    if (whole || !b.f.targets || !b.g) return -1;
+// The entry that has the gradient of a row's log probability, or -1; by a warp.  `left`: of a long list, whose target is not where the search finds it, if it has it.
+__device__ __forceinline__ int64_t lp_given(const LpBackward& b, int row, int64_t begin, int64_t end, bool& left) {
+    left = false;
+    if (!b.f.targets || !b.g) return -1;
     int64_t at = LpFind(b.f, row, begin, end)(b.f);
     if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) {
-        whole = end - begin > LP_LOOK;
-        if (!whole) {
+        left = end - begin > LP_LOOK;
+        if (!left) {
             at = lp_first_named<2>(b.f.ids - b.f.rows.shift, begin, end, __ldg(b.f.targets + row), threadIdx.x & 31, 32);
             const unsigned first = __reduce_min_sync(0xFFFFFFFFu, (unsigned)(at - begin));
             at = first < (unsigned)(end - begin) ? begin + first : -1;
@@ -844,10 +844,9 @@ __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_
     const int64_t span = begin / LP_ROW_SPAN<T> + (blockIdx.x - (unsigned)row * (unsigned)b.units);
     const int64_t from = max(span * LP_ROW_SPAN<T>, begin), to = min((span + 1) * LP_ROW_SPAN<T>, end);
     if (from >= to) return;
-    bool whole;
-    const int64_t target = lp_given(b, (int)row, begin, end, whole);
-    if (whole) return;
-    const LpRowTerms r = lp_row_terms(x, b, (int)row, target);
+    if (lp_far(b, (int)row)) return;
+    bool left;
+    const LpRowTerms r = lp_row_terms(x, b, (int)row, lp_given(b, (int)row, begin, end, left));
     lp_backward_span<ALIKE, false>(x, out + (row * b.ldo - begin), r, b.f.inv_t, from, to, threadIdx.x, LP_THREADS);
 }
 
@@ -864,20 +863,19 @@ __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_
         if (begin >= p1) break;
         const int64_t from = max(begin, p0), to = min(end, p1);
         if (from >= to) continue;
-        bool whole;
-        const int64_t target = lp_given(b, row, begin, end, whole);
-        if (whole) continue;
-        const LpRowTerms r = lp_row_terms(x, b, row, target);
+        if (lp_far(b, row)) continue;
+        bool left;  // then as if it had no target; log_probs_backward_whole_kernel looks for that
+        const LpRowTerms r = lp_row_terms(x, b, row, lp_given(b, row, begin, end, left));
         lp_backward_span<ALIKE, false>(x, out - rows.shift, r, b.f.inv_t, from, to, threadIdx.x & 31, 32);
     }
 }
 
-// Rows that have to be looked at as a whole before any of their gradient is known.  Lists whose target is not where a search finds it; and rows whose lse is large, so that it says p only to its
-// rounding (squared distances of bytes by a temperature of 0.05: to 10 %): their log p counts from the largest score, as in the forward pass, with sums made again.  The kernels with spans
-// leave such rows alone, so that this may run beside them: it waits for them at its end only.  (As CTAs of their launch it took registers from the spans: 1,000 x 200,003 bfloat16 186 us in
-// place of 157; behind them 1,000 lists of 200 took 24 us.)
+// Rows that have to be looked at as a whole, beside the kernel of the spans.  Rows whose lse is large, so that it says p only to its rounding (squared distances of bytes by a temperature of
+// 0.05: to 10 %), are left to this one: their log p counts from the largest score, as in the forward pass, with sums made again (1,000 x 200,003 bfloat16, all of them such rows, 450 us in place
+// of 157).  Long lists whose target is not where a search finds it are looked through; where it is found after all, the kernel of the spans is waited for and the list is done again.
+// (As CTAs of its launch this took registers from the spans: 186 us in place of 157; behind it 1,000 lists of 200 took 24 us, 17 beside.)
 template <bool ALIKE, typename T>
-__global__ void __launch_bounds__(LP_THREADS) log_probs_backward_whole_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+__global__ void __launch_bounds__(LP_THREADS, 4) log_probs_backward_whole_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
     __shared__ int64_t s_target;
     __shared__ LpPart s_parts[LP_WARPS];
     const LpRows& rows = b.f.rows;
@@ -888,26 +886,33 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_backward_whole_kernel(co
         b.f.m, (int)blockIdx.x / b.shares, b.whole / b.shares,
         [&](int row) { return (b.f.ids && b.g && rows.end(row) - rows.begin(row) > LP_LOOK) || lp_far(b, row); },
         [&](int row) {
-            bool whole;
-            lp_given(b, row, rows.begin(row), rows.end(row), whole);
-            return whole;
+            bool left = lp_far(b, row);
+            if (!left) lp_given(b, row, rows.begin(row), rows.end(row), left);
+            return left;
         },
         [&](int row) {
             const int64_t begin = rows.begin(row), end = rows.end(row);
             if (threadIdx.x == 0) s_target = -1;
             __syncthreads();
+            const bool far = lp_far(b, row);
             if (b.f.targets && b.g) {
-                const int64_t at = LpFind(b.f, row, begin, end)(b.f);  // the same in all warps
-                if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) lp_find_in_any_order(b.f, row, begin, end, s_target, LP_THREADS);
+                const int64_t at = far ? LpFind(b.f, row, begin, end)(b.f) : -1;  // the same in all warps; of the others it is known
+                if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) lp_find_in_any_order<8>(b.f, row, begin, end, s_target, LP_THREADS);
                 else if (threadIdx.x == 0) s_target = at;
             }
-            const bool far = lp_far(b, row);
             if (far) {
                 float largest = 0.f;
                 const LpPart mine = lp_chunks<false>(x, begin / LP_CHUNK<T> + warp, (end + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, b.f.c, lane, largest, [](int64_t, float) {});
                 if (lane == 0) s_parts[warp] = mine;
             }
             __syncthreads();
+            if (!far) {
+                if (s_target < 0) {  // it has none, as has been taken for granted
+                    __syncthreads();
+                    return;
+                }
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+            }
             LpRowTerms r = lp_row_terms(x, b, row, s_target);
             if (far) {
                 LpPart all = s_parts[0];
@@ -979,7 +984,7 @@ inline void log_probs(const CtxPtr& c, const T* scores, LpArgs a, void* workspac
         int th = mean <= 1024 || (a.m >= 32 * c->sm_count && mean <= 32768) ? 32 : a.m >= 16 * c->sm_count && mean <= 16384 ? 64 : 128;
         while (th < a.k) th *= 2;
         auto kern = th == 32 ? log_probs_row_kernel<32, T> : th == 64 ? log_probs_row_kernel<64, T> : log_probs_row_kernel<128, T>;
-        a.placed = a.ids && a.targets && mean > 1024;
+        a.placed = a.ids && a.targets && (mean > 8192 || (a.rows.total > 1 << 18 && a.m <= 1 << 11));  // the second: lists that are long among others
         if (a.placed) {
             log_probs_places_kernel<<<(unsigned)std::min((a.m - 1) / LP_WARPS + 1, 8 * c->sm_count), LP_THREADS, 0, stream>>>(a);
             KERNEL_CHECK();
@@ -1010,7 +1015,7 @@ inline void log_probs_backward(const CtxPtr& c, const T* scores, T* out, LpBackw
     const int64_t mean = r.total / b.f.m;
     b.span = mean >= 1024 ? 512 : mean >= 64 ? 128 : 32;
     b.units = r.offsets ? (int64_t)ceil_div((size_t)(r.total + r.shift), (size_t)b.span) : r.cols / LP_ROW_SPAN<T> + 2;
-    b.whole = 2 * c->sm_count;
+    b.whole = 4 * c->sm_count;
     b.shares = 1;
     while (b.shares < 16 && 2 * b.shares * ((b.f.m - 1) / LP_WARPS + 1) <= b.whole) b.shares *= 2;
     b.whole = std::min((b.f.m - 1) / LP_WARPS + 1, b.whole / b.shares) * b.shares;
