@@ -48,7 +48,8 @@ LpArgs log_probs_args(const void* scores, int m, int64_t cols, int64_t ld, const
                       const int64_t* targets) {
     need(scores || (offsets && total == 0), "null argument");
     need(m > 0, "rows must be positive");
-    need(temperature > 0 && std::isfinite(temperature) && std::isfinite(1 / (float)temperature), "temperature must be positive");
+    need(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+    need(temperature > 4.3e-39, "the temperature is too small: log2(e) by it has to be a float");
     if (offsets) {
         need(total >= 0, "total must not be negative");
         if (total >= (ids ? 1ll << 32 : 1ll << 31)) fail(CULSH_ERR_UNSUPPORTED, "%lld entries are too many for one call", (long long)total);  // places have 32 bits

@@ -318,6 +318,13 @@ def _targets(targets, lists, m, device):
     return targets if targets.dtype == torch.int64 and targets.is_contiguous() else targets.to(torch.int64).contiguous()
 
 
+def _temperature(temperature):
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError("temperature must be positive")
+    if temperature < 4.3e-39:  # below, log2(e) by it is no float
+        raise ValueError("temperature is too small")
+
+
 def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None, top_k: int = 0, temperature: float = 1.0) -> LogProbs:
     """Log probabilities under softmax(scores / temperature): of given entries, with the entropy and the most likely ones.
 
@@ -327,8 +334,7 @@ def log_probs(scores, targets=None, lists: Union[Candidates, Tuple, None] = None
     top_k = int(top_k)
     if not 0 <= top_k <= MAX_TOP_K:
         raise ValueError(f"top_k must be between 0 and {MAX_TOP_K}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError("temperature must be positive")
+    _temperature(temperature)
     scores, lists, m, cols, pitch = _scores(scores, lists)
     device = scores.device
     targets = _targets(targets, lists, m, device)
@@ -370,8 +376,7 @@ def log_probs_backward(scores, targets, lse, entropy, grad_log_probs=None, grad_
     """Gradient with respect to ``scores``, in their type, from the gradients of the log probabilities and of the entropies of
     ``log_probs(scores, targets, lists, temperature=temperature)``, whose ``lse`` and ``entropy`` it takes.  A target that is not in
     its row, or is masked with -inf, has no gradient."""
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError("temperature must be positive")
+    _temperature(temperature)
     scores, lists, m, cols, pitch = _scores(scores, lists)
     device = scores.device
     if grad_log_probs is not None and targets is None:

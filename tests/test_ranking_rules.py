@@ -127,3 +127,17 @@ int main() {
 }
 """ % (line, parity))
     assert out == "ok\n"
+
+
+def test_temperatures_that_no_float_divides_by_are_refused():
+    """Between them and the ones whose reciprocal is no float either, ties came out as NaN."""
+    import pytest
+    import torch
+
+    import culsh_b200 as culsh
+    s, one = torch.zeros(2, 2), torch.zeros(2)
+    for t in (4.2e-39, 3.5e-39, 1e-39, 1e-300):
+        with pytest.raises(ValueError, match="too small"):
+            culsh.log_probs(s, temperature=t)
+        with pytest.raises(ValueError, match="too small"):
+            culsh.log_probs_backward(s, None, one, one, temperature=t)
