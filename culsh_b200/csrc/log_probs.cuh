@@ -7,8 +7,9 @@
 // in 32 bits; entropy = log l - log(2) e / l.  A larger m rescales both.  d is one multiply-add, of s with the rounded product of m: what its rounding moved all d by is taken out of
 // the sums at the end; of scores of 2^24 bits and more, where it would move d by whole bits, d is (s - m) log2(e) / temperature as it stands.  Parts (m, l, e) are joined in a fixed order, so results do not depend on how CTAs are scheduled.  An entry of -inf counts as a score so low that 2^d is 0 and d is finite;
 // where m itself is that low, d is cut at -10,000 instead.  NaN and +inf reach the sums and make them NaN.
-// Bound by HBM with 32 bits (1,000 x 1M 584 us, 6.8 TB/s), by the issue of five instructions and an exponential for an entry with 16 (369 us, 5.4 TB/s, 325 of them without the k largest;
-// a pass of eight instructions 579). 10,000 lists of 18,000 float32 211 us, 148 without the k largest: what follows the pass is waits.
+// Bound by HBM with 32 bits (1,000 x 1M 584 us, 6.8 TB/s).  With 16, five instructions and an exponential for an entry: HBM, issue and exponentials are at half each, with a quarter of the warps
+// that an SM could hold (380 to 400 us, 5.2 TB/s; without the k largest 45 us less; a pass of eight instructions 579).  10,000 lists of 18,000 float32 205 us of 225 (the rest: targets that are in
+// no list), 60 less without the k largest: what follows the pass is waits.
 //
 // The k largest: the pass leaves the largest entry of each thread and of each chunk behind.  The k-th largest of the threads' is a bound that at least k entries reach, and hardly more do (of 1M
 // drawn at random and 256 threads about k + 1): only chunks that reach it are read again, and the entries that do are sorted, by score and then by place.  Where more entries are alike than
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __r
 }
 
 // ------------------------------------------------------------------------------------------
-// Gradient.  Bound by HBM: 1,000 x 200,003 bfloat16 151 us (5.3 TB/s, half of it written), float32 266 (6.0); rows of scores and gradient that begin differently 300 and 361.  Two loads of a thread
+// Gradient.  Bound by HBM and issue (59 and 74 %): 1,000 x 200,003 bfloat16 151 us (5.3 TB/s, half of it written), float32 266 (6.0); rows of scores and gradient that begin differently 300 and 361.  Two loads of a thread
 // in flight and six CTAs an SM: four loads and the four CTAs that they leave room for took 174 and 289.
 // ------------------------------------------------------------------------------------------
 struct LpBackward {

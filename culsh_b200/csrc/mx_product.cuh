@@ -27,7 +27,7 @@ constexpr int MXP_OUT_BYTES = 8192;  // 32 queries by 256 bytes
 
 // More than 64 queries; the same of 1,024 values and more; up to 64; up to 16.
 // With more queries, loads in flight and warps of epilogue share the SM: short rows wait for the scores to be stored (1,000 x 1M x 128 cosines: twelve warps 432 us, eight 507), long ones
-// for L2 (4,099 x 32,771 x 2,048: twelve warps and 102 KB of stages 244 us, eight and 136 KB 211, four and 170 KB 203).  The scores of 1,000 x 1M x 128 are written at 4.5 TB/s in bfloat16 and
+// for their loads and MMAs in turn, no unit above 37 % (4,099 x 32,771 x 2,048: twelve warps and 102 KB of stages 244 us, eight and 136 KB 211, four and 170 KB 203).  The scores of 1,000 x 1M x 128 are written at 4.5 TB/s in bfloat16 and
 // 5.3 in float32 (a fill of the memory: 3.9).  The fewer queries there are, the shorter is a unit, and the less of it the issuing warps and the epilogue can overlap: few queries have
 // two or four CTAs on an SM, which share its tensor memory (one query, 1M x 128 rows: one CTA with eight warps of epilogue 38 us, four 21; 11.6 at the copy's rate).
 enum MxpKind { MXP_MANY, MXP_LONG, MXP_FEW, MXP_FEWEST };

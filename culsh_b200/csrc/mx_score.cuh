@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(256) mx_score_kernel(const T* __restrict__ Q, 
 // lost (and no sum of such a query can pass float32, whatever the rows' scales).  The M side are 128 candidates of a list, whose codes
 // and scales are gathered by cp.async to where the MMAs take them, and the score is the sum of the accumulator's columns.  No code is unpacked by an instruction:
 // 180M candidates of 128 values 12.0 -> 3.7 ms.  Of 100,000 rows, which lie in L2, they take 2.5 ms: what a warp does for a
-// tile; of a million the gather takes longer: L2 gives 8 TB/s in pieces of 32 and 64 bytes, 174 bytes a candidate with its norm (3.1 ms without it).  Codes gathered by TMA took 3.4 ms
-// in either case.
+// tile; of a million the gather takes longer: 172 bytes a candidate from L2 in pieces of 32 and 64 bytes, 7.7 TB/s (3.1 ms without its norm), with L2's tags at 36 %, its sectors at
+// 22 and issue at 51: warps wait for gathers and for one another.  Codes gathered by TMA took 3.4 ms in either case.
 //
 // One persistent CTA per SM.  Warps 0 - 11 gather (four a stage), 12 loads slices, 13 - 18 issue MMAs (a tile each: what a warp does for one takes 1,300 cycles), 19 - 30 epilogue (four a tile).
 // All walk the same tiles: a CTA has those that begin in its share of the positions, where each list counts for 128 more than it has.

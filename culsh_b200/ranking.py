@@ -11,7 +11,8 @@ probabilities, and the entropy of the distribution; ``log_probs_backward`` is it
     best.top_ids, best.top_log_probs, best.entropy
 
 Results are torch tensors on the device of the rows.  Unlike the index's calls these run on torch's current stream and
-return when their work is queued.  In a graph, keep the Candidates that it reads.
+return when their work is queued.  In a graph, keep the Candidates that it reads.  Results are not part of autograd's graph: gradients come
+from ``log_probs_backward``.  Pairs (ids, offsets) have offsets from 0 to the number of ids.
 """
 from __future__ import annotations
 
