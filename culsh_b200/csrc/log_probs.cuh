@@ -33,7 +33,9 @@ constexpr int LP_LEAST_CHUNK = 512;
 constexpr int LP_MAX_K = 128;
 constexpr uint32_t LP_NO_PLACE = 0xFFFFFFFFu;
 constexpr float LP_FLOOR = -10000.f;
-constexpr int LP_LOOK = 1024;  // entries of a list that a warp of the gradient looks through by itself
+// Entries of a list that a warp of the gradient looks through by itself.  Of all lists together up to LP_ALONE, and up to 512 a list on average: all, and there is no second kernel (1,000 lists of
+// 200 15 us, 18 with it); of a matrix, rows of up to LP_ALONE_ROW, all together LP_ALONE_ALL: with more the registers that this takes tell.
+constexpr int LP_LOOK = 1024, LP_ALONE = 1 << 18, LP_ALONE_ROW = 1 << 14, LP_ALONE_ALL = 1 << 21;
 // Largest |lse| from which the gradient counts log p: the rounding of lse is an error of every p, of 4e-6 there.
 constexpr float LP_NEAR = 64.f;
 // Products of the largest score with c up to which d counts from the rounded product: that is half a bit off at most, and 2^d of the largest entry close to 1.
@@ -731,16 +733,24 @@ __device__ __forceinline__ bool lp_far(const LpBackward& b, int row) {
     const float lse = __ldg(b.lse + row);
     return fabsf(lse) > LP_NEAR && lse != -INFINITY;
 }
-// The entry that has the gradient of a row's log probability, or -1; by a warp.  `left`: of a long list, whose target is not where the search finds it, if it has it.
-__device__ __forceinline__ int64_t lp_given(const LpBackward& b, int row, int64_t begin, int64_t end, bool& left) {
+// Where the lse that is given is that of these scores but for its rounding, log p counts from the largest score.
+__device__ __forceinline__ void lp_count_from_largest(LpRowTerms& r, const LpPart& all, float inv_t) {
+    const float log_l = logf(all.l), lse = all.m * inv_t + log_l;
+    if (all.l > 0.f && (lse == r.lse || fabsf(lse - r.lse) <= 4.8e-7f * fabsf(lse))) {
+        r.base = all.m;
+        r.lse = log_l;
+    }
+}
+// The entry that has the gradient of a row's log probability, or -1; by a warp.  `left`: of a list of more than `look` entries, whose target is not where the search finds it, if it has it.
+__device__ __forceinline__ int64_t lp_given(const LpBackward& b, int row, int64_t begin, int64_t end, int64_t look, bool& left) {
     left = false;
     if (!b.f.targets || !b.g) return -1;
     int64_t at = LpFind(b.f, row, begin, end)(b.f);
     if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) {
-        left = end - begin > LP_LOOK;
+        left = end - begin > look;
         if (!left) {
             at = lp_first_named<2>(b.f.ids - b.f.rows.shift, begin, end, __ldg(b.f.targets + row), threadIdx.x & 31, 32);
-            const unsigned first = __reduce_min_sync(0xFFFFFFFFu, (unsigned)(at - begin));
+            const unsigned first = __reduce_min_sync(0xFFFFFFFFu, (unsigned)(at - begin));  // 32 bits are enough for the lists that are looked through here
             at = first < (unsigned)(end - begin) ? begin + first : -1;
         }
     }
@@ -835,25 +845,46 @@ __device__ __forceinline__ void lp_backward_span(const T* __restrict__ x, T* __r
     }
 }
 
+// Largest score and sums of a row, by a CTA.
+template <typename T>
+__device__ __forceinline__ LpPart lp_part_by_cta(const T* __restrict__ x, const LpBackward& b, int64_t begin, int64_t end, LpPart* s_parts) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float largest = 0.f;
+    const LpPart mine = lp_chunks<false>(x, begin / LP_CHUNK<T> + warp, (end + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, b.f.c, lane, largest, [](int64_t, float) {});
+    if (lane == 0) s_parts[warp] = mine;
+    __syncthreads();
+    LpPart all = s_parts[0];
+    for (int w = 1; w < LP_WARPS; ++w) all.join(s_parts[w], b.f.c);
+    return all;
+}
+
 // A CTA for a span of a matrix's row.
 template <typename T>
 constexpr int LP_ROW_SPAN = 4 * LP_THREADS * (16 / sizeof(T));
-template <bool ALIKE, typename T>
-__global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_rows_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+// ALONE: of short rows.  What a row that log_probs_backward_whole_kernel is there for needs to be looked at for, each span's CTA looks at by itself.
+template <bool ALIKE, bool ALONE, typename T>
+__global__ void __launch_bounds__(LP_THREADS, ALONE ? 3 : ALIKE ? 6 : 4) log_probs_backward_rows_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
     const int64_t row = blockIdx.x / (unsigned)b.units, begin = b.f.rows.begin((int)row), end = b.f.rows.end((int)row);
     const int64_t span = begin / LP_ROW_SPAN<T> + (blockIdx.x - (unsigned)row * (unsigned)b.units);
     const int64_t from = max(span * LP_ROW_SPAN<T>, begin), to = min((span + 1) * LP_ROW_SPAN<T>, end);
-    if (from >= to) return;
-    if (lp_far(b, (int)row)) return;
-    bool left;
-    const LpRowTerms r = lp_row_terms(x, b, (int)row, lp_given(b, (int)row, begin, end, left));
-    lp_backward_span<ALIKE, false>(x, out + (row * b.ldo - begin), r, b.f.inv_t, from, to, threadIdx.x, LP_THREADS);
+    const bool far = lp_far(b, (int)row);
+    if (from < to && (ALONE || !far)) {
+        bool left;
+        LpRowTerms r = lp_row_terms(x, b, (int)row, lp_given(b, (int)row, begin, end, LP_LOOK, left));
+        if constexpr (ALONE) {
+            if (far) {
+                __shared__ LpPart s_parts[LP_WARPS];
+                lp_count_from_largest(r, lp_part_by_cta(x, b, begin, end, s_parts), b.f.inv_t);
+            }
+        }
+        lp_backward_span<ALIKE, ALONE>(x, out + (row * b.ldo - begin), r, b.f.inv_t, from, to, threadIdx.x, LP_THREADS);
+    }
+    if (!ALONE && blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");  // what comes next waits for log_probs_backward_whole_kernel, too
 }
 
 // A warp for a span of all lists' positions, and for each list in it: what it has to know of a list takes longer than a short one.
-template <bool ALIKE, typename T>
-__global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_lists_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
+template <bool ALIKE, bool ALONE, typename T>
+__global__ void __launch_bounds__(LP_THREADS, ALONE ? 3 : ALIKE ? 6 : 4) log_probs_backward_lists_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int64_t n = (int64_t)blockIdx.x * LP_WARPS + (threadIdx.x >> 5);
     if (n >= b.units) return;
@@ -864,23 +895,31 @@ __global__ void __launch_bounds__(LP_THREADS, ALIKE ? 6 : 4) log_probs_backward_
         if (begin >= p1) break;
         const int64_t from = max(begin, p0), to = min(end, p1);
         if (from >= to) continue;
-        if (lp_far(b, row)) continue;
+        const bool far = lp_far(b, row);
+        if (!ALONE && far) continue;
         bool left;  // then as if it had no target; log_probs_backward_whole_kernel looks for that
-        const LpRowTerms r = lp_row_terms(x, b, row, lp_given(b, row, begin, end, left));
-        lp_backward_span<ALIKE, false>(x, out - rows.shift, r, b.f.inv_t, from, to, threadIdx.x & 31, 32);
+        LpRowTerms r = lp_row_terms(x, b, row, lp_given(b, row, begin, end, ALONE ? LP_ALONE : LP_LOOK, left));
+        if constexpr (ALONE) {
+            if (far) {
+                float largest = 0.f;
+                const LpPart all = lp_chunks<false>(x, begin / LP_CHUNK<T>, (end + LP_CHUNK<T> - 1) / LP_CHUNK<T>, 1, begin, end, b.f.c, threadIdx.x & 31, largest, [](int64_t, float) {});
+                lp_count_from_largest(r, all, b.f.inv_t);
+            }
+        }
+        lp_backward_span<ALIKE, ALONE>(x, out - rows.shift, r, b.f.inv_t, from, to, threadIdx.x & 31, 32);
     }
 }
 
 // Rows that have to be looked at as a whole, beside the kernel of the spans.  Rows whose lse is large, so that it says p only to its rounding (squared distances of bytes by a temperature of
 // 0.05: to 10 %), are left to this one: their log p counts from the largest score, as in the forward pass, with sums made again (1,000 x 200,003 bfloat16, all of them such rows, 450 us in place
 // of 157).  Long lists whose target is not where a search finds it are looked through; where it is found after all, the kernel of the spans is waited for and the list is done again.
-// (As CTAs of its launch this took registers from the spans: 186 us in place of 157; behind it 1,000 lists of 200 took 24 us, 17 beside.)
+// (As CTAs of its launch this took registers from the spans: 186 us in place of 157.)  Beside the spans of a matrix it is launched first, which is sooner, beside those of lists behind them.
 template <bool ALIKE, typename T>
 __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_backward_whole_kernel(const T* __restrict__ x, T* __restrict__ out, LpBackward b) {
     __shared__ int64_t s_target;
     __shared__ LpPart s_parts[LP_WARPS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a matrix's spans
     const LpRows& rows = b.f.rows;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // few rows have several CTAs each, which look through all of it and take their share of what follows
     const int share = (int)blockIdx.x % b.shares;
     lp_by_warps_then_ctas(
@@ -888,7 +927,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_backward_whole_kernel
         [&](int row) { return (b.f.ids && b.g && rows.end(row) - rows.begin(row) > LP_LOOK) || lp_far(b, row); },
         [&](int row) {
             bool left = lp_far(b, row);
-            if (!left) lp_given(b, row, rows.begin(row), rows.end(row), left);
+            if (!left) lp_given(b, row, rows.begin(row), rows.end(row), LP_LOOK, left);
             return left;
         },
         [&](int row) {
@@ -901,34 +940,21 @@ __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_backward_whole_kernel
                 if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) lp_find_in_any_order<8>(b.f, row, begin, end, s_target, LP_THREADS);
                 else if (threadIdx.x == 0) s_target = at;
             }
-            if (far) {
-                float largest = 0.f;
-                const LpPart mine = lp_chunks<false>(x, begin / LP_CHUNK<T> + warp, (end + LP_CHUNK<T> - 1) / LP_CHUNK<T>, LP_WARPS, begin, end, b.f.c, lane, largest, [](int64_t, float) {});
-                if (lane == 0) s_parts[warp] = mine;
-            }
             __syncthreads();
             if (!far) {
                 if (s_target < 0) {  // it has none, as has been taken for granted
                     __syncthreads();
                     return;
                 }
-                asm volatile("griddepcontrol.wait;" ::: "memory");
+                asm volatile("griddepcontrol.wait;" ::: "memory");  // for the spans of lists
             }
             LpRowTerms r = lp_row_terms(x, b, row, s_target);
-            if (far) {
-                LpPart all = s_parts[0];
-                for (int w = 1; w < LP_WARPS; ++w) all.join(s_parts[w], b.f.c);
-                const float log_l = logf(all.l), lse = all.m * b.f.inv_t + log_l;
-                if (all.l > 0.f && (lse == r.lse || fabsf(lse - r.lse) <= 4.8e-7f * fabsf(lse))) {  // it is that of these scores, but for its rounding
-                    r.base = all.m;
-                    r.lse = log_l;
-                }
-            }
+            if (far) lp_count_from_largest(r, lp_part_by_cta(x, b, begin, end, s_parts), b.f.inv_t);
             const int64_t each = ((end - begin) / b.shares / 16 + 1) * 16, from = begin + share * each;
             lp_backward_span<ALIKE, true>(x, rows.offsets ? out - rows.shift : out + ((int64_t)row * b.ldo - begin), r, b.f.inv_t, from, min(from + each, end), threadIdx.x, LP_THREADS);
             __syncthreads();
         });
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // what comes next waits for both
+    if (rows.offsets) asm volatile("griddepcontrol.wait;" ::: "memory");  // what comes next waits for both
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1016,18 +1042,34 @@ inline void log_probs_backward(const CtxPtr& c, const T* scores, T* out, LpBackw
     const int64_t mean = r.total / b.f.m;
     b.span = mean >= 1024 ? 512 : mean >= 64 ? 128 : 32;
     b.units = r.offsets ? (int64_t)ceil_div((size_t)(r.total + r.shift), (size_t)b.span) : r.cols / LP_ROW_SPAN<T> + 2;
-    b.whole = 4 * c->sm_count;
-    b.shares = 1;
-    while (b.shares < 16 && 2 * b.shares * ((b.f.m - 1) / LP_WARPS + 1) <= b.whole) b.shares *= 2;
-    b.whole = std::min((b.f.m - 1) / LP_WARPS + 1, b.whole / b.shares) * b.shares;
     const size_t grid = r.offsets ? ceil_div((size_t)b.units, LP_WARPS) : (size_t)b.units * b.f.m;
     if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "too many entries for one call");
     const bool alike = (((uintptr_t)(out - r.shift) | (r.offsets ? 0u : (uintptr_t)((b.ldo - r.ld) * (int64_t)sizeof(T)))) & 15u) == 0;
-    auto kern = r.offsets ? (alike ? log_probs_backward_lists_kernel<true, T> : log_probs_backward_lists_kernel<false, T>)
-                          : (alike ? log_probs_backward_rows_kernel<true, T> : log_probs_backward_rows_kernel<false, T>);
-    kern<<<(unsigned)grid, LP_THREADS, 0, stream>>>(scores - r.shift, out, b);
-    KERNEL_CHECK();
-    launch_beside(stream, alike ? log_probs_backward_whole_kernel<true, T> : log_probs_backward_whole_kernel<false, T>, (size_t)b.whole, LP_THREADS, scores - r.shift, out, b);
+    const T* const x = scores - r.shift;
+    auto by = [&](auto form) {
+        constexpr bool ALIKE = decltype(form)::value;
+        if (r.offsets ? mean <= 512 && r.total <= LP_ALONE : r.cols <= LP_ALONE_ROW && b.f.m * r.cols <= LP_ALONE_ALL) {
+            if (r.offsets) log_probs_backward_lists_kernel<ALIKE, true, T><<<(unsigned)grid, LP_THREADS, 0, stream>>>(x, out, b);
+            else log_probs_backward_rows_kernel<ALIKE, true, T><<<(unsigned)grid, LP_THREADS, 0, stream>>>(x, out, b);
+            KERNEL_CHECK();
+            return;
+        }
+        b.whole = 4 * c->sm_count;
+        b.shares = 1;
+        while (b.shares < 16 && 2 * b.shares * ((b.f.m - 1) / LP_WARPS + 1) <= b.whole) b.shares *= 2;
+        b.whole = std::min((b.f.m - 1) / LP_WARPS + 1, b.whole / b.shares) * b.shares;
+        if (r.offsets) {
+            log_probs_backward_lists_kernel<ALIKE, false, T><<<(unsigned)grid, LP_THREADS, 0, stream>>>(x, out, b);
+            KERNEL_CHECK();
+            launch_beside(stream, log_probs_backward_whole_kernel<ALIKE, T>, (size_t)b.whole, LP_THREADS, x, out, b);
+        } else {
+            log_probs_backward_whole_kernel<ALIKE, T><<<(unsigned)b.whole, LP_THREADS, 0, stream>>>(x, out, b);
+            KERNEL_CHECK();
+            launch_beside(stream, log_probs_backward_rows_kernel<ALIKE, false, T>, grid, LP_THREADS, x, out, b);
+        }
+    };
+    if (alike) by(std::true_type());
+    else by(std::false_type());
 }
 
 }  // namespace culsh_b200

@@ -82,7 +82,7 @@ def mixed(lengths, n, order, seed):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("order", ["last", "down", "any"])
 @pytest.mark.parametrize("lengths", [[31, 0, 32, 33, 64, 1, 65, 0, 2, 129, 1000, 2050, 7], [64] * 600, [50_000, 0, 3, 70_001], [300_000] + [40] * 2000, [40] * 9 + [3] * 20_000,
-                                     [3000] * 200, [20_000] * 300])
+                                     [3000] * 200, [20_000] * 300, [100_000] + [3] * 1000])
 def test_targets_of_lists_in_any_order(culsh, lengths, order, dtype):
     n, temperature = 3 * max(lengths), 0.5
     all_ids, offsets = mixed(lengths, n, order, 5)
@@ -425,3 +425,29 @@ def test_cosines_of_rows_of_any_length(culsh, d, nq):
     check(rows.product(held, metric="cosine"), held.dequantize(torch.float64))
     for scores in few_and_many(rows, Q, 66, "cosine"):
         check(scores, Q.double())
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.05])
+@pytest.mark.parametrize("lengths", [[100_000] + [3] * 1000, [3] * 40 + [1] + [5000] * 30, [400_000, 7, 0, 2_000] + [30] * 900])
+def test_gradient_of_large_scores_of_uneven_lists(culsh, lengths, temperature):
+    """Targets in no order, in some lists not there, scores around squared distances of bytes in every other list."""
+    m, n = len(lengths), 3 * max(lengths)
+    ids, offsets = mixed(lengths, n, "any", 9)
+    ends, total = offsets.tolist(), ids.shape[0]
+    owner = torch.repeat_interleave(torch.arange(m, device="cuda"), torch.tensor(lengths, device="cuda"))
+    s = 3 * temperature * torch.randn(total, generator=gen(1), device="cuda") - torch.where(owner % 2 == 0, 2.0e5, 0.0)
+    at = [(7 * i + 3) % k if k else 0 for i, k in enumerate(lengths)]
+    mine = ids.cpu()[(offsets[:-1].cpu() + torch.tensor(at)).clamp(max=total - 1)].tolist()
+    t = torch.tensor([n + 1 if i % 5 == 4 or not lengths[i] else v for i, v in enumerate(mine)], device="cuda")
+    gl, ge = torch.randn(m, generator=gen(6), device="cuda"), torch.randn(m, generator=gen(7), device="cuda")
+    r = culsh.log_probs(s, t, (ids, offsets), temperature=temperature)
+    got = culsh.log_probs_backward(s, t, r.lse, r.entropy, gl, ge, (ids, offsets), temperature).double().cpu().numpy()
+    z = s.double().cpu().numpy()
+    for i in list(range(min(m, 45))) + [m - 2, m - 1]:
+        if not lengths[i]:
+            continue
+        one = z[ends[i]:ends[i + 1]]
+        a, h = float(gl[i]), float(ge[i])
+        want = gradient_of((one - one.max()) / temperature, None if int(t[i]) > n else at[i], a, h, temperature)
+        bound = 8 * ULP * 64 * (abs(a) + 64 * abs(h)) / temperature + HALF_ULP[torch.float32] * np.abs(want)
+        assert np.all(np.abs(got[ends[i]:ends[i + 1]] - want) <= bound), i
