@@ -41,15 +41,25 @@ constexpr float LP_NEAR = 64.f;
 // Products of the largest score with c up to which d counts from the rounded product: that is half a bit off at most, and 2^d of the largest entry close to 1.
 constexpr float LP_SHORT = 16777216.f;
 
+// What a kernel in front may have written: by L2 in a kernel that is launched EARLY, else by L1 (gradient of 1,000 lists of 18,000 51 us, 55 by L2;
+// of 600,000 entries and 700 lists of two 97 and 113).
+template <bool EARLY, typename T>
+__device__ __forceinline__ T lp_get(const T* p) {
+    if constexpr (EARLY) return __ldcg(p);
+    else return __ldg(p);
+}
+
 // Where rows are: a matrix with rows `ld` apart and `cols` long, or lists.  Positions of row r: [begin, end).
 struct LpRows {
     const int64_t* offsets;
     int64_t ld, cols, shift, total;  // shift: entries between the boundary and the array; total: entries of all lists
+    template <bool EARLY = false>
     __device__ __forceinline__ int64_t begin(int r) const {
-        return (offsets ? min(max(__ldcg(offsets + r), (int64_t)0), total) : (int64_t)r * ld) + shift;
+        return (offsets ? min(max(lp_get<EARLY>(offsets + r), (int64_t)0), total) : (int64_t)r * ld) + shift;
     }
+    template <bool EARLY = false>
     __device__ __forceinline__ int64_t end(int r) const {
-        return offsets ? max(min(__ldcg(offsets + r + 1), total) + shift, begin(r)) : (int64_t)r * ld + cols + shift;
+        return offsets ? max(min(lp_get<EARLY>(offsets + r + 1), total) + shift, begin<EARLY>(r)) : (int64_t)r * ld + cols + shift;
     }
 };
 
@@ -393,15 +403,16 @@ __device__ __forceinline__ float lp_bound(LpShared<TH>& sh, float mine, int k) {
 
 // Position of the entry that a target names in a row, or -1 where it does not stand where ascending ids would have it; by one warp.  The first 32 ids that it looks at (all, where there
 // are no more) can be asked for long before.
+template <bool EARLY = false>
 struct LpFind {
     int64_t lo, hi, step, target;  // ids below lo are smaller, at and behind hi larger
     int32_t id;
     __device__ __forceinline__ void probe(const int32_t* __restrict__ ids) {
         step = (hi - lo + 31) / 32;
         const int64_t p = lo + (threadIdx.x & 31) * step;
-        id = p < hi ? __ldcg(ids + p) : 0x7FFFFFFF;
+        id = p < hi ? lp_get<EARLY>(ids + p) : 0x7FFFFFFF;
     }
-    __device__ __forceinline__ LpFind(const LpArgs& a, int row, int64_t begin, int64_t end) : lo(begin), hi(end), step(1), target(__ldcg(a.targets + row)), id(0) {
+    __device__ __forceinline__ LpFind(const LpArgs& a, int row, int64_t begin, int64_t end) : lo(begin), hi(end), step(1), target(lp_get<EARLY>(a.targets + row)), id(0) {
         if (a.ids && hi > lo) probe(a.ids - a.rows.shift);
     }
     __device__ __forceinline__ int64_t operator()(const LpArgs& a) {
@@ -566,7 +577,7 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_places_kernel(LpArgs a) 
     lp_by_warps_then_ctas(
         a.m, blockIdx.x, gridDim.x, [](int) { return true; },
         [&](int row) {
-            const int64_t begin = a.rows.begin(row), end = a.rows.end(row), at = LpFind(a, row, begin, end)(a);
+            const int64_t begin = a.rows.begin(row), end = a.rows.end(row), at = LpFind<>(a, row, begin, end)(a);
             if ((threadIdx.x & 31) == 0) places[row] = at < 0 ? LP_NO_PLACE : (uint32_t)(at - begin);
             return at < 0 && lp_may_be_left(begin, end);
         },
@@ -599,7 +610,7 @@ __global__ void __launch_bounds__(TH) log_probs_row_kernel(const T* __restrict__
     LpPart mine;
     float largest = -INFINITY;
     if (warp == TH / 32 - 1 && a.targets && !a.placed) {  // the warp with the fewest chunks
-        LpFind find(a, row, begin, end);
+        LpFind<> find(a, row, begin, end);
         mine = lp_chunks<false>(x, first + warp, last, TH / 32, begin, end, a.c, lane, largest, leave);
         const int64_t at = find(a);
         if (lane == 0) sh.target = at;
@@ -629,16 +640,16 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_unit_kernel(const T* __r
         int lo = 0, hi = a.m;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (lp_slot(a, mid, a.rows.begin(mid), a.unit, 0) <= (int64_t)blockIdx.x) lo = mid;
+            if (lp_slot(a, mid, a.rows.begin<true>(mid), a.unit, 0) <= (int64_t)blockIdx.x) lo = mid;
             else hi = mid;
         }
         row = lo;
-        nth = (int64_t)blockIdx.x - lp_slot(a, row, a.rows.begin(row), a.unit, 0);
+        nth = (int64_t)blockIdx.x - lp_slot(a, row, a.rows.begin<true>(row), a.unit, 0);
     } else {
         row = (int)(blockIdx.x / (unsigned)a.units_per_row);
         nth = blockIdx.x - (unsigned)row * (unsigned)a.units_per_row;
     }
-    const int64_t begin = a.rows.begin(row), end = a.rows.end(row);
+    const int64_t begin = a.rows.begin<true>(row), end = a.rows.end<true>(row);
     const int64_t from = max((begin / a.unit + nth) * a.unit, begin), to = min((begin / a.unit + nth + 1) * a.unit, end);
     if (from >= to) return;
     const int64_t slot = lp_slot(a, row, begin, LP_CHUNK<T>, lp_chunks_per_row<T>(a)), first = begin / LP_CHUNK<T>;
@@ -655,9 +666,9 @@ __global__ void __launch_bounds__(LP_THREADS) log_probs_join_kernel(const T* __r
     behind_kernel_before(x, before);
     __shared__ LpShared<LP_THREADS> sh;
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t begin = a.rows.begin(row), end = a.rows.end(row);
+    const int64_t begin = a.rows.begin<true>(row), end = a.rows.end<true>(row);
     if (warp == 0 && a.targets) {
-        const int64_t at = LpFind(a, row, begin, end)(a);
+        const int64_t at = LpFind<true>(a, row, begin, end)(a);
         if (lane == 0) sh.target = at;
     }
     const int64_t units = end > begin ? (end - 1) / a.unit - begin / a.unit + 1 : 0, slot = lp_slot(a, row, begin, a.unit, a.units_per_row);
@@ -745,7 +756,7 @@ __device__ __forceinline__ void lp_count_from_largest(LpRowTerms& r, const LpPar
 __device__ __forceinline__ int64_t lp_given(const LpBackward& b, int row, int64_t begin, int64_t end, int64_t look, bool& left) {
     left = false;
     if (!b.f.targets || !b.g) return -1;
-    int64_t at = LpFind(b.f, row, begin, end)(b.f);
+    int64_t at = LpFind<>(b.f, row, begin, end)(b.f);
     if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) {
         left = end - begin > look;
         if (!left) {
@@ -936,7 +947,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_backward_whole_kernel
             __syncthreads();
             const bool far = lp_far(b, row);
             if (b.f.targets && b.g) {
-                const int64_t at = far ? LpFind(b.f, row, begin, end)(b.f) : -1;  // the same in all warps; of the others it is known
+                const int64_t at = far ? LpFind<>(b.f, row, begin, end)(b.f) : -1;  // the same in all warps; of the others it is known
                 if (at < 0 && b.f.ids && lp_may_be_left(begin, end)) lp_find_in_any_order<8>(b.f, row, begin, end, s_target, LP_THREADS);
                 else if (threadIdx.x == 0) s_target = at;
             }

@@ -75,7 +75,10 @@ def test_kernels_launched_early_read_by_l2():
     rows, score, lp = (Functions(f) for f in ("mx_rows.cuh", "mx_score.cuh", "log_probs.cuh"))
     used = [rows["EightOf"], rows["mx_quantize_kernel"], score["mx_slices_kernel"]]
     used += [lp[n] for n in ("LpRows", "lp_load", "lp_chunks", "LpFind", "lp_first_named", "lp_find_in_any_order", "lp_finish", "log_probs_unit_kernel", "log_probs_join_kernel")]
-    assert "EARLY ? __ldcg(x + p) : x[p]" in lp["lp_load"] and "<false" not in lp["log_probs_unit_kernel"] + lp["log_probs_join_kernel"]
+    early = lp["log_probs_unit_kernel"] + lp["log_probs_join_kernel"]
+    assert "EARLY ? __ldcg(x + p) : x[p]" in lp["lp_load"] and "<false" not in early and "LpFind<>" not in early
+    assert not re.search(r"\.(?:begin|end)\(", early) and early.count("rows.begin<true>(") >= 4
+    assert re.search(r"if constexpr \(EARLY\) return __ldcg\(p\);", lp["lp_get"])
     for body in used:
         body = body.replace("EARLY ? __ldcg(x + p) : x[p]", "")
         assert "__ldg" not in body
