@@ -370,7 +370,8 @@ int culsh_log_probs(culsh_handle* h, const void* scores, int type, int m, int64_
                     float* entropy, float* lse, float* top_log_probs, int32_t* top_ids, void* workspace,
                     uint64_t workspace_bytes, void* stream);
 /* grad_scores ([m][cols], rows ld_grad apart, or as the lists; the scores' type) from the gradients of log_probs
- * and entropy (either may be NULL) and what the forward call returned.  A log probability of -inf has
+ * and entropy (either may be NULL) and what the forward call returned.  Where |lse| is above 64 and that of these scores
+ * but for its rounding, which would be an error of every p, p comes from the scores alone.  A log probability of -inf has
  * no gradient, nor has an entry of -inf. */
 int culsh_log_probs_backward(culsh_handle* h, const void* scores, int type, int m, int64_t cols, int64_t ld,
                              const int64_t* offsets, const int32_t* ids, int64_t total, double temperature,

@@ -82,7 +82,7 @@ def mixed(lengths, n, order, seed):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("order", ["last", "down", "any"])
 @pytest.mark.parametrize("lengths", [[31, 0, 32, 33, 64, 1, 65, 0, 2, 129, 1000, 2050, 7], [64] * 600, [50_000, 0, 3, 70_001], [300_000] + [40] * 2000, [40] * 9 + [3] * 20_000,
-                                     [3000] * 200, [20_000] * 300, [100_000] + [3] * 1000])
+                                     [3000] * 200, [20_000] * 300, [100_000] + [3] * 1000, [70_000, 90_001, 80_002]])
 def test_targets_of_lists_in_any_order(culsh, lengths, order, dtype):
     n, temperature = 3 * max(lengths), 0.5
     all_ids, offsets = mixed(lengths, n, order, 5)
@@ -451,3 +451,33 @@ def test_gradient_of_large_scores_of_uneven_lists(culsh, lengths, temperature):
         want = gradient_of((one - one.max()) / temperature, None if int(t[i]) > n else at[i], a, h, temperature)
         bound = 8 * ULP * 64 * (abs(a) + 64 * abs(h)) / temperature + HALF_ULP[torch.float32] * np.abs(want)
         assert np.all(np.abs(got[ends[i]:ends[i + 1]] - want) <= bound), i
+
+
+@pytest.mark.parametrize("lengths", [[20_000] * 50, [700] * 30, [90_000] * 3])
+def test_lists_in_a_graph(culsh, lengths):
+    """Kernels that begin beside the one in front of them, replayed on changing scores and targets."""
+    m, total = len(lengths), sum(lengths)
+    ids, offsets = mixed(lengths, 3 * max(lengths), "any", 1)
+    s, t = torch.randn(total, generator=gen(1), device="cuda"), ids[offsets[:-1] + 5].long()
+    gl = torch.randn(m, generator=gen(2), device="cuda")
+
+    def step():
+        r = culsh.log_probs(s, t, (ids, offsets), top_k=4, temperature=0.1)
+        return r.lse, r.entropy, r.log_probs, r.top_ids, culsh.log_probs_backward(s, t, r.lse, r.entropy, gl, gl, (ids, offsets), 0.1)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in range(3):
+        s.copy_(torch.randn(total, generator=gen(seed + 5), device="cuda") - (2e5 if seed == 2 else 0))
+        t.copy_(torch.where(torch.arange(m, device="cuda") % 3 == seed, 10 ** 9, ids[offsets[:-1] + 7 * seed + 1].long()))
+        graph.replay()
+        torch.cuda.synchronize()
+        first = [x.clone() for x in got]
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(first, want))
+        assert bool(torch.isfinite(want[2]).any()) and bool((want[2] == -math.inf).any())
