@@ -24,15 +24,19 @@ if not _building:
     from .rp_lsh import RPLSH, RPLSHModel  # noqa: E402
 
     __all__ = ["RPLSH", "RPLSHModel", "MinHashLSH", "MinHashLSHModel", "PStableLSH", "PStableLSHModel",
-               "Candidates", "MXRows", "LogProbs", "log_probs", "log_probs_backward", "rank"]
+               "Candidates", "MXRows", "Int8Rows", "LogProbs", "log_probs", "log_probs_backward", "rank",
+               "CrossEntropy", "cross_entropy", "cross_entropy_backward"]
 
-    # the ranking layer works on torch tensors; it is imported when one of its names is first used, so that programs that only
+    # the ranking layer and the loss work on torch tensors; they are imported when one of their names is first used, so that programs that only
     # build and query indexes do not import torch
-    _RANKING = ("MXRows", "LogProbs", "log_probs", "log_probs_backward", "rank")
+    _RANKING = ("MXRows", "Int8Rows", "LogProbs", "log_probs", "log_probs_backward", "rank")
+    _LOSS = ("CrossEntropy", "cross_entropy", "cross_entropy_backward")
 
     def __getattr__(name):
-        if name in _RANKING:
-            from . import ranking
-            globals().update((n, getattr(ranking, n)) for n in _RANKING)
-            return globals()[name]
+        for names, module in ((_RANKING, "ranking"), (_LOSS, "loss")):
+            if name in names:
+                from importlib import import_module
+                found = import_module("." + module, __name__)
+                globals().update((n, getattr(found, n)) for n in names)
+                return globals()[name]
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

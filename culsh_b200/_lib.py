@@ -110,6 +110,14 @@ SIGNATURES = {
     "culsh_log_probs_workspace": [VP, I, I, I64, I, I64, C.POINTER(C.c_uint64)],
     "culsh_log_probs": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, I, VP, VP, VP, VP, VP, VP, U64, VP],
     "culsh_log_probs_backward": [VP, VP, I, I, I64, I64, VP, VP, I64, C.c_double, VP, VP, VP, VP, VP, VP, I64, VP],
+    "culsh_i8_quantize": [VP, VP, I, I, I, I64, VP, VP, VP, VP],
+    "culsh_i8_dequantize": [VP, VP, VP, I, I, VP, I, VP],
+    "culsh_i8_product": [VP, VP, VP, VP, I, VP, VP, VP, I, I, I, VP, I, I64, VP],
+    "culsh_i8_product_dense": [VP, VP, I, I, I64, VP, VP, VP, I, I, I, VP, I, I64, VP, U64, VP],
+    "culsh_i8_score": [VP, VP, I, I, I64, VP, VP, VP, I, I, I, VP, VP, I64, VP, VP, U64, VP],
+    "culsh_cross_entropy_workspace": [VP, VP, I64, VP, I64, I, I, I, I, I, I, C.POINTER(C.c_uint64)],
+    "culsh_cross_entropy": [VP, VP, I64, VP, I64, I, I, I, I, VP, VP, C.c_double, VP, VP, VP, VP, U64, VP],
+    "culsh_cross_entropy_backward": [VP, VP, I64, VP, I64, I, I, I, I, VP, VP, C.c_double, VP, VP, VP, VP, VP, VP, I64, VP, I64, VP, U64, VP],
 }
 _VOID = {"culsh_index_free": [VP], "culsh_candidates_free": [VP]}
 _CHARP = {"culsh_last_error": []}

@@ -12,7 +12,7 @@ import sys
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRCS = [os.path.join(HERE, "csrc", f) for f in ("culsh_b200.cu", "ranking.cu")]
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("culsh_b200.cu", "ranking.cu", "int8.cu", "cross_entropy.cu")]
 OBJECTS = os.path.join(os.path.dirname(HERE), "build")
 OUT = os.path.join(HERE, "libculsh_b200.so")
 

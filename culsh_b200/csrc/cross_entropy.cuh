@@ -1,0 +1,760 @@
+// Softmax cross entropy of queries over every row, whose scores are not kept, and its gradient.
+//
+//   z_ij = q_i . x_j / T + b_j      lse_i = log sum_j exp(z_ij)      loss_i = lse_i - z_i,t(i)
+//   G_ij = (g_i + e_i) p_ij - g_i [j = t(i)],  p = exp(z - lse)      dQ = G X / T      dX = G^T Q / T
+//
+// with g and e the gradients that come from the losses and from lse.  Everything is taken in powers of two: c = log2(e) / T and b log2(e).
+//
+// Forward: products on the tensor cores (tc_gemm.cuh), queries on the M side, so that a thread holds neighbouring scores of one query and keeps the running maximum and sum of
+// a block of rows by itself; blocks are joined in 64 bits.  lse comes as two floats, of which the second is what the first leaves: a score of a thousand would leave p an error of 2^-14 otherwise.
+//
+// Backward: rows in pieces whose G fits L2; for each, G once more from the products, and two products with it.  The target's own entry stays out of G: where p is near 1 it is a small
+// difference, and where it is not, it outweighs the rest and so would its rounding to 16 bits; its coefficient g expm1(-loss) + e exp(-loss) is taken in 32 bits, and times the row or the
+// query added to the sums.  Sums of one row's gradient over its queries are taken in ascending order: nothing depends on the order of atomics.
+//
+// 32-bit floats are held as three bfloat16 planes each (24 bits), products as six of 16 bits; G of 32-bit inputs likewise.  G of half precision is scaled by a power of two that brings the
+// largest coefficient to 2^15, so that p down to 2^-39 of it is there.
+#pragma once
+
+#include <type_traits>
+
+#include "tc_gemm.cuh"
+
+namespace culsh_b200 {
+
+constexpr float CE_LOG2E = 1.4426950408889634f;
+constexpr int CE_BN = 256, CE_HALF = CE_BN / 2;
+constexpr int CE_SEGMENT = 8;  // steps of 64
+
+template <typename T>
+__device__ __forceinline__ float ce_float(T v) { return (float)v; }
+__device__ __forceinline__ float ce_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct CeScoreArgs {
+    int* d_error;
+    unsigned units;
+    uint32_t idesc;
+    int m, kb;                // queries; steps of K
+    int n0, n1;               // rows of this call
+    int block, tiles_q;       // tiles of rows in a unit, tiles of queries
+    unsigned tiles_n;
+    float c;
+    const float* bias;        // of the rows, in powers of two, or NULL
+    const int64_t* targets;   // (forward) of the queries, or -1
+    // forward
+    float2* partial;          // [m][slots]: reference and sum
+    int slots;
+    float* target_scores;     // [m]
+    // gradient
+    const float* terms;       // [m] what goes to the exponent: -lse
+    const float* factors;     // [m] what p is multiplied by
+    const uint32_t* amax;     // largest magnitude among the factors, as bits (half precision only)
+    const int* target_cols;   // [m] or -1
+    void* G;                  // [planes][m][pitch]
+    int64_t pitch, plane;
+};
+
+struct CeUnit {
+    int m0, tile0, tiles, k0, k1, block;
+    __device__ __forceinline__ CeUnit(const CeScoreArgs& a, unsigned u) {
+        block = (int)(u / (unsigned)a.tiles_q);
+        m0 = (int)(u - (unsigned)block * a.tiles_q) * TG_M;
+        tile0 = block * a.block;
+        tiles = min(a.block, (int)a.tiles_n - tile0);
+        k0 = 0, k1 = a.kb;
+    }
+};
+
+template <int PLANES, bool SEGMENTS>
+struct CeScoreBase {
+    static constexpr bool A_MN = false, B_MN = false, I8 = false, HALVES = true;
+    static constexpr int BN = CE_BN, SEGMENT = SEGMENTS ? CE_SEGMENT : 0;
+    static constexpr int EPI_BYTES = TG_EPI_WARPS * (BN / 2) * 4;
+    using Pairs = PlanePairs<PLANES>;
+    using Args = CeScoreArgs;
+    using Unit = CeUnit;
+    static __device__ __forceinline__ void load(const Args& a, const Unit& u, int t, int pa, int pb, int k, const CUtensorMap* ta, const CUtensorMap* tb, unsigned char* sa,
+                                                unsigned char* sb, uint64_t* bar) {
+        tma_load_3d(sa, ta, bar, k * 64, u.m0, pa);
+        tma_load_3d(sb, tb, bar, k * 64, a.n0 + (u.tile0 + t) * BN, pb);
+    }
+    static __device__ __forceinline__ int n_mma(const Args& a, const Unit& u, int t) { return min(BN, (a.n1 - a.n0 - (u.tile0 + t) * BN + 15) & ~15); }
+};
+
+// The rows' terms of half a tile, for one warp.
+__device__ __forceinline__ void ce_bias_tile(const float* bias, int n0, int n1, float* s, int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int i = lane; i < CE_HALF; i += 32) s[i] = n0 + i < n1 ? __ldcg(bias + n0 + i) : 0.f;
+    __syncwarp();
+}
+
+// The sums of a tile's segments, for a thread's 128 columns of one lane.
+template <bool SEGMENTS>
+struct CeSums {
+    float v[SEGMENTS ? CE_HALF : 1];
+    __device__ __forceinline__ void segment(const CeScoreArgs&, bool first, uint32_t taddr, bool live) {
+        if constexpr (SEGMENTS) {
+#pragma unroll
+            for (int c0 = 0; c0 < CE_HALF; c0 += 16) {
+                uint32_t r[16];
+                tc_ld16(taddr + c0, r);
+                tc_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[c0 + j] = !live ? __int_as_float(0x7FFFFFFF) : first ? __uint_as_float(r[j]) : v[c0 + j] + __uint_as_float(r[j]);
+            }
+        }
+    }
+    // 32 columns from c0 on, where the last segment has been added.
+    __device__ __forceinline__ void read(uint32_t taddr, int c0, bool live, uint32_t (&r)[32]) {
+        if constexpr (SEGMENTS) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(v[c0 + j]);
+        } else {
+            tg_read(taddr + c0, live, r);
+        }
+    }
+};
+
+template <int PLANES, bool BIAS, bool SEGMENTS>
+struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS> {
+    struct Epilogue : CeSums<SEGMENTS> {
+        int q, quarter, group, lane, target;
+        bool idle;
+        float ref, sum;
+        float* s_bias;
+        __device__ __forceinline__ Epilogue(const CeScoreArgs&, unsigned char* smem, int warp, int quarter_, int group_, int lane_)
+            : quarter(quarter_), group(group_), lane(lane_), s_bias(reinterpret_cast<float*>(smem) + warp * CE_HALF) {}
+        __device__ __forceinline__ void unit_begin(const CeScoreArgs& a, const CeUnit& u) {
+            q = u.m0 + quarter * 32 + lane;
+            idle = q - lane >= a.m;
+            ref = -INFINITY, sum = 0.f;
+            const int64_t t = q < a.m && a.targets ? __ldcg(a.targets + q) : -1;
+            target = t < 0 || t >= a.n1 ? -1 : (int)t;
+        }
+        __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more) {
+            if (idle) return;
+            if (SEGMENTS) this->segment(a, !more, taddr, live);
+            const int n0 = a.n0 + (u.tile0 + t) * CE_BN + group * CE_HALF;
+            if (BIAS) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
+#pragma unroll(SEGMENTS ? CE_HALF / 32 : 1)
+            for (int c0 = 0; c0 < CE_HALF; c0 += 32) {
+                const int left = a.n1 - n0 - c0;
+                if (left <= 0) break;
+                uint32_t r[32];
+                this->read(taddr, c0, live, r);
+                const int at = target - (n0 + c0);
+                if (__any_sync(0xFFFFFFFFu, (unsigned)at < 32u)) {
+                    float v = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j == at) v = __uint_as_float(r[j]);
+                    if ((unsigned)at < 32u) a.target_scores[q] = v;
+                }
+                float x[32], top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    x[j] = __uint_as_float(r[j]);
+                    if (BIAS) {  // a row that is masked may hold anything
+                        const float b = s_bias[c0 + j];
+                        x[j] = b == -INFINITY ? b : fmaf(x[j], a.c, b);
+                    }
+                    if (j >= left) x[j] = -INFINITY;
+                    top = fmaxf(top, x[j]);
+                }
+                const float next = fmaxf(ref, BIAS ? top : top * a.c), base = next == -INFINITY ? 0.f : next;
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < 32; ++j) part[j & 3] += ce_exp2(BIAS ? x[j] - base : fmaf(x[j], a.c, -base));
+                sum = fmaf(sum, ce_exp2(ref - base), (part[0] + part[1]) + (part[2] + part[3]));
+                ref = next;
+            }
+        }
+        __device__ __forceinline__ void unit_end(const CeScoreArgs& a, const CeUnit& u) {
+            if (q < a.m) a.partial[(int64_t)q * a.slots + u.block * 2 + group] = make_float2(ref, sum);
+        }
+    };
+};
+
+// What a power of two brings the largest factor to [2^14, 2^15].
+__device__ __forceinline__ int ce_scale_exponent(const uint32_t* amax) {
+    const uint32_t bits = amax ? __ldcg(amax) : 0u;
+    return bits == 0u ? 0 : min(max(14 + 127 - (int)(bits >> 23), -100), 100);
+}
+
+template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS>
+struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS> {
+    struct Epilogue : CeSums<SEGMENTS> {
+        int q, quarter, group, lane, target;
+        bool idle;
+        float term, factor;
+        float* s_bias;
+        __device__ __forceinline__ Epilogue(const CeScoreArgs&, unsigned char* smem, int warp, int quarter_, int group_, int lane_)
+            : quarter(quarter_), group(group_), lane(lane_), s_bias(reinterpret_cast<float*>(smem) + warp * CE_HALF) {}
+        __device__ __forceinline__ void unit_begin(const CeScoreArgs& a, const CeUnit& u) {
+            q = u.m0 + quarter * 32 + lane;
+            idle = q - lane >= a.m;
+            const bool in = q < a.m;
+            term = in ? __ldcg(a.terms + q) : 0.f;
+            factor = in ? __ldcg(a.factors + q) : 0.f;
+            target = in ? __ldcg(a.target_cols + q) : -1;
+            if (HALF) factor = ldexpf(factor, ce_scale_exponent(a.amax));
+        }
+        __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more) {
+            if (idle) return;
+            if (SEGMENTS) this->segment(a, !more, taddr, live);
+            const int first = (u.tile0 + t) * CE_BN + group * CE_HALF, n0 = a.n0 + first;
+            if (BIAS) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
+            uint16_t* const out = reinterpret_cast<uint16_t*>(a.G) + (int64_t)q * a.pitch + first;
+#pragma unroll(SEGMENTS ? CE_HALF / 32 : 1)
+            for (int c0 = 0; c0 < CE_HALF; c0 += 32) {
+                const int left = a.n1 - n0 - c0;  // behind the last row G has zeros
+                uint32_t r[32];
+                this->read(taddr, c0, live, r);
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float s = __uint_as_float(r[j]);
+                    v[j] = ce_exp2(fmaf(s, a.c, BIAS ? term + s_bias[c0 + j] : term)) * factor;
+                    if (j >= left) v[j] = 0.f;
+                }
+                const int at = target - (n0 + c0);
+                if (__any_sync(0xFFFFFFFFu, (unsigned)at < 32u)) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j == at) v[j] = 0.f;
+                }
+                if (q < a.m) {
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            if (HALF) {
+                                w[j] = pack_scores(static_cast<const __half*>(nullptr), v[2 * j], v[2 * j + 1]);
+                            } else {
+                                w[j] = pack_scores(static_cast<const __nv_bfloat16*>(nullptr), v[2 * j], v[2 * j + 1]);
+                                if (p + 1 < PLANES) {
+                                    v[2 * j] -= __uint_as_float(w[j] << 16);
+                                    v[2 * j + 1] -= __uint_as_float(w[j] & 0xFFFF0000u);
+                                }
+                            }
+                        }
+                        uint4* const o = reinterpret_cast<uint4*>(out + p * a.plane + c0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    }
+                }
+            }
+        }
+        __device__ __forceinline__ void unit_end(const CeScoreArgs&, const CeUnit&) {}
+    };
+};
+
+// Products with G: out[split][row][col] (+)= sum over a split of K of A's row by B's column.
+struct CeProductArgs {
+    int* d_error;
+    unsigned units;
+    uint32_t idesc;
+    int rows, cols;
+    int b0;                   // entry of K that B begins with
+    int kb, kper;             // steps of K, and as many in a split
+    int tiles_m, tiles_n;
+    bool accumulate;
+    float* out;
+};
+struct CeProductUnit {
+    static constexpr int tiles = 1;
+    int m0, nt, k0, k1, split;
+    __device__ __forceinline__ CeProductUnit(const CeProductArgs& a, unsigned u) {
+        const int mt = (int)(u % (unsigned)a.tiles_m);
+        u /= (unsigned)a.tiles_m;
+        nt = (int)(u % (unsigned)a.tiles_n);
+        split = (int)(u / (unsigned)a.tiles_n);
+        m0 = mt * TG_M;
+        k0 = split * a.kper, k1 = min(a.kb, k0 + a.kper);
+    }
+};
+template <int PLANES, bool AMN, int N>
+struct CeProductPolicy {
+    static constexpr bool A_MN = AMN, B_MN = true, I8 = false, HALVES = true;
+    static constexpr int BN = N, SEGMENT = 0, EPI_BYTES = 0;
+    using Pairs = PlanePairs<PLANES>;
+    using Args = CeProductArgs;
+    using Unit = CeProductUnit;
+    static __device__ __forceinline__ void load(const Args& a, const Unit& u, int, int pa, int pb, int k, const CUtensorMap* ta, const CUtensorMap* tb, unsigned char* sa,
+                                                unsigned char* sb, uint64_t* bar) {
+        if (AMN) {
+            tma_load_3d(sa, ta, bar, u.m0, k * 64, pa);
+            tma_load_3d(sa + TG_BOX_BYTES, ta, bar, u.m0 + 64, k * 64, pa);
+        } else {
+            tma_load_3d(sa, ta, bar, k * 64, u.m0, pa);
+        }
+#pragma unroll
+        for (int i = 0; i < BN / 64; ++i) tma_load_3d(sb + i * TG_BOX_BYTES, tb, bar, u.nt * BN + i * 64, a.b0 + k * 64, pb);
+    }
+    static __device__ __forceinline__ int n_mma(const Args& a, const Unit& u, int) { return min(BN, (a.cols - u.nt * BN + 15) & ~15); }
+
+    struct Epilogue {
+        int quarter, group, lane;
+        __device__ __forceinline__ Epilogue(const Args&, unsigned char*, int, int quarter_, int group_, int lane_) : quarter(quarter_), group(group_), lane(lane_) {}
+        __device__ __forceinline__ void unit_begin(const Args&, const Unit&) {}
+        __device__ __forceinline__ void unit_end(const Args&, const Unit&) {}
+        __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool) {
+            const int row = u.m0 + quarter * 32 + lane;
+            if (row - lane >= a.rows) return;
+            float* const out = a.out + ((int64_t)u.split * a.rows + row) * a.cols + u.nt * BN + group * (BN / 2);
+            const int width = min(BN / 2, a.cols - u.nt * BN - group * (BN / 2));
+            const bool wide = (a.cols & 3) == 0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < width; c0 += 32) {
+                uint32_t r[32];
+                tg_read(taddr + c0, live, r);
+                if (row < a.rows) {
+                    if (wide) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            if (c0 + j >= width) break;
+                            float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+                            float4* const o = reinterpret_cast<float4*>(out + c0 + j);
+                            if (a.accumulate) {
+                                const float4 w = __ldcg(o);
+                                v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+                            }
+                            *o = v;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            if (c0 + j >= width) break;
+                            out[c0 + j] = __uint_as_float(r[j]) + (a.accumulate ? __ldcg(out + c0 + j) : 0.f);
+                        }
+                    }
+                }
+            }
+        }
+    };
+};
+
+// A matrix as planes of 16 bits with rows of `pitch` entries, zeros behind a row's end: three bfloat16 that sum up to each float, or the values as they are.  Rows that the bias masks become
+// zeros: G has zeros for them, and what they hold may not be finite.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) ce_planes_kernel(const T* __restrict__ X, int64_t ld, int64_t rows, int d, int pitch, const float* __restrict__ bias,
+                                                        uint16_t* __restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = rows * (pitch / 2);
+    if (i >= total) return;
+    const int64_t row = i / (pitch / 2);
+    const int col = (int)(i - row * (pitch / 2)) * 2;
+    const T* const x = X + row * ld + col;
+    const T zero = (T)0.f;
+    const bool some = !(bias && bias[row] == -INFINITY);
+    const T v0 = some && col < d ? x[0] : zero, v1 = some && col + 1 < d ? x[1] : zero;
+    uint32_t* const o = reinterpret_cast<uint32_t*>(out) + i;
+    if constexpr (PLANES == 1) {
+        uint16_t b[2];
+        memcpy(b, &v0, 2);
+        memcpy(b + 1, &v1, 2);
+        *o = b[0] | (uint32_t)b[1] << 16;
+    } else {
+        float f0 = v0, f1 = v1;
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) {
+            const uint32_t w = pack_scores(static_cast<const __nv_bfloat16*>(nullptr), f0, f1);
+            o[p * total] = w;
+            f0 -= __uint_as_float(w << 16);
+            f1 -= __uint_as_float(w & 0xFFFF0000u);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ bias, int n, float* __restrict__ out) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) out[i] = bias[i] * CE_LOG2E;
+}
+
+// A warp joins a query's blocks.
+__global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__ partial, int slots, int m, int n, const int64_t* __restrict__ targets,
+                                                      const float* __restrict__ target_scores, const float* __restrict__ bias2, float c, float* __restrict__ losses,
+                                                      float* __restrict__ lse, float* __restrict__ lse_low) {
+    const int q = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+    if (q >= m) return;
+    const float2* const p = partial + (int64_t)q * slots;
+    float top = -INFINITY;
+    for (int i = lane; i < slots; i += 32) top = fmaxf(top, p[i].x);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const float base = top == -INFINITY ? 0.f : top;
+    double sum = 0.;
+    for (int i = lane; i < slots; i += 32) {
+        const float2 v = p[i];
+        sum += (double)v.y * (double)exp2f(v.x - base);
+    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane) return;
+    const double ln2 = 0.69314718055994530942, two = (double)base + log2(sum), whole = two * ln2;
+    const float high = (float)whole;
+    lse[q] = high;
+    lse_low[q] = isfinite(high) ? (float)(whole - (double)high) : 0.f;
+    float loss = 0.f;
+    const int64_t t = targets ? targets[q] : -1;
+    if (t >= 0 && t < n) {
+        const double z = (double)target_scores[q] * (double)c + (bias2 ? (double)bias2[t] : 0.);
+        loss = z == -INFINITY && two == two ? INFINITY : (float)((two - z) * ln2);
+        if (loss < 0.f) loss = 0.f;
+    }
+    losses[q] = loss;
+}
+
+// What the gradient takes of a query.
+__global__ void __launch_bounds__(256) ce_terms_kernel(const float* __restrict__ losses, const float* __restrict__ lse, const float* __restrict__ lse_low,
+                                                       const int64_t* __restrict__ targets, const float* __restrict__ grad_losses, const float* __restrict__ grad_lse, int m,
+                                                       int n, float* __restrict__ terms, float* __restrict__ factors, float* __restrict__ own, int* __restrict__ cols,
+                                                       uint32_t* __restrict__ amax) {
+    const int q = blockIdx.x * 256 + threadIdx.x;
+    if (q >= m) return;
+    const double two = ((double)lse[q] + (double)lse_low[q]) * 1.4426950408889634074;
+    const float high = (float)two;
+    const bool none = high == -INFINITY;
+    const float loss = losses[q];
+    const int64_t t = targets ? targets[q] : -1;
+    const bool has = t >= 0 && t < n && loss < INFINITY;
+    const float g = has && grad_losses ? grad_losses[q] : 0.f, e = grad_lse ? grad_lse[q] : 0.f;
+    terms[q] = none ? -INFINITY : -high;
+    const float f = (g + e) * (isfinite(high) ? (float)exp2(-(two - (double)high)) : 1.f);
+    factors[q] = f;
+    cols[q] = has ? (int)t : -1;
+    own[q] = has ? g * expm1f(-loss) + e * expf(-loss) : 0.f;
+    if (amax && isfinite(f)) atomicMax(amax, __float_as_uint(fabsf(f)));
+}
+
+// Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes CE_OWN_ROWS rows and looks
+// through all targets; they come in ascending order.
+constexpr int CE_OWN_ROWS = 128, CE_OWN_LIST = 1024;
+template <typename T>
+__global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ cols, const float* __restrict__ own, const T* __restrict__ Q, int64_t ldq, int m, int n, int d,
+                                                     float* __restrict__ sums, int* __restrict__ where) {
+    __shared__ int s_first[CE_OWN_ROWS];
+    __shared__ int s_query[CE_OWN_LIST + 256];
+    __shared__ unsigned char s_row[CE_OWN_LIST + 256];
+    __shared__ int s_count[9];
+    const int row0 = blockIdx.x * CE_OWN_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = threadIdx.x; r < CE_OWN_ROWS; r += 256) s_first[r] = -1;
+    int held = 0;  // the same for all threads
+    for (int64_t i0 = 0; i0 < m; i0 += 256) {
+        const int i = (int)i0 + threadIdx.x;
+        const int r = i0 + threadIdx.x < m ? cols[i] - row0 : -1;
+        const bool hit = (unsigned)r < (unsigned)CE_OWN_ROWS;
+        if (__syncthreads_or(hit)) {
+            const unsigned ballot = __ballot_sync(0xFFFFFFFFu, hit);
+            if (lane == 0) s_count[warp] = __popc(ballot);
+            __syncthreads();
+            int at = held, all = 0;
+            for (int w = 0; w < 8; ++w) {
+                if (w < warp) at += s_count[w];
+                all += s_count[w];
+            }
+            if (hit) {
+                at += __popc(ballot & ((1u << lane) - 1u));
+                s_query[at] = i;
+                s_row[at] = (unsigned char)r;
+            }
+            held += all;
+            __syncthreads();
+        }
+        if (held && (held >= CE_OWN_LIST || i0 + 256 >= m)) {
+            for (int rr = warp; rr < CE_OWN_ROWS; rr += 8) {  // a warp takes a row
+                int first = -1;
+                for (int e0 = 0; e0 < held && first < 0; e0 += 32) {
+                    const unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
+                    if (b) first = e0 + __ffs(b) - 1;
+                }
+                if (first < 0) continue;
+                const bool fresh = s_first[rr] < 0;
+                const int slot = fresh ? s_query[first] : s_first[rr];
+                for (int c0 = 0; c0 < d; c0 += 128) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int e0 = first & ~31; e0 < held; e0 += 32) {
+                        unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
+                        while (b) {
+                            const int e = e0 + __ffs(b) - 1;
+                            b &= b - 1u;
+                            const int query = s_query[e];
+                            const float f = own[query];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const int col = c0 + k * 32 + lane;
+                                if (col < d) acc[k] = fmaf(f, ce_float(Q[(int64_t)query * ldq + col]), acc[k]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int col = c0 + k * 32 + lane;
+                        if (col < d) {
+                            float* const s = sums + (int64_t)slot * d + col;
+                            *s = fresh ? acc[k] : *s + acc[k];
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0 && fresh) s_first[rr] = slot;
+                __syncwarp();
+            }
+            held = 0;
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < CE_OWN_ROWS && row0 + r < n; r += 256) where[row0 + r] = s_first[r];
+}
+
+// Gradients from sums: out[row][col] = (sum over the splits / scale + the target's part) / T.  QUERIES: the target's part is own[row] times the row cols[row] of X; else sums[where[row]].
+template <typename T, bool QUERIES>
+__global__ void __launch_bounds__(256) ce_finish_kernel(const float* __restrict__ parts, int splits, int64_t split_stride, int64_t rows, int d, const uint32_t* __restrict__ amax,
+                                                        const int* __restrict__ which, const float* __restrict__ own, const T* __restrict__ X, int64_t ldx,
+                                                        const float* __restrict__ sums, float inv_t, T* __restrict__ out, int64_t ldo) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * d) return;
+    const int64_t row = i / d;
+    const int col = (int)(i - row * d);
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += parts[s * split_stride + i];
+    if (amax) v = ldexpf(v, -ce_scale_exponent(amax));
+    const int w = which[row];
+    if (w >= 0) v += QUERIES ? own[row] * ce_float(X[(int64_t)w * ldx + col]) : sums[(int64_t)w * d + col];
+    out[row * ldo + col] = (T)(v * inv_t);
+}
+
+// ------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------
+struct CeCall {
+    CtxPtr c;
+    const void *Q, *X;
+    int64_t ldq, ldx;
+    int type, m, n, d;
+    const int64_t* targets;
+    const float* bias;
+    double temperature;
+    int* d_error;
+    cudaStream_t stream;
+    int planes() const { return type == CULSH_F32 ? 3 : 1; }
+    int pitch() const { return (d + 7) & ~7; }
+    bool copies(const void* p, int64_t ld) const { return type == CULSH_F32 || !aligned16(p, ld * 2); }
+    TgType tg() const { return type == CULSH_F16 ? TG_F16 : TG_BF16; }
+    float c2() const { return (float)(1.4426950408889634 / temperature); }
+};
+
+// Pieces of the workspace, each at a multiple of 256 bytes.
+struct CeSpace {
+    char* base;
+    size_t used = 0;
+    template <typename T>
+    T* take(size_t count) {
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used += (count * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+};
+
+constexpr size_t CE_G_BYTES = 64u << 20, CE_PARTS_BYTES = 256u << 20;
+
+struct CePlan {
+    CeSpace space;
+    uint16_t *q_planes = nullptr, *x_planes = nullptr;
+    float* bias2 = nullptr;
+    // forward
+    int block = 0, slots = 0;
+    float2* partial = nullptr;
+    float* target_scores = nullptr;
+    // backward
+    float *terms = nullptr, *factors = nullptr, *own = nullptr, *sums = nullptr;
+    int *cols = nullptr, *where = nullptr;
+    uint32_t* amax = nullptr;
+    int piece = 0;  // rows
+    uint16_t* G = nullptr;
+    int splits_q = 0, per_q = 0, splits_x = 0, per_x = 0;
+    float *acc_q = nullptr, *parts_x = nullptr;
+
+    CePlan(const CeCall& k, bool backward, bool need_q, bool need_x, void* base) : space{static_cast<char*>(base)} {
+        const int sms = k.c->sm_count;
+        if (k.copies(k.Q, k.ldq)) q_planes = space.take<uint16_t>((size_t)k.planes() * k.m * k.pitch());
+        if (k.copies(k.X, k.ldx) || (backward && k.bias)) x_planes = space.take<uint16_t>((size_t)k.planes() * k.n * k.pitch());
+        if (k.bias) bias2 = space.take<float>(k.n);
+        const size_t tiles_q = ceil_div(k.m, TG_M), tiles_n = ceil_div(k.n, CE_BN);
+        if (!backward) {
+            block = (int)std::max<size_t>(1, std::min<size_t>(16, tiles_q * tiles_n / ((size_t)sms * 8)));
+            slots = 2 * (int)ceil_div(tiles_n, block);
+            partial = space.take<float2>((size_t)k.m * slots);
+            target_scores = space.take<float>(k.m);
+            return;
+        }
+        terms = space.take<float>(k.m), factors = space.take<float>(k.m), own = space.take<float>(k.m);
+        cols = space.take<int>(k.m);
+        if (k.type == CULSH_F16) amax = space.take<uint32_t>(1);
+        const size_t row_bytes = (size_t)2 * k.planes() * k.m;
+        const size_t fit = std::min(CE_G_BYTES / row_bytes, need_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : CE_G_BYTES) / CE_BN * CE_BN;
+        piece = (int)std::min<size_t>(std::max<size_t>(fit, CE_BN), tiles_n * CE_BN);
+        G = space.take<uint16_t>((size_t)k.planes() * k.m * piece);
+        const int bn = product_bn(k.d);
+        const size_t tn = ceil_div(k.d, bn);
+        auto split = [&](size_t tiles, int kb, int& splits, int& per) {
+            const int most = k.type == CULSH_F32 ? 16 : 512;  // steps of 64 in one accumulator: its adds cut off, 2^-24 of it at a time
+            const size_t want = std::max<size_t>(ceil_div(kb, most), std::min<size_t>(sms / std::max<size_t>(tiles, 1), kb / 8));
+            per = (int)ceil_div(kb, std::max<size_t>(want, 1));
+            splits = (int)ceil_div(kb, per);
+        };
+        if (need_q) {
+            split(tiles_q * tn, (int)ceil_div(std::min(piece, k.n), 64), splits_q, per_q);
+            acc_q = space.take<float>((size_t)splits_q * k.m * k.d);
+        }
+        if (need_x) {
+            sums = space.take<float>((size_t)k.m * k.d);
+            where = space.take<int>(k.n);
+            split(ceil_div(std::min(piece, k.n), TG_M) * tn, (int)ceil_div(k.m, 64), splits_x, per_x);
+            parts_x = space.take<float>((size_t)splits_x * piece * k.d);
+        }
+    }
+    static int product_bn(int d) { return d > 128 ? 256 : d > 64 ? 128 : 64; }
+};
+
+inline unsigned ce_grid(size_t threads) {
+    const size_t g = ceil_div(threads, 256);
+    if (g > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "the matrices are too large for one call");
+    return (unsigned)g;
+}
+
+// Planes where they are needed, and where the products find both operands.
+struct CeOperands {
+    const void *q, *x;
+    int64_t ldq, ldx;
+    CeOperands(const CeCall& k, const CePlan& p) : q(k.Q), x(k.X), ldq(k.ldq), ldx(k.ldx) {
+        auto bring = [&](const void* from, int64_t ld, int rows, const float* bias, uint16_t* to) {
+            const unsigned grid = ce_grid((size_t)rows * k.pitch() / 2);
+            if (k.type == CULSH_F32) ce_planes_kernel<float, 3><<<grid, 256, 0, k.stream>>>(static_cast<const float*>(from), ld, rows, k.d, k.pitch(), bias, to);
+            else ce_planes_kernel<__half, 1><<<grid, 256, 0, k.stream>>>(static_cast<const __half*>(from), ld, rows, k.d, k.pitch(), bias, to);  // bits are bits
+            KERNEL_CHECK();
+        };
+        if (p.q_planes) bring(k.Q, k.ldq, k.m, nullptr, p.q_planes), q = p.q_planes, ldq = k.pitch();
+        if (p.x_planes) bring(k.X, k.ldx, k.n, k.bias, p.x_planes), x = p.x_planes, ldx = k.pitch();
+        if (p.bias2) {
+            ce_bias_kernel<<<ce_grid(k.n), 256, 0, k.stream>>>(k.bias, k.n, p.bias2);
+            KERNEL_CHECK();
+        }
+    }
+    CUtensorMap map_q(const CeCall& k, int box) const { return tg_map(q, k.tg(), k.m, k.d, ldq, k.planes(), (int64_t)k.m * ldq * 2, box); }
+    CUtensorMap map_x(const CeCall& k, int box) const { return tg_map(x, k.tg(), k.n, k.d, ldx, k.planes(), (int64_t)k.n * ldx * 2, box); }
+};
+
+inline CeScoreArgs ce_score_args(const CeCall& k, const CePlan& p) {
+    CeScoreArgs a{};
+    a.d_error = k.d_error, a.idesc = tg_idesc(k.tg(), false, false);
+    a.m = k.m, a.kb = (int)ceil_div(k.d, 64), a.n0 = 0, a.n1 = k.n;
+    a.tiles_q = (int)ceil_div(k.m, TG_M), a.tiles_n = (unsigned)ceil_div(k.n, CE_BN);
+    a.c = k.c2(), a.bias = p.bias2, a.targets = k.targets;
+    return a;
+}
+
+// f(number of planes, whether there is a bias, whether K is taken in segments), as types.
+template <typename F>
+inline void ce_by(F&& f, bool three, bool bias, bool segments) {
+    using Y = std::true_type;
+    using N = std::false_type;
+    auto with = [&](auto p) {
+        if (bias && segments) f(p, Y(), Y());
+        else if (bias) f(p, Y(), N());
+        else if (segments) f(p, N(), Y());
+        else f(p, N(), N());
+    };
+    if (three) with(std::integral_constant<int, 3>());
+    else with(std::integral_constant<int, 1>());
+}
+
+inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse_low, void* workspace) {
+    const CePlan p(k, false, false, false, workspace);
+    const CeOperands ops(k, p);
+    CeScoreArgs a = ce_score_args(k, p);
+    a.block = p.block, a.slots = p.slots, a.partial = p.partial, a.target_scores = p.target_scores;
+    const size_t units = ceil_div(a.tiles_n, p.block) * a.tiles_q;
+    if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
+    a.units = (unsigned)units;
+    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CE_BN);
+    const bool segments = a.kb > CE_SEGMENT;
+    ce_by([&](auto planes, auto bias, auto segs) { tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value>>(k.c, tq, tx, a, k.stream); },
+          k.planes() == 3, k.bias != nullptr, segments);
+    ce_join_kernel<<<ce_grid((size_t)k.m * 32), 256, 0, k.stream>>>(p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
+    KERNEL_CHECK();
+}
+
+template <int PLANES, bool AMN>
+inline void ce_product(const CeCall& k, const CUtensorMap& tg, const void* b, int64_t ldb, int64_t b_rows, CeProductArgs a, int per, int splits) {
+    const int bn = CePlan::product_bn(k.d);
+    a.d_error = k.d_error, a.idesc = tg_idesc(k.tg(), AMN, true);
+    a.cols = k.d, a.kper = per;
+    a.tiles_m = (int)ceil_div(a.rows, TG_M), a.tiles_n = (int)ceil_div(k.d, bn);
+    splits = (int)std::min<size_t>(splits, ceil_div(a.kb, per));
+    a.units = (unsigned)a.tiles_m * a.tiles_n * splits;
+    const CUtensorMap tb = tg_map(b, k.tg(), b_rows, k.d, ldb, k.planes(), b_rows * ldb * 2, 64);
+    if (bn == 256) tc_gemm<CeProductPolicy<PLANES, AMN, 256>>(k.c, tg, tb, a, k.stream);
+    else if (bn == 128) tc_gemm<CeProductPolicy<PLANES, AMN, 128>>(k.c, tg, tb, a, k.stream);
+    else tc_gemm<CeProductPolicy<PLANES, AMN, 64>>(k.c, tg, tb, a, k.stream);
+}
+
+template <typename T>
+inline void cross_entropy_backward(const CeCall& k, const float* losses, const float* lse, const float* lse_low, const float* grad_losses, const float* grad_lse, T* grad_Q,
+                                   int64_t ld_gq, T* grad_X, int64_t ld_gx, void* workspace) {
+    constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    const CePlan p(k, true, grad_Q != nullptr, grad_X != nullptr, workspace);
+    const CeOperands ops(k, p);
+    const float inv_t = (float)(1 / k.temperature);
+    if (p.amax) CU_CHECK(cudaMemsetAsync(p.amax, 0, 4, k.stream));
+    ce_terms_kernel<<<ce_grid(k.m), 256, 0, k.stream>>>(losses, lse, lse_low, k.targets, grad_losses, grad_lse, k.m, k.n, p.terms, p.factors, p.own, p.cols, p.amax);
+    KERNEL_CHECK();
+    if (grad_X) {
+        ce_own_kernel<<<(unsigned)ceil_div(k.n, CE_OWN_ROWS), 256, 0, k.stream>>>(p.cols, p.own, static_cast<const T*>(k.Q), k.ldq, k.m, k.n, k.d, p.sums, p.where);
+        KERNEL_CHECK();
+    }
+    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CE_BN);
+    const int64_t g_plane = (int64_t)k.m * p.piece;
+    CeScoreArgs s = ce_score_args(k, p);
+    s.terms = p.terms, s.factors = p.factors, s.amax = p.amax, s.target_cols = p.cols, s.G = p.G, s.pitch = p.piece, s.plane = g_plane;
+    s.block = 1;
+    for (int64_t n0 = 0; n0 < k.n; n0 += p.piece) {
+        const int here = (int)std::min<int64_t>(p.piece, k.n - n0);
+        s.n0 = (int)n0, s.n1 = (int)(n0 + here);
+        s.tiles_n = (unsigned)ceil_div(here, CE_BN);
+        const size_t units = (size_t)s.tiles_n * s.tiles_q;
+        if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
+        s.units = (unsigned)units;
+        ce_by([&](auto planes, auto bias, auto segs) {
+            // 16-bit results are none the worse for the segments' sums being one
+            if constexpr (decltype(planes)::value == PLANES && (PLANES == 3 || !decltype(segs)::value))
+                tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value>>(k.c, tq, tx, s, k.stream);
+        }, PLANES == 3, k.bias != nullptr, PLANES == 3 && s.kb > CE_SEGMENT);
+        const int64_t g_cols = (int64_t)s.tiles_n * CE_BN;
+        if (grad_X) {
+            CeProductArgs a{};
+            a.rows = here, a.b0 = 0, a.kb = (int)ceil_div(k.m, 64), a.out = p.parts_x;
+            ce_product<PLANES, true>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, 64), ops.q, ops.ldq, k.m, a, p.per_x, p.splits_x);
+            ce_finish_kernel<T, false><<<ce_grid((size_t)here * k.d), 256, 0, k.stream>>>(p.parts_x, p.splits_x, (int64_t)here * k.d, here, k.d, p.amax, p.where + n0, nullptr,
+                                                                                           nullptr, 0, p.sums, inv_t, grad_X + n0 * ld_gx, ld_gx);
+            KERNEL_CHECK();
+        }
+        if (grad_Q) {
+            CeProductArgs a{};
+            a.rows = k.m, a.b0 = (int)n0, a.kb = (int)ceil_div(here, 64), a.out = p.acc_q, a.accumulate = n0 > 0;
+            ce_product<PLANES, false>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, TG_M), ops.x, ops.ldx, k.n, a, p.per_q, p.splits_q);
+        }
+    }
+    if (grad_Q) {
+        ce_finish_kernel<T, true><<<ce_grid((size_t)k.m * k.d), 256, 0, k.stream>>>(p.acc_q, p.splits_q, (int64_t)k.m * k.d, k.m, k.d, p.amax, p.cols, p.own,
+                                                                                     static_cast<const T*>(k.X), k.ldx, nullptr, inv_t, grad_Q, ld_gq);
+        KERNEL_CHECK();
+    }
+}
+
+}  // namespace culsh_b200

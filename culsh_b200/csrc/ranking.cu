@@ -1,5 +1,5 @@
 // Entry points of the ranking operators: rows in 4 bits, products and scores, log probabilities (see include/culsh_b200.h).
-#include "api.cuh"
+#include "entry.cuh"
 #include "log_probs.cuh"
 #include "mx_product.cuh"
 #include "mx_rows.cuh"
@@ -12,25 +12,6 @@ using namespace culsh_b200;
 
 namespace {
 
-// Calls f(pointer of the type) for one of the types that are allowed (a mask of 1 << type).
-template <typename P, typename F>
-void by_type(int type, unsigned allowed, P* p, F&& f) {
-    if (type < 0 || type > 3 || !(allowed >> type & 1)) fail(CULSH_ERR_INVALID, "type %d is not supported here", type);
-    constexpr bool in = std::is_const<P>::value;
-    auto as = [&](auto t) {
-        using T = decltype(t);
-        return static_cast<std::conditional_t<in, const T*, T*>>(p);
-    };
-    if (type == CULSH_F32) f(as(float()));
-    else if (type == CULSH_F16) f(as(__half()));
-    else if (type == CULSH_BF16) f(as(__nv_bfloat16()));
-    else f(as(double()));
-}
-constexpr unsigned ALL_TYPES = 15, SCORE_TYPES = 1u << CULSH_F32 | 1u << CULSH_F16 | 1u << CULSH_BF16;
-
-void need(bool ok, const char* what) {
-    if (!ok) fail(CULSH_ERR_INVALID, "%s", what);
-}
 void check_rows(const void* codes, const void* scales, int n, int d) {
     need(n > 0 && d > 0, "rows and features must be positive");
     need(n <= 0x7FFFFF80, "at most 2,147,483,520 rows");
@@ -38,12 +19,6 @@ void check_rows(const void* codes, const void* scales, int n, int d) {
     need(codes && scales, "null argument");
     need((((uintptr_t)codes | (uintptr_t)scales) & 15) == 0, "codes and scales have to begin at a multiple of 16 bytes");
 }
-void need_workspace(const void* p, uint64_t have, size_t bytes) {
-    if (bytes && (have < bytes || !p || ((uintptr_t)p & 15))) fail(CULSH_ERR_INVALID, "the workspace has to be %zu bytes, aligned to 16", bytes);
-}
-cudaStream_t stream_of(void* stream) { return static_cast<cudaStream_t>(stream); }
-int* wait_word(const CtxPtr& c) { return c->d_error + 6; }
-
 LpArgs log_probs_args(const void* scores, int m, int64_t cols, int64_t ld, const int64_t* offsets, const int32_t* ids, int64_t total, double temperature,
                       const int64_t* targets) {
     need(scores || (offsets && total == 0), "null argument");

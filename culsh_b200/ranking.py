@@ -1,8 +1,8 @@
-"""Ranking of candidates: rows held in 4 bits, their scores against queries, and log probabilities over scores.
+"""Ranking of candidates: rows held in 4 or 8 bits, their scores against queries, and log probabilities over scores.
 
 ``query`` answers with the ids of candidate rows, not ranked.  Here the rows are kept in microscaled 4-bit floating point
-(``MXRows``: 17 bytes for 32 values), queries are scored against their candidates (``MXRows.score``) or against every
-row (``MXRows.product``), and ``log_probs`` turns scores into what an answer needs: the most likely rows, their log
+(``MXRows``: 17 bytes for 32 values) or in 8-bit integers (``Int8Rows``), queries are scored against their candidates (``score``) or against every
+row (``product``), and ``log_probs`` turns scores into what an answer needs: the most likely rows, their log
 probabilities, and the entropy of the distribution; ``log_probs_backward`` is its gradient, for training an encoder on candidate lists.
 
     rows = culsh.MXRows(X)
@@ -30,6 +30,7 @@ METRICS = {"dot": 0, "cosine": 1, "euclidean": 2}
 _TYPES = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloat16: 3}
 _SCORE_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 MAX_TOP_K = 128
+MAX_INT8_FEATURES = 1 << 17
 
 
 def _on_device(x, device=None) -> torch.Tensor:
@@ -69,6 +70,15 @@ def _metric(name: str) -> int:
     if name not in METRICS:
         raise ValueError(f"metric must be one of {tuple(METRICS)}")
     return METRICS[name]
+
+
+def _score_matrix(nq, n, dtype, device):
+    """An array for scores [nq, n] and the distance of its rows: rows that share their first and last 32 bytes with others take the memory twice as long
+    (1,000 x 999,999 float32 scores 2,036 us against 792)."""
+    line = 128 // dtype.itemsize
+    pitch = n if n < 8 * line else -(-n // line) * line
+    out = torch.empty((nq, pitch), dtype=dtype, device=device)
+    return (out[:, :n] if pitch != n else out), pitch
 
 
 def _floats(x, name, shape, device) -> torch.Tensor:
@@ -226,12 +236,7 @@ class MXRows:
         if d != self._d:
             raise ValueError(f"Query features ({d}) != row features ({self._d})")
         n = self._n
-        # rows that share their first and last 32 bytes with others take the memory twice as long (1,000 x 999,999 float32 scores 2,036 us against 792)
-        line = 128 // dtype.itemsize
-        pitch = n if n < 8 * line else -(-n // line) * line
-        out = torch.empty((nq, pitch), dtype=dtype, device=device)
-        if pitch != n:
-            out = out[:, :n]
+        out, pitch = _score_matrix(nq, n, dtype, device)
         if n and nq:
             h, stream = self._h, _stream(device)
             if held:
@@ -273,6 +278,161 @@ class MXRows:
             _lib.check(h.lib.culsh_mx_score(
                 h.ptr, Q.data_ptr(), _TYPES[Q.dtype], lists.n, _pitch(Q), *self._at, self._n, self._d, m, lists.ids, lists.offsets, lists.total,
                 out.data_ptr(), work.data_ptr() if need.value else None, need.value, stream))
+            lists.done(h, stream)
+        return out
+
+
+class Int8Rows:
+    """Rows in 8-bit integers with a scale for each: what is held is a whole number from -127 to 127 times the row's scale, the nearest to the value.
+
+    ``X``: 2-D, float32, float64, float16 or bfloat16, at most 131,072 features.  A row with a NaN or an infinity becomes NaN.  Queries are held the same way for a
+    ``product`` or ``score``: sums of the whole numbers' products are exact."""
+
+    def __init__(self, X):
+        X = _matrix(X)
+        if X.dtype not in _TYPES:
+            raise TypeError(f"Unsupported dtype: {X.dtype}. Supported dtypes are float32, float64, float16, bfloat16.")
+        n, d = int(X.shape[0]), int(X.shape[1])
+        if d == 0:
+            raise ValueError("rows have no features")
+        if d > MAX_INT8_FEATURES:
+            raise ValueError(f"at most {MAX_INT8_FEATURES} features")
+        self._n, self._d, self._h = n, d, get_handle(X.device.index)
+        # one allocation; the tensors that show its parts are made when they are asked for
+        pitch = -(-d // 16) * 16
+        self._codes = self._scales = self._squares = None
+        self._held = torch.empty(n * (pitch + 8), dtype=torch.uint8, device=X.device)
+        at = self._held.data_ptr()
+        self._at = (at, at + n * pitch, at + n * (pitch + 4))
+        self.device = X.device
+        if n:
+            h = self._h
+            _lib.check(h.lib.culsh_i8_quantize(h.ptr, X.data_ptr(), _TYPES[X.dtype], n, d, _pitch(X), *self._at, _stream(X.device)))
+
+    @classmethod
+    def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, squares: torch.Tensor, n_features: int) -> "Int8Rows":
+        """Rows from the arrays of another Int8Rows, e.g. loaded from a file: ``codes`` [n, P] int8 with P = n_features rounded up to a multiple of 16, zeros behind a
+        row's end, ``scales`` [n] float32, ``squares`` [n] int32 (sums of the rows' squared codes, -1 for a row that is NaN)."""
+        d = int(n_features)
+        if not 0 < d <= MAX_INT8_FEATURES:
+            raise ValueError(f"n_features must be between 1 and {MAX_INT8_FEATURES}")
+        pitch = -(-d // 16) * 16
+        if codes.ndim != 2 or codes.dtype != torch.int8 or codes.shape[1] != pitch:
+            raise ValueError(f"codes must be int8 of the shape [n, {pitch}]")
+        n = int(codes.shape[0])
+        if scales.dtype != torch.float32 or tuple(scales.shape) != (n,):
+            raise ValueError(f"scales must be float32 of the shape {(n,)}")
+        if squares.dtype != torch.int32 or tuple(squares.shape) != (n,):
+            raise ValueError(f"squares must be int32 of the shape {(n,)}")
+        if not (codes.is_cuda and codes.device == scales.device == squares.device):
+            raise ValueError("codes, scales and squares must be on one CUDA device")
+        codes = codes.contiguous()
+        if codes.data_ptr() & 15:
+            codes = codes.clone()
+        self = cls.__new__(cls)
+        self._n, self._d, self._h, self.device = n, d, get_handle(codes.device.index), codes.device
+        self._codes, self._scales, self._squares = codes, scales.contiguous(), squares.contiguous()
+        self._at = (self._codes.data_ptr(), self._scales.data_ptr(), self._squares.data_ptr())
+        return self
+
+    n_rows = property(lambda self: self._n)
+    n_features = property(lambda self: self._d)
+
+    def _part(self, first, last, dtype):
+        return self._held[first * self._n:last * self._n].view(dtype)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            pitch = -(-self._d // 16) * 16
+            self._codes = self._part(0, pitch, torch.int8).view(self._n, pitch)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            pitch = -(-self._d // 16) * 16
+            self._scales = self._part(pitch, pitch + 4, torch.float32)
+        return self._scales
+
+    @property
+    def squares(self) -> torch.Tensor:
+        if self._squares is None:
+            pitch = -(-self._d // 16) * 16
+            self._squares = self._part(pitch + 4, pitch + 8, torch.int32)
+        return self._squares
+
+    def size_bytes(self) -> int:
+        return self._n * (-(-self._d // 16) * 16 + 8)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values that are held, [n_rows, n_features]."""
+        if dtype not in _TYPES:
+            raise TypeError(f"Unsupported dtype: {dtype}. Supported dtypes are float32, float64, float16, bfloat16.")
+        out = torch.empty((self._n, self._d), dtype=dtype, device=self.device)
+        if self._n:
+            h = self._h
+            _lib.check(h.lib.culsh_i8_dequantize(h.ptr, self._at[0], self._at[1], self._n, self._d, out.data_ptr(), _TYPES[dtype], _stream(self.device)))
+        return out
+
+    def product(self, Q, metric: str = "dot", dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Scores [n_queries, n_rows] of queries against every row: dot products, cosines (0 with a row of zeros) or negative squared
+        distances ("euclidean").  ``Q``: Int8Rows, or an array that is held in 8 bits for the call.  Rows of many scores begin at multiples of
+        128 bytes, so that the result of an odd number of rows is not contiguous."""
+        m = _metric(metric)
+        if dtype not in _SCORE_TYPES:
+            raise TypeError(f"Unsupported dtype: {dtype}. Supported dtypes are float32, float16, bfloat16.")
+        device = self.device
+        held = isinstance(Q, Int8Rows)
+        if held:
+            if Q.device != device:
+                raise ValueError(f"queries are on {Q.device}, rows on {device}")
+            nq, d = Q._n, Q._d
+        else:
+            Q = _matrix(Q, device)
+            if Q.dtype not in _TYPES:
+                raise TypeError(f"Unsupported dtype: {Q.dtype}. Supported dtypes are float32, float64, float16, bfloat16.")
+            nq, d = Q.shape
+        if d != self._d:
+            raise ValueError(f"Query features ({d}) != row features ({self._d})")
+        n = self._n
+        out, pitch = _score_matrix(nq, n, dtype, device)
+        if n and nq:
+            h, stream = self._h, _stream(device)
+            if held:
+                _lib.check(h.lib.culsh_i8_product(h.ptr, *Q._at, nq, *self._at, n, d, m, out.data_ptr(), _TYPES[dtype], pitch, stream))
+            else:
+                need = (-(-d // 16) * 16 + 8) * nq
+                work = torch.empty(need, dtype=torch.uint8, device=device)
+                _lib.check(h.lib.culsh_i8_product_dense(h.ptr, Q.data_ptr(), _TYPES[Q.dtype], nq, _pitch(Q), *self._at, n, d, m, out.data_ptr(),
+                                                        _TYPES[dtype], pitch, work.data_ptr(), need, stream))
+        return out
+
+    def check(self) -> None:
+        """Waits for the current stream; raises if a product had to give up a wait (and is NaN in part)."""
+        _lib.check(self._h.lib.culsh_mx_product_check(self._h.ptr, _stream(self.device)))
+
+    def score(self, Q, candidates: Union[Candidates, Tuple], metric: str = "dot") -> torch.Tensor:
+        """Scores of queries, held in 8 bits for the call, against their candidates, float32, in the order of the candidates' ids.  ``candidates``: what ``query`` returned
+        for Q, or a pair (ids, offsets) of int32 and int64.  A candidate that is no row gets NaN, and so do all of a query that has an infinity or a NaN."""
+        m = _metric(metric)
+        Q = _matrix(Q, self.device)
+        if Q.dtype not in _TYPES:
+            raise TypeError(f"Unsupported dtype: {Q.dtype}. Supported dtypes are float32, float64, float16, bfloat16.")
+        if Q.shape[1] != self._d:
+            raise ValueError(f"Query features ({Q.shape[1]}) != row features ({self._d})")
+        lists = _Lists(candidates, self.device)
+        if lists.n != Q.shape[0]:
+            raise ValueError(f"{Q.shape[0]} queries, but {lists.n} lists")
+        out = torch.empty(lists.total, dtype=torch.float32, device=self.device)
+        if lists.total:
+            if not self._n:
+                return out.fill_(float("nan"))
+            h, stream = self._h, _stream(self.device)
+            need = (-(-self._d // 16) * 16 + 8) * lists.n
+            work = torch.empty(need, dtype=torch.uint8, device=self.device)
+            _lib.check(h.lib.culsh_i8_score(h.ptr, Q.data_ptr(), _TYPES[Q.dtype], lists.n, _pitch(Q), *self._at, self._n, self._d, m, lists.ids, lists.offsets,
+                                            lists.total, out.data_ptr(), work.data_ptr(), need, stream))
             lists.done(h, stream)
         return out
 
@@ -399,7 +559,7 @@ def log_probs_backward(scores, targets, lse, entropy, grad_log_probs=None, grad_
     return out
 
 
-def rank(rows: MXRows, Q, candidates: Union[Candidates, Tuple, None] = None, top_k: int = 10, metric: str = "dot", temperature: float = 1.0,
+def rank(rows: Union[MXRows, Int8Rows], Q, candidates: Union[Candidates, Tuple, None] = None, top_k: int = 10, metric: str = "dot", temperature: float = 1.0,
          targets=None) -> LogProbs:
     """The ``top_k`` best rows of each query with their log probabilities: among its candidates, or among all rows without any."""
     if candidates is None:

@@ -378,6 +378,59 @@ int culsh_log_probs_backward(culsh_handle* h, const void* scores, int type, int 
                              const int64_t* targets, const float* lse, const float* entropy, const float* grad_log_probs,
                              const float* grad_entropy, void* grad_scores, int64_t ld_grad, void* stream);
 
+/* ---- rows in 8-bit integers (no upstream counterpart) ------------------------------------ */
+/* On the caller's stream and device memory, as the ranking calls.  X: [n][d], rows ld entries apart, of any type.
+ * scale = max(largest magnitude of the row / 127 in 32 bits, 2^-126), a code is the nearest whole number to x / scale,
+ * ties to the even one.  With P = d rounded up to a multiple of 16:
+ *   codes   [n][P]  zeros behind a row's end; begin at a multiple of 16 bytes
+ *   scales  [n]     NaN for a row with a NaN or an infinity (or of a scale beyond float32), whose codes are 0
+ *   squares [n]     sum of the row's squared codes; -1 for such a row
+ * At most 131,072 features. */
+int culsh_i8_quantize(culsh_handle* h, const void* X, int type, int n, int d, int64_t ld, int8_t* codes, float* scales,
+                      int32_t* squares, void* stream);
+/* out: [n][d] of any type. */
+int culsh_i8_dequantize(culsh_handle* h, const int8_t* codes, const float* scales, int n, int d, void* out, int type,
+                        void* stream);
+/* out[q][i] (float32, float16 or bfloat16, rows ld entries apart): the metric of query q and row i, both held in 8 bits; sums
+ * of products of codes are exact.  Cosines with a row of zeros are 0.  A row of the scale NaN has scores of NaN.
+ * culsh_mx_product_check says whether a bounded wait ran out here too. */
+int culsh_i8_product(culsh_handle* h, const int8_t* q_codes, const float* q_scales, const int32_t* q_squares, int n_queries,
+                     const int8_t* codes, const float* scales, const int32_t* squares, int n, int d, int metric, void* out,
+                     int type, int64_t ld, void* stream);
+/* The same for queries of any type (rows ldq apart), which are held in 8 bits for the call: in workspace, device, aligned to
+ * 16, of (P + 8) n_queries bytes. */
+int culsh_i8_product_dense(culsh_handle* h, const void* Q, int q_type, int n_queries, int64_t ldq, const int8_t* codes,
+                           const float* scales, const int32_t* squares, int n, int d, int metric, void* out, int type, int64_t ld,
+                           void* workspace, uint64_t workspace_bytes, void* stream);
+/* out[c], c in [offsets[q], offsets[q + 1]): the metric of query q, held in 8 bits for the call as above, and row ids[c];
+ * NaN where ids[c] is no row.  offsets: n_queries + 1, from 0 to total. */
+int culsh_i8_score(culsh_handle* h, const void* Q, int type, int n_queries, int64_t ldq, const int8_t* codes,
+                   const float* scales, const int32_t* squares, int n, int d, int metric, const int32_t* ids,
+                   const int64_t* offsets, int64_t total, float* out, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ---- softmax cross entropy over every row (no upstream counterpart) ---------------------- */
+/* Q: [m][d], X: [n][d], both float32, float16 or bfloat16, rows ldq and ldx entries apart.  With
+ * z[i][j] = Q[i] . X[j] / temperature + bias[j] (bias: [n] float32 or NULL; -inf takes a row out):
+ *   lse     [m]  log of the sum of exp(z[i]); -inf where no row is left.  lse + lse_low is the same in twice the bits
+ *   losses  [m]  lse - z[i][targets[i]], never negative; 0 where the target is not in 0 .. n - 1 (or targets is NULL), inf
+ *                where it is masked
+ * The scores are not kept.  A NaN or an infinity in a query, or in a row that is not masked, makes the numbers NaN that it has
+ * a part in (but scores of 16-bit values that come out as -inf have none).  workspace: device, as many bytes as culsh_cross_entropy_workspace says for the same arrays (gradients: 0 for
+ * the losses, 1 for the gradient of Q, 2 of X, 3 of both), aligned to 16. */
+int culsh_cross_entropy_workspace(culsh_handle* h, const void* Q, int64_t ldq, const void* X, int64_t ldx, int type, int m, int n,
+                                  int d, int has_bias, int gradients, uint64_t* bytes);
+int culsh_cross_entropy(culsh_handle* h, const void* Q, int64_t ldq, const void* X, int64_t ldx, int type, int m, int n, int d,
+                        const int64_t* targets, const float* bias, double temperature, float* losses, float* lse, float* lse_low,
+                        void* workspace, uint64_t workspace_bytes, void* stream);
+/* Gradients with respect to Q and X, in their type (either may be NULL), from those of losses and of lse (either may be NULL) and
+ * what the forward call returned.  A target that is not in 0 .. n - 1 or is masked has no loss to go by.  The bias has no
+ * gradient here.  Results do not depend on the order in which anything runs. */
+int culsh_cross_entropy_backward(culsh_handle* h, const void* Q, int64_t ldq, const void* X, int64_t ldx, int type, int m, int n,
+                                 int d, const int64_t* targets, const float* bias, double temperature, const float* losses,
+                                 const float* lse, const float* lse_low, const float* grad_losses, const float* grad_lse,
+                                 void* grad_Q, int64_t ld_gq, void* grad_X, int64_t ld_gx, void* workspace,
+                                 uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
