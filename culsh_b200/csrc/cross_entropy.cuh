@@ -18,21 +18,13 @@
 
 #include <type_traits>
 
+#include "ce_fused.cuh"
 #include "tc_gemm.cuh"
 
 namespace culsh_b200 {
 
-constexpr float CE_LOG2E = 1.4426950408889634f;
 constexpr int CE_BN = 256, CE_HALF = CE_BN / 2;
 constexpr int CE_SEGMENT = 8;  // steps of 64
-
-template <typename T>
-__device__ __forceinline__ float ce_float(T v) { return (float)v; }
-__device__ __forceinline__ float ce_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 struct CeScoreArgs {
     int* d_error;
@@ -179,12 +171,6 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS> {
         }
     };
 };
-
-// What a power of two brings the largest factor to [2^14, 2^15].
-__device__ __forceinline__ int ce_scale_exponent(const uint32_t* amax) {
-    const uint32_t bits = amax ? __ldcg(amax) : 0u;
-    return bits == 0u ? 0 : min(max(14 + 127 - (int)(bits >> 23), -100), 100);
-}
 
 template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS>
 struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS> {
@@ -578,6 +564,8 @@ struct CePlan {
     uint16_t* G = nullptr;
     int splits_q = 0, per_q = 0, splits_x = 0, per_x = 0;
     float *acc_q = nullptr, *parts_x = nullptr;
+    bool fused_q = false, fused_x = false;
+    int fused_block = 0;  // tiles of rows in a unit of dQ
 
     CePlan(const CeCall& k, bool backward, bool need_q, bool need_x, void* base) : space{static_cast<char*>(base)} {
         const int sms = k.c->sm_count;
@@ -595,8 +583,28 @@ struct CePlan {
         terms = space.take<float>(k.m), factors = space.take<float>(k.m), own = space.take<float>(k.m);
         cols = space.take<int>(k.m);
         if (k.type == CULSH_F16) amax = space.take<uint32_t>(1);
+        // G stays on the SM where rows are short enough; sums of more than 32,768 entries would have to be split for dX too
+        const bool fused = k.planes() == 1 && k.d <= 256;
+        fused_q = need_q && fused, fused_x = need_x && fused && k.m <= 32768;
+        if (need_x) {
+            sums = space.take<float>((size_t)k.m * k.d);
+            where = space.take<int>(k.n);
+        }
+        if (fused_q) {
+            const int nb = k.d > 128 ? 64 : 128;
+            const size_t tiles = ceil_div(k.n, nb), least = ceil_div(tiles, 32768 / nb), most = std::min(tiles, least + ceil_div((size_t)4 * sms, tiles_q));
+            size_t best = ~(size_t)0;
+            for (size_t blocks = least; blocks <= most; ++blocks) {  // the last wave full, and four tiles' time for the units' ends
+                const size_t per = ceil_div(tiles, blocks), time = ceil_div(tiles_q * ceil_div(tiles, per), sms) * (per + 4);
+                if (time < best) best = time, fused_block = (int)per;
+            }
+            splits_q = (int)ceil_div(tiles, fused_block);
+            acc_q = space.take<float>((size_t)splits_q * k.m * k.d);
+        }
+        if ((!need_q || fused_q) && (!need_x || fused_x)) return;
+        const bool pieces_x = need_x && !fused_x;
         const size_t row_bytes = (size_t)2 * k.planes() * k.m;
-        const size_t fit = std::min(CE_G_BYTES / row_bytes, need_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : CE_G_BYTES) / CE_BN * CE_BN;
+        const size_t fit = std::min(CE_G_BYTES / row_bytes, pieces_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : CE_G_BYTES) / CE_BN * CE_BN;
         piece = (int)std::min<size_t>(std::max<size_t>(fit, CE_BN), tiles_n * CE_BN);
         G = space.take<uint16_t>((size_t)k.planes() * k.m * piece);
         const int bn = product_bn(k.d);
@@ -607,13 +615,11 @@ struct CePlan {
             per = (int)ceil_div(kb, std::max<size_t>(want, 1));
             splits = (int)ceil_div(kb, per);
         };
-        if (need_q) {
+        if (need_q && !fused_q) {
             split(tiles_q * tn, (int)ceil_div(std::min(piece, k.n), 64), splits_q, per_q);
             acc_q = space.take<float>((size_t)splits_q * k.m * k.d);
         }
-        if (need_x) {
-            sums = space.take<float>((size_t)k.m * k.d);
-            where = space.take<int>(k.n);
+        if (pieces_x) {
             split(ceil_div(std::min(piece, k.n), TG_M) * tn, (int)ceil_div(k.m, 64), splits_x, per_x);
             parts_x = space.take<float>((size_t)splits_x * piece * k.d);
         }
@@ -703,6 +709,31 @@ inline void ce_product(const CeCall& k, const CUtensorMap& tg, const void* b, in
     else tc_gemm<CeProductPolicy<PLANES, AMN, 64>>(k.c, tg, tb, a, k.stream);
 }
 
+template <bool ROWS, bool HALF>
+inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, void* out, int64_t ld) {
+    const int nb = k.d > 128 ? 64 : 128, kb = k.d > 128 ? 4 : k.d > 64 ? 2 : 1;
+    CeFusedArgs a{};
+    a.d_error = k.d_error;
+    a.idesc_s = tg_idesc(k.tg(), false, false) | ((uint32_t)(nb >> 3) << 17);
+    a.idesc_o = tg_idesc(k.tg(), false, true) | ((uint32_t)(kb * 64 >> 3) << 17);
+    a.own = ROWS ? k.n : k.m, a.other = ROWS ? k.m : k.n;
+    a.tiles_own = (int)ceil_div(a.own, TG_M), a.tiles_other = (int)ceil_div(a.other, nb), a.block = ROWS ? a.tiles_other : p.fused_block;
+    const size_t units = ceil_div(a.tiles_other, a.block) * a.tiles_own;
+    if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
+    a.units = (unsigned)units;
+    a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = p.terms, a.factors = p.factors, a.amax = p.amax, a.target_cols = p.cols;
+    a.parts = p.acc_q, a.out = out, a.ld = ld, a.where = p.where, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
+    const CUtensorMap own = ROWS ? ops.map_x(k, TG_M) : ops.map_q(k, TG_M), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
+    auto go = [&](auto boxes) {
+        constexpr int KB = decltype(boxes)::value;
+        if (k.bias) ce_fused_launch<KB, ROWS, true, HALF>(k.c, own, other, a, k.stream);
+        else ce_fused_launch<KB, ROWS, false, HALF>(k.c, own, other, a, k.stream);
+    };
+    if (kb == 4) go(std::integral_constant<int, 4>());
+    else if (kb == 2) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 1>());
+}
+
 template <typename T>
 inline void cross_entropy_backward(const CeCall& k, const float* losses, const float* lse, const float* lse_low, const float* grad_losses, const float* grad_lse, T* grad_Q,
                                    int64_t ld_gq, T* grad_X, int64_t ld_gx, void* workspace) {
@@ -718,12 +749,17 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         ce_own_kernel<<<(unsigned)ceil_div(k.n, CE_OWN_ROWS), 256, 0, k.stream>>>(p.cols, p.own, static_cast<const T*>(k.Q), k.ldq, k.m, k.n, k.d, p.sums, p.where);
         KERNEL_CHECK();
     }
+    if constexpr (PLANES == 1) {
+        if (p.fused_x) ce_fused<true, HALF>(k, p, ops, grad_X, ld_gx);
+        if (p.fused_q) ce_fused<false, HALF>(k, p, ops, nullptr, 0);
+    }
+    const bool pieces_q = grad_Q && !p.fused_q, pieces_x = grad_X && !p.fused_x;
     const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CE_BN);
     const int64_t g_plane = (int64_t)k.m * p.piece;
     CeScoreArgs s = ce_score_args(k, p);
     s.terms = p.terms, s.factors = p.factors, s.amax = p.amax, s.target_cols = p.cols, s.G = p.G, s.pitch = p.piece, s.plane = g_plane;
     s.block = 1;
-    for (int64_t n0 = 0; n0 < k.n; n0 += p.piece) {
+    for (int64_t n0 = 0; (pieces_q || pieces_x) && n0 < k.n; n0 += p.piece) {
         const int here = (int)std::min<int64_t>(p.piece, k.n - n0);
         s.n0 = (int)n0, s.n1 = (int)(n0 + here);
         s.tiles_n = (unsigned)ceil_div(here, CE_BN);
@@ -736,7 +772,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
                 tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value>>(k.c, tq, tx, s, k.stream);
         }, PLANES == 3, k.bias != nullptr, PLANES == 3 && s.kb > CE_SEGMENT);
         const int64_t g_cols = (int64_t)s.tiles_n * CE_BN;
-        if (grad_X) {
+        if (pieces_x) {
             CeProductArgs a{};
             a.rows = here, a.b0 = 0, a.kb = (int)ceil_div(k.m, 64), a.out = p.parts_x;
             ce_product<PLANES, true>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, 64), ops.q, ops.ldq, k.m, a, p.per_x, p.splits_x);
@@ -744,7 +780,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
                                                                                            nullptr, 0, p.sums, inv_t, grad_X + n0 * ld_gx, ld_gx);
             KERNEL_CHECK();
         }
-        if (grad_Q) {
+        if (pieces_q) {
             CeProductArgs a{};
             a.rows = k.m, a.b0 = (int)n0, a.kb = (int)ceil_div(here, 64), a.out = p.acc_q, a.accumulate = n0 > 0;
             ce_product<PLANES, false>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, TG_M), ops.x, ops.ldx, k.n, a, p.per_q, p.splits_q);
