@@ -1,12 +1,15 @@
 // Gradient of the cross entropy for rows of up to 256 values of 16 bits: G does not leave the SM.
 //
-// A CTA keeps 128 entries of one side ("own": rows for dX, queries for dQ) and goes through the other, a tile at a time:  S = own . other^T into tensor memory,  G = factor exp2(c S + term)
-// by the epilogue's threads and back into tensor memory as 16 bits, on top of S,  O += G . other with G as the operand that lies in tensor memory.  The other side's tile is loaded once for
+// A CTA keeps 128 entries of one side ("own": rows for dX, queries for dQ) and goes through the other, a tile at a time:  S = own . other^T into tensor memory,  G = 2^(c S + term)
+// by the epilogue's threads and back into tensor memory as 16 bits,  O += G . other with G as the operand that lies in tensor memory.  The other side's tile is loaded once for
 // both products: K along its rows for the first, across them for the second.  S is made again for the other gradient: 8 m n d operations in place of 6, against 6 bytes of G written and read
 // for each of the m n entries.
 //
-// One warp loads, one issues the MMAs, groups of four warps take the tiles in turn, one for each buffer of S.  The second product of a tile is issued BUFS - 1 tiles behind its first, so that
-// neither waits for the exponentials.  Sums of more than 32,768 entries are split (the accumulators cut off, see tc_gemm.cuh), those of dQ over units, whose sums ce_finish_kernel adds up.
+// The factor of a query's entries is a part of its term (log2 of its magnitude) where queries are the columns, and goes to the sums where they are the lanes.
+// One warp loads, one issues the MMAs, two groups of eight warps take the tiles in turn, a thread half the columns of a lane.  S and G have two places each, and the second product of a tile is
+// issued two tiles behind its first: what an MMA writes over has been read by the epilogue long before, and the tensor pipe has another product to do while a G is made.  (G on top of S, in three
+// places: the first product had to wait until the second one in front of it was done, 4,096 x 1M x 128 4.34 ms.)  Sums of more than 32,768 entries are split (the accumulators cut off,
+// see tc_gemm.cuh), those of dQ over units, whose sums ce_finish_kernel adds up.
 #pragma once
 
 #include <type_traits>
@@ -38,11 +41,11 @@ struct CeFusedArgs {
     int tiles_own, tiles_other, block;
     int d;
     float c;
-    const float* bias;        // of the rows, in powers of two, or NULL
-    const float* terms;       // of the queries
-    const float* factors;
-    const uint32_t* amax;
+    const float* bias;        // of the rows, in powers of two, or NULL; in lines of 128
+    const float* terms;       // of the queries: -lse in powers of two, for dX with log2 of the factor's magnitude
     const int* target_cols;
+    const int* marks;         // of the queries, for dX: target + 1, or 0, and the factor's sign in the highest bit; as `terms` in lines of 128 with -inf and 0 behind the last query
+    const uint32_t* amax;
     float* parts;             // dQ: [block][query][d]
     void* out;                // dX
     int64_t ld;
@@ -55,13 +58,14 @@ struct CeFusedArgs {
 template <int KB>
 struct CeFusedCfg {
     static constexpr int NB = KB == 4 ? 64 : 128;             // entries of a tile of the other side
-    static constexpr int O_COLS = KB * 64, BUFS = KB == 4 ? 4 : 3, GROUPS = BUFS;
-    static constexpr int OWN_BYTES = KB * TG_M * 128, OWNS = KB == 4 ? 1 : 2;
-    static constexpr int STAGE_BYTES = KB * NB * 128, STAGES = KB == 1 ? 8 : 4;
-    static constexpr int THREADS = 64 + 128 * GROUPS;
-    static constexpr int COLUMN_BYTES = GROUPS * 4 * NB * 8;
-    static constexpr int SMEM = OWNS * OWN_BYTES + STAGES * STAGE_BYTES + COLUMN_BYTES + 1024 /*barriers*/ + 1024 /*alignment slack*/;
-    static_assert(O_COLS + BUFS * NB <= 512 && SMEM <= 227 * 1024 && STAGES >= BUFS, "");
+    static constexpr int O_COLS = KB * 64, BUFS = 2, GROUPS = 2, WARPS = 8;  // of a group
+    static constexpr int CW = NB / 2;                         // columns of a warp
+    static constexpr int OWN_BYTES = KB * TG_M * 128, OWNS = KB == 1 ? 2 : 1;
+    static constexpr int STAGE_BYTES = KB * NB * 128, COLUMN_BYTES = NB * 4, STAGES = KB == 1 ? 8 : KB == 2 ? 5 : 4;
+    static constexpr int THREADS = 64 + 32 * WARPS * GROUPS;
+// (terms and marks, or the bias, of a stage's entries lie behind the stages)
+    static constexpr int SMEM = OWNS * OWN_BYTES + STAGES * (STAGE_BYTES + 2 * COLUMN_BYTES) + 1024 /*barriers*/ + 1024 /*alignment slack*/;
+    static_assert(O_COLS + BUFS * (NB + NB / 2) <= 512 && SMEM <= 227 * 1024 && STAGES > BUFS, "");
 };
 
 __device__ __forceinline__ void tc_mma_ts_warp(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -82,44 +86,42 @@ __device__ __forceinline__ void tg_store16(uint32_t taddr, const uint32_t (&r)[1
 }
 __device__ __forceinline__ void tg_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two floats in a register pair.
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+
+// CTAs that work on units next to one another begin at different tiles: those that ask for the same lines at the same time wait for the few slices of L2 that hold them.
 struct CeFusedUnit {
-    int own0, tile0, tiles, block;
+    int own0, tile0, tiles, block, turn;
     __device__ __forceinline__ CeFusedUnit(const CeFusedArgs& a, unsigned u) {
         block = (int)(u / (unsigned)a.tiles_own);
         own0 = (int)(u - (unsigned)block * a.tiles_own) * TG_M;
         tile0 = block * a.block;
         tiles = min(a.block, a.tiles_other - tile0);
+        turn = (int)((int64_t)tiles * (u & 31u) >> 5);
     }
-};
-
-// What the columns of a tile bring, for one warp: lane i of a warp has columns i, i + 32 ...  ROWS (own: rows, columns: queries): term, factor and target; else the rows' bias.
-template <int NB, bool ROWS, bool BIAS, bool HALF>
-struct CeColumns {
-    float term[NB / 32], factor[NB / 32];
-    int target[NB / 32];
-    __device__ __forceinline__ void fetch(const CeFusedArgs& a, int first, int end, int lane) {
-#pragma unroll
-        for (int i = 0; i < NB / 32; ++i) {
-            const int j = first + i * 32 + lane;
-            const bool in = j < end;
-            if (ROWS) {
-                term[i] = in ? __ldcg(a.terms + j) : -INFINITY;  // no entry: 0, whatever the bias
-                factor[i] = in ? __ldcg(a.factors + j) : 0.f;
-                target[i] = in ? __ldcg(a.target_cols + j) : -1;
-            } else if (BIAS) {
-                term[i] = in ? __ldcg(a.bias + j) : 0.f;
-            }
-        }
-    }
-    __device__ __forceinline__ void put(float* s, int exponent, int lane) const {
-        if (!ROWS && !BIAS) return;
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < NB / 32; ++i) {
-            s[i * 32 + lane] = term[i];
-            if (ROWS) s[NB + i * 32 + lane] = HALF ? ldexpf(factor[i], exponent) : factor[i];
-        }
-        __syncwarp();
+    __device__ __forceinline__ int tile(int t) const {
+        t += turn;
+        return tile0 + (t >= tiles ? t - tiles : t);
     }
 };
 
@@ -133,15 +135,16 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
     extern __shared__ unsigned char cf_smem_raw[];
     unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(cf_smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* const s_other = base + OWNS * Cfg::OWN_BYTES;
-    float* const s_columns = reinterpret_cast<float*>(s_other + STAGES * Cfg::STAGE_BYTES);
-    uint64_t* const own_full = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(s_columns) + Cfg::COLUMN_BYTES);
+    unsigned char* const s_columns = s_other + STAGES * Cfg::STAGE_BYTES;
+    uint64_t* const own_full = reinterpret_cast<uint64_t*>(s_columns + STAGES * 2 * Cfg::COLUMN_BYTES);
     uint64_t* const own_empty = own_full + OWNS;
     uint64_t* const full = own_empty + OWNS;
     uint64_t* const empty = full + STAGES;
     uint64_t* const s_full = empty + STAGES;   // S is there
-    uint64_t* const s_empty = s_full + BUFS;   // and its place free again
+    uint64_t* const s_empty = s_full + BUFS;   // and has been read
     uint64_t* const g_full = s_empty + BUFS;   // G is there
-    uint64_t* const o_full = g_full + BUFS;
+    uint64_t* const g_empty = g_full + BUFS;   // and its product done
+    uint64_t* const o_full = g_empty + BUFS;
     uint64_t* const o_empty = o_full + 1;
     uint64_t* const drained = o_empty + 1;
     uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
@@ -152,9 +155,9 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < OWNS; ++i) mbar_init(&own_full[i], 1), mbar_init(&own_empty[i], 1);
         for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int i = 0; i < BUFS; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], 1), mbar_init(&g_full[i], 4);
+        for (int i = 0; i < BUFS; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], Cfg::WARPS), mbar_init(&g_full[i], Cfg::WARPS), mbar_init(&g_empty[i], 1);
         mbar_init(o_full, 1);
-        mbar_init(o_empty, 4 * GROUPS);
+        mbar_init(o_empty, Cfg::WARPS * GROUPS);
         mbar_init(drained, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -166,7 +169,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *s_tmem, tmem_s = tmem + Cfg::O_COLS;
+    const uint32_t tmem = *s_tmem, tmem_s = tmem + Cfg::O_COLS, tmem_g = tmem_s + BUFS * NB;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -181,9 +184,16 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                 ++owns;
                 for (int t = 0; t < unit.tiles; ++t) {
                     if (!mbar_wait(&empty[s], parity, s_abort, a.d_error)) { live = false; break; }
-                    mbar_expect_tx(&full[s], Cfg::STAGE_BYTES);
+                    unsigned char* const column = s_columns + s * 2 * Cfg::COLUMN_BYTES;
+                    mbar_expect_tx(&full[s], Cfg::STAGE_BYTES + (ROWS ? 2 : BIAS ? 1 : 0) * Cfg::COLUMN_BYTES);
+                    if (ROWS) {
+                        bulk_load(column, a.terms + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
+                        bulk_load(column + Cfg::COLUMN_BYTES, a.marks + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
+                    } else if (BIAS) {
+                        bulk_load(column, a.bias + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
+                    }
                     for (int k = 0; k < KB; ++k)
-                        tma_load_3d(s_other + s * Cfg::STAGE_BYTES + k * (NB * 128), &tmOther, &full[s], k * 64, (unit.tile0 + t) * NB, 0);
+                        tma_load_3d(s_other + s * Cfg::STAGE_BYTES + k * (NB * 128), &tmOther, &full[s], k * 64, unit.tile(t) * NB, 0);
                     ++fills;
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
@@ -192,7 +202,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             s_fills[1] = owns;
         }
     } else if (warp == 1) {
-        constexpr int LAG = BUFS - 1;
+        constexpr int LAG = BUFS;
         // The second products follow the first ones by LAG tiles: where they are in the units.
         uint32_t n1 = 0, n2 = 0, owns = 0, units2 = 0;  // tiles, units
         unsigned u2 = blockIdx.x;
@@ -205,9 +215,9 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             tc_fence_after();
             const uint64_t db = tg_desc<false>(smem_u32(s_other + s * Cfg::STAGE_BYTES)) | ((uint64_t)((NB * 128) >> 4) << 16);
 #pragma unroll
-            for (int i = 0; i < NB / 16; ++i) tc_mma_ts_warp(tmem, tmem_s + b * NB + i * 8, db + i * 128, a.idesc_o, (t2 | i) != 0);
+            for (int k = 0; k < NB / 16; ++k) tc_mma_ts_warp(tmem, tmem_g + b * (NB / 2) + k * 8, db + k * 128, a.idesc_o, (t2 | k) != 0);
             tc_commit_warp(&empty[s]);
-            tc_commit_warp(&s_empty[b]);
+            tc_commit_warp(&g_empty[b]);
             ++n2;
             if (++t2 == tiles2) {
                 tc_commit_warp(o_full);
@@ -235,8 +245,8 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
 #pragma unroll
                 for (int k = 0; k < KB; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        tc_mma_warp<false>(tmem_s + b * NB, da + k * (TG_M * 128 / 16) + i * 2, db + k * (NB * 128 / 16) + i * 2, a.idesc_s, (k | i) != 0);
+                    for (int j = 0; j < 4; ++j)
+                        tc_mma_warp<false>(tmem_s + b * NB, da + k * (TG_M * 128 / 16) + j * 2, db + k * (NB * 128 / 16) + j * 2, a.idesc_s, (k | j) != 0);
                 tc_commit_warp(&s_full[b]);
                 if (t + 1 == unit.tiles) tc_commit_warp(&own_empty[o]);
                 if (n1 >= LAG && !second()) { live = false; break; }
@@ -244,93 +254,131 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
         }
         while (live && n2 < n1) live = second();
     } else {
-        const int quarter = warp & 3, group = (warp - 2) >> 2;
-        float* const columns = s_columns + (warp - 2) * (2 * NB);
+        constexpr int CW = Cfg::CW;
+        const int quarter = warp & 3, group = (warp - 2) / Cfg::WARPS, col0 = (warp - 2) % Cfg::WARPS / 4 * CW;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const int exponent = HALF ? ce_scale_exponent(a.amax) : 0;
+        // half precision: what brings the largest p (of queries), or p times its factor (of rows), next to 2^15
+        const int exponent = !HALF ? 0 : ROWS ? ce_scale_exponent(a.amax) : 14;
+        const uint64_t cc = f2_pack(a.c, a.c);
         bool live = true;
         uint32_t nth = 0, units = 0;
         for (unsigned u = blockIdx.x; u < a.units; u += gridDim.x, ++units) {
             const CeFusedUnit unit(a, u);
             const int first_own = unit.own0 + quarter * 32, mine = first_own + lane;
             const bool in = mine < a.own;
-            float my_term = 0.f, my_factor = 0.f;
-            int my_target = -1;
-            if (!ROWS && in) {
-                my_term = __ldcg(a.terms + mine);
-                my_factor = __ldcg(a.factors + mine);
-                if (HALF) my_factor = ldexpf(my_factor, exponent);
-                my_target = __ldcg(a.target_cols + mine);
+            float my_term = (float)exponent;
+            int my_target = -1, slot = -1;
+            if (in) {
+                if (!ROWS) {
+                    my_term += __ldcg(a.terms + mine);
+                    my_target = __ldcg(a.target_cols + mine);
+                } else {
+                    slot = __ldcg(a.where + mine);
+                    if (BIAS) my_term += __ldcg(a.bias + mine);
+                }
             }
-            if (ROWS && BIAS && in) my_term = __ldcg(a.bias + mine);
-            CeColumns<NB, ROWS, BIAS, HALF> next;
+            const uint64_t term2 = f2_pack(my_term, my_term);
             const int ahead = (int)((GROUPS + group - nth % GROUPS) % GROUPS);  // the group's first tile of the unit
-            if (ahead < unit.tiles) next.fetch(a, (unit.tile0 + ahead) * NB, a.other, lane);
             for (int t = ahead; t < unit.tiles; t += GROUPS) {
                 const uint32_t n = nth + t, b = n % BUFS;
-                const int first = (unit.tile0 + t) * NB;
-                int target[NB / 32];
+                const int first = unit.tile(t) * NB + col0;
+                const float* const columns = reinterpret_cast<const float*>(s_columns + n % STAGES * (2 * Cfg::COLUMN_BYTES)) + col0;
+                const int* const marks = reinterpret_cast<const int*>(columns + NB);
+                if ((ROWS || BIAS) && live) live = mbar_wait_warp(&full[n % STAGES], (n / STAGES) & 1u, s_abort, a.d_error);
+                // what is seldom: a target in the warp's part of the tile, the end of the other side; and negative factors
+                bool seldom, negative = false;
                 if (ROWS) {
+                    bool hit = false;
 #pragma unroll
-                    for (int i = 0; i < NB / 32; ++i) target[i] = next.target[i] - first_own;
+                    for (int i = 0; i < CW / 32; ++i) {
+                        const int mark = marks[i * 32 + lane];
+                        hit = hit || (unsigned)((mark & 0x7FFFFFFF) - 1 - first_own) < 32u;
+                        negative = negative || mark < 0;
+                    }
+                    seldom = __any_sync(0xFFFFFFFFu, hit);
+                    negative = __any_sync(0xFFFFFFFFu, negative);
+                } else {
+                    seldom = a.other - first < CW || __any_sync(0xFFFFFFFFu, (unsigned)(my_target - first) < (unsigned)CW);
                 }
-                next.put(columns, exponent, lane);
-                if (t + GROUPS < unit.tiles) next.fetch(a, first + GROUPS * NB, a.other, lane);
                 if (live) live = mbar_wait_warp(&s_full[b], (n / BUFS) & 1u, s_abort, a.d_error);
                 tc_fence_after();
-                const uint32_t place = tmem_s + lanes + b * NB;
+                const uint32_t from = tmem_s + lanes + b * NB + col0, to = tmem_g + lanes + b * (NB / 2) + col0 / 2;
+                uint32_t r[CW / 32][32];
 #pragma unroll
-                for (int c0 = 0; c0 < NB; c0 += 32) {
-                    uint32_t r[32];
-                    tc_ld32(place + c0, r);
-                    tc_ld_wait();
-                    float v[32];
+                for (int i = 0; i < CW / 32; ++i) tc_ld32(from + i * 32, r[i]);
+                tc_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_empty[b]);
+                if (live) live = mbar_wait_warp(&g_empty[b], ((n / BUFS) & 1u) ^ 1u, s_abort, a.d_error);
+                tc_fence_after();
+                auto make = [&](auto checked, auto signed_) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float s = __uint_as_float(r[j]);
-                        if (ROWS) v[j] = ce_exp2(fmaf(s, a.c, BIAS ? columns[c0 + j] + my_term : columns[c0 + j])) * columns[NB + c0 + j];
-                        else v[j] = ce_exp2(fmaf(s, a.c, BIAS ? my_term + columns[c0 + j] : my_term)) * my_factor;
-                    }
-                    if (ROWS) {
-                        unsigned hits = __ballot_sync(0xFFFFFFFFu, (unsigned)target[c0 / 32] < 32u);
-                        if (hits) {  // columns whose target is one of the warp's rows
-                            unsigned zero = 0;
-                            while (hits) {
-                                const int j = __ffs(hits) - 1;
-                                hits &= hits - 1u;
-                                if (__shfl_sync(0xFFFFFFFFu, target[c0 / 32], j) == lane) zero |= 1u << j;
+                    for (int i = 0; i < CW / 32; ++i) {
+                        float v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            uint64_t t0 = term2, t1 = term2;
+                            if (ROWS || BIAS) {
+                                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(columns + i * 32 + j);
+                                // queries: the exponent of half precision and the row's bias; rows: the query's term
+                                t0 = !ROWS || BIAS || HALF ? f2_add(x.x, term2) : x.x, t1 = !ROWS || BIAS || HALF ? f2_add(x.y, term2) : x.y;
                             }
+                            t0 = f2_fma(f2_pack(__uint_as_float(r[i][j]), __uint_as_float(r[i][j + 1])), cc, t0);
+                            t1 = f2_fma(f2_pack(__uint_as_float(r[i][j + 2]), __uint_as_float(r[i][j + 3])), cc, t1);
+                            f2_unpack(t0, v[j], v[j + 1]);
+                            f2_unpack(t1, v[j + 2], v[j + 3]);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (zero >> j & 1u) v[j] = 0.f;
+                            for (int k = j; k < j + 4; ++k) v[k] = ce_exp2(v[k]);
                         }
-                    } else {
-                        const int at = my_target - (first + c0), left = a.other - (first + c0);
-                        if (left < 32 || __any_sync(0xFFFFFFFFu, (unsigned)at < 32u)) {
+                        if (decltype(checked)::value) {
+                            if (ROWS) {
+                                const int target = (marks[i * 32 + lane] & 0x7FFFFFFF) - 1 - first_own;
+                                unsigned hits = __ballot_sync(0xFFFFFFFFu, (unsigned)target < 32u), zero = 0;
+                                while (hits) {  // columns whose target is one of the warp's rows
+                                    const int j = __ffs(hits) - 1;
+                                    hits &= hits - 1u;
+                                    if (__shfl_sync(0xFFFFFFFFu, target, j) == lane) zero |= 1u << j;
+                                }
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j == at || j >= left) v[j] = 0.f;
+                                for (int j = 0; j < 32; ++j)
+                                    if (zero >> j & 1u) v[j] = 0.f;
+                            } else {
+                                const int at = my_target - (first + i * 32), left = a.other - (first + i * 32);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (j == at || j >= left) v[j] = 0.f;
+                            }
                         }
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] = pack_scores(static_cast<const T*>(nullptr), v[2 * j], v[2 * j + 1]);
+                        if (ROWS && decltype(signed_)::value) {
+#pragma unroll
+                            for (int j = 0; j < 16; j += 2) {
+                                const int4 x = *reinterpret_cast<const int4*>(marks + i * 32 + 2 * j);
+                                w[j] ^= (uint32_t)(x.y & (int)0x80000000) | ((uint32_t)x.x >> 31) << 15;
+                                w[j + 1] ^= (uint32_t)(x.w & (int)0x80000000) | ((uint32_t)x.z >> 31) << 15;
+                            }
+                        }
+                        tg_store16(to + i * 16, w);
                     }
-                    uint32_t w[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) w[j] = pack_scores(static_cast<const T*>(nullptr), v[2 * j], v[2 * j + 1]);
-                    tg_store16(place + c0 / 2, w);
-                }
+                };
+                if (seldom) make(std::true_type(), std::true_type());
+                else if (negative) make(std::false_type(), std::bool_constant<ROWS>());
+                else make(std::false_type(), std::false_type());
                 tg_store_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&g_full[b]);
             }
             nth += unit.tiles;
-            // the sums, 32 columns to a group in turn
+            // the sums, 32 columns to four warps in turn
             if (live) live = mbar_wait_warp(o_full, units & 1u, s_abort, a.d_error);
             tc_fence_after();
-            int slot = -1;
-            if (ROWS && in) slot = __ldcg(a.where + mine);
             const bool wide = ROWS ? (a.d & 7) == 0 && (a.ld & 7) == 0 && ((uintptr_t)a.out & 15) == 0 : (a.d & 3) == 0;
 #pragma unroll 1
-            for (int c0 = group * 32; c0 < a.d; c0 += GROUPS * 32) {
+            for (int c0 = (warp - 2) / 4 * 32; c0 < a.d; c0 += Cfg::WARPS * GROUPS / 4 * 32) {
                 uint32_t r[32];
                 tg_read(tmem + lanes + c0, live, r);
                 if (!in) continue;

@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(256) ce_planes_kernel(const T* __restrict__ X,
 __global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ bias, int n, float* __restrict__ out) {
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i < n) out[i] = bias[i] * CE_LOG2E;
+    else if (i < ((n + 127) & ~127)) out[i] = 0.f;
 }
 
 // A warp joins a query's blocks.
@@ -397,10 +398,13 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
 // What the gradient takes of a query.
 __global__ void __launch_bounds__(256) ce_terms_kernel(const float* __restrict__ losses, const float* __restrict__ lse, const float* __restrict__ lse_low,
                                                        const int64_t* __restrict__ targets, const float* __restrict__ grad_losses, const float* __restrict__ grad_lse, int m,
-                                                       int n, float* __restrict__ terms, float* __restrict__ factors, float* __restrict__ own, int* __restrict__ cols,
-                                                       uint32_t* __restrict__ amax) {
+                                                       int n, float* __restrict__ terms, float* __restrict__ log_terms, int* __restrict__ marks, float* __restrict__ factors,
+                                                       float* __restrict__ own, int* __restrict__ cols, uint32_t* __restrict__ amax) {
     const int q = blockIdx.x * 256 + threadIdx.x;
-    if (q >= m) return;
+    if (q >= m) {
+        if (log_terms && q < ((m + 127) & ~127)) log_terms[q] = -INFINITY, marks[q] = 0;
+        return;
+    }
     const double two = ((double)lse[q] + (double)lse_low[q]) * 1.4426950408889634074;
     const float high = (float)two;
     const bool none = high == -INFINITY;
@@ -411,6 +415,10 @@ __global__ void __launch_bounds__(256) ce_terms_kernel(const float* __restrict__
     terms[q] = none ? -INFINITY : -high;
     const float f = (g + e) * (isfinite(high) ? (float)exp2(-(two - (double)high)) : 1.f);
     factors[q] = f;
+    if (log_terms) {
+        log_terms[q] = none ? -INFINITY : (float)(log2((double)fabsf(f)) - (double)high);
+        marks[q] = (has ? (int)t + 1 : 0) | (f < 0.f ? (int)0x80000000 : 0);
+    }
     cols[q] = has ? (int)t : -1;
     own[q] = has ? g * expm1f(-loss) + e * expf(-loss) : 0.f;
     if (amax && isfinite(f)) atomicMax(amax, __float_as_uint(fabsf(f)));
@@ -497,10 +505,11 @@ __global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ col
     for (int r = threadIdx.x; r < CE_OWN_ROWS && row0 + r < n; r += 256) where[row0 + r] = s_first[r];
 }
 
-// Gradients from sums: out[row][col] = (sum over the splits / scale + the target's part) / T.  QUERIES: the target's part is own[row] times the row cols[row] of X; else sums[where[row]].
+// Gradients from sums: out[row][col] = (sum over the splits / scale + the target's part) / T.  factors: of the rows, where the sums are of p alone.  QUERIES: the target's part is own[row] times the row cols[row] of X; else sums[where[row]].
 template <typename T, bool QUERIES>
 __global__ void __launch_bounds__(256) ce_finish_kernel(const float* __restrict__ parts, int splits, int64_t split_stride, int64_t rows, int d, const uint32_t* __restrict__ amax,
-                                                        const int* __restrict__ which, const float* __restrict__ own, const T* __restrict__ X, int64_t ldx,
+                                                        const float* __restrict__ factors, const int* __restrict__ which, const float* __restrict__ own,
+                                                        const T* __restrict__ X, int64_t ldx,
                                                         const float* __restrict__ sums, float inv_t, T* __restrict__ out, int64_t ldo) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= rows * d) return;
@@ -508,7 +517,8 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(const float* __restrict_
     const int col = (int)(i - row * d);
     float v = 0.f;
     for (int s = 0; s < splits; ++s) v += parts[s * split_stride + i];
-    if (amax) v = ldexpf(v, -ce_scale_exponent(amax));
+    if (factors) v *= std::is_same<T, __half>::value ? ldexpf(factors[row], -14) : factors[row];
+    else if (amax) v = ldexpf(v, -ce_scale_exponent(amax));
     const int w = which[row];
     if (w >= 0) v += QUERIES ? own[row] * ce_float(X[(int64_t)w * ldx + col]) : sums[(int64_t)w * d + col];
     out[row * ldo + col] = (T)(v * inv_t);
@@ -557,8 +567,8 @@ struct CePlan {
     float2* partial = nullptr;
     float* target_scores = nullptr;
     // backward
-    float *terms = nullptr, *factors = nullptr, *own = nullptr, *sums = nullptr;
-    int *cols = nullptr, *where = nullptr;
+    float *terms = nullptr, *log_terms = nullptr, *factors = nullptr, *own = nullptr, *sums = nullptr;
+    int *cols = nullptr, *marks = nullptr, *where = nullptr;
     uint32_t* amax = nullptr;
     int piece = 0;  // rows
     uint16_t* G = nullptr;
@@ -571,7 +581,7 @@ struct CePlan {
         const int sms = k.c->sm_count;
         if (k.copies(k.Q, k.ldq)) q_planes = space.take<uint16_t>((size_t)k.planes() * k.m * k.pitch());
         if (k.copies(k.X, k.ldx) || (backward && k.bias)) x_planes = space.take<uint16_t>((size_t)k.planes() * k.n * k.pitch());
-        if (k.bias) bias2 = space.take<float>(k.n);
+        if (k.bias) bias2 = space.take<float>(ceil_div(k.n, 128) * 128);
         const size_t tiles_q = ceil_div(k.m, TG_M), tiles_n = ceil_div(k.n, CE_BN);
         if (!backward) {
             block = (int)std::max<size_t>(1, std::min<size_t>(16, tiles_q * tiles_n / ((size_t)sms * 8)));
@@ -586,6 +596,7 @@ struct CePlan {
         // G stays on the SM where rows are short enough; sums of more than 32,768 entries would have to be split for dX too
         const bool fused = k.planes() == 1 && k.d <= 256;
         fused_q = need_q && fused, fused_x = need_x && fused && k.m <= 32768;
+        if (fused_x) log_terms = space.take<float>(tiles_q * TG_M), marks = space.take<int>(tiles_q * TG_M);
         if (need_x) {
             sums = space.take<float>((size_t)k.m * k.d);
             where = space.take<int>(k.n);
@@ -721,7 +732,7 @@ inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, vo
     const size_t units = ceil_div(a.tiles_other, a.block) * a.tiles_own;
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
-    a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = p.terms, a.factors = p.factors, a.amax = p.amax, a.target_cols = p.cols;
+    a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = ROWS ? p.log_terms : p.terms, a.marks = p.marks, a.amax = p.amax, a.target_cols = p.cols;
     a.parts = p.acc_q, a.out = out, a.ld = ld, a.where = p.where, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
     const CUtensorMap own = ROWS ? ops.map_x(k, TG_M) : ops.map_q(k, TG_M), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
     auto go = [&](auto boxes) {
@@ -743,7 +754,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
     const CeOperands ops(k, p);
     const float inv_t = (float)(1 / k.temperature);
     if (p.amax) CU_CHECK(cudaMemsetAsync(p.amax, 0, 4, k.stream));
-    ce_terms_kernel<<<ce_grid(k.m), 256, 0, k.stream>>>(losses, lse, lse_low, k.targets, grad_losses, grad_lse, k.m, k.n, p.terms, p.factors, p.own, p.cols, p.amax);
+    ce_terms_kernel<<<ce_grid(k.m), 256, 0, k.stream>>>(losses, lse, lse_low, k.targets, grad_losses, grad_lse, k.m, k.n, p.terms, p.log_terms, p.marks, p.factors, p.own, p.cols, p.amax);
     KERNEL_CHECK();
     if (grad_X) {
         ce_own_kernel<<<(unsigned)ceil_div(k.n, CE_OWN_ROWS), 256, 0, k.stream>>>(p.cols, p.own, static_cast<const T*>(k.Q), k.ldq, k.m, k.n, k.d, p.sums, p.where);
@@ -776,7 +787,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
             CeProductArgs a{};
             a.rows = here, a.b0 = 0, a.kb = (int)ceil_div(k.m, 64), a.out = p.parts_x;
             ce_product<PLANES, true>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, 64), ops.q, ops.ldq, k.m, a, p.per_x, p.splits_x);
-            ce_finish_kernel<T, false><<<ce_grid((size_t)here * k.d), 256, 0, k.stream>>>(p.parts_x, p.splits_x, (int64_t)here * k.d, here, k.d, p.amax, p.where + n0, nullptr,
+            ce_finish_kernel<T, false><<<ce_grid((size_t)here * k.d), 256, 0, k.stream>>>(p.parts_x, p.splits_x, (int64_t)here * k.d, here, k.d, p.amax, nullptr, p.where + n0, nullptr,
                                                                                            nullptr, 0, p.sums, inv_t, grad_X + n0 * ld_gx, ld_gx);
             KERNEL_CHECK();
         }
@@ -787,7 +798,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         }
     }
     if (grad_Q) {
-        ce_finish_kernel<T, true><<<ce_grid((size_t)k.m * k.d), 256, 0, k.stream>>>(p.acc_q, p.splits_q, (int64_t)k.m * k.d, k.m, k.d, p.amax, p.cols, p.own,
+        ce_finish_kernel<T, true><<<ce_grid((size_t)k.m * k.d), 256, 0, k.stream>>>(p.acc_q, p.splits_q, (int64_t)k.m * k.d, k.m, k.d, p.amax, p.fused_q ? p.factors : nullptr, p.cols, p.own,
                                                                                      static_cast<const T*>(k.X), k.ldx, nullptr, inv_t, grad_Q, ld_gq);
         KERNEL_CHECK();
     }
