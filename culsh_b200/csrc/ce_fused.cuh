@@ -6,7 +6,7 @@
 // for each of the m n entries.
 //
 // The factor of a query's entries is a part of its term (log2 of its magnitude) where queries are the columns, and goes to the sums where they are the lanes.
-// One warp loads, one issues the MMAs, two groups of eight warps take the tiles in turn, a thread half the columns of a lane.  S and G have two places each, and the second product of a tile is
+// One warp loads, one issues the first products and one the second (a single one, issuing 16 MMAs a tile and waiting three times, held them up), two groups of eight warps take the tiles in turn, a thread half the columns of a lane.  S and G have two places each, and the second product of a tile is
 // issued two tiles behind its first: what an MMA writes over has been read by the epilogue long before, and the tensor pipe has another product to do while a G is made.  (G on top of S, in three
 // places: the first product had to wait until the second one in front of it was done, 4,096 x 1M x 128 4.34 ms.)  Sums of more than 32,768 entries are split (the accumulators cut off,
 // see tc_gemm.cuh), those of dQ over units, whose sums ce_finish_kernel adds up.
@@ -62,8 +62,11 @@ struct CeFusedCfg {
     static constexpr int CW = NB / 2;                         // columns of a warp
     static constexpr int OWN_BYTES = KB * TG_M * 128, OWNS = KB == 1 ? 2 : 1;
     static constexpr int STAGE_BYTES = KB * NB * 128, COLUMN_BYTES = NB * 4, STAGES = KB == 1 ? 8 : KB == 2 ? 5 : 4;
-    static constexpr int THREADS = 64 + 32 * WARPS * GROUPS;
+    static constexpr int THREADS = 128 + 32 * WARPS * GROUPS;  // warps for the loads, either product, and one that idles
 // (terms and marks, or the bias, of a stage's entries lie behind the stages)
+    // 640 threads are launched with 96 registers each; four warps give up some, which the others take: 128 x 32 + 512 x 112 = 640 x 96
+    static constexpr int REGS = 96, FEW_REGS = 32, MANY_REGS = 112;
+    static_assert(128 * FEW_REGS + 32 * WARPS * GROUPS * MANY_REGS <= THREADS * REGS, "");
     static constexpr int SMEM = OWNS * OWN_BYTES + STAGES * (STAGE_BYTES + 2 * COLUMN_BYTES) + 1024 /*barriers*/ + 1024 /*alignment slack*/;
     static_assert(O_COLS + BUFS * (NB + NB / 2) <= 512 && SMEM <= 227 * 1024 && STAGES > BUFS, "");
 };
@@ -158,7 +161,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
         for (int i = 0; i < BUFS; ++i) mbar_init(&s_full[i], 1), mbar_init(&s_empty[i], Cfg::WARPS), mbar_init(&g_full[i], Cfg::WARPS), mbar_init(&g_empty[i], 1);
         mbar_init(o_full, 1);
         mbar_init(o_empty, Cfg::WARPS * GROUPS);
-        mbar_init(drained, 1);
+        mbar_init(drained, 2);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -172,6 +175,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
     const uint32_t tmem = *s_tmem, tmem_s = tmem + Cfg::O_COLS, tmem_g = tmem_s + BUFS * NB;
 
     if (warp == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::FEW_REGS));
         if (lane == 0) {
             uint32_t s = 0, parity = 1, fills = 0, owns = 0;
             bool live = true;
@@ -201,42 +205,19 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             s_fills[0] = fills;
             s_fills[1] = owns;
         }
-    } else if (warp == 1) {
-        constexpr int LAG = BUFS;
-        // The second products follow the first ones by LAG tiles: where they are in the units.
-        uint32_t n1 = 0, n2 = 0, owns = 0, units2 = 0;  // tiles, units
-        unsigned u2 = blockIdx.x;
-        int t2 = 0, tiles2 = u2 < a.units ? CeFusedUnit(a, u2).tiles : 0;
+    } else if (warp == 1) {  // first products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::FEW_REGS));
+        uint32_t n = 0, s = 0, s_parity = 0, owns = 0;
         bool live = true;
-        auto second = [&]() {
-            const uint32_t b = n2 % BUFS, s = n2 % STAGES;
-            if (t2 == 0 && !mbar_wait_warp(o_empty, (units2 & 1u) ^ 1u, s_abort, a.d_error)) return false;
-            if (!mbar_wait_warp(&g_full[b], (n2 / BUFS) & 1u, s_abort, a.d_error)) return false;
-            tc_fence_after();
-            const uint64_t db = tg_desc<false>(smem_u32(s_other + s * Cfg::STAGE_BYTES)) | ((uint64_t)((NB * 128) >> 4) << 16);
-#pragma unroll
-            for (int k = 0; k < NB / 16; ++k) tc_mma_ts_warp(tmem, tmem_g + b * (NB / 2) + k * 8, db + k * 128, a.idesc_o, (t2 | k) != 0);
-            tc_commit_warp(&empty[s]);
-            tc_commit_warp(&g_empty[b]);
-            ++n2;
-            if (++t2 == tiles2) {
-                tc_commit_warp(o_full);
-                ++units2;
-                t2 = 0;
-                u2 += gridDim.x;
-                tiles2 = u2 < a.units ? CeFusedUnit(a, u2).tiles : 0;
-            }
-            return true;
-        };
         for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x) {
             const CeFusedUnit unit(a, u);
             const uint32_t o = owns % OWNS;
-            if (!mbar_wait_warp(&own_full[o], (owns / OWNS) & 1u, s_abort, a.d_error)) { live = false; break; }
+            if (!mbar_wait_warp(&own_full[o], (owns / OWNS) & 1u, s_abort, a.d_error)) break;
             ++owns;
             const uint64_t da = tg_desc<false>(smem_u32(base + o * Cfg::OWN_BYTES));
-            for (int t = 0; t < unit.tiles; ++t, ++n1) {
-                const uint32_t b = n1 % BUFS, s = n1 % STAGES;
-                if (!mbar_wait_warp(&s_empty[b], ((n1 / BUFS) & 1u) ^ 1u, s_abort, a.d_error) || !mbar_wait_warp(&full[s], (n1 / STAGES) & 1u, s_abort, a.d_error)) {
+            for (int t = 0; t < unit.tiles; ++t, ++n) {
+                const uint32_t b = n % BUFS;
+                if (!mbar_wait_warp(&s_empty[b], ((n / BUFS) & 1u) ^ 1u, s_abort, a.d_error) || !mbar_wait_warp(&full[s], s_parity, s_abort, a.d_error)) {
                     live = false;
                     break;
                 }
@@ -249,13 +230,35 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                         tc_mma_warp<false>(tmem_s + b * NB, da + k * (TG_M * 128 / 16) + j * 2, db + k * (NB * 128 / 16) + j * 2, a.idesc_s, (k | j) != 0);
                 tc_commit_warp(&s_full[b]);
                 if (t + 1 == unit.tiles) tc_commit_warp(&own_empty[o]);
-                if (n1 >= LAG && !second()) { live = false; break; }
+                if (++s == STAGES) { s = 0; s_parity ^= 1u; }
             }
         }
-        while (live && n2 < n1) live = second();
+    } else if (warp == 2) {  // second products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::FEW_REGS));
+        uint32_t n = 0, s = 0, units = 0;
+        bool live = true;
+        for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x, ++units) {
+            const CeFusedUnit unit(a, u);
+            if (!mbar_wait_warp(o_empty, (units & 1u) ^ 1u, s_abort, a.d_error)) break;
+            for (int t = 0; t < unit.tiles; ++t, ++n) {
+                const uint32_t b = n % BUFS;
+                if (!mbar_wait_warp(&g_full[b], (n / BUFS) & 1u, s_abort, a.d_error)) { live = false; break; }
+                tc_fence_after();
+                const uint64_t db = tg_desc<false>(smem_u32(s_other + s * Cfg::STAGE_BYTES)) | ((uint64_t)((NB * 128) >> 4) << 16);
+#pragma unroll
+                for (int k = 0; k < NB / 16; ++k) tc_mma_ts_warp(tmem, tmem_g + b * (NB / 2) + k * 8, db + k * 128, a.idesc_o, (t | k) != 0);
+                tc_commit_warp(&empty[s]);
+                tc_commit_warp(&g_empty[b]);
+                if (++s == STAGES) s = 0;
+            }
+            if (live) tc_commit_warp(o_full);
+        }
+    } else if (warp == 3) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::FEW_REGS));
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::MANY_REGS));
         constexpr int CW = Cfg::CW;
-        const int quarter = warp & 3, group = (warp - 2) / Cfg::WARPS, col0 = (warp - 2) % Cfg::WARPS / 4 * CW;
+        const int quarter = warp & 3, group = (warp - 4) / Cfg::WARPS, col0 = (warp - 4) % Cfg::WARPS / 4 * CW;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         // half precision: what brings the largest p (of queries), or p times its factor (of rows), next to 2^15
         const int exponent = !HALF ? 0 : ROWS ? ce_scale_exponent(a.amax) : 14;
@@ -378,7 +381,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             tc_fence_after();
             const bool wide = ROWS ? (a.d & 7) == 0 && (a.ld & 7) == 0 && ((uintptr_t)a.out & 15) == 0 : (a.d & 3) == 0;
 #pragma unroll 1
-            for (int c0 = (warp - 2) / 4 * 32; c0 < a.d; c0 += Cfg::WARPS * GROUPS / 4 * 32) {
+            for (int c0 = (warp - 4) / 4 * 32; c0 < a.d; c0 += Cfg::WARPS * GROUPS / 4 * 32) {
                 uint32_t r[32];
                 tg_read(tmem + lanes + c0, live, r);
                 if (!in) continue;
@@ -435,7 +438,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             mbar_wait_landed(full, STAGES, s_fills[0]);
             mbar_wait_landed(own_full, OWNS, s_fills[1]);
         }
-        if (warp == 1) {
+        if (warp == 1 || warp == 2) {
             tc_commit_warp(drained);
             mbar_wait_landed(drained, 1, 1);
         }
@@ -452,6 +455,9 @@ inline void ce_fused_launch(const CtxPtr& c, const CUtensorMap& own, const CUten
     using Cfg = CeFusedCfg<KB>;
     static thread_local uint64_t ready = 0;  // devices whose limit is set
     if (c->device >= 64 || !(ready >> c->device & 1)) {
+        cudaFuncAttributes is;
+        CU_CHECK(cudaFuncGetAttributes(&is, ce_fused_kernel<KB, ROWS, BIAS, HALF>));
+        if (is.numRegs != Cfg::REGS) fail(CULSH_ERR_INTERNAL, "built with %d registers a thread in place of %d", is.numRegs, Cfg::REGS);  // the warps' shares would not add up
         CU_CHECK(cudaFuncSetAttribute(ce_fused_kernel<KB, ROWS, BIAS, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
         if (c->device < 64) ready |= 1ull << c->device;
     }
