@@ -23,8 +23,9 @@
 
 namespace culsh_b200 {
 
-constexpr int CE_BN = 256, CE_HALF = CE_BN / 2;
+constexpr int CE_BN = 256, CE_PART = CE_BN / 4;  // columns of a tile, and of it for a warp
 constexpr int CE_SEGMENT = 8;  // steps of 64
+constexpr int CE_SLOTS = CE_BN / CE_PART;  // partial sums of a block of rows
 
 struct CeScoreArgs {
     int* d_error;
@@ -32,7 +33,7 @@ struct CeScoreArgs {
     uint32_t idesc;
     int m, kb;                // queries; steps of K
     int n0, n1;               // rows of this call
-    int block, tiles_q;       // tiles of rows in a unit, tiles of queries
+    int block, tiles_q, m_tile;  // tiles of rows in a unit; tiles of queries, and their size
     unsigned tiles_n;
     float c;
     const float* bias;        // of the rows, in powers of two, or NULL
@@ -54,135 +55,157 @@ struct CeUnit {
     int m0, tile0, tiles, k0, k1, block;
     __device__ __forceinline__ CeUnit(const CeScoreArgs& a, unsigned u) {
         block = (int)(u / (unsigned)a.tiles_q);
-        m0 = (int)(u - (unsigned)block * a.tiles_q) * TG_M;
+        m0 = (int)(u - (unsigned)block * a.tiles_q) * a.m_tile;
         tile0 = block * a.block;
         tiles = min(a.block, (int)a.tiles_n - tile0);
         k0 = 0, k1 = a.kb;
     }
 };
 
-template <int PLANES, bool SEGMENTS>
+template <int PLANES, bool SEGMENTS, bool PAIRS>
 struct CeScoreBase {
-    static constexpr bool A_MN = false, B_MN = false, I8 = false, HALVES = true;
-    static constexpr int BN = CE_BN, SEGMENT = SEGMENTS ? CE_SEGMENT : 0;
-    static constexpr int EPI_BYTES = TG_EPI_WARPS * (BN / 2) * 4;
+    static constexpr bool A_MN = false, B_MN = false, I8 = false, PARTS = true, PAIR = PAIRS;
+    static constexpr int BN = CE_BN, SEGMENT = SEGMENTS ? CE_SEGMENT : 0, EPI_WARPS = 16;
+    static constexpr int EPI_BYTES = EPI_WARPS * CE_PART * 4;
     using Pairs = PlanePairs<PLANES>;
     using Args = CeScoreArgs;
     using Unit = CeUnit;
     static __device__ __forceinline__ void load(const Args& a, const Unit& u, int t, int pa, int pb, int k, const CUtensorMap* ta, const CUtensorMap* tb, unsigned char* sa,
-                                                unsigned char* sb, uint64_t* bar) {
-        tma_load_3d(sa, ta, bar, k * 64, u.m0, pa);
-        tma_load_3d(sb, tb, bar, k * 64, a.n0 + (u.tile0 + t) * BN, pb);
+                                                unsigned char* sb, uint32_t bar, int rank) {
+        tma_load_3d<PAIR>(sa, ta, bar, k * 64, u.m0 + rank * TG_M, pa);
+        tma_load_3d<PAIR>(sb, tb, bar, k * 64, a.n0 + (u.tile0 + t) * BN + rank * (BN / 2), pb);
     }
     static __device__ __forceinline__ int n_mma(const Args& a, const Unit& u, int t) { return min(BN, (a.n1 - a.n0 - (u.tile0 + t) * BN + 15) & ~15); }
 };
 
-// The rows' terms of half a tile, for one warp.
+// The rows' terms of a warp's part of a tile.
 __device__ __forceinline__ void ce_bias_tile(const float* bias, int n0, int n1, float* s, int lane) {
     __syncwarp();
 #pragma unroll
-    for (int i = lane; i < CE_HALF; i += 32) s[i] = n0 + i < n1 ? __ldcg(bias + n0 + i) : 0.f;
+    for (int i = lane; i < CE_PART; i += 32) s[i] = n0 + i < n1 ? __ldcg(bias + n0 + i) : -INFINITY;
     __syncwarp();
 }
 
-// The sums of a tile's segments, for a thread's 128 columns of one lane.
+// The sums of a tile's segments, for a thread's columns of one lane.
 template <bool SEGMENTS>
 struct CeSums {
-    float v[SEGMENTS ? CE_HALF : 1];
+    static_assert(CE_PART == 64, "");
+    float v[SEGMENTS ? CE_PART : 1];
     __device__ __forceinline__ void segment(const CeScoreArgs&, bool first, uint32_t taddr, bool live) {
         if constexpr (SEGMENTS) {
+            auto each = [&](auto&& f) {
 #pragma unroll
-            for (int c0 = 0; c0 < CE_HALF; c0 += 16) {
-                uint32_t r[16];
-                tc_ld16(taddr + c0, r);
-                tc_ld_wait();
+                for (int c0 = 0; c0 < CE_PART; c0 += 16) {
+                    uint32_t r[16];
+                    tc_ld16(taddr + c0, r);
+                    tc_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[c0 + j] = !live ? __int_as_float(0x7FFFFFFF) : first ? __uint_as_float(r[j]) : v[c0 + j] + __uint_as_float(r[j]);
-            }
+                    for (int j = 0; j < 16; ++j) f(v[c0 + j], live ? __uint_as_float(r[j]) : __int_as_float(0x7FFFFFFF));
+                }
+            };
+            if (first) each([](float& to, float from) { to = from; });
+            else each([](float& to, float from) { to += from; });
         }
     }
-    // 32 columns from c0 on, where the last segment has been added.
-    __device__ __forceinline__ void read(uint32_t taddr, int c0, bool live, uint32_t (&r)[32]) {
+    // All of them, where this is the last segment: f(columns).
+    template <typename F>
+    __device__ __forceinline__ void read(const CeScoreArgs& a, uint32_t taddr, bool live, bool more, F&& f) {
         if constexpr (SEGMENTS) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(v[c0 + j]);
+            segment(a, !more, taddr, live);
+            f(v);
         } else {
-            tg_read(taddr + c0, live, r);
+            uint32_t r[2][32];
+            tc_ld32(taddr, r[0]);
+            tc_ld32(taddr + 32, r[1]);
+            tc_ld_wait();
+            float x[CE_PART];
+#pragma unroll
+            for (int j = 0; j < CE_PART; ++j) x[j] = live ? __uint_as_float(r[j / 32][j % 32]) : __int_as_float(0x7FFFFFFF);
+            f(x);
         }
     }
 };
 
-template <int PLANES, bool BIAS, bool SEGMENTS>
-struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS> {
+// A thread keeps the running maximum (in powers of two) of its part of a query's scores, and the sum of exponentials by it.  Of a batch, bound by the exponentials (16 a cycle and SM).
+template <int PLANES, bool BIAS, bool SEGMENTS, bool PAIRS>
+struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
     struct Epilogue : CeSums<SEGMENTS> {
-        int q, quarter, group, lane, target;
+        int q, quarter, group, lane, rank, target;
         bool idle;
         float ref, sum;
         float* s_bias;
-        __device__ __forceinline__ Epilogue(const CeScoreArgs&, unsigned char* smem, int warp, int quarter_, int group_, int lane_)
-            : quarter(quarter_), group(group_), lane(lane_), s_bias(reinterpret_cast<float*>(smem) + warp * CE_HALF) {}
+        __device__ __forceinline__ Epilogue(const CeScoreArgs&, unsigned char* smem, int warp, int quarter_, int group_, int lane_, int rank_)
+            : quarter(quarter_), group(group_), lane(lane_), rank(rank_), s_bias(reinterpret_cast<float*>(smem) + warp * CE_PART) {}
         __device__ __forceinline__ void unit_begin(const CeScoreArgs& a, const CeUnit& u) {
-            q = u.m0 + quarter * 32 + lane;
+            q = u.m0 + rank * TG_M + quarter * 32 + lane;
             idle = q - lane >= a.m;
             ref = -INFINITY, sum = 0.f;
             const int64_t t = q < a.m && a.targets ? __ldcg(a.targets + q) : -1;
             target = t < 0 || t >= a.n1 ? -1 : (int)t;
         }
-        __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more) {
-            if (idle) return;
-            if (SEGMENTS) this->segment(a, !more, taddr, live);
-            const int n0 = a.n0 + (u.tile0 + t) * CE_BN + group * CE_HALF;
-            if (BIAS) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
-#pragma unroll(SEGMENTS ? CE_HALF / 32 : 1)
-            for (int c0 = 0; c0 < CE_HALF; c0 += 32) {
-                const int left = a.n1 - n0 - c0;
-                if (left <= 0) break;
-                uint32_t r[32];
-                this->read(taddr, c0, live, r);
-                const int at = target - (n0 + c0);
-                if (__any_sync(0xFFFFFFFFu, (unsigned)at < 32u)) {
-                    float v = 0.f;
+        // x: scores, or exponents where there is a bias
+        __device__ __forceinline__ void add(const CeScoreArgs& a, float (&x)[CE_PART]) {
+            float top = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (j == at) v = __uint_as_float(r[j]);
-                    if ((unsigned)at < 32u) a.target_scores[q] = v;
-                }
-                float x[32], top = -INFINITY;
+            for (int j = 0; j < CE_PART; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
+            const float next = fmaxf(ref, BIAS ? top : top * a.c), base = next == -INFINITY ? 0.f : next;
+            const uint64_t cc = f2_pack(a.c, a.c), minus = f2_pack(-base, -base);
+            uint64_t part[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    x[j] = __uint_as_float(r[j]);
-                    if (BIAS) {  // a row that is masked may hold anything
-                        const float b = s_bias[c0 + j];
-                        x[j] = b == -INFINITY ? b : fmaf(x[j], a.c, b);
-                    }
-                    if (j >= left) x[j] = -INFINITY;
-                    top = fmaxf(top, x[j]);
-                }
-                const float next = fmaxf(ref, BIAS ? top : top * a.c), base = next == -INFINITY ? 0.f : next;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < 32; ++j) part[j & 3] += ce_exp2(BIAS ? x[j] - base : fmaf(x[j], a.c, -base));
-                sum = fmaf(sum, ce_exp2(ref - base), (part[0] + part[1]) + (part[2] + part[3]));
-                ref = next;
+            for (int j = 0; j < CE_PART; j += 2) {
+                const uint64_t pair = f2_pack(x[j], x[j + 1]);
+                float e0, e1;
+                f2_unpack(BIAS ? f2_add(pair, minus) : f2_fma(pair, cc, minus), e0, e1);
+                part[j / 2 & 3] = f2_add(part[j / 2 & 3], f2_pack(ce_exp2(e0), ce_exp2(e1)));
             }
+            float lo, hi;
+            f2_unpack(f2_add(f2_add(part[0], part[1]), f2_add(part[2], part[3])), lo, hi);
+            sum = fmaf(sum, ce_exp2(ref - base), lo + hi);
+            ref = next;
+        }
+        template <typename D>
+        __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more, D&& done) {
+            const int n0 = a.n0 + (u.tile0 + t) * CE_BN + group * CE_PART, left = a.n1 - n0, at = target - n0;
+            if (BIAS && !idle) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
+            this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
+            done();
+            if (idle) return;
+            if (left < CE_PART || __any_sync(0xFFFFFFFFu, (unsigned)at < (unsigned)CE_PART)) {  // seldom
+                float v = 0.f;
+#pragma unroll
+                for (int j = 0; j < CE_PART; ++j) {
+                    if (j == at) v = x[j];
+                    if (!BIAS && j >= left) x[j] = -INFINITY;
+                }
+                if ((unsigned)at < (unsigned)CE_PART) a.target_scores[q] = v;
+            }
+            if (BIAS) {
+#pragma unroll
+                for (int j = 0; j < CE_PART; ++j) {  // a row that is masked may hold anything
+                    const float b = s_bias[j];
+                    x[j] = b == -INFINITY ? b : fmaf(x[j], a.c, b);
+                }
+            }
+            add(a, x);
+            });
         }
         __device__ __forceinline__ void unit_end(const CeScoreArgs& a, const CeUnit& u) {
-            if (q < a.m) a.partial[(int64_t)q * a.slots + u.block * 2 + group] = make_float2(ref, sum);
+            if (q < a.m) a.partial[(int64_t)q * a.slots + u.block * CE_SLOTS + group] = make_float2(ref, sum);
         }
     };
 };
 
-template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS>
-struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS> {
+template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS, bool PAIRS>
+struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
     struct Epilogue : CeSums<SEGMENTS> {
-        int q, quarter, group, lane, target;
+        int q, quarter, group, lane, rank, target;
         bool idle;
         float term, factor;
         float* s_bias;
-        __device__ __forceinline__ Epilogue(const CeScoreArgs&, unsigned char* smem, int warp, int quarter_, int group_, int lane_)
-            : quarter(quarter_), group(group_), lane(lane_), s_bias(reinterpret_cast<float*>(smem) + warp * CE_HALF) {}
+        __device__ __forceinline__ Epilogue(const CeScoreArgs&, unsigned char* smem, int warp, int quarter_, int group_, int lane_, int rank_)
+            : quarter(quarter_), group(group_), lane(lane_), rank(rank_), s_bias(reinterpret_cast<float*>(smem) + warp * CE_PART) {}
         __device__ __forceinline__ void unit_begin(const CeScoreArgs& a, const CeUnit& u) {
-            q = u.m0 + quarter * 32 + lane;
+            q = u.m0 + rank * TG_M + quarter * 32 + lane;
             idle = q - lane >= a.m;
             const bool in = q < a.m;
             term = in ? __ldcg(a.terms + q) : 0.f;
@@ -190,52 +213,42 @@ struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS> {
             target = in ? __ldcg(a.target_cols + q) : -1;
             if (HALF) factor = ldexpf(factor, ce_scale_exponent(a.amax));
         }
-        __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more) {
+        template <typename D>
+        __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more, D&& done) {
+            const int first = (u.tile0 + t) * CE_BN + group * CE_PART, n0 = a.n0 + first, left = a.n1 - n0, at = target - n0;
+            if (BIAS && !idle) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
+            this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
+            done();
             if (idle) return;
-            if (SEGMENTS) this->segment(a, !more, taddr, live);
-            const int first = (u.tile0 + t) * CE_BN + group * CE_HALF, n0 = a.n0 + first;
-            if (BIAS) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
+#pragma unroll
+            for (int j = 0; j < CE_PART; ++j) x[j] = ce_exp2(fmaf(x[j], a.c, BIAS ? term + s_bias[j] : term)) * factor;
+            if (left < CE_PART || __any_sync(0xFFFFFFFFu, (unsigned)at < (unsigned)CE_PART)) {  // seldom; behind the last row G has zeros
+#pragma unroll
+                for (int j = 0; j < CE_PART; ++j)
+                    if (j == at || j >= left) x[j] = 0.f;
+            }
+            if (q >= a.m) return;
             uint16_t* const out = reinterpret_cast<uint16_t*>(a.G) + (int64_t)q * a.pitch + first;
-#pragma unroll(SEGMENTS ? CE_HALF / 32 : 1)
-            for (int c0 = 0; c0 < CE_HALF; c0 += 32) {
-                const int left = a.n1 - n0 - c0;  // behind the last row G has zeros
-                uint32_t r[32];
-                this->read(taddr, c0, live, r);
-                float v[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float s = __uint_as_float(r[j]);
-                    v[j] = ce_exp2(fmaf(s, a.c, BIAS ? term + s_bias[c0 + j] : term)) * factor;
-                    if (j >= left) v[j] = 0.f;
-                }
-                const int at = target - (n0 + c0);
-                if (__any_sync(0xFFFFFFFFu, (unsigned)at < 32u)) {
+            for (int p = 0; p < PLANES; ++p) {
+                uint4* const o = reinterpret_cast<uint4*>(out + p * a.plane);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (j == at) v[j] = 0.f;
-                }
-                if (q < a.m) {
+                for (int i = 0; i < CE_PART / 8; ++i) {
+                    uint32_t w[4];
 #pragma unroll
-                    for (int p = 0; p < PLANES; ++p) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            if (HALF) {
-                                w[j] = pack_scores(static_cast<const __half*>(nullptr), v[2 * j], v[2 * j + 1]);
-                            } else {
-                                w[j] = pack_scores(static_cast<const __nv_bfloat16*>(nullptr), v[2 * j], v[2 * j + 1]);
-                                if (p + 1 < PLANES) {
-                                    v[2 * j] -= __uint_as_float(w[j] << 16);
-                                    v[2 * j + 1] -= __uint_as_float(w[j] & 0xFFFF0000u);
-                                }
-                            }
+                    for (int k = 0; k < 4; ++k) {
+                        float &lo = x[8 * i + 2 * k], &hi = x[8 * i + 2 * k + 1];
+                        if (HALF) {
+                            w[k] = pack_scores(static_cast<const __half*>(nullptr), lo, hi);
+                        } else {
+                            w[k] = pack_scores(static_cast<const __nv_bfloat16*>(nullptr), lo, hi);
+                            if (p + 1 < PLANES) lo -= __uint_as_float(w[k] << 16), hi -= __uint_as_float(w[k] & 0xFFFF0000u);
                         }
-                        uint4* const o = reinterpret_cast<uint4*>(out + p * a.plane + c0);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                     }
+                    o[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
+            });
         }
         __device__ __forceinline__ void unit_end(const CeScoreArgs&, const CeUnit&) {}
     };
@@ -249,7 +262,7 @@ struct CeProductArgs {
     int rows, cols;
     int b0;                   // entry of K that B begins with
     int kb, kper;             // steps of K, and as many in a split
-    int tiles_m, tiles_n;
+    int tiles_m, tiles_n, m_tile;
     bool accumulate;
     float* out;
 };
@@ -261,38 +274,45 @@ struct CeProductUnit {
         u /= (unsigned)a.tiles_m;
         nt = (int)(u % (unsigned)a.tiles_n);
         split = (int)(u / (unsigned)a.tiles_n);
-        m0 = mt * TG_M;
+        m0 = mt * a.m_tile;
         k0 = split * a.kper, k1 = min(a.kb, k0 + a.kper);
     }
 };
-template <int PLANES, bool AMN, int N>
+template <int PLANES, bool AMN, int N, bool PAIRS>
 struct CeProductPolicy {
-    static constexpr bool A_MN = AMN, B_MN = true, I8 = false, HALVES = true;
-    static constexpr int BN = N, SEGMENT = 0, EPI_BYTES = 0;
+    static constexpr bool A_MN = AMN, B_MN = true, I8 = false, PARTS = true, PAIR = PAIRS;
+    static constexpr int BN = N, SEGMENT = 0, EPI_BYTES = 0, EPI_WARPS = 8;
     using Pairs = PlanePairs<PLANES>;
     using Args = CeProductArgs;
     using Unit = CeProductUnit;
     static __device__ __forceinline__ void load(const Args& a, const Unit& u, int, int pa, int pb, int k, const CUtensorMap* ta, const CUtensorMap* tb, unsigned char* sa,
-                                                unsigned char* sb, uint64_t* bar) {
+                                                unsigned char* sb, uint32_t bar, int rank) {
+        const int m0 = u.m0 + rank * TG_M;
         if (AMN) {
-            tma_load_3d(sa, ta, bar, u.m0, k * 64, pa);
-            tma_load_3d(sa + TG_BOX_BYTES, ta, bar, u.m0 + 64, k * 64, pa);
+            tma_load_3d<PAIR>(sa, ta, bar, m0, k * 64, pa);
+            tma_load_3d<PAIR>(sa + TG_BOX_BYTES, ta, bar, m0 + 64, k * 64, pa);
         } else {
-            tma_load_3d(sa, ta, bar, k * 64, u.m0, pa);
+            tma_load_3d<PAIR>(sa, ta, bar, k * 64, m0, pa);
         }
+        constexpr int HERE = BN / (PAIR ? 2 : 1);
 #pragma unroll
-        for (int i = 0; i < BN / 64; ++i) tma_load_3d(sb + i * TG_BOX_BYTES, tb, bar, u.nt * BN + i * 64, a.b0 + k * 64, pb);
+        for (int i = 0; i < HERE / 64; ++i) tma_load_3d<PAIR>(sb + i * TG_BOX_BYTES, tb, bar, u.nt * BN + rank * HERE + i * 64, a.b0 + k * 64, pb);
     }
     static __device__ __forceinline__ int n_mma(const Args& a, const Unit& u, int) { return min(BN, (a.cols - u.nt * BN + 15) & ~15); }
 
     struct Epilogue {
-        int quarter, group, lane;
-        __device__ __forceinline__ Epilogue(const Args&, unsigned char*, int, int quarter_, int group_, int lane_) : quarter(quarter_), group(group_), lane(lane_) {}
+        int quarter, group, lane, rank;
+        __device__ __forceinline__ Epilogue(const Args&, unsigned char*, int, int quarter_, int group_, int lane_, int rank_)
+            : quarter(quarter_), group(group_), lane(lane_), rank(rank_) {}
         __device__ __forceinline__ void unit_begin(const Args&, const Unit&) {}
         __device__ __forceinline__ void unit_end(const Args&, const Unit&) {}
-        __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool) {
-            const int row = u.m0 + quarter * 32 + lane;
-            if (row - lane >= a.rows) return;
+        template <typename D>
+        __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
+            const int row = u.m0 + rank * TG_M + quarter * 32 + lane;
+            if (row - lane >= a.rows) {
+                done();
+                return;
+            }
             float* const out = a.out + ((int64_t)u.split * a.rows + row) * a.cols + u.nt * BN + group * (BN / 2);
             const int width = min(BN / 2, a.cols - u.nt * BN - group * (BN / 2));
             const bool wide = (a.cols & 3) == 0;
@@ -322,6 +342,7 @@ struct CeProductPolicy {
                     }
                 }
             }
+            done();
         }
     };
 };
@@ -585,7 +606,7 @@ struct CePlan {
         const size_t tiles_q = ceil_div(k.m, TG_M), tiles_n = ceil_div(k.n, CE_BN);
         if (!backward) {
             block = (int)std::max<size_t>(1, std::min<size_t>(16, tiles_q * tiles_n / ((size_t)sms * 8)));
-            slots = 2 * (int)ceil_div(tiles_n, block);
+            slots = CE_SLOTS * (int)ceil_div(tiles_n, block);
             partial = space.take<float2>((size_t)k.m * slots);
             target_scores = space.take<float>(k.m);
             return;
@@ -635,6 +656,8 @@ struct CePlan {
             parts_x = space.take<float>((size_t)splits_x * piece * k.d);
         }
     }
+    // A pair of CTAs wants 256 entries of the M side; fewer are left to single ones.
+    static bool pairs(int64_t rows) { return rows > TG_M; }
     static int product_bn(int d) { return d > 128 ? 256 : d > 64 ? 128 : 64; }
 };
 
@@ -670,24 +693,27 @@ inline CeScoreArgs ce_score_args(const CeCall& k, const CePlan& p) {
     CeScoreArgs a{};
     a.d_error = k.d_error, a.idesc = tg_idesc(k.tg(), false, false);
     a.m = k.m, a.kb = (int)ceil_div(k.d, 64), a.n0 = 0, a.n1 = k.n;
-    a.tiles_q = (int)ceil_div(k.m, TG_M), a.tiles_n = (unsigned)ceil_div(k.n, CE_BN);
+    a.m_tile = CePlan::pairs(k.m) ? 2 * TG_M : TG_M;
+    a.tiles_q = (int)ceil_div(k.m, a.m_tile), a.tiles_n = (unsigned)ceil_div(k.n, CE_BN);
     a.c = k.c2(), a.bias = p.bias2, a.targets = k.targets;
     return a;
 }
 
-// f(number of planes, whether there is a bias, whether K is taken in segments), as types.
+// f(number of planes, whether there is a bias, whether K is taken in segments, whether by pairs of CTAs), as types.
 template <typename F>
-inline void ce_by(F&& f, bool three, bool bias, bool segments) {
-    using Y = std::true_type;
-    using N = std::false_type;
-    auto with = [&](auto p) {
-        if (bias && segments) f(p, Y(), Y());
-        else if (bias) f(p, Y(), N());
-        else if (segments) f(p, N(), Y());
-        else f(p, N(), N());
+inline void ce_by(F&& f, bool three, bool bias, bool segments, bool pairs) {
+    auto one = [](bool v, auto&& g) {
+        if (v) g(std::true_type());
+        else g(std::false_type());
     };
-    if (three) with(std::integral_constant<int, 3>());
-    else with(std::integral_constant<int, 1>());
+    one(bias, [&](auto b) {
+        one(segments, [&](auto s) {
+            one(pairs, [&](auto p) {
+                if (three) f(std::integral_constant<int, 3>(), b, s, p);
+                else f(std::integral_constant<int, 1>(), b, s, p);
+            });
+        });
+    });
 }
 
 inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse_low, void* workspace) {
@@ -698,10 +724,11 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     const size_t units = ceil_div(a.tiles_n, p.block) * a.tiles_q;
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
-    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CE_BN);
+    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CePlan::pairs(k.m) ? CE_BN / 2 : CE_BN);
     const bool segments = a.kb > CE_SEGMENT;
-    ce_by([&](auto planes, auto bias, auto segs) { tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value>>(k.c, tq, tx, a, k.stream); },
-          k.planes() == 3, k.bias != nullptr, segments);
+    ce_by([&](auto planes, auto bias, auto segs, auto pairs) {
+        tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value, decltype(pairs)::value>>(k.c, tq, tx, a, k.stream);
+    }, k.planes() == 3, k.bias != nullptr, segments, CePlan::pairs(k.m));
     ce_join_kernel<<<ce_grid((size_t)k.m * 32), 256, 0, k.stream>>>(p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
     KERNEL_CHECK();
 }
@@ -711,13 +738,16 @@ inline void ce_product(const CeCall& k, const CUtensorMap& tg, const void* b, in
     const int bn = CePlan::product_bn(k.d);
     a.d_error = k.d_error, a.idesc = tg_idesc(k.tg(), AMN, true);
     a.cols = k.d, a.kper = per;
-    a.tiles_m = (int)ceil_div(a.rows, TG_M), a.tiles_n = (int)ceil_div(k.d, bn);
+    const bool pairs = bn == 256 && CePlan::pairs(a.rows);
+    a.m_tile = pairs ? 2 * TG_M : TG_M;
+    a.tiles_m = (int)ceil_div(a.rows, a.m_tile), a.tiles_n = (int)ceil_div(k.d, bn);
     splits = (int)std::min<size_t>(splits, ceil_div(a.kb, per));
     a.units = (unsigned)a.tiles_m * a.tiles_n * splits;
     const CUtensorMap tb = tg_map(b, k.tg(), b_rows, k.d, ldb, k.planes(), b_rows * ldb * 2, 64);
-    if (bn == 256) tc_gemm<CeProductPolicy<PLANES, AMN, 256>>(k.c, tg, tb, a, k.stream);
-    else if (bn == 128) tc_gemm<CeProductPolicy<PLANES, AMN, 128>>(k.c, tg, tb, a, k.stream);
-    else tc_gemm<CeProductPolicy<PLANES, AMN, 64>>(k.c, tg, tb, a, k.stream);
+    if (pairs) tc_gemm<CeProductPolicy<PLANES, AMN, 256, true>>(k.c, tg, tb, a, k.stream);
+    else if (bn == 256) tc_gemm<CeProductPolicy<PLANES, AMN, 256, false>>(k.c, tg, tb, a, k.stream);
+    else if (bn == 128) tc_gemm<CeProductPolicy<PLANES, AMN, 128, false>>(k.c, tg, tb, a, k.stream);
+    else tc_gemm<CeProductPolicy<PLANES, AMN, 64, false>>(k.c, tg, tb, a, k.stream);
 }
 
 template <bool ROWS, bool HALF>
@@ -725,8 +755,9 @@ inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, vo
     const int nb = k.d > 128 ? 64 : 128, kb = k.d > 128 ? 4 : k.d > 64 ? 2 : 1;
     CeFusedArgs a{};
     a.d_error = k.d_error;
-    a.idesc_s = tg_idesc(k.tg(), false, false) | ((uint32_t)(nb >> 3) << 17);
-    a.idesc_o = tg_idesc(k.tg(), false, true) | ((uint32_t)(kb * 64 >> 3) << 17);
+    constexpr uint32_t M = (uint32_t)(TG_M >> 4) << 24;
+    a.idesc_s = tg_idesc(k.tg(), false, false) | M | ((uint32_t)(nb >> 3) << 17);
+    a.idesc_o = tg_idesc(k.tg(), false, true) | M | ((uint32_t)(kb * 64 >> 3) << 17);
     a.own = ROWS ? k.n : k.m, a.other = ROWS ? k.m : k.n;
     a.tiles_own = (int)ceil_div(a.own, TG_M), a.tiles_other = (int)ceil_div(a.other, nb), a.block = ROWS ? a.tiles_other : p.fused_block;
     const size_t units = ceil_div(a.tiles_other, a.block) * a.tiles_own;
@@ -765,7 +796,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         if (p.fused_q) ce_fused<false, HALF>(k, p, ops, nullptr, 0);
     }
     const bool pieces_q = grad_Q && !p.fused_q, pieces_x = grad_X && !p.fused_x;
-    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CE_BN);
+    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CePlan::pairs(k.m) ? CE_BN / 2 : CE_BN);
     const int64_t g_plane = (int64_t)k.m * p.piece;
     CeScoreArgs s = ce_score_args(k, p);
     s.terms = p.terms, s.factors = p.factors, s.amax = p.amax, s.target_cols = p.cols, s.G = p.G, s.pitch = p.piece, s.plane = g_plane;
@@ -777,11 +808,11 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         const size_t units = (size_t)s.tiles_n * s.tiles_q;
         if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
         s.units = (unsigned)units;
-        ce_by([&](auto planes, auto bias, auto segs) {
+        ce_by([&](auto planes, auto bias, auto segs, auto pairs) {
             // 16-bit results are none the worse for the segments' sums being one
             if constexpr (decltype(planes)::value == PLANES && (PLANES == 3 || !decltype(segs)::value))
-                tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value>>(k.c, tq, tx, s, k.stream);
-        }, PLANES == 3, k.bias != nullptr, PLANES == 3 && s.kb > CE_SEGMENT);
+                tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value, decltype(pairs)::value>>(k.c, tq, tx, s, k.stream);
+        }, PLANES == 3, k.bias != nullptr, PLANES == 3 && s.kb > CE_SEGMENT, CePlan::pairs(k.m));
         const int64_t g_cols = (int64_t)s.tiles_n * CE_BN;
         if (pieces_x) {
             CeProductArgs a{};

@@ -30,7 +30,7 @@ struct I8ProductArgs {
     int64_t ld;
     bool wide;
 };
-constexpr int I8_BN = 128;
+constexpr int I8_BN = 256;
 struct I8Unit {
     static constexpr int tiles = 1, k0 = 0;
     int tile, chunk, k1;
@@ -42,40 +42,45 @@ struct I8Unit {
         k1 = a.kb;
     }
 };
-template <typename OUT>
+template <typename OUT, bool PAIRS>
 struct I8ProductPolicy {
-    static constexpr bool A_MN = false, B_MN = false, I8 = true, HALVES = false;
-    static constexpr int BN = I8_BN, SEGMENT = 0, EPI_BYTES = TG_EPI_WARPS * (MXP_OUT_BYTES + I8_BN * 8);
+    static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = true, PAIR = PAIRS;
+    static constexpr int BN = I8_BN, PART = BN / 2, SEGMENT = 0, EPI_WARPS = 8, EPI_BYTES = EPI_WARPS * (MXP_OUT_BYTES + PART * 8);
     using Pairs = PlanePairs<1>;
     using Args = I8ProductArgs;
     using Unit = I8Unit;
     static __device__ __forceinline__ void load(const Args&, const Unit& u, int, int, int, int k, const CUtensorMap* ta, const CUtensorMap* tb, unsigned char* sa, unsigned char* sb,
-                                                uint64_t* bar) {
-        tma_load_3d(sa, ta, bar, k * 128, u.chunk * TG_M, 0);
-        tma_load_3d(sb, tb, bar, k * 128, u.tile * BN, 0);
+                                                uint32_t bar, int rank) {
+        tma_load_3d<PAIR>(sa, ta, bar, k * 128, u.chunk * (PAIR ? 2 * TG_M : TG_M) + rank * TG_M, 0);
+        tma_load_3d<PAIR>(sb, tb, bar, k * 128, u.tile * BN + rank * (BN / 2), 0);
     }
     static __device__ __forceinline__ int n_mma(const Args& a, const Unit& u, int) { return min(BN, (a.n - u.tile * BN + 15) & ~15); }
     struct Epilogue {
-        int quarter, lane;
+        int quarter, group, lane, rank;
         unsigned char* piece;
         float2* terms;
-        __device__ __forceinline__ Epilogue(const Args&, unsigned char* smem, int warp, int quarter_, int, int lane_)
-            : quarter(quarter_), lane(lane_), piece(smem + warp * MXP_OUT_BYTES), terms(reinterpret_cast<float2*>(smem + TG_EPI_WARPS * MXP_OUT_BYTES) + warp * I8_BN) {}
+        __device__ __forceinline__ Epilogue(const Args&, unsigned char* smem, int warp, int quarter_, int group_, int lane_, int rank_)
+            : quarter(quarter_), group(group_), lane(lane_), rank(rank_), piece(smem + warp * MXP_OUT_BYTES),
+              terms(reinterpret_cast<float2*>(smem + EPI_WARPS * MXP_OUT_BYTES) + warp * PART) {}
         __device__ __forceinline__ void unit_begin(const Args&, const Unit&) {}
         __device__ __forceinline__ void unit_end(const Args&, const Unit&) {}
-        __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool) {
+        template <typename D>
+        __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
             constexpr int PER = 256 / sizeof(OUT), V = 16 / sizeof(OUT);  // scores of a query in a piece, in a store
-            const int q0 = u.chunk * TG_M + quarter * 32, n0 = u.tile * BN;
-            if (q0 >= a.nq) return;
+            const int q0 = u.chunk * (PAIR ? 2 * TG_M : TG_M) + rank * TG_M + quarter * 32, n0 = u.tile * BN + group * PART;
+            if (q0 >= a.nq || n0 >= a.n) {
+                done();
+                return;
+            }
             const int q = q0 + lane;
             float2 mine = q < a.nq ? i8_terms(a.metric, __ldcg(a.q_scales + q), __ldcg(a.q_squares + q)) : make_float2(0.f, 0.f);
             if (!live) mine.x = __int_as_float(0x7FFFFFFF);
 #pragma unroll
-            for (int i = lane; i < BN; i += 32) terms[i] = n0 + i < a.n ? i8_terms(a.metric, __ldcg(a.scales + n0 + i), __ldcg(a.squares + n0 + i)) : make_float2(0.f, 0.f);
+            for (int i = lane; i < PART; i += 32) terms[i] = n0 + i < a.n ? i8_terms(a.metric, __ldcg(a.scales + n0 + i), __ldcg(a.squares + n0 + i)) : make_float2(0.f, 0.f);
             __syncwarp();
             OUT* const o = reinterpret_cast<OUT*>(a.out) + (int64_t)q0 * a.ld + n0;
 #pragma unroll 1
-            for (int p0 = 0; p0 < BN; p0 += PER) {
+            for (int p0 = 0; p0 < PART; p0 += PER) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < PER; c0 += 32) {
                     uint32_t r[32];
@@ -96,6 +101,7 @@ struct I8ProductPolicy {
                         *reinterpret_cast<uint4*>(piece + lane * 256 + (((c0 / V + i) ^ (lane & 7)) << 4)) = w;
                     }
                 }
+                if (p0 + PER >= PART) done();
                 __syncwarp();
                 if (a.wide) copy_piece<OUT, true>(o + p0, a.ld, piece, a.nq - q0, a.n - n0 - p0, lane);
                 else copy_piece<OUT, false>(o + p0, a.ld, piece, a.nq - q0, a.n - n0 - p0, lane);
@@ -170,13 +176,16 @@ inline void i8_product(const CtxPtr& c, const int8_t* q_codes, const float* q_sc
     I8ProductArgs a{};
     a.d_error = d_error, a.idesc = tg_idesc(TG_I8, false, false);
     a.n = n, a.nq = nq, a.kb = (int)ceil_div(i8_pitch(d), 128), a.metric = metric;
-    a.chunks = (int)ceil_div(nq, TG_M), a.tiles = (unsigned)ceil_div(n, I8_BN), a.block = 2 * c->sm_count;
+    const bool pairs = nq > TG_M;
+    a.chunks = (int)ceil_div(nq, pairs ? 2 * TG_M : TG_M), a.tiles = (unsigned)ceil_div(n, I8_BN), a.block = 2 * c->sm_count;
     if ((uint64_t)a.tiles * a.chunks >= (1ull << 31)) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", nq, n);
     a.units = a.tiles * (unsigned)a.chunks;
     a.scales = scales, a.q_scales = q_scales, a.squares = squares, a.q_squares = q_squares, a.out = out, a.ld = ld;
     a.wide = aligned16(out, ld * (int64_t)sizeof(OUT));
     const int pitch = i8_pitch(d);
-    tc_gemm<I8ProductPolicy<OUT>>(c, tg_map(q_codes, TG_I8, nq, pitch, pitch, 1, 0, TG_M), tg_map(codes, TG_I8, n, pitch, pitch, 1, 0, I8_BN), a, stream);
+    const CUtensorMap tq = tg_map(q_codes, TG_I8, nq, pitch, pitch, 1, 0, TG_M), tx = tg_map(codes, TG_I8, n, pitch, pitch, 1, 0, pairs ? I8_BN / 2 : I8_BN);
+    if (pairs) tc_gemm<I8ProductPolicy<OUT, true>>(c, tq, tx, a, stream);
+    else tc_gemm<I8ProductPolicy<OUT, false>>(c, tq, tx, a, stream);
 }
 
 inline void i8_score_lists(const CtxPtr& c, I8ScoreArgs a, cudaStream_t stream) {

@@ -1,8 +1,10 @@
 // Matrix products on the 5th-generation tensor cores, with what is done to a tile of them left to a policy: 16-bit floats (tcgen05.mma kind::f16, fp32
 // accumulators) and 8-bit integers (kind::i8, int32 accumulators, exact).
 //
-// Persistent CTAs with a warp for the TMA loads, one for the MMAs and eight of epilogue, in two groups of four, which take the tiles in turn or the halves of a tile's columns: a warp
-// of a group reads its quarter of the accumulator's 128 lanes.  A tile is 128 entries of the M side by up to P::BN of the N side; a stage holds 128 bytes of K for both.  Either
+// Persistent CTAs with a warp for the TMA loads, one for the MMAs and eight or sixteen of epilogue, in groups of four, which take the tiles in turn or a part of a tile's columns each: a
+// warp of a group reads its quarter of the accumulator's 128 lanes.  A tile is 128 entries of the M side by up to P::BN of the N side; a stage holds 128 bytes of K for both.  Two CTAs can
+// work as a pair (PAIR) on 256 entries of the M side: each loads its 128 and half of the N side, which the MMAs, issued by the first of the two, read from both (cta_group::2): two thirds of the
+// bytes from L2 and of the reads of shared memory.  Either
 // operand may lie with K or with the other side along its rows ("MN-major"): both are loaded in boxes of 128 bytes by so many rows, swizzled over 128 bytes, and
 // only the descriptors differ.  Operands that are held as sums of planes (32-bit floats as three bfloat16) are multiplied pair by pair, the small ones first, so that the
 // accumulator is small while they come.  Every wait is bounded (mbar_wait); a CTA whose wait ran out records it, its tiles are NaN, and it waits for what it has in flight
@@ -11,8 +13,8 @@
 // The accumulators cut off what their adds leave behind 32 bits, half a unit each time on average and always to the same side: 128 adds (K of 2,048) leave a sum 4e-6 of it too small.  A
 // policy may have K taken in segments of SEGMENT steps, each in an accumulator of its own, which its epilogue adds up.
 //
-// A policy has:  Args with `units` and `d_error`;  Unit(args, u) with `tiles`, `k0`, `k1` (steps of K);  load(), which brings a step of a tile;  n_mma(args, unit, tile), columns of
-// a tile;  HALVES, whether the groups share a tile;  SEGMENT, 0 for none;  Epilogue with unit_begin(), segment() of all accumulators of a tile but the last, tile() and unit_end().
+// A policy has:  Args with `units` and `d_error`;  Unit(args, u) with `tiles`, `k0`, `k1` (steps of K);  load(), which brings a step of a tile (rank: which
+// of a pair's CTAs);  n_mma(args, unit, tile), columns of a tile;  EPI_WARPS;  PARTS, whether the groups share a tile;  SEGMENT, 0 for none;  Epilogue with unit_begin(), segment() of all accumulators of a tile but the last, tile() and unit_end().
 #pragma once
 
 #include "tc_ptx.cuh"
@@ -20,7 +22,7 @@
 
 namespace culsh_b200 {
 
-constexpr int TG_M = 128, TG_EPI_WARPS = 8, TG_THREADS = 64 + 32 * TG_EPI_WARPS;
+constexpr int TG_M = 128, TG_SMEM = 224 * 1024;
 constexpr int TG_BOX_BYTES = 8192;  // of an MN-major operand: 64 entries by 64 of K
 
 // Pairs of planes, in the order in which they are multiplied.  Of three planes each: what is left out is below 2^-24 of the product.
@@ -39,28 +41,61 @@ struct PlanePairs<3> {  // (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
     static __device__ __forceinline__ int b(int p) { return p == 1 ? 2 : p == 2 || p == 4 ? 1 : 0; }
 };
 
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_u32(smem_dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
-}
-template <bool I8>
-__device__ __forceinline__ void tc_mma_warp(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    if constexpr (I8)
+// PAIR: the barrier is the first CTA's of the two.
+template <bool PAIR>
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    if constexpr (PAIR)
         asm volatile(
-            "{\n\t.reg .pred p, e;\n\t"
-            "elect.sync _|e, 0xFFFFFFFF;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+            ::"r"(smem_u32(smem_dst)), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
             : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p, e;\n\t"
-            "elect.sync _|e, 0xFFFFFFFF;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+            ::"r"(smem_u32(smem_dst)), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
             : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    tma_load_3d<false>(smem_dst, map, smem_u32(bar), x, y, z);
+}
+#define TG_MMA(GROUP, KIND)                                                                          \
+    asm volatile(                                                                                     \
+        "{\n\t.reg .pred p, e;\n\t"                                                                  \
+        "elect.sync _|e, 0xFFFFFFFF;\n\t"                                                             \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                                   \
+        "@e tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}"                \
+        ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)                                    \
+        : "memory")
+template <bool I8, bool PAIR = false>
+__device__ __forceinline__ void tc_mma_warp(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (I8 && PAIR) TG_MMA("2", "i8");
+    else if constexpr (I8) TG_MMA("1", "i8");
+    else if constexpr (PAIR) TG_MMA("2", "f16");
+    else TG_MMA("1", "f16");
+}
+#undef TG_MMA
+// The barrier at the same place of both CTAs of a pair.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xFFFFFFFF;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t first_of_pair(const void* p) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(p)));
+    return at;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t at) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory"); }
+// A wait for what the other CTA of a pair has a part in.
+__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_error) {
+    const bool ok = mbar_wait_warp(bar, parity, abort_flag, d_error);
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    return ok;
+}
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 // K along the rows: groups of 8 rows of 128 bytes one behind the other.  Else: rows of 64 entries, one for each of K; groups of 8 rows, and boxes for the next 64 entries.
 template <bool MN>
@@ -72,7 +107,7 @@ enum TgType : int { TG_F16 = 0, TG_BF16 = 1, TG_I8 = 2 };
 // Both operands of one type: float accumulators, or int32 of signed 8-bit integers.
 inline uint32_t tg_idesc(TgType t, bool a_mn, bool b_mn) {
     const uint32_t type = t == TG_F16 ? 0u : 1u;
-    return ((t == TG_I8 ? 2u : 1u) << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(TG_M >> 4) << 24);
+    return ((t == TG_I8 ? 2u : 1u) << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
 }
 
 template <typename P>
@@ -82,19 +117,21 @@ __device__ __forceinline__ int tg_segments(const typename P::Unit& u) {
 
 template <typename P>
 struct TgCfg {
-    static constexpr int A_BYTES = TG_M * 128, B_BYTES = P::BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int STAGES = (200 * 1024 - P::EPI_BYTES) / STAGE_BYTES;
-    static constexpr int ACCS = 512 / P::BN;
+    static constexpr int A_BYTES = TG_M * 128, B_ROWS = P::BN / (P::PAIR ? 2 : 1), B_BYTES = B_ROWS * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = (TG_SMEM - P::EPI_BYTES) / STAGE_BYTES;
+    static constexpr int ACCS = 512 / P::BN, GROUPS = P::EPI_WARPS / 4, THREADS = 64 + 32 * P::EPI_WARPS;
     static constexpr int SMEM = STAGES * STAGE_BYTES + P::EPI_BYTES + 1024 /*barriers*/ + 1024 /*alignment slack*/;
-    static_assert(STAGES >= 2 && (2 * STAGES + 2 * ACCS + 1) * 8 + 16 <= 1024 && SMEM <= 227 * 1024, "");
+    static constexpr uint32_t M_BITS = (uint32_t)((P::PAIR ? 2 * TG_M : TG_M) >> 4) << 24;
+    static_assert(STAGES >= 2 && (2 * STAGES + 2 * ACCS + 1) * 8 + 16 <= 1024 && SMEM <= 227 * 1024 && (P::PARTS || ACCS % GROUPS == 0), "");
 };
 
 template <typename P>
-__global__ void __launch_bounds__(TG_THREADS, 1)
+__global__ void __launch_bounds__(TgCfg<P>::THREADS, 1)
 tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, typename P::Args a, KernelBefore before) {
     behind_kernel_before(before);
     using Cfg = TgCfg<P>;
     constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS;
+    constexpr bool PAIR = P::PAIR;
     extern __shared__ unsigned char tg_smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tg_smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* s_epi = base + (size_t)STAGES * Cfg::STAGE_BYTES;
@@ -107,6 +144,8 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
     uint32_t* s_fills = s_tmem + 2;  // stages that have been loaded
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // a pair takes a unit; its first CTA issues the MMAs, and has the barriers that loads and epilogues of both arrive at
+    const unsigned rank = PAIR ? blockIdx.x & 1u : 0u, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -115,18 +154,24 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
         for (int b = 0; b < ACCS; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], P::HALVES ? 8 : 4);
+            mbar_init(&acc_empty[b], (P::PARTS ? P::EPI_WARPS : 4) * (PAIR ? 2 : 1));
         }
         mbar_init(drained, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) pair_sync();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
 
@@ -134,7 +179,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         if (lane == 0) {
             uint32_t s = 0, parity = 1, fills = 0;
             bool live = true;
-            for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x) {
+            for (unsigned u = first; u < a.units && live; u += step) {
                 const typename P::Unit unit(a, u);
                 for (int at = 0; at < unit.tiles * tg_segments<P>(unit) && live; ++at) {
                     const int t = at / tg_segments<P>(unit), k0 = unit.k0 + (at - t * tg_segments<P>(unit)) * P::SEGMENT;
@@ -143,8 +188,9 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                         for (int k = k0; k < k1; ++k) {
                             if (!mbar_wait(&empty[s], parity, s_abort, a.d_error)) { live = false; break; }
                             unsigned char* st = base + (size_t)s * Cfg::STAGE_BYTES;
-                            mbar_expect_tx(&full[s], Cfg::STAGE_BYTES);
-                            P::load(a, unit, t, P::Pairs::a(pair), P::Pairs::b(pair), k, &tmA, &tmB, st, st + Cfg::A_BYTES, &full[s]);
+                            if (rank == 0) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * Cfg::STAGE_BYTES);
+                            P::load(a, unit, t, P::Pairs::a(pair), P::Pairs::b(pair), k, &tmA, &tmB, st, st + Cfg::A_BYTES, PAIR ? first_of_pair(&full[s]) : smem_u32(&full[s]),
+                                    (int)rank);
                             ++fills;
                             if (++s == STAGES) { s = 0; parity ^= 1u; }
                         }
@@ -155,16 +201,19 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
     } else if (warp == 1) {
         uint32_t s = 0, parity = 0, ab = 0, acc_parity = 1;
-        bool live = true;
-        for (unsigned u = blockIdx.x; u < a.units && live; u += gridDim.x) {
+        bool live = rank == 0;
+        for (unsigned u = first; u < a.units && live; u += step) {
             const typename P::Unit unit(a, u);
             for (int at = 0; at < unit.tiles * tg_segments<P>(unit) && live; ++at) {
                 const int t = at / tg_segments<P>(unit), k0 = unit.k0 + (at - t * tg_segments<P>(unit)) * P::SEGMENT;
                 const int k1 = P::SEGMENT ? min(unit.k1, k0 + P::SEGMENT) : unit.k1;
-                if (!mbar_wait_warp(&acc_empty[ab], acc_parity, s_abort, a.d_error)) { live = false; break; }
+                if (!(PAIR ? mbar_wait_pair(&acc_empty[ab], acc_parity, s_abort, a.d_error) : mbar_wait_warp(&acc_empty[ab], acc_parity, s_abort, a.d_error))) {
+                    live = false;
+                    break;
+                }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + ab * P::BN;
-                const uint32_t idesc = a.idesc | ((uint32_t)(P::n_mma(a, unit, t) >> 3) << 17);
+                const uint32_t idesc = a.idesc | Cfg::M_BITS | ((uint32_t)((PAIR ? P::BN : P::n_mma(a, unit, t)) >> 3) << 17);  // a pair's CTAs hold half of N each, whatever is used of it
                 const int steps = (k1 - k0) * P::Pairs::N;
                 for (int k = 0; k < steps; ++k) {
                     if (!mbar_wait_warp(&full[s], parity, s_abort, a.d_error)) { live = false; break; }
@@ -173,37 +222,47 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     const uint64_t da = tg_desc<P::A_MN>(st), db = tg_desc<P::B_MN>(st + Cfg::A_BYTES);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)  // 32 bytes of K, or 16 rows of it
-                        tc_mma_warp<P::I8>(d_tmem, da + i * (P::A_MN ? 128 : 2), db + i * (P::B_MN ? 128 : 2), idesc, (k | i) != 0);
-                    tc_commit_warp(&empty[s]);
+                        tc_mma_warp<P::I8, PAIR>(d_tmem, da + i * (P::A_MN ? 128 : 2), db + i * (P::B_MN ? 128 : 2), idesc, (k | i) != 0);
+                    if (PAIR) tc_commit_pair(&empty[s]);
+                    else tc_commit_warp(&empty[s]);
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
-                if (live) tc_commit_warp(&acc_full[ab]);
+                if (live) {
+                    if (PAIR) tc_commit_pair(&acc_full[ab]);
+                    else tc_commit_warp(&acc_full[ab]);
+                }
                 if (++ab == ACCS) { ab = 0; acc_parity ^= 1u; }
             }
         }
     } else {
         const int quarter = warp & 3, group = (warp - 2) >> 2;
-        typename P::Epilogue epi(a, s_epi, warp - 2, quarter, group, lane);
+        typename P::Epilogue epi(a, s_epi, warp - 2, quarter, group, lane, (int)rank);
         bool live = true;
         uint32_t nth = 0;  // accumulator of the CTA
-        for (unsigned u = blockIdx.x; u < a.units; u += gridDim.x) {
+        for (unsigned u = first; u < a.units; u += step) {
             const typename P::Unit unit(a, u);
             const int segments = tg_segments<P>(unit);
             epi.unit_begin(a, unit);
             for (int t = 0; t < unit.tiles; ++t) {
                 for (int g = 0; g < segments; ++g, ++nth) {
-                    if (!P::HALVES && (int)(nth & 1u) != group) continue;
-                    const uint32_t ab = nth % ACCS, taddr = tmem + ((uint32_t)(quarter * 32) << 16) + ab * P::BN + (P::HALVES ? group * (P::BN / 2) : 0);
+                    if (!P::PARTS && (int)(nth % Cfg::GROUPS) != group) continue;
+                    const uint32_t ab = nth % ACCS, taddr = tmem + ((uint32_t)(quarter * 32) << 16) + ab * P::BN + (P::PARTS ? group * (P::BN / Cfg::GROUPS) : 0);
                     if (live) live = mbar_wait_warp(&acc_full[ab], (nth / ACCS) & 1u, s_abort, a.d_error);
                     tc_fence_after();
+                    auto done = [&] {  // the accumulator has been read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (PAIR) mbar_arrive_at(first_of_pair(&acc_empty[ab]));
+                            else mbar_arrive(&acc_empty[ab]);
+                        }
+                    };
                     if (P::SEGMENT && g + 1 < segments) {
                         if constexpr (P::SEGMENT != 0) epi.segment(a, g == 0, taddr, live);
+                        done();
                     } else {
-                        epi.tile(a, unit, t, taddr, live, segments > 1);
+                        epi.tile(a, unit, t, taddr, live, segments > 1, done);
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[ab]);
                 }
             }
             epi.unit_end(a, unit);
@@ -213,14 +272,19 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     if (*s_abort) {  // all roles are done: what they issued may not be
-        if (threadIdx.x == 0) mbar_wait_landed(full, STAGES, *s_fills);
-        if (warp == 1) {
-            tc_commit_warp(drained);
+        if (threadIdx.x == 0 && rank == 0) mbar_wait_landed(full, STAGES, *s_fills);
+        if (warp == 1 && rank == 0) {
+            if (PAIR) tc_commit_pair(drained);
+            else tc_commit_warp(drained);
             mbar_wait_landed(drained, 1, 1);
         }
         __syncthreads();
     }
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (PAIR) pair_sync();  // neither goes while the other may still arrive at its barriers, or read its half
+    if (warp == 1) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
 }
 
 // 32 columns of an accumulator, NaN where a wait ran out.
@@ -261,8 +325,13 @@ inline void tc_gemm(const CtxPtr& c, const CUtensorMap& ta, const CUtensorMap& t
         CU_CHECK(cudaFuncSetAttribute(tc_gemm_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
         if (c->device < 64) ready |= 1ull << c->device;
     }
-    launch_next(stream, tc_gemm_kernel<P>, std::min<unsigned>(a.units, (unsigned)c->sm_count), (unsigned)TG_THREADS, (size_t)Cfg::SMEM, ta, tb, a);
-    KERNEL_CHECK();
+    const unsigned size = (unsigned)Cfg::SMEM, threads = (unsigned)Cfg::THREADS;
+    if (P::PAIR) {
+        launch_cluster(stream, tc_gemm_kernel<P>, 2 * std::min<unsigned>(a.units, (unsigned)c->sm_count / 2), 2u, threads, (size_t)size, ta, tb, a);
+    } else {
+        launch_next(stream, tc_gemm_kernel<P>, std::min<unsigned>(a.units, (unsigned)c->sm_count), threads, (size_t)size, ta, tb, a);
+        KERNEL_CHECK();
+    }
 }
 
 }  // namespace culsh_b200
