@@ -91,7 +91,7 @@ template <bool SEGMENTS>
 struct CeSums {
     static_assert(CE_PART == 64, "");
     float v[SEGMENTS ? CE_PART : 1];
-    __device__ __forceinline__ void segment(const CeScoreArgs&, bool first, uint32_t taddr, bool live) {
+    __device__ __forceinline__ void segment(const CeScoreArgs&, bool first, uint32_t taddr, bool) {
         if constexpr (SEGMENTS) {
             auto each = [&](auto&& f) {
 #pragma unroll
@@ -100,7 +100,7 @@ struct CeSums {
                     tc_ld16(taddr + c0, r);
                     tc_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) f(v[c0 + j], live ? __uint_as_float(r[j]) : __int_as_float(0x7FFFFFFF));
+                    for (int j = 0; j < 16; ++j) f(v[c0 + j], __uint_as_float(r[j]));
                 }
             };
             if (first) each([](float& to, float from) { to = from; });
@@ -120,7 +120,7 @@ struct CeSums {
             tc_ld_wait();
             float x[CE_PART];
 #pragma unroll
-            for (int j = 0; j < CE_PART; ++j) x[j] = live ? __uint_as_float(r[j / 32][j % 32]) : __int_as_float(0x7FFFFFFF);
+            for (int j = 0; j < CE_PART; ++j) x[j] = __uint_as_float(r[j / 32][j % 32]);
             f(x);
         }
     }
@@ -187,6 +187,7 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
                 }
             }
             add(a, x);
+            if (!live) sum = __int_as_float(0x7FFFFFFF);
             });
         }
         __device__ __forceinline__ void unit_end(const CeScoreArgs& a, const CeUnit& u) {
@@ -220,6 +221,7 @@ struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
             this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
             done();
             if (idle) return;
+            if (!live) factor = __int_as_float(0x7FFFFFFF);
 #pragma unroll
             for (int j = 0; j < CE_PART; ++j) x[j] = ce_exp2(fmaf(x[j], a.c, BIAS ? term + s_bias[j] : term)) * factor;
             if (left < CE_PART || __any_sync(0xFFFFFFFFu, (unsigned)at < (unsigned)CE_PART)) {  // seldom; behind the last row G has zeros
@@ -265,6 +267,13 @@ struct CeProductArgs {
     int tiles_m, tiles_n, m_tile;
     bool accumulate;
     float* out;
+    // dX from sums that are complete: 16-bit values with the targets' part, over the temperature
+    void* typed;
+    int64_t ld;
+    const uint32_t* amax;
+    const int* where;
+    const float* sums;
+    float inv_t;
 };
 struct CeProductUnit {
     static constexpr int tiles = 1;
@@ -278,7 +287,45 @@ struct CeProductUnit {
         k0 = split * a.kper, k1 = min(a.kb, k0 + a.kper);
     }
 };
-template <int PLANES, bool AMN, int N, bool PAIRS>
+// N columns of a row of dX from column col0 on.
+template <typename T, int N>
+__device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, int col0, uint32_t taddr, bool live) {
+    const bool in = row < a.rows;
+    const int slot = in ? __ldcg(a.where + row) : -1;
+    const float scale = ldexpf(a.inv_t, std::is_same<T, __half>::value ? -ce_scale_exponent(a.amax) : 0);
+    const float* const extra = a.sums + (int64_t)max(slot, 0) * a.cols + col0;
+    T* const o = reinterpret_cast<T*>(a.typed) + (int64_t)row * a.ld + col0;
+    const bool wide = (a.cols & 7) == 0 && (a.ld & 7) == 0 && ((uintptr_t)a.typed & 15) == 0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) {
+        uint32_t r[32];
+        tg_read(taddr + c0, live, r);
+        if (!in) continue;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
+        if (slot >= 0) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col0 + c0 + j < a.cols) v[j] = fmaf(__ldcg(extra + c0 + j), a.inv_t, v[j]);
+        }
+        if (wide) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+                if (col0 + c0 + j >= a.cols) break;
+                const T* const t = nullptr;
+                *reinterpret_cast<uint4*>(o + c0 + j) =
+                    make_uint4(pack_scores(t, v[j], v[j + 1]), pack_scores(t, v[j + 2], v[j + 3]), pack_scores(t, v[j + 4], v[j + 5]), pack_scores(t, v[j + 6], v[j + 7]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col0 + c0 + j < a.cols) store_score(o + c0 + j, v[j]);
+        }
+    }
+}
+// TYPED: 0: sums in 32 bits; 1, 2: bfloat16, float16.
+template <int PLANES, bool AMN, int N, bool PAIRS, int TYPED>
 struct CeProductPolicy {
     static constexpr bool A_MN = AMN, B_MN = true, I8 = false, PARTS = true, PAIR = PAIRS;
     static constexpr int BN = N, SEGMENT = 0, EPI_BYTES = 0, EPI_WARPS = 8;
@@ -310,6 +357,11 @@ struct CeProductPolicy {
         __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
             const int row = u.m0 + rank * TG_M + quarter * 32 + lane;
             if (row - lane >= a.rows) {
+                done();
+                return;
+            }
+            if constexpr (TYPED != 0) {
+                ce_store_typed<std::conditional_t<TYPED == 2, __half, __nv_bfloat16>, BN / 2>(a, row, u.nt * BN + group * (BN / 2), taddr, live);
                 done();
                 return;
             }
@@ -447,7 +499,7 @@ __global__ void __launch_bounds__(256) ce_terms_kernel(const float* __restrict__
 
 // Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes CE_OWN_ROWS rows and looks
 // through all targets; they come in ascending order.
-constexpr int CE_OWN_ROWS = 128, CE_OWN_LIST = 1024;
+constexpr int CE_OWN_ROWS = 128, CE_OWN_LIST = 1024, CE_OWN_COLS = 16;  // columns of a lane at a time
 template <typename T>
 __global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ cols, const float* __restrict__ own, const T* __restrict__ Q, int64_t ldq, int m, int n, int d,
                                                      float* __restrict__ sums, int* __restrict__ where) {
@@ -489,8 +541,10 @@ __global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ col
                 if (first < 0) continue;
                 const bool fresh = s_first[rr] < 0;
                 const int slot = fresh ? s_query[first] : s_first[rr];
-                for (int c0 = 0; c0 < d; c0 += 128) {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int c0 = 0; c0 < d; c0 += 32 * CE_OWN_COLS) {
+                    float acc[CE_OWN_COLS];
+#pragma unroll
+                    for (int k = 0; k < CE_OWN_COLS; ++k) acc[k] = 0.f;
                     for (int e0 = first & ~31; e0 < held; e0 += 32) {
                         unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
                         while (b) {
@@ -498,15 +552,14 @@ __global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ col
                             b &= b - 1u;
                             const int query = s_query[e];
                             const float f = own[query];
+                            const T* const from = Q + (int64_t)query * ldq + c0 + lane;
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const int col = c0 + k * 32 + lane;
-                                if (col < d) acc[k] = fmaf(f, ce_float(Q[(int64_t)query * ldq + col]), acc[k]);
-                            }
+                            for (int k = 0; k < CE_OWN_COLS; ++k)
+                                if (c0 + k * 32 + lane < d) acc[k] = fmaf(f, ce_float(from[k * 32]), acc[k]);
                         }
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+                    for (int k = 0; k < CE_OWN_COLS; ++k) {
                         const int col = c0 + k * 32 + lane;
                         if (col < d) {
                             float* const s = sums + (int64_t)slot * d + col;
@@ -527,22 +580,37 @@ __global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ col
 }
 
 // Gradients from sums: out[row][col] = (sum over the splits / scale + the target's part) / T.  factors: of the rows, where the sums are of p alone.  QUERIES: the target's part is own[row] times the row cols[row] of X; else sums[where[row]].
-template <typename T, bool QUERIES>
-__global__ void __launch_bounds__(256) ce_finish_kernel(const float* __restrict__ parts, int splits, int64_t split_stride, int64_t rows, int d, const uint32_t* __restrict__ amax,
+template <typename T, bool QUERIES, int V>
+__global__ void __launch_bounds__(256) ce_finish_kernel(const float* __restrict__ parts, int splits, int64_t split_stride, unsigned units, int d, const uint32_t* __restrict__ amax,
                                                         const float* __restrict__ factors, const int* __restrict__ which, const float* __restrict__ own,
-                                                        const T* __restrict__ X, int64_t ldx,
-                                                        const float* __restrict__ sums, float inv_t, T* __restrict__ out, int64_t ldo) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * d) return;
-    const int64_t row = i / d;
-    const int col = (int)(i - row * d);
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += parts[s * split_stride + i];
-    if (factors) v *= std::is_same<T, __half>::value ? ldexpf(factors[row], -14) : factors[row];
-    else if (amax) v = ldexpf(v, -ce_scale_exponent(amax));
+                                                        const T* __restrict__ X, int64_t ldx, const float* __restrict__ sums, float inv_t, T* __restrict__ out, int64_t ldo) {
+    const unsigned i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= units) return;
+    const unsigned each = (unsigned)d / V, row = i / each, col = (i - row * each) * V;
+    const float* const from = parts + (int64_t)row * d + col;
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        float w[V];
+        if (V == 4) *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(from + s * split_stride);
+        else w[0] = from[s * split_stride];
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += w[k];
+    }
     const int w = which[row];
-    if (w >= 0) v += QUERIES ? own[row] * ce_float(X[(int64_t)w * ldx + col]) : sums[(int64_t)w * d + col];
-    out[row * ldo + col] = (T)(v * inv_t);
+    const float f = factors ? (std::is_same<T, __half>::value ? ldexpf(factors[row], -14) : factors[row]) : amax ? ldexpf(1.f, -ce_scale_exponent(amax)) : 1.f;
+    const float mine = QUERIES && w >= 0 ? own[row] : 0.f;
+    struct alignas(V * sizeof(T)) Some { T v[V]; };
+    Some o;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        float x = v[k] * f;
+        if (w >= 0) x += QUERIES ? mine * ce_float(X[(int64_t)w * ldx + col + k]) : sums[(int64_t)w * d + col + k];
+        o.v[k] = (T)(x * inv_t);
+    }
+    *reinterpret_cast<Some*>(out + (int64_t)row * ldo + col) = o;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -637,7 +705,13 @@ struct CePlan {
         const bool pieces_x = need_x && !fused_x;
         const size_t row_bytes = (size_t)2 * k.planes() * k.m;
         const size_t fit = std::min(CE_G_BYTES / row_bytes, pieces_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : CE_G_BYTES) / CE_BN * CE_BN;
-        piece = (int)std::min<size_t>(std::max<size_t>(fit, CE_BN), tiles_n * CE_BN);
+        // the last wave of the products' units full, with as few pieces as that allows
+        const size_t most = std::min(std::max<size_t>(fit / CE_BN, 1), tiles_n), wide = pairs(k.m) ? sms / 2 : sms, high = ceil_div(k.m, pairs(k.m) ? 2 * TG_M : TG_M);
+        size_t least_time = ~(size_t)0;
+        for (size_t p = most; p >= std::max<size_t>(1, most / 3); --p) {
+            const size_t rest = tiles_n % p, time = tiles_n / p * (ceil_div(high * p, wide) * 8 + 1) + (rest ? ceil_div(high * rest, wide) * 8 + 1 : 0);
+            if (time < least_time) least_time = time, piece = (int)(p * CE_BN);
+        }
         G = space.take<uint16_t>((size_t)k.planes() * k.m * piece);
         const int bn = product_bn(k.d);
         const size_t tn = ceil_div(k.d, bn);
@@ -653,7 +727,7 @@ struct CePlan {
         }
         if (pieces_x) {
             split(ceil_div(std::min(piece, k.n), TG_M) * tn, (int)ceil_div(k.m, 64), splits_x, per_x);
-            parts_x = space.take<float>((size_t)splits_x * piece * k.d);
+            if (splits_x > 1 || k.planes() == 3) parts_x = space.take<float>((size_t)splits_x * piece * k.d);
         }
     }
     // A pair of CTAs wants 256 entries of the M side; fewer are left to single ones.
@@ -733,6 +807,25 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     KERNEL_CHECK();
 }
 
+template <typename T, bool QUERIES>
+inline void ce_finish(const CeCall& k, const float* parts, int splits, int64_t split_stride, int64_t rows, const uint32_t* amax, const float* factors, const int* which, const float* own,
+                      const T* X, int64_t ldx, const float* sums, T* out, int64_t ldo) {
+    const float inv_t = (float)(1 / k.temperature);
+    const bool wide = k.d % 4 == 0 && ldo % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
+    const int64_t step = std::max<int64_t>(1, 0x70000000 / k.d);  // rows of a launch
+    for (int64_t r0 = 0; r0 < rows; r0 += step) {
+        const int64_t here = std::min(step, rows - r0);
+        const unsigned units = (unsigned)(here * (k.d / (wide ? 4 : 1)));
+        auto go = [&](auto kern) {
+            kern<<<ce_grid(units), 256, 0, k.stream>>>(parts + r0 * k.d, splits, split_stride, units, k.d, amax, factors ? factors + r0 : nullptr, which + r0, own ? own + r0 : nullptr, X,
+                                                       ldx, sums, inv_t, out + r0 * ldo, ldo);
+            KERNEL_CHECK();
+        };
+        if (wide) go(ce_finish_kernel<T, QUERIES, 4>);
+        else go(ce_finish_kernel<T, QUERIES, 1>);
+    }
+}
+
 template <int PLANES, bool AMN>
 inline void ce_product(const CeCall& k, const CUtensorMap& tg, const void* b, int64_t ldb, int64_t b_rows, CeProductArgs a, int per, int splits) {
     const int bn = CePlan::product_bn(k.d);
@@ -744,10 +837,21 @@ inline void ce_product(const CeCall& k, const CUtensorMap& tg, const void* b, in
     splits = (int)std::min<size_t>(splits, ceil_div(a.kb, per));
     a.units = (unsigned)a.tiles_m * a.tiles_n * splits;
     const CUtensorMap tb = tg_map(b, k.tg(), b_rows, k.d, ldb, k.planes(), b_rows * ldb * 2, 64);
-    if (pairs) tc_gemm<CeProductPolicy<PLANES, AMN, 256, true>>(k.c, tg, tb, a, k.stream);
-    else if (bn == 256) tc_gemm<CeProductPolicy<PLANES, AMN, 256, false>>(k.c, tg, tb, a, k.stream);
-    else if (bn == 128) tc_gemm<CeProductPolicy<PLANES, AMN, 128, false>>(k.c, tg, tb, a, k.stream);
-    else tc_gemm<CeProductPolicy<PLANES, AMN, 64, false>>(k.c, tg, tb, a, k.stream);
+    auto go = [&](auto typed) {
+        constexpr int TYPED = decltype(typed)::value;
+        if (pairs) tc_gemm<CeProductPolicy<PLANES, AMN, 256, true, TYPED>>(k.c, tg, tb, a, k.stream);
+        else if (bn == 256) tc_gemm<CeProductPolicy<PLANES, AMN, 256, false, TYPED>>(k.c, tg, tb, a, k.stream);
+        else if (bn == 128) tc_gemm<CeProductPolicy<PLANES, AMN, 128, false, TYPED>>(k.c, tg, tb, a, k.stream);
+        else tc_gemm<CeProductPolicy<PLANES, AMN, 64, false, TYPED>>(k.c, tg, tb, a, k.stream);
+    };
+    if constexpr (PLANES == 1 && AMN) {
+        if (a.typed) {
+            if (k.type == CULSH_F16) go(std::integral_constant<int, 2>());
+            else go(std::integral_constant<int, 1>());
+            return;
+        }
+    }
+    go(std::integral_constant<int, 0>());
 }
 
 template <bool ROWS, bool HALF>
@@ -783,7 +887,6 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
     constexpr bool HALF = std::is_same<T, __half>::value;
     const CePlan p(k, true, grad_Q != nullptr, grad_X != nullptr, workspace);
     const CeOperands ops(k, p);
-    const float inv_t = (float)(1 / k.temperature);
     if (p.amax) CU_CHECK(cudaMemsetAsync(p.amax, 0, 4, k.stream));
     ce_terms_kernel<<<ce_grid(k.m), 256, 0, k.stream>>>(losses, lse, lse_low, k.targets, grad_losses, grad_lse, k.m, k.n, p.terms, p.log_terms, p.marks, p.factors, p.own, p.cols, p.amax);
     KERNEL_CHECK();
@@ -817,10 +920,13 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         if (pieces_x) {
             CeProductArgs a{};
             a.rows = here, a.b0 = 0, a.kb = (int)ceil_div(k.m, 64), a.out = p.parts_x;
+            if (PLANES == 1 && p.splits_x == 1) {
+                a.typed = grad_X + n0 * ld_gx, a.ld = ld_gx, a.amax = p.amax, a.where = p.where + n0, a.sums = p.sums;
+                a.inv_t = (float)(1 / k.temperature);
+            }
             ce_product<PLANES, true>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, 64), ops.q, ops.ldq, k.m, a, p.per_x, p.splits_x);
-            ce_finish_kernel<T, false><<<ce_grid((size_t)here * k.d), 256, 0, k.stream>>>(p.parts_x, p.splits_x, (int64_t)here * k.d, here, k.d, p.amax, nullptr, p.where + n0, nullptr,
-                                                                                           nullptr, 0, p.sums, inv_t, grad_X + n0 * ld_gx, ld_gx);
-            KERNEL_CHECK();
+            if (p.splits_x > 1 || PLANES == 3)
+                ce_finish<T, false>(k, p.parts_x, p.splits_x, (int64_t)here * k.d, here, p.amax, nullptr, p.where + n0, nullptr, nullptr, 0, p.sums, grad_X + n0 * ld_gx, ld_gx);
         }
         if (pieces_q) {
             CeProductArgs a{};
@@ -829,9 +935,8 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         }
     }
     if (grad_Q) {
-        ce_finish_kernel<T, true><<<ce_grid((size_t)k.m * k.d), 256, 0, k.stream>>>(p.acc_q, p.splits_q, (int64_t)k.m * k.d, k.m, k.d, p.amax, p.fused_q ? p.factors : nullptr, p.cols, p.own,
-                                                                                     static_cast<const T*>(k.X), k.ldx, nullptr, inv_t, grad_Q, ld_gq);
-        KERNEL_CHECK();
+        ce_finish<T, true>(k, p.acc_q, p.splits_q, (int64_t)k.m * k.d, k.m, p.amax, p.fused_q ? p.factors : nullptr, p.cols, p.own, static_cast<const T*>(k.X), k.ldx, nullptr, grad_Q,
+                           ld_gq);
     }
 }
 

@@ -87,13 +87,8 @@ __device__ __forceinline__ uint32_t first_of_pair(const void* p) {
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(p)));
     return at;
 }
-__device__ __forceinline__ void mbar_arrive_at(uint32_t at) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory"); }
-// A wait for what the other CTA of a pair has a part in.
-__device__ __forceinline__ bool mbar_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_error) {
-    const bool ok = mbar_wait_warp(bar, parity, abort_flag, d_error);
-    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    return ok;
-}
+// For what has been read of tensor memory, which tcgen05.fence orders; an arrival that releases writes to the whole cluster waits for all of the warp's memory operations.
+__device__ __forceinline__ void mbar_arrive_at(uint32_t at) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory"); }
 __device__ __forceinline__ void pair_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
@@ -207,10 +202,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             for (int at = 0; at < unit.tiles * tg_segments<P>(unit) && live; ++at) {
                 const int t = at / tg_segments<P>(unit), k0 = unit.k0 + (at - t * tg_segments<P>(unit)) * P::SEGMENT;
                 const int k1 = P::SEGMENT ? min(unit.k1, k0 + P::SEGMENT) : unit.k1;
-                if (!(PAIR ? mbar_wait_pair(&acc_empty[ab], acc_parity, s_abort, a.d_error) : mbar_wait_warp(&acc_empty[ab], acc_parity, s_abort, a.d_error))) {
-                    live = false;
-                    break;
-                }
+                if (!mbar_wait_warp(&acc_empty[ab], acc_parity, s_abort, a.d_error)) { live = false; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + ab * P::BN;
                 const uint32_t idesc = a.idesc | Cfg::M_BITS | ((uint32_t)((PAIR ? P::BN : P::n_mma(a, unit, t)) >> 3) << 17);  // a pair's CTAs hold half of N each, whatever is used of it
