@@ -20,7 +20,7 @@ __device__ __forceinline__ float i8_score(int metric, int dot, float2 q, float2 
 
 struct I8ProductArgs {
     int* d_error;
-    unsigned units;
+    unsigned units, step;     // units between one of a CTA, or of a pair, and its next
     uint32_t idesc;
     int n, nq, kb, metric, chunks, block;
     unsigned tiles;
@@ -28,13 +28,14 @@ struct I8ProductArgs {
     const int32_t *squares, *q_squares;
     void* out;
     int64_t ld;
-    bool wide;
+    bool wide, small;         // rows of the result begin at multiples of 16 bytes; sums are below 2^22
 };
-constexpr int I8_BN = 256;
+constexpr int I8_BN = 256, I8_FEW = 64, I8_FEWEST = 16;
 struct I8Unit {
     static constexpr int tiles = 1, k0 = 0;
+    unsigned u;
     int tile, chunk, k1;
-    __device__ __forceinline__ I8Unit(const I8ProductArgs& a, unsigned u) {  // blocks of neighbouring tiles, a chunk of the queries after the other in each
+    __device__ __forceinline__ I8Unit(const I8ProductArgs& a, unsigned u_) : u(u_) {  // blocks of neighbouring tiles, a chunk of the queries after the other in each
         const unsigned b = (unsigned)(u / ((uint64_t)a.block * a.chunks)), left = (unsigned)(u - (uint64_t)b * a.block * a.chunks);
         const unsigned here = min((unsigned)a.block, a.tiles - b * (unsigned)a.block);
         chunk = (int)(left / here);
@@ -42,10 +43,48 @@ struct I8Unit {
         k1 = a.kb;
     }
 };
+// A scale and squares on their way.
+struct I8Fetch {
+    float scale = 0.f;
+    int squares = 0;
+    __device__ __forceinline__ void get(const float* scales, const int32_t* from, int at, int end) {
+        const bool in = at < end;
+        scale = in ? __ldcg(scales + at) : 0.f;
+        squares = in ? __ldcg(from + at) : 0;
+    }
+};
+// The scores of N sums; conversions of whole numbers run at an eighth of the rate of additions, which do the same for what fits the fraction of a float.
+template <int N>
+__device__ __forceinline__ void i8_scores(int metric, bool small, uint32_t (&r)[N], float2 q, const float* factors, const float* terms) {
+    const uint64_t qq = f2_pack(q.x, q.x);
+    auto all = [&](auto convert) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(factors + j);
+            float v[4];
+            f2_unpack(f2_mul(convert(r[j], r[j + 1]), f2_mul(qq, x.x)), v[0], v[1]);
+            f2_unpack(f2_mul(convert(r[j + 2], r[j + 3]), f2_mul(qq, x.y)), v[2], v[3]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[j + k] = __float_as_uint(v[k]);
+        }
+    };
+    if (small) {
+        const uint64_t minus = f2_pack(-12582912.f, -12582912.f);  // 1.5 x 2^23
+        all([&](uint32_t lo, uint32_t hi) { return f2_add(f2_pack(__uint_as_float(0x4B400000u + lo), __uint_as_float(0x4B400000u + hi)), minus); });
+    } else {
+        all([](uint32_t lo, uint32_t hi) { return f2_pack((float)(int)lo, (float)(int)hi); });
+    }
+    if (metric == MX_EUCLIDEAN) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) r[j] = __float_as_uint(fmaf(2.f, __uint_as_float(r[j]), -q.y) - terms[j]);
+    }
+}
+
+// More than 64 queries: they are the M side, a lane of the accumulator a query.  A warp has 32 queries by 64 rows and stores 128 bytes of each at a time, by way of shared memory.
 template <typename OUT, bool PAIRS>
 struct I8ProductPolicy {
     static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = true, PAIR = PAIRS;
-    static constexpr int BN = I8_BN, PART = BN / 2, SEGMENT = 0, EPI_WARPS = 8, EPI_BYTES = EPI_WARPS * (MXP_OUT_BYTES + PART * 8);
+    static constexpr int BN = I8_BN, EPI_WARPS = 16, PART = BN / 4, SEGMENT = 0, PIECE = 32 * 128, EPI_BYTES = EPI_WARPS * (PIECE + PART * 8);
     using Pairs = PlanePairs<1>;
     using Args = I8ProductArgs;
     using Unit = I8Unit;
@@ -58,35 +97,49 @@ struct I8ProductPolicy {
     struct Epilogue {
         int quarter, group, lane, rank;
         unsigned char* piece;
-        float2* terms;
+        float *factors, *terms;
+        I8Fetch row[PART / 32], query;
         __device__ __forceinline__ Epilogue(const Args&, unsigned char* smem, int warp, int quarter_, int group_, int lane_, int rank_)
-            : quarter(quarter_), group(group_), lane(lane_), rank(rank_), piece(smem + warp * MXP_OUT_BYTES),
-              terms(reinterpret_cast<float2*>(smem + EPI_WARPS * MXP_OUT_BYTES) + warp * PART) {}
-        __device__ __forceinline__ void unit_begin(const Args&, const Unit&) {}
+            : quarter(quarter_), group(group_), lane(lane_), rank(rank_), piece(smem + warp * PIECE),
+              factors(reinterpret_cast<float*>(smem + EPI_WARPS * PIECE) + warp * 2 * PART), terms(factors + PART) {}
+        __device__ __forceinline__ int first_query(const Unit& u) const { return u.chunk * (PAIR ? 2 * TG_M : TG_M) + rank * TG_M + quarter * 32; }
+        __device__ __forceinline__ int first_row(const Unit& u) const { return u.tile * BN + group * PART; }
+        __device__ __forceinline__ void fetch(const Args& a, const Unit& u) {
+            query.get(a.q_scales, a.q_squares, first_query(u) + lane, a.nq);
+#pragma unroll
+            for (int i = 0; i < PART / 32; ++i) row[i].get(a.scales, a.squares, first_row(u) + i * 32 + lane, a.n);
+        }
+        __device__ __forceinline__ void unit_begin(const Args& a, const Unit& u) {
+            if (u.u < a.step) fetch(a, u);
+        }
         __device__ __forceinline__ void unit_end(const Args&, const Unit&) {}
         template <typename D>
         __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
-            constexpr int PER = 256 / sizeof(OUT), V = 16 / sizeof(OUT);  // scores of a query in a piece, in a store
-            const int q0 = u.chunk * (PAIR ? 2 * TG_M : TG_M) + rank * TG_M + quarter * 32, n0 = u.tile * BN + group * PART;
+            constexpr int PER = 128 / sizeof(OUT), V = 16 / sizeof(OUT);  // scores of a query in a piece, in a store
+            const int q0 = first_query(u), n0 = first_row(u);
+            float2 mine = i8_terms(a.metric, query.scale, query.squares);
+            if (!live) mine.x = __int_as_float(0x7FFFFFFF);
+#pragma unroll
+            for (int i = 0; i < PART / 32; ++i) {
+                const float2 x = i8_terms(a.metric, row[i].scale, row[i].squares);
+                factors[i * 32 + lane] = x.x, terms[i * 32 + lane] = x.y;
+            }
+            __syncwarp();
+            if (a.units - u.u > a.step) fetch(a, Unit(a, u.u + a.step));  // on its way while this unit is worked on
             if (q0 >= a.nq || n0 >= a.n) {
                 done();
                 return;
             }
-            const int q = q0 + lane;
-            float2 mine = q < a.nq ? i8_terms(a.metric, __ldcg(a.q_scales + q), __ldcg(a.q_squares + q)) : make_float2(0.f, 0.f);
-            if (!live) mine.x = __int_as_float(0x7FFFFFFF);
-#pragma unroll
-            for (int i = lane; i < PART; i += 32) terms[i] = n0 + i < a.n ? i8_terms(a.metric, __ldcg(a.scales + n0 + i), __ldcg(a.squares + n0 + i)) : make_float2(0.f, 0.f);
-            __syncwarp();
             OUT* const o = reinterpret_cast<OUT*>(a.out) + (int64_t)q0 * a.ld + n0;
 #pragma unroll 1
             for (int p0 = 0; p0 < PART; p0 += PER) {
-#pragma unroll 1
+#pragma unroll
                 for (int c0 = 0; c0 < PER; c0 += 32) {
                     uint32_t r[32];
-                    tg_read(taddr + p0 + c0, live, r);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(i8_score(a.metric, (int)r[j], mine, terms[p0 + c0 + j]));
+                    tc_ld32(taddr + p0 + c0, r);
+                    tc_ld_wait();
+                    if (p0 + c0 + 32 == PART) done();
+                    i8_scores(a.metric, a.small, r, mine, factors + p0 + c0, terms + p0 + c0);
 #pragma unroll
                     for (int i = 0; i < 32 / V; ++i) {  // 16 bytes each, where neither these stores nor the loads meet in a bank
                         uint4 w;
@@ -98,14 +151,98 @@ struct I8ProductPolicy {
                             w = make_uint4(pack_scores(t, __uint_as_float(v[0]), __uint_as_float(v[1])), pack_scores(t, __uint_as_float(v[2]), __uint_as_float(v[3])),
                                            pack_scores(t, __uint_as_float(v[4]), __uint_as_float(v[5])), pack_scores(t, __uint_as_float(v[6]), __uint_as_float(v[7])));
                         }
-                        *reinterpret_cast<uint4*>(piece + lane * 256 + (((c0 / V + i) ^ (lane & 7)) << 4)) = w;
+                        *reinterpret_cast<uint4*>(piece + lane * 128 + (((c0 / V + i) ^ (lane & 7)) << 4)) = w;
                     }
                 }
-                if (p0 + PER >= PART) done();
                 __syncwarp();
-                if (a.wide) copy_piece<OUT, true>(o + p0, a.ld, piece, a.nq - q0, a.n - n0 - p0, lane);
-                else copy_piece<OUT, false>(o + p0, a.ld, piece, a.nq - q0, a.n - n0 - p0, lane);
+                const int rows = a.nq - q0, left = a.n - n0 - p0;
+                if (a.wide && rows >= 32 && left >= PER) {  // eight lanes a row
+                    OUT* to = o + p0 + (lane >> 3) * a.ld + (lane & 7) * V;
+                    uint4 w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int line = i * 4 + (lane >> 3);
+                        w[i] = *reinterpret_cast<const uint4*>(piece + line * 128 + (((lane & 7) ^ (line & 7)) << 4));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i, to += 4 * a.ld) *reinterpret_cast<uint4*>(to) = w[i];
+                } else {
+#pragma unroll 4
+                    for (int i = 0; i < min(rows, 32); ++i) {
+#pragma unroll
+                        for (int j = lane; j < PER; j += 32) {
+                            const OUT* const from = reinterpret_cast<const OUT*>(piece + i * 128 + (((j / V) ^ (i & 7)) << 4)) + j % V;
+                            if (j < left) o[i * a.ld + p0 + j] = *from;
+                        }
+                    }
+                }
                 __syncwarp();
+            }
+        }
+    };
+};
+
+// Up to 64 queries: the rows are the M side, so that no lane is idle, and a warp's store of a query is 32 neighbouring scores.
+template <typename OUT, int N>
+struct I8FewPolicy {
+    static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = false, PAIR = false;
+    static constexpr int BN = N, EPI_WARPS = 8, SEGMENT = 0, EPI_BYTES = 1024;
+    using Pairs = PlanePairs<1>;
+    using Args = I8ProductArgs;
+    struct Unit {
+        static constexpr int tiles = 1, k0 = 0;
+        unsigned u;
+        int k1;
+        __device__ __forceinline__ Unit(const Args& a, unsigned u_) : u(u_), k1(a.kb) {}
+    };
+    static __device__ __forceinline__ void load(const Args&, const Unit& u, int, int, int, int k, const CUtensorMap* ta, const CUtensorMap* tb, unsigned char* sa, unsigned char* sb,
+                                                uint32_t bar, int) {
+        tma_load_3d<false>(sa, ta, bar, k * 128, (int)u.u * TG_M, 0);
+        tma_load_3d<false>(sb, tb, bar, k * 128, 0, 0);
+    }
+    static __device__ __forceinline__ int n_mma(const Args& a, const Unit&, int) { return (a.nq + 15) & ~15; }
+    struct Epilogue {
+        int quarter, group, lane;
+        float *factors, *terms;  // of the queries, the same for all warps
+        I8Fetch row;
+        __device__ __forceinline__ Epilogue(const Args& a, unsigned char* smem, int, int quarter_, int group_, int lane_, int)
+            : quarter(quarter_), group(group_), lane(lane_), factors(reinterpret_cast<float*>(smem)), terms(factors + I8_FEW) {
+#pragma unroll
+            for (int i = lane; i < I8_FEW; i += 32) {
+                I8Fetch f;
+                f.get(a.q_scales, a.q_squares, i, a.nq);
+                const float2 q = i8_terms(a.metric, f.scale, f.squares);
+                factors[i] = q.x, terms[i] = q.y;
+            }
+            __syncwarp();
+            // the groups take the CTA's units in turn
+            const unsigned first = blockIdx.x + group * a.step;
+            if (first < a.units) row.get(a.scales, a.squares, (int)first * TG_M + quarter * 32 + lane, a.n);
+        }
+        __device__ __forceinline__ void unit_begin(const Args&, const Unit&) {}
+        __device__ __forceinline__ void unit_end(const Args&, const Unit&) {}
+        template <typename D>
+        __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
+            const int at = (int)u.u * TG_M + quarter * 32 + lane;
+            float2 mine = i8_terms(a.metric, row.scale, row.squares);
+            if (!live) mine.x = __int_as_float(0x7FFFFFFF);
+            const uint64_t next = (uint64_t)u.u + 2ull * a.step;
+            if (next < a.units) row.get(a.scales, a.squares, (int)next * TG_M + quarter * 32 + lane, a.n);
+            OUT* o = reinterpret_cast<OUT*>(a.out) + at;
+#pragma unroll 1
+            for (int q0 = 0; q0 < a.nq; q0 += 16) {
+                uint32_t r[16];
+                tc_ld16(taddr + q0, r);
+                tc_ld_wait();
+                if (q0 + 16 >= a.nq) done();
+                if (at >= a.n) continue;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    if (q0 + j >= a.nq) break;
+                    const float v = (float)(int)r[j] * (factors[q0 + j] * mine.x);
+                    store_score(o, a.metric == MX_EUCLIDEAN ? fmaf(2.f, v, -terms[q0 + j]) - mine.y : v);
+                    o += a.ld;
+                }
             }
         }
     };
@@ -119,7 +256,8 @@ struct I8ScoreArgs {
     const int64_t* offsets;
     float* out;
     int64_t total;
-    int n, nq, pitch, metric, lanes;
+    int64_t share;            // candidates of a warp
+    int n, nq, pitch, metric;
 };
 // The list that entry c belongs to, from list `low` on: the last one that begins at or before it.
 __device__ __forceinline__ int i8_owner(const int64_t* offsets, int low, int nq, int64_t c) {
@@ -131,37 +269,83 @@ __device__ __forceinline__ int i8_owner(const int64_t* offsets, int low, int nq,
     }
     return low;
 }
-// A warp takes 32 candidates after the others; `lanes` threads (a power of two up to 32) one of them, 16 bytes of its row each at a time.
+// A warp takes its share of the candidates, 32 at a time; LANES threads one of them, 16 bytes of its row each (and every 16 LANES of a longer one), with up to eight rows' loads in flight.
+// The list that a candidate belongs to is searched for once, and again where it ends.  Bound by the gathers.
+template <int LANES>
 __global__ void __launch_bounds__(256) i8_score_kernel(I8ScoreArgs a, KernelBefore before) {
     behind_kernel_before(before);
-    const int lane = threadIdx.x & 31, at = lane & (a.lanes - 1), groups = 32 / a.lanes, group = lane / a.lanes;
-    const int64_t warps = (int64_t)gridDim.x * 8, spans = (a.total + 31) / 32;
-    for (int64_t s = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); s < spans; s += warps) {
-        const int64_t c = s * 32 + lane;
-        const bool in = c < a.total;
+    constexpr int GROUPS = 32 / LANES, AHEAD = LANES < 8 ? LANES : 8;
+    const int lane = threadIdx.x & 31, at = lane % LANES, group = lane / LANES;
+    const int64_t warp = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), first = warp * a.share, last = min(first + a.share, a.total);
+    if (first >= last) return;
+    int list = i8_owner(a.offsets, 0, a.nq, first);
+    int64_t end = __ldcg(a.offsets + list + 1);
+    const int64_t column = (int64_t)at * 16;
+    const bool one = a.pitch <= LANES * 16, mine_in = column < a.pitch;
+    uint4 held = make_uint4(0u, 0u, 0u, 0u);  // of the query that is worked on
+    int held_list = -1;
+    for (int64_t c0 = first; c0 < last; c0 += 32) {
+        const int64_t c = c0 + lane, to = min(c0 + 31, last - 1);
+        const bool in = c < last;
         const int id = in ? __ldcg(a.ids + c) : -1;
-        const int owner = i8_owner(a.offsets, 0, a.nq, in ? c : a.total - 1);
+        const bool real = (unsigned)id < (unsigned)a.n;
+        const float scale = real ? __ldcg(a.scales + id) : 0.f;
+        const int squares = real ? __ldcg(a.squares + id) : 0;
+        int owner = list;
+        const bool same = to < end;  // for the whole warp
+        if (!same) {
+            owner = i8_owner(a.offsets, list, a.nq, in ? c : to);
+            list = __shfl_sync(0xFFFFFFFFu, owner, 31);
+            end = __ldcg(a.offsets + list + 1);
+        }
+        if (same && one && held_list != list) {
+            if (mine_in) held = __ldcg(reinterpret_cast<const uint4*>(a.q_codes + (int64_t)list * a.pitch + column));
+            held_list = list;
+        }
         float score = __int_as_float(0x7FFFFFFF);
-        for (int i = 0; i < a.lanes; ++i) {
-            const int which = i * groups + group;
-            const int row = __shfl_sync(0xFFFFFFFFu, id, which), q = __shfl_sync(0xFFFFFFFFu, owner, which);
-            int dot = 0;
-            if ((unsigned)row < (unsigned)a.n) {
-                const uint4* const x = reinterpret_cast<const uint4*>(a.codes + (int64_t)row * a.pitch);
-                const uint4* const y = reinterpret_cast<const uint4*>(a.q_codes + (int64_t)q * a.pitch);
-                for (int k = at; k < a.pitch / 16; k += a.lanes) {
-                    const uint4 v = __ldcg(x + k), w = __ldcg(y + k);
-                    dot = __dp4a((int)v.x, (int)w.x, dot);
-                    dot = __dp4a((int)v.y, (int)w.y, dot);
-                    dot = __dp4a((int)v.z, (int)w.z, dot);
-                    dot = __dp4a((int)v.w, (int)w.w, dot);
+        const float2 q = i8_terms(a.metric, __ldcg(a.q_scales + owner), __ldcg(a.q_squares + owner)), x = i8_terms(a.metric, scale, squares);
+#pragma unroll 1
+        for (int i0 = 0; i0 < LANES; i0 += AHEAD) {
+            int dot[AHEAD];
+            if (one) {
+                uint4 v[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int row = __shfl_sync(0xFFFFFFFFu, id, (i0 + i) * GROUPS + group);
+                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if ((unsigned)row < (unsigned)a.n && mine_in) v[i] = __ldcg(reinterpret_cast<const uint4*>(a.codes + (int64_t)row * a.pitch + column));
+                }
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    uint4 w = held;
+                    if (!same) {
+                        const int from = __shfl_sync(0xFFFFFFFFu, owner, (i0 + i) * GROUPS + group);
+                        if (mine_in) w = __ldcg(reinterpret_cast<const uint4*>(a.q_codes + (int64_t)from * a.pitch + column));
+                    }
+                    dot[i] = __dp4a((int)v[i].w, (int)w.w, __dp4a((int)v[i].z, (int)w.z, __dp4a((int)v[i].y, (int)w.y, __dp4a((int)v[i].x, (int)w.x, 0))));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int row = __shfl_sync(0xFFFFFFFFu, id, (i0 + i) * GROUPS + group), from = __shfl_sync(0xFFFFFFFFu, owner, (i0 + i) * GROUPS + group);
+                    dot[i] = 0;
+                    if ((unsigned)row < (unsigned)a.n) {
+                        const int8_t *const rows = a.codes + (int64_t)row * a.pitch, *const queries = a.q_codes + (int64_t)from * a.pitch;
+#pragma unroll 4
+                        for (int k = (int)column; k < a.pitch; k += LANES * 16) {
+                            const uint4 v = __ldcg(reinterpret_cast<const uint4*>(rows + k)), w = __ldcg(reinterpret_cast<const uint4*>(queries + k));
+                            dot[i] = __dp4a((int)v.w, (int)w.w, __dp4a((int)v.z, (int)w.z, __dp4a((int)v.y, (int)w.y, __dp4a((int)v.x, (int)w.x, dot[i]))));
+                        }
+                    }
                 }
             }
-            for (int o = 1; o < a.lanes; o *= 2) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
-            const int mine = __shfl_sync(0xFFFFFFFFu, dot, (lane % groups) * a.lanes);
-            if (lane / groups == i && (unsigned)id < (unsigned)a.n)
-                score = i8_score(a.metric, mine, i8_terms(a.metric, __ldcg(a.q_scales + owner), __ldcg(a.q_squares + owner)),
-                                 i8_terms(a.metric, __ldcg(a.scales + id), __ldcg(a.squares + id)));
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+#pragma unroll
+                for (int o = 1; o < LANES; o *= 2) dot[i] += __shfl_xor_sync(0xFFFFFFFFu, dot[i], o);
+                const int sum = __shfl_sync(0xFFFFFFFFu, dot[i], (lane % GROUPS) * LANES);
+                if (lane / GROUPS == i0 + i && real) score = i8_score(a.metric, sum, q, x);
+            }
         }
         if (in) a.out[c] = score;
     }
@@ -176,23 +360,34 @@ inline void i8_product(const CtxPtr& c, const int8_t* q_codes, const float* q_sc
     I8ProductArgs a{};
     a.d_error = d_error, a.idesc = tg_idesc(TG_I8, false, false);
     a.n = n, a.nq = nq, a.kb = (int)ceil_div(i8_pitch(d), 128), a.metric = metric;
-    const bool pairs = nq > TG_M;
-    a.chunks = (int)ceil_div(nq, pairs ? 2 * TG_M : TG_M), a.tiles = (unsigned)ceil_div(n, I8_BN), a.block = 2 * c->sm_count;
+    const int pitch = i8_pitch(d);
+    const bool few = nq <= I8_FEW, pairs = nq > TG_M;
+    const int side = few ? TG_M : I8_BN;  // rows of a tile
+    a.chunks = few ? 1 : (int)ceil_div(nq, pairs ? 2 * TG_M : TG_M), a.tiles = (unsigned)ceil_div(n, side), a.block = 2 * c->sm_count;
     if ((uint64_t)a.tiles * a.chunks >= (1ull << 31)) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", nq, n);
     a.units = a.tiles * (unsigned)a.chunks;
+    a.step = std::min<unsigned>(a.units, (unsigned)(pairs ? c->sm_count / 2 : c->sm_count));
     a.scales = scales, a.q_scales = q_scales, a.squares = squares, a.q_squares = q_squares, a.out = out, a.ld = ld;
     a.wide = aligned16(out, ld * (int64_t)sizeof(OUT));
-    const int pitch = i8_pitch(d);
-    const CUtensorMap tq = tg_map(q_codes, TG_I8, nq, pitch, pitch, 1, 0, TG_M), tx = tg_map(codes, TG_I8, n, pitch, pitch, 1, 0, pairs ? I8_BN / 2 : I8_BN);
-    if (pairs) tc_gemm<I8ProductPolicy<OUT, true>>(c, tq, tx, a, stream);
+    a.small = (int64_t)pitch * 127 * 127 < 1 << 22;
+    const int box_q = few ? (nq <= I8_FEWEST ? I8_FEWEST : I8_FEW) : TG_M, box_x = few ? TG_M : pairs ? I8_BN / 2 : I8_BN;
+    const CUtensorMap tq = tg_map(q_codes, TG_I8, nq, pitch, pitch, 1, 0, box_q), tx = tg_map(codes, TG_I8, n, pitch, pitch, 1, 0, box_x);
+    if (nq <= I8_FEWEST) tc_gemm<I8FewPolicy<OUT, I8_FEWEST>>(c, tx, tq, a, stream);
+    else if (few) tc_gemm<I8FewPolicy<OUT, I8_FEW>>(c, tx, tq, a, stream);
+    else if (pairs) tc_gemm<I8ProductPolicy<OUT, true>>(c, tq, tx, a, stream);
     else tc_gemm<I8ProductPolicy<OUT, false>>(c, tq, tx, a, stream);
 }
 
 inline void i8_score_lists(const CtxPtr& c, I8ScoreArgs a, cudaStream_t stream) {
-    a.lanes = 1;
-    while (a.lanes < 32 && a.lanes * 16 < a.pitch) a.lanes *= 2;
-    const size_t grid = std::min<size_t>(ceil_div(a.total, 256), (size_t)c->sm_count * 8 * 8);
-    launch_next(stream, i8_score_kernel, grid, 256u, 0, a);
+    const int64_t spans = (int64_t)ceil_div(a.total, 32), most = (int64_t)c->sm_count * 8 * 6;  // warps at a time
+    a.share = 32 * (int64_t)ceil_div(spans, std::min<int64_t>(spans, 4 * most));
+    const size_t grid = ceil_div(ceil_div(a.total, a.share), 8);
+    if (a.pitch <= 16) launch_next(stream, i8_score_kernel<1>, grid, 256u, 0, a);
+    else if (a.pitch <= 32) launch_next(stream, i8_score_kernel<2>, grid, 256u, 0, a);
+    else if (a.pitch <= 64) launch_next(stream, i8_score_kernel<4>, grid, 256u, 0, a);
+    else if (a.pitch <= 128) launch_next(stream, i8_score_kernel<8>, grid, 256u, 0, a);
+    else if (a.pitch <= 256) launch_next(stream, i8_score_kernel<16>, grid, 256u, 0, a);
+    else launch_next(stream, i8_score_kernel<32>, grid, 256u, 0, a);
     KERNEL_CHECK();
 }
 
