@@ -20,6 +20,7 @@ __device__ __forceinline__ float i8_score(int metric, int dot, float2 q, float2 
 
 struct I8ProductArgs {
     int* d_error;
+    unsigned block_units;     // of a block of tiles, all chunks
     unsigned units, step;     // units between one of a CTA, or of a pair, and its next
     uint32_t idesc;
     int n, nq, kb, metric, chunks, block;
@@ -36,7 +37,7 @@ struct I8Unit {
     unsigned u;
     int tile, chunk, k1;
     __device__ __forceinline__ I8Unit(const I8ProductArgs& a, unsigned u_) : u(u_) {  // blocks of neighbouring tiles, a chunk of the queries after the other in each
-        const unsigned b = (unsigned)(u / ((uint64_t)a.block * a.chunks)), left = (unsigned)(u - (uint64_t)b * a.block * a.chunks);
+        const unsigned b = u / a.block_units, left = u - b * a.block_units;
         const unsigned here = min((unsigned)a.block, a.tiles - b * (unsigned)a.block);
         chunk = (int)(left / here);
         tile = (int)(b * (unsigned)a.block + (left - (unsigned)chunk * here));
@@ -289,8 +290,9 @@ __global__ void __launch_bounds__(256) i8_score_kernel(I8ScoreArgs a, KernelBefo
         const bool in = c < last;
         const int id = in ? __ldcg(a.ids + c) : -1;
         const bool real = (unsigned)id < (unsigned)a.n;
-        const float scale = real ? __ldcg(a.scales + id) : 0.f;
-        const int squares = real ? __ldcg(a.squares + id) : 0;
+        // a sector each: only what the metric takes
+        const float scale = real && a.metric != MX_COSINE ? __ldcg(a.scales + id) : 0.f;
+        const int squares = real && a.metric != MX_DOT ? __ldcg(a.squares + id) : 0;
         int owner = list;
         const bool same = to < end;  // for the whole warp
         if (!same) {
@@ -367,6 +369,7 @@ inline void i8_product(const CtxPtr& c, const int8_t* q_codes, const float* q_sc
     if ((uint64_t)a.tiles * a.chunks >= (1ull << 31)) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", nq, n);
     a.units = a.tiles * (unsigned)a.chunks;
     a.step = std::min<unsigned>(a.units, (unsigned)(pairs ? c->sm_count / 2 : c->sm_count));
+    a.block_units = (unsigned)std::min<uint64_t>((uint64_t)a.block * a.chunks, 1ull << 31);
     a.scales = scales, a.q_scales = q_scales, a.squares = squares, a.q_squares = q_squares, a.out = out, a.ld = ld;
     a.wide = aligned16(out, ld * (int64_t)sizeof(OUT));
     a.small = (int64_t)pitch * 127 * 127 < 1 << 22;
