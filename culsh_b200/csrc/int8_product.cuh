@@ -31,7 +31,7 @@ struct I8ProductArgs {
     int64_t ld;
     bool wide, small;         // rows of the result begin at multiples of 16 bytes; sums are below 2^22
 };
-constexpr int I8_BN = 256, I8_FEW = 64, I8_FEWEST = 16;
+constexpr int I8_FEW = 64, I8_FEWEST = 16, I8_SHORT = 2;  // queries; steps of K of short rows
 struct I8Unit {
     static constexpr int tiles = 1, k0 = 0;
     unsigned u;
@@ -81,11 +81,12 @@ __device__ __forceinline__ void i8_scores(int metric, bool small, uint32_t (&r)[
     }
 }
 
-// More than 64 queries: they are the M side, a lane of the accumulator a query.  A warp has 32 queries by 64 rows and stores 128 bytes of each at a time, by way of shared memory.
-template <typename OUT, bool PAIRS>
+// More than 64 queries: they are the M side, a lane of the accumulator a query.  Short rows leave the time to the epilogue: a warp has 32 queries by all 128 rows of a tile, and groups of four
+// take tiles in turn; of long rows a tile has 256, and a warp 64 of them.  128 bytes of each query are stored at a time, by way of shared memory.
+template <typename OUT, bool PAIRS, int N>
 struct I8ProductPolicy {
-    static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = true, PAIR = PAIRS;
-    static constexpr int BN = I8_BN, EPI_WARPS = 16, PART = BN / 4, SEGMENT = 0, PIECE = 32 * 128, EPI_BYTES = EPI_WARPS * (PIECE + PART * 8);
+    static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = N == 256, PAIR = PAIRS;
+    static constexpr int BN = N, EPI_WARPS = 16, PART = PARTS ? BN / 4 : BN, TURNS = PARTS ? 1 : EPI_WARPS / 4, SEGMENT = 0, PIECE = 32 * 128, EPI_BYTES = EPI_WARPS * (PIECE + PART * 8);
     using Pairs = PlanePairs<1>;
     using Args = I8ProductArgs;
     using Unit = I8Unit;
@@ -100,19 +101,20 @@ struct I8ProductPolicy {
         unsigned char* piece;
         float *factors, *terms;
         I8Fetch row[PART / 32], query;
-        __device__ __forceinline__ Epilogue(const Args&, unsigned char* smem, int warp, int quarter_, int group_, int lane_, int rank_)
+        __device__ __forceinline__ Epilogue(const Args& a, unsigned char* smem, int warp, int quarter_, int group_, int lane_, int rank_)
             : quarter(quarter_), group(group_), lane(lane_), rank(rank_), piece(smem + warp * PIECE),
-              factors(reinterpret_cast<float*>(smem + EPI_WARPS * PIECE) + warp * 2 * PART), terms(factors + PART) {}
+              factors(reinterpret_cast<float*>(smem + EPI_WARPS * PIECE) + warp * 2 * PART), terms(factors + PART) {
+            const unsigned first = (PAIR ? blockIdx.x >> 1 : blockIdx.x) + (PARTS ? 0u : group * a.step);
+            if (first < a.units) fetch(a, Unit(a, first));
+        }
         __device__ __forceinline__ int first_query(const Unit& u) const { return u.chunk * (PAIR ? 2 * TG_M : TG_M) + rank * TG_M + quarter * 32; }
-        __device__ __forceinline__ int first_row(const Unit& u) const { return u.tile * BN + group * PART; }
+        __device__ __forceinline__ int first_row(const Unit& u) const { return u.tile * BN + (PARTS ? group * PART : 0); }
         __device__ __forceinline__ void fetch(const Args& a, const Unit& u) {
             query.get(a.q_scales, a.q_squares, first_query(u) + lane, a.nq);
 #pragma unroll
             for (int i = 0; i < PART / 32; ++i) row[i].get(a.scales, a.squares, first_row(u) + i * 32 + lane, a.n);
         }
-        __device__ __forceinline__ void unit_begin(const Args& a, const Unit& u) {
-            if (u.u < a.step) fetch(a, u);
-        }
+        __device__ __forceinline__ void unit_begin(const Args&, const Unit&) {}
         __device__ __forceinline__ void unit_end(const Args&, const Unit&) {}
         template <typename D>
         __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
@@ -126,7 +128,7 @@ struct I8ProductPolicy {
                 factors[i * 32 + lane] = x.x, terms[i * 32 + lane] = x.y;
             }
             __syncwarp();
-            if (a.units - u.u > a.step) fetch(a, Unit(a, u.u + a.step));  // on its way while this unit is worked on
+            if (a.units - u.u > TURNS * a.step) fetch(a, Unit(a, u.u + TURNS * a.step));  // on its way while this unit is worked on
             if (q0 >= a.nq || n0 >= a.n) {
                 done();
                 return;
@@ -364,8 +366,9 @@ inline void i8_product(const CtxPtr& c, const int8_t* q_codes, const float* q_sc
     a.n = n, a.nq = nq, a.kb = (int)ceil_div(i8_pitch(d), 128), a.metric = metric;
     const int pitch = i8_pitch(d);
     const bool few = nq <= I8_FEW, pairs = nq > TG_M;
-    const int side = few ? TG_M : I8_BN;  // rows of a tile
-    a.chunks = few ? 1 : (int)ceil_div(nq, pairs ? 2 * TG_M : TG_M), a.tiles = (unsigned)ceil_div(n, side), a.block = 2 * c->sm_count;
+    const bool brief = a.kb <= I8_SHORT;
+    const int side = few || brief ? 128 : 256;  // rows of a tile
+    a.chunks = few ? 1 : (int)ceil_div(nq, pairs ? 2 * TG_M : TG_M), a.tiles = (unsigned)ceil_div(n, side), a.block = c->sm_count / 2;
     if ((uint64_t)a.tiles * a.chunks >= (1ull << 31)) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", nq, n);
     a.units = a.tiles * (unsigned)a.chunks;
     a.step = std::min<unsigned>(a.units, (unsigned)(pairs ? c->sm_count / 2 : c->sm_count));
@@ -373,12 +376,14 @@ inline void i8_product(const CtxPtr& c, const int8_t* q_codes, const float* q_sc
     a.scales = scales, a.q_scales = q_scales, a.squares = squares, a.q_squares = q_squares, a.out = out, a.ld = ld;
     a.wide = aligned16(out, ld * (int64_t)sizeof(OUT));
     a.small = (int64_t)pitch * 127 * 127 < 1 << 22;
-    const int box_q = few ? (nq <= I8_FEWEST ? I8_FEWEST : I8_FEW) : TG_M, box_x = few ? TG_M : pairs ? I8_BN / 2 : I8_BN;
+    const int box_q = few ? (nq <= I8_FEWEST ? I8_FEWEST : I8_FEW) : TG_M, box_x = few ? TG_M : pairs ? side / 2 : side;
     const CUtensorMap tq = tg_map(q_codes, TG_I8, nq, pitch, pitch, 1, 0, box_q), tx = tg_map(codes, TG_I8, n, pitch, pitch, 1, 0, box_x);
     if (nq <= I8_FEWEST) tc_gemm<I8FewPolicy<OUT, I8_FEWEST>>(c, tx, tq, a, stream);
     else if (few) tc_gemm<I8FewPolicy<OUT, I8_FEW>>(c, tx, tq, a, stream);
-    else if (pairs) tc_gemm<I8ProductPolicy<OUT, true>>(c, tq, tx, a, stream);
-    else tc_gemm<I8ProductPolicy<OUT, false>>(c, tq, tx, a, stream);
+    else if (pairs && brief) tc_gemm<I8ProductPolicy<OUT, true, 128>>(c, tq, tx, a, stream);
+    else if (pairs) tc_gemm<I8ProductPolicy<OUT, true, 256>>(c, tq, tx, a, stream);
+    else if (brief) tc_gemm<I8ProductPolicy<OUT, false, 128>>(c, tq, tx, a, stream);
+    else tc_gemm<I8ProductPolicy<OUT, false, 256>>(c, tq, tx, a, stream);
 }
 
 inline void i8_score_lists(const CtxPtr& c, I8ScoreArgs a, cudaStream_t stream) {

@@ -31,7 +31,7 @@ struct I8Magnitude<double> {
     static __device__ __forceinline__ float scale(Bits m) { return (float)(__longlong_as_double((long long)m) / 127.); }
 };
 // Four codes in a word.  A product with the reciprocal is up to 127 x 2^-23 (1.52e-5) off the quotient; the addition of 1.5 x 2^23 rounds it to a whole number, which is in the low bits.
-// `far` is the largest distance from one: where it is so near a half that the quotient may lie on the other side, the caller has to take the quotients.
+// `far` is the largest distance from one: where it is so near a half that the quotient may lie on the other side, the caller has to look at what is left.
 constexpr float I8_NEAR_HALF = 0.5f - 1.6e-5f;
 __device__ __forceinline__ uint32_t i8_word(const uint32_t (&k)[4]) { return __byte_perm(__byte_perm(k[0], k[1], 0x0040), __byte_perm(k[2], k[3], 0x0040), 0x5410); }
 template <typename T>
@@ -45,10 +45,23 @@ __device__ __forceinline__ uint32_t i8_codes(const T* x, float inv, float& far) 
     }
     return i8_word(k);
 }
+// The same with each code the nearest: what x leaves over k * scale is, near half a scale, a multiple of 2^-24 of the scale's power of two, and so the fused multiply-add has no rounding;
+// beyond a half the next number is nearer, at a half it is taken if it is the even one.
 template <typename T>
-__device__ __noinline__ uint32_t i8_codes_exact(T x0, T x1, T x2, T x3, float scale) {
+__device__ __forceinline__ uint32_t i8_codes_near(const T* x, float scale, float inv) {
+    uint32_t k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float v = (float)x[i], t = fmaf(v, inv, 12582912.f), left = fmaf(12582912.f - t, scale, v), half = 0.5f * scale;
+        k[i] = __float_as_uint(t);
+        if (fabsf(left) > half || (fabsf(left) == half && (k[i] & 1u))) k[i] += left > 0.f ? 1u : ~0u;
+    }
+    return i8_word(k);
+}
+template <>
+__device__ __forceinline__ uint32_t i8_codes_near<double>(const double* x, float scale, float) {
     const double s = (double)scale;
-    const uint32_t k[4] = {(uint32_t)(int)rint((double)x0 / s), (uint32_t)(int)rint((double)x1 / s), (uint32_t)(int)rint((double)x2 / s), (uint32_t)(int)rint((double)x3 / s)};
+    const uint32_t k[4] = {(uint32_t)(int)rint(x[0] / s), (uint32_t)(int)rint(x[1] / s), (uint32_t)(int)rint(x[2] / s), (uint32_t)(int)rint(x[3] / s)};
     return i8_word(k);
 }
 
@@ -124,7 +137,7 @@ __global__ void __launch_bounds__(256) i8_quantize_kernel(const T* __restrict__ 
 #pragma unroll
             for (int i = 0; i < I8_VECS; ++i)
 #pragma unroll
-                for (int j = 0; j < V; j += 4) k[i][j / 4] = i8_codes_exact(held[i].v[j], held[i].v[j + 1], held[i].v[j + 2], held[i].v[j + 3], scale);
+                for (int j = 0; j < V; j += 4) k[i][j / 4] = i8_codes_near(held[i].v + j, scale, inv);
         }
 #pragma unroll
         for (int i = 0; i < I8_VECS; ++i) {
