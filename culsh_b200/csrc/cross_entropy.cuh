@@ -399,20 +399,40 @@ struct CeProductPolicy {
     };
 };
 
+// ---- what the products need beforehand: one launch, whose CTAs have a share of one of five jobs each --------------------------------------------------------------------
+struct CePlanes {  // of a matrix
+    const void* from;
+    int64_t ld, rows;
+    const float* bias;
+    uint16_t* to;
+};
+struct CePrepare {
+    unsigned ends[5];         // CTAs up to the end of each job: planes of Q, of X, the bias, the queries' terms, the targets' sums
+    int m, n, d, pitch, own_rows;
+    CePlanes planes[2];
+    const float* bias;
+    float* bias2;
+    const float *losses, *lse, *lse_low, *grad_losses, *grad_lse;
+    const int64_t* targets;
+    float *terms, *log_terms, *factors, *own, *sums;
+    int *marks, *cols, *where;
+    uint32_t* amax;
+    const void* Q;
+    int64_t ldq;
+};
 // A matrix as planes of 16 bits with rows of `pitch` entries, zeros behind a row's end: three bfloat16 that sum up to each float, or the values as they are.  Rows that the bias masks become
 // zeros: G has zeros for them, and what they hold may not be finite.
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) ce_planes_kernel(const T* __restrict__ X, int64_t ld, int64_t rows, int d, int pitch, const float* __restrict__ bias,
-                                                        uint16_t* __restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, total = rows * (pitch / 2);
+__device__ __forceinline__ void ce_planes_part(const CePrepare& a, const CePlanes& p, unsigned block) {
+    const int64_t i = (int64_t)block * 256 + threadIdx.x, total = p.rows * (a.pitch / 2);
     if (i >= total) return;
-    const int64_t row = i / (pitch / 2);
-    const int col = (int)(i - row * (pitch / 2)) * 2;
-    const T* const x = X + row * ld + col;
+    const int64_t row = total >> 32 ? i / (a.pitch / 2) : (int64_t)((uint32_t)i / (uint32_t)(a.pitch / 2));
+    const int col = (int)(i - row * (a.pitch / 2)) * 2;
+    const T* const x = static_cast<const T*>(p.from) + row * p.ld + col;
     const T zero = (T)0.f;
-    const bool some = !(bias && bias[row] == -INFINITY);
-    const T v0 = some && col < d ? x[0] : zero, v1 = some && col + 1 < d ? x[1] : zero;
-    uint32_t* const o = reinterpret_cast<uint32_t*>(out) + i;
+    const bool some = !(p.bias && __ldcg(p.bias + row) == -INFINITY);
+    const T v0 = some && col < a.d ? __ldcg(x) : zero, v1 = some && col + 1 < a.d ? __ldcg(x + 1) : zero;
+    uint32_t* const o = reinterpret_cast<uint32_t*>(p.to) + i;
     if constexpr (PLANES == 1) {
         uint16_t b[2];
         memcpy(b, &v0, 2);
@@ -421,35 +441,35 @@ __global__ void __launch_bounds__(256) ce_planes_kernel(const T* __restrict__ X,
     } else {
         float f0 = v0, f1 = v1;
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
+        for (int k = 0; k < PLANES; ++k) {
             const uint32_t w = pack_scores(static_cast<const __nv_bfloat16*>(nullptr), f0, f1);
-            o[p * total] = w;
+            o[k * total] = w;
             f0 -= __uint_as_float(w << 16);
             f1 -= __uint_as_float(w & 0xFFFF0000u);
         }
     }
 }
-
-__global__ void __launch_bounds__(256) ce_bias_kernel(const float* __restrict__ bias, int n, float* __restrict__ out) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n) out[i] = bias[i] * CE_LOG2E;
-    else if (i < ((n + 127) & ~127)) out[i] = 0.f;
+__device__ __forceinline__ void ce_bias_part(const CePrepare& a, unsigned block) {
+    const int i = block * 256 + threadIdx.x;
+    if (i < a.n) a.bias2[i] = __ldcg(a.bias + i) * CE_LOG2E;
+    else if (i < ((a.n + 127) & ~127)) a.bias2[i] = 0.f;
 }
 
 // A warp joins a query's blocks.
 __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__ partial, int slots, int m, int n, const int64_t* __restrict__ targets,
                                                       const float* __restrict__ target_scores, const float* __restrict__ bias2, float c, float* __restrict__ losses,
-                                                      float* __restrict__ lse, float* __restrict__ lse_low) {
+                                                      float* __restrict__ lse, float* __restrict__ lse_low, KernelBefore before) {
+    behind_kernel_before(partial, targets, target_scores, bias2, losses, lse, lse_low, before);
     const int q = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     if (q >= m) return;
     const float2* const p = partial + (int64_t)q * slots;
     float top = -INFINITY;
-    for (int i = lane; i < slots; i += 32) top = fmaxf(top, p[i].x);
+    for (int i = lane; i < slots; i += 32) top = fmaxf(top, __ldcg(p + i).x);
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     const float base = top == -INFINITY ? 0.f : top;
     double sum = 0.;
     for (int i = lane; i < slots; i += 32) {
-        const float2 v = p[i];
+        const float2 v = __ldcg(p + i);
         sum += (double)v.y * (double)exp2f(v.x - base);
     }
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -459,61 +479,66 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
     lse[q] = high;
     lse_low[q] = isfinite(high) ? (float)(whole - (double)high) : 0.f;
     float loss = 0.f;
-    const int64_t t = targets ? targets[q] : -1;
+    const int64_t t = targets ? __ldcg(targets + q) : -1;
     if (t >= 0 && t < n) {
-        const double z = (double)target_scores[q] * (double)c + (bias2 ? (double)bias2[t] : 0.);
+        const double z = (double)__ldcg(target_scores + q) * (double)c + (bias2 ? (double)__ldcg(bias2 + t) : 0.);
         loss = z == -INFINITY && two == two ? INFINITY : (float)((two - z) * ln2);
         if (loss < 0.f) loss = 0.f;
     }
     losses[q] = loss;
 }
 
-// What the gradient takes of a query.
-__global__ void __launch_bounds__(256) ce_terms_kernel(const float* __restrict__ losses, const float* __restrict__ lse, const float* __restrict__ lse_low,
-                                                       const int64_t* __restrict__ targets, const float* __restrict__ grad_losses, const float* __restrict__ grad_lse, int m,
-                                                       int n, float* __restrict__ terms, float* __restrict__ log_terms, int* __restrict__ marks, float* __restrict__ factors,
-                                                       float* __restrict__ own, int* __restrict__ cols, uint32_t* __restrict__ amax) {
-    const int q = blockIdx.x * 256 + threadIdx.x;
-    if (q >= m) {
-        if (log_terms && q < ((m + 127) & ~127)) log_terms[q] = -INFINITY, marks[q] = 0;
+// The target of a query that has a loss to go by, or -1; and what its own entry puts into the gradients.
+__device__ __forceinline__ int ce_target(const CePrepare& a, int q) {
+    const int64_t t = a.targets ? __ldcg(a.targets + q) : -1;
+    return t >= 0 && t < a.n && __ldcg(a.losses + q) < INFINITY ? (int)t : -1;
+}
+__device__ __forceinline__ float ce_own(const CePrepare& a, int q) {
+    const float loss = __ldcg(a.losses + q), g = a.grad_losses ? __ldcg(a.grad_losses + q) : 0.f, e = a.grad_lse ? __ldcg(a.grad_lse + q) : 0.f;
+    return g * expm1f(-loss) + e * expf(-loss);
+}
+__device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block) {
+    const int q = block * 256 + threadIdx.x;
+    if (q >= a.m) {
+        if (a.log_terms && q < ((a.m + 127) & ~127)) a.log_terms[q] = -INFINITY, a.marks[q] = 0;
         return;
     }
-    const double two = ((double)lse[q] + (double)lse_low[q]) * 1.4426950408889634074;
+    const double two = ((double)__ldcg(a.lse + q) + (double)__ldcg(a.lse_low + q)) * 1.4426950408889634074;
     const float high = (float)two;
     const bool none = high == -INFINITY;
-    const float loss = losses[q];
-    const int64_t t = targets ? targets[q] : -1;
-    const bool has = t >= 0 && t < n && loss < INFINITY;
-    const float g = has && grad_losses ? grad_losses[q] : 0.f, e = grad_lse ? grad_lse[q] : 0.f;
-    terms[q] = none ? -INFINITY : -high;
+    const int t = ce_target(a, q);
+    const float g = t >= 0 && a.grad_losses ? __ldcg(a.grad_losses + q) : 0.f, e = a.grad_lse ? __ldcg(a.grad_lse + q) : 0.f;
+    a.terms[q] = none ? -INFINITY : -high;
     const float f = (g + e) * (isfinite(high) ? (float)exp2(-(two - (double)high)) : 1.f);
-    factors[q] = f;
-    if (log_terms) {
-        log_terms[q] = none ? -INFINITY : (float)(log2((double)fabsf(f)) - (double)high);
-        marks[q] = (has ? (int)t + 1 : 0) | (f < 0.f ? (int)0x80000000 : 0);
+    a.factors[q] = f;
+    if (a.log_terms) {
+        a.log_terms[q] = none ? -INFINITY : (float)(log2((double)fabsf(f)) - (double)high);
+        a.marks[q] = (t + 1) | (f < 0.f ? (int)0x80000000 : 0);
     }
-    cols[q] = has ? (int)t : -1;
-    own[q] = has ? g * expm1f(-loss) + e * expf(-loss) : 0.f;
-    if (amax && isfinite(f)) atomicMax(amax, __float_as_uint(fabsf(f)));
+    a.cols[q] = t;
+    a.own[q] = t >= 0 ? ce_own(a, q) : 0.f;
+    if (a.amax && isfinite(f)) atomicMax(a.amax, __float_as_uint(fabsf(f)));
 }
 
-// Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes CE_OWN_ROWS rows and looks
+// Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes own_rows rows and looks
 // through all targets; they come in ascending order.
-constexpr int CE_OWN_ROWS = 128, CE_OWN_LIST = 1024, CE_OWN_COLS = 16;  // columns of a lane at a time
+constexpr int CE_OWN_ROWS = 1024, CE_OWN_LIST = 1024, CE_OWN_COLS = 16;  // rows at most; entries; columns of a lane at a time
 template <typename T>
-__global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ cols, const float* __restrict__ own, const T* __restrict__ Q, int64_t ldq, int m, int n, int d,
-                                                     float* __restrict__ sums, int* __restrict__ where) {
+__device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) {
     __shared__ int s_first[CE_OWN_ROWS];
     __shared__ int s_query[CE_OWN_LIST + 256];
-    __shared__ unsigned char s_row[CE_OWN_LIST + 256];
-    __shared__ int s_count[9];
-    const int row0 = blockIdx.x * CE_OWN_ROWS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = threadIdx.x; r < CE_OWN_ROWS; r += 256) s_first[r] = -1;
+    __shared__ uint16_t s_row[CE_OWN_LIST + 256];
+    __shared__ int s_count[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row0 = (int64_t)block * a.own_rows;
+    const T* const Q = static_cast<const T*>(a.Q);
+    for (int r = threadIdx.x; r < a.own_rows; r += 256) s_first[r] = -1;
     int held = 0;  // the same for all threads
-    for (int64_t i0 = 0; i0 < m; i0 += 256) {
+    for (int64_t i0 = 0; i0 < a.m; i0 += 256) {
         const int i = (int)i0 + threadIdx.x;
-        const int r = i0 + threadIdx.x < m ? cols[i] - row0 : -1;
-        const bool hit = (unsigned)r < (unsigned)CE_OWN_ROWS;
+        const int t = i0 + threadIdx.x < a.m ? ce_target(a, i) : -1;
+        const int64_t r = t < 0 ? -1 : t - row0;
+        const bool hit = r >= 0 && r < a.own_rows;
         if (__syncthreads_or(hit)) {
             const unsigned ballot = __ballot_sync(0xFFFFFFFFu, hit);
             if (lane == 0) s_count[warp] = __popc(ballot);
@@ -526,43 +551,40 @@ __global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ col
             if (hit) {
                 at += __popc(ballot & ((1u << lane) - 1u));
                 s_query[at] = i;
-                s_row[at] = (unsigned char)r;
+                s_row[at] = (uint16_t)r;
             }
             held += all;
             __syncthreads();
         }
-        if (held && (held >= CE_OWN_LIST || i0 + 256 >= m)) {
-            for (int rr = warp; rr < CE_OWN_ROWS; rr += 8) {  // a warp takes a row
-                int first = -1;
-                for (int e0 = 0; e0 < held && first < 0; e0 += 32) {
-                    const unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
-                    if (b) first = e0 + __ffs(b) - 1;
-                }
-                if (first < 0) continue;
+        if (held && (held >= CE_OWN_LIST || i0 + 256 >= a.m)) {
+            for (int e = warp; e < held; e += 8) {  // a warp takes an entry, if it is the first of its row, with those that follow
+                const int rr = s_row[e];
+                bool first = true;
+                for (int e0 = 0; e0 < e && first; e0 += 32) first = !__any_sync(0xFFFFFFFFu, e0 + lane < e && s_row[e0 + lane] == rr);
+                if (!first) continue;
                 const bool fresh = s_first[rr] < 0;
-                const int slot = fresh ? s_query[first] : s_first[rr];
-                for (int c0 = 0; c0 < d; c0 += 32 * CE_OWN_COLS) {
+                const int slot = fresh ? s_query[e] : s_first[rr];
+                for (int c0 = 0; c0 < a.d; c0 += 32 * CE_OWN_COLS) {
                     float acc[CE_OWN_COLS];
 #pragma unroll
                     for (int k = 0; k < CE_OWN_COLS; ++k) acc[k] = 0.f;
-                    for (int e0 = first & ~31; e0 < held; e0 += 32) {
+                    for (int e0 = e & ~31; e0 < held; e0 += 32) {
                         unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
                         while (b) {
-                            const int e = e0 + __ffs(b) - 1;
+                            const int query = s_query[e0 + __ffs(b) - 1];
                             b &= b - 1u;
-                            const int query = s_query[e];
-                            const float f = own[query];
-                            const T* const from = Q + (int64_t)query * ldq + c0 + lane;
+                            const float f = ce_own(a, query);
+                            const T* const from = Q + (int64_t)query * a.ldq + c0 + lane;
 #pragma unroll
                             for (int k = 0; k < CE_OWN_COLS; ++k)
-                                if (c0 + k * 32 + lane < d) acc[k] = fmaf(f, ce_float(from[k * 32]), acc[k]);
+                                if (c0 + k * 32 + lane < a.d) acc[k] = fmaf(f, ce_float(__ldcg(from + k * 32)), acc[k]);
                         }
                     }
 #pragma unroll
                     for (int k = 0; k < CE_OWN_COLS; ++k) {
                         const int col = c0 + k * 32 + lane;
-                        if (col < d) {
-                            float* const s = sums + (int64_t)slot * d + col;
+                        if (col < a.d) {
+                            float* const s = a.sums + (int64_t)slot * a.d + col;
                             *s = fresh ? acc[k] : *s + acc[k];
                         }
                     }
@@ -576,41 +598,87 @@ __global__ void __launch_bounds__(256) ce_own_kernel(const int* __restrict__ col
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x; r < CE_OWN_ROWS && row0 + r < n; r += 256) where[row0 + r] = s_first[r];
+    for (int r = threadIdx.x; r < a.own_rows && row0 + r < a.n; r += 256) a.where[row0 + r] = s_first[r];
 }
 
-// Gradients from sums: out[row][col] = (sum over the splits / scale + the target's part) / T.  factors: of the rows, where the sums are of p alone.  QUERIES: the target's part is own[row] times the row cols[row] of X; else sums[where[row]].
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) ce_prepare_kernel(CePrepare a, KernelBefore before) {
+    behind_kernel_before(before);
+    const unsigned b = blockIdx.x;
+    if (b < a.ends[0]) ce_planes_part<T, PLANES>(a, a.planes[0], b);
+    else if (b < a.ends[1]) ce_planes_part<T, PLANES>(a, a.planes[1], b - a.ends[0]);
+    else if (b < a.ends[2]) ce_bias_part(a, b - a.ends[1]);
+    else if (b < a.ends[3]) ce_terms_part(a, b - a.ends[2]);
+    else ce_own_part<T>(a, b - a.ends[3]);
+}
+
+// Gradients from sums: out[row][col] = (sum over the splits, scaled back, + the target's part) / T.  For queries the target's part is own[row] times the row which[row] of X, for rows
+// sums[which[row]].  factors: of the queries, where the sums are of p alone.  One launch for both.
+struct CeFinish {
+    unsigned blocks;
+    const float* parts;
+    int splits;
+    int64_t split_stride, units;  // units of V columns
+    bool wide;                    // V = 4, else 1
+    const float* factors;
+    const int* which;
+    void* out;
+    int64_t ldo;
+};
+struct CeFinishArgs {
+    CeFinish rows, queries;
+    int d;
+    const uint32_t* amax;
+    const float *own, *sums;
+    const void* X;
+    int64_t ldx;
+    float inv_t;
+};
 template <typename T, bool QUERIES, int V>
-__global__ void __launch_bounds__(256) ce_finish_kernel(const float* __restrict__ parts, int splits, int64_t split_stride, unsigned units, int d, const uint32_t* __restrict__ amax,
-                                                        const float* __restrict__ factors, const int* __restrict__ which, const float* __restrict__ own,
-                                                        const T* __restrict__ X, int64_t ldx, const float* __restrict__ sums, float inv_t, T* __restrict__ out, int64_t ldo) {
-    const unsigned i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= units) return;
-    const unsigned each = (unsigned)d / V, row = i / each, col = (i - row * each) * V;
-    const float* const from = parts + (int64_t)row * d + col;
+__device__ __forceinline__ void ce_finish_part(const CeFinishArgs& a, const CeFinish& f, unsigned block) {
+    const int64_t i = (int64_t)block * 256 + threadIdx.x;
+    if (i >= f.units) return;
+    const unsigned each = (unsigned)a.d / V;
+    const int64_t row = f.units >> 32 ? i / each : (int64_t)((uint32_t)i / each);
+    const int col = (int)(i - row * each) * V;
+    const float* const from = f.parts + row * a.d + col;
     float v[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
+    for (int s = 0; s < f.splits; ++s) {
         float w[V];
-        if (V == 4) *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(from + s * split_stride);
-        else w[0] = from[s * split_stride];
+        if (V == 4) *reinterpret_cast<float4*>(w) = __ldcg(reinterpret_cast<const float4*>(from + s * f.split_stride));
+        else w[0] = __ldcg(from + s * f.split_stride);
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] += w[k];
     }
-    const int w = which[row];
-    const float f = factors ? (std::is_same<T, __half>::value ? ldexpf(factors[row], -14) : factors[row]) : amax ? ldexpf(1.f, -ce_scale_exponent(amax)) : 1.f;
-    const float mine = QUERIES && w >= 0 ? own[row] : 0.f;
+    const int w = __ldcg(f.which + row);
+    float scale = 1.f;
+    if (f.factors) scale = std::is_same<T, __half>::value ? ldexpf(__ldcg(f.factors + row), -14) : __ldcg(f.factors + row);
+    else if (a.amax) scale = ldexpf(1.f, -ce_scale_exponent(a.amax));
+    const float mine = QUERIES && w >= 0 ? __ldcg(a.own + row) : 0.f;
     struct alignas(V * sizeof(T)) Some { T v[V]; };
     Some o;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        float x = v[k] * f;
-        if (w >= 0) x += QUERIES ? mine * ce_float(X[(int64_t)w * ldx + col + k]) : sums[(int64_t)w * d + col + k];
-        o.v[k] = (T)(x * inv_t);
+        float x = v[k] * scale;
+        if (w >= 0) x += QUERIES ? mine * ce_float(__ldcg(static_cast<const T*>(a.X) + (int64_t)w * a.ldx + col + k)) : __ldcg(a.sums + (int64_t)w * a.d + col + k);
+        o.v[k] = (T)(x * a.inv_t);
     }
-    *reinterpret_cast<Some*>(out + (int64_t)row * ldo + col) = o;
+    *reinterpret_cast<Some*>(static_cast<T*>(f.out) + row * f.ldo + col) = o;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) ce_finish_kernel(CeFinishArgs a, KernelBefore before) {
+    behind_kernel_before(before);
+    const unsigned b = blockIdx.x;
+    if (b < a.rows.blocks) {
+        if (a.rows.wide) ce_finish_part<T, false, 4>(a, a.rows, b);
+        else ce_finish_part<T, false, 1>(a, a.rows, b);
+    } else {
+        if (a.queries.wide) ce_finish_part<T, true, 4>(a, a.queries, b - a.rows.blocks);
+        else ce_finish_part<T, true, 1>(a, a.queries, b - a.rows.blocks);
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -745,19 +813,33 @@ inline unsigned ce_grid(size_t threads) {
 struct CeOperands {
     const void *q, *x;
     int64_t ldq, ldx;
-    CeOperands(const CeCall& k, const CePlan& p) : q(k.Q), x(k.X), ldq(k.ldq), ldx(k.ldx) {
-        auto bring = [&](const void* from, int64_t ld, int rows, const float* bias, uint16_t* to) {
-            const unsigned grid = ce_grid((size_t)rows * k.pitch() / 2);
-            if (k.type == CULSH_F32) ce_planes_kernel<float, 3><<<grid, 256, 0, k.stream>>>(static_cast<const float*>(from), ld, rows, k.d, k.pitch(), bias, to);
-            else ce_planes_kernel<__half, 1><<<grid, 256, 0, k.stream>>>(static_cast<const __half*>(from), ld, rows, k.d, k.pitch(), bias, to);  // bits are bits
-            KERNEL_CHECK();
+    // Also what the gradient needs of the queries, where `a` says where it comes from.
+    CeOperands(const CeCall& k, const CePlan& p, CePrepare a) : q(k.Q), x(k.X), ldq(k.ldq), ldx(k.ldx) {
+        a.m = k.m, a.n = k.n, a.d = k.d, a.pitch = k.pitch(), a.bias = k.bias, a.bias2 = p.bias2, a.targets = k.targets, a.Q = k.Q, a.ldq = k.ldq;
+        uint64_t end = 0;
+        auto job = [&](int i, size_t ctas) {
+            end += ctas;
+            if (end > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "the matrices are too large for one call");
+            a.ends[i] = (unsigned)end;
         };
-        if (p.q_planes) bring(k.Q, k.ldq, k.m, nullptr, p.q_planes), q = p.q_planes, ldq = k.pitch();
-        if (p.x_planes) bring(k.X, k.ldx, k.n, k.bias, p.x_planes), x = p.x_planes, ldx = k.pitch();
-        if (p.bias2) {
-            ce_bias_kernel<<<ce_grid(k.n), 256, 0, k.stream>>>(k.bias, k.n, p.bias2);
-            KERNEL_CHECK();
-        }
+        auto planes = [&](const void* from, int64_t ld, int rows, const float* bias, uint16_t* to) {
+            a.planes[to == p.x_planes] = CePlanes{from, ld, rows, bias, to};
+            return to ? ceil_div((size_t)rows * k.pitch() / 2, 256) : 0;
+        };
+        job(0, p.q_planes ? planes(k.Q, k.ldq, k.m, nullptr, p.q_planes) : 0);
+        job(1, p.x_planes ? planes(k.X, k.ldx, k.n, k.bias, p.x_planes) : 0);
+        job(2, p.bias2 ? ceil_div((size_t)k.n + 127, 256) : 0);
+        job(3, p.terms ? ceil_div((size_t)k.m + 127, 256) : 0);
+        a.terms = p.terms, a.log_terms = p.log_terms, a.factors = p.factors, a.own = p.own, a.sums = p.sums, a.marks = p.marks, a.cols = p.cols, a.where = p.where, a.amax = p.amax;
+        a.own_rows = (int)std::min<size_t>(CE_OWN_ROWS, ceil_div(ceil_div(k.n, 2 * (size_t)k.c->sm_count), 128) * 128);
+        job(4, p.where ? ceil_div(k.n, a.own_rows) : 0);
+        if (p.q_planes) q = p.q_planes, ldq = k.pitch();
+        if (p.x_planes) x = p.x_planes, ldx = k.pitch();
+        if (!end) return;
+        if (k.type == CULSH_F32) launch_next(k.stream, ce_prepare_kernel<float, 3>, (size_t)end, 256u, 0, a);
+        else if (k.type == CULSH_F16) launch_next(k.stream, ce_prepare_kernel<__half, 1>, (size_t)end, 256u, 0, a);
+        else launch_next(k.stream, ce_prepare_kernel<__nv_bfloat16, 1>, (size_t)end, 256u, 0, a);
+        KERNEL_CHECK();
     }
     CUtensorMap map_q(const CeCall& k, int box) const { return tg_map(q, k.tg(), k.m, k.d, ldq, k.planes(), (int64_t)k.m * ldq * 2, box); }
     CUtensorMap map_x(const CeCall& k, int box) const { return tg_map(x, k.tg(), k.n, k.d, ldx, k.planes(), (int64_t)k.n * ldx * 2, box); }
@@ -792,7 +874,7 @@ inline void ce_by(F&& f, bool three, bool bias, bool segments, bool pairs) {
 
 inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse_low, void* workspace) {
     const CePlan p(k, false, false, false, workspace);
-    const CeOperands ops(k, p);
+    const CeOperands ops(k, p, CePrepare{});
     CeScoreArgs a = ce_score_args(k, p);
     a.block = p.block, a.slots = p.slots, a.partial = p.partial, a.target_scores = p.target_scores;
     const size_t units = ceil_div(a.tiles_n, p.block) * a.tiles_q;
@@ -803,27 +885,29 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     ce_by([&](auto planes, auto bias, auto segs, auto pairs) {
         tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value, decltype(pairs)::value>>(k.c, tq, tx, a, k.stream);
     }, k.planes() == 3, k.bias != nullptr, segments, CePlan::pairs(k.m));
-    ce_join_kernel<<<ce_grid((size_t)k.m * 32), 256, 0, k.stream>>>(p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
+    launch_next(k.stream, ce_join_kernel, ce_grid((size_t)k.m * 32), 256u, 0, (const float2*)p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
     KERNEL_CHECK();
 }
 
-template <typename T, bool QUERIES>
-inline void ce_finish(const CeCall& k, const float* parts, int splits, int64_t split_stride, int64_t rows, const uint32_t* amax, const float* factors, const int* which, const float* own,
-                      const T* X, int64_t ldx, const float* sums, T* out, int64_t ldo) {
-    const float inv_t = (float)(1 / k.temperature);
-    const bool wide = k.d % 4 == 0 && ldo % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
-    const int64_t step = std::max<int64_t>(1, 0x70000000 / k.d);  // rows of a launch
-    for (int64_t r0 = 0; r0 < rows; r0 += step) {
-        const int64_t here = std::min(step, rows - r0);
-        const unsigned units = (unsigned)(here * (k.d / (wide ? 4 : 1)));
-        auto go = [&](auto kern) {
-            kern<<<ce_grid(units), 256, 0, k.stream>>>(parts + r0 * k.d, splits, split_stride, units, k.d, amax, factors ? factors + r0 : nullptr, which + r0, own ? own + r0 : nullptr, X,
-                                                       ldx, sums, inv_t, out + r0 * ldo, ldo);
-            KERNEL_CHECK();
-        };
-        if (wide) go(ce_finish_kernel<T, QUERIES, 4>);
-        else go(ce_finish_kernel<T, QUERIES, 1>);
-    }
+// One side of the last launch.
+template <typename T>
+inline CeFinish ce_finish_of(const CeCall& k, const float* parts, int splits, int64_t rows, const float* factors, const int* which, T* out, int64_t ldo) {
+    CeFinish f{};
+    f.parts = parts, f.splits = splits, f.split_stride = rows * k.d, f.factors = factors, f.which = which, f.out = out, f.ldo = ldo;
+    f.wide = k.d % 4 == 0 && ldo % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
+    f.units = rows * (k.d / (f.wide ? 4 : 1));
+    f.blocks = ce_grid((size_t)f.units);
+    return f;
+}
+template <typename T>
+inline void ce_finish(const CeCall& k, const CePlan& p, const CeFinish& rows, const CeFinish& queries) {
+    CeFinishArgs a{};
+    a.rows = rows, a.queries = queries, a.d = k.d, a.amax = p.amax, a.own = p.own, a.sums = p.sums, a.X = k.X, a.ldx = k.ldx, a.inv_t = (float)(1 / k.temperature);
+    const size_t grid = (size_t)rows.blocks + queries.blocks;
+    if (!grid) return;
+    if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "the matrices are too large for one call");
+    launch_next(k.stream, ce_finish_kernel<T>, grid, 256u, 0, a);
+    KERNEL_CHECK();
 }
 
 template <int PLANES, bool AMN>
@@ -886,14 +970,11 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
     constexpr int PLANES = std::is_same<T, float>::value ? 3 : 1;
     constexpr bool HALF = std::is_same<T, __half>::value;
     const CePlan p(k, true, grad_Q != nullptr, grad_X != nullptr, workspace);
-    const CeOperands ops(k, p);
     if (p.amax) CU_CHECK(cudaMemsetAsync(p.amax, 0, 4, k.stream));
-    ce_terms_kernel<<<ce_grid(k.m), 256, 0, k.stream>>>(losses, lse, lse_low, k.targets, grad_losses, grad_lse, k.m, k.n, p.terms, p.log_terms, p.marks, p.factors, p.own, p.cols, p.amax);
-    KERNEL_CHECK();
-    if (grad_X) {
-        ce_own_kernel<<<(unsigned)ceil_div(k.n, CE_OWN_ROWS), 256, 0, k.stream>>>(p.cols, p.own, static_cast<const T*>(k.Q), k.ldq, k.m, k.n, k.d, p.sums, p.where);
-        KERNEL_CHECK();
-    }
+    CePrepare before{};
+    before.losses = losses, before.lse = lse, before.lse_low = lse_low, before.grad_losses = grad_losses, before.grad_lse = grad_lse;
+    const CeOperands ops(k, p, before);
+    CeFinish last{};  // of dX, for the launch that finishes dQ
     if constexpr (PLANES == 1) {
         if (p.fused_x) ce_fused<true, HALF>(k, p, ops, grad_X, ld_gx);
         if (p.fused_q) ce_fused<false, HALF>(k, p, ops, nullptr, 0);
@@ -925,8 +1006,10 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
                 a.inv_t = (float)(1 / k.temperature);
             }
             ce_product<PLANES, true>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, 64), ops.q, ops.ldq, k.m, a, p.per_x, p.splits_x);
-            if (p.splits_x > 1 || PLANES == 3)
-                ce_finish<T, false>(k, p.parts_x, p.splits_x, (int64_t)here * k.d, here, p.amax, nullptr, p.where + n0, nullptr, nullptr, 0, p.sums, grad_X + n0 * ld_gx, ld_gx);
+            if (p.splits_x > 1 || PLANES == 3) {
+                last = ce_finish_of(k, p.parts_x, p.splits_x, here, nullptr, p.where + n0, grad_X + n0 * ld_gx, ld_gx);
+                if (n0 + here < k.n) ce_finish<T>(k, p, last, CeFinish{}), last = CeFinish{};
+            }
         }
         if (pieces_q) {
             CeProductArgs a{};
@@ -934,10 +1017,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
             ce_product<PLANES, false>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, TG_M), ops.x, ops.ldx, k.n, a, p.per_q, p.splits_q);
         }
     }
-    if (grad_Q) {
-        ce_finish<T, true>(k, p.acc_q, p.splits_q, (int64_t)k.m * k.d, k.m, p.amax, p.fused_q ? p.factors : nullptr, p.cols, p.own, static_cast<const T*>(k.X), k.ldx, nullptr, grad_Q,
-                           ld_gq);
-    }
+    ce_finish<T>(k, p, last, grad_Q ? ce_finish_of(k, p.acc_q, p.splits_q, k.m, p.fused_q ? p.factors : nullptr, p.cols, grad_Q, ld_gq) : CeFinish{});
 }
 
 }  // namespace culsh_b200
