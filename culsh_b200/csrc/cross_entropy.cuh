@@ -522,11 +522,12 @@ __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block
 
 // Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes own_rows rows and looks
 // through all targets; they come in ascending order.
-constexpr int CE_OWN_ROWS = 1024, CE_OWN_LIST = 1024, CE_OWN_COLS = 16;  // rows at most; entries; columns of a lane at a time
+constexpr int CE_OWN_ROWS = 1024, CE_OWN_LIST = 1024, CE_OWN_COLS = 16, CE_OWN_AHEAD = 8;  // rows at most; entries; columns of a lane at a time; targets of a thread
 template <typename T>
 __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) {
     __shared__ int s_first[CE_OWN_ROWS];
     __shared__ int s_query[CE_OWN_LIST + 256];
+    __shared__ float s_own[CE_OWN_LIST + 256];
     __shared__ uint16_t s_row[CE_OWN_LIST + 256];
     __shared__ int s_count[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -534,11 +535,29 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
     const T* const Q = static_cast<const T*>(a.Q);
     for (int r = threadIdx.x; r < a.own_rows; r += 256) s_first[r] = -1;
     int held = 0;  // the same for all threads
+    int64_t of[CE_OWN_AHEAD];
     for (int64_t i0 = 0; i0 < a.m; i0 += 256) {
+        const int ahead = (int)(i0 / 256 % CE_OWN_AHEAD);
+        if (ahead == 0) {  // targets of the next steps; most CTAs have none of them
+            bool any = false;
+#pragma unroll
+            for (int k = 0; k < CE_OWN_AHEAD; ++k) {
+                const int64_t i = i0 + k * 256 + threadIdx.x;
+                const int64_t r = (a.targets && i < a.m ? __ldcg(a.targets + i) : -1) - row0;
+                of[k] = r >= 0 && r < a.own_rows && r + row0 < a.n ? r : -1;
+                any = any || of[k] >= 0;
+            }
+            if (!__syncthreads_or(any) && !held) {
+                i0 += (CE_OWN_AHEAD - 1) * 256;
+                continue;
+            }
+        }
+        int64_t r = -1;
+#pragma unroll
+        for (int k = 0; k < CE_OWN_AHEAD; ++k)
+            if (k == ahead) r = of[k];
         const int i = (int)i0 + threadIdx.x;
-        const int t = i0 + threadIdx.x < a.m ? ce_target(a, i) : -1;
-        const int64_t r = t < 0 ? -1 : t - row0;
-        const bool hit = r >= 0 && r < a.own_rows;
+        const bool hit = r >= 0 && __ldcg(a.losses + i) < INFINITY;
         if (__syncthreads_or(hit)) {
             const unsigned ballot = __ballot_sync(0xFFFFFFFFu, hit);
             if (lane == 0) s_count[warp] = __popc(ballot);
@@ -552,6 +571,7 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
                 at += __popc(ballot & ((1u << lane) - 1u));
                 s_query[at] = i;
                 s_row[at] = (uint16_t)r;
+                s_own[at] = ce_own(a, i);
             }
             held += all;
             __syncthreads();
@@ -571,9 +591,9 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
                     for (int e0 = e & ~31; e0 < held; e0 += 32) {
                         unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
                         while (b) {
-                            const int query = s_query[e0 + __ffs(b) - 1];
+                            const int at = e0 + __ffs(b) - 1, query = s_query[at];
                             b &= b - 1u;
-                            const float f = ce_own(a, query);
+                            const float f = s_own[at];
                             const T* const from = Q + (int64_t)query * a.ldq + c0 + lane;
 #pragma unroll
                             for (int k = 0; k < CE_OWN_COLS; ++k)
@@ -785,7 +805,7 @@ struct CePlan {
         const size_t tn = ceil_div(k.d, bn);
         auto split = [&](size_t tiles, int kb, int& splits, int& per) {
             const int most = k.type == CULSH_F32 ? 16 : 512;  // steps of 64 in one accumulator: its adds cut off, 2^-24 of it at a time
-            const size_t want = std::max<size_t>(ceil_div(kb, most), std::min<size_t>(sms / std::max<size_t>(tiles, 1), kb / 8));
+            const size_t want = std::max<size_t>(ceil_div(kb, most), std::min<size_t>(sms / std::max<size_t>(tiles, 1), kb / 2));
             per = (int)ceil_div(kb, std::max<size_t>(want, 1));
             splits = (int)ceil_div(kb, per);
         };

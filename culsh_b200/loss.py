@@ -13,6 +13,7 @@ graph.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -47,11 +48,18 @@ def _sides(Q, X, bias):
     return Q, X, None if bias is None else _floats(bias, "bias", (X.shape[0],), Q.device)
 
 
-def _workspace(h, Q, X, bias, gradients):
-    need = C.c_uint64()
-    _lib.check(h.lib.culsh_cross_entropy_workspace(h.ptr, Q.data_ptr(), _pitch(Q), X.data_ptr(), _pitch(X), _TYPES[Q.dtype], Q.shape[0], X.shape[0], Q.shape[1],
-                                                   bias is not None, gradients, C.byref(need)))
-    return torch.empty(need.value, dtype=torch.uint8, device=Q.device), need.value
+@functools.lru_cache(maxsize=256)
+def _workspace_size(device, q_at, q_pitch, x_at, x_pitch, dtype, m, n, d, has_bias, gradients):
+    """A workspace's size goes by sizes and alignments alone: the addresses are what they leave by 16, and 16."""
+    h, need = get_handle(device), C.c_uint64()
+    _lib.check(h.lib.culsh_cross_entropy_workspace(h.ptr, q_at + 16, q_pitch, x_at + 16, x_pitch, _TYPES[dtype], m, n, d, has_bias, gradients, C.byref(need)))
+    return need.value
+
+
+def _workspace(Q, X, m, n, d, bias, gradients):
+    device = Q.device
+    size = _workspace_size(device.index, Q.data_ptr() & 15, _pitch(Q), X.data_ptr() & 15, _pitch(X), Q.dtype, m, n, d, bias is not None, gradients)
+    return torch.empty(size, dtype=torch.uint8, device=device), size
 
 
 def cross_entropy(Q, X, targets, bias=None, temperature: float = 1.0) -> CrossEntropy:
@@ -69,7 +77,7 @@ def cross_entropy(Q, X, targets, bias=None, temperature: float = 1.0) -> CrossEn
     result = CrossEntropy(*out.unbind())
     if m:
         h = get_handle(device.index)
-        work, size = _workspace(h, Q, X, bias, 0)
+        work, size = _workspace(Q, X, m, int(X.shape[0]), int(Q.shape[1]), bias, 0)
         at = out.data_ptr()
         _lib.check(h.lib.culsh_cross_entropy(h.ptr, Q.data_ptr(), _pitch(Q), X.data_ptr(), _pitch(X), _TYPES[Q.dtype], m, X.shape[0], Q.shape[1], targets.data_ptr(),
                                              None if bias is None else bias.data_ptr(), float(temperature), at, at + 4 * m, at + 8 * m, work.data_ptr(), size,
@@ -98,7 +106,7 @@ def cross_entropy_backward(Q, X, targets, result: CrossEntropy, grad_losses=None
         return grad_Q, None if grad_X is None else grad_X.zero_()
     if queries or rows:
         h = get_handle(device.index)
-        work, size = _workspace(h, Q, X, bias, bool(queries) + 2 * bool(rows))
+        work, size = _workspace(Q, X, m, n, d, bias, bool(queries) + 2 * bool(rows))
         _lib.check(h.lib.culsh_cross_entropy_backward(
             h.ptr, Q.data_ptr(), _pitch(Q), X.data_ptr(), _pitch(X), _TYPES[Q.dtype], m, n, d, None if targets is None else targets.data_ptr(),
             None if bias is None else bias.data_ptr(), float(temperature), losses.data_ptr(), lse.data_ptr(), low.data_ptr(), None if g is None else g.data_ptr(),

@@ -298,16 +298,14 @@ class Int8Rows:
         if d > MAX_INT8_FEATURES:
             raise ValueError(f"at most {MAX_INT8_FEATURES} features")
         self._n, self._d, self._h = n, d, get_handle(X.device.index)
-        # one allocation; the tensors that show its parts are made when they are asked for
-        pitch = -(-d // 16) * 16
-        self._codes = self._scales = self._squares = None
-        self._held = torch.empty(n * (pitch + 8), dtype=torch.uint8, device=X.device)
-        at = self._held.data_ptr()
-        self._at = (at, at + n * pitch, at + n * (pitch + 4))
-        self.device = X.device
+        device = self.device = X.device
+        self.codes = torch.empty((n, -(-d // 16) * 16), dtype=torch.int8, device=device)
+        self.scales = torch.empty(n, dtype=torch.float32, device=device)
+        self.squares = torch.empty(n, dtype=torch.int32, device=device)
+        self._at = (self.codes.data_ptr(), self.scales.data_ptr(), self.squares.data_ptr())
         if n:
             h = self._h
-            _lib.check(h.lib.culsh_i8_quantize(h.ptr, X.data_ptr(), _TYPES[X.dtype], n, d, _pitch(X), *self._at, _stream(X.device)))
+            _lib.check(h.lib.culsh_i8_quantize(h.ptr, X.data_ptr(), _TYPES[X.dtype], n, d, _pitch(X), *self._at, _stream(device)))
 
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, squares: torch.Tensor, n_features: int) -> "Int8Rows":
@@ -331,36 +329,12 @@ class Int8Rows:
             codes = codes.clone()
         self = cls.__new__(cls)
         self._n, self._d, self._h, self.device = n, d, get_handle(codes.device.index), codes.device
-        self._codes, self._scales, self._squares = codes, scales.contiguous(), squares.contiguous()
-        self._at = (self._codes.data_ptr(), self._scales.data_ptr(), self._squares.data_ptr())
+        self.codes, self.scales, self.squares = codes, scales.contiguous(), squares.contiguous()
+        self._at = (codes.data_ptr(), self.scales.data_ptr(), self.squares.data_ptr())
         return self
 
     n_rows = property(lambda self: self._n)
     n_features = property(lambda self: self._d)
-
-    def _part(self, first, last, dtype):
-        return self._held[first * self._n:last * self._n].view(dtype)
-
-    @property
-    def codes(self) -> torch.Tensor:
-        if self._codes is None:
-            pitch = -(-self._d // 16) * 16
-            self._codes = self._part(0, pitch, torch.int8).view(self._n, pitch)
-        return self._codes
-
-    @property
-    def scales(self) -> torch.Tensor:
-        if self._scales is None:
-            pitch = -(-self._d // 16) * 16
-            self._scales = self._part(pitch, pitch + 4, torch.float32)
-        return self._scales
-
-    @property
-    def squares(self) -> torch.Tensor:
-        if self._squares is None:
-            pitch = -(-self._d // 16) * 16
-            self._squares = self._part(pitch + 4, pitch + 8, torch.int32)
-        return self._squares
 
     def size_bytes(self) -> int:
         return self._n * (-(-self._d // 16) * 16 + 8)
