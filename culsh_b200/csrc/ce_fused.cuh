@@ -33,6 +33,19 @@ __device__ __forceinline__ int ce_scale_exponent(const uint32_t* amax) {
     return bits == 0u ? 0 : min(max(14 + 127 - (int)(bits >> 23), -100), 100);
 }
 
+// 32 rows of 32 values, a row to a lane, turned: lane i gets column i, v[j] that of row j.
+__device__ __forceinline__ void ce_turn(float (&v)[32], int lane) {
+#pragma unroll
+    for (int s = 16; s; s >>= 1)
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (!(j & s)) {
+                const bool high = lane & s;
+                const float got = __shfl_xor_sync(0xFFFFFFFFu, high ? v[j] : v[j | s], s);
+                if (high) v[j] = got;
+                else v[j | s] = got;
+            }
+}
 struct CeFusedArgs {
     int* d_error;
     unsigned units;
@@ -46,7 +59,7 @@ struct CeFusedArgs {
     const int* target_cols;
     const int* marks;         // of the queries, for dX: target + 1, or 0, and the factor's sign in the highest bit; as `terms` in lines of 128 with -inf and 0 behind the last query
     const uint32_t* amax;
-    float* parts;             // dQ: [block][query][d]
+    float* parts;             // sums: [block][own entry][d]; of dX NULL where they are complete
     void* out;                // dX
     int64_t ld;
     const int* where;
@@ -356,49 +369,51 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             // the sums, 32 columns to four warps in turn
             if (live) live = mbar_wait_warp(o_full, units & 1u, s_abort, a.d_error);
             tc_fence_after();
-            const bool wide = ROWS ? (a.d & 7) == 0 && (a.ld & 7) == 0 && ((uintptr_t)a.out & 15) == 0 : (a.d & 3) == 0;
+            const bool typed = ROWS && !a.parts;
+            const bool wide = typed ? (a.d & 7) == 0 && (a.ld & 7) == 0 && ((uintptr_t)a.out & 15) == 0 : (a.d & 3) == 0;
 #pragma unroll 1
             for (int c0 = (warp - 4) / 4 * 32; c0 < a.d; c0 += Cfg::WARPS * GROUPS / 4 * 32) {
                 uint32_t r[32];
                 tg_read(tmem + lanes + c0, live, r);
-                if (!in) continue;
-                if constexpr (ROWS) {
-                    const float scale = a.inv_t;
-                    T* const o = reinterpret_cast<T*>(a.out) + (int64_t)mine * a.ld + c0;
-                    const float* const extra = a.sums + (int64_t)slot * a.d + c0;
-                    float v[32];
+                float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        v[j] = __uint_as_float(r[j]);
-                        if (HALF) v[j] = ldexpf(v[j], -exponent);
-                        if (slot >= 0 && c0 + j < a.d) v[j] += __ldcg(extra + j);
-                        v[j] *= scale;
-                    }
-                    if (wide) {
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+                if (typed) {
+                    const float scale = HALF ? ldexpf(a.inv_t, -exponent) : a.inv_t;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            if (c0 + j >= a.d) break;
-                            const T* const t = nullptr;
-                            *reinterpret_cast<uint4*>(o + j) = make_uint4(pack_scores(t, v[j], v[j + 1]), pack_scores(t, v[j + 2], v[j + 3]), pack_scores(t, v[j + 4], v[j + 5]),
-                                                                          pack_scores(t, v[j + 6], v[j + 7]));
-                        }
-                    } else {
+                    for (int j = 0; j < 32; ++j) v[j] *= scale;
+                    if (slot >= 0) {
+                        const float* const extra = a.sums + (int64_t)slot * a.d + c0;
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (c0 + j < a.d) store_score(o + j, v[j]);
+                            if (c0 + j < a.d) v[j] = fmaf(__ldcg(extra + j), a.inv_t, v[j]);
                     }
-                } else {
-                    float* const o = a.parts + ((int64_t)unit.block * a.own + mine) * a.d + c0;
-                    if (wide) {
+                }
+                T* const o = reinterpret_cast<T*>(a.out) + (int64_t)mine * a.ld + c0;
+                float* const part = a.parts + ((int64_t)unit.block * a.own + mine) * a.d + c0;
+                if (!wide) {
+                    ce_turn(v, lane);
+                    if (c0 + lane < a.d) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            if (c0 + j >= a.d) break;
-                            *reinterpret_cast<uint4*>(o + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+                        for (int j = 0; j < 32; ++j) {
+                            if (first_own + j >= a.own) break;
+                            if (typed) store_score(o + (int64_t)(j - lane) * a.ld + lane, v[j]);
+                            else part[(int64_t)(j - lane) * a.d + lane] = v[j];
                         }
-                    } else {
+                    }
+                } else if (in && typed) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c0 + j < a.d) o[j] = __uint_as_float(r[j]);
+                    for (int j = 0; j < 32; j += 8) {
+                        if (c0 + j >= a.d) break;
+                        const T* const t = nullptr;
+                        *reinterpret_cast<uint4*>(o + j) =
+                            make_uint4(pack_scores(t, v[j], v[j + 1]), pack_scores(t, v[j + 2], v[j + 3]), pack_scores(t, v[j + 4], v[j + 5]), pack_scores(t, v[j + 6], v[j + 7]));
+                    }
+                } else if (in) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        if (c0 + j >= a.d) break;
+                        *reinterpret_cast<float4*>(part + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                     }
                 }
             }

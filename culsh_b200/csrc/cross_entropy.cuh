@@ -288,14 +288,37 @@ struct CeProductUnit {
     }
 };
 // N columns of a row of dX from column col0 on.
+template <typename T>
+__device__ __noinline__ void ce_store_turned(const CeProductArgs& a, int row, int lane, int col, float scale, const float* extra, uint32_t taddr, bool live) {
+    uint32_t r[32];
+    tg_read(taddr, live, r);
+    float v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
+    if (extra) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (col + j < a.cols) v[j] = fmaf(__ldcg(extra + j), a.inv_t, v[j]);
+    }
+    ce_turn(v, lane);
+    T* const to = reinterpret_cast<T*>(a.typed) + (int64_t)(row - lane) * a.ld + col + lane;
+    if (col + lane < a.cols) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (row - lane + j < a.rows) store_score(to + j * a.ld, v[j]);
+    }
+}
 template <typename T, int N>
-__device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, int col0, uint32_t taddr, bool live) {
+__device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, int lane, int col0, uint32_t taddr, bool live) {
     const bool in = row < a.rows;
     const int slot = in ? __ldcg(a.where + row) : -1;
     const float scale = ldexpf(a.inv_t, std::is_same<T, __half>::value ? -ce_scale_exponent(a.amax) : 0);
     const float* const extra = a.sums + (int64_t)max(slot, 0) * a.cols + col0;
+    if ((a.cols & 7) != 0 || (a.ld & 7) != 0 || ((uintptr_t)a.typed & 15) != 0) {  // no 16 bytes of a row lie together: rows turned, so that neighbouring lanes have neighbouring columns
+        for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) ce_store_turned<T>(a, row, lane, col0 + c0, scale, slot >= 0 ? extra + c0 : nullptr, taddr + c0, live);
+        return;
+    }
     T* const o = reinterpret_cast<T*>(a.typed) + (int64_t)row * a.ld + col0;
-    const bool wide = (a.cols & 7) == 0 && (a.ld & 7) == 0 && ((uintptr_t)a.typed & 15) == 0;
 #pragma unroll 1
     for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) {
         uint32_t r[32];
@@ -309,18 +332,12 @@ __device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, 
             for (int j = 0; j < 32; ++j)
                 if (col0 + c0 + j < a.cols) v[j] = fmaf(__ldcg(extra + c0 + j), a.inv_t, v[j]);
         }
-        if (wide) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-                if (col0 + c0 + j >= a.cols) break;
-                const T* const t = nullptr;
-                *reinterpret_cast<uint4*>(o + c0 + j) =
-                    make_uint4(pack_scores(t, v[j], v[j + 1]), pack_scores(t, v[j + 2], v[j + 3]), pack_scores(t, v[j + 4], v[j + 5]), pack_scores(t, v[j + 6], v[j + 7]));
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (col0 + c0 + j < a.cols) store_score(o + c0 + j, v[j]);
+        for (int j = 0; j < 32; j += 8) {
+            if (col0 + c0 + j >= a.cols) break;
+            const T* const t = nullptr;
+            *reinterpret_cast<uint4*>(o + c0 + j) =
+                make_uint4(pack_scores(t, v[j], v[j + 1]), pack_scores(t, v[j + 2], v[j + 3]), pack_scores(t, v[j + 4], v[j + 5]), pack_scores(t, v[j + 6], v[j + 7]));
         }
     }
 }
@@ -361,7 +378,7 @@ struct CeProductPolicy {
                 return;
             }
             if constexpr (TYPED != 0) {
-                ce_store_typed<std::conditional_t<TYPED == 2, __half, __nv_bfloat16>, BN / 2>(a, row, u.nt * BN + group * (BN / 2), taddr, live);
+                ce_store_typed<std::conditional_t<TYPED == 2, __half, __nv_bfloat16>, BN / 2>(a, row, lane, u.nt * BN + group * (BN / 2), taddr, live);
                 done();
                 return;
             }
@@ -372,25 +389,29 @@ struct CeProductPolicy {
             for (int c0 = 0; c0 < width; c0 += 32) {
                 uint32_t r[32];
                 tg_read(taddr + c0, live, r);
-                if (row < a.rows) {
-                    if (wide) {
+                if (wide) {
+                    if (row >= a.rows) continue;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            if (c0 + j >= width) break;
-                            float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-                            float4* const o = reinterpret_cast<float4*>(out + c0 + j);
-                            if (a.accumulate) {
-                                const float4 w = __ldcg(o);
-                                v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-                            }
-                            *o = v;
+                    for (int j = 0; j < 32; j += 4) {
+                        if (c0 + j >= width) break;
+                        float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+                        float4* const o = reinterpret_cast<float4*>(out + c0 + j);
+                        if (a.accumulate) {
+                            const float4 w = __ldcg(o);
+                            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
                         }
-                    } else {
+                        *o = v;
+                    }
+                } else {
+                    float v[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (c0 + j >= width) break;
-                            out[c0 + j] = __uint_as_float(r[j]) + (a.accumulate ? __ldcg(out + c0 + j) : 0.f);
-                        }
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+                    ce_turn(v, lane);
+                    float* const column = out - (int64_t)lane * a.cols + c0 + lane;
+                    if (c0 + lane < width) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (row - lane + j < a.rows) column[(int64_t)j * a.cols] = v[j] + (a.accumulate ? __ldcg(column + (int64_t)j * a.cols) : 0.f);
                     }
                 }
             }
@@ -405,10 +426,11 @@ struct CePlanes {  // of a matrix
     int64_t ld, rows;
     const float* bias;
     uint16_t* to;
+    bool wide;  // rows begin at multiples of 16 bytes
 };
 struct CePrepare {
     unsigned ends[5];         // CTAs up to the end of each job: planes of Q, of X, the bias, the queries' terms, the targets' sums
-    int m, n, d, pitch, own_rows;
+    int m, n, d, pitch, own_rows, own_shares, own_cols;
     CePlanes planes[2];
     const float* bias;
     float* bias2;
@@ -424,56 +446,78 @@ struct CePrepare {
 // zeros: G has zeros for them, and what they hold may not be finite.
 template <typename T, int PLANES>
 __device__ __forceinline__ void ce_planes_part(const CePrepare& a, const CePlanes& p, unsigned block) {
-    const int64_t i = (int64_t)block * 256 + threadIdx.x, total = p.rows * (a.pitch / 2);
+    const int each = a.pitch / 8;  // eight columns to a thread
+    const int64_t i = (int64_t)block * 256 + threadIdx.x, total = p.rows * each;
     if (i >= total) return;
-    const int64_t row = total >> 32 ? i / (a.pitch / 2) : (int64_t)((uint32_t)i / (uint32_t)(a.pitch / 2));
-    const int col = (int)(i - row * (a.pitch / 2)) * 2;
+    const int64_t row = total >> 32 ? i / each : (int64_t)((uint32_t)i / (uint32_t)each);
+    const int col = (int)(i - row * each) * 8;
     const T* const x = static_cast<const T*>(p.from) + row * p.ld + col;
-    const T zero = (T)0.f;
-    const bool some = !(p.bias && __ldcg(p.bias + row) == -INFINITY);
-    const T v0 = some && col < a.d ? __ldcg(x) : zero, v1 = some && col + 1 < a.d ? __ldcg(x + 1) : zero;
-    uint32_t* const o = reinterpret_cast<uint32_t*>(p.to) + i;
-    if constexpr (PLANES == 1) {
-        uint16_t b[2];
-        memcpy(b, &v0, 2);
-        memcpy(b + 1, &v1, 2);
-        *o = b[0] | (uint32_t)b[1] << 16;
+    const bool some = !(p.bias && p.bias[row] == -INFINITY);
+    alignas(16) T v[8];
+    if (some && p.wide && col + 8 <= a.d) {
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(v)[k] = reinterpret_cast<const uint4*>(x)[k];
     } else {
-        float f0 = v0, f1 = v1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = some && col + k < a.d ? x[k] : (T)0.f;
+    }
+    uint4* const o = reinterpret_cast<uint4*>(p.to) + i;
+    if constexpr (PLANES == 1) {
+        *o = *reinterpret_cast<const uint4*>(v);
+    } else {
 #pragma unroll
         for (int k = 0; k < PLANES; ++k) {
-            const uint32_t w = pack_scores(static_cast<const __nv_bfloat16*>(nullptr), f0, f1);
-            o[k * total] = w;
-            f0 -= __uint_as_float(w << 16);
-            f1 -= __uint_as_float(w & 0xFFFF0000u);
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = pack_scores(static_cast<const __nv_bfloat16*>(nullptr), v[2 * j], v[2 * j + 1]);
+                v[2 * j] -= __uint_as_float(w[j] << 16);
+                v[2 * j + 1] -= __uint_as_float(w[j] & 0xFFFF0000u);
+            }
+            o[k * total] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
 __device__ __forceinline__ void ce_bias_part(const CePrepare& a, unsigned block) {
     const int i = block * 256 + threadIdx.x;
-    if (i < a.n) a.bias2[i] = __ldcg(a.bias + i) * CE_LOG2E;
+    if (i < a.n) a.bias2[i] = a.bias[i] * CE_LOG2E;
     else if (i < ((a.n + 127) & ~127)) a.bias2[i] = 0.f;
 }
 
-// A warp joins a query's blocks.
+// WARPS warps join a query's blocks.
+template <int WARPS>
 __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__ partial, int slots, int m, int n, const int64_t* __restrict__ targets,
                                                       const float* __restrict__ target_scores, const float* __restrict__ bias2, float c, float* __restrict__ losses,
                                                       float* __restrict__ lse, float* __restrict__ lse_low, KernelBefore before) {
     behind_kernel_before(partial, targets, target_scores, bias2, losses, lse, lse_low, before);
-    const int q = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-    if (q >= m) return;
-    const float2* const p = partial + (int64_t)q * slots;
+    __shared__ float s_top[8];
+    __shared__ double s_sum[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = blockIdx.x * (8 / WARPS) + warp / WARPS, first = (warp % WARPS) * 32 + lane;
+    const float2* const p = partial + (int64_t)min(q, m - 1) * slots;
     float top = -INFINITY;
-    for (int i = lane; i < slots; i += 32) top = fmaxf(top, __ldcg(p + i).x);
+#pragma unroll 8
+    for (int i = first; i < slots; i += 32 * WARPS) top = fmaxf(top, __ldcg(p + i).x);
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (WARPS > 1) {
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_top[warp / WARPS * WARPS + w]);
+    }
     const float base = top == -INFINITY ? 0.f : top;
     double sum = 0.;
-    for (int i = lane; i < slots; i += 32) {
+#pragma unroll 8
+    for (int i = first; i < slots; i += 32 * WARPS) {
         const float2 v = __ldcg(p + i);
         sum += (double)v.y * (double)exp2f(v.x - base);
     }
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (lane) return;
+    if (WARPS > 1) {
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        sum = 0.;
+        for (int w = 0; w < WARPS; ++w) sum += s_sum[warp / WARPS * WARPS + w];
+    }
+    if (first || q >= m) return;
     const double ln2 = 0.69314718055994530942, two = (double)base + log2(sum), whole = two * ln2;
     const float high = (float)whole;
     lse[q] = high;
@@ -490,11 +534,11 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
 
 // The target of a query that has a loss to go by, or -1; and what its own entry puts into the gradients.
 __device__ __forceinline__ int ce_target(const CePrepare& a, int q) {
-    const int64_t t = a.targets ? __ldcg(a.targets + q) : -1;
-    return t >= 0 && t < a.n && __ldcg(a.losses + q) < INFINITY ? (int)t : -1;
+    const int64_t t = a.targets ? a.targets[q] : -1;
+    return t >= 0 && t < a.n && a.losses[q] < INFINITY ? (int)t : -1;
 }
 __device__ __forceinline__ float ce_own(const CePrepare& a, int q) {
-    const float loss = __ldcg(a.losses + q), g = a.grad_losses ? __ldcg(a.grad_losses + q) : 0.f, e = a.grad_lse ? __ldcg(a.grad_lse + q) : 0.f;
+    const float loss = a.losses[q], g = a.grad_losses ? a.grad_losses[q] : 0.f, e = a.grad_lse ? a.grad_lse[q] : 0.f;
     return g * expm1f(-loss) + e * expf(-loss);
 }
 __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block) {
@@ -503,11 +547,11 @@ __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block
         if (a.log_terms && q < ((a.m + 127) & ~127)) a.log_terms[q] = -INFINITY, a.marks[q] = 0;
         return;
     }
-    const double two = ((double)__ldcg(a.lse + q) + (double)__ldcg(a.lse_low + q)) * 1.4426950408889634074;
+    const double two = ((double)a.lse[q] + (double)a.lse_low[q]) * 1.4426950408889634074;
     const float high = (float)two;
     const bool none = high == -INFINITY;
     const int t = ce_target(a, q);
-    const float g = t >= 0 && a.grad_losses ? __ldcg(a.grad_losses + q) : 0.f, e = a.grad_lse ? __ldcg(a.grad_lse + q) : 0.f;
+    const float g = t >= 0 && a.grad_losses ? a.grad_losses[q] : 0.f, e = a.grad_lse ? a.grad_lse[q] : 0.f;
     a.terms[q] = none ? -INFINITY : -high;
     const float f = (g + e) * (isfinite(high) ? (float)exp2(-(two - (double)high)) : 1.f);
     a.factors[q] = f;
@@ -520,63 +564,52 @@ __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block
     if (a.amax && isfinite(f)) atomicMax(a.amax, __float_as_uint(fabsf(f)));
 }
 
-// Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes own_rows rows and looks
-// through all targets; they come in ascending order.
-constexpr int CE_OWN_ROWS = 1024, CE_OWN_LIST = 1024, CE_OWN_COLS = 16, CE_OWN_AHEAD = 8;  // rows at most; entries; columns of a lane at a time; targets of a thread
+// Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes own_rows rows, or own_cols columns of
+// them, and looks through all targets; they come in ascending order.
+constexpr int CE_OWN_ROWS = 1024, CE_OWN_LIST = 2560, CE_OWN_COLS = 8, CE_OWN_BATCH = 4, CE_OWN_AHEAD = 5;  // rows at most; entries; columns of a lane and entries at a time; targets of a thread
 template <typename T>
 __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) {
     __shared__ int s_first[CE_OWN_ROWS];
-    __shared__ int s_query[CE_OWN_LIST + 256];
-    __shared__ float s_own[CE_OWN_LIST + 256];
-    __shared__ uint16_t s_row[CE_OWN_LIST + 256];
-    __shared__ int s_count[8];
+    __shared__ int s_query[CE_OWN_LIST];
+    __shared__ float s_own[CE_OWN_LIST];
+    __shared__ uint16_t s_row[CE_OWN_LIST];
+    __shared__ unsigned s_hits[CE_OWN_AHEAD * 8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row0 = (int64_t)block * a.own_rows;
+    const unsigned share = block % (unsigned)a.own_shares;
+    const int64_t row0 = (int64_t)(block / (unsigned)a.own_shares) * a.own_rows;
+    const int first_col = (int)share * a.own_cols, last_col = min(a.d, first_col + a.own_cols);
     const T* const Q = static_cast<const T*>(a.Q);
     for (int r = threadIdx.x; r < a.own_rows; r += 256) s_first[r] = -1;
     int held = 0;  // the same for all threads
-    int64_t of[CE_OWN_AHEAD];
-    for (int64_t i0 = 0; i0 < a.m; i0 += 256) {
-        const int ahead = (int)(i0 / 256 % CE_OWN_AHEAD);
-        if (ahead == 0) {  // targets of the next steps; most CTAs have none of them
-            bool any = false;
+    constexpr int STEP = CE_OWN_AHEAD * 256;
+    for (int64_t i0 = 0; i0 < a.m; i0 += STEP) {
+        int64_t of[CE_OWN_AHEAD];
+        bool any = false;
 #pragma unroll
-            for (int k = 0; k < CE_OWN_AHEAD; ++k) {
-                const int64_t i = i0 + k * 256 + threadIdx.x;
-                const int64_t r = (a.targets && i < a.m ? __ldcg(a.targets + i) : -1) - row0;
-                of[k] = r >= 0 && r < a.own_rows && r + row0 < a.n ? r : -1;
-                any = any || of[k] >= 0;
-            }
-            if (!__syncthreads_or(any) && !held) {
-                i0 += (CE_OWN_AHEAD - 1) * 256;
-                continue;
-            }
+        for (int k = 0; k < CE_OWN_AHEAD; ++k) {
+            const int64_t i = i0 + k * 256 + threadIdx.x, r = (a.targets && i < a.m ? a.targets[i] : -1) - row0;
+            of[k] = r >= 0 && r < a.own_rows && r + row0 < a.n && a.losses[i] < INFINITY ? r : -1;
+            const unsigned hits = __ballot_sync(0xFFFFFFFFu, of[k] >= 0);
+            if (lane == 0) s_hits[k * 8 + warp] = hits;
+            any = any || of[k] >= 0;
         }
-        int64_t r = -1;
+        if (__syncthreads_or(any)) {
 #pragma unroll
-        for (int k = 0; k < CE_OWN_AHEAD; ++k)
-            if (k == ahead) r = of[k];
-        const int i = (int)i0 + threadIdx.x;
-        const bool hit = r >= 0 && __ldcg(a.losses + i) < INFINITY;
-        if (__syncthreads_or(hit)) {
-            const unsigned ballot = __ballot_sync(0xFFFFFFFFu, hit);
-            if (lane == 0) s_count[warp] = __popc(ballot);
-            __syncthreads();
-            int at = held, all = 0;
-            for (int w = 0; w < 8; ++w) {
-                if (w < warp) at += s_count[w];
-                all += s_count[w];
-            }
-            if (hit) {
-                at += __popc(ballot & ((1u << lane) - 1u));
-                s_query[at] = i;
-                s_row[at] = (uint16_t)r;
-                s_own[at] = ce_own(a, i);
-            }
-            held += all;
+            for (int k = 0; k < CE_OWN_AHEAD; ++k)
+                for (int w = 0; w < 8; ++w) {
+                    const unsigned hits = s_hits[k * 8 + w];
+                    if (w == warp && of[k] >= 0) {
+                        const int at = held + __popc(hits & ((1u << lane) - 1u));
+                        s_query[at] = (int)i0 + k * 256 + threadIdx.x;
+                        s_row[at] = (uint16_t)of[k];
+                    }
+                    held += __popc(hits);
+                }
             __syncthreads();
         }
-        if (held && (held >= CE_OWN_LIST || i0 + 256 >= a.m)) {
+        if (held && (held + STEP > CE_OWN_LIST || i0 + STEP >= a.m)) {
+            for (int e = threadIdx.x; e < held; e += 256) s_own[e] = ce_own(a, s_query[e]);
+            __syncthreads();
             for (int e = warp; e < held; e += 8) {  // a warp takes an entry, if it is the first of its row, with those that follow
                 const int rr = s_row[e];
                 bool first = true;
@@ -584,21 +617,33 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
                 if (!first) continue;
                 const bool fresh = s_first[rr] < 0;
                 const int slot = fresh ? s_query[e] : s_first[rr];
-                for (int c0 = 0; c0 < a.d; c0 += 32 * CE_OWN_COLS) {
-                    float acc[CE_OWN_COLS];
+                for (int c0 = first_col; c0 < last_col; c0 += 32 * CE_OWN_COLS) {
+                    float acc[CE_OWN_COLS] = {};
+                    int e0 = e & ~31;
+                    unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
+                    while (e0 < held) {
+                        float f[CE_OWN_BATCH];
+                        const T* from[CE_OWN_BATCH];
 #pragma unroll
-                    for (int k = 0; k < CE_OWN_COLS; ++k) acc[k] = 0.f;
-                    for (int e0 = e & ~31; e0 < held; e0 += 32) {
-                        unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
-                        while (b) {
-                            const int at = e0 + __ffs(b) - 1, query = s_query[at];
+                        for (int h = 0; h < CE_OWN_BATCH; ++h) {  // the next entries of the row, whose loads are in flight together
+                            while (!b && e0 < held) {
+                                e0 += 32;
+                                b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
+                            }
+                            const int at = b ? e0 + __ffs(b) - 1 : -1;
                             b &= b - 1u;
-                            const float f = s_own[at];
-                            const T* const from = Q + (int64_t)query * a.ldq + c0 + lane;
-#pragma unroll
-                            for (int k = 0; k < CE_OWN_COLS; ++k)
-                                if (c0 + k * 32 + lane < a.d) acc[k] = fmaf(f, ce_float(__ldcg(from + k * 32)), acc[k]);
+                            f[h] = at < 0 ? 0.f : s_own[at];
+                            from[h] = at < 0 ? nullptr : Q + (int64_t)s_query[at] * a.ldq + c0 + lane;
                         }
+                        float v[CE_OWN_BATCH][CE_OWN_COLS];
+#pragma unroll
+                        for (int h = 0; h < CE_OWN_BATCH; ++h)
+#pragma unroll
+                            for (int k = 0; k < CE_OWN_COLS; ++k) v[h][k] = from[h] && c0 + k * 32 + lane < a.d ? ce_float(from[h][k * 32]) : 0.f;
+#pragma unroll
+                        for (int h = 0; h < CE_OWN_BATCH; ++h)
+#pragma unroll
+                            for (int k = 0; k < CE_OWN_COLS; ++k) acc[k] = from[h] ? fmaf(f[h], v[h][k], acc[k]) : acc[k];
                     }
 #pragma unroll
                     for (int k = 0; k < CE_OWN_COLS; ++k) {
@@ -618,12 +663,12 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x; r < a.own_rows && row0 + r < a.n; r += 256) a.where[row0 + r] = s_first[r];
+    if (share == 0)
+        for (int r = threadIdx.x; r < a.own_rows && row0 + r < a.n; r += 256) a.where[row0 + r] = s_first[r];
 }
 
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) ce_prepare_kernel(CePrepare a, KernelBefore before) {
-    behind_kernel_before(before);
+__global__ void __launch_bounds__(256) ce_prepare_kernel(CePrepare a) {
     const unsigned b = blockIdx.x;
     if (b < a.ends[0]) ce_planes_part<T, PLANES>(a, a.planes[0], b);
     else if (b < a.ends[1]) ce_planes_part<T, PLANES>(a, a.planes[1], b - a.ends[0]);
@@ -752,7 +797,7 @@ struct CePlan {
     int splits_q = 0, per_q = 0, splits_x = 0, per_x = 0;
     float *acc_q = nullptr, *parts_x = nullptr;
     bool fused_q = false, fused_x = false;
-    int fused_block = 0;  // tiles of rows in a unit of dQ
+    int fused_block = 0, fused_block_x = 0;  // tiles of the other side in a unit of dQ, of dX
 
     CePlan(const CeCall& k, bool backward, bool need_q, bool need_x, void* base) : space{static_cast<char*>(base)} {
         const int sms = k.c->sm_count;
@@ -778,16 +823,29 @@ struct CePlan {
             sums = space.take<float>((size_t)k.m * k.d);
             where = space.take<int>(k.n);
         }
-        if (fused_q) {
-            const int nb = k.d > 128 ? 64 : 128;
-            const size_t tiles = ceil_div(k.n, nb), least = ceil_div(tiles, 32768 / nb), most = std::min(tiles, least + ceil_div((size_t)4 * sms, tiles_q));
+        // a unit's tiles of the other side: the last wave full, and four tiles' time for the units' ends; at most 32,768 entries in a sum
+        const int nb = k.d > 128 ? 64 : 128;
+        auto block_of = [&](size_t own, size_t tiles, size_t most) {
             size_t best = ~(size_t)0;
-            for (size_t blocks = least; blocks <= most; ++blocks) {  // the last wave full, and four tiles' time for the units' ends
-                const size_t per = ceil_div(tiles, blocks), time = ceil_div(tiles_q * ceil_div(tiles, per), sms) * (per + 4);
-                if (time < best) best = time, fused_block = (int)per;
+            int block = 1;
+            const size_t least = ceil_div(tiles, 32768 / nb);
+            for (size_t blocks = least; blocks <= std::min(tiles, least + most); ++blocks) {
+                const size_t per = ceil_div(tiles, blocks), time = ceil_div(own * ceil_div(tiles, per), sms) * (per + 4);
+                if (time < best) best = time, block = (int)per;
             }
+            return block;
+        };
+        if (fused_q) {
+            const size_t tiles = ceil_div(k.n, nb);
+            fused_block = block_of(tiles_q, tiles, ceil_div((size_t)4 * sms, tiles_q));
             splits_q = (int)ceil_div(tiles, fused_block);
             acc_q = space.take<float>((size_t)splits_q * k.m * k.d);
+        }
+        if (fused_x) {  // sums of few rows are split too
+            const size_t own = ceil_div(k.n, TG_M), tiles = ceil_div(k.m, nb);
+            fused_block_x = own >= (size_t)sms ? (int)tiles : block_of(own, tiles, sms / own);
+            splits_x = (int)ceil_div(tiles, fused_block_x);
+            if (splits_x > 1) parts_x = space.take<float>((size_t)splits_x * k.n * k.d);
         }
         if ((!need_q || fused_q) && (!need_x || fused_x)) return;
         const bool pieces_x = need_x && !fused_x;
@@ -843,22 +901,27 @@ struct CeOperands {
             a.ends[i] = (unsigned)end;
         };
         auto planes = [&](const void* from, int64_t ld, int rows, const float* bias, uint16_t* to) {
-            a.planes[to == p.x_planes] = CePlanes{from, ld, rows, bias, to};
-            return to ? ceil_div((size_t)rows * k.pitch() / 2, 256) : 0;
+            a.planes[to == p.x_planes] = CePlanes{from, ld, rows, bias, to, aligned16(from, ld * (k.type == CULSH_F32 ? 4 : 2))};
+            return ceil_div((size_t)rows * k.pitch() / 8, 256);
         };
         job(0, p.q_planes ? planes(k.Q, k.ldq, k.m, nullptr, p.q_planes) : 0);
         job(1, p.x_planes ? planes(k.X, k.ldx, k.n, k.bias, p.x_planes) : 0);
         job(2, p.bias2 ? ceil_div((size_t)k.n + 127, 256) : 0);
         job(3, p.terms ? ceil_div((size_t)k.m + 127, 256) : 0);
         a.terms = p.terms, a.log_terms = p.log_terms, a.factors = p.factors, a.own = p.own, a.sums = p.sums, a.marks = p.marks, a.cols = p.cols, a.where = p.where, a.amax = p.amax;
-        a.own_rows = (int)std::min<size_t>(CE_OWN_ROWS, ceil_div(ceil_div(k.n, 2 * (size_t)k.c->sm_count), 128) * 128);
-        job(4, p.where ? ceil_div(k.n, a.own_rows) : 0);
+        // rows, and where they are few and long columns, in shares for two CTAs an SM
+        const size_t ctas = 2 * (size_t)k.c->sm_count;
+        a.own_rows = (int)std::min<size_t>(CE_OWN_ROWS, ceil_div(ceil_div(k.n, ctas), 8) * 8);
+        const size_t tiles = ceil_div(k.n, a.own_rows), shares = std::min(ceil_div(k.d, 32 * CE_OWN_COLS), std::max<size_t>(1, 4 * ctas / tiles));
+        a.own_cols = (int)(ceil_div(ceil_div(k.d, shares), 32 * CE_OWN_COLS) * 32 * CE_OWN_COLS);
+        a.own_shares = (int)ceil_div(k.d, a.own_cols);
+        job(4, p.where ? tiles * a.own_shares : 0);
         if (p.q_planes) q = p.q_planes, ldq = k.pitch();
         if (p.x_planes) x = p.x_planes, ldx = k.pitch();
         if (!end) return;
-        if (k.type == CULSH_F32) launch_next(k.stream, ce_prepare_kernel<float, 3>, (size_t)end, 256u, 0, a);
-        else if (k.type == CULSH_F16) launch_next(k.stream, ce_prepare_kernel<__half, 1>, (size_t)end, 256u, 0, a);
-        else launch_next(k.stream, ce_prepare_kernel<__nv_bfloat16, 1>, (size_t)end, 256u, 0, a);
+        if (k.type == CULSH_F32) ce_prepare_kernel<float, 3><<<(unsigned)end, 256, 0, k.stream>>>(a);
+        else if (k.type == CULSH_F16) ce_prepare_kernel<__half, 1><<<(unsigned)end, 256, 0, k.stream>>>(a);
+        else ce_prepare_kernel<__nv_bfloat16, 1><<<(unsigned)end, 256, 0, k.stream>>>(a);
         KERNEL_CHECK();
     }
     CUtensorMap map_q(const CeCall& k, int box) const { return tg_map(q, k.tg(), k.m, k.d, ldq, k.planes(), (int64_t)k.m * ldq * 2, box); }
@@ -905,7 +968,8 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     ce_by([&](auto planes, auto bias, auto segs, auto pairs) {
         tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value, decltype(pairs)::value>>(k.c, tq, tx, a, k.stream);
     }, k.planes() == 3, k.bias != nullptr, segments, CePlan::pairs(k.m));
-    launch_next(k.stream, ce_join_kernel, ce_grid((size_t)k.m * 32), 256u, 0, (const float2*)p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
+    auto join = p.slots > 256 ? ce_join_kernel<8> : ce_join_kernel<1>;
+    launch_next(k.stream, join, ceil_div(k.m, p.slots > 256 ? 1 : 8), 256u, 0, (const float2*)p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
     KERNEL_CHECK();
 }
 
@@ -967,12 +1031,12 @@ inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, vo
     a.idesc_s = tg_idesc(k.tg(), false, false) | M | ((uint32_t)(nb >> 3) << 17);
     a.idesc_o = tg_idesc(k.tg(), false, true) | M | ((uint32_t)(kb * 64 >> 3) << 17);
     a.own = ROWS ? k.n : k.m, a.other = ROWS ? k.m : k.n;
-    a.tiles_own = (int)ceil_div(a.own, TG_M), a.tiles_other = (int)ceil_div(a.other, nb), a.block = ROWS ? a.tiles_other : p.fused_block;
+    a.tiles_own = (int)ceil_div(a.own, TG_M), a.tiles_other = (int)ceil_div(a.other, nb), a.block = ROWS ? p.fused_block_x : p.fused_block;
     const size_t units = ceil_div(a.tiles_other, a.block) * a.tiles_own;
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
     a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = ROWS ? p.log_terms : p.terms, a.marks = p.marks, a.amax = p.amax, a.target_cols = p.cols;
-    a.parts = p.acc_q, a.out = out, a.ld = ld, a.where = p.where, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
+    a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
     const CUtensorMap own = ROWS ? ops.map_x(k, TG_M) : ops.map_q(k, TG_M), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
     auto go = [&](auto boxes) {
         constexpr int KB = decltype(boxes)::value;
@@ -996,7 +1060,10 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
     const CeOperands ops(k, p, before);
     CeFinish last{};  // of dX, for the launch that finishes dQ
     if constexpr (PLANES == 1) {
-        if (p.fused_x) ce_fused<true, HALF>(k, p, ops, grad_X, ld_gx);
+        if (p.fused_x) {
+            ce_fused<true, HALF>(k, p, ops, grad_X, ld_gx);
+            if (p.splits_x > 1) last = ce_finish_of(k, p.parts_x, p.splits_x, k.n, nullptr, p.where, grad_X, ld_gx);
+        }
         if (p.fused_q) ce_fused<false, HALF>(k, p, ops, nullptr, 0);
     }
     const bool pieces_q = grad_Q && !p.fused_q, pieces_x = grad_X && !p.fused_x;
