@@ -46,6 +46,18 @@ __device__ __forceinline__ void ce_turn(float (&v)[32], int lane) {
                 else v[j | s] = got;
             }
 }
+// Adds the sums of a row's targets, d columns each, over the temperature: 32 columns from `col` on.
+__device__ __forceinline__ void ce_add_own(float (&v)[32], const int* where, int64_t stride, int splits, const float* sums, int d, int col, float inv_t) {
+    for (int s = 0; s < splits; ++s) {
+        const int slot = __ldcg(where + s * stride);
+        if (slot < 0) continue;
+        const float* const extra = sums + (int64_t)slot * d + col;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (col + j < d) v[j] = fmaf(__ldcg(extra + j), inv_t, v[j]);
+    }
+}
+
 struct CeFusedArgs {
     int* d_error;
     unsigned units;
@@ -63,6 +75,7 @@ struct CeFusedArgs {
     void* out;                // dX
     int64_t ld;
     const int* where;
+    int own_splits;
     const float* sums;
     float inv_t;
 };
@@ -260,14 +273,13 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             const int first_own = unit.own0 + quarter * 32, mine = first_own + lane;
             const bool in = mine < a.own;
             float my_term = (float)exponent;
-            int my_target = -1, slot = -1;
+            int my_target = -1;
             if (in) {
                 if (!ROWS) {
                     my_term += __ldcg(a.terms + mine);
                     my_target = __ldcg(a.target_cols + mine);
-                } else {
-                    slot = __ldcg(a.where + mine);
-                    if (BIAS) my_term += __ldcg(a.bias + mine);
+                } else if (BIAS) {
+                    my_term += __ldcg(a.bias + mine);
                 }
             }
             const uint64_t term2 = f2_pack(my_term, my_term);
@@ -382,12 +394,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                     const float scale = HALF ? ldexpf(a.inv_t, -exponent) : a.inv_t;
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] *= scale;
-                    if (slot >= 0) {
-                        const float* const extra = a.sums + (int64_t)slot * a.d + c0;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c0 + j < a.d) v[j] = fmaf(__ldcg(extra + j), a.inv_t, v[j]);
-                    }
+                    ce_add_own(v, a.where + mine, a.own, in ? a.own_splits : 0, a.sums, a.d, c0, a.inv_t);
                 }
                 T* const o = reinterpret_cast<T*>(a.out) + (int64_t)mine * a.ld + c0;
                 float* const part = a.parts + ((int64_t)unit.block * a.own + mine) * a.d + c0;

@@ -272,6 +272,8 @@ struct CeProductArgs {
     int64_t ld;
     const uint32_t* amax;
     const int* where;
+    int own_splits;
+    int64_t where_stride;
     const float* sums;
     float inv_t;
 };
@@ -287,19 +289,18 @@ struct CeProductUnit {
         k0 = split * a.kper, k1 = min(a.kb, k0 + a.kper);
     }
 };
-// N columns of a row of dX from column col0 on.
-template <typename T>
-__device__ __noinline__ void ce_store_turned(const CeProductArgs& a, int row, int lane, int col, float scale, const float* extra, uint32_t taddr, bool live) {
+// 32 columns of a row of dX from `col` on, times `scale`, with the targets' part.
+__device__ __forceinline__ void ce_with_own(const CeProductArgs& a, int row, int col, float scale, uint32_t taddr, bool live, float (&v)[32]) {
     uint32_t r[32];
     tg_read(taddr, live, r);
-    float v[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
-    if (extra) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (col + j < a.cols) v[j] = fmaf(__ldcg(extra + j), a.inv_t, v[j]);
-    }
+    ce_add_own(v, a.where + row, a.where_stride, row < a.rows ? a.own_splits : 0, a.sums, a.cols, col, a.inv_t);
+}
+template <typename T>
+__device__ __noinline__ void ce_store_turned(const CeProductArgs& a, int row, int lane, int col, float scale, uint32_t taddr, bool live) {
+    float v[32];
+    ce_with_own(a, row, col, scale, taddr, live, v);
     ce_turn(v, lane);
     T* const to = reinterpret_cast<T*>(a.typed) + (int64_t)(row - lane) * a.ld + col + lane;
     if (col + lane < a.cols) {
@@ -308,40 +309,35 @@ __device__ __noinline__ void ce_store_turned(const CeProductArgs& a, int row, in
             if (row - lane + j < a.rows) store_score(to + j * a.ld, v[j]);
     }
 }
+// N columns of a row of dX from column col0 on.
 template <typename T, int N>
 __device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, int lane, int col0, uint32_t taddr, bool live) {
-    const bool in = row < a.rows;
-    const int slot = in ? __ldcg(a.where + row) : -1;
+    constexpr int V = 16 / sizeof(T);
     const float scale = ldexpf(a.inv_t, std::is_same<T, __half>::value ? -ce_scale_exponent(a.amax) : 0);
-    const float* const extra = a.sums + (int64_t)max(slot, 0) * a.cols + col0;
-    if ((a.cols & 7) != 0 || (a.ld & 7) != 0 || ((uintptr_t)a.typed & 15) != 0) {  // no 16 bytes of a row lie together: rows turned, so that neighbouring lanes have neighbouring columns
-        for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) ce_store_turned<T>(a, row, lane, col0 + c0, scale, slot >= 0 ? extra + c0 : nullptr, taddr + c0, live);
+    if (a.cols % V != 0 || a.ld % V != 0 || ((uintptr_t)a.typed & 15) != 0) {  // no 16 bytes of a row lie together: rows turned, so that neighbouring lanes have neighbouring columns
+        for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) ce_store_turned<T>(a, row, lane, col0 + c0, scale, taddr + c0, live);
         return;
     }
     T* const o = reinterpret_cast<T*>(a.typed) + (int64_t)row * a.ld + col0;
 #pragma unroll 1
     for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) {
-        uint32_t r[32];
-        tg_read(taddr + c0, live, r);
-        if (!in) continue;
         float v[32];
+        ce_with_own(a, row, col0 + c0, scale, taddr + c0, live, v);
+        if (row >= a.rows) continue;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * scale;
-        if (slot >= 0) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (col0 + c0 + j < a.cols) v[j] = fmaf(__ldcg(extra + c0 + j), a.inv_t, v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
+        for (int j = 0; j < 32; j += V) {
             if (col0 + c0 + j >= a.cols) break;
-            const T* const t = nullptr;
-            *reinterpret_cast<uint4*>(o + c0 + j) =
-                make_uint4(pack_scores(t, v[j], v[j + 1]), pack_scores(t, v[j + 2], v[j + 3]), pack_scores(t, v[j + 4], v[j + 5]), pack_scores(t, v[j + 6], v[j + 7]));
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4*>(o + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            } else {
+                const T* const t = nullptr;
+                *reinterpret_cast<uint4*>(o + c0 + j) =
+                    make_uint4(pack_scores(t, v[j], v[j + 1]), pack_scores(t, v[j + 2], v[j + 3]), pack_scores(t, v[j + 4], v[j + 5]), pack_scores(t, v[j + 6], v[j + 7]));
+            }
         }
     }
 }
-// TYPED: 0: sums in 32 bits; 1, 2: bfloat16, float16.
+// TYPED: 0: sums in 32 bits; 1, 2, 3: results in bfloat16, float16, float32.
 template <int PLANES, bool AMN, int N, bool PAIRS, int TYPED>
 struct CeProductPolicy {
     static constexpr bool A_MN = AMN, B_MN = true, I8 = false, PARTS = true, PAIR = PAIRS;
@@ -378,7 +374,7 @@ struct CeProductPolicy {
                 return;
             }
             if constexpr (TYPED != 0) {
-                ce_store_typed<std::conditional_t<TYPED == 2, __half, __nv_bfloat16>, BN / 2>(a, row, lane, u.nt * BN + group * (BN / 2), taddr, live);
+                ce_store_typed<std::conditional_t<TYPED == 3, float, std::conditional_t<TYPED == 2, __half, __nv_bfloat16>>, BN / 2>(a, row, lane, u.nt * BN + group * (BN / 2), taddr, live);
                 done();
                 return;
             }
@@ -420,6 +416,82 @@ struct CeProductPolicy {
     };
 };
 
+// Losses of up to 16 queries in 32 bits, which would leave the tensor cores' lanes empty and cost the planes' reads and writes: bound by reading the rows once.  A thread has a row, 32 columns of
+// 256 rows at a time come through shared memory; the queries' values are read from there by all lanes at once.  Maxima and sums are a thread's until the end.
+constexpr int CE_FEW = 16, CE_FEW_COLS = 32, CE_FEW_THREADS = 256;
+template <int M, bool BIAS>
+__global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* __restrict__ Q, int64_t ldq, const float* __restrict__ X, int64_t ldx, int m, int n, int d,
+                                                                const float* __restrict__ bias, float c, const int64_t* __restrict__ targets, float2* __restrict__ partial,
+                                                                float* __restrict__ target_scores, KernelBefore before) {
+    behind_kernel_before(Q, X, bias, targets, partial, target_scores, before);
+    __shared__ float s_x[CE_FEW_COLS][CE_FEW_THREADS + 1];
+    __shared__ alignas(16) float s_q[CE_FEW_COLS][M < 4 ? 4 : M];
+    __shared__ float2 s_part[CE_FEW_THREADS / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float ref[M], sum[M];
+    int target[M];
+#pragma unroll
+    for (int q = 0; q < M; ++q) {
+        const int64_t t = q < m && targets ? __ldcg(targets + q) : -1;
+        target[q] = t < 0 || t >= n ? -1 : (int)t;
+        ref[q] = -INFINITY, sum[q] = 0.f;
+    }
+    for (int64_t row0 = (int64_t)blockIdx.x * CE_FEW_THREADS; row0 < n; row0 += (int64_t)gridDim.x * CE_FEW_THREADS) {
+        float acc[M] = {};
+        for (int c0 = 0; c0 < d; c0 += CE_FEW_COLS) {
+            float v[CE_FEW_COLS];  // a warp's 32 rows, a column to a lane
+#pragma unroll
+            for (int j = 0; j < CE_FEW_COLS; ++j) {
+                const int64_t row = row0 + warp * 32 + j;
+                v[j] = row < n && c0 + lane < d ? __ldcg(X + row * ldx + c0 + lane) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < CE_FEW_COLS; ++j) s_x[lane][warp * 32 + j] = v[j];
+            for (int i = threadIdx.x; i < CE_FEW_COLS * M; i += CE_FEW_THREADS) {
+                const int q = i / CE_FEW_COLS, k = i % CE_FEW_COLS;
+                s_q[k][q] = q < m && c0 + k < d ? __ldcg(Q + q * ldq + c0 + k) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll 8
+            for (int k = 0; k < min(CE_FEW_COLS, d - c0); ++k) {
+                const float x = s_x[k][threadIdx.x];
+#pragma unroll
+                for (int q = 0; q < M; ++q) acc[q] = fmaf(s_q[k][q], x, acc[q]);
+            }
+        }
+        const int64_t row = row0 + threadIdx.x;
+        if (row < n) {
+            const float b = BIAS ? __ldcg(bias + row) * CE_LOG2E : 0.f;
+#pragma unroll
+            for (int q = 0; q < M; ++q) {
+                if (target[q] == row) target_scores[q] = acc[q];
+                const float z = BIAS && b == -INFINITY ? b : fmaf(acc[q], c, b), next = fmaxf(ref[q], z), base = next == -INFINITY ? 0.f : next;
+                sum[q] = fmaf(sum[q], ce_exp2(ref[q] - base), ce_exp2(BIAS ? z - base : fmaf(acc[q], c, -base)));
+                ref[q] = next;
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < M; ++q) {
+        if (q >= m) break;
+        float top = ref[q];
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        float all = sum[q] * ce_exp2(ref[q] - (top == -INFINITY ? 0.f : top));
+        for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+        __syncthreads();
+        if (lane == 0) s_part[warp] = make_float2(top, all);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < CE_FEW_THREADS / 32; ++w) top = fmaxf(top, s_part[w].x);
+            const float base = top == -INFINITY ? 0.f : top;
+            all = 0.f;
+            for (int w = 0; w < CE_FEW_THREADS / 32; ++w) all = fmaf(s_part[w].y, ce_exp2(s_part[w].x - base), all);
+            partial[(int64_t)q * gridDim.x + blockIdx.x] = make_float2(top, all);
+        }
+    }
+}
+
 // ---- what the products need beforehand: one launch, whose CTAs have a share of one of five jobs each --------------------------------------------------------------------
 struct CePlanes {  // of a matrix
     const void* from;
@@ -430,7 +502,7 @@ struct CePlanes {  // of a matrix
 };
 struct CePrepare {
     unsigned ends[5];         // CTAs up to the end of each job: planes of Q, of X, the bias, the queries' terms, the targets' sums
-    int m, n, d, pitch, own_rows, own_shares, own_cols;
+    int m, n, d, pitch, own_rows, own_tiles, own_shares, own_cols, own_queries;
     CePlanes planes[2];
     const float* bias;
     float* bias2;
@@ -525,7 +597,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
     float loss = 0.f;
     const int64_t t = targets ? __ldcg(targets + q) : -1;
     if (t >= 0 && t < n) {
-        const double z = (double)__ldcg(target_scores + q) * (double)c + (bias2 ? (double)__ldcg(bias2 + t) : 0.);
+        const double b = bias2 ? (double)__ldcg(bias2 + t) : 0., z = b == -INFINITY ? b : (double)__ldcg(target_scores + q) * (double)c + b;
         loss = z == -INFINITY && two == two ? INFINITY : (float)((two - z) * ln2);
         if (loss < 0.f) loss = 0.f;
     }
@@ -564,9 +636,9 @@ __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block
     if (a.amax && isfinite(f)) atomicMax(a.amax, __float_as_uint(fabsf(f)));
 }
 
-// Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none).  A CTA takes own_rows rows, or own_cols columns of
+// Sums over the queries whose target is a row, own[i] q_i: sums[first query of the row][d], and which one that is for each row (-1: none); of few rows for each of own_queries queries.  A CTA takes own_rows rows, or own_cols columns of
 // them, and looks through all targets; they come in ascending order.
-constexpr int CE_OWN_ROWS = 1024, CE_OWN_LIST = 2560, CE_OWN_COLS = 8, CE_OWN_BATCH = 4, CE_OWN_AHEAD = 5;  // rows at most; entries; columns of a lane and entries at a time; targets of a thread
+constexpr int CE_OWN_ROWS = 1024, CE_OWN_LIST = 2560, CE_OWN_COLS = 8, CE_OWN_AHEAD = 5;  // rows at most; entries; columns of a lane at a time; targets of a thread
 template <typename T>
 __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) {
     __shared__ int s_first[CE_OWN_ROWS];
@@ -575,19 +647,19 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
     __shared__ uint16_t s_row[CE_OWN_LIST];
     __shared__ unsigned s_hits[CE_OWN_AHEAD * 8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned share = block % (unsigned)a.own_shares;
-    const int64_t row0 = (int64_t)(block / (unsigned)a.own_shares) * a.own_rows;
+    const unsigned share = block % (unsigned)a.own_shares, tile = block / (unsigned)a.own_shares % (unsigned)a.own_tiles, split = block / (unsigned)a.own_shares / (unsigned)a.own_tiles;
+    const int64_t row0 = (int64_t)tile * a.own_rows, q0 = (int64_t)split * a.own_queries, q1 = min((int64_t)a.m, q0 + a.own_queries);
     const int first_col = (int)share * a.own_cols, last_col = min(a.d, first_col + a.own_cols);
     const T* const Q = static_cast<const T*>(a.Q);
     for (int r = threadIdx.x; r < a.own_rows; r += 256) s_first[r] = -1;
     int held = 0;  // the same for all threads
     constexpr int STEP = CE_OWN_AHEAD * 256;
-    for (int64_t i0 = 0; i0 < a.m; i0 += STEP) {
+    for (int64_t i0 = q0; i0 < q1; i0 += STEP) {
         int64_t of[CE_OWN_AHEAD];
         bool any = false;
 #pragma unroll
         for (int k = 0; k < CE_OWN_AHEAD; ++k) {
-            const int64_t i = i0 + k * 256 + threadIdx.x, r = (a.targets && i < a.m ? a.targets[i] : -1) - row0;
+            const int64_t i = i0 + k * 256 + threadIdx.x, r = (a.targets && i < q1 ? a.targets[i] : -1) - row0;
             of[k] = r >= 0 && r < a.own_rows && r + row0 < a.n && a.losses[i] < INFINITY ? r : -1;
             const unsigned hits = __ballot_sync(0xFFFFFFFFu, of[k] >= 0);
             if (lane == 0) s_hits[k * 8 + warp] = hits;
@@ -607,7 +679,7 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
                 }
             __syncthreads();
         }
-        if (held && (held + STEP > CE_OWN_LIST || i0 + STEP >= a.m)) {
+        if (held && (held + STEP > CE_OWN_LIST || i0 + STEP >= q1)) {
             for (int e = threadIdx.x; e < held; e += 256) s_own[e] = ce_own(a, s_query[e]);
             __syncthreads();
             for (int e = warp; e < held; e += 8) {  // a warp takes an entry, if it is the first of its row, with those that follow
@@ -617,43 +689,47 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
                 if (!first) continue;
                 const bool fresh = s_first[rr] < 0;
                 const int slot = fresh ? s_query[e] : s_first[rr];
-                for (int c0 = first_col; c0 < last_col; c0 += 32 * CE_OWN_COLS) {
-                    float acc[CE_OWN_COLS] = {};
-                    int e0 = e & ~31;
-                    unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
-                    while (e0 < held) {
-                        float f[CE_OWN_BATCH];
-                        const T* from[CE_OWN_BATCH];
+                auto columns = [&](auto of_lane) {
+                    constexpr int COLS = decltype(of_lane)::value, BATCH = 32 / COLS;  // 32 loads in flight
+                    for (int c0 = first_col; c0 < last_col; c0 += 32 * COLS) {
+                        float acc[COLS] = {};
+                        int e0 = e & ~31;
+                        unsigned b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
+                        while (e0 < held) {
+                            float f[BATCH], v[BATCH][COLS];
+                            unsigned real = 0;
 #pragma unroll
-                        for (int h = 0; h < CE_OWN_BATCH; ++h) {  // the next entries of the row, whose loads are in flight together
-                            while (!b && e0 < held) {
-                                e0 += 32;
-                                b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
+                            for (int h = 0; h < BATCH; ++h) {  // the next entries of the row
+                                while (!b && e0 < held) {
+                                    e0 += 32;
+                                    b = __ballot_sync(0xFFFFFFFFu, e0 + lane < held && s_row[e0 + lane] == rr);
+                                }
+                                const int at = b ? e0 + __ffs(b) - 1 : 0;
+                                real |= (b != 0u) << h;
+                                const T* const from = Q + (int64_t)s_query[at] * a.ldq + c0 + lane;
+                                f[h] = s_own[at];
+#pragma unroll
+                                for (int k = 0; k < COLS; ++k) v[h][k] = b && c0 + k * 32 + lane < a.d ? ce_float(from[k * 32]) : 0.f;
+                                b &= b - 1u;
                             }
-                            const int at = b ? e0 + __ffs(b) - 1 : -1;
-                            b &= b - 1u;
-                            f[h] = at < 0 ? 0.f : s_own[at];
-                            from[h] = at < 0 ? nullptr : Q + (int64_t)s_query[at] * a.ldq + c0 + lane;
+#pragma unroll
+                            for (int h = 0; h < BATCH; ++h)
+#pragma unroll
+                                for (int k = 0; k < COLS; ++k)
+                                    if (real >> h & 1u) acc[k] = fmaf(f[h], v[h][k], acc[k]);
                         }
-                        float v[CE_OWN_BATCH][CE_OWN_COLS];
 #pragma unroll
-                        for (int h = 0; h < CE_OWN_BATCH; ++h)
-#pragma unroll
-                            for (int k = 0; k < CE_OWN_COLS; ++k) v[h][k] = from[h] && c0 + k * 32 + lane < a.d ? ce_float(from[h][k * 32]) : 0.f;
-#pragma unroll
-                        for (int h = 0; h < CE_OWN_BATCH; ++h)
-#pragma unroll
-                            for (int k = 0; k < CE_OWN_COLS; ++k) acc[k] = from[h] ? fmaf(f[h], v[h][k], acc[k]) : acc[k];
-                    }
-#pragma unroll
-                    for (int k = 0; k < CE_OWN_COLS; ++k) {
-                        const int col = c0 + k * 32 + lane;
-                        if (col < a.d) {
-                            float* const s = a.sums + (int64_t)slot * a.d + col;
-                            *s = fresh ? acc[k] : *s + acc[k];
+                        for (int k = 0; k < COLS; ++k) {
+                            const int col = c0 + k * 32 + lane;
+                            if (col < a.d) {
+                                float* const s = a.sums + (int64_t)slot * a.d + col;
+                                *s = fresh ? acc[k] : *s + acc[k];
+                            }
                         }
                     }
-                }
+                };
+                if (last_col - first_col > 64) columns(std::integral_constant<int, CE_OWN_COLS>());
+                else columns(std::integral_constant<int, 2>());
                 __syncwarp();
                 if (lane == 0 && fresh) s_first[rr] = slot;
                 __syncwarp();
@@ -664,11 +740,11 @@ __device__ __forceinline__ void ce_own_part(const CePrepare& a, unsigned block) 
     }
     __syncthreads();
     if (share == 0)
-        for (int r = threadIdx.x; r < a.own_rows && row0 + r < a.n; r += 256) a.where[row0 + r] = s_first[r];
+        for (int r = threadIdx.x; r < a.own_rows && row0 + r < a.n; r += 256) a.where[(int64_t)split * a.n + row0 + r] = s_first[r];
 }
 
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) ce_prepare_kernel(CePrepare a) {
+__global__ void __launch_bounds__(256, 4) ce_prepare_kernel(CePrepare a) {
     const unsigned b = blockIdx.x;
     if (b < a.ends[0]) ce_planes_part<T, PLANES>(a, a.planes[0], b);
     else if (b < a.ends[1]) ce_planes_part<T, PLANES>(a, a.planes[1], b - a.ends[0]);
@@ -692,7 +768,8 @@ struct CeFinish {
 };
 struct CeFinishArgs {
     CeFinish rows, queries;
-    int d;
+    int d, own_splits;
+    int64_t where_stride;
     const uint32_t* amax;
     const float *own, *sums;
     const void* X;
@@ -718,7 +795,7 @@ __device__ __forceinline__ void ce_finish_part(const CeFinishArgs& a, const CeFi
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] += w[k];
     }
-    const int w = __ldcg(f.which + row);
+    int w = __ldcg(f.which + row);
     float scale = 1.f;
     if (f.factors) scale = std::is_same<T, __half>::value ? ldexpf(__ldcg(f.factors + row), -14) : __ldcg(f.factors + row);
     else if (a.amax) scale = ldexpf(1.f, -ce_scale_exponent(a.amax));
@@ -726,11 +803,16 @@ __device__ __forceinline__ void ce_finish_part(const CeFinishArgs& a, const CeFi
     struct alignas(V * sizeof(T)) Some { T v[V]; };
     Some o;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        float x = v[k] * scale;
-        if (w >= 0) x += QUERIES ? mine * ce_float(__ldcg(static_cast<const T*>(a.X) + (int64_t)w * a.ldx + col + k)) : __ldcg(a.sums + (int64_t)w * a.d + col + k);
-        o.v[k] = (T)(x * a.inv_t);
+    for (int k = 0; k < V; ++k) v[k] *= scale;
+    for (int s = 0; s < (QUERIES ? 1 : a.own_splits); ++s) {
+        if (s) w = __ldcg(f.which + s * a.where_stride + row);
+        if (w < 0) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            v[k] += QUERIES ? mine * ce_float(__ldcg(static_cast<const T*>(a.X) + (int64_t)w * a.ldx + col + k)) : __ldcg(a.sums + (int64_t)w * a.d + col + k);
     }
+#pragma unroll
+    for (int k = 0; k < V; ++k) o.v[k] = (T)(v[k] * a.inv_t);
     *reinterpret_cast<Some*>(static_cast<T*>(f.out) + row * f.ldo + col) = o;
 }
 template <typename T>
@@ -785,12 +867,14 @@ struct CePlan {
     uint16_t *q_planes = nullptr, *x_planes = nullptr;
     float* bias2 = nullptr;
     // forward
+    bool few = false;
     int block = 0, slots = 0;
     float2* partial = nullptr;
     float* target_scores = nullptr;
     // backward
     float *terms = nullptr, *log_terms = nullptr, *factors = nullptr, *own = nullptr, *sums = nullptr;
     int *cols = nullptr, *marks = nullptr, *where = nullptr;
+    int own_splits = 1;
     uint32_t* amax = nullptr;
     int piece = 0;  // rows
     uint16_t* G = nullptr;
@@ -801,6 +885,14 @@ struct CePlan {
 
     CePlan(const CeCall& k, bool backward, bool need_q, bool need_x, void* base) : space{static_cast<char*>(base)} {
         const int sms = k.c->sm_count;
+        few = !backward && k.type == CULSH_F32 && k.m <= CE_FEW;
+        if (few) {
+            slots = (int)std::min<size_t>(ceil_div(k.n, CE_FEW_THREADS), (size_t)sms * 3);
+            partial = space.take<float2>((size_t)k.m * slots);
+            target_scores = space.take<float>(k.m);
+            if (k.bias) bias2 = space.take<float>(ceil_div(k.n, 128) * 128);
+            return;
+        }
         if (k.copies(k.Q, k.ldq)) q_planes = space.take<uint16_t>((size_t)k.planes() * k.m * k.pitch());
         if (k.copies(k.X, k.ldx) || (backward && k.bias)) x_planes = space.take<uint16_t>((size_t)k.planes() * k.n * k.pitch());
         if (k.bias) bias2 = space.take<float>(ceil_div(k.n, 128) * 128);
@@ -821,7 +913,9 @@ struct CePlan {
         if (fused_x) log_terms = space.take<float>(tiles_q * TG_M), marks = space.take<int>(tiles_q * TG_M);
         if (need_x) {
             sums = space.take<float>((size_t)k.m * k.d);
-            where = space.take<int>(k.n);
+            // targets of few rows, which many queries share, are summed up for some hundred queries at a time
+            own_splits = (int)std::max<size_t>(1, std::min<size_t>({ceil_div(k.m, 512), 16, (size_t)k.c->sm_count / ceil_div(k.n, own_rows(k))}));
+            where = space.take<int>((size_t)own_splits * k.n);
         }
         // a unit's tiles of the other side: the last wave full, and four tiles' time for the units' ends; at most 32,768 entries in a sum
         const int nb = k.d > 128 ? 64 : 128;
@@ -850,7 +944,8 @@ struct CePlan {
         if ((!need_q || fused_q) && (!need_x || fused_x)) return;
         const bool pieces_x = need_x && !fused_x;
         const size_t row_bytes = (size_t)2 * k.planes() * k.m;
-        const size_t fit = std::min(CE_G_BYTES / row_bytes, pieces_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : CE_G_BYTES) / CE_BN * CE_BN;
+        const size_t space_g = k.planes() * k.planes() / 2 * CE_G_BYTES;  // 32 bits: six products for each read
+        const size_t fit = std::min((space_g ? space_g : CE_G_BYTES) / row_bytes, pieces_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : ~(size_t)0) / CE_BN * CE_BN;
         // the last wave of the products' units full, with as few pieces as that allows
         const size_t most = std::min(std::max<size_t>(fit / CE_BN, 1), tiles_n), wide = pairs(k.m) ? sms / 2 : sms, high = ceil_div(k.m, pairs(k.m) ? 2 * TG_M : TG_M);
         size_t least_time = ~(size_t)0;
@@ -873,9 +968,10 @@ struct CePlan {
         }
         if (pieces_x) {
             split(ceil_div(std::min(piece, k.n), TG_M) * tn, (int)ceil_div(k.m, 64), splits_x, per_x);
-            if (splits_x > 1 || k.planes() == 3) parts_x = space.take<float>((size_t)splits_x * piece * k.d);
+            if (splits_x > 1) parts_x = space.take<float>((size_t)splits_x * piece * k.d);
         }
     }
+    static int own_rows(const CeCall& k) { return (int)std::min<size_t>(CE_OWN_ROWS, ceil_div(ceil_div(k.n, 2 * (size_t)k.c->sm_count), 8) * 8); }
     // A pair of CTAs wants 256 entries of the M side; fewer are left to single ones.
     static bool pairs(int64_t rows) { return rows > TG_M; }
     static int product_bn(int d) { return d > 128 ? 256 : d > 64 ? 128 : 64; }
@@ -909,13 +1005,14 @@ struct CeOperands {
         job(2, p.bias2 ? ceil_div((size_t)k.n + 127, 256) : 0);
         job(3, p.terms ? ceil_div((size_t)k.m + 127, 256) : 0);
         a.terms = p.terms, a.log_terms = p.log_terms, a.factors = p.factors, a.own = p.own, a.sums = p.sums, a.marks = p.marks, a.cols = p.cols, a.where = p.where, a.amax = p.amax;
-        // rows, and where they are few and long columns, in shares for two CTAs an SM
+        // rows, and where they are few and long columns, in shares for some CTAs an SM
         const size_t ctas = 2 * (size_t)k.c->sm_count;
-        a.own_rows = (int)std::min<size_t>(CE_OWN_ROWS, ceil_div(ceil_div(k.n, ctas), 8) * 8);
+        a.own_rows = CePlan::own_rows(k);
         const size_t tiles = ceil_div(k.n, a.own_rows), shares = std::min(ceil_div(k.d, 32 * CE_OWN_COLS), std::max<size_t>(1, 4 * ctas / tiles));
         a.own_cols = (int)(ceil_div(ceil_div(k.d, shares), 32 * CE_OWN_COLS) * 32 * CE_OWN_COLS);
         a.own_shares = (int)ceil_div(k.d, a.own_cols);
-        job(4, p.where ? tiles * a.own_shares : 0);
+        a.own_tiles = (int)tiles, a.own_queries = (int)ceil_div(k.m, p.own_splits);
+        job(4, p.where ? tiles * a.own_shares * p.own_splits : 0);
         if (p.q_planes) q = p.q_planes, ldq = k.pitch();
         if (p.x_planes) x = p.x_planes, ldx = k.pitch();
         if (!end) return;
@@ -959,6 +1056,19 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     const CePlan p(k, false, false, false, workspace);
     const CeOperands ops(k, p, CePrepare{});
     CeScoreArgs a = ce_score_args(k, p);
+    if (p.few) {
+        auto go = [&](auto queries) {
+            constexpr int M = decltype(queries)::value;
+            auto kern = k.bias ? ce_few_kernel<M, true> : ce_few_kernel<M, false>;
+            launch_next(k.stream, kern, (size_t)p.slots, (unsigned)CE_FEW_THREADS, 0, static_cast<const float*>(k.Q), k.ldq, static_cast<const float*>(k.X), k.ldx, k.m, k.n, k.d, k.bias,
+                        a.c, k.targets, p.partial, p.target_scores);
+            KERNEL_CHECK();
+        };
+        if (k.m == 1) go(std::integral_constant<int, 1>());
+        else if (k.m <= 4) go(std::integral_constant<int, 4>());
+        else if (k.m <= 8) go(std::integral_constant<int, 8>());
+        else go(std::integral_constant<int, CE_FEW>());
+    } else {
     a.block = p.block, a.slots = p.slots, a.partial = p.partial, a.target_scores = p.target_scores;
     const size_t units = ceil_div(a.tiles_n, p.block) * a.tiles_q;
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
@@ -968,6 +1078,7 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     ce_by([&](auto planes, auto bias, auto segs, auto pairs) {
         tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value, decltype(pairs)::value>>(k.c, tq, tx, a, k.stream);
     }, k.planes() == 3, k.bias != nullptr, segments, CePlan::pairs(k.m));
+    }
     auto join = p.slots > 256 ? ce_join_kernel<8> : ce_join_kernel<1>;
     launch_next(k.stream, join, ceil_div(k.m, p.slots > 256 ? 1 : 8), 256u, 0, (const float2*)p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
     KERNEL_CHECK();
@@ -986,6 +1097,7 @@ inline CeFinish ce_finish_of(const CeCall& k, const float* parts, int splits, in
 template <typename T>
 inline void ce_finish(const CeCall& k, const CePlan& p, const CeFinish& rows, const CeFinish& queries) {
     CeFinishArgs a{};
+    a.own_splits = p.own_splits, a.where_stride = k.n;
     a.rows = rows, a.queries = queries, a.d = k.d, a.amax = p.amax, a.own = p.own, a.sums = p.sums, a.X = k.X, a.ldx = k.ldx, a.inv_t = (float)(1 / k.temperature);
     const size_t grid = (size_t)rows.blocks + queries.blocks;
     if (!grid) return;
@@ -1012,9 +1124,10 @@ inline void ce_product(const CeCall& k, const CUtensorMap& tg, const void* b, in
         else if (bn == 128) tc_gemm<CeProductPolicy<PLANES, AMN, 128, false, TYPED>>(k.c, tg, tb, a, k.stream);
         else tc_gemm<CeProductPolicy<PLANES, AMN, 64, false, TYPED>>(k.c, tg, tb, a, k.stream);
     };
-    if constexpr (PLANES == 1 && AMN) {
+    if constexpr (AMN) {
         if (a.typed) {
-            if (k.type == CULSH_F16) go(std::integral_constant<int, 2>());
+            if constexpr (PLANES == 3) go(std::integral_constant<int, 3>());
+            else if (k.type == CULSH_F16) go(std::integral_constant<int, 2>());
             else go(std::integral_constant<int, 1>());
             return;
         }
@@ -1036,7 +1149,7 @@ inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, vo
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
     a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = ROWS ? p.log_terms : p.terms, a.marks = p.marks, a.amax = p.amax, a.target_cols = p.cols;
-    a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
+    a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where, a.own_splits = p.own_splits, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
     const CUtensorMap own = ROWS ? ops.map_x(k, TG_M) : ops.map_q(k, TG_M), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
     auto go = [&](auto boxes) {
         constexpr int KB = decltype(boxes)::value;
@@ -1088,12 +1201,13 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         if (pieces_x) {
             CeProductArgs a{};
             a.rows = here, a.b0 = 0, a.kb = (int)ceil_div(k.m, 64), a.out = p.parts_x;
-            if (PLANES == 1 && p.splits_x == 1) {
+            if (p.splits_x == 1) {
                 a.typed = grad_X + n0 * ld_gx, a.ld = ld_gx, a.amax = p.amax, a.where = p.where + n0, a.sums = p.sums;
+                a.own_splits = p.own_splits, a.where_stride = k.n;
                 a.inv_t = (float)(1 / k.temperature);
             }
             ce_product<PLANES, true>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, 64), ops.q, ops.ldq, k.m, a, p.per_x, p.splits_x);
-            if (p.splits_x > 1 || PLANES == 3) {
+            if (p.splits_x > 1) {
                 last = ce_finish_of(k, p.parts_x, p.splits_x, here, nullptr, p.where + n0, grad_X + n0 * ld_gx, ld_gx);
                 if (n0 + here < k.n) ce_finish<T>(k, p, last, CeFinish{}), last = CeFinish{};
             }

@@ -102,7 +102,7 @@ def check_gradients(got, Q, X, targets, bias, temperature, g, e):
         assert float(off.max()) <= 0, (name, float(off.max()), float(tol.max()))
 
 
-SHAPES = [(1, 1, 1), (1, 300, 64), (64, 1000, 100), (130, 257, 128), (129, 513, 31), (300, 70, 520), (2, 5000, 200), (700, 3, 16), (257, 1025, 1100)]
+SHAPES = [(1, 1, 1), (1, 300, 64), (5, 3000, 33), (16, 700, 300), (64, 1000, 100), (130, 257, 128), (129, 513, 31), (300, 70, 520), (2, 5000, 200), (700, 3, 16), (257, 1025, 1100)]
 
 
 @pytest.mark.parametrize("temperature", [1.0, 0.05])
@@ -124,7 +124,7 @@ def test_losses_and_gradients(culsh, m, n, d, dtype, temperature):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,n,d", [(64, 1000, 100), (130, 257, 1100), (3, 5, 7)])
+@pytest.mark.parametrize("m,n,d", [(64, 1000, 100), (130, 257, 1100), (3, 5, 7), (70, 600, 64), (200, 300, 256), (12, 2000, 640)])
 def test_bias_and_masked_rows(culsh, m, n, d, dtype):
     Q, X, targets = sides(m, n, d, dtype)
     bias = torch.randn(n, generator=gen(7), device="cuda")
