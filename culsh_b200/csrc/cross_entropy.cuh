@@ -25,7 +25,6 @@ namespace culsh_b200 {
 
 constexpr int CE_BN = 256, CE_PART = CE_BN / 4;  // columns of a tile, and of it for a warp
 constexpr int CE_SEGMENT = 8;  // steps of 64
-constexpr int CE_SLOTS = CE_BN / CE_PART;  // partial sums of a block of rows
 
 struct CeScoreArgs {
     int* d_error;
@@ -62,10 +61,12 @@ struct CeUnit {
     }
 };
 
-template <int PLANES, bool SEGMENTS, bool PAIRS>
+// Tiles of 256 rows, of a CTA or of a pair of them, and of 64 where those would leave most SMs idle.
+enum CeTile : int { CE_ONE = 0, CE_PAIR = 1, CE_SMALL = 2 };
+template <int PLANES, bool SEGMENTS, int TILE>
 struct CeScoreBase {
-    static constexpr bool A_MN = false, B_MN = false, I8 = false, PARTS = true, PAIR = PAIRS;
-    static constexpr int BN = CE_BN, SEGMENT = SEGMENTS ? CE_SEGMENT : 0, EPI_WARPS = 16;
+    static constexpr bool A_MN = false, B_MN = false, I8 = false, PARTS = true, PAIR = TILE == CE_PAIR;
+    static constexpr int BN = TILE == CE_SMALL ? CE_PART : CE_BN, SEGMENT = SEGMENTS ? CE_SEGMENT : 0, EPI_WARPS = BN / 16;
     static constexpr int EPI_BYTES = EPI_WARPS * CE_PART * 4;
     using Pairs = PlanePairs<PLANES>;
     using Args = CeScoreArgs;
@@ -127,8 +128,9 @@ struct CeSums {
 };
 
 // A thread keeps the running maximum (in powers of two) of its part of a query's scores, and the sum of exponentials by it.  Of a batch, bound by the exponentials (16 a cycle and SM).
-template <int PLANES, bool BIAS, bool SEGMENTS, bool PAIRS>
-struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
+template <int PLANES, bool BIAS, bool SEGMENTS, int TILE>
+struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
+    static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
     struct Epilogue : CeSums<SEGMENTS> {
         int q, quarter, group, lane, rank, target;
         bool idle;
@@ -165,7 +167,7 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
         }
         template <typename D>
         __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more, D&& done) {
-            const int n0 = a.n0 + (u.tile0 + t) * CE_BN + group * CE_PART, left = a.n1 - n0, at = target - n0;
+            const int n0 = a.n0 + (u.tile0 + t) * BN + group * CE_PART, left = a.n1 - n0, at = target - n0;
             if (BIAS && !idle) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
             this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
             done();
@@ -191,13 +193,14 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
             });
         }
         __device__ __forceinline__ void unit_end(const CeScoreArgs& a, const CeUnit& u) {
-            if (q < a.m) a.partial[(int64_t)q * a.slots + u.block * CE_SLOTS + group] = make_float2(ref, sum);
+            if (q < a.m) a.partial[(int64_t)q * a.slots + u.block * (BN / CE_PART) + group] = make_float2(ref, sum);
         }
     };
 };
 
-template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS, bool PAIRS>
-struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
+template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS, int TILE>
+struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
+    static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
     struct Epilogue : CeSums<SEGMENTS> {
         int q, quarter, group, lane, rank, target;
         bool idle;
@@ -216,7 +219,7 @@ struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, PAIRS> {
         }
         template <typename D>
         __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more, D&& done) {
-            const int first = (u.tile0 + t) * CE_BN + group * CE_PART, n0 = a.n0 + first, left = a.n1 - n0, at = target - n0;
+            const int first = (u.tile0 + t) * BN + group * CE_PART, n0 = a.n0 + first, left = a.n1 - n0, at = target - n0;
             if (BIAS && !idle) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
             this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
             done();
@@ -868,6 +871,7 @@ struct CePlan {
     float* bias2 = nullptr;
     // forward
     bool few = false;
+    CeTile tile = CE_ONE;
     int block = 0, slots = 0;
     float2* partial = nullptr;
     float* target_scores = nullptr;
@@ -898,8 +902,10 @@ struct CePlan {
         if (k.bias) bias2 = space.take<float>(ceil_div(k.n, 128) * 128);
         const size_t tiles_q = ceil_div(k.m, TG_M), tiles_n = ceil_div(k.n, CE_BN);
         if (!backward) {
-            block = (int)std::max<size_t>(1, std::min<size_t>(16, tiles_q * tiles_n / ((size_t)sms * 8)));
-            slots = CE_SLOTS * (int)ceil_div(tiles_n, block);
+            tile = tile_of(k, k.n);
+            const size_t tiles = ceil_div(k.n, tile_rows(tile));
+            block = (int)std::max<size_t>(1, std::min<size_t>(16, tiles_q * tiles / ((size_t)sms * 8)));
+            slots = tile_rows(tile) / CE_PART * (int)ceil_div(tiles, block);
             partial = space.take<float2>((size_t)k.m * slots);
             target_scores = space.take<float>(k.m);
             return;
@@ -974,6 +980,12 @@ struct CePlan {
     static int own_rows(const CeCall& k) { return (int)std::min<size_t>(CE_OWN_ROWS, ceil_div(ceil_div(k.n, 2 * (size_t)k.c->sm_count), 8) * 8); }
     // A pair of CTAs wants 256 entries of the M side; fewer are left to single ones.
     static bool pairs(int64_t rows) { return rows > TG_M; }
+    // Of the scores of n rows.
+    static CeTile tile_of(const CeCall& k, int64_t n) {
+        if (ceil_div(k.m, TG_M) * ceil_div(n, CE_BN) <= (size_t)k.c->sm_count / 4) return CE_SMALL;
+        return pairs(k.m) ? CE_PAIR : CE_ONE;
+    }
+    static int tile_rows(CeTile t) { return t == CE_SMALL ? CE_PART : CE_BN; }
     static int product_bn(int d) { return d > 128 ? 256 : d > 64 ? 128 : 64; }
 };
 
@@ -1025,37 +1037,40 @@ struct CeOperands {
     CUtensorMap map_x(const CeCall& k, int box) const { return tg_map(x, k.tg(), k.n, k.d, ldx, k.planes(), (int64_t)k.n * ldx * 2, box); }
 };
 
-inline CeScoreArgs ce_score_args(const CeCall& k, const CePlan& p) {
-    CeScoreArgs a{};
-    a.d_error = k.d_error, a.idesc = tg_idesc(k.tg(), false, false);
-    a.m = k.m, a.kb = (int)ceil_div(k.d, 64), a.n0 = 0, a.n1 = k.n;
-    a.m_tile = CePlan::pairs(k.m) ? 2 * TG_M : TG_M;
-    a.tiles_q = (int)ceil_div(k.m, a.m_tile), a.tiles_n = (unsigned)ceil_div(k.n, CE_BN);
-    a.c = k.c2(), a.bias = p.bias2, a.targets = k.targets;
-    return a;
-}
-
-// f(number of planes, whether there is a bias, whether K is taken in segments, whether by pairs of CTAs), as types.
+// f(number of planes, whether there is a bias, whether K is taken in segments, the tile), as types.
 template <typename F>
-inline void ce_by(F&& f, bool three, bool bias, bool segments, bool pairs) {
+inline void ce_by(F&& f, bool three, bool bias, bool segments, CeTile tile) {
     auto one = [](bool v, auto&& g) {
         if (v) g(std::true_type());
         else g(std::false_type());
     };
     one(bias, [&](auto b) {
         one(segments, [&](auto s) {
-            one(pairs, [&](auto p) {
-                if (three) f(std::integral_constant<int, 3>(), b, s, p);
-                else f(std::integral_constant<int, 1>(), b, s, p);
-            });
+            auto with = [&](auto t) {
+                if (three) f(std::integral_constant<int, 3>(), b, s, t);
+                else f(std::integral_constant<int, 1>(), b, s, t);
+            };
+            if (tile == CE_PAIR) with(std::integral_constant<int, CE_PAIR>());
+            else if (tile == CE_SMALL) with(std::integral_constant<int, CE_SMALL>());
+            else with(std::integral_constant<int, CE_ONE>());
         });
     });
 }
+inline CeScoreArgs ce_score_args(const CeCall& k, const CePlan& p, CeTile tile, int n0, int n1) {
+    CeScoreArgs a{};
+    a.d_error = k.d_error, a.idesc = tg_idesc(k.tg(), false, false);
+    a.m = k.m, a.kb = (int)ceil_div(k.d, 64), a.n0 = n0, a.n1 = n1;
+    a.m_tile = tile == CE_PAIR ? 2 * TG_M : TG_M;
+    a.tiles_q = (int)ceil_div(k.m, a.m_tile), a.tiles_n = (unsigned)ceil_div(n1 - n0, CePlan::tile_rows(tile));
+    a.c = k.c2(), a.bias = p.bias2, a.targets = k.targets;
+    return a;
+}
+inline int ce_box_x(CeTile tile) { return tile == CE_PAIR ? CE_BN / 2 : CePlan::tile_rows(tile); }
 
 inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse_low, void* workspace) {
     const CePlan p(k, false, false, false, workspace);
     const CeOperands ops(k, p, CePrepare{});
-    CeScoreArgs a = ce_score_args(k, p);
+    CeScoreArgs a = ce_score_args(k, p, p.tile, 0, k.n);
     if (p.few) {
         auto go = [&](auto queries) {
             constexpr int M = decltype(queries)::value;
@@ -1073,11 +1088,11 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     const size_t units = ceil_div(a.tiles_n, p.block) * a.tiles_q;
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
-    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CePlan::pairs(k.m) ? CE_BN / 2 : CE_BN);
+    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, ce_box_x(p.tile));
     const bool segments = a.kb > CE_SEGMENT;
-    ce_by([&](auto planes, auto bias, auto segs, auto pairs) {
-        tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value, decltype(pairs)::value>>(k.c, tq, tx, a, k.stream);
-    }, k.planes() == 3, k.bias != nullptr, segments, CePlan::pairs(k.m));
+    ce_by([&](auto planes, auto bias, auto segs, auto tile) {
+        tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value, decltype(tile)::value>>(k.c, tq, tx, a, k.stream);
+    }, k.planes() == 3, k.bias != nullptr, segments, p.tile);
     }
     auto join = p.slots > 256 ? ce_join_kernel<8> : ce_join_kernel<1>;
     launch_next(k.stream, join, ceil_div(k.m, p.slots > 256 ? 1 : 8), 256u, 0, (const float2*)p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
@@ -1180,24 +1195,24 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         if (p.fused_q) ce_fused<false, HALF>(k, p, ops, nullptr, 0);
     }
     const bool pieces_q = grad_Q && !p.fused_q, pieces_x = grad_X && !p.fused_x;
-    const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, CePlan::pairs(k.m) ? CE_BN / 2 : CE_BN);
+    const CUtensorMap tq = ops.map_q(k, TG_M);
     const int64_t g_plane = (int64_t)k.m * p.piece;
-    CeScoreArgs s = ce_score_args(k, p);
-    s.terms = p.terms, s.factors = p.factors, s.amax = p.amax, s.target_cols = p.cols, s.G = p.G, s.pitch = p.piece, s.plane = g_plane;
-    s.block = 1;
     for (int64_t n0 = 0; (pieces_q || pieces_x) && n0 < k.n; n0 += p.piece) {
         const int here = (int)std::min<int64_t>(p.piece, k.n - n0);
-        s.n0 = (int)n0, s.n1 = (int)(n0 + here);
-        s.tiles_n = (unsigned)ceil_div(here, CE_BN);
+        const CeTile tile = CePlan::tile_of(k, here);
+        CeScoreArgs s = ce_score_args(k, p, tile, (int)n0, (int)(n0 + here));
+        s.terms = p.terms, s.factors = p.factors, s.amax = p.amax, s.target_cols = p.cols, s.G = p.G, s.pitch = p.piece, s.plane = g_plane;
+        s.block = 1;
         const size_t units = (size_t)s.tiles_n * s.tiles_q;
         if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
         s.units = (unsigned)units;
-        ce_by([&](auto planes, auto bias, auto segs, auto pairs) {
+        const CUtensorMap tx = ops.map_x(k, ce_box_x(tile));
+        ce_by([&](auto planes, auto bias, auto segs, auto type) {
             // 16-bit results are none the worse for the segments' sums being one
             if constexpr (decltype(planes)::value == PLANES && (PLANES == 3 || !decltype(segs)::value))
-                tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value, decltype(pairs)::value>>(k.c, tq, tx, s, k.stream);
-        }, PLANES == 3, k.bias != nullptr, PLANES == 3 && s.kb > CE_SEGMENT, CePlan::pairs(k.m));
-        const int64_t g_cols = (int64_t)s.tiles_n * CE_BN;
+                tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value, decltype(type)::value>>(k.c, tq, tx, s, k.stream);
+        }, PLANES == 3, k.bias != nullptr, PLANES == 3 && s.kb > CE_SEGMENT, tile);
+        const int64_t g_cols = (int64_t)s.tiles_n * CePlan::tile_rows(tile);  // behind the last row G has zeros
         if (pieces_x) {
             CeProductArgs a{};
             a.rows = here, a.b0 = 0, a.kb = (int)ceil_div(k.m, 64), a.out = p.parts_x;
