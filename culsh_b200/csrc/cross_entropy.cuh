@@ -421,6 +421,9 @@ struct CeProductPolicy {
 
 // Losses of up to 16 queries in 32 bits, which would leave the tensor cores' lanes empty and cost the planes' reads and writes: bound by reading the rows once.  A thread has a row, 32 columns of
 // 256 rows at a time come through shared memory; the queries' values are read from there by all lanes at once.  Maxima and sums are a thread's until the end.
+// Where it is taken, on the tensor cores | here (us): losses of 500,000 x 16, 1 query 126 | 24, 16 of them 129 | 82; 128,000 x 500, 1 query 297 | 83, but 16 of 2,000 x 500 29 | 85.  Gradients of
+// 500,000 x 128, 1 query 660 | 279, 16 of them 621 | 461, of 2,000 x 128 44 | 50, but of 8,000 x 500 81 | 159.  16 bits are none the better for it (500,000 x 128, 4 queries 229 | 439).
+constexpr int CE_FEW_LOSS = 1024, CE_FEW_GRAD = 192;  // queries by columns; columns
 constexpr int CE_FEW = 16, CE_FEW_COLS = 32, CE_FEW_THREADS = 256;
 template <int M, bool BIAS>
 __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* __restrict__ Q, int64_t ldq, const float* __restrict__ X, int64_t ldx, int m, int n, int d,
@@ -493,6 +496,95 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
             partial[(int64_t)q * gridDim.x + blockIdx.x] = make_float2(top, all);
         }
     }
+}
+
+// Gradients of up to 16 queries, likewise.  First the scores of 256 rows, a row to a thread, and G, to which the target's own coefficient belongs here (nothing is rounded to 16 bits); then, a
+// column to a lane, what the rows put into dQ, and dX.  dQ's sums are a CTA's, in shared memory; ce_finish_kernel adds them up.
+template <typename T, int M, bool BIAS>
+__global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_grad_kernel(const T* __restrict__ Q, int64_t ldq, const T* __restrict__ X, int64_t ldx, int m, int n, int d,
+                                                                        const float* __restrict__ bias, float c, float inv_t, const float* __restrict__ terms,
+                                                                        const float* __restrict__ factors, const float* __restrict__ own, const int* __restrict__ cols,
+                                                                        float* __restrict__ parts, T* __restrict__ dX, int64_t ldo, KernelBefore before) {
+    behind_kernel_before(Q, X, bias, terms, factors, own, cols, parts, dX, before);
+    constexpr int MQ = M < 4 ? 4 : M;
+    __shared__ alignas(16) float s_x[CE_FEW_COLS][CE_FEW_THREADS + 1];
+    __shared__ alignas(16) float s_q[CE_FEW_COLS][MQ];
+    extern __shared__ float s_sums[];  // [m][d]
+    float* const s_add = &s_x[0][0];   // [warp][query][column of 32], where the rows' values are no longer needed
+    float(*const s_g)[MQ] = reinterpret_cast<float(*)[MQ]>(s_add + CE_FEW_THREADS * M);
+    static_assert(CE_FEW_THREADS * (M + MQ) <= CE_FEW_COLS * (CE_FEW_THREADS + 1), "");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = threadIdx.x; parts && i < m * d; i += CE_FEW_THREADS) s_sums[i] = 0.f;
+    for (int64_t row0 = (int64_t)blockIdx.x * CE_FEW_THREADS; row0 < n; row0 += (int64_t)gridDim.x * CE_FEW_THREADS) {
+        float acc[M] = {};
+        for (int c0 = 0; c0 < d; c0 += CE_FEW_COLS) {
+            float v[CE_FEW_COLS];  // a warp's 32 rows, a column to a lane
+#pragma unroll
+            for (int j = 0; j < CE_FEW_COLS; ++j) {
+                const int64_t row = row0 + warp * 32 + j;
+                v[j] = row < n && c0 + lane < d ? ce_float(__ldcg(X + row * ldx + c0 + lane)) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < CE_FEW_COLS; ++j) s_x[lane][warp * 32 + j] = v[j];
+            for (int i = threadIdx.x; i < CE_FEW_COLS * M; i += CE_FEW_THREADS) {
+                const int q = i / CE_FEW_COLS, k = i % CE_FEW_COLS;
+                s_q[k][q] = q < m && c0 + k < d ? ce_float(__ldcg(Q + q * ldq + c0 + k)) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll 8
+            for (int k = 0; k < min(CE_FEW_COLS, d - c0); ++k) {
+                const float x = s_x[k][threadIdx.x];
+#pragma unroll
+                for (int q = 0; q < M; ++q) acc[q] = fmaf(s_q[k][q], x, acc[q]);
+            }
+        }
+        __syncthreads();
+        const int64_t row = row0 + threadIdx.x;
+        const float b = BIAS && row < n ? __ldcg(bias + row) * CE_LOG2E : 0.f;
+        const bool masked = row >= n || (BIAS && b == -INFINITY);
+#pragma unroll
+        for (int q = 0; q < M; ++q) {
+            float g = 0.f;
+            if (q < m && !masked) g = __ldcg(cols + q) == row ? __ldcg(own + q) : ce_exp2(fmaf(acc[q], c, __ldcg(terms + q) + b)) * __ldcg(factors + q);
+            s_g[threadIdx.x][q] = g;
+        }
+        const unsigned live = __ballot_sync(0xFFFFFFFFu, !masked);  // a row that is masked may hold anything
+        for (int c0 = 0; c0 < d; c0 += CE_FEW_COLS) {
+            const int col = c0 + lane;
+            float q_of[M], sum[M] = {};
+#pragma unroll
+            for (int q = 0; q < M; ++q) q_of[q] = dX && q < m && col < d ? ce_float(__ldcg(Q + q * ldq + col)) * inv_t : 0.f;
+            __syncwarp();
+#pragma unroll 4
+            for (int j = 0; j < 32; ++j) {
+                const int64_t at = row0 + warp * 32 + j;
+                const float x = parts && live >> j & 1u && col < d ? ce_float(__ldcg(X + at * ldx + col)) : 0.f;
+                float out = 0.f;
+#pragma unroll
+                for (int q = 0; q < M; ++q) {
+                    const float g = s_g[warp * 32 + j][q];
+                    sum[q] = fmaf(g, x, sum[q]);
+                    out = fmaf(g, q_of[q], out);
+                }
+                if (dX && at < n && col < d) dX[at * ldo + col] = (T)out;
+            }
+            if (parts) {
+                __syncthreads();
+#pragma unroll
+                for (int q = 0; q < M; ++q) s_add[(warp * M + q) * 32 + lane] = sum[q];
+                __syncthreads();
+                for (int i = threadIdx.x; i < 32 * M; i += CE_FEW_THREADS) {
+                    const int q = i / 32, k = i % 32;
+                    float all = 0.f;
+                    for (int w = 0; w < CE_FEW_THREADS / 32; ++w) all += s_add[(w * M + q) * 32 + k];
+                    if (q < m && c0 + k < d) s_sums[q * d + c0 + k] += all;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; parts && i < m * d; i += CE_FEW_THREADS) parts[(int64_t)blockIdx.x * m * d + i] = s_sums[i];
 }
 
 // ---- what the products need beforehand: one launch, whose CTAs have a share of one of five jobs each --------------------------------------------------------------------
@@ -798,7 +890,7 @@ __device__ __forceinline__ void ce_finish_part(const CeFinishArgs& a, const CeFi
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] += w[k];
     }
-    int w = __ldcg(f.which + row);
+    int w = f.which ? __ldcg(f.which + row) : -1;
     float scale = 1.f;
     if (f.factors) scale = std::is_same<T, __half>::value ? ldexpf(__ldcg(f.factors + row), -14) : __ldcg(f.factors + row);
     else if (a.amax) scale = ldexpf(1.f, -ce_scale_exponent(a.amax));
@@ -889,12 +981,20 @@ struct CePlan {
 
     CePlan(const CeCall& k, bool backward, bool need_q, bool need_x, void* base) : space{static_cast<char*>(base)} {
         const int sms = k.c->sm_count;
-        few = !backward && k.type == CULSH_F32 && k.m <= CE_FEW;
+        few = !backward && k.type == CULSH_F32 && k.m <= CE_FEW && (int64_t)k.m * k.d <= CE_FEW_LOSS;
         if (few) {
             slots = (int)std::min<size_t>(ceil_div(k.n, CE_FEW_THREADS), (size_t)sms * 3);
             partial = space.take<float2>((size_t)k.m * slots);
             target_scores = space.take<float>(k.m);
             if (k.bias) bias2 = space.take<float>(ceil_div(k.n, 128) * 128);
+            return;
+        }
+        if (backward && k.type == CULSH_F32 && k.m <= CE_FEW && k.d <= CE_FEW_GRAD) {
+            few = true;
+            terms = space.take<float>(k.m), factors = space.take<float>(k.m), own = space.take<float>(k.m);
+            cols = space.take<int>(k.m);
+            splits_q = (int)std::min<size_t>(ceil_div(k.n, CE_FEW_THREADS), (size_t)sms * 2);
+            if (need_q) acc_q = space.take<float>((size_t)splits_q * k.m * k.d);
             return;
         }
         if (k.copies(k.Q, k.ldq)) q_planes = space.take<uint16_t>((size_t)k.planes() * k.m * k.pitch());
@@ -1186,6 +1286,27 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
     CePrepare before{};
     before.losses = losses, before.lse = lse, before.lse_low = lse_low, before.grad_losses = grad_losses, before.grad_lse = grad_lse;
     const CeOperands ops(k, p, before);
+    if constexpr (PLANES == 3) {
+        if (p.few) {
+            auto go = [&](auto queries) {
+                constexpr int M = decltype(queries)::value;
+                auto kern = k.bias ? ce_few_grad_kernel<T, M, true> : ce_few_grad_kernel<T, M, false>;
+                static thread_local uint64_t ready[2] = {};  // devices whose limit is set
+                uint64_t& is = ready[k.bias != nullptr];
+                if (k.c->device >= 64 || !(is >> k.c->device & 1)) {
+                    CU_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, CE_FEW * CE_FEW_GRAD * 4));
+                    if (k.c->device < 64) is |= 1ull << k.c->device;
+                }
+                launch_next(k.stream, kern, (size_t)p.splits_q, (unsigned)CE_FEW_THREADS, grad_Q ? (size_t)k.m * k.d * 4 : 0, static_cast<const T*>(k.Q), k.ldq, static_cast<const T*>(k.X), k.ldx,
+                            k.m, k.n, k.d, k.bias, k.c2(), (float)(1 / k.temperature), p.terms, p.factors, p.own, p.cols, p.acc_q, grad_X, ld_gx);
+                KERNEL_CHECK();
+            };
+            if (k.m <= 4) go(std::integral_constant<int, 4>());
+            else go(std::integral_constant<int, CE_FEW>());
+            if (grad_Q) ce_finish<T>(k, p, CeFinish{}, ce_finish_of(k, p.acc_q, p.splits_q, k.m, nullptr, nullptr, grad_Q, ld_gq));
+            return;
+        }
+    }
     CeFinish last{};  // of dX, for the launch that finishes dQ
     if constexpr (PLANES == 1) {
         if (p.fused_x) {

@@ -102,7 +102,7 @@ def check_gradients(got, Q, X, targets, bias, temperature, g, e):
         assert float(off.max()) <= 0, (name, float(off.max()), float(tol.max()))
 
 
-SHAPES = [(1, 1, 1), (1, 300, 64), (5, 3000, 33), (16, 700, 300), (64, 1000, 100), (130, 257, 128), (129, 513, 31), (300, 70, 520), (2, 5000, 200), (700, 3, 16), (257, 1025, 1100)]
+SHAPES = [(1, 1, 1), (1, 300, 64), (5, 3000, 33), (16, 700, 300), (16, 90_000, 5), (3, 400, 2730), (64, 1000, 100), (130, 257, 128), (129, 513, 31), (300, 70, 520), (2, 5000, 200), (700, 3, 16), (257, 1025, 1100)]
 
 
 @pytest.mark.parametrize("temperature", [1.0, 0.05])
