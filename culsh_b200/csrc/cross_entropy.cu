@@ -13,7 +13,7 @@ CeCall call_of(culsh_handle* h, const void* Q, int64_t ldq, const void* X, int64
     need(h && Q && X, "null argument");
     need(type >= 0 && type <= 3 && (SCORE_TYPES >> type & 1), "queries and rows have to be float32, float16 or bfloat16");
     need(m > 0 && n > 0 && d > 0, "queries, rows and features must be positive");
-    need(m <= 0x7FFFFF00 && n <= 0x7FFFFF00, "at most 2,147,483,392 queries and rows");
+    need(m <= 0x7FFF0000 && n <= 0x7FFF0000, "at most 2,147,418,112 queries and rows");  // places a tile behind the last one are still below 2^31
     need(d <= 1 << 16, "at most 65,536 features");
     need(ldq >= d && ldx >= d, "rows must not overlap");
     need(temperature > 0 && std::isfinite(temperature), "temperature must be positive");

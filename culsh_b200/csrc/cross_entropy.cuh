@@ -127,7 +127,8 @@ struct CeSums {
     }
 };
 
-// A thread keeps the running maximum (in powers of two) of its part of a query's scores, and the sum of exponentials by it.  Of a batch, bound by the exponentials (16 a cycle and SM).
+// A thread keeps the running maximum (in powers of two) of its part of a query's scores, and the sum of exponentials by it.  Of a batch, bound by the exponentials, 16 a cycle and SM: 4,096 x
+// 1M x 128 bfloat16 1.25 ms, their unit busy for 80 %, the tensor pipe for 39.  (Eight warps in place of sixteen 2.0 ms; an arrival that releases to the cluster, for each tile of each warp, 1.9.)
 template <int PLANES, bool BIAS, bool SEGMENTS, int TILE>
 struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
     static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
@@ -198,6 +199,7 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
     };
 };
 
+// G of a piece, 128 neighbouring bytes of a query to a thread.  4,099 x 6,656 x 2,048 float16 82 us, 1,355 TFLOP/s.
 template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS, int TILE>
 struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
     static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
@@ -259,6 +261,7 @@ struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
     };
 };
 
+// Bound by the tensor pipe and by the ends of the few waves: 6,656 x 2,048 by 4,099 88 us, 4,099 x 2,048 by 6,656 97.
 // Products with G: out[split][row][col] (+)= sum over a split of K of A's row by B's column.
 struct CeProductArgs {
     int* d_error;

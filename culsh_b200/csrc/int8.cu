@@ -8,7 +8,7 @@ namespace {
 
 void check_rows(const void* codes, const void* scales, const void* squares, int n, int d) {
     need(n > 0 && d > 0, "rows and features must be positive");
-    need(n <= 0x7FFFFF80, "at most 2,147,483,520 rows");
+    need(n <= 0x7FFF0000, "at most 2,147,418,112 rows");  // places a tile behind the last one are still below 2^31
     need(d <= I8_MAX_FEATURES, "at most 131,072 features");
     need(codes && scales && squares, "null argument");
     need(((uintptr_t)codes & 15) == 0, "codes have to begin at a multiple of 16 bytes");

@@ -357,3 +357,14 @@ def test_refusals(culsh):
                 lambda: culsh.cross_entropy_backward(Q, X, targets, r, one[:3]), lambda: culsh.cross_entropy_backward(Q[:3], X, targets[:3], r, one[:3])):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_sizes_beyond_an_index_are_refused(culsh):
+    import ctypes as C
+
+    from culsh_b200 import _lib
+    from culsh_b200._culsh_core import get_handle
+    h, need = get_handle(0), C.c_uint64()
+    for m, n, d in ((2 ** 31 - 1, 5, 1), (5, 2 ** 31 - 1, 1), (5, 5, 65_537), (0, 5, 5)):
+        assert h.lib.culsh_cross_entropy_workspace(h.ptr, 16, 65_537, 16, 65_537, 0, m, n, d, 0, 3, C.byref(need)) == -1
+    assert h.lib.culsh_cross_entropy_workspace(h.ptr, 16, 4, 16, 4, 1, 5, 5, 4, 0, 3, C.byref(need)) == -1 and b"float" in _lib.load().culsh_last_error()
