@@ -1008,7 +1008,9 @@ struct CePlan {
             tile = tile_of(k, k.n);
             const size_t tiles = ceil_div(k.n, tile_rows(tile));
             block = (int)std::max<size_t>(1, std::min<size_t>(16, tiles_q * tiles / ((size_t)sms * 8)));
-            slots = tile_rows(tile) / CE_PART * (int)ceil_div(tiles, block);
+            auto parts = [&] { return (size_t)(tile_rows(tile) / CE_PART) * ceil_div(tiles, block); };
+            while (parts() * k.m * sizeof(float2) > CE_PARTS_BYTES && (size_t)block < tiles) block *= 2;  // more tiles to a unit where there are very many queries
+            slots = (int)parts();
             partial = space.take<float2>((size_t)k.m * slots);
             target_scores = space.take<float>(k.m);
             return;
@@ -1058,7 +1060,7 @@ struct CePlan {
         // the last wave of the products' units full, with as few pieces as that allows
         const size_t most = std::min(std::max<size_t>(fit / CE_BN, 1), tiles_n), wide = pairs(k.m) ? sms / 2 : sms, high = ceil_div(k.m, pairs(k.m) ? 2 * TG_M : TG_M);
         size_t least_time = ~(size_t)0;
-        for (size_t p = most; p >= std::max<size_t>(1, most / 3); --p) {
+        for (size_t p = most, step = most / 64 + 1; p >= std::max<size_t>(1, most / 3); p -= std::min(p, step)) {
             const size_t rest = tiles_n % p, time = tiles_n / p * (ceil_div(high * p, wide) * 8 + 1) + (rest ? ceil_div(high * rest, wide) * 8 + 1 : 0);
             if (time < least_time) least_time = time, piece = (int)(p * CE_BN);
         }

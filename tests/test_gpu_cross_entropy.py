@@ -207,6 +207,51 @@ def test_gradients_of_targets_that_many_queries_share(culsh):
         check_gradients(culsh.cross_entropy_backward(Q, X, targets, r, g, temperature=0.2), Q, X, targets, None, 0.2, g, None)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,d", [(33_000, 300, 24), (600, 500, 5_000), (3_000, 40, 300), (2_000, 20_000, 70)])
+def test_gradients_of_many_queries_and_of_long_rows(culsh, m, n, d, dtype):
+    """More queries than one accumulator takes, targets summed up for some hundred queries at a time, rows in one piece and in several."""
+    Q, X, targets = sides(m, n, d, dtype)
+    r = culsh.cross_entropy(Q, X, targets, temperature=0.3)
+    check_losses(r, Q, X, targets, None, 0.3)
+    g, e = torch.randn(m, generator=gen(5), device="cuda"), torch.randn(m, generator=gen(6), device="cuda")
+    check_gradients(culsh.cross_entropy_backward(Q, X, targets, r, g, e, temperature=0.3), Q, X, targets, None, 0.3, g, e)
+
+
+def test_another_thread_and_a_first_call_in_a_graph(culsh):
+    """A handle of its own for each thread; a shape that is new when it is captured."""
+    import threading
+    Q, X, targets = sides(90, 700, 48, torch.float16)
+    g = torch.ones(90, device="cuda")
+    want = culsh.cross_entropy(Q, X, targets, temperature=0.2)
+    got = {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            r = culsh.cross_entropy(Q, X, targets, temperature=0.2)
+            got[i] = (*r, *culsh.cross_entropy_backward(Q, X, targets, r, g, temperature=0.2), culsh.Int8Rows(X).product(Q))
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 4
+    for out in got.values():
+        assert torch.equal(out[0], want.losses) and all(torch.equal(a, b) for a, b in zip(out, got[0]))
+    q, x = Q[:33, :40].float().contiguous(), X[:, :40].float().contiguous()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r = culsh.cross_entropy(q, x, targets[:33], temperature=0.4)
+        grads = culsh.cross_entropy_backward(q, x, targets[:33], r, g[:33], temperature=0.4)
+    graph.replay()
+    torch.cuda.synchronize()
+    check_losses(r, q, x, targets[:33], None, 0.4)
+    check_gradients(grads, q, x, targets[:33], None, 0.4, g[:33], None)
+
+
 def test_nearly_certain_targets(culsh):
     """p of the target next to 1: its coefficient is a small difference, which is not rounded with it."""
     for dtype in TYPES:
