@@ -8,9 +8,10 @@
 // Forward: products on the tensor cores (tc_gemm.cuh), queries on the M side, so that a thread holds neighbouring scores of one query and keeps the running maximum and sum of
 // a block of rows by itself; blocks are joined in 64 bits.  lse comes as two floats, of which the second is what the first leaves: a score of a thousand would leave p an error of 2^-14 otherwise.
 //
-// Backward: rows in pieces whose G fits L2; for each, G once more from the products, and two products with it.  The target's own entry stays out of G: where p is near 1 it is a small
+// Backward: rows in pieces whose G fits L2 (twice that in 32 bits, where six products read it); for each, G once more from the products, and two products with it.  Rows of up to 256 values of 16 bits
+// keep it on the SM (ce_fused.cuh).  The target's own entry stays out of G: where p is near 1 it is a small
 // difference, and where it is not, it outweighs the rest and so would its rounding to 16 bits; its coefficient g expm1(-loss) + e exp(-loss) is taken in 32 bits, and times the row or the
-// query added to the sums.  Sums of one row's gradient over its queries are taken in ascending order: nothing depends on the order of atomics.
+// query added to the sums (ce_prepare_kernel, ce_finish_kernel).  Sums of one row's gradient over its queries are taken in ascending order: nothing depends on the order of atomics.
 //
 // 32-bit floats are held as three bfloat16 planes each (24 bits), products as six of 16 bits; G of 32-bit inputs likewise.  G of half precision is scaled by a power of two that brings the
 // largest coefficient to 2^15, so that p down to 2^-39 of it is there.
@@ -127,8 +128,9 @@ struct CeSums {
     }
 };
 
-// A thread keeps the running maximum (in powers of two) of its part of a query's scores, and the sum of exponentials by it.  Of a batch, bound by the exponentials, 16 a cycle and SM: 4,096 x
-// 1M x 128 bfloat16 1.25 ms, their unit busy for 80 %, the tensor pipe for 39.  (Eight warps in place of sixteen 2.0 ms; an arrival that releases to the cluster, for each tile of each warp, 1.9.)
+// A thread keeps the largest of its part of a query's scores (of the exponents, where there is a bias) and the sum of exponentials by it; the largest one's is exactly 1, and so the loss of a query
+// that has but one row is exactly 0.  Of a batch, bound by the exponentials, 16 a cycle and SM: 4,096 x
+// 1M x 128 bfloat16 1.29 ms, their unit busy for 80 %, the tensor pipe for 39.  (Eight warps in place of sixteen 2.0 ms; an arrival that releases to the cluster, for each tile of each warp, 1.9.)
 template <int PLANES, bool BIAS, bool SEGMENTS, int TILE>
 struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
     static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
@@ -151,19 +153,19 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < CE_PART; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
-            const float next = fmaxf(ref, BIAS ? top : top * a.c), base = next == -INFINITY ? 0.f : next;
+            const float next = fmaxf(ref, top), base = next == -INFINITY ? 0.f : next;
             const uint64_t cc = f2_pack(a.c, a.c), minus = f2_pack(-base, -base);
             uint64_t part[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
             for (int j = 0; j < CE_PART; j += 2) {
                 const uint64_t pair = f2_pack(x[j], x[j + 1]);
                 float e0, e1;
-                f2_unpack(BIAS ? f2_add(pair, minus) : f2_fma(pair, cc, minus), e0, e1);
+                f2_unpack(BIAS ? f2_add(pair, minus) : f2_mul(f2_add(pair, minus), cc), e0, e1);
                 part[j / 2 & 3] = f2_add(part[j / 2 & 3], f2_pack(ce_exp2(e0), ce_exp2(e1)));
             }
             float lo, hi;
             f2_unpack(f2_add(f2_add(part[0], part[1]), f2_add(part[2], part[3])), lo, hi);
-            sum = fmaf(sum, ce_exp2(ref - base), lo + hi);
+            sum = fmaf(sum, ce_exp2(BIAS ? ref - base : (ref - base) * a.c), lo + hi);
             ref = next;
         }
         template <typename D>
@@ -437,6 +439,7 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
     __shared__ alignas(16) float s_q[CE_FEW_COLS][M < 4 ? 4 : M];
     __shared__ float2 s_part[CE_FEW_THREADS / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float by = BIAS ? 1.f : c;
     float ref[M], sum[M];
     int target[M];
 #pragma unroll
@@ -475,8 +478,8 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
 #pragma unroll
             for (int q = 0; q < M; ++q) {
                 if (target[q] == row) target_scores[q] = acc[q];
-                const float z = BIAS && b == -INFINITY ? b : fmaf(acc[q], c, b), next = fmaxf(ref[q], z), base = next == -INFINITY ? 0.f : next;
-                sum[q] = fmaf(sum[q], ce_exp2(ref[q] - base), ce_exp2(BIAS ? z - base : fmaf(acc[q], c, -base)));
+                const float z = !BIAS ? acc[q] : b == -INFINITY ? b : fmaf(acc[q], c, b), next = fmaxf(ref[q], z), base = next == -INFINITY ? 0.f : next;
+                sum[q] = fmaf(sum[q], ce_exp2((ref[q] - base) * by), ce_exp2((z - base) * by));
                 ref[q] = next;
             }
         }
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
         if (q >= m) break;
         float top = ref[q];
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        float all = sum[q] * ce_exp2(ref[q] - (top == -INFINITY ? 0.f : top));
+        float all = sum[q] * ce_exp2((ref[q] - (top == -INFINITY ? 0.f : top)) * by);
         for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
         __syncthreads();
         if (lane == 0) s_part[warp] = make_float2(top, all);
@@ -495,7 +498,7 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
             for (int w = 1; w < CE_FEW_THREADS / 32; ++w) top = fmaxf(top, s_part[w].x);
             const float base = top == -INFINITY ? 0.f : top;
             all = 0.f;
-            for (int w = 0; w < CE_FEW_THREADS / 32; ++w) all = fmaf(s_part[w].y, ce_exp2(s_part[w].x - base), all);
+            for (int w = 0; w < CE_FEW_THREADS / 32; ++w) all = fmaf(s_part[w].y, ce_exp2((s_part[w].x - base) * by), all);
             partial[(int64_t)q * gridDim.x + blockIdx.x] = make_float2(top, all);
         }
     }
@@ -673,12 +676,12 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
         __syncthreads();
         for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_top[warp / WARPS * WARPS + w]);
     }
-    const float base = top == -INFINITY ? 0.f : top;
+    const float base = top == -INFINITY ? 0.f : top, by = bias2 ? 1.f : c;  // scores, or exponents
     double sum = 0.;
 #pragma unroll 8
     for (int i = first; i < slots; i += 32 * WARPS) {
         const float2 v = __ldcg(p + i);
-        sum += (double)v.y * (double)exp2f(v.x - base);
+        sum += (double)v.y * (double)exp2f((v.x - base) * by);
     }
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (WARPS > 1) {
@@ -688,14 +691,15 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
         for (int w = 0; w < WARPS; ++w) sum += s_sum[warp / WARPS * WARPS + w];
     }
     if (first || q >= m) return;
-    const double ln2 = 0.69314718055994530942, two = (double)base + log2(sum), whole = two * ln2;
+    const double ln2 = 0.69314718055994530942, two = (double)base * (double)by + log2(sum), whole = two * ln2;
     const float high = (float)whole;
     lse[q] = high;
     lse_low[q] = isfinite(high) ? (float)(whole - (double)high) : 0.f;
     float loss = 0.f;
     const int64_t t = targets ? __ldcg(targets + q) : -1;
     if (t >= 0 && t < n) {
-        const double b = bias2 ? (double)__ldcg(bias2 + t) : 0., z = b == -INFINITY ? b : (double)__ldcg(target_scores + q) * (double)c + b;
+        const float b = bias2 ? __ldcg(bias2 + t) : 0.f, s = __ldcg(target_scores + q);
+        const double z = b == -INFINITY ? (double)b : bias2 ? (double)fmaf(s, c, b) : (double)s * (double)c;  // as in the sums
         loss = z == -INFINITY && two == two ? INFINITY : (float)((two - z) * ln2);
         if (loss < 0.f) loss = 0.f;
     }

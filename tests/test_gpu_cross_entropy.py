@@ -218,6 +218,19 @@ def test_gradients_of_many_queries_and_of_long_rows(culsh, m, n, d, dtype):
     check_gradients(culsh.cross_entropy_backward(Q, X, targets, r, g, e, temperature=0.3), Q, X, targets, None, 0.3, g, e)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_loss_of_one_row_is_0(culsh, dtype):
+    for m, n, d in ((3, 1, 70), (200, 1, 640), (40, 1, 64)):
+        Q, X, targets = sides(m, n, d, dtype)
+        assert not culsh.cross_entropy(Q, X, targets, temperature=0.3).losses.any()
+        assert not culsh.cross_entropy(Q, X, targets, torch.full((1,), 0.7, device="cuda"), temperature=0.3).losses.any()
+    Q, X, targets = sides(50, 900, 96, dtype)
+    bias = torch.full((900,), -np.inf, device="cuda")
+    bias[17] = -3.3
+    r = culsh.cross_entropy(Q, X, torch.full_like(targets, 17), bias)
+    assert not r.losses.any()
+
+
 def test_another_thread_and_a_first_call_in_a_graph(culsh):
     """A handle of its own for each thread; a shape that is new when it is captured."""
     import threading
