@@ -8,7 +8,7 @@
 // Forward: products on the tensor cores (tc_gemm.cuh), queries on the M side, so that a thread holds neighbouring scores of one query and keeps the running maximum and sum of
 // a block of rows by itself; blocks are joined in 64 bits.  lse comes as two floats, of which the second is what the first leaves: a score of a thousand would leave p an error of 2^-14 otherwise.
 //
-// Backward: rows in pieces whose G fits L2 (twice that in 32 bits, where six products read it); for each, G once more from the products, and two products with it.  Rows of up to 256 values of 16 bits
+// Backward: rows in pieces whose G fits L2 (four times as much in 32 bits, where six products read it); for each, G once more from the products, and two products with it.  Rows of up to 256 values of 16 bits
 // keep it on the SM (ce_fused.cuh).  The target's own entry stays out of G: where p is near 1 it is a small
 // difference, and where it is not, it outweighs the rest and so would its rounding to 16 bits; its coefficient g expm1(-loss) + e exp(-loss) is taken in 32 bits, and times the row or the
 // query added to the sums (ce_prepare_kernel, ce_finish_kernel).  Sums of one row's gradient over its queries are taken in ascending order: nothing depends on the order of atomics.
@@ -1059,8 +1059,7 @@ struct CePlan {
         if ((!need_q || fused_q) && (!need_x || fused_x)) return;
         const bool pieces_x = need_x && !fused_x;
         const size_t row_bytes = (size_t)2 * k.planes() * k.m;
-        const size_t space_g = k.planes() * k.planes() / 2 * CE_G_BYTES;  // 32 bits: six products for each read
-        const size_t fit = std::min((space_g ? space_g : CE_G_BYTES) / row_bytes, pieces_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : ~(size_t)0) / CE_BN * CE_BN;
+        const size_t fit = std::min((k.planes() == 3 ? 4 : 1) * CE_G_BYTES / row_bytes, pieces_x ? CE_PARTS_BYTES / ((size_t)4 * k.d) : ~(size_t)0) / CE_BN * CE_BN;
         // the last wave of the products' units full, with as few pieces as that allows
         const size_t most = std::min(std::max<size_t>(fit / CE_BN, 1), tiles_n), wide = pairs(k.m) ? sms / 2 : sms, high = ceil_div(k.m, pairs(k.m) ? 2 * TG_M : TG_M);
         size_t least_time = ~(size_t)0;
