@@ -311,7 +311,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                 const uint32_t from = tmem_s + lanes + b * NB + col0, to = tmem_g + lanes + b * (NB / 2) + col0 / 2;
                 uint32_t r[CW / 32][32];
 #pragma unroll
-                for (int i = 0; i < CW / 32; ++i) tc_ld32(from + i * 32, r[i]);
+                for (int i = 0; i < CW / 32; ++i) tg_ld32(from + i * 32, r[i]);
                 tc_ld_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -367,6 +367,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                                 w[j + 1] ^= (uint32_t)(x.w & (int)0x80000000) | ((uint32_t)x.z >> 31) << 15;
                             }
                         }
+                        if (decltype(checked)::value) __syncwarp();  // all lanes store together
                         tg_store16(to + i * 16, w);
                     }
                 };

@@ -99,7 +99,7 @@ struct CeSums {
 #pragma unroll
                 for (int c0 = 0; c0 < CE_PART; c0 += 16) {
                     uint32_t r[16];
-                    tc_ld16(taddr + c0, r);
+                    tg_ld16(taddr + c0, r);
                     tc_ld_wait();
 #pragma unroll
                     for (int j = 0; j < 16; ++j) f(v[c0 + j], __uint_as_float(r[j]));
@@ -117,8 +117,8 @@ struct CeSums {
             f(v);
         } else {
             uint32_t r[2][32];
-            tc_ld32(taddr, r[0]);
-            tc_ld32(taddr + 32, r[1]);
+            tg_ld32(taddr, r[0]);
+            tg_ld32(taddr + 32, r[1]);
             tc_ld_wait();
             float x[CE_PART];
 #pragma unroll
@@ -331,10 +331,9 @@ __device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, 
     for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) {
         float v[32];
         ce_with_own(a, row, col0 + c0, scale, taddr + c0, live, v);
-        if (row >= a.rows) continue;
 #pragma unroll
         for (int j = 0; j < 32; j += V) {
-            if (col0 + c0 + j >= a.cols) break;
+            if (row >= a.rows || col0 + c0 + j >= a.cols) break;
             if constexpr (sizeof(T) == 4) {
                 *reinterpret_cast<float4*>(o + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             } else {
@@ -394,10 +393,9 @@ struct CeProductPolicy {
                 uint32_t r[32];
                 tg_read(taddr + c0, live, r);
                 if (wide) {
-                    if (row >= a.rows) continue;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        if (c0 + j >= width) break;
+                        if (row >= a.rows || c0 + j >= width) break;
                         float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
                         float4* const o = reinterpret_cast<float4*>(out + c0 + j);
                         if (a.accumulate) {

@@ -140,7 +140,7 @@ struct I8ProductPolicy {
 #pragma unroll
                 for (int c0 = 0; c0 < PER; c0 += 32) {
                     uint32_t r[32];
-                    tc_ld32(taddr + p0 + c0, r);
+                    tg_ld32(taddr + p0 + c0, r);
                     tc_ld_wait();
                     if (p0 + c0 + 32 == PART) done();
                     i8_scores(a.metric, a.small, r, mine, factors + p0 + c0, terms + p0 + c0);
@@ -236,13 +236,12 @@ struct I8FewPolicy {
 #pragma unroll 1
             for (int q0 = 0; q0 < a.nq; q0 += 16) {
                 uint32_t r[16];
-                tc_ld16(taddr + q0, r);
+                tg_ld16(taddr + q0, r);
                 tc_ld_wait();
                 if (q0 + 16 >= a.nq) done();
-                if (at >= a.n) continue;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    if (q0 + j >= a.nq) break;
+                    if (at >= a.n || q0 + j >= a.nq) break;
                     const float v = (float)(int)r[j] * (factors[q0 + j] * mine.x);
                     store_score(o, a.metric == MX_EUCLIDEAN ? fmaf(2.f, v, -terms[q0 + j]) - mine.y : v);
                     o += a.ld;

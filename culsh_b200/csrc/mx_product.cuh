@@ -199,6 +199,7 @@ __device__ __forceinline__ void mx_epilogue_few(const MxProductArgs& a, uint32_t
         OUT* o = reinterpret_cast<OUT*>(a.out) + row;
         for (int q0 = 0; q0 < a.nq; q0 += 16) {
             uint32_t r[16];
+            __syncwarp();  // rows behind the last one have not been stored
             if (live) {  // the same for the warp
                 tc_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + ab * a.acc_cols + q0, r);
                 tc_ld_wait();

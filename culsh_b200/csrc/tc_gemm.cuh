@@ -302,10 +302,19 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     return v;
 }
 
-// 32 columns of an accumulator, NaN where a wait ran out.
+// Columns of an accumulator.  These instructions want all 32 lanes at the same place, and what stands in front may have let some go their own way (rows behind the last one are not stored).
+__device__ __forceinline__ void tg_ld16(uint32_t taddr, uint32_t* r) {
+    __syncwarp();
+    tc_ld16(taddr, r);
+}
+__device__ __forceinline__ void tg_ld32(uint32_t taddr, uint32_t* r) {
+    __syncwarp();
+    tc_ld32(taddr, r);
+}
+// 32 of them, NaN where a wait ran out.
 __device__ __forceinline__ void tg_read(uint32_t taddr, bool live, uint32_t (&r)[32]) {
     if (live) {  // the same for the warp
-        tc_ld32(taddr, r);
+        tg_ld32(taddr, r);
         tc_ld_wait();
     } else {
 #pragma unroll
