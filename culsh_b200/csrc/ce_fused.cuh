@@ -5,7 +5,9 @@
 // both products: K along its rows for the first, across them for the second.  S is made again for the other gradient: 8 m n d operations in place of 6, against 6 bytes of G written and read
 // for each of the m n entries.
 //
-// The factor of a query's entries is a part of its term (log2 of its magnitude) where queries are the columns, and goes to the sums where they are the lanes.
+// The factor of a query's entries is multiplied in where queries are the columns, and goes to the sums where they are the lanes.  It holds what the term, lse in powers of two as one float, leaves
+// behind its last bit (as a part of the term, log2 of its magnitude, it would lose that again: all p of a query off by lse 2^-24, 5e-3 where lse is 1e5).  What is added to a score comes in the order of
+// the losses' pass, the bias first: their difference from lse is then that of the same numbers.
 // One warp loads, one issues the first products and one the second (a single one, issuing 16 MMAs a tile and waiting three times, held them up: 4,096 x 1M x 128 4.12 ms in place of 3.7), two groups of
 // eight warps take the tiles in turn, a thread half the columns of a lane.  S and G have two places each: what an MMA writes over has been read by the epilogue long before, and the tensor pipe has
 // another product to do while a G is made.  (G on top of S, in three places, 4.34 ms: the first product had to wait until the second one in front of it was done.)  dQ of that case takes 1.4 ms, bound
@@ -27,6 +29,8 @@ __device__ __forceinline__ float ce_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+constexpr int CE_HALF_SHIFT = 14;  // p of half precision is held times 2^14, down to 2^-38
 
 // What a power of two brings the largest factor to [2^14, 2^15].
 __device__ __forceinline__ int ce_scale_exponent(const uint32_t* amax) {
@@ -68,9 +72,10 @@ struct CeFusedArgs {
     int d;
     float c;
     const float* bias;        // of the rows, in powers of two, or NULL; in lines of 128
-    const float* terms;       // of the queries: -lse in powers of two, for dX with log2 of the factor's magnitude
+    // of the queries, for dX in lines of 128 with -inf, 0 and -1 behind the last one
+    const float* terms;       // -lse in powers of two, in half precision CE_HALF_SHIFT more
+    const float* factors;
     const int* target_cols;
-    const int* marks;         // of the queries, for dX: target + 1, or 0, and the factor's sign in the highest bit; as `terms` in lines of 128 with -inf and 0 behind the last query
     const uint32_t* amax;
     float* parts;             // sums: [block][own entry][d]; of dX NULL where they are complete
     void* out;                // dX
@@ -90,11 +95,11 @@ struct CeFusedCfg {
     static constexpr int OWN_BYTES = KB * TG_M * 128, OWNS = KB == 1 ? 2 : 1;
     static constexpr int STAGE_BYTES = KB * NB * 128, COLUMN_BYTES = NB * 4, STAGES = KB == 1 ? 8 : KB == 2 ? 5 : 4;
     static constexpr int THREADS = 128 + 32 * WARPS * GROUPS;  // warps for the loads, either product, and one that idles
-// (terms and marks, or the bias, of a stage's entries lie behind the stages)
+    static constexpr int COLUMNS = 3;  // terms, factors and targets, or the bias, of a stage's entries, which lie behind the stages
     // 640 threads are launched with 96 registers each; four warps give up some, which the others take: 128 x 32 + 512 x 112 = 640 x 96
     static constexpr int REGS = 96, FEW_REGS = 32, MANY_REGS = 112;
     static_assert(128 * FEW_REGS + 32 * WARPS * GROUPS * MANY_REGS <= THREADS * REGS, "");
-    static constexpr int SMEM = OWNS * OWN_BYTES + STAGES * (STAGE_BYTES + 2 * COLUMN_BYTES) + 1024 /*barriers*/ + 1024 /*alignment slack*/;
+    static constexpr int SMEM = OWNS * OWN_BYTES + STAGES * (STAGE_BYTES + COLUMNS * COLUMN_BYTES) + 1024 /*barriers*/ + 1024 /*alignment slack*/;
     static_assert(O_COLS + BUFS * (NB + NB / 2) <= 512 && SMEM <= 227 * 1024 && STAGES > BUFS, "");
 };
 
@@ -143,7 +148,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
     unsigned char* const base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(cf_smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* const s_other = base + OWNS * Cfg::OWN_BYTES;
     unsigned char* const s_columns = s_other + STAGES * Cfg::STAGE_BYTES;
-    uint64_t* const own_full = reinterpret_cast<uint64_t*>(s_columns + STAGES * 2 * Cfg::COLUMN_BYTES);
+    uint64_t* const own_full = reinterpret_cast<uint64_t*>(s_columns + STAGES * Cfg::COLUMNS * Cfg::COLUMN_BYTES);
     uint64_t* const own_empty = own_full + OWNS;
     uint64_t* const full = own_empty + OWNS;
     uint64_t* const empty = full + STAGES;
@@ -192,11 +197,12 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                 ++owns;
                 for (int t = 0; t < unit.tiles; ++t) {
                     if (!mbar_wait(&empty[s], parity, s_abort, a.d_error)) { live = false; break; }
-                    unsigned char* const column = s_columns + s * 2 * Cfg::COLUMN_BYTES;
-                    mbar_expect_tx(&full[s], Cfg::STAGE_BYTES + (ROWS ? 2 : BIAS ? 1 : 0) * Cfg::COLUMN_BYTES);
+                    unsigned char* const column = s_columns + s * Cfg::COLUMNS * Cfg::COLUMN_BYTES;
+                    mbar_expect_tx(&full[s], Cfg::STAGE_BYTES + (ROWS ? Cfg::COLUMNS : BIAS ? 1 : 0) * Cfg::COLUMN_BYTES);
                     if (ROWS) {
                         bulk_load(column, a.terms + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
-                        bulk_load(column + Cfg::COLUMN_BYTES, a.marks + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
+                        bulk_load(column + Cfg::COLUMN_BYTES, a.factors + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
+                        bulk_load(column + 2 * Cfg::COLUMN_BYTES, a.target_cols + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
                     } else if (BIAS) {
                         bulk_load(column, a.bias + (int64_t)unit.tile(t) * NB, Cfg::COLUMN_BYTES, &full[s]);
                     }
@@ -264,23 +270,24 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
         constexpr int CW = Cfg::CW;
         const int quarter = warp & 3, group = (warp - 4) / Cfg::WARPS, col0 = (warp - 4) % Cfg::WARPS / 4 * CW;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        // half precision: what brings the largest p (of queries), or p times its factor (of rows), next to 2^15
-        const int exponent = !HALF ? 0 : ROWS ? ce_scale_exponent(a.amax) : 14;
-        const uint64_t cc = f2_pack(a.c, a.c);
+        // dX in half precision: what brings the largest factor next to 2^15
+        const int exponent = HALF && ROWS ? ce_scale_exponent(a.amax) : 0;
+        const float up = ldexpf(1.f, exponent - CE_HALF_SHIFT);
+        const uint64_t cc = f2_pack(a.c, a.c), up2 = f2_pack(up, up);
         bool live = true;
         uint32_t nth = 0, units = 0;
         for (unsigned u = blockIdx.x; u < a.units; u += gridDim.x, ++units) {
             const CeFusedUnit unit(a, u);
             const int first_own = unit.own0 + quarter * 32, mine = first_own + lane;
             const bool in = mine < a.own;
-            float my_term = (float)exponent;
+            float my_term = 0.f;  // of a query, or a row's bias
             int my_target = -1;
             if (in) {
                 if (!ROWS) {
-                    my_term += __ldcg(a.terms + mine);
+                    my_term = __ldcg(a.terms + mine);
                     my_target = __ldcg(a.target_cols + mine);
                 } else if (BIAS) {
-                    my_term += __ldcg(a.bias + mine);
+                    my_term = __ldcg(a.bias + mine);
                 }
             }
             const uint64_t term2 = f2_pack(my_term, my_term);
@@ -288,21 +295,17 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
             for (int t = ahead; t < unit.tiles; t += GROUPS) {
                 const uint32_t n = nth + t, b = n % BUFS;
                 const int first = unit.tile(t) * NB + col0;
-                const float* const columns = reinterpret_cast<const float*>(s_columns + n % STAGES * (2 * Cfg::COLUMN_BYTES)) + col0;
-                const int* const marks = reinterpret_cast<const int*>(columns + NB);
+                const float* const columns = reinterpret_cast<const float*>(s_columns + n % STAGES * (Cfg::COLUMNS * Cfg::COLUMN_BYTES)) + col0;
+                const float* const factors = columns + NB;
+                const int* const targets = reinterpret_cast<const int*>(factors + NB);
                 if ((ROWS || BIAS) && live) live = mbar_wait_warp(&full[n % STAGES], (n / STAGES) & 1u, s_abort, a.d_error);
-                // what is seldom: a target in the warp's part of the tile, the end of the other side; and negative factors
-                bool seldom, negative = false;
+                // what is seldom: a target in the warp's part of the tile, the end of the other side
+                bool seldom;
                 if (ROWS) {
                     bool hit = false;
 #pragma unroll
-                    for (int i = 0; i < CW / 32; ++i) {
-                        const int mark = marks[i * 32 + lane];
-                        hit = hit || (unsigned)((mark & 0x7FFFFFFF) - 1 - first_own) < 32u;
-                        negative = negative || mark < 0;
-                    }
+                    for (int i = 0; i < CW / 32; ++i) hit = hit || (unsigned)(targets[i * 32 + lane] - first_own) < 32u;
                     seldom = __any_sync(0xFFFFFFFFu, hit);
-                    negative = __any_sync(0xFFFFFFFFu, negative);
                 } else {
                     seldom = a.other - first < CW || __any_sync(0xFFFFFFFFu, (unsigned)(my_target - first) < (unsigned)CW);
                 }
@@ -318,28 +321,33 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                 if (lane == 0) mbar_arrive(&s_empty[b]);
                 if (live) live = mbar_wait_warp(&g_empty[b], ((n / BUFS) & 1u) ^ 1u, s_abort, a.d_error);
                 tc_fence_after();
-                auto make = [&](auto checked, auto signed_) {
+                auto make = [&](auto checked) {
 #pragma unroll
                     for (int i = 0; i < CW / 32; ++i) {
                         float v[32];
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
-                            uint64_t t0 = term2, t1 = term2;
-                            if (ROWS || BIAS) {
-                                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(columns + i * 32 + j);
-                                // queries: the exponent of half precision and the row's bias; rows: the query's term
-                                t0 = !ROWS || BIAS || HALF ? f2_add(x.x, term2) : x.x, t1 = !ROWS || BIAS || HALF ? f2_add(x.y, term2) : x.y;
-                            }
-                            t0 = f2_fma(f2_pack(__uint_as_float(r[i][j]), __uint_as_float(r[i][j + 1])), cc, t0);
-                            t1 = f2_fma(f2_pack(__uint_as_float(r[i][j + 2]), __uint_as_float(r[i][j + 3])), cc, t1);
+                            ulonglong2 x = make_ulonglong2(term2, term2);
+                            if (ROWS || BIAS) x = *reinterpret_cast<const ulonglong2*>(columns + i * 32 + j);
+                            // a row's bias, then the query's term
+                            const bool own_first = ROWS && BIAS;
+                            uint64_t t0 = f2_fma(f2_pack(__uint_as_float(r[i][j]), __uint_as_float(r[i][j + 1])), cc, own_first ? term2 : x.x);
+                            uint64_t t1 = f2_fma(f2_pack(__uint_as_float(r[i][j + 2]), __uint_as_float(r[i][j + 3])), cc, own_first ? term2 : x.y);
+                            if (BIAS) t0 = f2_add(t0, own_first ? x.x : term2), t1 = f2_add(t1, own_first ? x.y : term2);
                             f2_unpack(t0, v[j], v[j + 1]);
                             f2_unpack(t1, v[j + 2], v[j + 3]);
 #pragma unroll
                             for (int k = j; k < j + 4; ++k) v[k] = ce_exp2(v[k]);
+                            if (ROWS) {
+                                ulonglong2 f = *reinterpret_cast<const ulonglong2*>(factors + i * 32 + j);
+                                if (HALF) f = make_ulonglong2(f2_mul(f.x, up2), f2_mul(f.y, up2));
+                                f2_unpack(f2_mul(f2_pack(v[j], v[j + 1]), f.x), v[j], v[j + 1]);
+                                f2_unpack(f2_mul(f2_pack(v[j + 2], v[j + 3]), f.y), v[j + 2], v[j + 3]);
+                            }
                         }
                         if (decltype(checked)::value) {
                             if (ROWS) {
-                                const int target = (marks[i * 32 + lane] & 0x7FFFFFFF) - 1 - first_own;
+                                const int target = targets[i * 32 + lane] - first_own;
                                 unsigned hits = __ballot_sync(0xFFFFFFFFu, (unsigned)target < 32u), zero = 0;
                                 while (hits) {  // columns whose target is one of the warp's rows
                                     const int j = __ffs(hits) - 1;
@@ -359,21 +367,12 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                         uint32_t w[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j) w[j] = pack_scores(static_cast<const T*>(nullptr), v[2 * j], v[2 * j + 1]);
-                        if (ROWS && decltype(signed_)::value) {
-#pragma unroll
-                            for (int j = 0; j < 16; j += 2) {
-                                const int4 x = *reinterpret_cast<const int4*>(marks + i * 32 + 2 * j);
-                                w[j] ^= (uint32_t)(x.y & (int)0x80000000) | ((uint32_t)x.x >> 31) << 15;
-                                w[j + 1] ^= (uint32_t)(x.w & (int)0x80000000) | ((uint32_t)x.z >> 31) << 15;
-                            }
-                        }
                         if (decltype(checked)::value) __syncwarp();  // all lanes store together
                         tg_store16(to + i * 16, w);
                     }
                 };
-                if (seldom) make(std::true_type(), std::true_type());
-                else if (negative) make(std::false_type(), std::bool_constant<ROWS>());
-                else make(std::false_type(), std::false_type());
+                if (seldom) make(std::true_type());
+                else make(std::false_type());
                 tg_store_wait();
                 tc_fence_before();
                 __syncwarp();

@@ -43,8 +43,9 @@ struct CeScoreArgs {
     int slots;
     float* target_scores;     // [m]
     // gradient
-    const float* terms;       // [m] what goes to the exponent: -lse
+    const float* terms;       // [m] what goes to the exponent: -lse, plus `shift`
     const float* factors;     // [m] what p is multiplied by
+    int shift;
     const uint32_t* amax;     // largest magnitude among the factors, as bits (half precision only)
     const int* target_cols;   // [m] or -1
     void* G;                  // [planes][m][pitch]
@@ -219,7 +220,7 @@ struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
             term = in ? __ldcg(a.terms + q) : 0.f;
             factor = in ? __ldcg(a.factors + q) : 0.f;
             target = in ? __ldcg(a.target_cols + q) : -1;
-            if (HALF) factor = ldexpf(factor, ce_scale_exponent(a.amax));
+            if (HALF) factor = ldexpf(factor, ce_scale_exponent(a.amax) - a.shift);
         }
         template <typename D>
         __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more, D&& done) {
@@ -230,7 +231,7 @@ struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
             if (idle) return;
             if (!live) factor = __int_as_float(0x7FFFFFFF);
 #pragma unroll
-            for (int j = 0; j < CE_PART; ++j) x[j] = ce_exp2(fmaf(x[j], a.c, BIAS ? term + s_bias[j] : term)) * factor;
+            for (int j = 0; j < CE_PART; ++j) x[j] = ce_exp2(BIAS ? fmaf(x[j], a.c, s_bias[j]) + term : fmaf(x[j], a.c, term)) * factor;  // as in the losses' pass: the bias first
             if (left < CE_PART || __any_sync(0xFFFFFFFFu, (unsigned)at < (unsigned)CE_PART)) {  // seldom; behind the last row G has zeros
 #pragma unroll
                 for (int j = 0; j < CE_PART; ++j)
@@ -550,7 +551,10 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_grad_kernel(const T*
 #pragma unroll
         for (int q = 0; q < M; ++q) {
             float g = 0.f;
-            if (q < m && !masked) g = __ldcg(cols + q) == row ? __ldcg(own + q) : ce_exp2(fmaf(acc[q], c, __ldcg(terms + q) + b)) * __ldcg(factors + q);
+            if (q < m && !masked) {
+                const float term = __ldcg(terms + q);
+                g = __ldcg(cols + q) == row ? __ldcg(own + q) : ce_exp2(BIAS ? fmaf(acc[q], c, b) + term : fmaf(acc[q], c, term)) * __ldcg(factors + q);
+            }
             s_g[threadIdx.x][q] = g;
         }
         const unsigned live = __ballot_sync(0xFFFFFFFFu, !masked);  // a row that is masked may hold anything
@@ -607,8 +611,10 @@ struct CePrepare {
     float* bias2;
     const float *losses, *lse, *lse_low, *grad_losses, *grad_lse;
     const int64_t* targets;
-    float *terms, *log_terms, *factors, *own, *sums;
-    int *marks, *cols, *where;
+    float *terms, *factors, *own, *sums;
+    int *cols, *where;
+    int shift;
+    bool lines;               // terms, factors and cols in lines of 128
     uint32_t* amax;
     const void* Q;
     int64_t ldq;
@@ -716,10 +722,10 @@ __device__ __forceinline__ float ce_own(const CePrepare& a, int q) {
 __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block) {
     const int q = block * 256 + threadIdx.x;
     if (q >= a.m) {
-        if (a.log_terms && q < ((a.m + 127) & ~127)) a.log_terms[q] = -INFINITY, a.marks[q] = 0;
+        if (a.lines && q < ((a.m + 127) & ~127)) a.terms[q] = -INFINITY, a.factors[q] = 0.f, a.cols[q] = -1;
         return;
     }
-    const double two = ((double)a.lse[q] + (double)a.lse_low[q]) * 1.4426950408889634074;
+    const double two = ((double)a.lse[q] + (double)a.lse_low[q]) * 1.4426950408889634074 - (double)a.shift;
     const float high = (float)two;
     const bool none = high == -INFINITY;
     const int t = ce_target(a, q);
@@ -727,10 +733,6 @@ __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block
     a.terms[q] = none ? -INFINITY : -high;
     const float f = (g + e) * (isfinite(high) ? (float)exp2(-(two - (double)high)) : 1.f);
     a.factors[q] = f;
-    if (a.log_terms) {
-        a.log_terms[q] = none ? -INFINITY : (float)(log2((double)fabsf(f)) - (double)high);
-        a.marks[q] = (t + 1) | (f < 0.f ? (int)0x80000000 : 0);
-    }
     a.cols[q] = t;
     a.own[q] = t >= 0 ? ce_own(a, q) : 0.f;
     if (a.amax && isfinite(f)) atomicMax(a.amax, __float_as_uint(fabsf(f)));
@@ -897,7 +899,7 @@ __device__ __forceinline__ void ce_finish_part(const CeFinishArgs& a, const CeFi
     }
     int w = f.which ? __ldcg(f.which + row) : -1;
     float scale = 1.f;
-    if (f.factors) scale = std::is_same<T, __half>::value ? ldexpf(__ldcg(f.factors + row), -14) : __ldcg(f.factors + row);
+    if (f.factors) scale = std::is_same<T, __half>::value ? ldexpf(__ldcg(f.factors + row), -CE_HALF_SHIFT) : __ldcg(f.factors + row);
     else if (a.amax) scale = ldexpf(1.f, -ce_scale_exponent(a.amax));
     const float mine = QUERIES && w >= 0 ? __ldcg(a.own + row) : 0.f;
     struct alignas(V * sizeof(T)) Some { T v[V]; };
@@ -973,8 +975,9 @@ struct CePlan {
     float2* partial = nullptr;
     float* target_scores = nullptr;
     // backward
-    float *terms = nullptr, *log_terms = nullptr, *factors = nullptr, *own = nullptr, *sums = nullptr;
-    int *cols = nullptr, *marks = nullptr, *where = nullptr;
+    float *terms = nullptr, *factors = nullptr, *own = nullptr, *sums = nullptr;
+    int *cols = nullptr, *where = nullptr;
+    int shift = 0;
     int own_splits = 1;
     uint32_t* amax = nullptr;
     int piece = 0;  // rows
@@ -1017,13 +1020,14 @@ struct CePlan {
             target_scores = space.take<float>(k.m);
             return;
         }
-        terms = space.take<float>(k.m), factors = space.take<float>(k.m), own = space.take<float>(k.m);
-        cols = space.take<int>(k.m);
+        const size_t lines = tiles_q * TG_M;
+        terms = space.take<float>(lines), factors = space.take<float>(lines), own = space.take<float>(k.m);
+        cols = space.take<int>(lines);
         if (k.type == CULSH_F16) amax = space.take<uint32_t>(1);
         // G stays on the SM where rows are short enough; sums of more than 32,768 entries would have to be split for dX too
         const bool fused = k.planes() == 1 && k.d <= 256;
         fused_q = need_q && fused, fused_x = need_x && fused && k.m <= 32768;
-        if (fused_x) log_terms = space.take<float>(tiles_q * TG_M), marks = space.take<int>(tiles_q * TG_M);
+        shift = k.type == CULSH_F16 && (fused_q || fused_x) ? CE_HALF_SHIFT : 0;
         if (need_x) {
             sums = space.take<float>((size_t)k.m * k.d);
             // targets of few rows, which many queries share, are summed up for some hundred queries at a time
@@ -1122,7 +1126,8 @@ struct CeOperands {
         job(1, p.x_planes ? planes(k.X, k.ldx, k.n, k.bias, p.x_planes) : 0);
         job(2, p.bias2 ? ceil_div((size_t)k.n + 127, 256) : 0);
         job(3, p.terms ? ceil_div((size_t)k.m + 127, 256) : 0);
-        a.terms = p.terms, a.log_terms = p.log_terms, a.factors = p.factors, a.own = p.own, a.sums = p.sums, a.marks = p.marks, a.cols = p.cols, a.where = p.where, a.amax = p.amax;
+        a.terms = p.terms, a.factors = p.factors, a.own = p.own, a.sums = p.sums, a.cols = p.cols, a.where = p.where, a.amax = p.amax;
+        a.shift = p.shift, a.lines = p.fused_x;
         // rows, and where they are few and long columns, in shares for some CTAs an SM
         const size_t ctas = 2 * (size_t)k.c->sm_count;
         a.own_rows = CePlan::own_rows(k);
@@ -1269,7 +1274,7 @@ inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, vo
     const size_t units = ceil_div(a.tiles_other, a.block) * a.tiles_own;
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
-    a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = ROWS ? p.log_terms : p.terms, a.marks = p.marks, a.amax = p.amax, a.target_cols = p.cols;
+    a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = p.terms, a.factors = p.factors, a.amax = p.amax, a.target_cols = p.cols;
     a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where, a.own_splits = p.own_splits, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
     const CUtensorMap own = ROWS ? ops.map_x(k, TG_M) : ops.map_q(k, TG_M), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
     auto go = [&](auto boxes) {
@@ -1328,7 +1333,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         const int here = (int)std::min<int64_t>(p.piece, k.n - n0);
         const CeTile tile = CePlan::tile_of(k, here);
         CeScoreArgs s = ce_score_args(k, p, tile, (int)n0, (int)(n0 + here));
-        s.terms = p.terms, s.factors = p.factors, s.amax = p.amax, s.target_cols = p.cols, s.G = p.G, s.pitch = p.piece, s.plane = g_plane;
+        s.terms = p.terms, s.factors = p.factors, s.shift = p.shift, s.amax = p.amax, s.target_cols = p.cols, s.G = p.G, s.pitch = p.piece, s.plane = g_plane;
         s.block = 1;
         const size_t units = (size_t)s.tiles_n * s.tiles_q;
         if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);

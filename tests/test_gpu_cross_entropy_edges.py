@@ -1,0 +1,63 @@
+"""Cross entropy where a rounding in the wrong place shows: lse of tens of thousands, temperatures near either end, long rows, very many queries."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+LEAST = {torch.float32: 2.0 ** -140, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -130}
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def culsh():
+    import culsh_b200
+    return culsh_b200
+
+
+def gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("m,d", [(16, 64), (20, 64), (20, 128), (20, 256), (20, 300), (20, 700)])
+@pytest.mark.parametrize("far", [40, 256, -256])
+def test_gradients_do_not_go_with_the_rounding_of_lse(culsh, far, m, d, bias, dtype):
+    """Scores of whole numbers of up to 65,548, exact in every type, times log2(e) / T = c, which is a float and no power of two: lse is next to no float (its last bit is up to 2^-7).  Columns of
+    the gradients are single entries of G: dX[j, 1 + i] and dQ[i, 1 + m + j].
+
+    p is exp2 of a difference that is exact (of no bias: rounded once), off by 2^-22, by a factor that is rounded once, and lse's sum by 24 additions and exponentials of 2^-22: 2^-19 together.
+    G is rounded to its type, and the result: half a unit each."""
+    n, c = 24, float(np.float32(1.371))
+    t = 1.4426950408889634 / c
+    Q, X = torch.zeros(m, d, device="cuda"), torch.zeros(n, d, device="cuda")
+    Q[:, 0], X[:, 0] = far, 256
+    i, j = torch.arange(m, device="cuda"), torch.arange(n, device="cuda")
+    Q[:, 1 + m:1 + m + n] = torch.randint(-3, 4, (m, n), generator=gen(1), device="cuda").float()
+    X[:, 1:1 + m] = torch.randint(-3, 4, (n, m), generator=gen(2), device="cuda").float()
+    Q[i, 1 + i], X[j, 1 + m + j] = 1, 1
+    Q, X = Q.to(dtype), X.to(dtype)
+    targets = torch.randint(0, n, (m,), generator=gen(3), device="cuda")
+    targets[::3] = -1
+    b = 0.5 * torch.randn(n, generator=gen(4), device="cuda") if bias else None
+    two = Q.double() @ X.double().T * c
+    if bias:  # exponents are floats
+        two = (two + (b * np.float32(1.4426950408889634)).double()).float().double()
+    p = torch.softmax(two * np.log(2.0), 1)
+    g, e = torch.randn(m, generator=gen(5), device="cuda"), 1 + torch.rand(m, generator=gen(6), device="cuda")
+    real = targets >= 0
+    gg = torch.where(real, g.double(), 0.0)
+    G = p * (gg + e.double())[:, None]
+    G[i[real], targets[real]] -= gg[real]
+    r = culsh.cross_entropy(Q, X, targets, b, temperature=t)
+    dq, dx = culsh.cross_entropy_backward(Q, X, targets, r, g, e, b, temperature=t)
+    size = p * (gg.abs() + e.double())[:, None]
+    size[i[real], targets[real]] += gg.abs()[real]
+    # a target's loss is rounded: its p by |loss| 2^-24
+    err = 2 * HALF[dtype] + HALF[dtype] ** 2 + 2.0 ** -19 + 40 * 2.0 ** -24
+    tol = (err * size + 4 * 2.0 ** -39) / t + LEAST[dtype]
+    for out in (dq[i[:, None], 1 + m + j[None, :]], dx[j[None, :], 1 + i[:, None]]):
+        off = (out.double() - G / t).abs() - tol
+        assert float(off.max()) <= 0, (float(off.max()), float(((out.double() * t - G).abs() / size).max()))
