@@ -61,3 +61,24 @@ def test_gradients_do_not_go_with_the_rounding_of_lse(culsh, far, m, d, bias, dt
     for out in (dq[i[:, None], 1 + m + j[None, :]], dx[j[None, :], 1 + i[:, None]]):
         off = (out.double() - G / t).abs() - tol
         assert float(off.max()) <= 0, (float(off.max()), float(((out.double() * t - G).abs() / size).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [128, 300])
+def test_gradients_of_16_bits_are_off_by_the_rounding_of_the_result(culsh, d, dtype):
+    """G is rounded to 16 bits: what that leaves in a sum is at most half a unit of the root of its terms' squares (independent roundings), beside the result's rounding, and sums in 32 bits."""
+    m, n, t = 1_000, 20_000, 0.05
+    X = torch.nn.functional.normalize(torch.randn(n, d, generator=gen(), device="cuda"))
+    targets = torch.randint(0, n, (m,), generator=gen(1), device="cuda")
+    Q = torch.nn.functional.normalize(X[targets] + torch.randn(m, d, generator=gen(2), device="cuda") * (2.5 / d ** 0.5)).to(dtype)
+    X, g, e = X.to(dtype), 1 + 0.2 * torch.randn(m, generator=gen(3), device="cuda"), 0.01 * torch.randn(m, generator=gen(4), device="cuda")
+    r = culsh.cross_entropy(Q, X, targets, temperature=t)
+    out = culsh.cross_entropy_backward(Q, X, targets, r, g, e, temperature=t)
+    P = torch.softmax(Q.double() @ X.double().T / t, 1) * (g + e).double()[:, None]
+    G = P.scatter_add(1, targets[:, None], -g.double()[:, None])
+    P.scatter_(1, targets[:, None], 0.0)
+    for got, want, rest in ((out[0], G @ X.double() / t, (P ** 2 @ X.double() ** 2).sqrt() / t), (out[1], G.T @ Q.double() / t, ((P ** 2).T @ Q.double() ** 2).sqrt() / t)):
+        once = (want.to(dtype).double() - want).norm()
+        assert float((got.double() - want).norm()) <= float(once + HALF[dtype] * rest.norm() + 2.0 ** -20 * want.norm())
+    again = culsh.cross_entropy_backward(Q, X, targets, r, g, e, temperature=t)
+    assert all(torch.equal(a, b) for a, b in zip(out, again))
