@@ -27,7 +27,10 @@
 namespace culsh_b200 {
 
 constexpr int CE_BN = 256, CE_PART = CE_BN / 4;  // columns of a tile, and of it for a warp
-constexpr int CE_SEGMENT = 8;  // steps of 64
+// Steps of 64 in a segment of K (tc_gemm.cuh), and in one of the gradient's scores of 16-bit rows: 128 adds, which cut off 8e-6 of a score at most.  That makes p smaller than the losses' pass has it, by
+// 3e-4 of it where scores are 40 (half a unit of float16 is 4.9e-4); in one sum over 65,536 values it would be 1.3e-2.  By segments of 16 that is halved and 4,099 x 32,771 x 2,048 float16 takes 1.60 ms
+// in place of 1.47, by the losses' own 1.75; 4,099 x 16,000 x 4,096 in one sum 1.49, by 32 1.55, by 16 1.62.
+constexpr int CE_SEGMENT = 8, CE_SEGMENT_16 = 32;
 
 struct CeScoreArgs {
     int* d_error;
@@ -67,10 +70,10 @@ struct CeUnit {
 
 // Tiles of 256 rows, of a CTA or of a pair of them, and of 64 where those would leave most SMs idle.
 enum CeTile : int { CE_ONE = 0, CE_PAIR = 1, CE_SMALL = 2 };
-template <int PLANES, bool SEGMENTS, int TILE>
+template <int PLANES, int SEGMENTS, int TILE>
 struct CeScoreBase {
     static constexpr bool A_MN = false, B_MN = false, I8 = false, PARTS = true, PAIR = TILE == CE_PAIR;
-    static constexpr int BN = TILE == CE_SMALL ? CE_PART : CE_BN, SEGMENT = SEGMENTS ? CE_SEGMENT : 0, EPI_WARPS = BN / 16;
+    static constexpr int BN = TILE == CE_SMALL ? CE_PART : CE_BN, SEGMENT = SEGMENTS, EPI_WARPS = BN / 16;
     static constexpr int EPI_BYTES = EPI_WARPS * CE_PART * 4;
     using Pairs = PlanePairs<PLANES>;
     using Args = CeScoreArgs;
@@ -135,8 +138,8 @@ struct CeSums {
 // that has but one row is exactly 0.  Of a batch, bound by the exponentials, 16 a cycle and SM: 4,096 x
 // 1M x 128 bfloat16 1.29 ms, their unit busy for 80 %, the tensor pipe for 39.  (Eight warps in place of sixteen 2.0 ms; an arrival that releases to the cluster, for each tile of each warp, 1.9.)
 template <int PLANES, bool BIAS, bool SEGMENTS, int TILE>
-struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
-    static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
+struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
+    static constexpr int BN = CeScoreBase<PLANES, 0, TILE>::BN;
     struct Epilogue : CeSums<SEGMENTS> {
         int q, quarter, group, lane, rank, target;
         bool idle;
@@ -206,8 +209,8 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
 
 // G of a piece, 128 neighbouring bytes of a query to a thread.  4,099 x 6,656 x 2,048 float16 82 us, 1,355 TFLOP/s.
 template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS, int TILE>
-struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
-    static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
+struct CeGradPolicy : CeScoreBase<PLANES, !SEGMENTS ? 0 : PLANES == 1 ? CE_SEGMENT_16 : CE_SEGMENT, TILE> {
+    static constexpr int BN = CeScoreBase<PLANES, 0, TILE>::BN;
     struct Epilogue : CeSums<SEGMENTS> {
         int q, quarter, group, lane, rank, target;
         bool idle;
@@ -1342,10 +1345,9 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         s.units = (unsigned)units;
         const CUtensorMap tx = ops.map_x(k, ce_box_x(tile));
         ce_by([&](auto planes, auto bias, auto segs, auto type) {
-            // 16-bit results are none the worse for the segments' sums being one
-            if constexpr (decltype(planes)::value == PLANES && (PLANES == 3 || !decltype(segs)::value))
+            if constexpr (decltype(planes)::value == PLANES)
                 tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value, decltype(type)::value>>(k.c, tq, tx, s, k.stream);
-        }, PLANES == 3, k.bias != nullptr, PLANES == 3 && s.kb > CE_SEGMENT, tile);
+        }, PLANES == 3, k.bias != nullptr, s.kb > (PLANES == 1 ? CE_SEGMENT_16 : CE_SEGMENT), tile);
         const int64_t g_cols = (int64_t)s.tiles_n * CePlan::tile_rows(tile);  // behind the last row G has zeros
         if (pieces_x) {
             CeProductArgs a{};

@@ -82,3 +82,34 @@ def test_gradients_of_16_bits_are_off_by_the_rounding_of_the_result(culsh, d, dt
         assert float((got.double() - want).norm()) <= float(once + HALF[dtype] * rest.norm() + 2.0 ** -20 * want.norm())
     again = culsh.cross_entropy_backward(Q, X, targets, r, g, e, temperature=t)
     assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [700, 2_048, 16_384, 65_536])
+def test_p_of_long_rows_sum_up_to_1(culsh, d, dtype):
+    """Scores of about 40 from positive products, of which accumulators cut off something at every step: in one sum over K a score of 65,536 products would be 3e-4 of itself smaller than in the
+    losses' segments of 512, and all p with it 1e-2.  Columns of the gradients are single entries of G, as above.
+
+    A query's G, half a unit of rounding each and half a unit of the results, sum up to the gradient of lse, but for what longer segments of 16 bits cut off: 128 adds of 2^-23, from one sum on where
+    the losses' pass has several.  Each entry: the losses' segments of 32 adds and their sum's roundings, twice, and that."""
+    m, n = 20, 24
+    Q, X = 0.5 + torch.rand(m, d, generator=gen(1), device="cuda"), 0.5 + torch.rand(n, d, generator=gen(2), device="cuda")
+    i, j = torch.arange(m, device="cuda"), torch.arange(n, device="cuda")
+    Q[:, :m + n], X[:, :m + n] = 0, 0
+    Q[i, i], X[j, m + j] = 16, 16
+    Q, X = Q.to(dtype), X.to(dtype)
+    t = float((Q.double() @ X.double().T).mean()) / 40
+    e, targets = 1 + torch.rand(m, generator=gen(3), device="cuda"), torch.full((m,), -1, device="cuda")
+    r = culsh.cross_entropy(Q, X, targets, temperature=t)
+    dq, dx = culsh.cross_entropy_backward(Q, X, targets, r, None, e, temperature=t)
+    z = Q.double() @ X.double().T / t
+    want = torch.softmax(z, 1) * e.double()[:, None]
+    score = float(z.max()) * (33 * 2.0 ** -23 + d / 512 * 2.0 ** -24) + 2.0 ** -20
+    assert float((r.lse.double() - torch.logsumexp(z, 1)).abs().max()) <= score + 2.0 ** -24 * float(r.lse.max())
+    err = 2 * HALF[dtype] + HALF[dtype] ** 2 + 2.0 ** -18
+    if dtype != torch.float32 and d > 512:
+        err += float(z.max()) * (min(d, 2048) / 16 * 2.0 ** -23 + d // 2048 * 2.0 ** -24)
+    for out in (dq[:, m:m + n], dx[:, :m].T):
+        G = out.double() * t / 16
+        assert float((G.sum(1) / e.double() - 1).abs().max()) <= err
+        assert float((G / want - 1).abs().max()) <= 2 * score + err
