@@ -13,9 +13,23 @@ __device__ __forceinline__ float2 i8_terms(int metric, float scale, int squares)
     if (metric == MX_COSINE) return make_float2(squares > 0 ? __frsqrt_rn((float)squares) : squares == 0 ? 0.f : __int_as_float(0x7FFFFFFF), 0.f);
     return make_float2(scale, metric == MX_EUCLIDEAN ? (float)squares * (scale * scale) : 0.f);
 }
-__device__ __forceinline__ float i8_score(int metric, int dot, float2 q, float2 x) {
-    const float v = (float)dot * (q.x * x.x);
-    return metric == MX_EUCLIDEAN ? fmaf(2.f, v, -q.y) - x.y : v;
+// Products of two scales, squares of one and sums by them are floats where scales are from 2^-62 to 2^46 (a row of zeros may have any): 2^-124 to 2^123.  Elsewhere they may leave the range that the
+// score itself is in, and are taken in parts.
+__device__ __forceinline__ bool i8_far(int metric, float scale, int squares) {
+    return metric != MX_COSINE && squares != 0 && __float_as_uint(scale) - __float_as_uint(0x1p-62f) >= __float_as_uint(0x1p46f) - __float_as_uint(0x1p-62f);  // as floats are in their bits' order
+}
+__device__ __forceinline__ int i8_exponent(float scale) { return (__float_as_int(scale) >> 23 & 255) - 127; }
+__device__ __forceinline__ float i8_power(int e) { return __int_as_float((e + 127) << 23); }
+// Each scale as two of half its exponent; distances by scales over the larger one's power of two.
+__device__ __forceinline__ float i8_score_far(int metric, int dot, float q_scale, float q_squares, float x_scale, float x_squares) {
+    const int eq = i8_exponent(q_scale), ex = i8_exponent(x_scale);
+    if (metric == MX_EUCLIDEAN) {
+        const int e = min(max(eq, ex), 126);
+        const float q = q_scale * i8_power(-e), x = x_scale * i8_power(-e);
+        return (fmaf(2.f, (float)dot * (q * x), -(q_squares * (q * q))) - x_squares * (x * x)) * i8_power(e) * i8_power(e);
+    }
+    const int hq = eq >> 1, hx = ex >> 1;
+    return (float)dot * (q_scale * i8_power(-hq) * (x_scale * i8_power(-hx))) * (i8_power(hq) * i8_power(hx));
 }
 
 struct I8ProductArgs {
@@ -53,7 +67,17 @@ struct I8Fetch {
         scale = in ? __ldcg(scales + at) : 0.f;
         squares = in ? __ldcg(from + at) : 0;
     }
+    __device__ __forceinline__ bool far(int metric) const { return i8_far(metric, scale, squares); }
+    // What a score takes, and a far one.
+    __device__ __forceinline__ float2 terms(int metric) const { return i8_terms(metric, scale, squares); }
+    __device__ __forceinline__ float2 far_terms() const { return make_float2(scale, (float)squares); }
 };
+__device__ __forceinline__ float i8_score(int metric, int dot, const I8Fetch& q, const I8Fetch& x) {
+    if (q.far(metric) || x.far(metric)) return i8_score_far(metric, dot, q.scale, (float)q.squares, x.scale, (float)x.squares);
+    const float2 qt = q.terms(metric), xt = x.terms(metric);
+    const float v = (float)dot * (qt.x * xt.x);
+    return metric == MX_EUCLIDEAN ? fmaf(2.f, v, -qt.y) - xt.y : v;
+}
 // The scores of N sums; conversions of whole numbers run at an eighth of the rate of additions, which do the same for what fits the fraction of a float.
 template <int N>
 __device__ __forceinline__ void i8_scores(int metric, bool small, uint32_t (&r)[N], float2 q, const float* factors, const float* terms) {
@@ -79,6 +103,22 @@ __device__ __forceinline__ void i8_scores(int metric, bool small, uint32_t (&r)[
 #pragma unroll
         for (int j = 0; j < N; ++j) r[j] = __float_as_uint(fmaf(2.f, __uint_as_float(r[j]), -q.y) - terms[j]);
     }
+}
+
+// A lane's `columns` scores of a tile with far ones, the first `left` of them stored `step` entries apart.  Seldom taken, and apart: in the loop of the others its registers made
+// 1,000 x 1M x 128 take 642 to 770 us in place of 623.
+template <typename OUT>
+__device__ __noinline__ void i8_store_far(int metric, uint32_t taddr, int columns, int left, float2 mine, const float* factors, const float* squares, OUT* out, int64_t step) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < columns; c0 += 16) {
+        uint32_t r[16];
+        tg_ld16(taddr + c0, r);
+        tc_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (c0 + j < left) store_score(out + (c0 + j) * step, i8_score_far(metric, (int)r[j], mine.x, mine.y, factors[c0 + j], squares[c0 + j]));
+    }
+    __syncwarp();
 }
 
 // More than 64 queries: they are the M side, a lane of the accumulator a query.  Short rows leave the time to the epilogue: a warp has 32 queries by all 128 rows of a tile, and groups of four
@@ -121,13 +161,24 @@ struct I8ProductPolicy {
         __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
             constexpr int PER = 128 / sizeof(OUT), V = 16 / sizeof(OUT);  // scores of a query in a piece, in a store
             const int q0 = first_query(u), n0 = first_row(u);
-            float2 mine = i8_terms(a.metric, query.scale, query.squares);
-            if (!live) mine.x = __int_as_float(0x7FFFFFFF);
+            float2 mine = query.terms(a.metric);
+            bool far = query.far(a.metric);
 #pragma unroll
             for (int i = 0; i < PART / 32; ++i) {
-                const float2 x = i8_terms(a.metric, row[i].scale, row[i].squares);
+                const float2 x = row[i].terms(a.metric);
                 factors[i * 32 + lane] = x.x, terms[i * 32 + lane] = x.y;
+                far = far || row[i].far(a.metric);
             }
+            far = __any_sync(0xFFFFFFFFu, far);
+            if (far) {
+                mine = query.far_terms();
+#pragma unroll
+                for (int i = 0; i < PART / 32; ++i) {
+                    const float2 x = row[i].far_terms();
+                    factors[i * 32 + lane] = x.x, terms[i * 32 + lane] = x.y;
+                }
+            }
+            if (!live) mine.x = __int_as_float(0x7FFFFFFF);
             __syncwarp();
             if (a.units - u.u > TURNS * a.step) fetch(a, Unit(a, u.u + TURNS * a.step));  // on its way while this unit is worked on
             if (q0 >= a.nq || n0 >= a.n) {
@@ -135,6 +186,11 @@ struct I8ProductPolicy {
                 return;
             }
             OUT* const o = reinterpret_cast<OUT*>(a.out) + (int64_t)q0 * a.ld + n0;
+            if (far) {
+                i8_store_far(a.metric, taddr, PART, q0 + lane < a.nq ? a.n - n0 : 0, mine, factors, terms, o + lane * a.ld, 1);
+                done();
+                return;
+            }
 #pragma unroll 1
             for (int p0 = 0; p0 < PART; p0 += PER) {
 #pragma unroll
@@ -207,18 +263,20 @@ struct I8FewPolicy {
     static __device__ __forceinline__ int n_mma(const Args& a, const Unit&, int) { return (a.nq + 15) & ~15; }
     struct Epilogue {
         int quarter, group, lane;
-        float *factors, *terms;  // of the queries, the same for all warps
+        float *factors, *terms, *squares;  // of the queries, the same for all warps
+        bool far = false;                  // one of them is
         I8Fetch row;
         __device__ __forceinline__ Epilogue(const Args& a, unsigned char* smem, int, int quarter_, int group_, int lane_, int)
-            : quarter(quarter_), group(group_), lane(lane_), factors(reinterpret_cast<float*>(smem)), terms(factors + I8_FEW) {
+            : quarter(quarter_), group(group_), lane(lane_), factors(reinterpret_cast<float*>(smem)), terms(factors + I8_FEW), squares(terms + I8_FEW) {
 #pragma unroll
             for (int i = lane; i < I8_FEW; i += 32) {
                 I8Fetch f;
                 f.get(a.q_scales, a.q_squares, i, a.nq);
                 const float2 q = i8_terms(a.metric, f.scale, f.squares);
-                factors[i] = q.x, terms[i] = q.y;
+                factors[i] = q.x, terms[i] = q.y, squares[i] = (float)f.squares;
+                far = far || f.far(a.metric);
             }
-            __syncwarp();
+            far = __any_sync(0xFFFFFFFFu, far);
             // the groups take the CTA's units in turn
             const unsigned first = blockIdx.x + group * a.step;
             if (first < a.units) row.get(a.scales, a.squares, (int)first * TG_M + quarter * 32 + lane, a.n);
@@ -228,11 +286,17 @@ struct I8FewPolicy {
         template <typename D>
         __device__ __forceinline__ void tile(const Args& a, const Unit& u, int, uint32_t taddr, bool live, bool, D&& done) {
             const int at = (int)u.u * TG_M + quarter * 32 + lane;
-            float2 mine = i8_terms(a.metric, row.scale, row.squares);
+            const bool some_far = far || __any_sync(0xFFFFFFFFu, row.far(a.metric));
+            float2 mine = some_far ? row.far_terms() : row.terms(a.metric);
             if (!live) mine.x = __int_as_float(0x7FFFFFFF);
             const uint64_t next = (uint64_t)u.u + 2ull * a.step;
             if (next < a.units) row.get(a.scales, a.squares, (int)next * TG_M + quarter * 32 + lane, a.n);
             OUT* o = reinterpret_cast<OUT*>(a.out) + at;
+            if (some_far) {
+                i8_store_far(a.metric, taddr, a.nq, at < a.n ? a.nq : 0, mine, factors, squares, o, a.ld);
+                done();
+                return;
+            }
 #pragma unroll 1
             for (int q0 = 0; q0 < a.nq; q0 += 16) {
                 uint32_t r[16];
@@ -306,8 +370,10 @@ __global__ void __launch_bounds__(256) i8_score_kernel(I8ScoreArgs a, KernelBefo
             if (mine_in) held = __ldcg(reinterpret_cast<const uint4*>(a.q_codes + (int64_t)list * a.pitch + column));
             held_list = list;
         }
-        float score = __int_as_float(0x7FFFFFFF);
-        const float2 q = i8_terms(a.metric, __ldcg(a.q_scales + owner), __ldcg(a.q_squares + owner)), x = i8_terms(a.metric, scale, squares);
+        I8Fetch q, x;
+        q.scale = __ldcg(a.q_scales + owner), q.squares = __ldcg(a.q_squares + owner);
+        x.scale = scale, x.squares = a.metric == MX_DOT ? 1 : squares;  // as if no row were zeros
+        int mine = 0;
 #pragma unroll 1
         for (int i0 = 0; i0 < LANES; i0 += AHEAD) {
             int dot[AHEAD];
@@ -348,10 +414,10 @@ __global__ void __launch_bounds__(256) i8_score_kernel(I8ScoreArgs a, KernelBefo
 #pragma unroll
                 for (int o = 1; o < LANES; o *= 2) dot[i] += __shfl_xor_sync(0xFFFFFFFFu, dot[i], o);
                 const int sum = __shfl_sync(0xFFFFFFFFu, dot[i], (lane % GROUPS) * LANES);
-                if (lane / GROUPS == i0 + i && real) score = i8_score(a.metric, sum, q, x);
+                if (lane / GROUPS == i0 + i) mine = sum;
             }
         }
-        if (in) a.out[c] = score;
+        if (in) a.out[c] = real ? i8_score(a.metric, mine, q, x) : __int_as_float(0x7FFFFFFF);
     }
 }
 
