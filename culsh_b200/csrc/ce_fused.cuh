@@ -38,6 +38,9 @@ __device__ __forceinline__ int ce_scale_exponent(const uint32_t* amax) {
     return bits == 0u ? 0 : min(max(14 + 127 - (int)(bits >> 23), -100), 100);
 }
 
+// 1 / T back by it, no infinity: a sum of 0 stays 0.
+__device__ __forceinline__ float ce_scale_back(float inv_t, int exponent) { return fminf(ldexpf(inv_t, -exponent), 0x1.fffffep127f); }
+
 // 32 rows of 32 values, a row to a lane, turned: lane i gets column i, v[j] that of row j.
 __device__ __forceinline__ void ce_turn(float (&v)[32], int lane) {
 #pragma unroll
@@ -392,7 +395,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
                 if (typed) {
-                    const float scale = HALF ? ldexpf(a.inv_t, -exponent) : a.inv_t;
+                    const float scale = HALF ? ce_scale_back(a.inv_t, exponent) : a.inv_t;
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] *= scale;
                     ce_add_own(v, a.where + mine, a.own, in ? a.own_splits : 0, a.sums, a.d, c0, a.inv_t);

@@ -19,6 +19,7 @@
 // largest coefficient to 2^15, so that p down to 2^-39 of it is there.
 #pragma once
 
+#include <cmath>
 #include <type_traits>
 
 #include "ce_fused.cuh"
@@ -44,6 +45,7 @@ struct CeScoreArgs {
     const float* bias;        // of the rows, in powers of two, or NULL
     const int64_t* targets;   // (forward) of the queries, or -1
     // forward
+    float down;               // what scores are multiplied by where their differences may not be floats (c is as much larger)
     float2* partial;          // [m][slots]: reference and sum
     int slots;
     float* target_scores;     // [m]
@@ -181,6 +183,10 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
             this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
             done();
             if (idle) return;
+            if (!BIAS && a.down != 1.f) {
+#pragma unroll
+                for (int j = 0; j < CE_PART; ++j) x[j] *= a.down;
+            }
             if (left < CE_PART || __any_sync(0xFFFFFFFFu, (unsigned)at < (unsigned)CE_PART)) {  // seldom
                 float v = 0.f;
 #pragma unroll
@@ -327,7 +333,7 @@ __device__ __noinline__ void ce_store_turned(const CeProductArgs& a, int row, in
 template <typename T, int N>
 __device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, int lane, int col0, uint32_t taddr, bool live) {
     constexpr int V = 16 / sizeof(T);
-    const float scale = ldexpf(a.inv_t, std::is_same<T, __half>::value ? -ce_scale_exponent(a.amax) : 0);
+    const float scale = std::is_same<T, __half>::value ? ce_scale_back(a.inv_t, ce_scale_exponent(a.amax)) : a.inv_t;
     if (a.cols % V != 0 || a.ld % V != 0 || ((uintptr_t)a.typed & 15) != 0) {  // no 16 bytes of a row lie together: rows turned, so that neighbouring lanes have neighbouring columns
         for (int c0 = 0; c0 < N && col0 + c0 < a.cols; c0 += 32) ce_store_turned<T>(a, row, lane, col0 + c0, scale, taddr + c0, live);
         return;
@@ -436,7 +442,7 @@ constexpr int CE_FEW_LOSS = 1024, CE_FEW_GRAD = 192;  // queries by columns; col
 constexpr int CE_FEW = 16, CE_FEW_COLS = 32, CE_FEW_THREADS = 256;
 template <int M, bool BIAS>
 __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* __restrict__ Q, int64_t ldq, const float* __restrict__ X, int64_t ldx, int m, int n, int d,
-                                                                const float* __restrict__ bias, float c, const int64_t* __restrict__ targets, float2* __restrict__ partial,
+                                                                const float* __restrict__ bias, float c, float down, const int64_t* __restrict__ targets, float2* __restrict__ partial,
                                                                 float* __restrict__ target_scores, KernelBefore before) {
     behind_kernel_before(Q, X, bias, targets, partial, target_scores, before);
     __shared__ float s_x[CE_FEW_COLS][CE_FEW_THREADS + 1];
@@ -481,6 +487,7 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
             const float b = BIAS ? __ldcg(bias + row) * CE_LOG2E : 0.f;
 #pragma unroll
             for (int q = 0; q < M; ++q) {
+                if (!BIAS) acc[q] *= down;
                 if (target[q] == row) target_scores[q] = acc[q];
                 const float z = !BIAS ? acc[q] : b == -INFINITY ? b : fmaf(acc[q], c, b), next = fmaxf(ref[q], z), base = next == -INFINITY ? 0.f : next;
                 sum[q] = fmaf(sum[q], ce_exp2((ref[q] - base) * by), ce_exp2((z - base) * by));
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_grad_kernel(const T*
             const int col = c0 + lane;
             float q_of[M], sum[M] = {};
 #pragma unroll
-            for (int q = 0; q < M; ++q) q_of[q] = dX && q < m && col < d ? ce_float(__ldcg(Q + q * ldq + col)) * inv_t : 0.f;
+            for (int q = 0; q < M; ++q) q_of[q] = dX && q < m && col < d ? ce_float(__ldcg(Q + q * ldq + col)) : 0.f;
             __syncwarp();
 #pragma unroll 4
             for (int j = 0; j < 32; ++j) {
@@ -580,7 +587,7 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_grad_kernel(const T*
                     sum[q] = fmaf(g, x, sum[q]);
                     out = fmaf(g, q_of[q], out);
                 }
-                if (dX && at < n && col < d) dX[at * ldo + col] = (T)out;
+                if (dX && at < n && col < d) dX[at * ldo + col] = (T)(out * inv_t);
             }
             if (parts) {
                 __syncthreads();
@@ -618,7 +625,7 @@ struct CePrepare {
     const int64_t* targets;
     float *terms, *factors, *own, *sums;
     int *cols, *where;
-    int shift;
+    int shift, t_shift;
     bool lines;               // terms, factors and cols in lines of 128
     uint32_t* amax;
     const void* Q;
@@ -722,7 +729,7 @@ __device__ __forceinline__ int ce_target(const CePrepare& a, int q) {
 }
 __device__ __forceinline__ float ce_own(const CePrepare& a, int q) {
     const float loss = a.losses[q], g = a.grad_losses ? a.grad_losses[q] : 0.f, e = a.grad_lse ? a.grad_lse[q] : 0.f;
-    return g * expm1f(-loss) + e * expf(-loss);
+    return ldexpf(g * expm1f(-loss) + e * expf(-loss), -a.t_shift);
 }
 __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block) {
     const int q = block * 256 + threadIdx.x;
@@ -736,7 +743,7 @@ __device__ __forceinline__ void ce_terms_part(const CePrepare& a, unsigned block
     const int t = ce_target(a, q);
     const float g = t >= 0 && a.grad_losses ? a.grad_losses[q] : 0.f, e = a.grad_lse ? a.grad_lse[q] : 0.f;
     a.terms[q] = none ? -INFINITY : -high;
-    const float f = (g + e) * (isfinite(high) ? (float)exp2(-(two - (double)high)) : 1.f);
+    const float f = ldexpf((g + e) * (isfinite(high) ? (float)exp2(-(two - (double)high)) : 1.f), -a.t_shift);
     a.factors[q] = f;
     a.cols[q] = t;
     a.own[q] = t >= 0 ? ce_own(a, q) : 0.f;
@@ -952,7 +959,13 @@ struct CeCall {
     int pitch() const { return (d + 7) & ~7; }
     bool copies(const void* p, int64_t ld) const { return type == CULSH_F32 || !aligned16(p, ld * 2); }
     TgType tg() const { return type == CULSH_F16 ? TG_F16 : TG_BF16; }
-    float c2() const { return (float)(1.4426950408889634 / temperature); }
+    // The losses take differences of scores, without a bias.  They may be beyond float32, and by temperatures beyond 2^100 small again: scores are multiplied by it first then.
+    float down() const { return !bias && temperature > 0x1p100 ? 0x1p-64f : 1.f; }
+    // Not 0, by which an infinity would be no number: of a temperature beyond 2^149 scores make no difference (at most 2^128 2^-149).
+    float c2() const { return std::max((float)(1.4426950408889634 / temperature), 0x1p-149f); }
+    // 1 / T as a float of all its bits, times a power of two that the queries' coefficients are less by.
+    int t_shift() const { return temperature > 0x1p126 ? std::ilogb(temperature) - 125 : 0; }
+    float inv_t() const { return (float)std::ldexp(1 / temperature, t_shift()); }
 };
 
 // Pieces of the workspace, each at a multiple of 256 bytes.
@@ -1132,7 +1145,7 @@ struct CeOperands {
         job(2, p.bias2 ? ceil_div((size_t)k.n + 127, 256) : 0);
         job(3, p.terms ? ceil_div((size_t)k.m + 127, 256) : 0);
         a.terms = p.terms, a.factors = p.factors, a.own = p.own, a.sums = p.sums, a.cols = p.cols, a.where = p.where, a.amax = p.amax;
-        a.shift = p.shift, a.lines = p.fused_x;
+        a.shift = p.shift, a.t_shift = k.t_shift(), a.lines = p.fused_x;
         // rows, and where they are few and long columns, in shares for some CTAs an SM
         const size_t ctas = 2 * (size_t)k.c->sm_count;
         a.own_rows = CePlan::own_rows(k);
@@ -1187,12 +1200,13 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     const CePlan p(k, false, false, false, workspace);
     const CeOperands ops(k, p, CePrepare{});
     CeScoreArgs a = ce_score_args(k, p, p.tile, 0, k.n);
+    a.down = k.down(), a.c /= a.down;
     if (p.few) {
         auto go = [&](auto queries) {
             constexpr int M = decltype(queries)::value;
             auto kern = k.bias ? ce_few_kernel<M, true> : ce_few_kernel<M, false>;
             launch_next(k.stream, kern, (size_t)p.slots, (unsigned)CE_FEW_THREADS, 0, static_cast<const float*>(k.Q), k.ldq, static_cast<const float*>(k.X), k.ldx, k.m, k.n, k.d, k.bias,
-                        a.c, k.targets, p.partial, p.target_scores);
+                        a.c, a.down, k.targets, p.partial, p.target_scores);
             KERNEL_CHECK();
         };
         if (k.m == 1) go(std::integral_constant<int, 1>());
@@ -1229,7 +1243,7 @@ template <typename T>
 inline void ce_finish(const CeCall& k, const CePlan& p, const CeFinish& rows, const CeFinish& queries) {
     CeFinishArgs a{};
     a.own_splits = p.own_splits, a.where_stride = k.n;
-    a.rows = rows, a.queries = queries, a.d = k.d, a.amax = p.amax, a.own = p.own, a.sums = p.sums, a.X = k.X, a.ldx = k.ldx, a.inv_t = (float)(1 / k.temperature);
+    a.rows = rows, a.queries = queries, a.d = k.d, a.amax = p.amax, a.own = p.own, a.sums = p.sums, a.X = k.X, a.ldx = k.ldx, a.inv_t = k.inv_t();
     const size_t grid = (size_t)rows.blocks + queries.blocks;
     if (!grid) return;
     if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "the matrices are too large for one call");
@@ -1280,7 +1294,7 @@ inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, vo
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
     a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = p.terms, a.factors = p.factors, a.amax = p.amax, a.target_cols = p.cols;
-    a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where, a.own_splits = p.own_splits, a.sums = p.sums, a.inv_t = (float)(1 / k.temperature);
+    a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where, a.own_splits = p.own_splits, a.sums = p.sums, a.inv_t = k.inv_t();
     const CUtensorMap own = ROWS ? ops.map_x(k, TG_M) : ops.map_q(k, TG_M), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
     auto go = [&](auto boxes) {
         constexpr int KB = decltype(boxes)::value;
@@ -1314,7 +1328,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
                     if (k.c->device < 64) is |= 1ull << k.c->device;
                 }
                 launch_next(k.stream, kern, (size_t)p.splits_q, (unsigned)CE_FEW_THREADS, grad_Q ? (size_t)k.m * k.d * 4 : 0, static_cast<const T*>(k.Q), k.ldq, static_cast<const T*>(k.X), k.ldx,
-                            k.m, k.n, k.d, k.bias, k.c2(), (float)(1 / k.temperature), p.terms, p.factors, p.own, p.cols, p.acc_q, grad_X, ld_gx);
+                            k.m, k.n, k.d, k.bias, k.c2(), k.inv_t(), p.terms, p.factors, p.own, p.cols, p.acc_q, grad_X, ld_gx);
                 KERNEL_CHECK();
             };
             if (k.m <= 4) go(std::integral_constant<int, 4>());
@@ -1355,7 +1369,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
             if (p.splits_x == 1) {
                 a.typed = grad_X + n0 * ld_gx, a.ld = ld_gx, a.amax = p.amax, a.where = p.where + n0, a.sums = p.sums;
                 a.own_splits = p.own_splits, a.where_stride = k.n;
-                a.inv_t = (float)(1 / k.temperature);
+                a.inv_t = k.inv_t();
             }
             ce_product<PLANES, true>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, 64), ops.q, ops.ldq, k.m, a, p.per_x, p.splits_x);
             if (p.splits_x > 1) {

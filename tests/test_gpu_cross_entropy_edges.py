@@ -113,3 +113,40 @@ def test_p_of_long_rows_sum_up_to_1(culsh, d, dtype):
         G = out.double() * t / 16
         assert float((G.sum(1) / e.double() - 1).abs().max()) <= err
         assert float((G / want - 1).abs().max()) <= 2 * score + err
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,d", [(3, 700, 40), (20, 70, 40), (70, 1000, 100), (20, 300, 300), (140, 90, 600)])
+@pytest.mark.parametrize("temperature,size", [(1e-30, 1e-15), (1e30, 1.0), (7e37, 1e30), (1e38, 1e30), (1e38, 1.0), (1.9e45, 1e30), (3e45, 1e36), (1e60, 1e36), (1e80, 1.0), (1e300, 1e36), (1e300, 1e38)])
+def test_temperatures_of_any_magnitude(culsh, temperature, size, m, n, d, dtype):
+    """Scores that are all next to 0: the loss is log(n).  One over the temperature, and log2(e) by it, are no floats of all their bits from 8e37 on, and none at all from 2e45 on.  `size`: of the
+    rows, so that the gradient of the queries is a number of its type where it can be one."""
+    if dtype == torch.float16:
+        size = min(max(size, 2.0 ** -6), 2.0 ** 12)
+        if temperature < 1:
+            temperature = 2.0 ** -10
+    Q = (torch.rand(m, d, generator=gen(1), device="cuda") - 0.5) * (size if temperature < 1 else 1.0)
+    X = (torch.rand(n, d, generator=gen(2), device="cuda") - 0.5) * size
+    Q, X = Q.to(dtype), X.to(dtype)
+    targets = torch.randint(0, n, (m,), generator=gen(3), device="cuda")
+    g, e = torch.randn(m, generator=gen(4), device="cuda"), torch.randn(m, generator=gen(5), device="cuda")
+    r = culsh.cross_entropy(Q, X, targets, temperature=temperature)
+    q, x = Q.double(), X.double()
+    z = q @ x.T / temperature
+    lse = torch.logsumexp(z, 1)
+    score = float((q.abs() @ x.abs().T).max()) / temperature * (d + 8) * 2.0 ** -23 + 2.0 ** -18
+    if float((q.abs() @ x.abs().T).max()) > 2.0 ** 127:  # the scores themselves, before they are divided, may be no floats: the query has no numbers then
+        fine = (q.abs() @ x.abs().T).max(1).values < 2.0 ** 127
+        assert not fine.any() or float((r.lse.double() - lse).abs()[fine].max()) <= score
+        return
+    assert float((r.lse.double() - lse).abs().max()) <= score and float((r.losses.double() - (lse - z.gather(1, targets[:, None])[:, 0])).abs().max()) <= 2 * score
+    dq, dx = culsh.cross_entropy_backward(Q, X, targets, r, g, e, temperature=temperature)
+    P = torch.softmax(z, 1) * (g + e).double()[:, None]
+    G = P.scatter_add(1, targets[:, None], -g.double()[:, None])
+    size_of = P.abs().scatter_add(1, targets[:, None], g.double().abs()[:, None])
+    err = 2 * HALF[dtype] + 4 * score + (m + n) * 2.0 ** -23
+    least = LEAST[dtype] + (2.0 ** -37 * float((g + e).abs().max()) * float(x.abs().max() + q.abs().max()) * (m + n) / temperature if dtype == torch.float16 else 0)
+    for out, want, tol in ((dq, G @ x / temperature, size_of @ x.abs() / temperature), (dx, G.T @ q / temperature, size_of.T @ q.abs() / temperature)):
+        fine = want.abs() + tol * err < torch.finfo(dtype).max / 2
+        off = (out.double() - want).abs() - (tol * err + least)
+        assert not torch.isnan(out).any() and float(off[fine].max()) <= 0, (float(off[fine].max()), float(want.abs().max()))
