@@ -12,7 +12,7 @@
 // eight warps take the tiles in turn, a thread half the columns of a lane.  S and G have two places each: what an MMA writes over has been read by the epilogue long before, and the tensor pipe has
 // another product to do while a G is made.  (G on top of S, in three places, 4.34 ms: the first product had to wait until the second one in front of it was done.)  dQ of that case takes 1.4 ms, bound
 // by the reads of shared memory, which the first product takes alone (tensor pipe 71 %); dX 2.1, with the terms of the columns read beside (47 %).  Sums of more than 32,768 entries are split (the accumulators cut off,
-// see tc_gemm.cuh), those of dQ over units, whose sums ce_finish_kernel adds up.
+// see tc_gemm.cuh) over units, and ce_finish_kernel adds them up: those of as many queries or rows at a time as 256 MB hold of (32,769 x 100,000 x 128 2.7 ms; dX by pieces of rows, with G in memory, 8.8).
 #pragma once
 
 #include <type_traits>
@@ -71,6 +71,7 @@ struct CeFusedArgs {
     unsigned units;
     uint32_t idesc_s, idesc_o;
     int own, other;           // entries of either side
+    int own0;                 // rows: the first one's number
     int tiles_own, tiles_other, block;
     int d;
     float c;
@@ -84,6 +85,7 @@ struct CeFusedArgs {
     void* out;                // dX
     int64_t ld;
     const int* where;
+    int64_t where_stride;
     int own_splits;
     const float* sums;
     float inv_t;
@@ -307,7 +309,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                 if (ROWS) {
                     bool hit = false;
 #pragma unroll
-                    for (int i = 0; i < CW / 32; ++i) hit = hit || (unsigned)(targets[i * 32 + lane] - first_own) < 32u;
+                    for (int i = 0; i < CW / 32; ++i) hit = hit || (unsigned)(targets[i * 32 + lane] - a.own0 - first_own) < 32u;
                     seldom = __any_sync(0xFFFFFFFFu, hit);
                 } else {
                     seldom = a.other - first < CW || __any_sync(0xFFFFFFFFu, (unsigned)(my_target - first) < (unsigned)CW);
@@ -350,7 +352,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                         }
                         if (decltype(checked)::value) {
                             if (ROWS) {
-                                const int target = targets[i * 32 + lane] - first_own;
+                                const int target = targets[i * 32 + lane] - a.own0 - first_own;
                                 unsigned hits = __ballot_sync(0xFFFFFFFFu, (unsigned)target < 32u), zero = 0;
                                 while (hits) {  // columns whose target is one of the warp's rows
                                     const int j = __ffs(hits) - 1;
@@ -398,7 +400,7 @@ ce_fused_kernel(const __grid_constant__ CUtensorMap tmOwn, const __grid_constant
                     const float scale = HALF ? ce_scale_back(a.inv_t, exponent) : a.inv_t;
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] *= scale;
-                    ce_add_own(v, a.where + mine, a.own, in ? a.own_splits : 0, a.sums, a.d, c0, a.inv_t);
+                    ce_add_own(v, a.where + mine, a.where_stride, in ? a.own_splits : 0, a.sums, a.d, c0, a.inv_t);
                 }
                 T* const o = reinterpret_cast<T*>(a.out) + (int64_t)mine * a.ld + c0;
                 float* const part = a.parts + ((int64_t)unit.block * a.own + mine) * a.d + c0;

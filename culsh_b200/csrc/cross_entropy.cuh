@@ -1004,6 +1004,7 @@ struct CePlan {
     float *acc_q = nullptr, *parts_x = nullptr;
     bool fused_q = false, fused_x = false;
     int fused_block = 0, fused_block_x = 0;  // tiles of the other side in a unit of dQ, of dX
+    int some_q = 0, some_x = 0;              // queries, rows whose sums lie in the workspace at a time
 
     CePlan(const CeCall& k, bool backward, bool need_q, bool need_x, void* base) : space{static_cast<char*>(base)} {
         const int sms = k.c->sm_count;
@@ -1042,9 +1043,9 @@ struct CePlan {
         terms = space.take<float>(lines), factors = space.take<float>(lines), own = space.take<float>(k.m);
         cols = space.take<int>(lines);
         if (k.type == CULSH_F16) amax = space.take<uint32_t>(1);
-        // G stays on the SM where rows are short enough; sums of more than 32,768 entries would have to be split for dX too
+        // G stays on the SM where rows are short enough
         const bool fused = k.planes() == 1 && k.d <= 256;
-        fused_q = need_q && fused, fused_x = need_x && fused && k.m <= 32768;
+        fused_q = need_q && fused, fused_x = need_x && fused;
         shift = k.type == CULSH_F16 && (fused_q || fused_x) ? CE_HALF_SHIFT : 0;
         if (need_x) {
             sums = space.take<float>((size_t)k.m * k.d);
@@ -1064,17 +1065,22 @@ struct CePlan {
             }
             return block;
         };
+        // split sums grow with both sides: as many queries or rows at a time as CE_PARTS_BYTES hold of
+        auto some = [&](int entries, int splits) {
+            const size_t fit = CE_PARTS_BYTES / ((size_t)splits * k.d * sizeof(float)) / TG_M * TG_M;
+            return (int)std::min<size_t>(entries, std::max<size_t>(fit, TG_M));
+        };
         if (fused_q) {
             const size_t tiles = ceil_div(k.n, nb);
             fused_block = block_of(tiles_q, tiles, ceil_div((size_t)4 * sms, tiles_q));
-            splits_q = (int)ceil_div(tiles, fused_block);
-            acc_q = space.take<float>((size_t)splits_q * k.m * k.d);
+            splits_q = (int)ceil_div(tiles, fused_block), some_q = some(k.m, splits_q);
+            acc_q = space.take<float>((size_t)splits_q * some_q * k.d);
         }
         if (fused_x) {  // sums of few rows are split too
             const size_t own = ceil_div(k.n, TG_M), tiles = ceil_div(k.m, nb);
-            fused_block_x = own >= (size_t)sms ? (int)tiles : block_of(own, tiles, sms / own);
-            splits_x = (int)ceil_div(tiles, fused_block_x);
-            if (splits_x > 1) parts_x = space.take<float>((size_t)splits_x * k.n * k.d);
+            fused_block_x = own >= (size_t)sms ? (int)ceil_div(tiles, ceil_div(tiles, 32768 / nb)) : block_of(own, tiles, sms / own);
+            splits_x = (int)ceil_div(tiles, fused_block_x), some_x = splits_x > 1 ? some(k.n, splits_x) : k.n;
+            if (splits_x > 1) parts_x = space.take<float>((size_t)splits_x * some_x * k.d);
         }
         if ((!need_q || fused_q) && (!need_x || fused_x)) return;
         const bool pieces_x = need_x && !fused_x;
@@ -1162,8 +1168,14 @@ struct CeOperands {
         else ce_prepare_kernel<__nv_bfloat16, 1><<<(unsigned)end, 256, 0, k.stream>>>(a);
         KERNEL_CHECK();
     }
-    CUtensorMap map_q(const CeCall& k, int box) const { return tg_map(q, k.tg(), k.m, k.d, ldq, k.planes(), (int64_t)k.m * ldq * 2, box); }
-    CUtensorMap map_x(const CeCall& k, int box) const { return tg_map(x, k.tg(), k.n, k.d, ldx, k.planes(), (int64_t)k.n * ldx * 2, box); }
+    CUtensorMap map_q(const CeCall& k, int box) const { return map_q(k, box, 0, k.m); }
+    CUtensorMap map_x(const CeCall& k, int box) const { return map_x(k, box, 0, k.n); }
+    // `count` of them from `first` on.
+    CUtensorMap map_q(const CeCall& k, int box, int first, int count) const { return map(k, q, ldq, k.m, box, first, count); }
+    CUtensorMap map_x(const CeCall& k, int box, int first, int count) const { return map(k, x, ldx, k.n, box, first, count); }
+    static CUtensorMap map(const CeCall& k, const void* from, int64_t ld, int rows, int box, int first, int count) {
+        return tg_map(static_cast<const uint16_t*>(from) + first * ld, k.tg(), count, k.d, ld, k.planes(), (int64_t)rows * ld * 2, box);
+    }
 };
 
 // f(number of planes, whether there is a bias, whether K is taken in segments, the tile), as types.
@@ -1240,10 +1252,10 @@ inline CeFinish ce_finish_of(const CeCall& k, const float* parts, int splits, in
     return f;
 }
 template <typename T>
-inline void ce_finish(const CeCall& k, const CePlan& p, const CeFinish& rows, const CeFinish& queries) {
+inline void ce_finish(const CeCall& k, const CePlan& p, const CeFinish& rows, const CeFinish& queries, int q0 = 0) {
     CeFinishArgs a{};
     a.own_splits = p.own_splits, a.where_stride = k.n;
-    a.rows = rows, a.queries = queries, a.d = k.d, a.amax = p.amax, a.own = p.own, a.sums = p.sums, a.X = k.X, a.ldx = k.ldx, a.inv_t = k.inv_t();
+    a.rows = rows, a.queries = queries, a.d = k.d, a.amax = p.amax, a.own = p.own + q0, a.sums = p.sums, a.X = k.X, a.ldx = k.ldx, a.inv_t = k.inv_t();
     const size_t grid = (size_t)rows.blocks + queries.blocks;
     if (!grid) return;
     if (grid > 0x7FFFFFFFull) fail(CULSH_ERR_UNSUPPORTED, "the matrices are too large for one call");
@@ -1280,22 +1292,24 @@ inline void ce_product(const CeCall& k, const CUtensorMap& tg, const void* b, in
     go(std::integral_constant<int, 0>());
 }
 
+// Sums of `count` queries or rows from own0 on.
 template <bool ROWS, bool HALF>
-inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, void* out, int64_t ld) {
+inline void ce_fused(const CeCall& k, const CePlan& p, const CeOperands& ops, int own0, int count, void* out, int64_t ld) {
     const int nb = k.d > 128 ? 64 : 128, kb = k.d > 128 ? 4 : k.d > 64 ? 2 : 1;
     CeFusedArgs a{};
     a.d_error = k.d_error;
     constexpr uint32_t M = (uint32_t)(TG_M >> 4) << 24;
     a.idesc_s = tg_idesc(k.tg(), false, false) | M | ((uint32_t)(nb >> 3) << 17);
     a.idesc_o = tg_idesc(k.tg(), false, true) | M | ((uint32_t)(kb * 64 >> 3) << 17);
-    a.own = ROWS ? k.n : k.m, a.other = ROWS ? k.m : k.n;
+    a.own = count, a.other = ROWS ? k.m : k.n, a.own0 = own0;
     a.tiles_own = (int)ceil_div(a.own, TG_M), a.tiles_other = (int)ceil_div(a.other, nb), a.block = ROWS ? p.fused_block_x : p.fused_block;
     const size_t units = ceil_div(a.tiles_other, a.block) * a.tiles_own;
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
-    a.d = k.d, a.c = k.c2(), a.bias = p.bias2, a.terms = p.terms, a.factors = p.factors, a.amax = p.amax, a.target_cols = p.cols;
-    a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where, a.own_splits = p.own_splits, a.sums = p.sums, a.inv_t = k.inv_t();
-    const CUtensorMap own = ROWS ? ops.map_x(k, TG_M) : ops.map_q(k, TG_M), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
+    const int q0 = ROWS ? 0 : own0;
+    a.d = k.d, a.c = k.c2(), a.bias = ROWS && p.bias2 ? p.bias2 + own0 : p.bias2, a.terms = p.terms + q0, a.factors = p.factors + q0, a.amax = p.amax, a.target_cols = p.cols + q0;
+    a.parts = !ROWS ? p.acc_q : p.splits_x > 1 ? p.parts_x : nullptr, a.out = out, a.ld = ld, a.where = p.where + own0, a.where_stride = k.n, a.own_splits = p.own_splits, a.sums = p.sums, a.inv_t = k.inv_t();
+    const CUtensorMap own = ROWS ? ops.map_x(k, TG_M, own0, count) : ops.map_q(k, TG_M, own0, count), other = ROWS ? ops.map_q(k, nb) : ops.map_x(k, nb);
     auto go = [&](auto boxes) {
         constexpr int KB = decltype(boxes)::value;
         if (k.bias) ce_fused_launch<KB, ROWS, true, HALF>(k.c, own, other, a, k.stream);
@@ -1338,12 +1352,24 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         }
     }
     CeFinish last{};  // of dX, for the launch that finishes dQ
+    int first_q = 0;  // of the queries that it finishes
     if constexpr (PLANES == 1) {
-        if (p.fused_x) {
-            ce_fused<true, HALF>(k, p, ops, grad_X, ld_gx);
-            if (p.splits_x > 1) last = ce_finish_of(k, p.parts_x, p.splits_x, k.n, nullptr, p.where, grad_X, ld_gx);
+        for (int64_t x0 = 0; p.fused_x && x0 < k.n; x0 += p.some_x) {
+            const int here = (int)std::min<int64_t>(p.some_x, k.n - x0);
+            ce_fused<true, HALF>(k, p, ops, (int)x0, here, grad_X + x0 * ld_gx, ld_gx);
+            if (p.splits_x == 1) continue;
+            last = ce_finish_of(k, p.parts_x, p.splits_x, here, nullptr, p.where + x0, grad_X + x0 * ld_gx, ld_gx);
+            if (x0 + here < k.n) ce_finish<T>(k, p, last, CeFinish{}), last = CeFinish{};
         }
-        if (p.fused_q) ce_fused<false, HALF>(k, p, ops, nullptr, 0);
+        for (int64_t q0 = 0; p.fused_q && q0 < k.m; q0 += p.some_q) {
+            const int here = (int)std::min<int64_t>(p.some_q, k.m - q0);
+            ce_fused<false, HALF>(k, p, ops, (int)q0, here, nullptr, 0);
+            first_q = (int)q0;
+            if (q0 + here < k.m) {
+                ce_finish<T>(k, p, last, ce_finish_of(k, p.acc_q, p.splits_q, here, p.factors + q0, p.cols + q0, grad_Q + q0 * ld_gq, ld_gq), first_q);
+                last = CeFinish{};
+            }
+        }
     }
     const bool pieces_q = grad_Q && !p.fused_q, pieces_x = grad_X && !p.fused_x;
     const CUtensorMap tq = ops.map_q(k, TG_M);
@@ -1383,7 +1409,9 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
             ce_product<PLANES, false>(k, tg_map(p.G, k.tg(), k.m, g_cols, p.piece, PLANES, g_plane * 2, TG_M), ops.x, ops.ldx, k.n, a, p.per_q, p.splits_q);
         }
     }
-    ce_finish<T>(k, p, last, grad_Q ? ce_finish_of(k, p.acc_q, p.splits_q, k.m, p.fused_q ? p.factors : nullptr, p.cols, grad_Q, ld_gq) : CeFinish{});
+    CeFinish queries{};
+    if (grad_Q) queries = ce_finish_of(k, p.acc_q, p.splits_q, k.m - first_q, p.fused_q ? p.factors + first_q : nullptr, p.cols + first_q, grad_Q + first_q * ld_gq, ld_gq);
+    ce_finish<T>(k, p, last, queries, first_q);
 }
 
 }  // namespace culsh_b200

@@ -414,9 +414,15 @@ int culsh_i8_score(culsh_handle* h, const void* Q, int type, int n_queries, int6
  *   lse     [m]  log of the sum of exp(z[i]); -inf where no row is left.  lse + lse_low is the same in twice the bits
  *   losses  [m]  lse - z[i][targets[i]], never negative; 0 where the target is not in 0 .. n - 1 (or targets is NULL), inf
  *                where it is masked
- * The scores are not kept; Q[i] . X[j] itself has to be within float32.  At most 65,536 features, 2,147,418,112 queries and rows.  A NaN or an infinity in a query, or in a row that is not masked, makes the numbers NaN that it has
- * a part in (but scores of 16-bit values that come out as -inf have none).  workspace: device, as many bytes as culsh_cross_entropy_workspace says for the same arrays (gradients: 0 for
- * the losses, 1 for the gradient of Q, 2 of X, 3 of both), aligned to 16. */
+ * The scores are not kept; Q[i] . X[j] itself has to be within float32.  At most 65,536 features, 2,147,418,112 queries and rows.
+ * A NaN or an infinity in a query, or in a row that is not masked, makes the numbers NaN that it has a part in (but scores of
+ * 16-bit values that come out as -inf have none).  workspace: device, aligned to 16, as many bytes as
+ * culsh_cross_entropy_workspace says for the same arrays (gradients: 0 for the losses, 1 for the gradient of Q, 2 of X, 3 of
+ * both).  It holds three 16-bit planes of 32-bit matrices, copies of 16-bit ones whose rows do not begin at multiples of 16 bytes
+ * (for gradients under a bias, of X), and some words for each query and row; for the losses up to 256 MB of partial sums; for
+ * gradients 4 d bytes for each query, and for 16-bit rows of up to 256 values up to 256 MB of partial sums for each output, else
+ * G for some rows and all queries (64 MB, 256 MB in 32 bits, but 256 rows at least) and partial sums, one for each 32,768
+ * (32 bits: 1,024) rows or queries that are added. */
 int culsh_cross_entropy_workspace(culsh_handle* h, const void* Q, int64_t ldq, const void* X, int64_t ldx, int type, int m, int n,
                                   int d, int has_bias, int gradients, uint64_t* bytes);
 int culsh_cross_entropy(culsh_handle* h, const void* Q, int64_t ldq, const void* X, int64_t ldx, int type, int m, int n, int d,

@@ -150,3 +150,69 @@ def test_temperatures_of_any_magnitude(culsh, temperature, size, m, n, d, dtype)
         fine = want.abs() + tol * err < torch.finfo(dtype).max / 2
         off = (out.double() - want).abs() - (tol * err + least)
         assert not torch.isnan(out).any() and float(off[fine].max()) <= 0, (float(off[fine].max()), float(want.abs().max()))
+
+
+def test_the_workspace_does_not_grow_with_both_sides(culsh):
+    """Sums that are split over the other side lie there for as many queries or rows as 256 MB hold: with a copy of what the queries and rows need each, a small multiple of the inputs."""
+    import ctypes as C
+
+    from culsh_b200._culsh_core import get_handle
+    h, need = get_handle(0), C.c_uint64()
+    for m, n, d in ((4_096, 1_000_000, 128), (32_768, 1_000_000, 128), (1_000_000, 1_000_000, 128), (1_000_000, 10_000_000, 128), (10_000_000, 1_000_000, 256), (50_000_000, 1_000_000, 8)):
+        for has_bias in (0, 1):
+            assert h.lib.culsh_cross_entropy_workspace(h.ptr, 16, d, 16, d, 3, m, n, d, has_bias, 3, C.byref(need)) == 0
+            # 512 MB of sums; planes of the rows, where there is a bias; sums of the targets' rows, of 32 bits; terms of queries, and up to 16 places for each row
+            assert need.value <= (512 << 20) + (2 * d * n if has_bias else 0) + 4 * d * m + 16 * (m + 128) + 68 * (n + 128) + 8192, (m, n, d, need.value)
+
+
+@pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, False), (torch.float16, True), (torch.float16, False)])
+@pytest.mark.parametrize("m,n,d", [(32_768, 20_000, 40), (32_769, 20_000, 40), (40_001, 700, 200), (300_001, 500_003, 16), (70_000, 260_001, 200)])
+def test_gradients_of_very_many_queries(culsh, m, n, d, dtype, bias):
+    """More queries than a sum takes, and more of both sides than the workspace holds sums of at a time: a few of the rows of each gradient against 64 bits.  Tolerances: a score errs by d + 8
+    units of the sum of its magnitudes (1 / t), p by twice that; G by half a unit, sums of 32,768 entries by as many cut-off units of 2^-23 of their magnitudes; the result by half a unit."""
+    t = 0.2
+    X = torch.nn.functional.normalize(torch.randn(n, d, generator=gen(1), device="cuda")).to(dtype)
+    Q = torch.nn.functional.normalize(torch.randn(m, d, generator=gen(2), device="cuda")).to(dtype)
+    targets = torch.randint(0, n, (m,), generator=gen(3), device="cuda")
+    some_rows = torch.tensor([0, 1, 127, 128, n // 2, n - 2, n - 1], device="cuda")
+    some = torch.tensor([0, 5, 127, 128, 32_767, m // 2, m - 2, m - 1], device="cuda")
+    targets[::7] = some_rows[torch.randint(0, 7, targets[::7].shape, generator=gen(4), device="cuda")]
+    b = None
+    if bias:
+        b = torch.randn(n, generator=gen(5), device="cuda")
+        b[5::11] = -np.inf
+        b[some_rows] = 0.5
+    g, e = torch.randn(m, generator=gen(6), device="cuda"), 0.1 * torch.randn(m, generator=gen(7), device="cuda")
+    r = culsh.cross_entropy(Q, X, targets, b, temperature=t)
+    dq, dx = culsh.cross_entropy_backward(Q, X, targets, r, g, e, b, temperature=t)
+    q, x, add = Q.double(), X.double(), 0.0 if b is None else b.double()
+    masked = torch.zeros(m, dtype=torch.bool, device="cuda") if b is None else b[targets] == -np.inf
+    gg = torch.where(masked, 0.0, g.double())
+    f, own = gg + e.double(), torch.where(masked, 0.0, -g.double())
+    # of some queries
+    z = q[some] @ x.T / t + add
+    lse = torch.logsumexp(z, 1)
+    score = (d + 8) * 2.0 ** -23 * 1.02 / t + 6 * 2.0 ** -23 * 8
+    assert float((r.lse[some].double() - lse).abs().max()) <= 2 * score + 2.0 ** -16
+    p = torch.exp(z - lse[:, None])
+    G = p * f[some][:, None]
+    one = torch.zeros_like(G).scatter_(1, targets[some][:, None], own[some][:, None])
+    err = 4 * score + 2.0 ** -16 + HALF[dtype] + 32_768 * 2.0 ** -23 + (m + n) // 32_768 * 2.0 ** -24
+    low = 2.0 ** -39 * float(f.abs().max()) if dtype == torch.float16 else 0.0
+
+    def check(out, want, size, ones):
+        tol = (err * size + low * ones) / t
+        off = (out.double() - want).abs() - (tol + HALF[dtype] * (want.abs() + tol) + LEAST[dtype])
+        assert float(off.max()) <= 0, (float(off.max()), float(tol.max()))
+
+    check(dq[some], (G + one) @ x / t, (G.abs() + one.abs()) @ x.abs(), torch.ones_like(G) @ x.abs())
+    # of some rows
+    z = q @ x[some_rows].T / t + (0.0 if b is None else b.double()[some_rows])
+    G = torch.exp(z - (r.lse.double() + r.lse_low.double())[:, None]) * f[:, None]
+    one = (targets[:, None] == some_rows[None, :]) * own[:, None]
+    check(dx[some_rows], (G + one).T @ q / t, (G.abs() + one.abs()).T @ q.abs(), torch.ones_like(G).T @ q.abs())
+    if b is not None:
+        assert not dx[5::11][b[5::11] == -np.inf].any()
+    only = culsh.cross_entropy_backward(Q, X, targets, r, g, e, b, temperature=t, queries=False)[1]
+    assert torch.equal(only, dx)
+    assert torch.equal(culsh.cross_entropy_backward(Q, X, targets, r, g, e, b, temperature=t, rows=False)[0], dq)
