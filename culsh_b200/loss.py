@@ -31,6 +31,11 @@ class CrossEntropy(NamedTuple):
     lse: torch.Tensor      # [m] log of the sum of exp(scores); -inf where the bias leaves no row
     lse_low: torch.Tensor  # [m] what lse leaves behind its last bit
 
+    def check(self) -> None:
+        """Waits for the current stream; raises if a product of this thread's losses or gradients had to give up a wait (what it should have made is NaN)."""
+        h = get_handle(self.losses.device.index)
+        _lib.check(h.lib.culsh_mx_product_check(h.ptr, _stream(self.losses.device)))
+
 
 def _sides(Q, X, bias):
     Q = _matrix(Q)

@@ -430,7 +430,8 @@ int culsh_cross_entropy(culsh_handle* h, const void* Q, int64_t ldq, const void*
                         void* workspace, uint64_t workspace_bytes, void* stream);
 /* Gradients with respect to Q and X, in their type (either may be NULL), from those of losses and of lse (either may be NULL) and
  * what the forward call returned.  A target that is not in 0 .. n - 1 or is masked has no loss to go by.  The bias has no
- * gradient here.  Results do not depend on the order in which anything runs. */
+ * gradient here.  Results do not depend on the order in which anything runs.  culsh_mx_product_check says whether a bounded
+ * wait ran out, here and in the losses. */
 int culsh_cross_entropy_backward(culsh_handle* h, const void* Q, int64_t ldq, const void* X, int64_t ldx, int type, int m, int n,
                                  int d, const int64_t* targets, const float* bias, double temperature, const float* losses,
                                  const float* lse, const float* lse_low, const float* grad_losses, const float* grad_lse,

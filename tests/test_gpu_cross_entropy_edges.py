@@ -216,3 +216,11 @@ def test_gradients_of_very_many_queries(culsh, m, n, d, dtype, bias):
     only = culsh.cross_entropy_backward(Q, X, targets, r, g, e, b, temperature=t, queries=False)[1]
     assert torch.equal(only, dx)
     assert torch.equal(culsh.cross_entropy_backward(Q, X, targets, r, g, e, b, temperature=t, rows=False)[0], dq)
+
+
+def test_no_wait_ran_out(culsh):
+    Q, X = torch.randn(300, 100, generator=gen(), device="cuda"), torch.randn(900, 100, generator=gen(1), device="cuda")
+    targets = torch.randint(0, 900, (300,), generator=gen(2), device="cuda")
+    r = culsh.cross_entropy(Q, X, targets)
+    culsh.cross_entropy_backward(Q, X, targets, r, torch.ones(300, device="cuda"))
+    r.check()
