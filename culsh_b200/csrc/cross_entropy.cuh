@@ -14,8 +14,8 @@
 // query added to the sums (ce_prepare_kernel, ce_finish_kernel).  Sums of one row's gradient over its queries are taken in ascending order: nothing depends on the order of atomics.
 //
 // 32-bit floats are held as three bfloat16 planes each (24 bits), products as six of 16 bits; G of 32-bit inputs likewise.  G of 16-bit inputs is rounded to their type, an operand of the tensor cores: its
-// errors average out over a sum, and the result's own rounding is some eighty times as much (4,096 x 100,000 x 128: rms 2.3e-5 of 1.7e-3 in bfloat16, 2.9e-6 of 2.1e-4 in float16), where a second plane
-// would double both products.  Against gradients from G in 32 bits that leaves 3e-4, values whose last bit falls the other way.  G of half precision is scaled by a power of two that brings the
+// errors average out over a long sum, and the result's own rounding is some eighty times as much (4,096 x 100,000 x 128: rms 2.3e-5 of 1.7e-3 in bfloat16, 2.9e-6 of 2.1e-4 in float16), where a second
+// plane would double both products.  Where a few entries make the sum, both roundings are alike (1.4 times the result's).  G of half precision is scaled by a power of two that brings the
 // largest coefficient to 2^15, so that p down to 2^-39 of it is there.
 #pragma once
 
@@ -45,7 +45,7 @@ struct CeScoreArgs {
     const float* bias;        // of the rows, in powers of two, or NULL
     const int64_t* targets;   // (forward) of the queries, or -1
     // forward
-    float down;               // what scores are multiplied by where their differences may not be floats (c is as much larger)
+    float down;               // what scores are multiplied by before differences are taken (c is as much larger)
     float2* partial;          // [m][slots]: reference and sum
     int slots;
     float* target_scores;     // [m]
@@ -162,18 +162,19 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
 #pragma unroll
             for (int j = 0; j < CE_PART; j += 2) top = fmaxf(fmaxf(top, x[j]), x[j + 1]);
             const float next = fmaxf(ref, top), base = next == -INFINITY ? 0.f : next;
-            const uint64_t cc = f2_pack(a.c, a.c), minus = f2_pack(-base, -base);
+            const float off = -base * a.down;
+            const uint64_t cc = f2_pack(a.c, a.c), down = f2_pack(a.down, a.down), minus = f2_pack(off, off);
             uint64_t part[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
             for (int j = 0; j < CE_PART; j += 2) {
                 const uint64_t pair = f2_pack(x[j], x[j + 1]);
                 float e0, e1;
-                f2_unpack(BIAS ? f2_add(pair, minus) : f2_mul(f2_add(pair, minus), cc), e0, e1);
+                f2_unpack(BIAS ? f2_add(pair, minus) : f2_mul(f2_fma(pair, down, minus), cc), e0, e1);
                 part[j / 2 & 3] = f2_add(part[j / 2 & 3], f2_pack(ce_exp2(e0), ce_exp2(e1)));
             }
             float lo, hi;
             f2_unpack(f2_add(f2_add(part[0], part[1]), f2_add(part[2], part[3])), lo, hi);
-            sum = fmaf(sum, ce_exp2(BIAS ? ref - base : (ref - base) * a.c), lo + hi);
+            sum = fmaf(sum, ce_exp2(BIAS ? ref - base : fmaf(ref, a.down, off) * a.c), lo + hi);
             ref = next;
         }
         template <typename D>
@@ -183,10 +184,6 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
             this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
             done();
             if (idle) return;
-            if (!BIAS && a.down != 1.f) {
-#pragma unroll
-                for (int j = 0; j < CE_PART; ++j) x[j] *= a.down;
-            }
             if (left < CE_PART || __any_sync(0xFFFFFFFFu, (unsigned)at < (unsigned)CE_PART)) {  // seldom
                 float v = 0.f;
 #pragma unroll
@@ -487,10 +484,9 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
             const float b = BIAS ? __ldcg(bias + row) * CE_LOG2E : 0.f;
 #pragma unroll
             for (int q = 0; q < M; ++q) {
-                if (!BIAS) acc[q] *= down;
                 if (target[q] == row) target_scores[q] = acc[q];
-                const float z = !BIAS ? acc[q] : b == -INFINITY ? b : fmaf(acc[q], c, b), next = fmaxf(ref[q], z), base = next == -INFINITY ? 0.f : next;
-                sum[q] = fmaf(sum[q], ce_exp2((ref[q] - base) * by), ce_exp2((z - base) * by));
+                const float z = !BIAS ? acc[q] : b == -INFINITY ? b : fmaf(acc[q], c, b), next = fmaxf(ref[q], z), off = next == -INFINITY ? 0.f : -next * down;
+                sum[q] = fmaf(sum[q], ce_exp2(fmaf(ref[q], down, off) * by), ce_exp2(fmaf(z, down, off) * by));
                 ref[q] = next;
             }
         }
@@ -500,16 +496,16 @@ __global__ void __launch_bounds__(CE_FEW_THREADS, 2) ce_few_kernel(const float* 
         if (q >= m) break;
         float top = ref[q];
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        float all = sum[q] * ce_exp2((ref[q] - (top == -INFINITY ? 0.f : top)) * by);
+        float all = sum[q] * ce_exp2(fmaf(ref[q], down, top == -INFINITY ? 0.f : -top * down) * by);
         for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
         __syncthreads();
         if (lane == 0) s_part[warp] = make_float2(top, all);
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int w = 1; w < CE_FEW_THREADS / 32; ++w) top = fmaxf(top, s_part[w].x);
-            const float base = top == -INFINITY ? 0.f : top;
+            const float off = top == -INFINITY ? 0.f : -top * down;
             all = 0.f;
-            for (int w = 0; w < CE_FEW_THREADS / 32; ++w) all = fmaf(s_part[w].y, ce_exp2((s_part[w].x - base) * by), all);
+            for (int w = 0; w < CE_FEW_THREADS / 32; ++w) all = fmaf(s_part[w].y, ce_exp2(fmaf(s_part[w].x, down, off) * by), all);
             partial[(int64_t)q * gridDim.x + blockIdx.x] = make_float2(top, all);
         }
     }
@@ -676,7 +672,7 @@ __device__ __forceinline__ void ce_bias_part(const CePrepare& a, unsigned block)
 // WARPS warps join a query's blocks.
 template <int WARPS>
 __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__ partial, int slots, int m, int n, const int64_t* __restrict__ targets,
-                                                      const float* __restrict__ target_scores, const float* __restrict__ bias2, float c, float* __restrict__ losses,
+                                                      const float* __restrict__ target_scores, const float* __restrict__ bias2, float c, float down, float* __restrict__ losses,
                                                       float* __restrict__ lse, float* __restrict__ lse_low, KernelBefore before) {
     behind_kernel_before(partial, targets, target_scores, bias2, losses, lse, lse_low, before);
     __shared__ float s_top[8];
@@ -692,12 +688,12 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
         __syncthreads();
         for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_top[warp / WARPS * WARPS + w]);
     }
-    const float base = top == -INFINITY ? 0.f : top, by = bias2 ? 1.f : c;  // scores, or exponents
+    const float base = top == -INFINITY ? 0.f : top * down, by = bias2 ? 1.f : c;  // scores, or exponents
     double sum = 0.;
 #pragma unroll 8
     for (int i = first; i < slots; i += 32 * WARPS) {
         const float2 v = __ldcg(p + i);
-        sum += (double)v.y * (double)exp2f((v.x - base) * by);
+        sum += (double)v.y * (double)exp2f(fmaf(v.x, down, -base) * by);
     }
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (WARPS > 1) {
@@ -715,7 +711,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* __restrict__
     const int64_t t = targets ? __ldcg(targets + q) : -1;
     if (t >= 0 && t < n) {
         const float b = bias2 ? __ldcg(bias2 + t) : 0.f, s = __ldcg(target_scores + q);
-        const double z = b == -INFINITY ? (double)b : bias2 ? (double)fmaf(s, c, b) : (double)s * (double)c;  // as in the sums
+        const double z = b == -INFINITY ? (double)b : bias2 ? (double)fmaf(s, c, b) : (double)(s * down) * (double)c;  // as in the sums
         loss = z == -INFINITY && two == two ? INFINITY : (float)((two - z) * ln2);
         if (loss < 0.f) loss = 0.f;
     }
@@ -959,7 +955,8 @@ struct CeCall {
     int pitch() const { return (d + 7) & ~7; }
     bool copies(const void* p, int64_t ld) const { return type == CULSH_F32 || !aligned16(p, ld * 2); }
     TgType tg() const { return type == CULSH_F16 ? TG_F16 : TG_BF16; }
-    // The losses take differences of scores, without a bias.  They may be beyond float32, and by temperatures beyond 2^100 small again: scores are multiplied by it first then.
+    // The losses take differences of scores, without a bias.  They may be beyond float32, and by temperatures beyond 2^100 small again: scores are multiplied by it then, in the same
+    // instruction that takes the difference.
     float down() const { return !bias && temperature > 0x1p100 ? 0x1p-64f : 1.f; }
     // Not 0, by which an infinity would be no number: of a temperature beyond 2^149 scores make no difference (at most 2^128 2^-149).
     float c2() const { return std::max((float)(1.4426950408889634 / temperature), 0x1p-149f); }
@@ -1237,7 +1234,7 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     }, k.planes() == 3, k.bias != nullptr, segments, p.tile);
     }
     auto join = p.slots > 256 ? ce_join_kernel<8> : ce_join_kernel<1>;
-    launch_next(k.stream, join, ceil_div(k.m, p.slots > 256 ? 1 : 8), 256u, 0, (const float2*)p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, losses, lse, lse_low);
+    launch_next(k.stream, join, ceil_div(k.m, p.slots > 256 ? 1 : 8), 256u, 0, (const float2*)p.partial, p.slots, k.m, k.n, k.targets, p.target_scores, p.bias2, a.c, a.down, losses, lse, lse_low);
     KERNEL_CHECK();
 }
 
