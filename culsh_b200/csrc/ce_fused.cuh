@@ -11,7 +11,7 @@
 // One warp loads, one issues the first products and one the second (a single one, issuing 16 MMAs a tile and waiting three times, held them up: 4,096 x 1M x 128 4.12 ms in place of 3.7), two groups of
 // eight warps take the tiles in turn, a thread half the columns of a lane.  S and G have two places each: what an MMA writes over has been read by the epilogue long before, and the tensor pipe has
 // another product to do while a G is made.  (G on top of S, in three places, 4.34 ms: the first product had to wait until the second one in front of it was done.)  dQ of that case takes 1.4 ms, bound
-// by the reads of shared memory, which the first product takes alone (tensor pipe 71 %); dX 2.1, with the terms of the columns read beside (47 %).  Sums of more than 32,768 entries are split (the accumulators cut off,
+// by the reads of shared memory, which the first product takes alone (tensor pipe 69 %); dX 2.2, with the terms, factors and targets of the columns read beside (46 %).  Sums of more than 32,768 entries are split (the accumulators cut off,
 // see tc_gemm.cuh) over units, and ce_finish_kernel adds them up: those of as many queries or rows at a time as 256 MB hold of (32,769 x 100,000 x 128 2.7 ms; dX by pieces of rows, with G in memory, 8.8).
 #pragma once
 

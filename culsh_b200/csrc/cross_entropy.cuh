@@ -138,7 +138,7 @@ struct CeSums {
 
 // A thread keeps the largest of its part of a query's scores (of the exponents, where there is a bias) and the sum of exponentials by it; the largest one's is exactly 1, and so the loss of a query
 // that has but one row is exactly 0.  Of a batch, bound by the exponentials, 16 a cycle and SM: 4,096 x
-// 1M x 128 bfloat16 1.29 ms, their unit busy for 80 %, the tensor pipe for 39.  (Eight warps in place of sixteen 2.0 ms; an arrival that releases to the cluster, for each tile of each warp, 1.9.)
+// 1M x 128 bfloat16 1.34 ms, their unit busy for 77 %, the tensor pipe for 38.  (Eight warps in place of sixteen 2.0 ms; an arrival that releases to the cluster, for each tile of each warp, 1.9.)
 template <int PLANES, bool BIAS, bool SEGMENTS, int TILE>
 struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
     static constexpr int BN = CeScoreBase<PLANES, 0, TILE>::BN;
@@ -1040,7 +1040,8 @@ struct CePlan {
         terms = space.take<float>(lines), factors = space.take<float>(lines), own = space.take<float>(k.m);
         cols = space.take<int>(lines);
         if (k.type == CULSH_F16) amax = space.take<uint32_t>(1);
-        // G stays on the SM where rows are short enough
+        // G stays on the SM where rows are short enough.  There | by pieces (us): 4,096 x 1M x 128 3,361 | 10,005, x 200,000 x 64 780 | 1,954, x 200,000 x 256 1,410 |
+        // 3,101; 500 x 200,000 x 256 286 | 441; but 64 x 200,000 x 128, half the lanes idle, 137 | 111
         const bool fused = k.planes() == 1 && k.d <= 256;
         fused_q = need_q && fused, fused_x = need_x && fused;
         shift = k.type == CULSH_F16 && (fused_q || fused_x) ? CE_HALF_SHIFT : 0;

@@ -122,8 +122,8 @@ __device__ __noinline__ void i8_store_far(int metric, uint32_t taddr, int column
 }
 
 // More than 64 queries: they are the M side, a lane of the accumulator a query.  Short rows leave the time to the epilogue: a warp has 32 queries by all 128 rows of a tile, and groups of four
-// take tiles in turn; of long rows a tile has 256, and a warp 64 of them.  128 bytes of each query are stored at a time, by way of shared memory.  4,099 x 32,771 x 2,048 260 us, the tensor pipe
-// busy for 68 % (one CTA by 128 rows 414); 1,000 x 1M x 128 bfloat16 609, no unit above 38 % (conversions in place of additions 923).
+// take tiles in turn; of long rows a tile has 256, and a warp 64 of them.  128 bytes of each query are stored at a time, by way of shared memory.  4,099 x 32,771 x 2,048 265 us, the tensor pipe
+// busy for 68 % (one CTA by 128 rows 414); 1,000 x 1M x 128 bfloat16 635, no unit above 38 % (conversions in place of additions 923).
 template <typename OUT, bool PAIRS, int N>
 struct I8ProductPolicy {
     static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = N == 256, PAIR = PAIRS;
@@ -242,7 +242,8 @@ struct I8ProductPolicy {
     };
 };
 
-// Up to 64 queries: the rows are the M side, so that no lane is idle, and a warp's store of a query is 32 neighbouring scores.  One query by 1M x 128 34 us, HBM 50 % (151 with the query there).
+// Up to 64 queries: the rows are the M side, so that no lane is idle, and a warp's store of a query is 32 neighbouring scores.  One query by 1M x 128 36 us, HBM 47 % (151 with the query
+// there).  Through the Python calls, here | with the queries there: 17 of them 49 | 100, 48 71 | 95, but 64 85 | 77; by 20,000 x 1,000 17 24.4 | 25.4, 64 24.5 | 18.3.
 template <typename OUT, int N>
 struct I8FewPolicy {
     static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = false, PAIR = false;

@@ -310,7 +310,8 @@ class Int8Rows:
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, squares: torch.Tensor, n_features: int) -> "Int8Rows":
         """Rows from the arrays of another Int8Rows, e.g. loaded from a file: ``codes`` [n, P] int8 with P = n_features rounded up to a multiple of 16, zeros behind a
-        row's end, ``scales`` [n] float32, ``squares`` [n] int32 (sums of the rows' squared codes, -1 for a row that is NaN)."""
+        row's end, ``scales`` [n] float32, ``squares`` [n] int32 (sums of the rows' squared codes, -1 for a row that is NaN).  Codes are from -127 to 127: what the arrays hold is taken as it is, as
+        looking would wait for the device."""
         d = int(n_features)
         if not 0 < d <= MAX_INT8_FEATURES:
             raise ValueError(f"n_features must be between 1 and {MAX_INT8_FEATURES}")
