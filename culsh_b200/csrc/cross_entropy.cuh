@@ -28,16 +28,17 @@
 namespace culsh_b200 {
 
 constexpr int CE_BN = 256, CE_PART = CE_BN / 4;  // columns of a tile, and of it for a warp
-// Steps of 64 in a segment of K (tc_gemm.cuh), and in one of the gradient's scores of 16-bit rows: 128 adds, which cut off 8e-6 of a score at most.  That makes p smaller than the losses' pass has it, by
-// 3e-4 of it where scores are 40 (half a unit of float16 is 4.9e-4); in one sum over 65,536 values it would be 1.3e-2.  By segments of 16 that is halved and 4,099 x 32,771 x 2,048 float16 takes 1.60 ms
-// in place of 1.47, by the losses' own 1.75; 4,099 x 16,000 x 4,096 in one sum 1.49, by 32 1.55, by 16 1.62.
-constexpr int CE_SEGMENT = 8, CE_SEGMENT_16 = 32;
+// Steps of 64 in a segment of K (tc_gemm.cuh), of the losses' scores and of the gradient's, so that p are a softmax of the same numbers: in one sum over 65,536 values the gradient's scores of 40 would
+// be 3e-4 of themselves smaller, and all p 1.3e-2.  A segment's 32 adds cut off 1e-6 of a score (32 x 2^-25 of it on average, as its sum grows).  4,099 x 32,771 x 2,048 float16: losses 380 us, by
+// segments of 256 values 414; gradient 1.51 ms, in one sum 1.46.  Calls of few tiles, which leave most SMs idle, have time for shorter ones: losses of 64 x 4,891 x 1,321 bfloat16 4.3e-7 off in place
+// of 1.6e-6 in the same 35 us (128 x 9,000 x 4,096 33 us in place of 26).
+constexpr int CE_SEGMENT = 8, CE_SEGMENT_SMALL = 2;
 
 struct CeScoreArgs {
     int* d_error;
     unsigned units;
     uint32_t idesc;
-    int m, kb;                // queries; steps of K
+    int m, kb, segment;       // queries; steps of K, and of a segment of it
     int n0, n1;               // rows of this call
     int block, tiles_q, m_tile;  // tiles of rows in a unit; tiles of queries, and their size
     unsigned tiles_n;
@@ -72,10 +73,10 @@ struct CeUnit {
 
 // Tiles of 256 rows, of a CTA or of a pair of them, and of 64 where those would leave most SMs idle.
 enum CeTile : int { CE_ONE = 0, CE_PAIR = 1, CE_SMALL = 2 };
-template <int PLANES, int SEGMENTS, int TILE>
+template <int PLANES, bool K_SEGMENTS, int TILE>
 struct CeScoreBase {
     static constexpr bool A_MN = false, B_MN = false, I8 = false, PARTS = true, PAIR = TILE == CE_PAIR;
-    static constexpr int BN = TILE == CE_SMALL ? CE_PART : CE_BN, SEGMENT = SEGMENTS, EPI_WARPS = BN / 16;
+    static constexpr int BN = TILE == CE_SMALL ? CE_PART : CE_BN, SEGMENTS = K_SEGMENTS, EPI_WARPS = BN / 16;
     static constexpr int EPI_BYTES = EPI_WARPS * CE_PART * 4;
     using Pairs = PlanePairs<PLANES>;
     using Args = CeScoreArgs;
@@ -96,21 +97,29 @@ __device__ __forceinline__ void ce_bias_tile(const float* bias, int n0, int n1, 
     __syncwarp();
 }
 
-// The sums of a tile's segments, for a thread's columns of one lane.
-template <bool SEGMENTS>
+// The sums of a tile's segments, for a thread's columns of one lane.  WIDE: all of them at a time (few warps, which have the registers).
+template <bool SEGMENTS, bool WIDE>
 struct CeSums {
     static_assert(CE_PART == 64, "");
     float v[SEGMENTS ? CE_PART : 1];
     __device__ __forceinline__ void segment(const CeScoreArgs&, bool first, uint32_t taddr, bool) {
         if constexpr (SEGMENTS) {
             auto each = [&](auto&& f) {
-#pragma unroll
-                for (int c0 = 0; c0 < CE_PART; c0 += 16) {
-                    uint32_t r[16];
-                    tg_ld16(taddr + c0, r);
+                if constexpr (WIDE) {
+                    uint32_t r[2][32];
+                    tg_ld64(taddr, r);
                     tc_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) f(v[c0 + j], __uint_as_float(r[j]));
+                    for (int j = 0; j < CE_PART; ++j) f(v[j], __uint_as_float(r[j / 32][j % 32]));
+                } else {
+#pragma unroll
+                    for (int c0 = 0; c0 < CE_PART; c0 += 16) {
+                        uint32_t r[16];
+                        tg_ld16(taddr + c0, r);
+                        tc_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) f(v[c0 + j], __uint_as_float(r[j]));
+                    }
                 }
             };
             if (first) each([](float& to, float from) { to = from; });
@@ -121,12 +130,11 @@ struct CeSums {
     template <typename F>
     __device__ __forceinline__ void read(const CeScoreArgs& a, uint32_t taddr, bool live, bool more, F&& f) {
         if constexpr (SEGMENTS) {
-            segment(a, !more, taddr, live);
+            CeSums::segment(a, !more, taddr, live);
             f(v);
         } else {
             uint32_t r[2][32];
-            tg_ld32(taddr, r[0]);
-            tg_ld32(taddr + 32, r[1]);
+            tg_ld64(taddr, r);
             tc_ld_wait();
             float x[CE_PART];
 #pragma unroll
@@ -140,9 +148,9 @@ struct CeSums {
 // that has but one row is exactly 0.  Of a batch, bound by the exponentials, 16 a cycle and SM: 4,096 x
 // 1M x 128 bfloat16 1.34 ms, their unit busy for 77 %, the tensor pipe for 38.  (Eight warps in place of sixteen 2.0 ms; an arrival that releases to the cluster, for each tile of each warp, 1.9.)
 template <int PLANES, bool BIAS, bool SEGMENTS, int TILE>
-struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
-    static constexpr int BN = CeScoreBase<PLANES, 0, TILE>::BN;
-    struct Epilogue : CeSums<SEGMENTS> {
+struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
+    static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
+    struct Epilogue : CeSums<SEGMENTS, TILE == CE_SMALL> {
         int q, quarter, group, lane, rank, target;
         bool idle;
         float ref, sum;
@@ -177,13 +185,19 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
             sum = fmaf(sum, ce_exp2(BIAS ? ref - base : fmaf(ref, a.down, off) * a.c), lo + hi);
             ref = next;
         }
+        __device__ __forceinline__ void segment(const CeScoreArgs& a, bool first, uint32_t taddr, bool live) {
+            if (!idle) CeSums<SEGMENTS, TILE == CE_SMALL>::segment(a, first, taddr, live);
+        }
         template <typename D>
         __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more, D&& done) {
+            if (idle) {  // no query is behind the warp's lanes
+                done();
+                return;
+            }
             const int n0 = a.n0 + (u.tile0 + t) * BN + group * CE_PART, left = a.n1 - n0, at = target - n0;
-            if (BIAS && !idle) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
+            if (BIAS) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
             this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
             done();
-            if (idle) return;
             if (left < CE_PART || __any_sync(0xFFFFFFFFu, (unsigned)at < (unsigned)CE_PART)) {  // seldom
                 float v = 0.f;
 #pragma unroll
@@ -212,9 +226,9 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS ? CE_SEGMENT : 0, TILE> {
 
 // G of a piece, 128 neighbouring bytes of a query to a thread.  4,099 x 6,656 x 2,048 float16 82 us, 1,355 TFLOP/s.
 template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS, int TILE>
-struct CeGradPolicy : CeScoreBase<PLANES, !SEGMENTS ? 0 : PLANES == 1 ? CE_SEGMENT_16 : CE_SEGMENT, TILE> {
-    static constexpr int BN = CeScoreBase<PLANES, 0, TILE>::BN;
-    struct Epilogue : CeSums<SEGMENTS> {
+struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
+    static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;
+    struct Epilogue : CeSums<SEGMENTS, TILE == CE_SMALL> {
         int q, quarter, group, lane, rank, target;
         bool idle;
         float term, factor;
@@ -230,13 +244,19 @@ struct CeGradPolicy : CeScoreBase<PLANES, !SEGMENTS ? 0 : PLANES == 1 ? CE_SEGME
             target = in ? __ldcg(a.target_cols + q) : -1;
             if (HALF) factor = ldexpf(factor, ce_scale_exponent(a.amax) - a.shift);
         }
+        __device__ __forceinline__ void segment(const CeScoreArgs& a, bool first, uint32_t taddr, bool live) {
+            if (!idle) CeSums<SEGMENTS, TILE == CE_SMALL>::segment(a, first, taddr, live);
+        }
         template <typename D>
         __device__ __forceinline__ void tile(const CeScoreArgs& a, const CeUnit& u, int t, uint32_t taddr, bool live, bool more, D&& done) {
+            if (idle) {  // no query is behind the warp's lanes
+                done();
+                return;
+            }
             const int first = (u.tile0 + t) * BN + group * CE_PART, n0 = a.n0 + first, left = a.n1 - n0, at = target - n0;
-            if (BIAS && !idle) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
+            if (BIAS) ce_bias_tile(a.bias, n0, a.n1, s_bias, lane);
             this->read(a, taddr, live, more, [&](float (&x)[CE_PART]) {
             done();
-            if (idle) return;
             if (!live) factor = __int_as_float(0x7FFFFFFF);
 #pragma unroll
             for (int j = 0; j < CE_PART; ++j) x[j] = ce_exp2(BIAS ? fmaf(x[j], a.c, s_bias[j]) + term : fmaf(x[j], a.c, term)) * factor;  // as in the losses' pass: the bias first
@@ -357,7 +377,7 @@ __device__ __forceinline__ void ce_store_typed(const CeProductArgs& a, int row, 
 template <int PLANES, bool AMN, int N, bool PAIRS, int TYPED>
 struct CeProductPolicy {
     static constexpr bool A_MN = AMN, B_MN = true, I8 = false, PARTS = true, PAIR = PAIRS;
-    static constexpr int BN = N, SEGMENT = 0, EPI_BYTES = 0, EPI_WARPS = 8;
+    static constexpr int BN = N, SEGMENTS = 0, EPI_BYTES = 0, EPI_WARPS = 8;
     using Pairs = PlanePairs<PLANES>;
     using Args = CeProductArgs;
     using Unit = CeProductUnit;
@@ -1117,6 +1137,7 @@ struct CePlan {
         if (ceil_div(k.m, TG_M) * ceil_div(n, CE_BN) <= (size_t)k.c->sm_count / 4) return CE_SMALL;
         return pairs(k.m) ? CE_PAIR : CE_ONE;
     }
+    static int segment_of(const CeCall& k) { return tile_of(k, k.n) == CE_SMALL ? CE_SEGMENT_SMALL : CE_SEGMENT; }
     static int tile_rows(CeTile t) { return t == CE_SMALL ? CE_PART : CE_BN; }
     static int product_bn(int d) { return d > 128 ? 256 : d > 64 ? 128 : 64; }
 };
@@ -1198,7 +1219,7 @@ inline void ce_by(F&& f, bool three, bool bias, bool segments, CeTile tile) {
 inline CeScoreArgs ce_score_args(const CeCall& k, const CePlan& p, CeTile tile, int n0, int n1) {
     CeScoreArgs a{};
     a.d_error = k.d_error, a.idesc = tg_idesc(k.tg(), false, false);
-    a.m = k.m, a.kb = (int)ceil_div(k.d, 64), a.n0 = n0, a.n1 = n1;
+    a.m = k.m, a.kb = (int)ceil_div(k.d, 64), a.segment = CePlan::segment_of(k), a.n0 = n0, a.n1 = n1;
     a.m_tile = tile == CE_PAIR ? 2 * TG_M : TG_M;
     a.tiles_q = (int)ceil_div(k.m, a.m_tile), a.tiles_n = (unsigned)ceil_div(n1 - n0, CePlan::tile_rows(tile));
     a.c = k.c2(), a.bias = p.bias2, a.targets = k.targets;
@@ -1229,7 +1250,7 @@ inline void cross_entropy(const CeCall& k, float* losses, float* lse, float* lse
     if (units >= 1ull << 31) fail(CULSH_ERR_UNSUPPORTED, "%d queries by %d rows are too many for one call", k.m, k.n);
     a.units = (unsigned)units;
     const CUtensorMap tq = ops.map_q(k, TG_M), tx = ops.map_x(k, ce_box_x(p.tile));
-    const bool segments = a.kb > CE_SEGMENT;
+    const bool segments = a.kb > a.segment;
     ce_by([&](auto planes, auto bias, auto segs, auto tile) {
         tc_gemm<CeLossPolicy<decltype(planes)::value, decltype(bias)::value, decltype(segs)::value, decltype(tile)::value>>(k.c, tq, tx, a, k.stream);
     }, k.planes() == 3, k.bias != nullptr, segments, p.tile);
@@ -1385,7 +1406,7 @@ inline void cross_entropy_backward(const CeCall& k, const float* losses, const f
         ce_by([&](auto planes, auto bias, auto segs, auto type) {
             if constexpr (decltype(planes)::value == PLANES)
                 tc_gemm<CeGradPolicy<PLANES, decltype(bias)::value, HALF, decltype(segs)::value, decltype(type)::value>>(k.c, tq, tx, s, k.stream);
-        }, PLANES == 3, k.bias != nullptr, s.kb > (PLANES == 1 ? CE_SEGMENT_16 : CE_SEGMENT), tile);
+        }, PLANES == 3, k.bias != nullptr, s.kb > s.segment, tile);
         const int64_t g_cols = (int64_t)s.tiles_n * CePlan::tile_rows(tile);  // behind the last row G has zeros
         if (pieces_x) {
             CeProductArgs a{};

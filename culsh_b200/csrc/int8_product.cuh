@@ -127,7 +127,7 @@ __device__ __noinline__ void i8_store_far(int metric, uint32_t taddr, int column
 template <typename OUT, bool PAIRS, int N>
 struct I8ProductPolicy {
     static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = N == 256, PAIR = PAIRS;
-    static constexpr int BN = N, EPI_WARPS = 16, PART = PARTS ? BN / 4 : BN, TURNS = PARTS ? 1 : EPI_WARPS / 4, SEGMENT = 0, PIECE = 32 * 128, EPI_BYTES = EPI_WARPS * (PIECE + PART * 8);
+    static constexpr int BN = N, EPI_WARPS = 16, PART = PARTS ? BN / 4 : BN, TURNS = PARTS ? 1 : EPI_WARPS / 4, SEGMENTS = 0, PIECE = 32 * 128, EPI_BYTES = EPI_WARPS * (PIECE + PART * 8);
     using Pairs = PlanePairs<1>;
     using Args = I8ProductArgs;
     using Unit = I8Unit;
@@ -247,7 +247,7 @@ struct I8ProductPolicy {
 template <typename OUT, int N>
 struct I8FewPolicy {
     static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = false, PAIR = false;
-    static constexpr int BN = N, EPI_WARPS = 8, SEGMENT = 0, EPI_BYTES = 1024;
+    static constexpr int BN = N, EPI_WARPS = 8, SEGMENTS = 0, EPI_BYTES = 1024;
     using Pairs = PlanePairs<1>;
     using Args = I8ProductArgs;
     struct Unit {

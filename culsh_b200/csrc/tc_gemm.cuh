@@ -11,10 +11,11 @@
 // before it gives its memory back.  No load uses cluster multicast.
 //
 // The accumulators cut off what their adds leave behind 32 bits, half a unit each time on average and always to the same side: 128 adds (K of 2,048) leave a sum 4e-6 of it too small.  A
-// policy may have K taken in segments of SEGMENT steps, each in an accumulator of its own, which its epilogue adds up.
+// policy may have K taken in segments of so many steps, each in an accumulator of its own, which its epilogue adds up.
 //
 // A policy has:  Args with `units` and `d_error`;  Unit(args, u) with `tiles`, `k0`, `k1` (steps of K);  load(), which brings a step of a tile (rank: which
-// of a pair's CTAs);  n_mma(args, unit, tile), columns of a tile;  EPI_WARPS;  PARTS, whether the groups share a tile;  SEGMENT, 0 for none;  Epilogue with unit_begin(), segment() of all accumulators of a tile but the last, tile() and unit_end().
+// of a pair's CTAs);  n_mma(args, unit, tile), columns of a tile;  EPI_WARPS;  PARTS, whether the groups share a tile;  SEGMENTS, whether K may be taken in them, of Args'
+// `segment` steps;  Epilogue with unit_begin(), segment() of all accumulators of a tile but the last, tile() and unit_end().
 #pragma once
 
 #include "tc_ptx.cuh"
@@ -106,8 +107,15 @@ inline uint32_t tg_idesc(TgType t, bool a_mn, bool b_mn) {
 }
 
 template <typename P>
-__device__ __forceinline__ int tg_segments(const typename P::Unit& u) {
-    return P::SEGMENT ? (u.k1 - u.k0 + P::SEGMENT - 1) / (P::SEGMENT ? P::SEGMENT : 1) : 1;
+__device__ __forceinline__ int tg_segments(const typename P::Args& a, const typename P::Unit& u) {
+    if constexpr (P::SEGMENTS) return (u.k1 - u.k0 + a.segment - 1) / a.segment;
+    else return 1;
+}
+// Steps of a segment: first and last.
+template <typename P>
+__device__ __forceinline__ int2 tg_segment(const typename P::Args& a, const typename P::Unit& u, int nth) {
+    if constexpr (P::SEGMENTS) return make_int2(u.k0 + nth * a.segment, min(u.k1, u.k0 + (nth + 1) * a.segment));
+    else return make_int2(u.k0, u.k1);
 }
 
 template <typename P>
@@ -176,11 +184,12 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             bool live = true;
             for (unsigned u = first; u < a.units && live; u += step) {
                 const typename P::Unit unit(a, u);
-                for (int at = 0; at < unit.tiles * tg_segments<P>(unit) && live; ++at) {
-                    const int t = at / tg_segments<P>(unit), k0 = unit.k0 + (at - t * tg_segments<P>(unit)) * P::SEGMENT;
-                    const int k1 = P::SEGMENT ? min(unit.k1, k0 + P::SEGMENT) : unit.k1;
+                const int segments = tg_segments<P>(a, unit);
+                for (int at = 0; at < unit.tiles * segments && live; ++at) {
+                    const int t = at / segments;
+                    const int2 steps = tg_segment<P>(a, unit, at - t * segments);
                     for (int pair = 0; pair < P::Pairs::N && live; ++pair) {
-                        for (int k = k0; k < k1; ++k) {
+                        for (int k = steps.x; k < steps.y; ++k) {
                             if (!mbar_wait(&empty[s], parity, s_abort, a.d_error)) { live = false; break; }
                             unsigned char* st = base + (size_t)s * Cfg::STAGE_BYTES;
                             if (rank == 0) mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * Cfg::STAGE_BYTES);
@@ -199,14 +208,15 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         bool live = rank == 0;
         for (unsigned u = first; u < a.units && live; u += step) {
             const typename P::Unit unit(a, u);
-            for (int at = 0; at < unit.tiles * tg_segments<P>(unit) && live; ++at) {
-                const int t = at / tg_segments<P>(unit), k0 = unit.k0 + (at - t * tg_segments<P>(unit)) * P::SEGMENT;
-                const int k1 = P::SEGMENT ? min(unit.k1, k0 + P::SEGMENT) : unit.k1;
+            const int segments = tg_segments<P>(a, unit);
+            for (int at = 0; at < unit.tiles * segments && live; ++at) {
+                const int t = at / segments;
+                const int2 range = tg_segment<P>(a, unit, at - t * segments);
                 if (!mbar_wait_warp(&acc_empty[ab], acc_parity, s_abort, a.d_error)) { live = false; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + ab * P::BN;
                 const uint32_t idesc = a.idesc | Cfg::M_BITS | ((uint32_t)((PAIR ? P::BN : P::n_mma(a, unit, t)) >> 3) << 17);  // a pair's CTAs hold half of N each, whatever is used of it
-                const int steps = (k1 - k0) * P::Pairs::N;
+                const int steps = (range.y - range.x) * P::Pairs::N;
                 for (int k = 0; k < steps; ++k) {
                     if (!mbar_wait_warp(&full[s], parity, s_abort, a.d_error)) { live = false; break; }
                     tc_fence_after();
@@ -233,7 +243,7 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         uint32_t nth = 0;  // accumulator of the CTA
         for (unsigned u = first; u < a.units; u += step) {
             const typename P::Unit unit(a, u);
-            const int segments = tg_segments<P>(unit);
+            const int segments = tg_segments<P>(a, unit);
             epi.unit_begin(a, unit);
             for (int t = 0; t < unit.tiles; ++t) {
                 for (int g = 0; g < segments; ++g, ++nth) {
@@ -249,8 +259,8 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                             else mbar_arrive(&acc_empty[ab]);
                         }
                     };
-                    if (P::SEGMENT && g + 1 < segments) {
-                        if constexpr (P::SEGMENT != 0) epi.segment(a, g == 0, taddr, live);
+                    if (P::SEGMENTS && g + 1 < segments) {
+                        if constexpr (P::SEGMENTS) epi.segment(a, g == 0, taddr, live);
                         done();
                     } else {
                         epi.tile(a, unit, t, taddr, live, segments > 1, done);
@@ -310,6 +320,10 @@ __device__ __forceinline__ void tg_ld16(uint32_t taddr, uint32_t* r) {
 __device__ __forceinline__ void tg_ld32(uint32_t taddr, uint32_t* r) {
     __syncwarp();
     tc_ld32(taddr, r);
+}
+__device__ __forceinline__ void tg_ld64(uint32_t taddr, uint32_t (&r)[2][32]) {
+    tg_ld32(taddr, r[0]);
+    tg_ld32(taddr + 32, r[1]);
 }
 // 32 of them, NaN where a wait ran out.
 __device__ __forceinline__ void tg_read(uint32_t taddr, bool live, uint32_t (&r)[32]) {
