@@ -238,3 +238,17 @@ def test_no_wait_ran_out(culsh):
     r = culsh.cross_entropy(Q, X, targets)
     culsh.cross_entropy_backward(Q, X, targets, r, torch.ones(300, device="cuda"))
     r.check()
+
+
+def test_scores_of_few_queries_are_sums_of_sums(culsh):
+    """Scores of 40 from 960 positive products.  A rounding is uniform within half a unit, 2^-25.2 of a sum that grows evenly: of one sum over all of them the root of the squares' mean is
+    40 x 2^-25.2 x sqrt(960 / 3) = 1.9e-5, of 30 sums of 32 and their sum 40 x 2^-25.2 x sqrt(30 / 3) = 3e-6, beside the loss's own rounding and exponentials of 2^-22."""
+    n, d = 300, 960
+    X = 0.5 + torch.rand(n, d, generator=gen(2), device="cuda")
+    off = []
+    for seed in range(16):
+        Q, targets = 0.5 + torch.rand(1, d, generator=gen(10 + seed), device="cuda"), torch.full((1,), 7 * seed, device="cuda")
+        t = float((Q.double() @ X.double().T).mean()) / 40
+        z = Q.double() @ X.double().T / t
+        off.append(float(culsh.cross_entropy(Q, X, targets, temperature=t).losses.double()[0] - (torch.logsumexp(z, 1) - z[:, 7 * seed])[0]))
+    assert float(np.sqrt(np.mean(np.square(off)))) <= 8e-6
