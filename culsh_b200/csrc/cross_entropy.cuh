@@ -31,7 +31,8 @@ constexpr int CE_BN = 256, CE_PART = CE_BN / 4;  // columns of a tile, and of it
 // Steps of 64 in a segment of K (tc_gemm.cuh), of the losses' scores and of the gradient's, so that p are a softmax of the same numbers: in one sum over 65,536 values the gradient's scores of 40 would
 // be 3e-4 of themselves smaller, and all p 1.3e-2.  A segment's 32 adds cut off 1e-6 of a score (32 x 2^-25 of it on average, as its sum grows).  4,099 x 32,771 x 2,048 float16: losses 380 us, by
 // segments of 256 values 414; gradient 1.51 ms, in one sum 1.46.  Calls of few tiles, which leave most SMs idle, have time for shorter ones: losses of 64 x 4,891 x 1,321 bfloat16 4.3e-7 off in place
-// of 1.6e-6 in the same 35 us (128 x 9,000 x 4,096 33 us in place of 26).
+// of 1.6e-6 in the same 35 us (128 x 9,000 x 4,096 33 us in place of 26).  So have those of up to 32 queries, where the rows' reads take the time and one warp in four has lanes to read: 4 x 100,000 x
+// 1,024 bfloat16 1.6e-7 off in place of 8.6e-7, 53 us either way (of 64 by 768 44 in place of 41, of 128 by 200,000 x 256 39 in place of 32).
 constexpr int CE_SEGMENT = 8, CE_SEGMENT_SMALL = 2;
 
 struct CeScoreArgs {
@@ -1143,7 +1144,7 @@ struct CePlan {
         if (ceil_div(k.m, TG_M) * ceil_div(n, CE_BN) <= (size_t)k.c->sm_count / 4) return CE_SMALL;
         return pairs(k.m) ? CE_PAIR : CE_ONE;
     }
-    static int segment_of(const CeCall& k) { return tile_of(k, k.n) == CE_SMALL ? CE_SEGMENT_SMALL : CE_SEGMENT; }
+    static int segment_of(const CeCall& k) { return k.m <= 32 || tile_of(k, k.n) == CE_SMALL ? CE_SEGMENT_SMALL : CE_SEGMENT; }
     static int tile_rows(CeTile t) { return t == CE_SMALL ? CE_PART : CE_BN; }
     static int product_bn(int d) { return d > 128 ? 256 : d > 64 ? 128 : 64; }
 };

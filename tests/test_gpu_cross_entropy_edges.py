@@ -21,11 +21,11 @@ def gen(seed=0):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("d", [300, 512, 1_321])
-def test_losses_of_small_calls_are_as_near_as_floats(culsh, d, dtype):
+@pytest.mark.parametrize("m,n,d", [(64, 4_891, 300), (64, 4_891, 512), (64, 4_891, 1_321), (32, 37_633, 862), (20, 30_000, 600)])
+def test_losses_of_small_calls_are_as_near_as_floats(culsh, m, n, d, dtype):
     """Scores of about 8, in segments of 128 values whose 8 adds cut off half a unit of 2^-23 of a sum that is half as large on average: 8 x 2^-25 x 8 = 2e-6, of which a target's loss keeps the share
     of the other rows, and of a mean loss of 1 to 3, 1e-6 of it."""
-    m, n, t = 64, 4_891, 0.05
+    t = 0.05
     X = torch.nn.functional.normalize(torch.randn(n, d, generator=gen(1), device="cuda"))
     targets = torch.randint(0, n, (m,), generator=gen(2), device="cuda")
     Q = torch.nn.functional.normalize(X[targets] + torch.randn(m, d, generator=gen(3), device="cuda") * (2.5 / d ** 0.5)).to(dtype)
