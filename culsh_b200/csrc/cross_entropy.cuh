@@ -225,7 +225,7 @@ struct CeLossPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
     };
 };
 
-// G of a piece, 128 neighbouring bytes of a query to a thread.  4,099 x 6,656 x 2,048 float16 82 us, 1,355 TFLOP/s.
+// G of a piece, 128 neighbouring bytes of a query to a thread.  4,099 x 6,656 x 2,048 float16 102 us, 1,095 TFLOP/s (in one sum over K 82; see CE_SEGMENT).
 template <int PLANES, bool BIAS, bool HALF, bool SEGMENTS, int TILE>
 struct CeGradPolicy : CeScoreBase<PLANES, SEGMENTS, TILE> {
     static constexpr int BN = CeScoreBase<PLANES, SEGMENTS, TILE>::BN;

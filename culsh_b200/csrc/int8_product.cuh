@@ -123,7 +123,7 @@ __device__ __noinline__ void i8_store_far(int metric, uint32_t taddr, int column
 
 // More than 64 queries: they are the M side, a lane of the accumulator a query.  Short rows leave the time to the epilogue: a warp has 32 queries by all 128 rows of a tile, and groups of four
 // take tiles in turn; of long rows a tile has 256, and a warp 64 of them.  128 bytes of each query are stored at a time, by way of shared memory.  4,099 x 32,771 x 2,048 265 us, the tensor pipe
-// busy for 68 % (one CTA by 128 rows 414); 1,000 x 1M x 128 bfloat16 635, no unit above 38 % (conversions in place of additions 923).
+// busy for 68 % (one CTA by 128 rows 414); 1,000 x 1M x 128 bfloat16 619 to 640, no unit above 38 % (conversions in place of additions 923).
 template <typename OUT, bool PAIRS, int N>
 struct I8ProductPolicy {
     static constexpr bool A_MN = false, B_MN = false, I8 = true, PARTS = N == 256, PAIR = PAIRS;
